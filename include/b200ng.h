@@ -563,6 +563,105 @@ int b2_lut_update(const void* delta, const void* idx, void* dW, int32_t flex, in
                   uint64_t* probe_out, int32_t probe, void* stream);
 
 /* ------------------------------------------------------------------------------------------
+ * Operators of a language model's training step.  No counterpart in the reference, whose lookup table
+ * (above), batch normalisation and optimizers they stand beside.  Results must lie on the current
+ * device; a launch goes to `stream` of that device.
+ * ------------------------------------------------------------------------------------------ */
+/* how tokens are held: fp32, int32, int64, or flex16 mantissas with the exponent of slot_idx */
+#define B2_IDX_F32 0
+#define B2_IDX_I32 1
+#define B2_IDX_I64 2
+#define B2_IDX_FLEX16 3
+
+/* Table lookup with a scale, and the table's gradient.  table / dW [V][F], out / delta [n_idx][F], dense.
+ *   fprop:  out[t] = scale * table[token[t]]; tokens outside [0, V), and NaN, read as zero
+ *   update: dW[v] = scale * sum of delta[t] over the t with token[t] = v, in ascending order of t (in parts of 32,
+ *           the parts' sums in order: the same bits in every run); rows without tokens, and row pad_idx (-1: none),
+ *           become zero; tokens outside [0, V) are left out.  onto != 0 (fp32): added to what dW holds, and only the
+ *           rows of tokens are touched.
+ * flex != 0: table, out, delta, dW hold int16 mantissas with the exponents of their slots in `scales`; the result is
+ * rounded to the nearest even mantissa, its largest goes to stats[slot]; probe != 0 stores nothing and leaves the bit
+ * pattern of the largest |value| in *probe_out (maximum with what it holds).
+ * `scratch` needs no initial value and may be used again by the next call on the stream, not by calls on two
+ * streams at once. */
+int b2_embed_fprop(const void* table, const void* idx, void* out, int32_t flex, int32_t idx_kind,
+                   int32_t V, int32_t F, int64_t n_idx, float scale, const b2_flex_scale* scales,
+                   int32_t slot_table, int32_t slot_idx, int32_t slot_out, int32_t* stats,
+                   uint64_t* probe_out, int32_t probe, void* stream);
+int b2_embed_update_scratch_bytes(int32_t V, int32_t F, int64_t n_idx, size_t* bytes);
+int b2_embed_update(const void* delta, const void* idx, void* dW, int32_t flex, int32_t idx_kind,
+                    int32_t V, int32_t F, int64_t n_idx, float scale, int64_t pad_idx, int32_t onto,
+                    const b2_flex_scale* scales, int32_t slot_delta, int32_t slot_idx, int32_t slot_dW,
+                    int32_t* stats, uint64_t* probe_out, int32_t probe, void* scratch,
+                    size_t scratch_bytes, void* stream);
+
+/* The edge between two blocks of a residual network, fp32.  With rms(x) = x / sqrt(mean(x^2) + eps) over the
+ * `features` of a row:
+ *   stream = residual_scale * residual + gate * (rms(block) * post_weight)
+ *   out    = rms(stream) * pre_weight
+ * block NULL: the stream is `residual` itself (residual_scale 1, no gate, no post_weight, stream NULL);
+ * post_weight NULL: the block's result is not normalised; pre_weight and out NULL: the stream alone.
+ * Tensors of rows have a stride in elements, at least `features` where there is more than one row.  `stream` may be
+ * the memory of `residual`.  block_rstd and stream_rstd [rows], where not NULL, receive 1 / sqrt(mean + eps), which
+ * the gradients read.
+ *   bprop: from d_out (NULL without pre_weight) and d_stream (NULL: zero), the gradients of all five operands; those
+ *          that are NULL are not stored.  Reads stream (residual where there is no block) and the rstd's as fprop
+ *          has left them.  d_residual may be the memory of d_stream.  Sums over rows (of the weights, of a gate per
+ *          feature) are added in an order that depends on the sizes alone; rows = 0 leaves them zero.
+ * The scratch needs no initial value; calls on two streams at once need one each. */
+#define B2_GATE_NONE 0
+#define B2_GATE_FEATURE 1 /* [features] */
+#define B2_GATE_ROW 2     /* [rows] */
+#define B2_GATE_FULL 3    /* [rows][features], with gate_stride */
+typedef struct {
+    int64_t rows;
+    int32_t features, gate_kind;
+    float residual_scale, eps;
+    const float *block, *residual, *gate, *post_weight, *pre_weight;
+    float *stream, *out, *block_rstd, *stream_rstd;
+    int64_t block_stride, residual_stride, gate_stride, stream_stride, out_stride;
+} b2_norm;
+typedef struct {
+    const float *d_out, *d_stream;
+    float *d_residual, *d_block, *d_gate, *d_post_weight, *d_pre_weight;
+    int64_t d_out_stride, d_stream_stride, d_residual_stride, d_block_stride, d_gate_stride;
+} b2_norm_grads;
+int b2_norm_fprop(const b2_norm* norm, void* stream);
+int b2_norm_bprop_scratch_bytes(const b2_norm* norm, size_t* bytes);
+int b2_norm_bprop(const b2_norm* norm, const b2_norm_grads* grads, void* scratch,
+                  size_t scratch_bytes, void* stream);
+
+/* One AdamW step over many fp32 tensors in one launch.  With t the number of the step, from 1 on:
+ *   m = beta1 m + (1 - beta1) g,  v = beta2 v + (1 - beta2) g^2
+ *   param = param (1 - lr weight_decay decay) - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
+ * state_bits 32: m and v are fp32.  8: m and sqrt(v) are e4m3 bytes times the scale of their 256 values (of the
+ * tensor, from its start), m_scales and v_scales [ceil(n / 256)]; the step uses the exact moments and then rounds
+ * them at random to one of the two neighbours, so that averages which move by less than a step of the format are
+ * held without bias.  The random bits are a hash of (seed, t, counter + position).  All zeros is the state before
+ * the first step.  A block whose largest moment is not above 2^-100 is held as zeros.
+ *   plan:  a table of the work on the device, made once for given addresses (not while a stream is captured);
+ *          the tensors must not overlap; n = 0 is allowed
+ *   step:  lr and grad_scale, where not NULL, point to a device float that replaces hyper->lr, and one that
+ *          multiplies every gradient; *step is a device float that holds t - 1 before and t after
+ * A plan is for one stream at a time. */
+typedef struct {
+    float* param;
+    const float* grad;
+    void *m, *v;
+    float *m_scales, *v_scales;
+    int64_t n;
+    float decay;
+    uint32_t counter;
+} b2_adamw_tensor;
+typedef struct { double lr, beta1, beta2, eps, weight_decay; } b2_adamw_hyper;
+int b2_adamw_plan_bytes(const b2_adamw_tensor* tensors, int32_t count, int32_t state_bits,
+                        size_t* bytes, int64_t* chunks);
+int b2_adamw_plan(const b2_adamw_tensor* tensors, int32_t count, int32_t state_bits, void* plan,
+                  size_t plan_bytes, void* stream);
+int b2_adamw_step(void* plan, int64_t chunks, int32_t state_bits, const b2_adamw_hyper* hyper,
+                  const float* lr, const float* grad_scale, float* step, uint32_t seed, void* stream);
+
+/* ------------------------------------------------------------------------------------------
  * Gradient allreduce over NCCL (NVLink / NVSwitch), one process per GPU.
  * Replaces: CudaAllReduceKernel and its reduction kernel (ngraph/transformers/gpu/tensor_ops.py:
  * 52-116, 416-618), which reduce one gradient tensor at a time with peer-to-peer copies, MPI

@@ -1,0 +1,368 @@
+// One AdamW step over many tensors.
+//
+//   m = beta1 m + (1 - beta1) g,  v = beta2 v + (1 - beta2) g^2
+//   p = p (1 - lr wd) - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
+//
+// Bound by memory: 28 bytes a value with fp32 moments, 16.06 with moments in 8 bits.  The tensors are cut into chunks
+// of 2048 values, one 64-byte record each, made once (the addresses of a program's tensors stay): a CTA reads a
+// record and its values, whatever tensor they belong to, so that many small tensors cost no launches.
+//
+// Moments in 8 bits: a warp holds 256 values and their two scales.  m and sqrt(v) are e4m3 values times the block's
+// largest / 448.  v itself spans the square of what its root does, and e4m3 covers 2.3e5 : 1.  An average with
+// beta2 = 0.999 moves by at most 0.05 % of its root in a step downwards where e4m3's neighbours are 6 to 12 % apart: rounded to
+// nearest it would never come down.  Rounded at random to either neighbour, with the chance that makes the mean
+// right, it does, on the average.  A root that is not zero is not rounded to zero, which would leave m / eps.
+#include <cmath>
+#include <cstdint>
+#include <new>
+#include <vector>
+
+#include <cuda_fp8.h>
+
+#include "b2_operators.h"
+
+namespace {
+
+constexpr int kChunk = 2048;
+constexpr int kThreads = 256;
+constexpr int kBlock = 256;             // values with one scale
+
+struct Chunk {
+    float* param;
+    const float* grad;
+    void *m, *v;
+    float *m_scales, *v_scales;
+    unsigned n, counter;
+    float decay;
+    unsigned vec;                       // all addresses allow vectors
+};
+static_assert(sizeof(Chunk) == 64, "records are read as four vectors");
+constexpr size_t kHeader = 256;         // of a plan: the count of CTAs that have finished, then the records
+
+struct Rates {
+    float b1, c1, b2, c2, eps;
+    double lr, wd, beta1, beta2;
+};
+
+struct Now {
+    float size, root, lr_wd, grad_scale;
+    unsigned key;
+};
+
+__device__ __forceinline__ unsigned mix(unsigned x) {
+    x = (x ^ (x >> 16)) * 0x9E3779B9u;          // (odd words: multiplication permutes)
+    x = (x ^ (x >> 15)) * 0xBB67AE85u;
+    return x ^ (x >> 16);
+}
+
+// x^t by squaring
+__device__ __forceinline__ double power(double x, unsigned t) {
+    double y = 1.0;
+    for (; t; t >>= 1, x *= x)
+        if (t & 1) y *= x;
+    return y;
+}
+
+// What depends on the number of the step, in 64 bits: 1 - beta^t cancels where beta^t is near 1.
+__device__ __forceinline__ float begin_step(const Rates& r, const float* lr_at, const float* scale_at, const float* step, unsigned seed, Now* now) {
+    const float before = *step;
+    const unsigned t = before >= 0.0f ? (unsigned)fminf(before, 4.0e9f) + 1u : 1u;
+    const double lr = lr_at ? (double)*lr_at : r.lr;
+    now->size = (float)(lr / (1.0 - power(r.beta1, t)));
+    now->root = (float)(1.0 / sqrt(1.0 - power(r.beta2, t)));
+    now->lr_wd = (float)(lr * r.wd);
+    now->grad_scale = scale_at ? *scale_at : 1.0f;
+    now->key = mix(seed + 0x9E3779B9u * t);
+    return before;
+}
+
+// The new moments, the root of the second, and the new value.  Every operation is rounded by itself: the result does
+// not depend on how the values are spread over threads.
+__device__ __forceinline__ float update(const Rates& r, const Now& now, float keep, float p, float g, float& m, float& v, float& root) {
+    g = __fmul_rn(g, now.grad_scale);
+    m = __fadd_rn(__fmul_rn(m, r.b1), __fmul_rn(g, r.c1));
+    v = __fadd_rn(__fmul_rn(v, r.b2), __fmul_rn(__fmul_rn(g, g), r.c2));
+    root = __fsqrt_rn(v);
+    const float d = __fdiv_rn(m, __fadd_rn(__fmul_rn(root, now.root), r.eps));
+    return __fsub_rn(__fmul_rn(p, keep), __fmul_rn(d, now.size));
+}
+
+// The step is counted by the CTA that finishes last: every other one has read the count by then.
+__device__ __forceinline__ void end_step(unsigned* finished, float* step, float before) {
+    if (threadIdx.x == 0 && atomicInc(finished, gridDim.x - 1) == gridDim.x - 1) *step = before + 1.0f;
+}
+
+__global__ void __launch_bounds__(kThreads)
+adamw32_kernel(unsigned* finished, const Chunk* __restrict__ chunks, long long n_chunks, Rates r, const float* lr_at, const float* scale_at, float* step,
+               unsigned seed) {
+    __shared__ Now shared_now;
+    after_earlier_kernels();
+    float before = 0.0f;
+    if (threadIdx.x == 0) before = begin_step(r, lr_at, scale_at, step, seed, &shared_now);
+    __syncthreads();
+    const Now now = shared_now;
+    for (long long k = blockIdx.x; k < n_chunks; k += gridDim.x) {
+        const Chunk c = chunks[k];
+        float* m = static_cast<float*>(c.m);
+        float* v = static_cast<float*>(c.v);
+        const float keep = __fsub_rn(1.0f, __fmul_rn(c.decay, now.lr_wd));
+        float unused;
+        if (c.vec) {
+            constexpr int UN = kChunk / kThreads / 4;
+            float4 p4[UN], g4[UN], m4[UN], v4[UN];
+#pragma unroll
+            for (int u = 0; u < UN; ++u) {
+                const int i = (u * kThreads + threadIdx.x) * 4;
+                if (i + 4 <= (int)c.n) {
+                    p4[u] = *reinterpret_cast<const float4*>(c.param + i);
+                    g4[u] = *reinterpret_cast<const float4*>(c.grad + i);
+                    m4[u] = *reinterpret_cast<const float4*>(m + i);
+                    v4[u] = *reinterpret_cast<const float4*>(v + i);
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < UN; ++u) {
+                const int i = (u * kThreads + threadIdx.x) * 4;
+                if (i + 4 <= (int)c.n) {
+                    p4[u].x = update(r, now, keep, p4[u].x, g4[u].x, m4[u].x, v4[u].x, unused);
+                    p4[u].y = update(r, now, keep, p4[u].y, g4[u].y, m4[u].y, v4[u].y, unused);
+                    p4[u].z = update(r, now, keep, p4[u].z, g4[u].z, m4[u].z, v4[u].z, unused);
+                    p4[u].w = update(r, now, keep, p4[u].w, g4[u].w, m4[u].w, v4[u].w, unused);
+                    *reinterpret_cast<float4*>(c.param + i) = p4[u];
+                    *reinterpret_cast<float4*>(m + i) = m4[u];
+                    *reinterpret_cast<float4*>(v + i) = v4[u];
+                }
+            }
+        }
+        for (int i = (c.vec ? (int)(c.n & ~3u) : 0) + threadIdx.x; i < (int)c.n; i += kThreads) {
+            float mi = m[i], vi = v[i];
+            c.param[i] = update(r, now, keep, c.param[i], c.grad[i], mi, vi, unused);
+            m[i] = mi;
+            v[i] = vi;
+        }
+    }
+    end_step(finished, step, before);
+}
+
+// q, |q| <= 448 but for a rounding, to one of its two neighbours in e4m3: the upper one with the chance that sixteen
+// random bits give it.  The bits of a mantissa that e4m3 does not have are added to and cut off; below 2^-6, where
+// its values are 2^-9 apart, the same between 2^-6 and 2^-5.
+__device__ __forceinline__ float to_e4m3(float q, unsigned bits) {
+    const float a = fminf(fabsf(q), 448.0f);
+    const bool low = a < 0.015625f;
+    const float b = low ? __fadd_rn(a, 0.015625f) : a;
+    const float c = __uint_as_float((__float_as_uint(b) + (bits << 4)) & ~0xFFFFFu);
+    return low ? __fsub_rn(c, 0.015625f) : c;
+}
+
+__device__ __forceinline__ float2 from_e4m3(unsigned two) {
+    const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)two, __NV_E4M3);
+    return __half22float2(__half2(h));
+}
+__device__ __forceinline__ unsigned codes(float x, float y) {
+    return __nv_cvt_float2_to_fp8x2(make_float2(x, y), __NV_SATFINITE, __NV_E4M3);
+}
+
+// 448 / top and the block's scale
+__device__ __forceinline__ float scale_of(float top, float& scale) {
+    const bool live = top > 7.888609052210118e-31f;             // 2^-100
+    scale = live ? __fdiv_rn(top, 448.0f) : 0.0f;
+    if (!(top <= 3.402823466e+38f)) scale = __int_as_float(0x7fffffff);
+    return live ? __fdiv_rn(448.0f, top) : 0.0f;
+}
+
+__global__ void __launch_bounds__(kThreads)
+adamw8_kernel(unsigned* finished, const Chunk* __restrict__ chunks, long long n_chunks, Rates r, const float* lr_at, const float* scale_at, float* step,
+              unsigned seed) {
+    __shared__ Now shared_now;
+    after_earlier_kernels();
+    float before = 0.0f;
+    if (threadIdx.x == 0) before = begin_step(r, lr_at, scale_at, step, seed, &shared_now);
+    __syncthreads();
+    const Now now = shared_now;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    for (long long k = blockIdx.x; k < n_chunks; k += gridDim.x) {
+        const Chunk c = chunks[k];
+        const int at = warp * kBlock;
+        const int n = (int)c.n - at;                    // of the warp's block
+        if (n <= 0) continue;
+        unsigned char* mc = static_cast<unsigned char*>(c.m) + at;
+        unsigned char* vc = static_cast<unsigned char*>(c.v) + at;
+        const float keep = __fsub_rn(1.0f, __fmul_rn(c.decay, now.lr_wd));
+        // a lane's values: four from 4 lane on, four from 128 + 4 lane on
+        float p[8], g[8], m[8], v[8], root[8];
+        const bool vec = c.vec && n >= kBlock;
+        const float ms = c.m_scales[warp], vs = c.v_scales[warp];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int i = h * 128 + lane * 4;
+            unsigned mw = 0, vw = 0;
+            if (vec) {
+                const float4 p4 = *reinterpret_cast<const float4*>(c.param + at + i), g4 = *reinterpret_cast<const float4*>(c.grad + at + i);
+                p[4 * h] = p4.x; p[4 * h + 1] = p4.y; p[4 * h + 2] = p4.z; p[4 * h + 3] = p4.w;
+                g[4 * h] = g4.x; g[4 * h + 1] = g4.y; g[4 * h + 2] = g4.z; g[4 * h + 3] = g4.w;
+                mw = *reinterpret_cast<const unsigned*>(mc + i);
+                vw = *reinterpret_cast<const unsigned*>(vc + i);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const bool there = i + j < n;
+                    p[4 * h + j] = there ? c.param[at + i + j] : 0.0f;
+                    g[4 * h + j] = there ? c.grad[at + i + j] : 0.0f;
+                    mw |= there ? (unsigned)mc[i + j] << (8 * j) : 0u;
+                    vw |= there ? (unsigned)vc[i + j] << (8 * j) : 0u;
+                }
+            }
+            const float2 ma = from_e4m3(mw & 0xffff), mb = from_e4m3(mw >> 16), va = from_e4m3(vw & 0xffff), vb = from_e4m3(vw >> 16);
+            m[4 * h] = ma.x; m[4 * h + 1] = ma.y; m[4 * h + 2] = mb.x; m[4 * h + 3] = mb.y;
+            v[4 * h] = va.x; v[4 * h + 1] = va.y; v[4 * h + 2] = vb.x; v[4 * h + 3] = vb.y;
+        }
+        unsigned top_m = 0, top_r = 0;                  // as bits, whose order is that of the values (NaN above all)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            m[e] = __fmul_rn(m[e], ms);
+            const float old = __fmul_rn(v[e], vs);
+            v[e] = __fmul_rn(old, old);
+            p[e] = update(r, now, keep, p[e], g[e], m[e], v[e], root[e]);
+            top_m = max(top_m, __float_as_uint(fabsf(m[e])));
+            top_r = max(top_r, __float_as_uint(fabsf(root[e])));
+        }
+        top_m = __reduce_max_sync(0xffffffffu, top_m);
+        top_r = __reduce_max_sync(0xffffffffu, top_r);
+        float new_ms, new_vs;
+        const float to_m = scale_of(__uint_as_float(top_m), new_ms), to_r = scale_of(__uint_as_float(top_r), new_vs);
+        if (lane == 0) {
+            c.m_scales[warp] = new_ms;
+            c.v_scales[warp] = new_vs;
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int i = h * 128 + lane * 4;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int e = 4 * h + j;
+                const unsigned bits = mix((c.counter + (unsigned)(at + i + j)) ^ now.key);
+                const float qm = __fmul_rn(m[e], to_m), qr = __fmul_rn(root[e], to_r);
+                m[e] = copysignf(to_e4m3(qm, bits & 0xffffu), qm);
+                const float cr = to_e4m3(qr, bits >> 16);
+                root[e] = qr > 0.0f ? fmaxf(cr, 0.001953125f) : cr;
+            }
+            const unsigned mw = codes(m[4 * h], m[4 * h + 1]) | codes(m[4 * h + 2], m[4 * h + 3]) << 16;
+            const unsigned vw = codes(root[4 * h], root[4 * h + 1]) | codes(root[4 * h + 2], root[4 * h + 3]) << 16;
+            if (vec) {
+                *reinterpret_cast<float4*>(c.param + at + i) = make_float4(p[4 * h], p[4 * h + 1], p[4 * h + 2], p[4 * h + 3]);
+                *reinterpret_cast<unsigned*>(mc + i) = mw;
+                *reinterpret_cast<unsigned*>(vc + i) = vw;
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (i + j < n) {
+                        c.param[at + i + j] = p[4 * h + j];
+                        mc[i + j] = (unsigned char)(mw >> (8 * j));
+                        vc[i + j] = (unsigned char)(vw >> (8 * j));
+                    }
+            }
+        }
+    }
+    end_step(finished, step, before);
+}
+
+int count_chunks(const b2_adamw_tensor* list, int count, int state_bits, long long* chunks) {
+    B2_REQUIRE(count >= 0 && (count == 0 || list), "bad list of tensors");
+    B2_REQUIRE(state_bits == 32 || state_bits == 8, "moments are held in 32 or 8 bits, not in %d", state_bits);
+    *chunks = 0;
+    for (int i = 0; i < count; ++i) {
+        const b2_adamw_tensor& t = list[i];
+        B2_REQUIRE(t.n >= 0, "tensor %d has %lld values", i, (long long)t.n);
+        B2_REQUIRE(t.n == 0 || (t.param && t.grad && t.m && t.v), "tensor %d: missing address", i);
+        B2_REQUIRE(t.n == 0 || state_bits == 32 || (t.m_scales && t.v_scales), "tensor %d: missing scales", i);
+        *chunks += (t.n + kChunk - 1) / kChunk;
+    }
+    return B2_OK;
+}
+
+}  // namespace
+
+extern "C" int b2_adamw_plan_bytes(const b2_adamw_tensor* tensors, int32_t count, int32_t state_bits, size_t* bytes, int64_t* chunks) {
+    B2_REQUIRE(bytes && chunks, "bad argument");
+    long long n = 0;
+    B2_CHECK(count_chunks(tensors, count, state_bits, &n));
+    *chunks = n;
+    *bytes = kHeader + (size_t)n * sizeof(Chunk) + 64;
+    return B2_OK;
+}
+
+static char* plan_base(void* plan) { return (char*)(((uintptr_t)plan + 63) / 64 * 64); }
+
+extern "C" int b2_adamw_plan(const b2_adamw_tensor* tensors, int32_t count, int32_t state_bits, void* plan, size_t plan_bytes, void* stream) {
+    size_t need = 0;
+    int64_t chunks = 0;
+    B2_CHECK(b2_adamw_plan_bytes(tensors, count, state_bits, &need, &chunks));
+    B2_REQUIRE(plan && plan_bytes >= need, "the plan needs %zu bytes, got %zu", need, plan_bytes);
+    B2_CHECK(b2::require_here(plan, "the plan"));
+    for (int i = 0; i < count; ++i) {
+        if (tensors[i].n == 0) continue;
+        const float* ends[2] = {tensors[i].param, tensors[i].grad};
+        for (const float* p : ends) B2_CHECK(b2::require_here(p, "a tensor of the plan"));
+        B2_CHECK(b2::require_here(tensors[i].m, "a moment of the plan"));
+        B2_CHECK(b2::require_here(tensors[i].v, "a moment of the plan"));
+    }
+    cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
+    B2_CUDA(cudaStreamIsCapturing((cudaStream_t)stream, &capturing));
+    B2_REQUIRE(capturing == cudaStreamCaptureStatusNone, "a plan is made before its stream is captured");
+    try {
+        std::vector<char> host(kHeader + (size_t)chunks * sizeof(Chunk), 0);
+        Chunk* c = reinterpret_cast<Chunk*>(host.data() + kHeader);
+        for (int i = 0; i < count; ++i) {
+            const b2_adamw_tensor& t = tensors[i];
+            for (int64_t at = 0; at < t.n; at += kChunk, ++c) {
+                const size_t state = state_bits == 32 ? 4 : 1;
+                c->param = t.param + at;
+                c->grad = t.grad + at;
+                c->m = static_cast<char*>(t.m) + at * state;
+                c->v = static_cast<char*>(t.v) + at * state;
+                if (state_bits == 8) {
+                    c->m_scales = t.m_scales + at / kBlock;
+                    c->v_scales = t.v_scales + at / kBlock;
+                }
+                c->n = (unsigned)(t.n - at < kChunk ? t.n - at : kChunk);
+                c->counter = t.counter + (unsigned)at;
+                c->decay = t.decay;
+                const uintptr_t states = (uintptr_t)c->m | (uintptr_t)c->v;
+                c->vec = b2::aligned16(c->param) && b2::aligned16(c->grad) && states % (4 * state) == 0;
+            }
+        }
+        // (pageable memory: the copy has been staged when the call returns)
+        B2_CUDA(cudaMemcpyAsync(plan_base(plan), host.data(), host.size(), cudaMemcpyHostToDevice, (cudaStream_t)stream));
+        B2_CUDA(cudaStreamSynchronize((cudaStream_t)stream));
+    } catch (const std::bad_alloc&) {
+        return b2::fail(B2_ERR_INVALID, "no memory for a plan of %zu bytes", need);
+    }
+    return B2_OK;
+}
+
+extern "C" int b2_adamw_step(void* plan, int64_t chunks, int32_t state_bits, const b2_adamw_hyper* h, const float* lr, const float* grad_scale, float* step,
+                             uint32_t seed, void* stream) {
+    B2_REQUIRE(plan && h && step && chunks >= 0, "bad argument");
+    B2_REQUIRE(state_bits == 32 || state_bits == 8, "moments are held in 32 or 8 bits, not in %d", state_bits);
+    B2_REQUIRE(h->beta1 >= 0.0 && h->beta1 < 1.0 && h->beta2 >= 0.0 && h->beta2 < 1.0 && h->eps >= 0.0 && std::isfinite(h->lr) &&
+                   std::isfinite(h->weight_decay) && std::isfinite(h->eps),
+               "bad rates: lr %g, beta1 %g, beta2 %g, eps %g, weight decay %g", h->lr, h->beta1, h->beta2, h->eps, h->weight_decay);
+    B2_CHECK(b2::require_here(step, "the number of the step"));
+    Rates r;
+    r.b1 = (float)h->beta1;
+    r.c1 = (float)(1.0 - h->beta1);
+    r.b2 = (float)h->beta2;
+    r.c2 = (float)(1.0 - h->beta2);
+    r.eps = (float)h->eps;
+    r.lr = h->lr;
+    r.wd = h->weight_decay;
+    r.beta1 = h->beta1;
+    r.beta2 = h->beta2;
+    char* base = plan_base(plan);
+    long long blocks = chunks < 1 ? 1 : chunks;
+    if (blocks > b2::kSms * 8) blocks = b2::kSms * 8;
+    B2_CUDA(b2::launch_after(state_bits == 32 ? adamw32_kernel : adamw8_kernel, dim3((unsigned)blocks), kThreads, 0, (cudaStream_t)stream,
+                             reinterpret_cast<unsigned*>(base), reinterpret_cast<const Chunk*>(base + kHeader), (long long)chunks, r, lr, grad_scale, step, seed));
+    return B2_OK;
+}

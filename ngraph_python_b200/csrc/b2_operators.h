@@ -1,0 +1,46 @@
+// Helpers shared by the language-model operators (b2_embed.cu, b2_norm.cu, b2_adamw.cu).
+#ifndef B2_OPERATORS_H
+#define B2_OPERATORS_H
+
+#include <atomic>
+
+#include "b2_common.h"
+
+namespace b2 {
+
+constexpr int kSms = 148;
+
+// Launches go to the current device.  A result that lies on another one, or on the host, is refused:
+// the kernel would fault, or write across the link.
+inline int require_here(const void* out, const char* what) {
+    int now = 0;
+    B2_CUDA(cudaGetDevice(&now));
+    cudaPointerAttributes a;
+    B2_CUDA(cudaPointerGetAttributes(&a, out));
+    B2_REQUIRE(a.type == cudaMemoryTypeDevice || a.type == cudaMemoryTypeManaged, "%s is not device memory", what);
+    B2_REQUIRE(a.type != cudaMemoryTypeDevice || a.device == now, "%s lies on device %d, the current device is %d", what, a.device, now);
+    return B2_OK;
+}
+
+// More than 48 KB of dynamic shared memory is asked for once per kernel and device.
+inline int allow_shared(const void* kernel, int bytes, std::atomic<unsigned long long>* done) {
+    int now = 0;
+    B2_CUDA(cudaGetDevice(&now));
+    const unsigned long long bit = 1ull << (now & 63);
+    if (done->load(std::memory_order_relaxed) & bit) return B2_OK;
+    B2_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    done->fetch_or(bit, std::memory_order_relaxed);
+    return B2_OK;
+}
+
+inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+}  // namespace b2
+
+#define B2_CHECK(call)              \
+    do {                            \
+        int rc__ = (call);          \
+        if (rc__ < 0) return rc__;  \
+    } while (0)
+
+#endif  // B2_OPERATORS_H

@@ -107,6 +107,31 @@ GEMM_DIRECT, GEMM_PAIRS, GEMM_TILES, GEMM_STREAM = 0, 1, 2, 3
 CALL_MAX_INPUTS, CALL_MAX_OUTPUTS = 16, 16
 
 
+class NormArgs(C.Structure):
+    """b2_norm: the edge between two blocks."""
+    _fields_ = [("rows", C.c_int64), ("features", C.c_int32), ("gate_kind", C.c_int32), ("residual_scale", C.c_float),
+                ("eps", C.c_float)] + \
+        [(f, C.c_void_p) for f in ("block", "residual", "gate", "post_weight", "pre_weight", "stream", "out", "block_rstd",
+                                   "stream_rstd")] + \
+        [(f, C.c_int64) for f in ("block_stride", "residual_stride", "gate_stride", "stream_stride", "out_stride")]
+
+
+class NormGrads(C.Structure):
+    _fields_ = [(f, C.c_void_p) for f in ("d_out", "d_stream", "d_residual", "d_block", "d_gate", "d_post_weight",
+                                          "d_pre_weight")] + \
+        [(f, C.c_int64) for f in ("d_out_stride", "d_stream_stride", "d_residual_stride", "d_block_stride", "d_gate_stride")]
+
+
+class AdamwTensor(C.Structure):
+    _fields_ = [("param", C.c_void_p), ("grad", C.c_void_p), ("m", C.c_void_p), ("v", C.c_void_p), ("m_scales", C.c_void_p),
+                ("v_scales", C.c_void_p), ("n", C.c_int64), ("decay", C.c_float), ("counter", C.c_uint32)]
+
+
+class AdamwHyper(C.Structure):
+    _fields_ = [("lr", C.c_double), ("beta1", C.c_double), ("beta2", C.c_double), ("eps", C.c_double),
+                ("weight_decay", C.c_double)]
+
+
 class CallArg(C.Structure):
     _fields_ = [("src", C.c_void_p), ("inv_scale", C.c_float), ("in_place", C.c_int32)]
 
@@ -214,6 +239,16 @@ def _load():
                                     C.POINTER(i64), vp]),
         "b2_rng_fill": (C.c_int, [vp, i32, i64, i32, C.c_float, C.c_float, C.c_uint64, C.c_uint64,
                                   vp, vp, i32, vp, vp, i32, vp]),
+        "b2_embed_fprop": (C.c_int, [vp, vp, vp, i32, i32, i32, i32, i64, C.c_float, vp, i32, i32, i32, vp, vp, i32, vp]),
+        "b2_embed_update_scratch_bytes": (C.c_int, [i32, i32, i64, C.POINTER(sz)]),
+        "b2_embed_update": (C.c_int, [vp, vp, vp, i32, i32, i32, i32, i64, C.c_float, i64, i32, vp, i32, i32, i32, vp, vp,
+                                      i32, vp, sz, vp]),
+        "b2_norm_fprop": (C.c_int, [C.POINTER(NormArgs), vp]),
+        "b2_norm_bprop_scratch_bytes": (C.c_int, [C.POINTER(NormArgs), C.POINTER(sz)]),
+        "b2_norm_bprop": (C.c_int, [C.POINTER(NormArgs), C.POINTER(NormGrads), vp, sz, vp]),
+        "b2_adamw_plan_bytes": (C.c_int, [C.POINTER(AdamwTensor), i32, i32, C.POINTER(sz), C.POINTER(i64)]),
+        "b2_adamw_plan": (C.c_int, [C.POINTER(AdamwTensor), i32, i32, vp, sz, vp]),
+        "b2_adamw_step": (C.c_int, [vp, i64, i32, C.POINTER(AdamwHyper), vp, vp, vp, C.c_uint32, vp]),
         "b2_selftest_bounded_wait": (C.c_int, [i32, vp, vp, vp]),
         "b2_set_nccl_path": (C.c_int, [C.c_char_p]),
         "b2_comm_version": (C.c_int, [C.POINTER(i32)]),
@@ -522,6 +557,29 @@ def conv_update_scratch_bytes(flex, dims):
     n = C.c_size_t()
     check(_lib.b2_conv_update_scratch_bytes(int(bool(flex)), C.byref(dims), C.byref(n)))
     return n.value
+
+
+def embed_update_scratch_bytes(V, F, n):
+    out = C.c_size_t()
+    check(_lib.b2_embed_update_scratch_bytes(V, F, n, C.byref(out)))
+    return int(out.value)
+
+
+def norm_bprop_scratch_bytes(norm):
+    out = C.c_size_t()
+    check(_lib.b2_norm_bprop_scratch_bytes(C.byref(norm), C.byref(out)))
+    return int(out.value)
+
+
+def adamw_plan_bytes(tensors, state_bits):
+    """(bytes of the plan, chunks of work) of a step over `tensors`, an array of AdamwTensor."""
+    nbytes, chunks = C.c_size_t(), C.c_int64()
+    check(_lib.b2_adamw_plan_bytes(tensors, len(tensors), state_bits, C.byref(nbytes), C.byref(chunks)))
+    return int(nbytes.value), int(chunks.value)
+
+
+def adamw_plan(tensors, state_bits, plan_ptr, plan_bytes, stream=0):
+    check(_lib.b2_adamw_plan(tensors, len(tensors), state_bits, plan_ptr, plan_bytes, stream))
 
 
 def dimshuffle(src_ptr, dst_ptr, elem_bytes, shape, src_strides, dst_strides, stream=0):

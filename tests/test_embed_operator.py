@@ -1,0 +1,300 @@
+"""Table lookups with a scale and the table's gradient by sorted tokens, through the C ABI: forward bit for bit,
+sums against 64 bits within what additions in fp32 round, flex16 mantissas exactly."""
+import ctypes
+import math
+
+import numpy as np
+import pytest
+
+from oracle import flex_oracle as fx
+
+KINDS = {"f32": 0, "i32": 1, "i64": 2, "flex16": 3}
+PLAIN = (None, -1, -1, -1, None, None, 0)
+
+
+def _tokens(idx, kind):
+    import torch
+    dtype = {"f32": np.float32, "i32": np.int32, "i64": np.int64, "flex16": np.int16}[kind]
+    return torch.from_numpy(np.asarray(idx).astype(dtype)).cuda()
+
+
+def _off(shape, dtype, offset):
+    """A dense device tensor that begins `offset` elements behind a 16-byte boundary."""
+    import torch
+    n = int(np.prod(shape))
+    return torch.zeros((n + 16,), dtype=dtype, device="cuda")[offset:offset + n].view(shape)
+
+
+def _lookup(table, idx, kind, scale, offset=0):
+    import torch
+    from ngraph_python_b200 import lib
+    V, F = table.shape
+    w = _off(table.shape, torch.float32, offset)
+    w.copy_(torch.from_numpy(table))
+    x = _tokens(idx, kind)
+    out = _off((len(idx), F), torch.float32, offset)
+    lib.check(lib.raw().b2_embed_fprop(w.data_ptr(), x.data_ptr(), out.data_ptr(), 0, KINDS[kind], V, F, len(idx), scale, *PLAIN, 0))
+    torch.cuda.synchronize()
+    return out.cpu().numpy()
+
+
+def _update(delta, idx, kind, V, scale, pad=-1, onto=None, offset=0, scratch=None):
+    import torch
+    from ngraph_python_b200 import lib
+    n, F = delta.shape
+    d = _off(delta.shape, torch.float32, offset)
+    d.copy_(torch.from_numpy(delta))
+    x = _tokens(idx, kind)
+    out = _off((V, F), torch.float32, offset)
+    out.copy_(torch.full((V, F), 7.0) if onto is None else torch.from_numpy(onto))
+    nbytes = lib.embed_update_scratch_bytes(V, F, n)
+    if scratch is None:
+        scratch = torch.full((nbytes,), 0xA5, dtype=torch.uint8, device="cuda")
+    lib.check(lib.raw().b2_embed_update(d.data_ptr(), x.data_ptr(), out.data_ptr(), 0, KINDS[kind], V, F, n, scale, pad, int(onto is not None), *PLAIN,
+                                        scratch.data_ptr(), scratch.numel(), 0))
+    torch.cuda.synchronize()
+    return out.cpu().numpy()
+
+
+def _sums(delta, idx, V, scale, pad):
+    """The sums in 64 bits, what their terms add up to, and how many there are."""
+    idx = np.asarray(idx).astype(np.int64)
+    keep = (idx >= 0) & (idx < V) & (idx != pad)
+    want, size = np.zeros((V, delta.shape[1])), np.zeros((V, delta.shape[1]))
+    np.add.at(want, idx[keep], delta[keep].astype(np.float64))
+    np.add.at(size, idx[keep], np.abs(delta[keep]).astype(np.float64))
+    return want * scale, size * abs(scale), np.bincount(idx[keep], minlength=V)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["f32", "i32", "i64"])
+@pytest.mark.parametrize("n,F,V,offset", [(1, 1, 1, 0), (1, 64, 9, 0), (7, 300, 11, 0), (5, 33, 40, 0), (600, 512, 1000, 0), (1000, 2048, 50, 0),
+                                          (4096, 64, 70000, 0), (900, 256, 33, 1), (30000, 7, 5, 3)])
+def test_lookup(kind, n, F, V, offset):
+    rng = np.random.RandomState(n + F)
+    table = rng.standard_normal((V, F)).astype(np.float32)
+    idx = rng.randint(0, V, n)
+    scale = np.float32(math.sqrt(F) * 0.7)
+    assert np.array_equal(_lookup(table, idx, kind, float(scale), offset), table[idx] * scale)
+
+
+@pytest.mark.gpu
+def test_tokens_that_name_no_row():
+    table = np.random.RandomState(0).standard_normal((10, 8)).astype(np.float32)
+    for kind, bad in (("f32", [-1, 10, 1e30, -1e30, np.nan, np.inf, -np.inf]), ("i32", [-1, 10, 2 ** 31 - 1, -2 ** 31]),
+                      ("i64", [-1, 10, 2 ** 32 + 3, -2 ** 63])):
+        idx = np.array(bad + [3], dtype=np.float64 if kind == "f32" else object)
+        out = _lookup(table, idx, kind, 2.0)
+        assert np.array_equal(out[-1], table[3] * np.float32(2)) and not out[:-1].any()
+        delta = np.ones((len(idx), 8), np.float32)
+        want = np.zeros((10, 8), np.float32)
+        want[3] = 2
+        assert np.array_equal(_update(delta, idx, kind, 10, 2.0), want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("onto", [False, True])
+@pytest.mark.parametrize("kind,n,F,V,pad,offset", [
+    ("f32", 1, 1, 1, -1, 0), ("f32", 1, 64, 9, -1, 0), ("i64", 33, 4, 1, -1, 0), ("f32", 32, 8, 2, -1, 0), ("i32", 65, 12, 3, 1, 0),
+    ("f32", 300, 24, 37, 5, 0), ("i64", 5000, 100, 7, 0, 0), ("f32", 3001, 301, 1009, 3, 0), ("i32", 2000, 516, 149, -1, 0),
+    ("i64", 4097, 256, 20000, 0, 1), ("f32", 100003, 8, 257, -1, 0), ("i32", 1000, 1, 1000003, 999999, 0), ("f32", 700, 2052, 300, -1, 0)])
+def test_gradient(kind, n, F, V, pad, offset, onto):
+    """One rounding an addition and one of the product: (additions + 2) half steps of the sum of the terms' sizes;
+    onto a table, one addition more."""
+    rng = np.random.RandomState(n + V)
+    delta = rng.standard_normal((n, F)).astype(np.float32)
+    idx = np.minimum((rng.uniform(1, V + 1, n) ** rng.uniform(0, 1, n)).astype(np.int64) - 1, V - 1).clip(0)
+    scale = float(np.float32(1.7))
+    old = rng.standard_normal((V, F)).astype(np.float32) if onto else None
+    got = _update(delta, idx, kind, V, scale, pad, old, offset)
+    want, size, count = _sums(delta, idx, V, scale, pad)
+    room = (count[:, None] + 2) * 2.0 ** -24 * size
+    if onto:
+        untouched = count == 0
+        assert np.array_equal(got[untouched], old[untouched])
+        want = want + old
+        room = room + 2.0 ** -24 * (np.abs(want) + room)
+    assert np.all(np.abs(got - want) <= room * 1.001)
+    assert np.array_equal(got, _update(delta, idx, kind, V, scale, pad, old, offset))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [31, 32, 33, 64, 65, 1000, 70001])
+def test_one_token_throughout(n):
+    """A row of many parts beside empty ones, whole numbers: exact."""
+    delta = np.random.RandomState(n).randint(-8, 9, (n, 36)).astype(np.float32)
+    for V, token in ((1, 0), (200, 149)):
+        want = np.zeros((V, 36), np.float32)
+        want[token] = delta.sum(0)
+        assert np.array_equal(_update(delta, np.full(n, token), "i32", V, 1.0), want)
+        assert not _update(delta, np.full(n, token), "i32", V, 1.0, pad=token).any()
+
+
+@pytest.mark.gpu
+def test_sums_are_added_in_the_order_of_the_tokens():
+    """Rows of at most 32 tokens: the bits of one addition after another."""
+    rng = np.random.RandomState(3)
+    delta = (rng.standard_normal((600, 20)) * 10.0 ** rng.randint(-3, 4, (600, 1))).astype(np.float32)
+    idx = np.repeat(np.arange(20), 30)
+    rng.shuffle(idx)
+    want = np.zeros((20, 20), np.float32)
+    for t, v in enumerate(idx):
+        want[v] = want[v] + delta[t]
+    assert np.array_equal(_update(delta, idx, "f32", 20, 1.0), want)
+
+
+@pytest.mark.gpu
+def test_no_tokens():
+    empty = np.zeros((0, 6), np.float32)
+    assert not _update(empty, [], "f32", 5, 1.0).any()
+    old = np.random.RandomState(0).standard_normal((5, 6)).astype(np.float32)
+    assert np.array_equal(_update(empty, [], "i64", 5, 1.0, onto=old), old)
+
+
+@pytest.mark.gpu
+def test_infinities_reach_their_rows_alone():
+    delta = np.ones((40, 8), np.float32)
+    delta[3, 2], delta[4, 5], delta[9, 0] = np.inf, np.nan, -np.inf
+    idx = np.arange(40) % 10
+    got = _update(delta, idx, "f32", 10, 1.0)
+    bad = ~np.isfinite(got)
+    assert np.array_equal(np.argwhere(bad), [[3, 2], [4, 5], [9, 0]]) and np.all(got[~bad] == 4)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,F,V,offset", [(1, 1, 1, 0), (300, 24, 37, 0), (3001, 301, 1009, 0), (900, 512, 30, 0), (500, 64, 9, 1)])
+def test_flex16(n, F, V, offset):
+    """Mantissas in and out, the largest of them, and what a measuring launch leaves."""
+    import torch
+    from ngraph_python_b200 import lib
+    rng = np.random.RandomState(n)
+    idx = rng.randint(0, V, n).astype(np.int16)
+    scale, decs = float(np.float32(math.sqrt(F))), (13, 0, 7)
+    scales = torch.tensor([[2.0 ** -d, 2.0 ** d] for d in decs], dtype=torch.float32, device="cuda")
+    x = torch.from_numpy(idx).cuda()
+    raw = lib.raw()
+
+    def device(a):
+        t = _off(a.shape, torch.int16, offset)
+        t.copy_(torch.from_numpy(a))
+        return t
+
+    def check(call, value, shape):
+        out = _off(shape, torch.int16, offset)
+        stats = torch.zeros((3,), dtype=torch.int32, device="cuda")
+        probe = torch.zeros((1,), dtype=torch.int64, device="cuda")
+        call(out, stats, probe, 1)
+        torch.cuda.synchronize()
+        assert not out.any() and not stats.any()
+        bits = np.array([int(probe.item()) & 0xffffffff], dtype=np.uint32).view(np.float32)[0]
+        assert bits == np.abs(value).max()
+        call(out, stats, probe, 0)
+        torch.cuda.synchronize()
+        want = fx.quantize(value, decs[2])
+        assert np.array_equal(out.cpu().numpy(), want)
+        assert stats.tolist() == [0, 0, fx.maxabs_stat(want)]
+
+    table = rng.randint(-30000, 30000, (V, F)).astype(np.int16)
+    w = device(table)
+    step = np.float32(2.0 ** -decs[0])
+    check(lambda out, stats, probe, p: lib.check(raw.b2_embed_fprop(
+        w.data_ptr(), x.data_ptr(), out.data_ptr(), 1, 3, V, F, n, scale, scales.data_ptr(), 0, 1, 2, stats.data_ptr(), probe.data_ptr(), p, 0)),
+        (table[idx].astype(np.float32) * step) * np.float32(scale), (n, F))
+    delta = rng.randint(-3000, 3000, (n, F)).astype(np.int16)
+    sums = np.zeros((V, F))
+    keep = idx != 0
+    np.add.at(sums, idx[keep], delta[keep].astype(np.float64))
+    assert np.abs(sums).max() < 2 ** 24                      # (exact in fp32)
+    d = device(delta)
+    nbytes = lib.embed_update_scratch_bytes(V, F, n)
+    scratch = torch.full((nbytes,), 0x5A, dtype=torch.uint8, device="cuda")
+    check(lambda out, stats, probe, p: lib.check(raw.b2_embed_update(
+        d.data_ptr(), x.data_ptr(), out.data_ptr(), 1, 3, V, F, n, scale, 0, 0, scales.data_ptr(), 0, 1, 2, stats.data_ptr(), probe.data_ptr(), p,
+        scratch.data_ptr(), nbytes, 0)),
+        (sums.astype(np.float32) * step) * np.float32(scale), (V, F))
+
+
+@pytest.mark.gpu
+def test_recorded_and_replayed_on_another_stream():
+    """Two gradients that share a scratch in one graph, replayed with other tokens."""
+    import torch
+    from ngraph_python_b200 import lib
+    V, F, n = 300, 40, 2000
+    g = torch.Generator(device="cuda")
+    g.manual_seed(1)
+    idx = torch.randint(0, V, (n,), device="cuda", generator=g)
+    deltas = [torch.randint(-8, 9, (n, F), device="cuda", generator=g).float() for _ in range(2)]
+    outs = [torch.empty((V, F), device="cuda") for _ in range(2)]
+    nbytes = lib.embed_update_scratch_bytes(V, F, n)
+    scratch = torch.empty((nbytes,), dtype=torch.uint8, device="cuda")
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+
+    def both():
+        for d, o in zip(deltas, outs):
+            lib.check(lib.raw().b2_embed_update(d.data_ptr(), idx.data_ptr(), o.data_ptr(), 0, 2, V, F, n, 1.0, -1, 0, *PLAIN, scratch.data_ptr(),
+                                                nbytes, torch.cuda.current_stream().cuda_stream))
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        both()
+        with torch.cuda.graph(graph, stream=side):
+            both()
+        for _ in range(3):
+            idx.copy_(torch.randint(0, V, (n,), device="cuda", generator=g))
+            graph.replay()
+            for d, o in zip(deltas, outs):
+                assert torch.equal(o, torch.zeros_like(o).index_add_(0, idx, d))
+    torch.cuda.synchronize()
+
+
+@pytest.mark.gpu
+def test_large_offsets():
+    """A table of more than 2^31 values, its last rows."""
+    import torch
+    from ngraph_python_b200 import lib
+    V, F = 1100001, 2048
+    table = torch.empty((V, F), device="cuda")
+    table[-3:] = torch.arange(3 * F, device="cuda").view(3, F).float()
+    idx = torch.tensor([V - 1, V - 3], dtype=torch.int32, device="cuda")
+    out = torch.empty((2, F), device="cuda")
+    lib.check(lib.raw().b2_embed_fprop(table.data_ptr(), idx.data_ptr(), out.data_ptr(), 0, 1, V, F, 2, 1.0, *PLAIN, 0))
+    assert torch.equal(out, table[idx.long()])
+    nbytes = lib.embed_update_scratch_bytes(V, F, 2)
+    scratch = torch.empty((nbytes,), dtype=torch.uint8, device="cuda")
+    lib.check(lib.raw().b2_embed_update(out.data_ptr(), idx.data_ptr(), table.data_ptr(), 0, 1, V, F, 2, 1.0, -1, 0, *PLAIN, scratch.data_ptr(),
+                                        nbytes, 0))
+    assert torch.equal(table[idx.long()], out)
+    assert int((table != 0).sum()) == int((out != 0).sum())
+
+
+def test_refusals():
+    from ngraph_python_b200 import lib
+    raw = lib.raw()
+    one = ctypes.c_void_p(256)
+    fwd = dict(table=one, idx=one, out=one, flex=0, kind=0, V=4, F=4, n=4)
+
+    def forward(**kw):
+        a = dict(fwd, **kw)
+        lib.check(raw.b2_embed_fprop(a["table"], a["idx"], a["out"], a["flex"], a["kind"], a["V"], a["F"], a["n"], 1.0, *PLAIN, 0))
+    for kw in (dict(V=0), dict(F=-1), dict(n=-1), dict(kind=4), dict(kind=-1), dict(flex=1), dict(kind=3), dict(table=None), dict(idx=None), dict(out=None)):
+        with pytest.raises(lib.B200Error, match="error -1"):
+            forward(**kw)
+    forward(n=0)
+
+    def update(onto=0, nbytes=1 << 20, scratch=one, delta=one, dW=one, flex=0, scales=PLAIN, **kw):
+        a = dict(fwd, **kw)
+        lib.check(raw.b2_embed_update(delta, a["idx"], dW, flex, a["kind"], a["V"], a["F"], a["n"], 1.0, -1, onto, *scales, scratch, nbytes, 0))
+    for kw in (dict(V=0), dict(n=-1), dict(n=1 << 31), dict(kind=9), dict(nbytes=16), dict(scratch=None), dict(delta=None), dict(dW=None), dict(flex=1),
+               dict(flex=1, onto=1, scales=(one, 0, 1, 2, one, one, 0)), dict(flex=1, scales=(one, 0, 1, 2, None, one, 0)),
+               dict(flex=1, scales=(one, 0, 1, 2, one, None, 1))):
+        with pytest.raises(lib.B200Error, match="error -1"):
+            update(**kw)
+
+
+@pytest.mark.gpu
+def test_host_memory_is_refused():
+    import torch
+    from ngraph_python_b200 import lib
+    table, idx = torch.zeros((4, 4), device="cuda"), torch.zeros((2,), device="cuda")
+    out = torch.zeros((2, 4))
+    with pytest.raises(lib.B200Error, match="device memory"):
+        lib.check(lib.raw().b2_embed_fprop(table.data_ptr(), idx.data_ptr(), out.data_ptr(), 0, 0, 4, 4, 2, 1.0, *PLAIN, 0))
