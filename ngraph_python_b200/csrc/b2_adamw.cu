@@ -144,25 +144,28 @@ adamw32_kernel(unsigned* finished, const Chunk* __restrict__ chunks, long long n
     end_step(finished, step, before);
 }
 
-// q, |q| <= 448 but for a rounding, to one of its two neighbours in e4m3: the upper one with the chance that sixteen
-// random bits give it.  The bits of a mantissa that e4m3 does not have are added to and cut off; below 2^-6, where
-// its values are 2^-9 apart, the same between 2^-6 and 2^-5.
-__device__ __forceinline__ float to_e4m3(float q, unsigned bits) {
-    const float a = fminf(fabsf(q), 448.0f);
+// The byte (without its sign) of one of the two neighbours in e4m3 of q, |q| <= 448 but for a rounding: of the upper one
+// with the chance that sixteen random bits, here in bits 4 to 19, give it.  What a mantissa has beyond e4m3's three bits is
+// added to and cut off; exponent and mantissa are the byte but for the bias, 120 * 8.  Below 2^-6, where the values
+// are 2^-9 apart, the same between 2^-6 and 2^-5, whose bytes are eight higher.  (No carry beyond 448: the bits end
+// above the roundings of q.)
+__device__ __forceinline__ unsigned to_e4m3(float q, unsigned bits) {
+    const float a = fabsf(q);
     const bool low = a < 0.015625f;
-    const float b = low ? __fadd_rn(a, 0.015625f) : a;
-    const float c = __uint_as_float((__float_as_uint(b) + (bits << 4)) & ~0xFFFFFu);
-    return low ? __fsub_rn(c, 0.015625f) : c;
+    const float b = __fadd_rn(a, low ? 0.015625f : 0.0f);
+    return (__float_as_uint(b) + bits - (low ? 0x3C8u << 20 : 0x3C0u << 20)) >> 20;
+}
+
+// the larger magnitude, NaN where there is one
+__device__ __forceinline__ float larger(float top, float x) {
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(top) : "f"(fabsf(x)));
+    return top;
 }
 
 __device__ __forceinline__ float2 from_e4m3(unsigned two) {
     const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)two, __NV_E4M3);
     return __half22float2(__half2(h));
 }
-__device__ __forceinline__ unsigned codes(float x, float y) {
-    return __nv_cvt_float2_to_fp8x2(make_float2(x, y), __NV_SATFINITE, __NV_E4M3);
-}
-
 // 448 / top and the block's scale
 __device__ __forceinline__ float scale_of(float top, float& scale) {
     const bool live = top > 7.888609052210118e-31f;             // 2^-100
@@ -171,7 +174,7 @@ __device__ __forceinline__ float scale_of(float top, float& scale) {
     return live ? __fdiv_rn(448.0f, top) : 0.0f;
 }
 
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, 4)
 adamw8_kernel(unsigned* finished, const Chunk* __restrict__ chunks, long long n_chunks, Rates r, const float* lr_at, const float* scale_at, float* step,
               unsigned seed) {
     __shared__ Now shared_now;
@@ -183,6 +186,7 @@ adamw8_kernel(unsigned* finished, const Chunk* __restrict__ chunks, long long n_
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     for (long long k = blockIdx.x; k < n_chunks; k += gridDim.x) {
         const Chunk c = chunks[k];
+        if (k + gridDim.x < n_chunks) asm volatile("prefetch.global.L1 [%0];" ::"l"(chunks + k + gridDim.x));
         const int at = warp * kBlock;
         const int n = (int)c.n - at;                    // of the warp's block
         if (n <= 0) continue;
@@ -217,18 +221,18 @@ adamw8_kernel(unsigned* finished, const Chunk* __restrict__ chunks, long long n_
             m[4 * h] = ma.x; m[4 * h + 1] = ma.y; m[4 * h + 2] = mb.x; m[4 * h + 3] = mb.y;
             v[4 * h] = va.x; v[4 * h + 1] = va.y; v[4 * h + 2] = vb.x; v[4 * h + 3] = vb.y;
         }
-        unsigned top_m = 0, top_r = 0;                  // as bits, whose order is that of the values (NaN above all)
+        float most_m = 0.0f, most_r = 0.0f;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             m[e] = __fmul_rn(m[e], ms);
             const float old = __fmul_rn(v[e], vs);
             v[e] = __fmul_rn(old, old);
             p[e] = update(r, now, keep, p[e], g[e], m[e], v[e], root[e]);
-            top_m = max(top_m, __float_as_uint(fabsf(m[e])));
-            top_r = max(top_r, __float_as_uint(fabsf(root[e])));
+            most_m = larger(most_m, m[e]);
+            most_r = larger(most_r, root[e]);
         }
-        top_m = __reduce_max_sync(0xffffffffu, top_m);
-        top_r = __reduce_max_sync(0xffffffffu, top_r);
+        // as bits, whose order is that of the values (NaN above all)
+        const unsigned top_m = __reduce_max_sync(0xffffffffu, __float_as_uint(most_m)), top_r = __reduce_max_sync(0xffffffffu, __float_as_uint(most_r));
         float new_ms, new_vs;
         const float to_m = scale_of(__uint_as_float(top_m), new_ms), to_r = scale_of(__uint_as_float(top_r), new_vs);
         if (lane == 0) {
@@ -238,17 +242,17 @@ adamw8_kernel(unsigned* finished, const Chunk* __restrict__ chunks, long long n_
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const int i = h * 128 + lane * 4;
+            unsigned mb[4], vb[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const int e = 4 * h + j;
                 const unsigned bits = mix((c.counter + (unsigned)(at + i + j)) ^ now.key);
                 const float qm = __fmul_rn(m[e], to_m), qr = __fmul_rn(root[e], to_r);
-                m[e] = copysignf(to_e4m3(qm, bits & 0xffffu), qm);
-                const float cr = to_e4m3(qr, bits >> 16);
-                root[e] = qr > 0.0f ? fmaxf(cr, 0.001953125f) : cr;
+                mb[j] = to_e4m3(qm, (bits << 4) & 0xFFFF0u) | (__float_as_uint(qm) >> 24 & 0x80u);
+                vb[j] = max(to_e4m3(qr, (bits >> 12) & 0xFFFF0u), qr > 0.0f ? 1u : 0u);
             }
-            const unsigned mw = codes(m[4 * h], m[4 * h + 1]) | codes(m[4 * h + 2], m[4 * h + 3]) << 16;
-            const unsigned vw = codes(root[4 * h], root[4 * h + 1]) | codes(root[4 * h + 2], root[4 * h + 3]) << 16;
+            const unsigned mw = __byte_perm(__byte_perm(mb[0], mb[1], 0x0040), __byte_perm(mb[2], mb[3], 0x0040), 0x5410);
+            const unsigned vw = __byte_perm(__byte_perm(vb[0], vb[1], 0x0040), __byte_perm(vb[2], vb[3], 0x0040), 0x5410);
             if (vec) {
                 *reinterpret_cast<float4*>(c.param + at + i) = make_float4(p[4 * h], p[4 * h + 1], p[4 * h + 2], p[4 * h + 3]);
                 *reinterpret_cast<unsigned*>(mc + i) = mw;

@@ -6,12 +6,10 @@
 // Both are bound by memory: one multiplication or addition a value.  The gradient is two launches.  The first
 // sorts: a CTA owns the rows v = b (mod CTAs), so that the frequent tokens of a vocabulary, which lie next to one
 // another, go to different CTAs; it reads every token, counts its own per warp, and writes their positions row by
-// row in ascending order, and a list of work items of at most kPart positions each.  No counter is shared between
-// CTAs -- where a CTA's positions begin is the number of tokens that lower CTAs own, which it counts as well -- so
-// that the order of every sum is that of the tokens, whatever runs when, and nothing has to be cleared in advance.
-// The same launch writes the zeros of rows that no token names (all but the sums is bandwidth there).  The second
-// adds: a warp takes an item and kCols columns.  Rows of more than kPart positions leave fp32 partial sums, which
-// the warp that comes last adds in their order.
+// row in ascending order.  No counter is shared between CTAs -- where a CTA's positions begin is the number of tokens
+// that lower CTAs own, which it counts as well -- so that the order of every sum is that of the tokens, whatever runs
+// when, and nothing has to be cleared in advance.  The second adds, in parts of at most kPart positions of a row; rows
+// of more leave fp32 partial sums, which the warp that comes last adds in their order.
 #include <cstdint>
 
 #include "b2_operators.h"
@@ -20,8 +18,10 @@ namespace {
 
 constexpr int kPart = 32;               // positions in one work item
 constexpr int kOrderThreads = 1024;
-constexpr int kMostRows = 6400;         // rows that a CTA of the first launch owns, at most
-constexpr int kCounters = 50000;        // words of shared memory for their counters
+constexpr int kMostRows = 4000;         // rows that a CTA of the first launch owns, at most
+constexpr int kCounters = 25000;        // words of shared memory for them
+constexpr int kListed = 128;            // own tokens that a warp remembers
+constexpr int kFlat = 2048;             // ... and a CTA
 
 struct FlexArgs {
     const b2_flex_scale* table;
@@ -31,20 +31,23 @@ struct FlexArgs {
     int probe;
 };
 
-// The token at position i, or -1 where it names no row (also for NaN).
+// How tokens of a kind are held, and the row that one names: -1 for none (also for NaN).  fp32 to the nearest row.
+template <int KIND> struct Held { using Type = float; };
+template <> struct Held<B2_IDX_I32> { using Type = int; };
+template <> struct Held<B2_IDX_I64> { using Type = long long; };
+template <> struct Held<B2_IDX_FLEX16> { using Type = short; };
+
+__device__ __forceinline__ int row_of(float x, int V, float) {
+    const int r = __float2int_rn(x);
+    return (unsigned)r < (unsigned)V && x == x ? r : -1;
+}
+__device__ __forceinline__ int row_of(int x, int V, float) { return (unsigned)x < (unsigned)V ? x : -1; }
+__device__ __forceinline__ int row_of(long long x, int V, float) { return (unsigned long long)x < (unsigned long long)V ? (int)x : -1; }
+__device__ __forceinline__ int row_of(short x, int V, float step) { return row_of(step * (float)x, V, 0.0f); }
+
 template <int KIND>
 __device__ __forceinline__ int token_at(const void* idx, long long i, int V, float step) {
-    if (KIND == B2_IDX_F32 || KIND == B2_IDX_FLEX16) {
-        const float x = KIND == B2_IDX_F32 ? static_cast<const float*>(idx)[i] : step * (float)static_cast<const short*>(idx)[i];
-        const float r = rintf(x);
-        return r >= 0.0f && r < (float)V ? (int)r : -1;
-    }
-    if (KIND == B2_IDX_I32) {
-        const int x = static_cast<const int*>(idx)[i];
-        return x >= 0 && x < V ? x : -1;
-    }
-    const long long x = static_cast<const long long*>(idx)[i];
-    return x >= 0 && x < V ? (int)x : -1;
+    return row_of(static_cast<const typename Held<KIND>::Type*>(idx)[i], V, step);
 }
 
 // V values next to one another, fp32 or mantissas
@@ -175,22 +178,29 @@ embed_kernel(const T* __restrict__ table, const void* __restrict__ idx, T* __res
 }
 
 // ---- gradient: order ----------------------------------------------------------------------------------------
-struct Item {
-    int row, first, count, slot;        // slot: where its partial sums go, -1 for a whole row
-    int slot0, parts, pad0, pad1;       // of the row
+// A position in the sorted list: of `count` positions of its row it is number `rank`.  row -1: none.
+struct Entry {
+    int pos, row, rank, count;
 };
 
 struct Scratch {
-    int* sorted;                        // [n] positions
-    Item* items;                        // [n], those with count 0 are none
+    Entry* sorted;                      // [n]
+    unsigned char* used;                // [CTAs][rows of one]: whether a token names the row
     unsigned* tickets;                  // [slots][column blocks]
     float* partial;                     // [slots][F]
     size_t bytes;
 };
 
+// CTAs of the first launch, and rows that each owns
+int owners_of(int V) {
+    const int least = (int)(((long long)V + kMostRows - 1) / kMostRows);
+    const int most = V < b2::kSms ? V : b2::kSms;
+    return most > least ? most : least;
+}
+
 // 2n / kPart + 2 slots: the ceil(c / kPart) parts of a row of c > kPart positions from `start` on fit between
 // 2 start / kPart and 2 (start + c) / kPart, where the next row's begin.
-Scratch scratch_of(void* base, int F, long long n, int col_blocks) {
+Scratch scratch_of(void* base, int V, int F, long long n, int col_blocks) {
     Scratch s;
     size_t at = 0;
     auto take = [&](size_t bytes) {
@@ -199,8 +209,8 @@ Scratch scratch_of(void* base, int F, long long n, int col_blocks) {
         return p;
     };
     const size_t slots = 2 * (size_t)n / kPart + 2;
-    s.items = reinterpret_cast<Item*>(take(n * sizeof(Item)));
-    s.sorted = reinterpret_cast<int*>(take(n * sizeof(int)));
+    s.sorted = reinterpret_cast<Entry*>(take(n * sizeof(Entry)));
+    s.used = reinterpret_cast<unsigned char*>(take((size_t)V + owners_of(V)));
     s.tickets = reinterpret_cast<unsigned*>(take(slots * col_blocks * sizeof(unsigned)));
     s.partial = reinterpret_cast<float*>(take(slots * (size_t)F * sizeof(float)));
     s.bytes = at;
@@ -209,7 +219,7 @@ Scratch scratch_of(void* base, int F, long long n, int col_blocks) {
 
 struct OrderArgs {
     const void* idx;
-    int V, F, n, rows, warps, pad, col_blocks;
+    int V, n, rows, warps, stride, pad, col_blocks;
     unsigned magic;                     // 2^32 / CTAs, rounded up
     Scratch s;
     const b2_flex_scale* table;
@@ -242,135 +252,164 @@ __device__ __forceinline__ unsigned block_scan(unsigned v, unsigned* sums, unsig
     return x - v + (warp ? sums[warp - 1] : 0u);
 }
 
-template <typename T>
-__device__ __forceinline__ void zero_row(T* p, int F, int lane) {
-    const int head = min(F, (int)((-(reinterpret_cast<uintptr_t>(p) / sizeof(T))) & (16 / sizeof(T) - 1)));
-    if (lane < head) p[lane] = (T)0;
-    const int vecs = (F - head) / (int)(16 / sizeof(T));
-    for (int i = lane; i < vecs; i += 32) reinterpret_cast<int4*>(p + head)[i] = make_int4(0, 0, 0, 0);
-    for (int i = head + vecs * (int)(16 / sizeof(T)) + lane; i < F; i += 32) p[i] = (T)0;
-}
-
-// `zeros`: the table of sums, whose rows without tokens become zero here; NULL where sums are added onto it.
-template <typename T, int KIND>
+// A CTA remembers its own tokens in the order of their positions (every warp a list, then one list of all).  One warp
+// goes through that, 32 at a time, and numbers the positions of each row; rows get their places in the order in which
+// they come up.  A CTA of more than kFlat tokens reads all tokens again: it counts rows per warp, and then places.
+template <int KIND>
 __global__ void __launch_bounds__(kOrderThreads)
-order_kernel(const OrderArgs a, T* __restrict__ zeros) {
-    extern __shared__ unsigned counters[];      // [warps][rows], then [rows] sums
-    __shared__ unsigned sums[33];
-    after_earlier_kernels();
+order_kernel(const OrderArgs a) {
+    extern __shared__ __align__(16) unsigned room[];
+    __shared__ unsigned sums[33], found_by[32];
+    constexpr int WARPS = kOrderThreads / 32;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const unsigned G = gridDim.x, b = blockIdx.x;
     const int rows = a.rows;
-    unsigned* mine = counters + (size_t)warp * rows;
-    unsigned* whole = counters + (size_t)a.warps * rows;
+    unsigned* whole = room;                     // [rows] positions of each row, then [rows] where they begin
+    unsigned* first = room + rows;
+    uint2* lists = reinterpret_cast<uint2*>(room + (2 * rows + 3) / 4 * 4);     // [WARPS][kListed] position and row
+    uint2* flat = lists + WARPS * kListed;
+    unsigned* ranks = reinterpret_cast<unsigned*>(flat + kFlat);
+    for (int i = threadIdx.x; i < rows; i += kOrderThreads) whole[i] = 0;
+    after_earlier_kernels();
     const float istep = KIND == B2_IDX_FLEX16 ? a.table[a.slot_idx].scale : 1.0f;
-    for (int i = threadIdx.x; i < a.warps * rows; i += kOrderThreads) counters[i] = 0;
-    __syncthreads();
-    // a warp's share of the positions, in whole lines of 32
-    const int per = ((a.n + a.warps - 1) / a.warps + 31) / 32 * 32;
-    const long long from = (long long)warp * per;
-    const int begin = (int)min(from, (long long)a.n), end = warp < a.warps ? (int)min(from + per, (long long)a.n) : begin;
 
-    constexpr int UN = 8;
-    // token -> row within the CTA (v / G) and owner (v % G); the estimate of the quotient is at most one too high
-    auto split = [&](int v, int& local) {
-        unsigned q = __umulhi((unsigned)v, a.magic);
-        int r = v - (int)(q * G);
-        if (r < 0) { --q; r += (int)G; }
-        if (r >= (int)G) { ++q; r -= (int)G; }      // (one CTA: its 2^32 has no word)
-        local = (int)q;
-        return (unsigned)r;
+    // the tokens of a warp's share of the positions, 32 at a time: visit(owner, row of the owner, position), by whole
+    // warps; owner G for none
+    auto tokens = [&](int warps, auto visit) {
+        using Type = typename Held<KIND>::Type;
+        constexpr int UN = 8;
+        const int per = ((a.n + warps - 1) / warps + 31) / 32 * 32;
+        const long long from = (long long)warp * per;
+        const int begin = (int)min(from, (long long)a.n), end = warp < warps ? (int)min(from + per, (long long)a.n) : begin;
+        const Type* list = static_cast<const Type*>(a.idx) + lane;
+        for (int at = begin; at < end; at += 32 * UN) {
+            Type x[UN];
+            if (at + 32 * UN <= end) {
+#pragma unroll
+                for (int u = 0; u < UN; ++u) x[u] = list[at + u * 32];
+            } else {
+#pragma unroll
+                for (int u = 0; u < UN; ++u) x[u] = at + u * 32 + lane < end ? list[at + u * 32] : (Type)-1;
+            }
+#pragma unroll
+            for (int u = 0; u < UN; ++u) {
+                const int v = row_of(x[u], a.V, istep);
+                // v / G, at most one too high, and v % G
+                unsigned q = __umulhi((unsigned)v, a.magic);
+                int r = v - (int)(q * G);
+                if (r < 0) { --q; r += (int)G; }
+                visit(v >= 0 && v != a.pad ? (unsigned)r : G, (int)q, at + u * 32 + lane);
+            }
+        }
     };
-    unsigned lower = 0;
-    for (int at = begin; at < end; at += 32 * UN) {
-        int tok[UN];
-#pragma unroll
-        for (int u = 0; u < UN; ++u) {
-            const int i = at + u * 32 + lane;
-            tok[u] = i < end ? token_at<KIND>(a.idx, i, a.V, istep) : -1;
-        }
-#pragma unroll
-        for (int u = 0; u < UN; ++u) {
-            if (tok[u] < 0 || tok[u] == a.pad) continue;
-            int local;
-            const unsigned owner = split(tok[u], local);
-            if (owner == b) atomicAdd(mine + local, 1u);
-            lower += owner < b;
-        }
-    }
+    unsigned lower = 0, found = 0;
+    tokens(WARPS, [&](unsigned owner, int local, int pos) {
+        lower += owner < b;
+        const unsigned those = __ballot_sync(0xffffffffu, owner == b);
+        if (!those) return;
+        const unsigned k = found + __popc(those & ((1u << lane) - 1u));
+        if (owner == b && k < kListed) lists[warp * kListed + k] = make_uint2((unsigned)pos, (unsigned)local);
+        found += __popc(those);
+    });
+    if (lane == 0) found_by[warp] = found;
     unsigned start;
-    block_scan(lower, sums, start);             // (its barriers also end the counting)
-    // counters become where each warp's positions of each row begin; rows' items are listed
-    unsigned items = start, begun = start;
-    for (int r0 = 0; r0 < rows; r0 += kOrderThreads) {
-        const int r = r0 + threadIdx.x;
-        unsigned c = 0;
-        if (r < rows)
-            for (int w = 0; w < a.warps; ++w) {
-                const unsigned x = counters[(size_t)w * rows + r];
-                counters[(size_t)w * rows + r] = c;
-                c += x;
-            }
-        unsigned all_c, all_p;
-        const unsigned first = begun + block_scan(c, sums, all_c);
-        const unsigned parts = (c + kPart - 1) / kPart;
-        const unsigned item = items + block_scan(parts, sums, all_p);
-        if (r < rows) {
-            whole[r] = c;
-            for (int w = 0; w < a.warps; ++w) counters[(size_t)w * rows + r] += first;
-            const int row = (int)(b + (unsigned)r * G);
-            const int slot0 = (int)(2ull * first / kPart);
-            for (unsigned p = 0; p < parts; ++p) {
-                Item it;
-                it.row = row;
-                it.first = (int)(first + p * kPart);
-                it.count = (int)min((unsigned)kPart, c - p * kPart);
-                it.slot = parts > 1 ? slot0 + (int)p : -1;
-                it.slot0 = slot0;
-                it.parts = (int)parts;
-                it.pad0 = it.pad1 = 0;
-                a.s.items[item + p] = it;
-            }
-            if (parts > 1)
-                for (int k = 0; k < a.col_blocks; ++k) a.s.tickets[(size_t)slot0 * a.col_blocks + k] = 0;
-        }
-        begun += all_c;
-        items += all_p;
+    block_scan(lower, sums, start);             // (its barriers stand behind the lists, too)
+    unsigned before = 0, all = 0, most = 0;
+    {
+        const unsigned c = found_by[lane];
+        all = __reduce_add_sync(0xffffffffu, c);
+        most = __reduce_max_sync(0xffffffffu, c);
+        before = __reduce_add_sync(0xffffffffu, lane < warp ? c : 0u);
     }
-    // items that are none: up to where the next CTA's begin, the last CTA's up to n
-    const unsigned last = b + 1 == G ? (unsigned)a.n : begun;
-    for (unsigned i = items + threadIdx.x; i < last; i += kOrderThreads) a.s.items[i].count = 0;
-    __syncthreads();
-    if (zeros)
-        for (int r = warp; r < rows; r += kOrderThreads / 32) {
-            const long long row = (long long)b + (long long)r * G;
-            if (row < a.V && whole[r] == 0) zero_row(zeros + row * a.F, a.F, lane);
+    auto begin_row = [&](unsigned c, unsigned at) {
+        if (c > kPart)
+            for (int k = 0; k < a.col_blocks; ++k) a.s.tickets[(size_t)(2ull * at / kPart) * a.col_blocks + k] = 0;
+    };
+    auto put_entry = [&](unsigned pos, unsigned local, unsigned rank) {
+        *reinterpret_cast<int4*>(a.s.sorted + first[local] + rank) = make_int4((int)pos, (int)(b + local * G), (int)rank, (int)whole[local]);
+    };
+    if (most <= kListed && all <= kFlat) {
+        for (unsigned k = lane; k < found; k += 32) flat[before + k] = lists[warp * kListed + k];
+        __syncthreads();
+        if (warp == 0)
+            for (unsigned k = lane; k - lane < all; k += 32) {
+                const unsigned mine = k < all ? flat[k].y : 0xffffffffu;
+                const unsigned same = __match_any_sync(0xffffffffu, mine);
+                const unsigned c = k < all ? whole[mine] : 0u, place = __popc(same & ((1u << lane) - 1u));
+                __syncwarp();
+                if (k < all) {
+                    ranks[k] = c + place;
+                    if (place == 0) whole[mine] = c + __popc(same);
+                }
+                __syncwarp();
+            }
+        __syncthreads();
+        unsigned at = start;
+        for (unsigned k0 = 0; k0 < all; k0 += kOrderThreads) {
+            const unsigned k = k0 + threadIdx.x;
+            const unsigned c = k < all && ranks[k] == 0 ? whole[flat[k].y] : 0u;
+            unsigned total;
+            const unsigned mine = at + block_scan(c, sums, total);
+            if (c) {
+                first[flat[k].y] = mine;
+                begin_row(c, mine);
+            }
+            at += total;
         }
-    // positions, in the order of the tokens
-    for (int at = begin; at < end; at += 32 * UN) {
-        int tok[UN];
+        start = at;
+        __syncthreads();
+        for (unsigned k = threadIdx.x; k < all; k += kOrderThreads) put_entry(flat[k].x, flat[k].y, ranks[k]);
+    } else {
+        unsigned* counters = room + 2 * rows;   // [rows][stride], a word for each warp
+        for (int i = threadIdx.x; i < rows * a.stride; i += kOrderThreads) counters[i] = 0;
+        __syncthreads();
+        tokens(a.warps, [&](unsigned owner, int local, int) {
+            if (owner == b) atomicAdd(counters + (size_t)local * a.stride + warp, 1u);
+        });
+        __syncthreads();
+        // a row's counters become where each warp's positions begin among the row's
+        for (int r = warp; r < rows; r += WARPS) {
+            unsigned* c = counters + (size_t)r * a.stride;
+            const unsigned v = lane < a.warps ? c[lane] : 0u;
+            unsigned x = v;
 #pragma unroll
-        for (int u = 0; u < UN; ++u) {
-            const int i = at + u * 32 + lane;
-            tok[u] = i < end ? token_at<KIND>(a.idx, i, a.V, istep) : -1;
+            for (int o = 1; o < 32; o <<= 1) {
+                const unsigned y = __shfl_up_sync(0xffffffffu, x, o);
+                if (lane >= o) x += y;
+            }
+            if (lane < a.warps) c[lane] = x - v;
+            if (lane == 31) whole[r] = x;
         }
-#pragma unroll
-        for (int u = 0; u < UN; ++u) {
-            int local = 0;
-            const bool ours = tok[u] >= 0 && tok[u] != a.pad && split(tok[u], local) == b;
-            const unsigned those = __ballot_sync(0xffffffffu, ours);
-            if (!those) continue;
-            if (ours) {
+        __syncthreads();
+        for (int r0 = 0; r0 < rows; r0 += kOrderThreads) {
+            const int r = r0 + threadIdx.x;
+            const unsigned c = r < rows ? whole[r] : 0u;
+            unsigned total;
+            const unsigned mine = start + block_scan(c, sums, total);
+            if (r < rows) {
+                first[r] = mine;
+                begin_row(c, mine);
+            }
+            start += total;
+        }
+        __syncthreads();
+        tokens(a.warps, [&](unsigned owner, int local, int pos) {
+            const unsigned those = __ballot_sync(0xffffffffu, owner == b);
+            if (!those) return;
+            if (owner == b) {
+                unsigned* c = counters + (size_t)local * a.stride + warp;
                 const unsigned same = __match_any_sync(those, local);
-                const unsigned before = mine[local];
+                const unsigned rank = *c, place = __popc(same & ((1u << lane) - 1u));
                 __syncwarp(those);
-                const int rank = __popc(same & ((1u << lane) - 1u));
-                a.s.sorted[before + rank] = at + u * 32 + lane;
-                if (rank == 0) mine[local] = before + __popc(same);
+                put_entry((unsigned)pos, (unsigned)local, rank + place);
+                if (place == 0) *c = rank + __popc(same);
             }
             __syncwarp();
-        }
+        });
     }
+    for (int r = threadIdx.x; r < rows; r += kOrderThreads) a.s.used[(size_t)b * rows + r] = whole[r] != 0;
+    if (b + 1 == G)                             // what is left is nobody's: tokens that name no row, or pad
+        for (unsigned i = start + threadIdx.x; i < (unsigned)a.n; i += kOrderThreads) a.s.sorted[i].row = -1;
 }
 
 // ---- gradient: sums -------------------------------------------------------------------------------------------
@@ -385,105 +424,196 @@ __device__ __forceinline__ void put_sums(float* p, const float* v) {
     }
 }
 template <int VEC>
-__device__ __forceinline__ void add_sums(const float* p, float* v) {
+__device__ __forceinline__ void get_sums(const float* p, float* v) {
     if constexpr (VEC % 4 == 0) {
 #pragma unroll
         for (int k = 0; k < VEC; k += 4) {
             const float4 w = __ldcg(reinterpret_cast<const float4*>(p + k));
-            v[k] += w.x; v[k + 1] += w.y; v[k + 2] += w.z; v[k + 3] += w.w;
+            v[k] = w.x; v[k + 1] = w.y; v[k + 2] = w.z; v[k + 3] = w.w;
         }
     } else {
-        v[0] += __ldcg(p);
+        v[0] = __ldcg(p);
     }
 }
 
-// A warp takes an item and 32 * VEC * UN columns.
-template <typename T, int VEC, int UN>
+template <typename T>
+__device__ __forceinline__ void zero_row(T* p, int F, int lane) {
+    const int head = min(F, (int)((-(reinterpret_cast<uintptr_t>(p) / sizeof(T))) & (16 / sizeof(T) - 1)));
+    if (lane < head) p[lane] = (T)0;
+    const int vecs = (F - head) / (int)(16 / sizeof(T));
+    for (int i = lane; i < vecs; i += 32) reinterpret_cast<int4*>(p + head)[i] = make_int4(0, 0, 0, 0);
+    for (int i = head + vecs * (int)(16 / sizeof(T)) + lane; i < F; i += 32) p[i] = (T)0;
+}
+
+struct SumArgs {
+    int V, F, n, rows, owners, zero_rows;      // rows without tokens are looked for among zero_rows by a warp
+    unsigned col_blocks, sum_blocks;
+    float scale;
+    Scratch s;
+};
+
+// A warp takes the parts that begin among kWindow places of the sorted list, and 32 * VEC * UN columns: first the
+// tokens of these places, loaded together whatever rows they belong to, then what the last part has beyond them, eight
+// at a time.  So a thousand tokens that occur once cost little more than one that occurs a thousand times.  The blocks
+// behind the first sum_blocks write the zeros of rows that no token names.  Windows of 4 against 8 and 16: 8192 x 1024 into 32000 rows 42, 43
+// and 46 us a call, 3001 x 301 flex16 18, 20 and 23.
+constexpr int kWindow = 4;
+
+template <typename T, int VEC, int UN, bool ONTO>
 __global__ void __launch_bounds__(256)
-sum_kernel(const T* __restrict__ delta, T* __restrict__ dW, int F, int n, float scale, int onto, int col_blocks, Scratch s, FlexArgs f) {
+sum_kernel(const T* __restrict__ delta, T* dW, const SumArgs a, const FlexArgs f) {
     after_earlier_kernels();
     constexpr int COLS = 32 * VEC;
-    const bool flex = sizeof(T) == 2;
+    constexpr bool flex = sizeof(T) == 2;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    if (blockIdx.x >= a.sum_blocks) {
+        const long long from = ((long long)(blockIdx.x - a.sum_blocks) * 8 + warp) * a.zero_rows, mine = from + lane;
+        const bool empty = lane < a.zero_rows && mine < (long long)a.owners * a.rows && !a.s.used[mine];
+        for (unsigned left = __ballot_sync(0xffffffffu, empty); left; left &= left - 1) {
+            const unsigned k = (unsigned)(from + __ffs(left) - 1);
+            const long long row = k / (unsigned)a.rows + (long long)(k % (unsigned)a.rows) * a.owners;
+            if (row < a.V) zero_row(dW + row * a.F, a.F, lane);
+        }
+        return;
+    }
+    const int F = a.F, block = blockIdx.x % a.col_blocks;
     const float step = flex ? f.table[f.slot_in].scale : 1.0f;
     Sink<T, VEC> sink(f);
-    const int lane = threadIdx.x & 31;
-    const long long units = (long long)n * col_blocks;
-    for (long long unit = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); unit < units; unit += (long long)gridDim.x * 8) {
-        const int which = (int)(unit / col_blocks), block = (int)(unit - (long long)which * col_blocks);
-        const int4 it = *reinterpret_cast<const int4*>(s.items + which);
-        const int row = it.x, first = it.y, count = it.z, slot = it.w;
-        if (count == 0) continue;
+    const int base = (int)(blockIdx.x / a.col_blocks * 8 + warp) * kWindow;
+    // entries of this window and of what a part that begins in it can reach
+    const int4 none = make_int4(0, -1, 0, 0);
+    const int4* list = reinterpret_cast<const int4*>(a.s.sorted);
+    const int4 near = base + lane < a.n ? list[base + lane] : none;
+    const int far = lane < kWindow && base + 32 + lane < a.n ? list[base + 32 + lane].x : 0;
+    // parts begin where the rank is a multiple of kPart; the last of this window ends where its row or its 32 do
+    const unsigned those = __ballot_sync(0xffffffffu, lane < kWindow && near.y >= 0 && near.z % kPart == 0);
+    if (those) {
+        const int from = __ffs(those) - 1, last = 31 - __clz(those);
+        const int upto = last + __shfl_sync(0xffffffffu, min(kPart, near.w - near.z), last);
         const int col0 = block * COLS * UN + lane * VEC;
         float acc[UN][VEC] = {};
-        const int at = lane < count ? s.sorted[first + lane] : 0;
-        constexpr int AHEAD = 4;
-        for (int j = 0; j < count; j += AHEAD) {
-            Pack<T, VEC> w[AHEAD][UN];
+        int join_row[2] = {-1, -1}, join_slot[2], join_parts[2];
+        auto store = [&](int row, const Pack<T, VEC>* old) {
+            T* p = dW + (long long)row * F + col0;
 #pragma unroll
-            for (int a = 0; a < AHEAD; ++a) {
-                const long long t = __shfl_sync(0xffffffffu, at, (j + a) & 31);
+            for (int u = 0; u < UN; ++u) {
+                if (col0 + u * COLS >= F) continue;
+                float v[VEC];
 #pragma unroll
-                for (int u = 0; u < UN; ++u)
-                    if (j + a < count && col0 + u * COLS < F) w[a][u].load(delta + t * F + col0 + u * COLS);
+                for (int c = 0; c < VEC; ++c) v[c] = flex ? (acc[u][c] * step) * a.scale : acc[u][c] * a.scale;
+                if constexpr (ONTO) {
+                    float o[VEC];
+                    old[u].get(o);
+#pragma unroll
+                    for (int c = 0; c < VEC; ++c) v[c] = o[c] + v[c];
+                }
+                sink.put(p + u * COLS, v);
             }
-#pragma unroll
-            for (int a = 0; a < AHEAD; ++a)
-#pragma unroll
-                for (int u = 0; u < UN; ++u)
-                    if (j + a < count && col0 + u * COLS < F) {
-                        float v[VEC];
-                        w[a][u].get(v);
-#pragma unroll
-                        for (int k = 0; k < VEC; ++k) acc[u][k] += v[k];
-                    }
-        }
-        if (slot >= 0) {
-            const int4 more = reinterpret_cast<const int4*>(s.items + which)[1];
-            const int slot0 = more.x, parts = more.y;
+        };
+        auto load = [&](const T* from_row, Pack<T, VEC>* w) {
 #pragma unroll
             for (int u = 0; u < UN; ++u)
-                if (col0 + u * COLS < F) put_sums<VEC>(s.partial + (long long)slot * F + col0 + u * COLS, acc[u]);
+                if (col0 + u * COLS < F) w[u].load(from_row + col0 + u * COLS);
+        };
+        auto add = [&](const Pack<T, VEC>* w) {
+#pragma unroll
+            for (int u = 0; u < UN; ++u)
+                if (col0 + u * COLS < F) {
+                    float v[VEC];
+                    w[u].get(v);
+#pragma unroll
+                    for (int c = 0; c < VEC; ++c) acc[u][c] += v[c];
+                }
+        };
+        // a part of a row of several ends: `at` is its last place
+        auto leave = [&](int which, int at, int row, int rank, int count) {
+            join_row[which] = row;
+            join_slot[which] = (int)(2ll * (base + at - rank) / kPart);
+            join_parts[which] = (count + kPart - 1) / kPart;
+#pragma unroll
+            for (int u = 0; u < UN; ++u)
+                if (col0 + u * COLS < F) put_sums<VEC>(a.s.partial + (long long)(join_slot[which] + rank / kPart) * F + col0 + u * COLS, acc[u]);
+        };
+        Pack<T, VEC> w[kWindow][UN], old[ONTO ? kWindow : 1][UN];
+#pragma unroll
+        for (int k = 0; k < kWindow; ++k) {
+            const long long t = __shfl_sync(0xffffffffu, near.x, k);
+            const int row = __shfl_sync(0xffffffffu, near.y, k), rank = __shfl_sync(0xffffffffu, near.z, k), count = __shfl_sync(0xffffffffu, near.w, k);
+            if (k < from || k >= upto) continue;
+            load(delta + t * F, w[k]);
+            if constexpr (ONTO)
+                if (count <= kPart && rank + 1 == count) load(dW + (long long)row * F, old[k]);
+        }
+#pragma unroll
+        for (int k = 0; k < kWindow; ++k) {
+            const int row = __shfl_sync(0xffffffffu, near.y, k), rank = __shfl_sync(0xffffffffu, near.z, k), count = __shfl_sync(0xffffffffu, near.w, k);
+            if (k < from || k >= upto) continue;
+            add(w[k]);
+            if (rank + 1 != count && rank % kPart != kPart - 1) continue;
+            if (count <= kPart) store(row, old[ONTO ? k : 0]);
+            else leave(0, k, row, rank, count);
+#pragma unroll
+            for (int u = 0; u < UN; ++u)
+#pragma unroll
+                for (int c = 0; c < VEC; ++c) acc[u][c] = 0.0f;
+        }
+        if (upto > kWindow) {
+            const int row = __shfl_sync(0xffffffffu, near.y, last), rank = __shfl_sync(0xffffffffu, near.z, last) + upto - 1 - last,
+                      count = __shfl_sync(0xffffffffu, near.w, last);
+            if constexpr (ONTO)
+                if (count <= kPart) load(dW + (long long)row * F, old[0]);
+            constexpr int AHEAD = UN == 1 ? 8 : 4;
+            for (int j = kWindow; j < upto; j += AHEAD) {
+                Pack<T, VEC> x[AHEAD][UN];
+#pragma unroll
+                for (int k = 0; k < AHEAD; ++k) {
+                    const int at = j + k;
+                    const long long t = __shfl_sync(0xffffffffu, at < 32 ? near.x : far, at & 31);
+                    if (at < upto) load(delta + t * F, x[k]);
+                }
+#pragma unroll
+                for (int k = 0; k < AHEAD; ++k)
+                    if (j + k < upto) add(x[k]);
+            }
+            if (count <= kPart) store(row, old[0]);
+            else leave(1, upto - 1, row, rank, count);
+        }
+        if (join_row[0] >= 0 || join_row[1] >= 0) {
             __threadfence();
             __syncwarp();
-            unsigned came = 0;
-            if (lane == 0) came = atomicAdd(s.tickets + (long long)slot0 * col_blocks + block, 1u);
-            came = __shfl_sync(0xffffffffu, came, 0);
-            if (came + 1 != (unsigned)parts) continue;
-            __threadfence();
 #pragma unroll
-            for (int u = 0; u < UN; ++u)
+            for (int which = 0; which < 2; ++which) {
+                if (join_row[which] < 0) continue;
+                const int parts = join_parts[which];
+                unsigned came = 0;
+                if (lane == 0) came = atomicAdd(a.s.tickets + (long long)join_slot[which] * a.col_blocks + block, 1u);
+                if (__shfl_sync(0xffffffffu, came, 0) + 1 != (unsigned)parts) continue;
+                __threadfence();
+                const float* p = a.s.partial + (long long)join_slot[which] * F + col0;
 #pragma unroll
-                for (int k = 0; k < VEC; ++k) acc[u][k] = 0.0f;
-            for (int p = 0; p < parts; ++p)
+                for (int u = 0; u < UN; ++u) {
 #pragma unroll
-                for (int u = 0; u < UN; ++u)
-                    if (col0 + u * COLS < F) add_sums<VEC>(s.partial + (long long)(slot0 + p) * F + col0 + u * COLS, acc[u]);
-        }
+                    for (int c = 0; c < VEC; ++c) acc[u][c] = 0.0f;
+                    if (col0 + u * COLS >= F) continue;
+                    for (int q = 0; q < parts; q += 8) {
+                        float v[8][VEC];
 #pragma unroll
-        for (int u = 0; u < UN; ++u) {
-            const int col = col0 + u * COLS;
-            if (col >= F) break;
-            T* p = dW + (long long)row * F + col;
-            float v[VEC];
+                        for (int x = 0; x < 8; ++x)
+                            if (q + x < parts) get_sums<VEC>(p + (long long)(q + x) * F + u * COLS, v[x]);
 #pragma unroll
-            for (int k = 0; k < VEC; ++k) v[k] = flex ? (acc[u][k] * step) * scale : acc[u][k] * scale;
-            if (!flex && onto) {
-                Pack<T, VEC> old;
-                old.load(p);
-                float o[VEC];
-                old.get(o);
+                        for (int x = 0; x < 8; ++x)
+                            if (q + x < parts)
 #pragma unroll
-                for (int k = 0; k < VEC; ++k) v[k] = o[k] + v[k];
+                                for (int c = 0; c < VEC; ++c) acc[u][c] += v[x][c];
+                    }
+                }
+                if constexpr (ONTO) load(dW + (long long)join_row[which] * F, old[0]);
+                store(join_row[which], old[0]);
             }
-            sink.put(p, v);
         }
     }
     sink.done(f);
 }
-
-// columns of a warp of sum_kernel in vectors of VEC
-constexpr int kUn = 2;
-int col_blocks_of(int F, int vec) { return (F + 32 * vec * kUn - 1) / (32 * vec * kUn); }
 
 template <typename T> constexpr int wide() { return 16 / (int)sizeof(T); }
 
@@ -506,49 +636,66 @@ int launch_embed(const void* table, const void* idx, void* out, int V, int F, lo
     return B2_OK;
 }
 
-template <typename T, int KIND>
-int launch_order(OrderArgs a, T* zeros, cudaStream_t st) {
+// Columns of a warp: 16 bytes to a lane, or four values apart where rows are not aligned.
+constexpr int kApart = 4;
+int col_blocks_of(int F, int vec) {
+    const int cols = vec > 1 ? 32 * vec : 32 * kApart;
+    return (F + cols - 1) / cols;
+}
+
+template <int KIND>
+int launch_order(const OrderArgs& a, int owners, cudaStream_t st) {
     static std::atomic<unsigned long long> done{0};
-    B2_CHECK(b2::allow_shared((const void*)order_kernel<T, KIND>, (kCounters + kMostRows) * 4, &done));
-    int ctas = a.V < b2::kSms ? a.V : b2::kSms;
-    const int least = (int)(((long long)a.V + kMostRows - 1) / kMostRows);
-    if (ctas < least) ctas = least;
-    a.rows = (a.V + ctas - 1) / ctas;
-    a.magic = ctas == 1 ? 0xffffffffu : (unsigned)((1ull << 32) / ctas + 1);
-    a.warps = kCounters / a.rows - 1;
-    if (a.warps > kOrderThreads / 32) a.warps = kOrderThreads / 32;
-    const size_t smem = (size_t)(a.warps + 1) * a.rows * 4;
-    B2_CUDA((b2::launch_after(order_kernel<T, KIND>, dim3((unsigned)ctas), kOrderThreads, smem, st, a, zeros)));
+    B2_CHECK(b2::allow_shared((const void*)order_kernel<KIND>, kCounters * 4, &done));
+    const size_t many = (size_t)a.rows * (a.stride + 2) * 4, few = (size_t)(2 * a.rows + 3) / 4 * 16 + kOrderThreads / 32 * kListed * 8 + kFlat * 12;
+    B2_CUDA((b2::launch_after(order_kernel<KIND>, dim3((unsigned)owners), kOrderThreads, many > few ? many : few, st, a)));
     return B2_OK;
 }
 
 template <typename T>
 int launch_update(const void* delta, const void* idx, void* dW, int kind, int V, int F, long long n, float scale, int pad, int onto, const FlexArgs& f,
                   void* scratch, cudaStream_t st) {
+    if (n == 0 && (onto || f.probe)) return B2_OK;
     constexpr int W = wide<T>();
     const bool vec = F % W == 0 && b2::aligned16(delta) && b2::aligned16(dW);
+    const int owners = owners_of(V);
     OrderArgs a;
     a.idx = idx;
     a.V = V;
-    a.F = F;
     a.n = (int)n;
     a.pad = pad;
+    a.rows = (V + owners - 1) / owners;
+    a.warps = kCounters / a.rows - 3;           // (a word for each, made odd, and two more)
+    if (a.warps > kOrderThreads / 32) a.warps = kOrderThreads / 32;
+    a.stride = a.warps | 1;
+    a.magic = owners == 1 ? 0u : (unsigned)((1ull << 32) / owners + 1);     // (one owner has one row)
     a.col_blocks = col_blocks_of(F, vec ? W : 1);
-    a.s = scratch_of(scratch, F, n, a.col_blocks);
+    a.s = scratch_of(scratch, V, F, n, a.col_blocks);
     a.table = f.table;
     a.slot_idx = f.slot_idx;
-    T* zeros = onto || f.probe ? nullptr : (T*)dW;
-    if (kind == B2_IDX_F32) B2_CHECK((launch_order<T, B2_IDX_F32>(a, zeros, st)));
-    else if (kind == B2_IDX_I32) B2_CHECK((launch_order<T, B2_IDX_I32>(a, zeros, st)));
-    else if (kind == B2_IDX_I64) B2_CHECK((launch_order<T, B2_IDX_I64>(a, zeros, st)));
-    else B2_CHECK((launch_order<T, B2_IDX_FLEX16>(a, zeros, st)));
-    if (n == 0) return B2_OK;
-    long long blocks = (n * a.col_blocks + 7) / 8;
-    if (blocks > b2::kSms * 8) blocks = b2::kSms * 8;
-    if (vec)
-        B2_CUDA((b2::launch_after(sum_kernel<T, W, kUn>, dim3((unsigned)blocks), 256, 0, st, (const T*)delta, (T*)dW, F, (int)n, scale, onto, a.col_blocks, a.s, f)));
-    else
-        B2_CUDA((b2::launch_after(sum_kernel<T, 1, kUn>, dim3((unsigned)blocks), 256, 0, st, (const T*)delta, (T*)dW, F, (int)n, scale, onto, a.col_blocks, a.s, f)));
+    switch (kind) {
+        case B2_IDX_F32: B2_CHECK(launch_order<B2_IDX_F32>(a, owners, st)); break;
+        case B2_IDX_I32: B2_CHECK(launch_order<B2_IDX_I32>(a, owners, st)); break;
+        case B2_IDX_I64: B2_CHECK(launch_order<B2_IDX_I64>(a, owners, st)); break;
+        default: B2_CHECK(launch_order<B2_IDX_FLEX16>(a, owners, st));
+    }
+    const long long sum_blocks = (n + 8 * kWindow - 1) / (8 * kWindow) * a.col_blocks;
+    // about 16 KB of zeros to a warp
+    const long long fit = 16384 / ((long long)F * (long long)sizeof(T));
+    const int zero_rows = fit < 1 ? 1 : fit > 32 ? 32 : (int)fit;
+    const long long zero_blocks = onto || f.probe ? 0 : ((long long)owners * a.rows + 8 * zero_rows - 1) / (8 * zero_rows);
+    B2_REQUIRE(sum_blocks + zero_blocks < (1ll << 31), "%lld tokens of %d features are too many for one launch", n, F);
+    const SumArgs sa = {V, F, (int)n, a.rows, owners, zero_rows, (unsigned)a.col_blocks, (unsigned)sum_blocks, scale, a.s};
+    const dim3 grid((unsigned)(sum_blocks + zero_blocks));
+#define B2_SUM(VEC, UN, ONTO) \
+    B2_CUDA((b2::launch_after(sum_kernel<T, VEC, UN, ONTO>, grid, 256, 0, st, (const T*)delta, (T*)dW, sa, f)))
+    if constexpr (sizeof(T) == 4) {
+        if (onto && vec) B2_SUM(W, 1, true);
+        else if (onto) B2_SUM(1, kApart, true);
+    }
+    if (!onto && vec) B2_SUM(W, 1, false);
+    else if (!onto) B2_SUM(1, kApart, false);
+#undef B2_SUM
     return B2_OK;
 }
 
@@ -587,7 +734,7 @@ extern "C" int b2_embed_fprop(const void* table, const void* idx, void* out, int
 
 extern "C" int b2_embed_update_scratch_bytes(int32_t V, int32_t F, int64_t n_idx, size_t* bytes) {
     B2_REQUIRE(bytes && V > 0 && F > 0 && n_idx >= 0 && n_idx <= (1ll << 30), "bad lookup: table %d x %d, %lld tokens", V, F, (long long)n_idx);
-    *bytes = scratch_of(nullptr, F, n_idx, col_blocks_of(F, 1)).bytes + 256;
+    *bytes = scratch_of(nullptr, V, F, n_idx, col_blocks_of(F, 1)).bytes + 256;
     return B2_OK;
 }
 

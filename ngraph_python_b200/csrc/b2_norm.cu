@@ -30,30 +30,32 @@ __device__ __forceinline__ void put(float* p, const float* v) {
     else *p = v[0];
 }
 
+// values that a pointer is behind a 16-byte boundary
+__device__ __host__ __forceinline__ int shift_of(const float* p) { return (int)((reinterpret_cast<uintptr_t>(p) >> 2) & 3); }
+
 // Sums of two values over the CTA, the same bits in every thread.  One barrier: calls write to two sets of words by
 // turns, and who comes to write to a set again has passed the barrier behind which everybody had read it.
 struct TwoSums {
     float words[2][2][32];
 };
-__device__ __forceinline__ void cta_sums(float& x, float& y, TwoSums& s, int& turn) {
+template <int N>
+__device__ __forceinline__ void cta_sums(float (&x)[N], TwoSums& s, int& turn) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        x += __shfl_xor_sync(0xffffffffu, x, o);
-        y += __shfl_xor_sync(0xffffffffu, y, o);
-    }
-    if (lane == 0) {
-        s.words[turn][0][warp] = x;
-        s.words[turn][1][warp] = y;
-    }
-    __syncthreads();
-    x = lane < warps ? s.words[turn][0][lane] : 0.0f;
-    y = lane < warps ? s.words[turn][1][lane] : 0.0f;
+    for (int o = 16; o > 0; o >>= 1)
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        x += __shfl_xor_sync(0xffffffffu, x, o);
-        y += __shfl_xor_sync(0xffffffffu, y, o);
-    }
+        for (int k = 0; k < N; ++k) x[k] += __shfl_xor_sync(0xffffffffu, x[k], o);
+    if (lane == 0)
+#pragma unroll
+        for (int k = 0; k < N; ++k) s.words[turn][k][warp] = x[k];
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < N; ++k) x[k] = lane < warps ? s.words[turn][k][lane] : 0.0f;
+    for (int o = warps > 16 ? 16 : warps > 8 ? 8 : warps > 4 ? 4 : warps > 2 ? 2 : warps - 1; o > 0; o >>= 1)
+#pragma unroll
+        for (int k = 0; k < N; ++k) x[k] += __shfl_xor_sync(0xffffffffu, x[k], o);
+#pragma unroll
+    for (int k = 0; k < N; ++k) x[k] = __shfl_sync(0xffffffffu, x[k], 0);
     turn ^= 1;
 }
 
@@ -69,7 +71,7 @@ __device__ __forceinline__ float block_sum(float v, float* words) {
     return v;
 }
 
-__device__ __forceinline__ float rstd_of(float squares, int F, float eps) { return 1.0f / sqrtf(squares / (float)F + eps); }
+__device__ __forceinline__ float rstd_of(float squares, int F, float eps) { return __frsqrt_rn(__fdividef(squares, (float)F) + eps); }
 
 __device__ __forceinline__ float gate_at(const b2_norm& a, long long row, int i) {
     switch (a.gate_kind) {
@@ -115,81 +117,122 @@ norm_any_kernel(const b2_norm a) {
     }
 }
 
-// A row to a CTA, held in registers: each tensor is read once.  Both operands are on their way before the first sum.
+// The first of a thread's IT vectors of a row: they are 32 vectors apart, a distance that addresses take as a constant.
 template <int VEC, int IT>
+__device__ __forceinline__ int first_of() { return ((int)(threadIdx.x >> 5) * IT * 32 + (int)(threadIdx.x & 31)) * VEC; }
+
+// A thread's vectors of a row.  Where rows are not aligned but all tensors' rows lie alike, some values behind a 16-byte
+// boundary, the vectors are those of memory, and the row's two ends are taken value by value -- behind all vectors,
+// since a branch between two loads keeps the second waiting.
+template <int VEC, int IT, bool RAGGED>
+__device__ __forceinline__ void get_row(const float* row, int i0, int F, float (*v)[VEC]) {
+#pragma unroll
+    for (int k = 0; k < IT; ++k) {
+        const int i = i0 + k * 32 * VEC;
+        if (RAGGED ? i >= 0 && i + VEC <= F : i < F) get<VEC>(row + i, v[k]);
+    }
+    if constexpr (RAGGED)
+#pragma unroll
+        for (int k = 0; k < IT; ++k) {
+            const int i = i0 + k * 32 * VEC;
+            if (i < 0 || (i < F && i + VEC > F))
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) v[k][j] = i + j >= 0 && i + j < F ? row[i + j] : 0.0f;
+        }
+}
+template <int VEC, int IT, bool RAGGED>
+__device__ __forceinline__ void put_row(float* row, int i0, int F, const float (*v)[VEC]) {
+#pragma unroll
+    for (int k = 0; k < IT; ++k) {
+        const int i = i0 + k * 32 * VEC;
+        if (RAGGED ? i >= 0 && i + VEC <= F : i < F) put<VEC>(row + i, v[k]);
+    }
+    if constexpr (RAGGED)
+#pragma unroll
+        for (int k = 0; k < IT; ++k) {
+            const int i = i0 + k * 32 * VEC;
+            if (i < 0 || (i < F && i + VEC > F))
+#pragma unroll
+                for (int j = 0; j < VEC; ++j)
+                    if (i + j >= 0 && i + j < F) row[i + j] = v[k][j];
+        }
+}
+// Of a vector over the features, which is not shifted.
+template <int VEC, bool RAGGED>
+__device__ __forceinline__ void get_weights(const float* w, int i, int F, float* v) {
+    if (RAGGED) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) v[j] = i + j >= 0 && i + j < F ? w[i + j] : 0.0f;
+    } else if (i < F) {
+        get<VEC>(w + i, v);
+    }
+}
+
+// A row to a CTA, held in registers: each tensor is read once.  Both operands are on their way before the first sum.
+template <int VEC, int IT, bool RAGGED, bool U, bool POST, int GATE>
 __global__ void __launch_bounds__(1024)
 norm_row_kernel(const b2_norm a) {
     __shared__ TwoSums sums;
     after_earlier_kernels();
-    const int F = a.features, T = blockDim.x;
+    constexpr int di = 32 * VEC;
+    const int F = a.features;
     int turn = 0;
     for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
         float x[IT][VEC] = {}, u[IT][VEC] = {};
         const float* r = a.residual + row * a.residual_stride;
-        const float* b = a.block ? a.block + row * a.block_stride : nullptr;
-#pragma unroll
-        for (int k = 0; k < IT; ++k) {
-            const int i = (k * T + threadIdx.x) * VEC;
-            if (i < F) {
-                if (b) get<VEC>(b + i, u[k]);
-                get<VEC>(r + i, x[k]);
-            }
-        }
-        if (b) {
+        const int i0 = first_of<VEC, IT>() - (RAGGED ? shift_of(r) : 0);
+        if (U) get_row<VEC, IT, RAGGED>(a.block + row * a.block_stride, i0, F, u);
+        get_row<VEC, IT, RAGGED>(r, i0, F, x);
+        if constexpr (U) {
             float rho = 1.0f;
-            if (a.post_weight) {
-                float q = 0.0f, none = 0.0f;
+            if (POST) {
+                float q[1] = {0.0f};
 #pragma unroll
                 for (int k = 0; k < IT; ++k)
 #pragma unroll
-                    for (int j = 0; j < VEC; ++j) q += u[k][j] * u[k][j];
-                cta_sums(q, none, sums, turn);
-                rho = rstd_of(q, F, a.eps);
+                    for (int j = 0; j < VEC; ++j) q[0] = fmaf(u[k][j], u[k][j], q[0]);
+                cta_sums(q, sums, turn);
+                rho = rstd_of(q[0], F, a.eps);
                 if (a.block_rstd && threadIdx.x == 0) a.block_rstd[row] = rho;
             }
-            const float row_gate = a.gate_kind == B2_GATE_ROW ? a.gate[row] : 1.0f;
-            const float* g = a.gate_kind == B2_GATE_FEATURE ? a.gate : a.gate_kind == B2_GATE_FULL ? a.gate + row * a.gate_stride : nullptr;
-            float* s = a.stream + row * a.stream_stride;
+            if (GATE == B2_GATE_ROW) rho *= a.gate[row];
 #pragma unroll
             for (int k = 0; k < IT; ++k) {
-                const int i = (k * T + threadIdx.x) * VEC;
-                if (i < F) {
-                    float w[VEC], gv[VEC];
-                    if (a.post_weight) get<VEC>(a.post_weight + i, w);
-                    if (g) get<VEC>(g + i, gv);
+                const int i = i0 + k * di;
+                float w[VEC], g[1][VEC];
+                if (POST) get_weights<VEC, RAGGED>(a.post_weight, i, F, w);
+                if (GATE == B2_GATE_FULL) get_row<VEC, 1, RAGGED>(a.gate + row * a.gate_stride, i, F, g);
+                if (GATE == B2_GATE_FEATURE) get_weights<VEC, RAGGED>(a.gate, i, F, g[0]);
 #pragma unroll
-                    for (int j = 0; j < VEC; ++j) {
-                        float y = u[k][j];
-                        if (a.post_weight) y = y * rho * w[j];
-                        y = y * (g ? gv[j] : row_gate);
-                        x[k][j] = a.residual_scale * x[k][j] + y;
-                    }
-                    put<VEC>(s + i, x[k]);
+                for (int j = 0; j < VEC; ++j) {
+                    float y = POST || GATE == B2_GATE_ROW ? u[k][j] * rho : u[k][j];
+                    if (POST) y *= w[j];
+                    if (GATE == B2_GATE_FULL || GATE == B2_GATE_FEATURE) y *= g[0][j];
+                    x[k][j] = fmaf(a.residual_scale, x[k][j], y);
+                    if (i + j >= F || (RAGGED && i + j < 0)) x[k][j] = 0.0f;
                 }
             }
+            put_row<VEC, IT, RAGGED>(a.stream + row * a.stream_stride, i0, F, x);
         }
         if (!a.out && !a.stream_rstd) continue;
-        float q = 0.0f, none = 0.0f;
+        float q[1] = {0.0f};
 #pragma unroll
         for (int k = 0; k < IT; ++k)
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) q += x[k][j] * x[k][j];
-        cta_sums(q, none, sums, turn);
-        const float rho = rstd_of(q, F, a.eps);
+            for (int j = 0; j < VEC; ++j) q[0] = fmaf(x[k][j], x[k][j], q[0]);
+        cta_sums(q, sums, turn);
+        const float rho = rstd_of(q[0], F, a.eps);
         if (a.stream_rstd && threadIdx.x == 0) a.stream_rstd[row] = rho;
         if (!a.out) continue;
-        float* o = a.out + row * a.out_stride;
 #pragma unroll
         for (int k = 0; k < IT; ++k) {
-            const int i = (k * T + threadIdx.x) * VEC;
-            if (i < F) {
-                float w[VEC];
-                get<VEC>(a.pre_weight + i, w);
+            const int i = i0 + k * di;
+            float w[VEC];
+            get_weights<VEC, RAGGED>(a.pre_weight, i, F, w);
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) w[j] = x[k][j] * rho * w[j];
-                put<VEC>(o + i, w);
-            }
+            for (int j = 0; j < VEC; ++j) x[k][j] = x[k][j] * rho * w[j];
         }
+        put_row<VEC, IT, RAGGED>(a.out + row * a.out_stride, i0, F, x);
     }
 }
 
@@ -204,21 +247,21 @@ struct Ring {
     int stages, slot;                   // bytes of one tensor's row, with room for its alignment
 };
 
-template <int VEC, int IT>
-__global__ void __launch_bounds__(512)
+template <int VEC, int IT, int MOST, bool U, bool POST, int GATE>
+__global__ void __launch_bounds__(MOST)
 norm_grad_row_kernel(const b2_norm a, const b2_norm_grads d, float* __restrict__ out_sums, const Ring ring) {
     extern __shared__ __align__(128) unsigned char room[];
     __shared__ unsigned long long first_full[kStages], then_full[kStages];
     __shared__ TwoSums sums;
-    constexpr bool HOLD = VEC * IT <= 8;        // weights stay in registers
-    const int F = a.features, T = blockDim.x, tid = threadIdx.x;
-    const bool has_dy = d.d_out != nullptr, has_ds = d.d_stream != nullptr, has_u = a.block != nullptr, post = a.post_weight != nullptr;
-    const bool full_gate = a.gate_kind == B2_GATE_FULL, feature_gate = a.gate_kind == B2_GATE_FEATURE;
+    constexpr bool HOLD = VEC * IT <= 8 && MOST <= 640;        // weights stay in registers
+    const int F = a.features, tid = threadIdx.x, i0 = first_of<VEC, IT>();
+    constexpr bool FULL = GATE == B2_GATE_FULL, FEATURE = GATE == B2_GATE_FEATURE;
+    const bool has_ds = d.d_stream != nullptr;
     // places of the tensors within a stage
-    const int at_dy = ring.slot, at_ds = has_dy ? 2 * ring.slot : 0, at_u = at_ds + (has_ds ? ring.slot : 0), at_g = at_u + (has_u ? ring.slot : 0);
-    const int stage_bytes = at_g + (full_gate ? ring.slot : 0);
-    const float* xs = has_u ? a.stream : a.residual;
-    const long long xs_stride = has_u ? a.stream_stride : a.residual_stride;
+    const int at_dy = ring.slot, at_ds = 2 * ring.slot, at_u = at_ds + (has_ds ? ring.slot : 0), at_g = at_u + (U ? ring.slot : 0);
+    const int stage_bytes = at_g + (FULL ? ring.slot : 0);
+    const float* xs = U ? a.stream : a.residual;
+    const long long xs_stride = U ? a.stream_stride : a.residual_stride;
     if (tid == 0) {
         for (int s = 0; s < ring.stages; ++s) {
             b2_mbar_init(first_full + s, 1);
@@ -229,19 +272,17 @@ norm_grad_row_kernel(const b2_norm a, const b2_norm_grads d, float* __restrict__
     __syncthreads();
     after_earlier_kernels();
 
-    auto shift_of = [](const float* p) { return (int)(((uintptr_t)p >> 2) & 3); };
     auto bytes_of = [&](const float* p) { return (unsigned)((shift_of(p) + F + 3) / 4 * 16); };
     auto copy = [&](const float* p, int to, unsigned long long* bar) { b2_bulk_g2s(room + to, p - shift_of(p), bytes_of(p), bar); };
     auto fetch_first = [&](long long row, int s) {
-        if (!has_dy) return;
         const float *x = xs + row * xs_stride, *dy = d.d_out + row * d.d_out_stride;
         b2_mbar_expect_tx(first_full + s, bytes_of(x) + bytes_of(dy));
         copy(x, s * stage_bytes, first_full + s);
         copy(dy, s * stage_bytes + at_dy, first_full + s);
     };
     auto fetch_then = [&](long long row, int s) {
-        const float *ds = has_ds ? d.d_stream + row * d.d_stream_stride : nullptr, *u = has_u ? a.block + row * a.block_stride : nullptr,
-                    *g = full_gate ? a.gate + row * a.gate_stride : nullptr;
+        const float *ds = has_ds ? d.d_stream + row * d.d_stream_stride : nullptr, *u = U ? a.block + row * a.block_stride : nullptr,
+                    *g = FULL ? a.gate + row * a.gate_stride : nullptr;
         if (!ds && !u && !g) return;
         b2_mbar_expect_tx(then_full + s, (ds ? bytes_of(ds) : 0u) + (u ? bytes_of(u) : 0u) + (g ? bytes_of(g) : 0u));
         if (ds) copy(ds, s * stage_bytes + at_ds, then_full + s);
@@ -260,17 +301,17 @@ norm_grad_row_kernel(const b2_norm a, const b2_norm_grads d, float* __restrict__
     float sum_pre[IT][VEC] = {}, sum_post[IT][VEC] = {}, sum_gate[IT][VEC] = {};
     float w_pre[IT][VEC] = {}, w_post[IT][VEC] = {}, w_gate[IT][VEC] = {};
     auto weights_first = [&](int k, int i) {
-        if (has_dy && i < F) get<VEC>(a.pre_weight + i, w_pre[k]);
+        if (i < F) get<VEC>(a.pre_weight + i, w_pre[k]);
     };
     auto weights_then = [&](int k, int i) {
-        if (post && i < F) get<VEC>(a.post_weight + i, w_post[k]);
-        if (feature_gate && i < F) get<VEC>(a.gate + i, w_gate[k]);
+        if (POST && i < F) get<VEC>(a.post_weight + i, w_post[k]);
+        if (FEATURE && i < F) get<VEC>(a.gate + i, w_gate[k]);
     };
     if constexpr (HOLD)
 #pragma unroll
         for (int k = 0; k < IT; ++k) {
-            weights_first(k, (k * T + tid) * VEC);
-            weights_then(k, (k * T + tid) * VEC);
+            weights_first(k, i0 + k * 32 * VEC);
+            weights_then(k, i0 + k * 32 * VEC);
         }
     const float over = 1.0f / (float)F;
     int turn = 0, s = 0;
@@ -280,17 +321,17 @@ norm_grad_row_kernel(const b2_norm a, const b2_norm_grads d, float* __restrict__
         const long long next = row + (long long)ring.stages * gridDim.x;
         const unsigned char* here = room + s * stage_bytes;
         float t[IT][VEC] = {};
-        const float rho = has_dy ? a.stream_rstd[row] : 0.0f, rho_u = post ? a.block_rstd[row] : 1.0f;
-        const float row_gate = a.gate_kind == B2_GATE_ROW ? a.gate[row] : 1.0f;
-        if (has_dy) {
+        const float rho = a.stream_rstd[row], rho_u = POST ? a.block_rstd[row] : 1.0f;
+        const float row_gate = GATE == B2_GATE_ROW ? a.gate[row] : 1.0f;
+        {
             late |= !b2_mbar_wait(first_full + s, phase);
             const float* x = reinterpret_cast<const float*>(here) + (VEC == 4 ? 0 : shift_of(xs + row * xs_stride));
             const float* dy = reinterpret_cast<const float*>(here + at_dy) + (VEC == 4 ? 0 : shift_of(d.d_out + row * d.d_out_stride));
             float xh[IT][VEC];
-            float q = 0.0f, none = 0.0f;
+            float q[1] = {0.0f};
 #pragma unroll
             for (int k = 0; k < IT; ++k) {
-                const int i = (k * T + tid) * VEC;
+                const int i = i0 + k * 32 * VEC;
                 if constexpr (!HOLD) weights_first(k, i);
                 float v[VEC] = {}, y[VEC] = {};
                 if (i < F) {
@@ -300,28 +341,28 @@ norm_grad_row_kernel(const b2_norm a, const b2_norm_grads d, float* __restrict__
 #pragma unroll
                 for (int j = 0; j < VEC; ++j) {
                     xh[k][j] = v[j] * rho;
-                    sum_pre[k][j] += y[j] * xh[k][j];
+                    sum_pre[k][j] = fmaf(y[j], xh[k][j], sum_pre[k][j]);
                     t[k][j] = y[j] * w_pre[k][j];
-                    q += t[k][j] * xh[k][j];
+                    q[0] = fmaf(t[k][j], xh[k][j], q[0]);
                 }
             }
-            cta_sums(q, none, sums, turn);
+            cta_sums(q, sums, turn);
             if (tid == 0 && next < a.rows) fetch_first(next, s);
-            const float mean = q * over;
+            const float mean = q[0] * over;
 #pragma unroll
             for (int k = 0; k < IT; ++k)
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) t[k][j] = rho * (t[k][j] - xh[k][j] * mean);
+                for (int j = 0; j < VEC; ++j) t[k][j] = rho * fmaf(xh[k][j], -mean, t[k][j]);
         }
-        if (has_ds || has_u || full_gate) late |= !b2_mbar_wait(then_full + s, phase);
+        if (has_ds || U) late |= !b2_mbar_wait(then_full + s, phase);
         const float* ds = has_ds ? reinterpret_cast<const float*>(here + at_ds) + (VEC == 4 ? 0 : shift_of(d.d_stream + row * d.d_stream_stride)) : nullptr;
-        const float* u = has_u ? reinterpret_cast<const float*>(here + at_u) + (VEC == 4 ? 0 : shift_of(a.block + row * a.block_stride)) : nullptr;
-        const float* g = full_gate ? reinterpret_cast<const float*>(here + at_g) + (VEC == 4 ? 0 : shift_of(a.gate + row * a.gate_stride)) : nullptr;
+        const float* u = U ? reinterpret_cast<const float*>(here + at_u) + (VEC == 4 ? 0 : shift_of(a.block + row * a.block_stride)) : nullptr;
+        const float* g = FULL ? reinterpret_cast<const float*>(here + at_g) + (VEC == 4 ? 0 : shift_of(a.gate + row * a.gate_stride)) : nullptr;
         float uh[IT][VEC] = {};
-        float dot = 0.0f, dgate = 0.0f;
+        float dots[2] = {0.0f, 0.0f};               // of the block's norm, of a row's gate
 #pragma unroll
         for (int k = 0; k < IT; ++k) {
-            const int i = (k * T + tid) * VEC;
+            const int i = i0 + k * 32 * VEC;
             if (i >= F) continue;
             float v[VEC];
             if (ds) {
@@ -337,37 +378,47 @@ norm_grad_row_kernel(const b2_norm a, const b2_norm_grads d, float* __restrict__
                 for (int j = 0; j < VEC; ++j) v[j] = a.residual_scale * t[k][j];
                 put<VEC>(d.d_residual + row * d.d_residual_stride + i, v);
             }
-            if (!u) continue;
+            if constexpr (!U) continue;
             if constexpr (!HOLD) weights_then(k, i);
             get<VEC>(u + i, uh[k]);
             float gv[VEC], dg[VEC];
-            if (g) get<VEC>(g + i, gv);
+            if constexpr (FULL) get<VEC>(g + i, gv);
 #pragma unroll
             for (int j = 0; j < VEC; ++j) {
-                uh[k][j] *= rho_u;
-                const float w = post ? w_post[k][j] : 1.0f;
-                dg[j] = t[k][j] * (uh[k][j] * w);
-                sum_gate[k][j] += dg[j];
-                dgate += dg[j];
-                t[k][j] *= g ? gv[j] : feature_gate ? w_gate[k][j] : row_gate;
-                sum_post[k][j] += t[k][j] * uh[k][j];
-                t[k][j] *= w;
-                dot += t[k][j] * uh[k][j];
+                if (POST) uh[k][j] *= rho_u;
+                const float value = POST ? uh[k][j] * w_post[k][j] : uh[k][j];
+                if (FULL) dg[j] = t[k][j] * value;
+                if (FEATURE) sum_gate[k][j] = fmaf(t[k][j], value, sum_gate[k][j]);
+                if (GATE == B2_GATE_ROW) dots[1] = fmaf(t[k][j], value, dots[1]);
+                if (GATE != B2_GATE_NONE) t[k][j] *= FULL ? gv[j] : FEATURE ? w_gate[k][j] : row_gate;
+                if (POST) {
+                    sum_post[k][j] = fmaf(t[k][j], uh[k][j], sum_post[k][j]);
+                    t[k][j] *= w_post[k][j];
+                    dots[0] = fmaf(t[k][j], uh[k][j], dots[0]);
+                }
             }
-            if (g && d.d_gate) put<VEC>(d.d_gate + row * d.d_gate_stride + i, dg);
+            if (FULL && d.d_gate) put<VEC>(d.d_gate + row * d.d_gate_stride + i, dg);
         }
-        cta_sums(dot, dgate, sums, turn);
+        if constexpr (GATE == B2_GATE_ROW) {
+            cta_sums(dots, sums, turn);
+        } else if constexpr (POST) {
+            float one[1] = {dots[0]};
+            cta_sums(one, sums, turn);
+            dots[0] = one[0];
+        } else {
+            __syncthreads();
+        }
         if (tid == 0 && next < a.rows) fetch_then(next, s);
-        if (a.gate_kind == B2_GATE_ROW && d.d_gate && tid == 0) d.d_gate[row] = dgate;
-        if (d.d_block) {
-            const float mean = post ? dot * over : 0.0f;
+        if (GATE == B2_GATE_ROW && d.d_gate && tid == 0) d.d_gate[row] = dots[1];
+        if (U && d.d_block) {
+            const float mean = POST ? dots[0] * over : 0.0f;
 #pragma unroll
             for (int k = 0; k < IT; ++k) {
-                const int i = (k * T + tid) * VEC;
+                const int i = i0 + k * 32 * VEC;
                 if (i >= F) continue;
                 float v[VEC];
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) v[j] = rho_u * (t[k][j] - uh[k][j] * mean);
+                for (int j = 0; j < VEC; ++j) v[j] = POST ? rho_u * fmaf(uh[k][j], -mean, t[k][j]) : t[k][j];
                 put<VEC>(d.d_block + row * d.d_block_stride + i, v);
             }
         }
@@ -379,11 +430,11 @@ norm_grad_row_kernel(const b2_norm a, const b2_norm_grads d, float* __restrict__
     float* mine = out_sums + (long long)blockIdx.x * 3 * F;
 #pragma unroll
     for (int k = 0; k < IT; ++k) {
-        const int i = (k * T + tid) * VEC;
+        const int i = i0 + k * 32 * VEC;
         if (i >= F) continue;
         if (d.d_pre_weight) put<VEC>(mine + i, sum_pre[k]);
-        if (d.d_post_weight) put<VEC>(mine + F + i, sum_post[k]);
-        if (feature_gate && d.d_gate) put<VEC>(mine + 2 * F + i, sum_gate[k]);
+        if (POST && d.d_post_weight) put<VEC>(mine + F + i, sum_post[k]);
+        if (FEATURE && d.d_gate) put<VEC>(mine + 2 * F + i, sum_gate[k]);
     }
 }
 
@@ -449,25 +500,30 @@ norm_grad_any_kernel(const b2_norm a, const b2_norm_grads d, float* __restrict__
     }
 }
 
-// The CTAs' sums: 32 columns to a block, whose warps take the CTAs by turns.
+// The CTAs' sums: COLS columns to a block of 1024 threads, which take the CTAs by turns.
+template <int COLS>
 __global__ void __launch_bounds__(1024)
 norm_sums_kernel(const float* __restrict__ sums, int ctas, int F, float* pre, float* post, float* gate) {
-    __shared__ float words[32][33];
+    constexpr int TURNS = 1024 / COLS;
+    __shared__ float words[TURNS][COLS + 1];
     after_earlier_kernels();
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int i = blockIdx.x * 32 + lane;
+    const int col = threadIdx.x % COLS, turn = threadIdx.x / COLS;
+    const int i = blockIdx.x * COLS + col;
     float* out = blockIdx.y == 0 ? pre : blockIdx.y == 1 ? post : gate;
     if (!out) return;
     float s = 0.0f;
     if (i < F)
-#pragma unroll 4
-        for (int c = warp; c < ctas; c += 32) s += sums[((long long)c * 3 + blockIdx.y) * F + i];
-    words[warp][lane] = s;
+#pragma unroll 8
+        for (int c = turn; c < ctas; c += TURNS) s += sums[((long long)c * 3 + blockIdx.y) * F + i];
+    words[turn][col] = s;
     __syncthreads();
-    if (warp == 0 && i < F) {
+    // (a warp to a column at a time)
+    for (int k = threadIdx.x / 32; k < COLS && blockIdx.x * COLS + k < F; k += 32) {
         s = 0.0f;
-        for (int w = 0; w < 32; ++w) s += words[w][lane];
-        out[i] = s;
+        for (int t = threadIdx.x % 32; t < TURNS; t += 32) s += words[t][k];
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+        if (threadIdx.x % 32 == 0) out[blockIdx.x * COLS + k] = s;
     }
 }
 
@@ -477,18 +533,17 @@ int threads_of(int F, int each, int most) {
     return t <= most ? t : 0;
 }
 
-// How the gradient is launched: eight values to a thread, sixteen from 4096 features on (a CTA of 512 threads then
-// has the registers of an SM), CTAs for about 512 threads an SM, three rows ahead where they fit.  CTAs also bound
-// the sums that are left to add.
+// How the gradient is launched: eight values of a row to a thread, CTAs for about 512 threads an SM (for 768 or 1024 no
+// registers are left: 16384 x 2048 125, 151 and 141 us) or one of more, three rows ahead where they fit.  Sixteen values
+// to a thread of rows beyond 4096 features: 4096 x 8192 161 us, 154 with eight; 3000 x 5001 180 and 83.
 struct GradPlan {
-    int threads, each, ctas;
+    int threads, ctas;
     Ring ring;
 };
 GradPlan grad_plan(const b2_norm& a, int tensors) {
     GradPlan p = {};
-    p.each = threads_of(a.features, 8, 512) ? 8 : 16;
-    p.threads = threads_of(a.features, p.each, 512);
-    long long per_sm = p.threads ? 512 / p.threads : 4;
+    p.threads = threads_of(a.features, 8, 1024);
+    long long per_sm = p.threads > 512 ? 1 : p.threads ? 512 / p.threads : 4;
     if (per_sm > 16) per_sm = 16;
     p.ctas = (int)(a.rows < b2::kSms * per_sm ? a.rows : b2::kSms * per_sm);
     if (!p.threads) return p;
@@ -516,12 +571,47 @@ int check_stride(const b2_norm* a, const void* p, int64_t stride, const char* wh
 
 bool rows_aligned(const void* p, int64_t stride) { return b2::aligned16(p) && stride % 4 == 0; }
 
-template <int VEC, int IT>
+template <int VEC, int IT, bool RAGGED>
+int launch_rows(const b2_norm& a, unsigned blocks, int threads, cudaStream_t st) {
+#define B2_LAUNCH(U, POST, GATE) \
+    B2_CUDA((b2::launch_after(norm_row_kernel<VEC, IT, RAGGED, U, POST, GATE>, dim3(blocks), threads, 0, st, a)))
+#define B2_GATED(POST)                                                        \
+    switch (a.gate_kind) {                                                    \
+        case B2_GATE_FEATURE: B2_LAUNCH(true, POST, B2_GATE_FEATURE); break;  \
+        case B2_GATE_ROW: B2_LAUNCH(true, POST, B2_GATE_ROW); break;          \
+        case B2_GATE_FULL: B2_LAUNCH(true, POST, B2_GATE_FULL); break;        \
+        default: B2_LAUNCH(true, POST, B2_GATE_NONE);                         \
+    }
+    if (!a.block) B2_LAUNCH(false, false, B2_GATE_NONE);
+    else if (a.post_weight) B2_GATED(true)
+    else B2_GATED(false)
+#undef B2_GATED
+#undef B2_LAUNCH
+    return B2_OK;
+}
+
+template <int VEC, int IT, int MOST, bool U, bool POST, int GATE>
 int launch_grad(const b2_norm& a, const b2_norm_grads& d, const GradPlan& p, int tensors, float* sums, cudaStream_t st) {
     static std::atomic<unsigned long long> done{0};
-    B2_CHECK(b2::allow_shared((const void*)norm_grad_row_kernel<VEC, IT>, 220 << 10, &done));
-    B2_CUDA((b2::launch_after(norm_grad_row_kernel<VEC, IT>, dim3(p.ctas), p.threads, (size_t)p.ring.stages * p.ring.slot * tensors, st, a, d, sums, p.ring)));
+    B2_CHECK(b2::allow_shared((const void*)norm_grad_row_kernel<VEC, IT, MOST, U, POST, GATE>, 220 << 10, &done));
+    B2_CUDA((b2::launch_after(norm_grad_row_kernel<VEC, IT, MOST, U, POST, GATE>, dim3(p.ctas), p.threads, (size_t)p.ring.stages * p.ring.slot * tensors, st, a, d,
+                              sums, p.ring)));
     return B2_OK;
+}
+
+template <int VEC, int IT, int MOST>
+int launch_grad_of(const b2_norm& a, const b2_norm_grads& d, const GradPlan& p, int tensors, float* sums, cudaStream_t st) {
+    if (!a.block) return launch_grad<VEC, IT, MOST, false, false, B2_GATE_NONE>(a, d, p, tensors, sums, st);
+#define B2_GATED(POST)                                                                                               \
+    switch (a.gate_kind) {                                                                                           \
+        case B2_GATE_FEATURE: return launch_grad<VEC, IT, MOST, true, POST, B2_GATE_FEATURE>(a, d, p, tensors, sums, st);  \
+        case B2_GATE_ROW: return launch_grad<VEC, IT, MOST, true, POST, B2_GATE_ROW>(a, d, p, tensors, sums, st);          \
+        case B2_GATE_FULL: return launch_grad<VEC, IT, MOST, true, POST, B2_GATE_FULL>(a, d, p, tensors, sums, st);        \
+        default: return launch_grad<VEC, IT, MOST, true, POST, B2_GATE_NONE>(a, d, p, tensors, sums, st);                  \
+    }
+    if (a.post_weight) B2_GATED(true)
+    B2_GATED(false)
+#undef B2_GATED
 }
 
 }  // namespace
@@ -546,22 +636,30 @@ extern "C" int b2_norm_fprop(const b2_norm* a, void* stream) {
                      rows_aligned(a->stream, a->stream_stride) && rows_aligned(a->out, a->out_stride) &&
                      (a->gate_kind != B2_GATE_FULL ? a->gate_kind == B2_GATE_ROW || b2::aligned16(a->gate) : rows_aligned(a->gate, a->gate_stride)) &&
                      b2::aligned16(a->post_weight) && b2::aligned16(a->pre_weight);
-    // few rows: as many threads as a row has vectors, for the least latency; many: eight values to a thread, so that
-    // several rows share an SM
-    const bool few = a->rows <= b2::kSms * 2;
-#define B2_ROWS(VEC, IT)                                                                                              \
-    if (const int t = threads_of(F, VEC * IT, 1024)) {                                                               \
-        B2_CUDA((b2::launch_after(norm_row_kernel<VEC, IT>, dim3(blocks), t, 0, st, *a)));                             \
-        return B2_OK;                                                                                                \
-    }
+    // all rows as far behind a boundary
+    auto alike = [&](const float* p, int64_t stride) {
+        return !p || (shift_of(p) == shift_of(a->residual) && (a->rows <= 1 || (stride - a->residual_stride) % 4 == 0));
+    };
+    const bool ragged = alike(a->block, a->block_stride) && alike(a->stream, a->stream_stride) && alike(a->out, a->out_stride) &&
+                        (a->gate_kind != B2_GATE_FULL || alike(a->gate, a->gate_stride));
+    // Few rows: as many threads as a row has vectors, for the least latency.  Many: eight values to a thread, sixteen from
+    // 2048 features on, so that several rows share an SM and the sums over the CTA weigh less (8192 x 4096: 100 us
+    // with eight, 85 with sixteen; 16384 x 512: 25 and 27).
+    const bool few = a->rows <= b2::kSms * 2, wide = F >= 2048;
+#define B2_ROWS(VEC, IT, RAGGED) \
+    if (const int t = threads_of(F + (RAGGED ? 3 : 0), VEC * IT, 1024)) return launch_rows<VEC, IT, RAGGED>(*a, blocks, t, st);
     if (vec) {
-        if (few) B2_ROWS(4, 1)
-        B2_ROWS(4, 2)
-        B2_ROWS(4, 4)
+        if (few) B2_ROWS(4, 1, false)
+        if (!wide) B2_ROWS(4, 2, false)
+        B2_ROWS(4, 4, false)
+    } else if (ragged) {
+        if (few) B2_ROWS(4, 1, true)
+        if (!wide) B2_ROWS(4, 2, true)
+        B2_ROWS(4, 4, true)
     } else {
-        if (few) B2_ROWS(1, 2)
-        B2_ROWS(1, 8)
-        B2_ROWS(1, 16)
+        if (few) B2_ROWS(1, 2, false)
+        B2_ROWS(1, 8, false)
+        B2_ROWS(1, 16, false)
     }
 #undef B2_ROWS
     B2_CUDA(b2::launch_after(norm_any_kernel, dim3(blocks), kThreads, 0, st, *a));
@@ -571,8 +669,7 @@ extern "C" int b2_norm_fprop(const b2_norm* a, void* stream) {
 extern "C" int b2_norm_bprop_scratch_bytes(const b2_norm* a, size_t* bytes) {
     B2_REQUIRE(bytes, "missing argument");
     B2_CHECK(check_norm(a));
-    const GradPlan one = grad_plan(*a, 1), five = grad_plan(*a, 5);
-    *bytes = (size_t)(one.ctas > five.ctas ? one.ctas : five.ctas) * 3 * a->features * sizeof(float) + 256;
+    *bytes = (size_t)grad_plan(*a, 1).ctas * 3 * a->features * sizeof(float) + 256;     // (CTAs do not depend on the tensors)
     return B2_OK;
 }
 
@@ -605,7 +702,6 @@ extern "C" int b2_norm_bprop(const b2_norm* a, const b2_norm_grads* d, void* scr
     float* gate = a->gate_kind == B2_GATE_FEATURE ? d->d_gate : nullptr;
     const bool full = a->gate_kind == B2_GATE_FULL;
     const int tensors = (d->d_out ? 2 : 0) + (d->d_stream ? 1 : 0) + (a->block ? 1 : 0) + (full ? 1 : 0);
-    const GradPlan p = grad_plan(*a, tensors);
     const float* x = a->block ? a->stream : a->residual;
     const int64_t x_stride = a->block ? a->stream_stride : a->residual_stride;
     const bool vec = a->features % 4 == 0 && rows_aligned(a->block, a->block_stride) && (!d->d_out || rows_aligned(x, x_stride)) &&
@@ -613,15 +709,26 @@ extern "C" int b2_norm_bprop(const b2_norm* a, const b2_norm_grads* d, void* scr
                      rows_aligned(d->d_residual, d->d_residual_stride) && rows_aligned(d->d_block, d->d_block_stride) &&
                      (full ? rows_aligned(a->gate, a->gate_stride) && rows_aligned(d->d_gate, d->d_gate_stride) : a->gate_kind == B2_GATE_ROW || b2::aligned16(a->gate)) &&
                      b2::aligned16(a->post_weight) && b2::aligned16(a->pre_weight);
+    const GradPlan p = grad_plan(*a, tensors);
     if (p.ctas > 0) {
-        if (!p.threads) B2_CUDA(b2::launch_after(norm_grad_any_kernel, dim3(p.ctas), kThreads, 0, st, *a, *d, sums));
-        else if (vec && p.each == 8) B2_CHECK((launch_grad<4, 2>(*a, *d, p, tensors, sums, st)));
-        else if (vec) B2_CHECK((launch_grad<4, 4>(*a, *d, p, tensors, sums, st)));
-        else if (p.each == 8) B2_CHECK((launch_grad<1, 8>(*a, *d, p, tensors, sums, st)));
-        else B2_CHECK((launch_grad<1, 16>(*a, *d, p, tensors, sums, st)));
+        if (!p.threads || !d->d_out) B2_CUDA(b2::launch_after(norm_grad_any_kernel, dim3(p.ctas), kThreads, 0, st, *a, *d, sums));
+#define B2_GRAD(MOST)                                                                                       \
+    else if (p.threads <= MOST) {                                                                            \
+        if (vec) B2_CHECK((launch_grad_of<4, 2, MOST>(*a, *d, p, tensors, sums, st)));                       \
+        else B2_CHECK((launch_grad_of<1, 8, MOST>(*a, *d, p, tensors, sums, st)));                           \
+    }
+        B2_GRAD(512)
+        B2_GRAD(640)
+        B2_GRAD(1024)
+#undef B2_GRAD
     }
     if (d->d_pre_weight || d->d_post_weight || gate)
-        B2_CUDA(b2::launch_after(norm_sums_kernel, dim3((a->features + 31) / 32, 3), 1024, 0, st, (const float*)sums, p.ctas, a->features, d->d_pre_weight,
-                                 d->d_post_weight, gate));
+    {
+        // (many CTAs' sums of few columns: fewer columns to a block)
+        const bool narrow = p.ctas > 512;
+        const int cols = narrow ? 8 : 32;
+        B2_CUDA(b2::launch_after(narrow ? norm_sums_kernel<8> : norm_sums_kernel<32>, dim3((a->features + cols - 1) / cols, 3), 1024, 0, st,
+                                 (const float*)sums, p.ctas, a->features, d->d_pre_weight, d->d_post_weight, gate));
+    }
     return B2_OK;
 }
