@@ -12,7 +12,7 @@
 
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 512;        // of a CTA for rows of any length
 
 // VEC values next to one another
 template <int VEC>
@@ -82,6 +82,8 @@ __device__ __forceinline__ float gate_at(const b2_norm& a, long long row, int i)
     }
 }
 
+// Rows of any length and alignment: what a row's sums need is read again.
+template <int VEC>
 __global__ void __launch_bounds__(kThreads)
 norm_any_kernel(const b2_norm a) {
     __shared__ float words[32];
@@ -94,26 +96,42 @@ norm_any_kernel(const b2_norm a) {
         float rho = 1.0f;
         if (a.post_weight) {
             float q = 0.0f;
-            for (int i = threadIdx.x; i < F; i += kThreads) q += u[i] * u[i];
+            for (int i = threadIdx.x * VEC; i < F; i += kThreads * VEC) {
+                float y[VEC];
+                get<VEC>(u + i, y);
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) q = fmaf(y[j], y[j], q);
+            }
             rho = rstd_of(block_sum(q, words), F, a.eps);
             if (a.block_rstd && threadIdx.x == 0) a.block_rstd[row] = rho;
         }
         float q = 0.0f;
-        for (int i = threadIdx.x; i < F; i += kThreads) {
-            float x = r[i];
+        for (int i = threadIdx.x * VEC; i < F; i += kThreads * VEC) {
+            float x[VEC], y[VEC];
+            get<VEC>(r + i, x);
             if (u) {
-                float y = u[i];
-                if (a.post_weight) y = y * rho * a.post_weight[i];
-                x = a.residual_scale * x + y * gate_at(a, row, i);
-                s[i] = x;
+                get<VEC>(u + i, y);
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) {
+                    if (a.post_weight) y[j] = y[j] * rho * a.post_weight[i + j];
+                    x[j] = fmaf(y[j], gate_at(a, row, i + j), a.residual_scale * x[j]);
+                }
+                put<VEC>(s + i, x);
             }
-            q += x * x;
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) q = fmaf(x[j], x[j], q);
         }
         if (!a.out && !a.stream_rstd) continue;
         rho = rstd_of(block_sum(q, words), F, a.eps);
         if (a.stream_rstd && threadIdx.x == 0) a.stream_rstd[row] = rho;
         if (a.out)
-            for (int i = threadIdx.x; i < F; i += kThreads) a.out[row * a.out_stride + i] = (s ? s[i] : r[i]) * rho * a.pre_weight[i];
+            for (int i = threadIdx.x * VEC; i < F; i += kThreads * VEC) {
+                float x[VEC];
+                get<VEC>((s ? s : r) + i, x);
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) x[j] = x[j] * rho * a.pre_weight[i + j];
+                put<VEC>(a.out + row * a.out_stride + i, x);
+            }
     }
 }
 
@@ -157,32 +175,47 @@ __device__ __forceinline__ void put_row(float* row, int i0, int F, const float (
                     if (i + j >= 0 && i + j < F) row[i + j] = v[k][j];
         }
 }
-// Of a vector over the features, which is not shifted.
-template <int VEC, bool RAGGED>
-__device__ __forceinline__ void get_weights(const float* w, int i, int F, float* v) {
-    if (RAGGED) {
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) v[j] = i + j >= 0 && i + j < F ? w[i + j] : 0.0f;
-    } else if (i < F) {
-        get<VEC>(w + i, v);
-    }
+
+__device__ __forceinline__ void fetch_ahead(const float* p, int n) {
+    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p), "r"(n * 4) : "memory");
 }
 
 // A row to a CTA, held in registers: each tensor is read once.  Both operands are on their way before the first sum.
+// Ragged rows: a CTA's are a multiple of four apart and so lie alike, and it keeps the weights in shared memory as they
+// lie beside them.
 template <int VEC, int IT, bool RAGGED, bool U, bool POST, int GATE>
 __global__ void __launch_bounds__(1024)
 norm_row_kernel(const b2_norm a) {
+    extern __shared__ __align__(16) float staged[];         // ragged: post_weight, a gate per feature, pre_weight
     __shared__ TwoSums sums;
     after_earlier_kernels();
     constexpr int di = 32 * VEC;
-    const int F = a.features;
+    const int F = a.features, width = (F + 6) / 4 * 4;
+    const int shift = RAGGED ? shift_of(a.residual + blockIdx.x * a.residual_stride) : 0, i0 = first_of<VEC, IT>() - shift;
+    if (RAGGED) {
+        for (int i = threadIdx.x; i < width; i += blockDim.x) {
+            const bool there = i >= shift && i - shift < F;
+            if (POST) staged[i] = there ? a.post_weight[i - shift] : 0.0f;
+            if (GATE == B2_GATE_FEATURE) staged[width + i] = there ? a.gate[i - shift] : 0.0f;
+            if (a.out) staged[2 * width + i] = there ? a.pre_weight[i - shift] : 0.0f;
+        }
+        __syncthreads();
+    }
+    auto get_weights = [&](int which, const float* w, int i, float* v) {
+        if (RAGGED ? i + shift < width : i < F) get<VEC>(RAGGED ? staged + which * width + i + shift : w + i, v);
+    };
     int turn = 0;
     for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
         float x[IT][VEC] = {}, u[IT][VEC] = {};
         const float* r = a.residual + row * a.residual_stride;
-        const int i0 = first_of<VEC, IT>() - (RAGGED ? shift_of(r) : 0);
         if (U) get_row<VEC, IT, RAGGED>(a.block + row * a.block_stride, i0, F, u);
         get_row<VEC, IT, RAGGED>(r, i0, F, x);
+        if (RAGGED && threadIdx.x == 0 && row + gridDim.x < a.rows) {
+            // the next row on its way to the second cache
+            const long long next = row + gridDim.x;
+            fetch_ahead(a.residual + next * a.residual_stride - shift, width);
+            if (U) fetch_ahead(a.block + next * a.block_stride - shift, width);
+        }
         if constexpr (U) {
             float rho = 1.0f;
             if (POST) {
@@ -200,9 +233,9 @@ norm_row_kernel(const b2_norm a) {
             for (int k = 0; k < IT; ++k) {
                 const int i = i0 + k * di;
                 float w[VEC], g[1][VEC];
-                if (POST) get_weights<VEC, RAGGED>(a.post_weight, i, F, w);
+                if (POST) get_weights(0, a.post_weight, i, w);
                 if (GATE == B2_GATE_FULL) get_row<VEC, 1, RAGGED>(a.gate + row * a.gate_stride, i, F, g);
-                if (GATE == B2_GATE_FEATURE) get_weights<VEC, RAGGED>(a.gate, i, F, g[0]);
+                if (GATE == B2_GATE_FEATURE) get_weights(1, a.gate, i, g[0]);
 #pragma unroll
                 for (int j = 0; j < VEC; ++j) {
                     float y = POST || GATE == B2_GATE_ROW ? u[k][j] * rho : u[k][j];
@@ -228,7 +261,7 @@ norm_row_kernel(const b2_norm a) {
         for (int k = 0; k < IT; ++k) {
             const int i = i0 + k * di;
             float w[VEC];
-            get_weights<VEC, RAGGED>(a.pre_weight, i, F, w);
+            get_weights(2, a.pre_weight, i, w);
 #pragma unroll
             for (int j = 0; j < VEC; ++j) x[k][j] = x[k][j] * rho * w[j];
         }
@@ -239,22 +272,23 @@ norm_row_kernel(const b2_norm a) {
 // Gradients, a row to a CTA at a time.  A CTA keeps its rows' sums for the weights and a gate per feature in registers.
 // The tensors of its next rows are on their way into shared memory meanwhile (bulk copies; a ring of `stages` rows),
 // since between the loads of a row and its stores there are two sums over the CTA: the first pair (stream, d_out) of a
-// place is free again behind the first of them, the others behind the second.  Rows of any alignment: a copy starts at
-// the 16-byte boundary below the row.  A wait that runs out turns the results into NaN.
+// place is free again behind the first of them, the others behind the second.  Ragged rows: a CTA's are a multiple of four
+// apart and so lie alike; a copy starts at the 16-byte boundary below the row, and a thread's columns, whose sums it keeps,
+// are the vectors of memory.  (Value by value 3000 x 5001 took 83 us.)  A wait that runs out turns the results into NaN.
 constexpr int kStages = 4;
 
 struct Ring {
     int stages, slot;                   // bytes of one tensor's row, with room for its alignment
 };
 
-template <int VEC, int IT, int MOST, bool U, bool POST, int GATE>
+template <bool RAGGED, int MOST, bool U, bool POST, int GATE>
 __global__ void __launch_bounds__(MOST)
 norm_grad_row_kernel(const b2_norm a, const b2_norm_grads d, float* __restrict__ out_sums, const Ring ring) {
     extern __shared__ __align__(128) unsigned char room[];
     __shared__ unsigned long long first_full[kStages], then_full[kStages];
     __shared__ TwoSums sums;
-    constexpr bool HOLD = VEC * IT <= 8 && MOST <= 640;        // weights stay in registers
-    const int F = a.features, tid = threadIdx.x, i0 = first_of<VEC, IT>();
+    constexpr int VEC = 4, IT = 2;
+    constexpr bool HOLD = MOST <= 640;          // weights stay in registers
     constexpr bool FULL = GATE == B2_GATE_FULL, FEATURE = GATE == B2_GATE_FEATURE;
     const bool has_ds = d.d_stream != nullptr;
     // places of the tensors within a stage
@@ -262,6 +296,7 @@ norm_grad_row_kernel(const b2_norm a, const b2_norm_grads d, float* __restrict__
     const int stage_bytes = at_g + (FULL ? ring.slot : 0);
     const float* xs = U ? a.stream : a.residual;
     const long long xs_stride = U ? a.stream_stride : a.residual_stride;
+    const int F = a.features, tid = threadIdx.x, shift = RAGGED ? shift_of(xs + blockIdx.x * xs_stride) : 0, i0 = first_of<VEC, IT>() - shift;
     if (tid == 0) {
         for (int s = 0; s < ring.stages; ++s) {
             b2_mbar_init(first_full + s, 1);
@@ -300,12 +335,36 @@ norm_grad_row_kernel(const b2_norm a, const b2_norm_grads d, float* __restrict__
 
     float sum_pre[IT][VEC] = {}, sum_post[IT][VEC] = {}, sum_gate[IT][VEC] = {};
     float w_pre[IT][VEC] = {}, w_post[IT][VEC] = {}, w_gate[IT][VEC] = {};
-    auto weights_first = [&](int k, int i) {
-        if (i < F) get<VEC>(a.pre_weight + i, w_pre[k]);
+    // vectors that reach beyond the row's ends: values of no row are zero, and are not stored
+    auto cut = [&](int i) { return RAGGED && (i < 0 || i + VEC > F); };
+    auto load = [&](const float* p, int i, float* v) {
+        get<VEC>(p + i, v);
+        if (cut(i))
+#pragma unroll
+            for (int j = 0; j < VEC; ++j)
+                if (i + j < 0 || i + j >= F) v[j] = 0.0f;
     };
+    auto store = [&](float* p, int i, const float* v) {
+        if (!cut(i)) {
+            put<VEC>(p + i, v);
+        } else {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j)
+                if (i + j >= 0 && i + j < F) p[i + j] = v[j];
+        }
+    };
+    auto weight = [&](const float* w, int i, float* v) {
+        if (RAGGED) {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) v[j] = i + j >= 0 && i + j < F ? w[i + j] : 0.0f;
+        } else if (i < F) {
+            get<VEC>(w + i, v);
+        }
+    };
+    auto weights_first = [&](int k, int i) { weight(a.pre_weight, i, w_pre[k]); };
     auto weights_then = [&](int k, int i) {
-        if (POST && i < F) get<VEC>(a.post_weight + i, w_post[k]);
-        if (FEATURE && i < F) get<VEC>(a.gate + i, w_gate[k]);
+        if (POST) weight(a.post_weight, i, w_post[k]);
+        if (FEATURE) weight(a.gate, i, w_gate[k]);
     };
     if constexpr (HOLD)
 #pragma unroll
@@ -325,8 +384,7 @@ norm_grad_row_kernel(const b2_norm a, const b2_norm_grads d, float* __restrict__
         const float row_gate = GATE == B2_GATE_ROW ? a.gate[row] : 1.0f;
         {
             late |= !b2_mbar_wait(first_full + s, phase);
-            const float* x = reinterpret_cast<const float*>(here) + (VEC == 4 ? 0 : shift_of(xs + row * xs_stride));
-            const float* dy = reinterpret_cast<const float*>(here + at_dy) + (VEC == 4 ? 0 : shift_of(d.d_out + row * d.d_out_stride));
+            const float *x = reinterpret_cast<const float*>(here) + shift, *dy = reinterpret_cast<const float*>(here + at_dy) + shift;
             float xh[IT][VEC];
             float q[1] = {0.0f};
 #pragma unroll
@@ -335,8 +393,8 @@ norm_grad_row_kernel(const b2_norm a, const b2_norm_grads d, float* __restrict__
                 if constexpr (!HOLD) weights_first(k, i);
                 float v[VEC] = {}, y[VEC] = {};
                 if (i < F) {
-                    get<VEC>(x + i, v);
-                    get<VEC>(dy + i, y);
+                    load(x, i, v);
+                    load(dy, i, y);
                 }
 #pragma unroll
                 for (int j = 0; j < VEC; ++j) {
@@ -355,9 +413,8 @@ norm_grad_row_kernel(const b2_norm a, const b2_norm_grads d, float* __restrict__
                 for (int j = 0; j < VEC; ++j) t[k][j] = rho * fmaf(xh[k][j], -mean, t[k][j]);
         }
         if (has_ds || U) late |= !b2_mbar_wait(then_full + s, phase);
-        const float* ds = has_ds ? reinterpret_cast<const float*>(here + at_ds) + (VEC == 4 ? 0 : shift_of(d.d_stream + row * d.d_stream_stride)) : nullptr;
-        const float* u = U ? reinterpret_cast<const float*>(here + at_u) + (VEC == 4 ? 0 : shift_of(a.block + row * a.block_stride)) : nullptr;
-        const float* g = FULL ? reinterpret_cast<const float*>(here + at_g) + (VEC == 4 ? 0 : shift_of(a.gate + row * a.gate_stride)) : nullptr;
+        const float *ds = reinterpret_cast<const float*>(here + at_ds) + shift, *u = reinterpret_cast<const float*>(here + at_u) + shift,
+                    *g = reinterpret_cast<const float*>(here + at_g) + shift;
         float uh[IT][VEC] = {};
         float dots[2] = {0.0f, 0.0f};               // of the block's norm, of a row's gate
 #pragma unroll
@@ -365,8 +422,8 @@ norm_grad_row_kernel(const b2_norm a, const b2_norm_grads d, float* __restrict__
             const int i = i0 + k * 32 * VEC;
             if (i >= F) continue;
             float v[VEC];
-            if (ds) {
-                get<VEC>(ds + i, v);
+            if (has_ds) {
+                load(ds, i, v);
 #pragma unroll
                 for (int j = 0; j < VEC; ++j) t[k][j] += v[j];
             }
@@ -376,13 +433,13 @@ norm_grad_row_kernel(const b2_norm a, const b2_norm_grads d, float* __restrict__
             if (d.d_residual) {
 #pragma unroll
                 for (int j = 0; j < VEC; ++j) v[j] = a.residual_scale * t[k][j];
-                put<VEC>(d.d_residual + row * d.d_residual_stride + i, v);
+                store(d.d_residual + row * d.d_residual_stride, i, v);
             }
             if constexpr (!U) continue;
             if constexpr (!HOLD) weights_then(k, i);
-            get<VEC>(u + i, uh[k]);
+            load(u, i, uh[k]);
             float gv[VEC], dg[VEC];
-            if constexpr (FULL) get<VEC>(g + i, gv);
+            if constexpr (FULL) load(g, i, gv);
 #pragma unroll
             for (int j = 0; j < VEC; ++j) {
                 if (POST) uh[k][j] *= rho_u;
@@ -397,7 +454,7 @@ norm_grad_row_kernel(const b2_norm a, const b2_norm_grads d, float* __restrict__
                     dots[0] = fmaf(t[k][j], uh[k][j], dots[0]);
                 }
             }
-            if (FULL && d.d_gate) put<VEC>(d.d_gate + row * d.d_gate_stride + i, dg);
+            if (FULL && d.d_gate) store(d.d_gate + row * d.d_gate_stride, i, dg);
         }
         if constexpr (GATE == B2_GATE_ROW) {
             cta_sums(dots, sums, turn);
@@ -419,7 +476,7 @@ norm_grad_row_kernel(const b2_norm a, const b2_norm_grads d, float* __restrict__
                 float v[VEC];
 #pragma unroll
                 for (int j = 0; j < VEC; ++j) v[j] = POST ? rho_u * fmaf(uh[k][j], -mean, t[k][j]) : t[k][j];
-                put<VEC>(d.d_block + row * d.d_block_stride + i, v);
+                store(d.d_block + row * d.d_block_stride, i, v);
             }
         }
         if (++s == ring.stages) {
@@ -432,13 +489,24 @@ norm_grad_row_kernel(const b2_norm a, const b2_norm_grads d, float* __restrict__
     for (int k = 0; k < IT; ++k) {
         const int i = i0 + k * 32 * VEC;
         if (i >= F) continue;
-        if (d.d_pre_weight) put<VEC>(mine + i, sum_pre[k]);
-        if (POST && d.d_post_weight) put<VEC>(mine + F + i, sum_post[k]);
-        if (FEATURE && d.d_gate) put<VEC>(mine + 2 * F + i, sum_gate[k]);
+        if (RAGGED) {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+                if (i + j < 0 || i + j >= F) continue;
+                if (d.d_pre_weight) mine[i + j] = sum_pre[k][j];
+                if (POST && d.d_post_weight) mine[F + i + j] = sum_post[k][j];
+                if (FEATURE && d.d_gate) mine[2 * F + i + j] = sum_gate[k][j];
+            }
+        } else {
+            if (d.d_pre_weight) put<VEC>(mine + i, sum_pre[k]);
+            if (POST && d.d_post_weight) put<VEC>(mine + F + i, sum_post[k]);
+            if (FEATURE && d.d_gate) put<VEC>(mine + 2 * F + i, sum_gate[k]);
+        }
     }
 }
 
-// Sums over rows: a CTA adds its rows into sums of its own, [CTAs][3][F] of scratch, which norm_sums_kernel adds.
+// Rows of any length and alignment: a CTA adds its rows into sums of its own, [CTAs][3][F] of scratch.
+template <int VEC>
 __global__ void __launch_bounds__(kThreads)
 norm_grad_any_kernel(const b2_norm a, const b2_norm_grads d, float* __restrict__ sums) {
     __shared__ float words[32];
@@ -449,6 +517,13 @@ norm_grad_any_kernel(const b2_norm a, const b2_norm_grads d, float* __restrict__
     float* gate = post + F;
     for (int i = threadIdx.x; i < 3 * F; i += kThreads) pre[i] = 0.0f;
     __syncthreads();
+    auto add = [&](float* to, int i, const float* v) {
+        float o[VEC];
+        get<VEC>(to + i, o);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) o[j] += v[j];
+        put<VEC>(to + i, o);
+    };
     for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
         const float* x = a.block ? a.stream + row * a.stream_stride : a.residual + row * a.residual_stride;
         const float* u = a.block ? a.block + row * a.block_stride : nullptr;
@@ -458,32 +533,52 @@ norm_grad_any_kernel(const b2_norm a, const b2_norm_grads d, float* __restrict__
         float mean = 0.0f;
         if (dy) {
             float q = 0.0f;
-            for (int i = threadIdx.x; i < F; i += kThreads) {
-                const float xh = x[i] * rho;
-                q += dy[i] * a.pre_weight[i] * xh;
-                pre[i] += dy[i] * xh;
+            for (int i = threadIdx.x * VEC; i < F; i += kThreads * VEC) {
+                float xv[VEC], yv[VEC];
+                get<VEC>(x + i, xv);
+                get<VEC>(dy + i, yv);
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) {
+                    xv[j] *= rho;
+                    q = fmaf(yv[j] * a.pre_weight[i + j], xv[j], q);
+                    xv[j] *= yv[j];
+                }
+                add(pre, i, xv);
             }
             mean = block_sum(q, words) / (float)F;
         }
         float dot = 0.0f, dgate = 0.0f;
-        for (int i = threadIdx.x; i < F; i += kThreads) {
-            float t = ds ? ds[i] : 0.0f;
-            if (dy) t += rho * (dy[i] * a.pre_weight[i] - x[i] * rho * mean);
-            if (d.d_residual) d.d_residual[row * d.d_residual_stride + i] = a.residual_scale * t;
+        for (int i = threadIdx.x * VEC; i < F; i += kThreads * VEC) {
+            float t[VEC] = {}, v[VEC], g[VEC];
+            if (ds) get<VEC>(ds + i, t);
+            if (dy) {
+                float xv[VEC], yv[VEC];
+                get<VEC>(x + i, xv);
+                get<VEC>(dy + i, yv);
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) t[j] += rho * (yv[j] * a.pre_weight[i + j] - xv[j] * rho * mean);
+            }
+            if (d.d_residual) {
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) v[j] = a.residual_scale * t[j];
+                put<VEC>(d.d_residual + row * d.d_residual_stride + i, v);
+            }
             if (!u) continue;
-            const float uh = u[i] * rho_u, w = a.post_weight ? a.post_weight[i] : 1.0f;
-            if (a.gate_kind) {
-                const float g = t * (uh * w);
-                if (a.gate_kind == B2_GATE_FEATURE) gate[i] += g;
-                else if (a.gate_kind == B2_GATE_ROW) dgate += g;
-                else if (d.d_gate) d.d_gate[row * d.d_gate_stride + i] = g;
-                t *= gate_at(a, row, i);
+            get<VEC>(u + i, v);
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+                v[j] *= rho_u;
+                const float w = a.post_weight ? a.post_weight[i + j] : 1.0f;
+                g[j] = t[j] * (v[j] * w);
+                dgate += g[j];
+                t[j] *= gate_at(a, row, i + j);
+                v[j] *= t[j];
+                dot = fmaf(v[j], w, dot);
             }
-            if (a.post_weight) {
-                dot += t * w * uh;
-                post[i] += t * uh;
-            }
-            if (d.d_block) d.d_block[row * d.d_block_stride + i] = t;
+            if (a.gate_kind == B2_GATE_FEATURE) add(gate, i, g);
+            else if (a.gate_kind == B2_GATE_FULL && d.d_gate) put<VEC>(d.d_gate + row * d.d_gate_stride + i, g);
+            if (a.post_weight) add(post, i, v);
+            if (d.d_block) put<VEC>(d.d_block + row * d.d_block_stride + i, t);
         }
         if (a.gate_kind == B2_GATE_ROW) {
             dgate = block_sum(dgate, words);
@@ -492,9 +587,13 @@ norm_grad_any_kernel(const b2_norm a, const b2_norm_grads d, float* __restrict__
         if (a.post_weight) {
             mean = block_sum(dot, words) / (float)F;
             if (d.d_block)
-                for (int i = threadIdx.x; i < F; i += kThreads) {
-                    float* p = d.d_block + row * d.d_block_stride + i;
-                    *p = rho_u * (*p * a.post_weight[i] - u[i] * rho_u * mean);
+                for (int i = threadIdx.x * VEC; i < F; i += kThreads * VEC) {
+                    float t[VEC], v[VEC];
+                    get<VEC>(d.d_block + row * d.d_block_stride + i, t);
+                    get<VEC>(u + i, v);
+#pragma unroll
+                    for (int j = 0; j < VEC; ++j) t[j] = rho_u * (t[j] * a.post_weight[i + j] - v[j] * rho_u * mean);
+                    put<VEC>(d.d_block + row * d.d_block_stride + i, t);
                 }
         }
     }
@@ -540,9 +639,9 @@ struct GradPlan {
     int threads, ctas;
     Ring ring;
 };
-GradPlan grad_plan(const b2_norm& a, int tensors) {
+GradPlan grad_plan(const b2_norm& a, int tensors, bool ragged) {
     GradPlan p = {};
-    p.threads = threads_of(a.features, 8, 1024);
+    p.threads = threads_of(a.features + (ragged ? 3 : 0), 8, 1024);
     long long per_sm = p.threads > 512 ? 1 : p.threads ? 512 / p.threads : 4;
     if (per_sm > 16) per_sm = 16;
     p.ctas = (int)(a.rows < b2::kSms * per_sm ? a.rows : b2::kSms * per_sm);
@@ -572,9 +671,17 @@ int check_stride(const b2_norm* a, const void* p, int64_t stride, const char* wh
 bool rows_aligned(const void* p, int64_t stride) { return b2::aligned16(p) && stride % 4 == 0; }
 
 template <int VEC, int IT, bool RAGGED>
-int launch_rows(const b2_norm& a, unsigned blocks, int threads, cudaStream_t st) {
-#define B2_LAUNCH(U, POST, GATE) \
-    B2_CUDA((b2::launch_after(norm_row_kernel<VEC, IT, RAGGED, U, POST, GATE>, dim3(blocks), threads, 0, st, a)))
+int launch_rows(const b2_norm& a, int threads, cudaStream_t st) {
+    // (148 and so every multiple of it is a multiple of four)
+    const long long most = RAGGED ? (long long)b2::kSms * (threads > 512 ? 1 : 1024 / threads > 16 ? 16 : 1024 / threads) : 1ll << 30;
+    const unsigned blocks = (unsigned)(a.rows < most ? a.rows : most);
+    const size_t room = RAGGED ? (size_t)3 * ((a.features + 6) / 4 * 4) * sizeof(float) : 0;
+#define B2_LAUNCH(U, POST, GATE)                                                                                                       \
+    do {                                                                                                                              \
+        static std::atomic<unsigned long long> done{0};                                                                               \
+        if (room > 48 << 10) B2_CHECK(b2::allow_shared((const void*)norm_row_kernel<VEC, IT, RAGGED, U, POST, GATE>, 220 << 10, &done)); \
+        B2_CUDA((b2::launch_after(norm_row_kernel<VEC, IT, RAGGED, U, POST, GATE>, dim3(blocks), threads, room, st, a)));              \
+    } while (0)
 #define B2_GATED(POST)                                                        \
     switch (a.gate_kind) {                                                    \
         case B2_GATE_FEATURE: B2_LAUNCH(true, POST, B2_GATE_FEATURE); break;  \
@@ -590,24 +697,24 @@ int launch_rows(const b2_norm& a, unsigned blocks, int threads, cudaStream_t st)
     return B2_OK;
 }
 
-template <int VEC, int IT, int MOST, bool U, bool POST, int GATE>
+template <bool RAGGED, int MOST, bool U, bool POST, int GATE>
 int launch_grad(const b2_norm& a, const b2_norm_grads& d, const GradPlan& p, int tensors, float* sums, cudaStream_t st) {
     static std::atomic<unsigned long long> done{0};
-    B2_CHECK(b2::allow_shared((const void*)norm_grad_row_kernel<VEC, IT, MOST, U, POST, GATE>, 220 << 10, &done));
-    B2_CUDA((b2::launch_after(norm_grad_row_kernel<VEC, IT, MOST, U, POST, GATE>, dim3(p.ctas), p.threads, (size_t)p.ring.stages * p.ring.slot * tensors, st, a, d,
+    B2_CHECK(b2::allow_shared((const void*)norm_grad_row_kernel<RAGGED, MOST, U, POST, GATE>, 220 << 10, &done));
+    B2_CUDA((b2::launch_after(norm_grad_row_kernel<RAGGED, MOST, U, POST, GATE>, dim3(p.ctas), p.threads, (size_t)p.ring.stages * p.ring.slot * tensors, st, a, d,
                               sums, p.ring)));
     return B2_OK;
 }
 
-template <int VEC, int IT, int MOST>
+template <bool RAGGED, int MOST>
 int launch_grad_of(const b2_norm& a, const b2_norm_grads& d, const GradPlan& p, int tensors, float* sums, cudaStream_t st) {
-    if (!a.block) return launch_grad<VEC, IT, MOST, false, false, B2_GATE_NONE>(a, d, p, tensors, sums, st);
+    if (!a.block) return launch_grad<RAGGED, MOST, false, false, B2_GATE_NONE>(a, d, p, tensors, sums, st);
 #define B2_GATED(POST)                                                                                               \
     switch (a.gate_kind) {                                                                                           \
-        case B2_GATE_FEATURE: return launch_grad<VEC, IT, MOST, true, POST, B2_GATE_FEATURE>(a, d, p, tensors, sums, st);  \
-        case B2_GATE_ROW: return launch_grad<VEC, IT, MOST, true, POST, B2_GATE_ROW>(a, d, p, tensors, sums, st);          \
-        case B2_GATE_FULL: return launch_grad<VEC, IT, MOST, true, POST, B2_GATE_FULL>(a, d, p, tensors, sums, st);        \
-        default: return launch_grad<VEC, IT, MOST, true, POST, B2_GATE_NONE>(a, d, p, tensors, sums, st);                  \
+        case B2_GATE_FEATURE: return launch_grad<RAGGED, MOST, true, POST, B2_GATE_FEATURE>(a, d, p, tensors, sums, st);  \
+        case B2_GATE_ROW: return launch_grad<RAGGED, MOST, true, POST, B2_GATE_ROW>(a, d, p, tensors, sums, st);          \
+        case B2_GATE_FULL: return launch_grad<RAGGED, MOST, true, POST, B2_GATE_FULL>(a, d, p, tensors, sums, st);        \
+        default: return launch_grad<RAGGED, MOST, true, POST, B2_GATE_NONE>(a, d, p, tensors, sums, st);                  \
     }
     if (a.post_weight) B2_GATED(true)
     B2_GATED(false)
@@ -647,7 +754,7 @@ extern "C" int b2_norm_fprop(const b2_norm* a, void* stream) {
     // with eight, 85 with sixteen; 16384 x 512: 25 and 27).
     const bool few = a->rows <= b2::kSms * 2, wide = F >= 2048;
 #define B2_ROWS(VEC, IT, RAGGED) \
-    if (const int t = threads_of(F + (RAGGED ? 3 : 0), VEC * IT, 1024)) return launch_rows<VEC, IT, RAGGED>(*a, blocks, t, st);
+    if (const int t = threads_of(F + (RAGGED ? 3 : 0), VEC * IT, 1024)) return launch_rows<VEC, IT, RAGGED>(*a, t, st);
     if (vec) {
         if (few) B2_ROWS(4, 1, false)
         if (!wide) B2_ROWS(4, 2, false)
@@ -656,20 +763,17 @@ extern "C" int b2_norm_fprop(const b2_norm* a, void* stream) {
         if (few) B2_ROWS(4, 1, true)
         if (!wide) B2_ROWS(4, 2, true)
         B2_ROWS(4, 4, true)
-    } else {
-        if (few) B2_ROWS(1, 2, false)
-        B2_ROWS(1, 8, false)
-        B2_ROWS(1, 16, false)
     }
 #undef B2_ROWS
-    B2_CUDA(b2::launch_after(norm_any_kernel, dim3(blocks), kThreads, 0, st, *a));
+    B2_CUDA(b2::launch_after(vec ? norm_any_kernel<4> : norm_any_kernel<1>, dim3(blocks), kThreads, 0, st, *a));
     return B2_OK;
 }
 
 extern "C" int b2_norm_bprop_scratch_bytes(const b2_norm* a, size_t* bytes) {
     B2_REQUIRE(bytes, "missing argument");
     B2_CHECK(check_norm(a));
-    *bytes = (size_t)grad_plan(*a, 1).ctas * 3 * a->features * sizeof(float) + 256;     // (CTAs do not depend on the tensors)
+    const int even = grad_plan(*a, 1, false).ctas, ragged = grad_plan(*a, 1, true).ctas;        // (they do not depend on the tensors)
+    *bytes = (size_t)(even > ragged ? even : ragged) * 3 * a->features * sizeof(float) + 256;
     return B2_OK;
 }
 
@@ -709,13 +813,19 @@ extern "C" int b2_norm_bprop(const b2_norm* a, const b2_norm_grads* d, void* scr
                      rows_aligned(d->d_residual, d->d_residual_stride) && rows_aligned(d->d_block, d->d_block_stride) &&
                      (full ? rows_aligned(a->gate, a->gate_stride) && rows_aligned(d->d_gate, d->d_gate_stride) : a->gate_kind == B2_GATE_ROW || b2::aligned16(a->gate)) &&
                      b2::aligned16(a->post_weight) && b2::aligned16(a->pre_weight);
-    const GradPlan p = grad_plan(*a, tensors);
+    auto alike = [&](const float* q, int64_t stride) {
+        return !q || (shift_of(q) == shift_of(x) && (a->rows <= 1 || (stride - x_stride) % 4 == 0));
+    };
+    const bool ragged = !vec && alike(a->block, a->block_stride) && alike(d->d_out, d->d_out_stride) && alike(d->d_stream, d->d_stream_stride) &&
+                        alike(d->d_residual, d->d_residual_stride) && alike(d->d_block, d->d_block_stride) &&
+                        (!full || (alike(a->gate, a->gate_stride) && alike(d->d_gate, d->d_gate_stride)));
+    const GradPlan p = grad_plan(*a, tensors, ragged);
     if (p.ctas > 0) {
-        if (!p.threads || !d->d_out) B2_CUDA(b2::launch_after(norm_grad_any_kernel, dim3(p.ctas), kThreads, 0, st, *a, *d, sums));
+        if (!p.threads || !d->d_out || !(vec || ragged)) B2_CUDA(b2::launch_after(vec ? norm_grad_any_kernel<4> : norm_grad_any_kernel<1>, dim3(p.ctas), kThreads, 0, st, *a, *d, sums));
 #define B2_GRAD(MOST)                                                                                       \
     else if (p.threads <= MOST) {                                                                            \
-        if (vec) B2_CHECK((launch_grad_of<4, 2, MOST>(*a, *d, p, tensors, sums, st)));                       \
-        else B2_CHECK((launch_grad_of<1, 8, MOST>(*a, *d, p, tensors, sums, st)));                           \
+        if (vec) B2_CHECK((launch_grad_of<false, MOST>(*a, *d, p, tensors, sums, st)));                      \
+        else B2_CHECK((launch_grad_of<true, MOST>(*a, *d, p, tensors, sums, st)));                           \
     }
         B2_GRAD(512)
         B2_GRAD(640)

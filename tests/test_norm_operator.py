@@ -185,6 +185,37 @@ def _backward(c, gate, x, rstd, rho, d_out, d_stream, pad=0, offset=0, in_place=
     return {names[k]: (v.t if isinstance(v, _Memory) else v).cpu().numpy() for k, v in list(ends.items()) + list(sums.items()) if k in names}
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("gate", ["feature", "row", "full"])
+@pytest.mark.parametrize("rows,F,pad", [(5000, 37, 0), (900, 1001, 0), (2400, 99, 2), (400, 4099, 0), (700, 2050, 3), (3000, 61, 3)])
+def test_many_ragged_rows(rows, F, pad, gate):
+    """More rows than blocks, each begun elsewhere within sixteen bytes."""
+    c = _case(rows, F, gate)
+    got, _ = _forward(c, gate) if not pad else _forward_alike(c, gate, pad)
+    _check_forward(got, c, F)
+    rng = np.random.RandomState(9)
+    x, rstd, rho = _stored(c)
+    d = [rng.standard_normal((rows, F)).astype(np.float32) for _ in range(2)]
+    _check_backward(_backward(c, gate, x, rstd, rho, *d), c, x, rstd, rho, *d)
+
+
+def _forward_alike(c, gate, pad):
+    """All rows `pad` apart."""
+    import torch
+    from ngraph_python_b200 import lib
+    rows, F = c["residual"].shape
+    mem = {k: _Memory(v, pad) for k, v in dict(residual=c["residual"], block=c["block"], stream=np.zeros((rows, F)), out=np.zeros((rows, F))).items()}
+    vecs = dict(post=_vec(c["post"]), pre=_vec(c["pre"]))
+    if gate == "full":
+        mem["gate"] = _Memory(c["gate"], pad)
+    else:
+        vecs["gate"] = _vec(c["gate"])
+    lib.check(lib.raw().b2_norm_fprop(ctypes.byref(_args(c, gate, mem, vecs, rows, F)), 0))
+    torch.cuda.synchronize()
+    assert all(m.intact() for m in mem.values())
+    return {k: mem[k].t.cpu().numpy() for k in ("stream", "out")}, None
+
+
 def _stored(c):
     """What a forward pass leaves, in fp32."""
     want, _ = no.forward(c["residual"], c["block"], c["gate"], c["post"], c["pre"], c["a"], 1e-6)
