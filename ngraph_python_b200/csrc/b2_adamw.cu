@@ -145,15 +145,49 @@ adamw32_kernel(unsigned* finished, const Chunk* __restrict__ chunks, long long n
 }
 
 // The byte (without its sign) of one of the two neighbours in e4m3 of q, |q| <= 448 but for a rounding: of the upper one
-// with the chance that sixteen random bits, here in bits 4 to 19, give it.  What a mantissa has beyond e4m3's three bits is
-// added to and cut off; exponent and mantissa are the byte but for the bias, 120 * 8.  Below 2^-6, where the values
-// are 2^-9 apart, the same between 2^-6 and 2^-5, whose bytes are eight higher.  (No carry beyond 448: the bits end
-// above the roundings of q.)
+// with the chance that sixteen random bits give it.  Times 2^-120, exponent and mantissa of an fp32 value have in their
+// upper bits the byte of e4m3, fp32's denormals that of e4m3's, which are 2^-9 apart; what is below these bits is added
+// to and cut off.  (No carry beyond 448: the random bits end above the roundings of q.)
 __device__ __forceinline__ unsigned to_e4m3(float q, unsigned bits) {
-    const float a = fabsf(q);
-    const bool low = a < 0.015625f;
-    const float b = __fadd_rn(a, low ? 0.015625f : 0.0f);
-    return (__float_as_uint(b) + bits - (low ? 0x3C8u << 20 : 0x3C0u << 20)) >> 20;
+    return (__float_as_uint(__fmul_rn(fabsf(q), 7.52316384526264e-37f)) + (bits << 4)) >> 20;
+}
+
+// Two products to an instruction.  Sums are taken one by one: the assembler joins a product and a sum of this form into one
+// operation, rounded once, .rn or not (seen in the bits of v).
+struct Two {
+    unsigned long long w;
+};
+__device__ __forceinline__ Two two(float x, float y) {
+    Two t;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(t.w) : "f"(x), "f"(y));
+    return t;
+}
+__device__ __forceinline__ void apart(Two t, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(t.w)); }
+__device__ __forceinline__ Two operator*(Two a, Two b) {
+    Two t;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(t.w) : "l"(a.w), "l"(b.w));
+    return t;
+}
+__device__ __forceinline__ Two operator+(Two a, Two b) {
+    float a0, a1, b0, b1;
+    apart(a, a0, a1);
+    apart(b, b0, b1);
+    return two(__fadd_rn(a0, b0), __fadd_rn(a1, b1));
+}
+
+// update() of two values
+__device__ __forceinline__ Two update(const Rates& r, const Now& now, float keep, Two p, Two g, Two& m, Two& v, float& r0, float& r1) {
+    auto both = [](float x) { return two(x, x); };
+    g = g * both(now.grad_scale);
+    m = m * both(r.b1) + g * both(r.c1);
+    v = v * both(r.b2) + (g * g) * both(r.c2);
+    float v0, v1, m0, m1, d0, d1;
+    apart(v, v0, v1);
+    apart(m, m0, m1);
+    r0 = __fsqrt_rn(v0);
+    r1 = __fsqrt_rn(v1);
+    apart(two(r0, r1) * both(now.root) + both(r.eps), d0, d1);
+    return p * both(keep) + two(__fdiv_rn(m0, d0), __fdiv_rn(m1, d1)) * both(-now.size);
 }
 
 // the larger magnitude, NaN where there is one
@@ -166,12 +200,17 @@ __device__ __forceinline__ float2 from_e4m3(unsigned two) {
     const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)two, __NV_E4M3);
     return __half22float2(__half2(h));
 }
-// 448 / top and the block's scale
-__device__ __forceinline__ float scale_of(float top, float& scale) {
+// 448 / top of both moments, and their scales top / 448: one division in each of four lanes.
+__device__ __forceinline__ void scales_of(float top_m, float top_r, float& to_m, float& to_r, float& new_ms, float& new_vs) {
+    const int lane = threadIdx.x & 31;
+    const float top = lane & 1 ? top_r : top_m;
     const bool live = top > 7.888609052210118e-31f;             // 2^-100
-    scale = live ? __fdiv_rn(top, 448.0f) : 0.0f;
-    if (!(top <= 3.402823466e+38f)) scale = __int_as_float(0x7fffffff);
-    return live ? __fdiv_rn(448.0f, top) : 0.0f;
+    float x = live ? __fdiv_rn(lane & 2 ? top : 448.0f, lane & 2 ? 448.0f : top) : 0.0f;
+    if ((lane & 2) && !(top <= 3.402823466e+38f)) x = __int_as_float(0x7fffffff);
+    to_m = __shfl_sync(0xffffffffu, x, 0);
+    to_r = __shfl_sync(0xffffffffu, x, 1);
+    new_ms = __shfl_sync(0xffffffffu, x, 2);
+    new_vs = __shfl_sync(0xffffffffu, x, 3);
 }
 
 __global__ void __launch_bounds__(kThreads, 4)
@@ -186,55 +225,72 @@ adamw8_kernel(unsigned* finished, const Chunk* __restrict__ chunks, long long n_
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     for (long long k = blockIdx.x; k < n_chunks; k += gridDim.x) {
         const Chunk c = chunks[k];
-        if (k + gridDim.x < n_chunks) asm volatile("prefetch.global.L1 [%0];" ::"l"(chunks + k + gridDim.x));
         const int at = warp * kBlock;
+        // the next chunk's values on their way to the second cache, a line to a lane, and the record behind it to the first
+        if (k + 2 * gridDim.x < n_chunks && lane == 31) asm volatile("prefetch.global.L1 [%0];" ::"l"(chunks + k + 2 * gridDim.x));
+        if (k + gridDim.x < n_chunks && lane < 20) {
+            const Chunk* next = chunks + k + gridDim.x;
+            const int line = lane < 16 ? lane & 7 : lane & 1, from = at + line * (lane < 16 ? 32 : 128);
+            const char* p = lane < 8 ? (const char*)(next->param + from) : lane < 16 ? (const char*)(next->grad + from)
+                          : lane < 18 ? static_cast<const char*>(next->m) + from : static_cast<const char*>(next->v) + from;
+            if (from < (int)next->n) asm volatile("prefetch.global.L2 [%0];" ::"l"(p));
+        }
         const int n = (int)c.n - at;                    // of the warp's block
         if (n <= 0) continue;
         unsigned char* mc = static_cast<unsigned char*>(c.m) + at;
         unsigned char* vc = static_cast<unsigned char*>(c.v) + at;
         const float keep = __fsub_rn(1.0f, __fmul_rn(c.decay, now.lr_wd));
         // a lane's values: four from 4 lane on, four from 128 + 4 lane on
-        float p[8], g[8], m[8], v[8], root[8];
+        Two p[4], g[4], m[4], v[4];
+        float root[8];
         const bool vec = c.vec && n >= kBlock;
         const float ms = c.m_scales[warp], vs = c.v_scales[warp];
+        unsigned mw[2], vw[2];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const int i = h * 128 + lane * 4;
-            unsigned mw = 0, vw = 0;
             if (vec) {
                 const float4 p4 = *reinterpret_cast<const float4*>(c.param + at + i), g4 = *reinterpret_cast<const float4*>(c.grad + at + i);
-                p[4 * h] = p4.x; p[4 * h + 1] = p4.y; p[4 * h + 2] = p4.z; p[4 * h + 3] = p4.w;
-                g[4 * h] = g4.x; g[4 * h + 1] = g4.y; g[4 * h + 2] = g4.z; g[4 * h + 3] = g4.w;
-                mw = *reinterpret_cast<const unsigned*>(mc + i);
-                vw = *reinterpret_cast<const unsigned*>(vc + i);
+                p[2 * h] = two(p4.x, p4.y);
+                p[2 * h + 1] = two(p4.z, p4.w);
+                g[2 * h] = two(g4.x, g4.y);
+                g[2 * h + 1] = two(g4.z, g4.w);
+                mw[h] = *reinterpret_cast<const unsigned*>(mc + i);
+                vw[h] = *reinterpret_cast<const unsigned*>(vc + i);
             } else {
+                float x[4], y[4];
+                mw[h] = vw[h] = 0;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const bool there = i + j < n;
-                    p[4 * h + j] = there ? c.param[at + i + j] : 0.0f;
-                    g[4 * h + j] = there ? c.grad[at + i + j] : 0.0f;
-                    mw |= there ? (unsigned)mc[i + j] << (8 * j) : 0u;
-                    vw |= there ? (unsigned)vc[i + j] << (8 * j) : 0u;
+                    x[j] = there ? c.param[at + i + j] : 0.0f;
+                    y[j] = there ? c.grad[at + i + j] : 0.0f;
+                    mw[h] |= there ? (unsigned)mc[i + j] << (8 * j) : 0u;
+                    vw[h] |= there ? (unsigned)vc[i + j] << (8 * j) : 0u;
                 }
+                p[2 * h] = two(x[0], x[1]);
+                p[2 * h + 1] = two(x[2], x[3]);
+                g[2 * h] = two(y[0], y[1]);
+                g[2 * h + 1] = two(y[2], y[3]);
             }
-            const float2 ma = from_e4m3(mw & 0xffff), mb = from_e4m3(mw >> 16), va = from_e4m3(vw & 0xffff), vb = from_e4m3(vw >> 16);
-            m[4 * h] = ma.x; m[4 * h + 1] = ma.y; m[4 * h + 2] = mb.x; m[4 * h + 3] = mb.y;
-            v[4 * h] = va.x; v[4 * h + 1] = va.y; v[4 * h + 2] = vb.x; v[4 * h + 3] = vb.y;
         }
         float most_m = 0.0f, most_r = 0.0f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            m[e] = __fmul_rn(m[e], ms);
-            const float old = __fmul_rn(v[e], vs);
-            v[e] = __fmul_rn(old, old);
-            p[e] = update(r, now, keep, p[e], g[e], m[e], v[e], root[e]);
-            most_m = larger(most_m, m[e]);
-            most_r = larger(most_r, root[e]);
+        for (int e = 0; e < 4; ++e) {
+            const float2 mf = from_e4m3(mw[e / 2] >> (16 * (e & 1)) & 0xffff), rf = from_e4m3(vw[e / 2] >> (16 * (e & 1)) & 0xffff);
+            m[e] = two(mf.x, mf.y) * two(ms, ms);
+            const Two old = two(rf.x, rf.y) * two(vs, vs);
+            v[e] = old * old;
+            p[e] = update(r, now, keep, p[e], g[e], m[e], v[e], root[2 * e], root[2 * e + 1]);
+            float m0, m1;
+            apart(m[e], m0, m1);
+            most_m = larger(larger(most_m, m0), m1);
+            most_r = larger(larger(most_r, root[2 * e]), root[2 * e + 1]);
         }
         // as bits, whose order is that of the values (NaN above all)
         const unsigned top_m = __reduce_max_sync(0xffffffffu, __float_as_uint(most_m)), top_r = __reduce_max_sync(0xffffffffu, __float_as_uint(most_r));
-        float new_ms, new_vs;
-        const float to_m = scale_of(__uint_as_float(top_m), new_ms), to_r = scale_of(__uint_as_float(top_r), new_vs);
+        float to_m, to_r, new_ms, new_vs;
+        scales_of(__uint_as_float(top_m), __uint_as_float(top_r), to_m, to_r, new_ms, new_vs);
         if (lane == 0) {
             c.m_scales[warp] = new_ms;
             c.v_scales[warp] = new_vs;
@@ -244,26 +300,33 @@ adamw8_kernel(unsigned* finished, const Chunk* __restrict__ chunks, long long n_
             const int i = h * 128 + lane * 4;
             unsigned mb[4], vb[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int e = 4 * h + j;
-                const unsigned bits = mix((c.counter + (unsigned)(at + i + j)) ^ now.key);
-                const float qm = __fmul_rn(m[e], to_m), qr = __fmul_rn(root[e], to_r);
-                mb[j] = to_e4m3(qm, (bits << 4) & 0xFFFF0u) | (__float_as_uint(qm) >> 24 & 0x80u);
-                vb[j] = max(to_e4m3(qr, (bits >> 12) & 0xFFFF0u), qr > 0.0f ? 1u : 0u);
+            for (int k = 0; k < 2; ++k) {
+                float qm[2], qr[2];
+                apart(m[2 * h + k] * two(to_m, to_m), qm[0], qm[1]);
+                apart(two(root[4 * h + 2 * k], root[4 * h + 2 * k + 1]) * two(to_r, to_r), qr[0], qr[1]);
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const unsigned bits = mix((c.counter + (unsigned)(at + i + 2 * k + j)) ^ now.key);
+                    mb[2 * k + j] = to_e4m3(qm[j], bits & 0xffffu) | (__float_as_uint(qm[j]) >> 24 & 0x80u);
+                    vb[2 * k + j] = max(to_e4m3(qr[j], bits >> 16), min(__float_as_uint(qr[j]), 1u));
+                }
             }
-            const unsigned mw = __byte_perm(__byte_perm(mb[0], mb[1], 0x0040), __byte_perm(mb[2], mb[3], 0x0040), 0x5410);
-            const unsigned vw = __byte_perm(__byte_perm(vb[0], vb[1], 0x0040), __byte_perm(vb[2], vb[3], 0x0040), 0x5410);
+            const unsigned mo = __byte_perm(__byte_perm(mb[0], mb[1], 0x0040), __byte_perm(mb[2], mb[3], 0x0040), 0x5410);
+            const unsigned vo = __byte_perm(__byte_perm(vb[0], vb[1], 0x0040), __byte_perm(vb[2], vb[3], 0x0040), 0x5410);
+            float x[4];
+            apart(p[2 * h], x[0], x[1]);
+            apart(p[2 * h + 1], x[2], x[3]);
             if (vec) {
-                *reinterpret_cast<float4*>(c.param + at + i) = make_float4(p[4 * h], p[4 * h + 1], p[4 * h + 2], p[4 * h + 3]);
-                *reinterpret_cast<unsigned*>(mc + i) = mw;
-                *reinterpret_cast<unsigned*>(vc + i) = vw;
+                *reinterpret_cast<float4*>(c.param + at + i) = make_float4(x[0], x[1], x[2], x[3]);
+                *reinterpret_cast<unsigned*>(mc + i) = mo;
+                *reinterpret_cast<unsigned*>(vc + i) = vo;
             } else {
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
                     if (i + j < n) {
-                        c.param[at + i + j] = p[4 * h + j];
-                        mc[i + j] = (unsigned char)(mw >> (8 * j));
-                        vc[i + j] = (unsigned char)(vw >> (8 * j));
+                        c.param[at + i + j] = x[j];
+                        mc[i + j] = (unsigned char)(mo >> (8 * j));
+                        vc[i + j] = (unsigned char)(vo >> (8 * j));
                     }
             }
         }
