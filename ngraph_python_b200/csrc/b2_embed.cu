@@ -284,16 +284,17 @@ order_kernel(const OrderArgs a) {
         const Type* list = static_cast<const Type*>(a.idx) + lane;
         for (int at = begin; at < end; at += 32 * UN) {
             Type x[UN];
-            if (at + 32 * UN <= end) {
+            const bool whole = at + 32 * UN <= end;
+            if (whole) {
 #pragma unroll
                 for (int u = 0; u < UN; ++u) x[u] = list[at + u * 32];
             } else {
 #pragma unroll
-                for (int u = 0; u < UN; ++u) x[u] = at + u * 32 + lane < end ? list[at + u * 32] : (Type)-1;
+                for (int u = 0; u < UN; ++u) x[u] = at + u * 32 + lane < end ? list[at + u * 32] : (Type)0;
             }
 #pragma unroll
             for (int u = 0; u < UN; ++u) {
-                const int v = row_of(x[u], a.V, istep);
+                const int v = whole || at + u * 32 + lane < end ? row_of(x[u], a.V, istep) : -1;
                 // v / G, at most one too high, and v % G
                 unsigned q = __umulhi((unsigned)v, a.magic);
                 int r = v - (int)(q * G);

@@ -215,6 +215,31 @@ def test_flex16(n, F, V, offset):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dec", [2, 9])
+@pytest.mark.parametrize("n", [1, 31, 60, 257, 300])
+def test_flex16_index_with_an_exponent(n, dec):
+    """Tokens as mantissas of a step below one, of which a single one is no token: what is read beside the list's end is
+    none."""
+    import torch
+    from ngraph_python_b200 import lib
+    V, F = 37, 12
+    rng = np.random.RandomState(n)
+    idx = rng.randint(1, V, n)
+    delta = rng.randint(-100, 100, (n, F)).astype(np.int16)
+    scales = torch.tensor([[1.0, 1.0], [2.0 ** -dec, 2.0 ** dec], [1.0, 1.0]], dtype=torch.float32, device="cuda")
+    x, d = torch.from_numpy((idx << dec).astype(np.int16)).cuda(), torch.from_numpy(delta).cuda()
+    out, stats = torch.full((V, F), 7, dtype=torch.int16, device="cuda"), torch.zeros((3,), dtype=torch.int32, device="cuda")
+    nbytes = lib.embed_update_scratch_bytes(V, F, n)
+    scratch = torch.zeros((nbytes + 4096,), dtype=torch.uint8, device="cuda")
+    lib.check(lib.raw().b2_embed_update(d.data_ptr(), x.data_ptr(), out.data_ptr(), 1, 3, V, F, n, 1.0, -1, 0, scales.data_ptr(), 0, 1, 2,
+                                        stats.data_ptr(), None, 0, scratch.data_ptr(), nbytes, 0))
+    torch.cuda.synchronize()
+    want = np.zeros((V, F), np.int64)
+    np.add.at(want, idx, delta)
+    assert np.array_equal(out.cpu().numpy(), want) and not scratch[nbytes:].any()
+
+
+@pytest.mark.gpu
 def test_recorded_and_replayed_on_another_stream():
     """Two gradients that share a scratch in one graph, replayed with other tokens."""
     import torch
