@@ -966,6 +966,211 @@ class LutUpdateStep(_Step):
         self._flex_probe_then(t, ov.buffer, [dv.buffer, xv.buffer], call)
 
 
+def rows_of(view, axes, apart):
+    """(rows, features, distance of the rows) of a view whose memory has `axes` in this order, the first
+    `apart` of which may lie apart from the others; None where it has not."""
+    rows, features = _merge(view, list(axes)[:apart]), _merge(view, list(axes)[apart:])
+    if rows is None or features is None or (features[0] > 1 and features[1] != 1):
+        return None
+    if rows[0] > 1 and rows[1] < features[0]:
+        return None
+    return rows[0], features[0], rows[1] if rows[0] > 1 else features[0]
+
+
+class EmbedStep(_Step):
+    """A table lookup with a scale."""
+    kind = "embed"
+    launches = 1
+    probe_is_float = True
+
+    def __init__(self, index, op, t):
+        super(EmbedStep, self).__init__(index, op)
+        self.in_views = [t._view_of(a) for a in op.args]
+        self.out_views = [t._view_of(op)]
+        self.V, self.F = op.args[0].axes.lengths
+        self.n = op.args[1].axes.size
+        self.flex = t.flex
+
+    def launch(self, t):
+        wv, xv = self.in_views
+        ov = self.out_views[0]
+        raw, st = lib.raw(), t.stream.cuda_stream
+        head = (self._ptr(wv), self._ptr(xv), self._ptr(ov))
+        dims = (self.V, self.F, self.n, self.op.scale)
+        if not self.flex:
+            lib.check(raw.b2_embed_fprop(*(head + (0, lib.IDX_F32) + dims + (None, -1, -1, -1, None, None, 0, st))))
+            t.kernel_launches += 1
+            return
+        slots = (t._slot_for_read(wv.buffer, self), t._slot_for_read(xv.buffer, self), ov.buffer.slot_write)
+
+        def call(probe):
+            lib.check(raw.b2_embed_fprop(*(head + (1, lib.IDX_FLEX16) + dims + (t._table.data_ptr(),) + slots + (
+                t._stats.data_ptr(), t._probe64.data_ptr(), probe, st))))
+        self._flex_probe_then(t, ov.buffer, [wv.buffer, xv.buffer], call)
+
+
+class EmbedGradStep(_Step):
+    """Gradient of the table of a lookup with a scale, by sorted tokens."""
+    kind = "embed_grad"
+    launches = 2
+    probe_is_float = True
+
+    def __init__(self, index, op, t):
+        super(EmbedGradStep, self).__init__(index, op)
+        self.in_views = [t._view_of(a) for a in op.args]
+        self.out_views = [t._view_of(op)]
+        self.V, self.F = op.axes.lengths
+        self.n = op.args[1].axes.size
+        pad = op.fprop.pad_idx
+        self.pad_idx = -1 if pad is None else pad
+        self.scratch_bytes = lib.embed_update_scratch_bytes(self.V, self.F, self.n)
+        self.flex = t.flex
+
+    def launch(self, t):
+        dv, xv = self.in_views
+        ov = self.out_views[0]
+        raw, st = lib.raw(), t.stream.cuda_stream
+        head = (self._ptr(dv), self._ptr(xv), self._ptr(ov))
+        dims = (self.V, self.F, self.n, self.op.fprop.scale, self.pad_idx, 0)
+        scratch = t._scratch_aligned()
+        if not self.flex:
+            lib.check(raw.b2_embed_update(*(head + (0, lib.IDX_F32) + dims + (None, -1, -1, -1, None, None, 0) + scratch + (st,))))
+            t.kernel_launches += self.launches
+            return
+        slots = (t._slot_for_read(dv.buffer, self), t._slot_for_read(xv.buffer, self), ov.buffer.slot_write)
+
+        def call(probe):
+            lib.check(raw.b2_embed_update(*(head + (1, lib.IDX_FLEX16) + dims + (t._table.data_ptr(),) + slots + (
+                t._stats.data_ptr(), t._probe64.data_ptr(), probe) + scratch + (st,))))
+        self._flex_probe_then(t, ov.buffer, [dv.buffer, xv.buffer], call)
+
+
+class _Fp32Step(_Step):
+    """Steps of fp32 tensors alone, with results of several ops."""
+
+    def __init__(self, index, op, t):
+        super(_Fp32Step, self).__init__(index, op)
+        if t.flex:
+            raise ValueError("Unhandled op: {} takes fp32 tensors, not flex16".format(op))
+
+    def output_buffers(self):
+        return []          # no exponents
+
+    def _results(self, op, t, present):
+        """Views of those results of `op` that the computation holds."""
+        found = {k: t._view_of(r) for k, r in op.results.items() if r in present}
+        self.out_views = list(found.values())
+        return found
+
+
+def _norm_args(op):
+    a = lib.NormArgs()
+    a.rows, a.features, a.gate_kind = op.row_axes.size, op.norm_axes.size, op.gate_kind
+    a.residual_scale, a.eps = op.residual_scale, op.eps
+    return a
+
+
+class NormStep(_Fp32Step):
+    """Residual sum and norms at the edge of a block."""
+    kind = "norm"
+    launches = 1
+
+    def __init__(self, index, op, t, present):
+        super(NormStep, self).__init__(index, op, t)
+        self.views = {k: t._view_of(getattr(op, k)) for k in ("residual", "block", "gate", "post_weight", "weight")
+                      if getattr(op, k) is not None}
+        self.in_views = list(self.views.values())
+        # (the kernel stores the stream of a block, and out where there is a weight, whoever reads them)
+        present = set(present) | set(r for k, r in op.results.items() if k in ("stream", "out"))
+        self.found = self._results(op, t, present)
+
+    def launch(self, t):
+        op, a = self.op, _norm_args(self.op)
+        both, rows = op.row_axes + op.norm_axes, len(op.row_axes)
+        for k, v in list(self.views.items()) + list(self.found.items()):
+            setattr(a, "pre_weight" if k == "weight" else k, self._ptr(v))
+            if k in ("residual", "block", "stream", "out") or (k == "gate" and op.gate_kind == 3):
+                setattr(a, k + "_stride", rows_of(v, both, rows)[2])
+        lib.check(lib.raw().b2_norm_fprop(C.byref(a), t.stream.cuda_stream))
+        t.kernel_launches += 1
+
+
+class NormGradStep(_Fp32Step):
+    """All gradients of a NormStep."""
+    kind = "norm_grad"
+    launches = 2
+
+    def __init__(self, index, op, t, present):
+        super(NormGradStep, self).__init__(index, op, t)
+        self.views = {k: t._view_of(x) for k, x in op.reads.items()}
+        self.in_views = list(self.views.values())
+        self.found = self._results(op, t, present)
+        a = _norm_args(op.fprop)
+        for k in ("block", "gate", "post_weight", "weight"):          # (what the arguments are checked for)
+            setattr(a, "pre_weight" if k == "weight" else k, 256 if k in op.reads else None)
+        self.scratch_bytes = lib.norm_bprop_scratch_bytes(a)
+
+    def launch(self, t):
+        op, a, d = self.op, _norm_args(self.op.fprop), lib.NormGrads()
+        both, rows = op.fprop.row_axes + op.fprop.norm_axes, len(op.fprop.row_axes)
+        for k, v in self.views.items():
+            to = d if k in ("d_out", "d_stream") else a
+            name = "pre_weight" if k == "weight" else "residual" if k == "stream" and op.fprop.block is None else k
+            setattr(to, name, self._ptr(v))
+            if k in ("block", "stream", "d_out", "d_stream") or (k == "gate" and op.fprop.gate_kind == 3):
+                setattr(to, name + "_stride", rows_of(v, both, rows)[2])
+        for k, v in self.found.items():
+            setattr(d, "d_pre_weight" if k == "weight" else "d_" + k, self._ptr(v))
+        d.d_residual_stride = d.d_block_stride = d.d_gate_stride = a.features
+        scratch = t._scratch_aligned()
+        lib.check(lib.raw().b2_norm_bprop(C.byref(a), C.byref(d), scratch[0], scratch[1], t.stream.cuda_stream))
+        t.kernel_launches += self.launches
+
+
+class AdamwStep(_Fp32Step):
+    """One AdamW step over many variables."""
+    kind = "adamw"
+    launches = 1
+
+    def __init__(self, index, op, t):
+        super(AdamwStep, self).__init__(index, op, t)
+        self.out_views = [t._view_of(x) for x in op.written()]
+        self.gradients = [t._view_of(g) for g in op.gradients]
+        self.numbers = [None if x is None or isinstance(x, float) else t._view_of(x) for x in (op.lr, op.grad_scale)]
+        self.scale = None              # a tensor of a grad_scale that is a number
+        self.in_views = self.gradients + self.out_views + [v for v in self.numbers if v is not None]
+        self.plan = None
+
+    def _make_plan(self, t):
+        """The table of the step's work on the device (outside recordings: before the first call's launch)."""
+        op = self.op
+        tensors = (lib.AdamwTensor * len(op.variables))()
+        counter = 0
+        for x, v, g, state, decayed in zip(tensors, op.variables, self.gradients, op.states, op.decayed):
+            x.param, x.grad = self._ptr(t._view_of(v)), self._ptr(g)
+            x.n, x.decay, x.counter = v.axes.size, float(decayed), counter & 0xffffffff
+            counter += -(-x.n // 256) * 256
+            for name, s in zip(("m", "v", "m_scales", "v_scales"), state):
+                setattr(x, name, self._ptr(t._view_of(s)))
+        nbytes, self.chunks = lib.adamw_plan_bytes(tensors, op.state_bits)
+        self.plan = t.torch.empty((nbytes,), dtype=t.torch.uint8, device=t.device)
+        if isinstance(op.grad_scale, float) and op.grad_scale != 1.0:
+            self.scale = t.torch.full((1,), op.grad_scale, device=t.device)
+        lib.adamw_plan(tensors, op.state_bits, self.plan.data_ptr(), nbytes, t.stream.cuda_stream)
+
+    def launch(self, t):
+        op = self.op
+        if self.plan is None:
+            self._make_plan(t)
+        lr, scale = [None if v is None else self._ptr(v) for v in self.numbers]
+        if self.scale is not None:
+            scale = self.scale.data_ptr()
+        h = lib.AdamwHyper(op.lr if lr is None else 0.0, op.rates["beta1"], op.rates["beta2"], op.rates["eps"], op.rates["weight_decay"])
+        lib.check(lib.raw().b2_adamw_step(self.plan.data_ptr(), self.chunks, op.state_bits, C.byref(h), lr, scale,
+                                          self._ptr(t._view_of(op.count)), op.seed, t.stream.cuda_stream))
+        t.kernel_launches += 1
+
+
 class RngStep(_Step):
     """Random fill (RngFillKernel / FlexRngFillKernel, ngraph/transformers/gpu/tensor_ops.py:
     621-661, 713-740).  The stream of numbers is fixed by the transformer's seed and the position

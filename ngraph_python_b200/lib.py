@@ -488,6 +488,7 @@ def conv_fprop_scratch_bytes(flex, dims):
 
 CONV_FPROP, CONV_BPROP, CONV_UPDATE = 0, 1, 2
 RNG_UNIFORM, RNG_NORMAL = 0, 1
+IDX_F32, IDX_I32, IDX_I64, IDX_FLEX16 = 0, 1, 2, 3
 
 
 def conv_launches(flex, dims, conv_pass):

@@ -747,6 +747,248 @@ def lookuptable_update(delta, lut, idx, fprop_op):
     return update_lut(delta, lut, idx, fprop_op)
 
 
+# ---- operators of a language model's training step ----------------------------------------------
+# (The reference has no counterpart; they stand beside its lookup table, batch normalisation and
+# optimizers.  Gradients are ops of their own, like those of convolutions.)
+class ResultOp(Op):
+    """One of several results of an op."""
+
+    def __init__(self, of, which, axes, **kw):
+        super(ResultOp, self).__init__((of,), axes, **kw)
+        self.which = which
+
+
+def _check_operand(what, op, axes):
+    if not op.axes.is_equal_set(axes):
+        raise ValueError("%s has the axes %s where %s are expected" % (what, op.axes, axes))
+
+
+class EmbeddingOp(Op):
+    """scale * table[idx]: args (table, idx), result on the axes of idx and the table's second."""
+
+    def __init__(self, table, idx, scale=1.0, pad_idx=None, **kw):
+        table, idx = as_op(table), as_op(idx)
+        if len(table.axes) != 2:
+            raise ValueError("embedding table shape must be length 2, found {}".format(len(table.axes)))
+        if len(idx.axes) == 0:
+            raise ValueError("embedding index needs an axis")
+        if table.axes[1] in idx.axes or table.axes[1].name in [a.name for a in idx.axes]:
+            raise ValueError("the table's axis %s is an axis of the index" % table.axes[1])
+        super(EmbeddingOp, self).__init__((table, idx), list(idx.axes) + [table.axes[1]], **kw)
+        self.scale = float(scale)
+        self.pad_idx = None if pad_idx is None else int(pad_idx)
+
+    def layouts(self):
+        """(argument, its axes in the order of memory, how many of them may lie apart)"""
+        return [(self.args[0], self.args[0].axes, 0), (self.args[1], self.args[1].axes, 0)]
+
+
+def embedding(table, idx, scale=1.0, pad_idx=None):
+    """Rows of `table` [tokens, features] looked up at `idx` (any axes) and scaled.  Indices outside
+    the table, and NaN, read as zero; the gradient of row pad_idx is zero."""
+    return EmbeddingOp(table, idx, scale, pad_idx)
+
+
+class EmbeddingGradOp(Op):
+    """The table's gradient: args (delta, idx); rows of delta added up per token in their order."""
+
+    def __init__(self, delta, fprop, **kw):
+        delta = as_op(delta)
+        if not isinstance(fprop, EmbeddingOp):
+            raise ValueError("embedding_grad needs the forward EmbeddingOp, got {}".format(fprop))
+        _check_operand("delta", delta, fprop.axes)
+        self.fprop = fprop
+        super(EmbeddingGradOp, self).__init__((delta, fprop.args[1]), fprop.args[0].axes, **kw)
+
+    def layouts(self):
+        return [(self.args[0], self.fprop.axes, 0), (self.args[1], self.args[1].axes, 0)]
+
+
+def embedding_grad(delta, fprop):
+    """Gradient of the table that the embedding `fprop` looks up, from that of its result."""
+    return EmbeddingGradOp(delta, fprop)
+
+
+class ResidualNormOp(Op):
+    """stream = residual_scale * residual + gate * (rms(block) * post_weight),
+    out = rms(stream) * weight, with rms(x) = x / sqrt(mean(x^2) + eps) over `axes`."""
+
+    def __init__(self, residual, block, weight, axes, post_weight=None, gate=None, residual_scale=1.0,
+                 eps=1e-6, **kw):
+        residual = as_op(residual)
+        self.norm_axes = make_axes(axes)
+        if not len(self.norm_axes) or not self.norm_axes.is_sub_set(residual.axes):
+            raise ValueError("the axes %s are not axes of the operand %s" % (self.norm_axes, residual.axes))
+        self.row_axes = residual.axes - self.norm_axes
+        both = self.row_axes + self.norm_axes
+        optional = lambda x: None if x is None else as_op(x)  # noqa: E731
+        self.residual, self.block, self.weight = residual, optional(block), optional(weight)
+        self.post_weight, self.gate = optional(post_weight), optional(gate)
+        if self.block is None and (self.gate is not None or self.post_weight is not None or float(residual_scale) != 1.0):
+            raise ValueError("a gate, a weight or a scale without a block")
+        if self.block is None and self.weight is None:
+            raise ValueError("nothing to compute: neither a block nor a weight")
+        if self.block is not None:
+            _check_operand("block", self.block, both)
+        for what, w in (("weight", self.weight), ("post_weight", self.post_weight)):
+            if w is not None:
+                _check_operand(what, w, self.norm_axes)
+        self.gate_kind = 0
+        if self.gate is not None:
+            kinds = [k for k, ax in ((1, self.norm_axes), (2, self.row_axes), (3, both))
+                     if len(ax) and self.gate.axes.is_equal_set(ax)]
+            if not kinds:
+                raise ValueError("a gate has the axes %s, %s or %s, not %s" %
+                                 (self.norm_axes, self.row_axes, both, self.gate.axes))
+            self.gate_kind = kinds[0]
+        self.residual_scale, self.eps = float(residual_scale), float(eps)
+        if not self.eps >= 0:
+            raise ValueError("eps is not negative: %r" % (eps,))
+        operands = [x for x in (self.residual, self.block, self.gate, self.post_weight, self.weight) if x is not None]
+        super(ResidualNormOp, self).__init__(operands, both, **kw)
+        self.results = {}
+        if self.block is not None:
+            self.results["stream"] = ResultOp(self, "stream", both)
+        if self.weight is not None:
+            self.results["out"] = ResultOp(self, "out", both)
+            self.results["stream_rstd"] = ResultOp(self, "stream_rstd", self.row_axes)
+        if self.post_weight is not None:
+            self.results["block_rstd"] = ResultOp(self, "block_rstd", self.row_axes)
+
+    @property
+    def gate_axes(self):
+        return (None, self.norm_axes, self.row_axes, self.row_axes + self.norm_axes)[self.gate_kind]
+
+    def layouts(self):
+        both, rows = self.row_axes + self.norm_axes, len(self.row_axes)
+        found = [(x, both, rows) for x in (self.residual, self.block) if x is not None]
+        found += [(x, self.norm_axes, 0) for x in (self.post_weight, self.weight) if x is not None]
+        if self.gate is not None:
+            found.append((self.gate, self.gate_axes, rows if self.gate_kind == 3 else 0))
+        return found
+
+
+def residual_norm(residual, block, weight, axes, post_weight=None, gate=None, residual_scale=1.0, eps=1e-6):
+    """The edge between two blocks of a residual network: (stream, out) with
+    stream = residual_scale * residual + gate * (rms(block) * post_weight) and out = rms(stream) * weight.
+    gate (per feature, per row or for every value) and post_weight may be None; weight None: out is None."""
+    op = ResidualNormOp(residual, block, weight, axes, post_weight, gate, residual_scale, eps)
+    return op.results.get("stream"), op.results.get("out")
+
+
+def rms_norm(x, weight, axes, eps=1e-6):
+    """x / sqrt(mean(x^2) + eps) * weight over `axes`."""
+    return ResidualNormOp(x, None, weight, axes, eps=eps).results["out"]
+
+
+class ResidualNormGradOp(Op):
+    """All gradients of a ResidualNormOp in one step."""
+
+    def __init__(self, fprop, d_out=None, d_stream=None, **kw):
+        if isinstance(fprop, ResultOp):
+            fprop = fprop.args[0]
+        if not isinstance(fprop, ResidualNormOp):
+            raise ValueError("residual_norm_grad needs a result of the forward op, got {}".format(fprop))
+        if (d_out is None) != (fprop.weight is None):
+            raise ValueError("the gradient of out and a weight go together")
+        if d_out is None and d_stream is None:
+            raise ValueError("no gradient to start from")
+        both = fprop.row_axes + fprop.norm_axes
+        self.fprop = fprop
+        self.d_out, self.d_stream = [None if d is None else as_op(d) for d in (d_out, d_stream)]
+        for what, d in (("d_out", self.d_out), ("d_stream", self.d_stream)):
+            if d is not None:
+                _check_operand(what, d, both)
+        self.reads = dict(d_out=self.d_out, d_stream=self.d_stream, block=fprop.block, gate=fprop.gate,
+                          post_weight=fprop.post_weight, weight=fprop.weight,
+                          stream=fprop.results.get("stream", fprop.residual) if fprop.weight is not None else None,
+                          stream_rstd=fprop.results.get("stream_rstd"), block_rstd=fprop.results.get("block_rstd"))
+        self.reads = {k: v for k, v in self.reads.items() if v is not None}
+        super(ResidualNormGradOp, self).__init__(list(self.reads.values()), both, **kw)
+        self.results = {"residual": ResultOp(self, "residual", both)}
+        if fprop.block is not None:
+            self.results["block"] = ResultOp(self, "block", both)
+        for name, ax in (("gate", fprop.gate_axes), ("post_weight", fprop.norm_axes), ("weight", fprop.norm_axes)):
+            if getattr(fprop, name) is not None:
+                self.results[name] = ResultOp(self, name, ax)
+
+    def layouts(self):
+        f = self.fprop
+        both, rows = f.row_axes + f.norm_axes, len(f.row_axes)
+        axes = dict(post_weight=(f.norm_axes, 0), weight=(f.norm_axes, 0), stream_rstd=(f.row_axes, 0), block_rstd=(f.row_axes, 0),
+                    gate=(f.gate_axes, rows if f.gate_kind == 3 else 0))
+        return [(x,) + axes.get(k, (both, rows)) for k, x in self.reads.items()]
+
+
+def residual_norm_grad(fprop, d_out=None, d_stream=None):
+    """Gradients of residual_norm or rms_norm (`fprop` is one of its results) from those of `out` and, where
+    later blocks read it, of `stream`: a dict of residual, block, gate, post_weight and weight, those of them
+    that the forward op has.  The gradient of rms_norm's operand is `residual`."""
+    return dict(ResidualNormGradOp(fprop, d_out, d_stream).results)
+
+
+class AdamWOp(Op):
+    """One AdamW step over all of `variables` (see adamw).  Its value is the number of steps made."""
+    is_tensor_op = False
+
+    def __init__(self, variables, gradients, lr, beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=0.01, no_decay=(),
+                 state_bits=32, grad_scale=None, seed=0, **kw):
+        variables, gradients = as_ops(variables), as_ops(gradients)
+        if len(variables) != len(gradients):
+            raise ValueError("%d variables and %d gradients" % (len(variables), len(gradients)))
+        if len(set(variables)) != len(variables):
+            raise ValueError("a variable occurs twice")
+        for v, g in zip(variables, gradients):
+            if not isinstance(v, AssignableTensorOp) or v.is_constant:
+                raise ValueError("{} is not assignable.".format(v))
+            _check_operand("the gradient of %s" % v, g, v.axes)
+        if state_bits not in (8, 32):
+            raise ValueError("moments are held in 32 or 8 bits, not in %r" % (state_bits,))
+        for x in no_decay:
+            if x not in variables:
+                raise ValueError("{} is not among the variables".format(x))
+        self.variables, self.gradients = variables, gradients
+        self.rates = dict(beta1=float(beta1), beta2=float(beta2), eps=float(eps), weight_decay=float(weight_decay))
+        if not (0 <= self.rates["beta1"] < 1 and 0 <= self.rates["beta2"] < 1 and self.rates["eps"] >= 0):
+            raise ValueError("bad rates: %s" % self.rates)
+        self.state_bits, self.seed = state_bits, int(seed) & 0xffffffff
+        self.decayed = [v not in no_decay for v in variables]
+        # (numbers stay as they are: an op of one would be rounded to fp32)
+        self.lr = float(lr) if isinstance(lr, numbers.Number) else as_op(lr)
+        self.grad_scale = float(grad_scale) if isinstance(grad_scale, numbers.Number) else None if grad_scale is None else as_op(grad_scale)
+        for what, x in (("lr", self.lr), ("grad_scale", self.grad_scale)):
+            if isinstance(x, Op) and x.axes.size != 1:
+                raise ValueError("%s is a number, not a tensor with axes %s" % (what, x.axes))
+        self.count = persistent_tensor([make_axis(1, name="steps")], initial_value=0.0)
+        # 32 bits: (m, v).  8: bytes of m and of sqrt(v), four to a word, and the scales of 256 values each
+        words = lambda n, per, name: persistent_tensor([make_axis(-(-n // per), name="words")], initial_value=0.0, name=name)  # noqa: E731
+        self.states = []
+        for v in variables:
+            n = v.axes.size
+            if state_bits == 32:
+                self.states.append(tuple(persistent_tensor(v.axes, initial_value=0.0, name="%s_%s" % (v.name, m)) for m in "mv"))
+            else:
+                self.states.append((words(n, 4, v.name + "_m"), words(n, 4, v.name + "_v"), words(n, 256, v.name + "_m_scales"),
+                                    words(n, 256, v.name + "_v_scales")))
+        args = list(variables) + list(gradients) + [s for x in self.states for s in x] + [self.count]
+        super(AdamWOp, self).__init__(args + [x for x in (self.lr, self.grad_scale) if isinstance(x, Op)], self.count.axes, **kw)
+
+    def layouts(self):
+        return [(g, v.axes, 0) for v, g in zip(self.variables, self.gradients)]
+
+    def written(self):
+        return list(self.variables) + [s for x in self.states for s in x] + [self.count]
+
+
+def adamw(variables, gradients, lr, beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=0.01, no_decay=(), state_bits=32,
+          grad_scale=None, seed=0):
+    """One AdamW step over many variables at once.  lr, and grad_scale, which multiplies every gradient, are
+    numbers or ops whose value is one.  no_decay: the variables without weight decay.  state_bits 8: moments as
+    e4m3 bytes with a scale for every 256, rounded at random (from `seed`, the position and the step).  The
+    moments (op.states) and the number of steps (op.count) are persistent tensors, zero before the first."""
+    return AdamWOp(variables, gradients, lr, beta1, beta2, eps, weight_decay, no_decay, state_bits, grad_scale, seed)
+
+
 # ---- communication ----------------------------------------------------------------------------
 class AllReduceOp(Op):
     """Sum (or mean) of a tensor over all data-parallel replicas; every replica gets the result

@@ -26,9 +26,10 @@ from . import kernels
 from . import lib
 from . import comm as commmod
 from . import tracing
-from .op_graph import (AllReduceOp, AssignableTensorOp, AssignOp, Axes, AxesCastOp, BroadcastOp,
+from .op_graph import (AdamWOp, AllReduceOp, AssignableTensorOp, AssignOp, Axes, AxesCastOp, BroadcastOp,
                        ConvolutionOp, DotOp, bprop_conv, update_conv,
-                       BpropPoolOp, ElementWiseOp, LookupTableOp, Op, PoolingOp, ReductionOp, RngOp,
+                       BpropPoolOp, ElementWiseOp, EmbeddingGradOp, EmbeddingOp, LookupTableOp, Op,
+                       PoolingOp, ReductionOp, ResidualNormGradOp, ResidualNormOp, ResultOp, RngOp,
                        ReorderAxes, ReshapeOp, SequentialOp, TensorSliceOp, update_lut,
                        ViewOp, as_op, make_axes)
 
@@ -825,6 +826,7 @@ class _Planner(object):
                 self.consumers[self._base_tensor(a)[0]].append(op)
         returned = set(self._base_tensor(r)[0] for r in returns)
         self.returned = returned
+        self.present = set(ordered)
         for buf in self.t._buffers.values():
             buf.last_write_step = -1
             buf.last_read_step = -1
@@ -855,8 +857,8 @@ class _Planner(object):
                 self._place_ew(op)
             elif isinstance(op, AllReduceOp):
                 self._place_allreduce(op)
-            elif isinstance(op, (AssignableTensorOp, ViewOp, SequentialOp)):
-                continue
+            elif isinstance(op, (AssignableTensorOp, ViewOp, SequentialOp, ResultOp)):
+                continue               # (results come with the op that they are of)
             else:
                 self._place_other(op)
         while self.deferred:                       # reduced tensors that are only returned
@@ -1257,6 +1259,10 @@ class _Planner(object):
                 for a in op.args:
                     if not self.t._view_of(a).is_dense():
                         self._densify(a, list(self.t._view_of(a).axes), saved)
+            elif hasattr(op, "layouts"):
+                for a, axes, apart in op.layouts():
+                    if kernels.rows_of(self.t._view_of(a), axes, apart) is None:
+                        self._densify(a, list(axes), saved)
             step = self._make_other_step(op, tail)
         finally:
             for key, old in saved.items():
@@ -1312,6 +1318,16 @@ class _Planner(object):
             step = kernels.LutUpdateStep(index, op, self.t)
         elif isinstance(op, RngOp):
             step = kernels.RngStep(index, op, self.t)
+        elif isinstance(op, EmbeddingOp):
+            step = kernels.EmbedStep(index, op, self.t)
+        elif isinstance(op, EmbeddingGradOp):
+            step = kernels.EmbedGradStep(index, op, self.t)
+        elif isinstance(op, ResidualNormOp):
+            step = kernels.NormStep(index, op, self.t, self.present)
+        elif isinstance(op, ResidualNormGradOp):
+            step = kernels.NormGradStep(index, op, self.t, self.present)
+        elif isinstance(op, AdamWOp):
+            step = kernels.AdamwStep(index, op, self.t)
         else:
             raise ValueError("Unhandled op: {}".format(op))
         if tail:
@@ -1345,6 +1361,12 @@ class _Planner(object):
                     step.reads_after_write.add(id(b))
         self.steps.append(step)
         self.producer[op] = index
+        for r in getattr(op, "results", {}).values():
+            self.producer[r] = index
+        if isinstance(op, AdamWOp):
+            for x in op.written():         # in place: later readers come behind this step
+                self.t._buffer_of(x).last_write_step = index
+                self.last_assign[x] = None
         self.t._need_scratch(step.scratch_bytes)
         for b in step.output_buffers():
             if b not in self.written_buffers:
@@ -1982,6 +2004,8 @@ class B200Transformer(object):
             v = View(src.buffer, op.axes, strides, offset)
         elif isinstance(op, AssignOp):
             v = self._view_of(op.args[0])
+        elif isinstance(op, AdamWOp):
+            v = self._view_of(op.count)
         else:
             v = View.dense(self._buffer_of(op))
         self._views[op] = v
