@@ -200,12 +200,13 @@ __device__ __forceinline__ float2 from_e4m3(unsigned two) {
     const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)two, __NV_E4M3);
     return __half22float2(__half2(h));
 }
-// 448 / top of both moments, and their scales top / 448: one division in each of four lanes.
+// What values are multiplied by, 448 (1 / top), and the scales, top (1 / 448), of both moments: one division, in different
+// lanes for both.
 __device__ __forceinline__ void scales_of(float top_m, float top_r, float& to_m, float& to_r, float& new_ms, float& new_vs) {
     const int lane = threadIdx.x & 31;
     const float top = lane & 1 ? top_r : top_m;
     const bool live = top > 7.888609052210118e-31f;             // 2^-100
-    float x = live ? __fdiv_rn(lane & 2 ? top : 448.0f, lane & 2 ? 448.0f : top) : 0.0f;
+    float x = live ? lane & 2 ? __fmul_rn(top, 1.0f / 448.0f) : __fmul_rn(__fdiv_rn(1.0f, top), 448.0f) : 0.0f;
     if ((lane & 2) && !(top <= 3.402823466e+38f)) x = __int_as_float(0x7fffffff);
     to_m = __shfl_sync(0xffffffffu, x, 0);
     to_r = __shfl_sync(0xffffffffu, x, 1);

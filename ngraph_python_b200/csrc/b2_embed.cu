@@ -681,8 +681,8 @@ int launch_update(const void* delta, const void* idx, void* dW, int kind, int V,
         default: B2_CHECK(launch_order<B2_IDX_FLEX16>(a, owners, st));
     }
     const long long sum_blocks = (n + 8 * kWindow - 1) / (8 * kWindow) * a.col_blocks;
-    // about 16 KB of zeros to a warp
-    const long long fit = 16384 / ((long long)F * (long long)sizeof(T));
+    // about 4 KB of zeros to a warp (16: 3001 x 301 flex16 into 10007 rows 22 us, 15 with 4)
+    const long long fit = 4096 / ((long long)F * (long long)sizeof(T));
     const int zero_rows = fit < 1 ? 1 : fit > 32 ? 32 : (int)fit;
     const long long zero_blocks = onto || f.probe ? 0 : ((long long)owners * a.rows + 8 * zero_rows - 1) / (8 * zero_rows);
     B2_REQUIRE(sum_blocks + zero_blocks < (1ll << 31), "%lld tokens of %d features are too many for one launch", n, F);

@@ -89,9 +89,9 @@ def step(param, grad, state, t, hyper, decay=1.0, grad_scale=1.0, seed=0, counte
         padded[:n] = np.abs(x)
         top = padded.reshape(blocks, BLOCK).max(1)
         live = top > F(2.0 ** -100)
-        with np.errstate(divide="ignore", over="ignore"):
-            inverse = np.where(live, F(448) / top, F(0)).astype(np.float32)
-        scale = np.where(live, top / F(448), F(0)).astype(np.float32)
+        with np.errstate(divide="ignore", over="ignore", invalid="ignore"):
+            inverse = np.where(live, F(1) / top * F(448), F(0)).astype(np.float32)
+        scale = np.where(live, top * (F(1) / F(448)), F(0)).astype(np.float32)
         q = x * inverse[at]
         c = to_e4m3(q, bits)
         if is_root:
