@@ -124,9 +124,12 @@ template <int VEC> struct Sink<short, VEC> {
     __device__ __forceinline__ void done(const FlexArgs& f) {
         unsigned bits = probe ? __float_as_uint(most) : (unsigned)(int)rintf(most);
         bits = __reduce_max_sync(0xffffffffu, bits);
-        if ((threadIdx.x & 31) == 0 && bits) {
-            if (probe) atomicMax(f.probe_out, (unsigned long long)bits);
-            else atomicMax(f.stats + f.slot_out, (int)bits);
+        if ((threadIdx.x & 31) != 0) return;
+        // (an atomic only where it would change the word: thousands of warps come with nothing new)
+        if (probe) {
+            if (bits > __ldcg(f.probe_out)) atomicMax(f.probe_out, (unsigned long long)bits);
+        } else if ((int)bits > __ldcg(f.stats + f.slot_out)) {
+            atomicMax(f.stats + f.slot_out, (int)bits);
         }
     }
 };
@@ -172,6 +175,40 @@ embed_kernel(const T* __restrict__ table, const void* __restrict__ idx, T* __res
                 for (int k = 0; k < VEC; ++k) v[k] = flex ? (v[k] * step) * scale : v[k] * scale;
             }
             sink.put(out + e * VEC, v);
+        }
+    }
+    sink.done(f);
+}
+
+// Rows that are not aligned: a warp takes 32 * UN columns of a token.  (In the order of the result's values, with a
+// division for each, 16384 x 1001 took 38 us, flex16 89.)
+template <typename T, int KIND, int UN>
+__global__ void __launch_bounds__(256)
+embed_apart_kernel(const T* __restrict__ table, const void* __restrict__ idx, T* __restrict__ out, int V, int F, long long n, unsigned col_blocks, float scale,
+                   FlexArgs f) {
+    after_earlier_kernels();
+    const bool flex = sizeof(T) == 2;
+    const float step = flex ? f.table[f.slot_in].scale : 1.0f;
+    const float istep = KIND == B2_IDX_FLEX16 ? f.table[f.slot_idx].scale : 1.0f;
+    Sink<T, 1> sink(f);
+    const long long units = n * col_blocks;
+    for (long long unit = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); unit < units; unit += (long long)gridDim.x * 8) {
+        const long long t = units <= 0xffffffffll ? (long long)((unsigned)unit / col_blocks) : unit / col_blocks;
+        const int col = (int)(unit - t * col_blocks) * 32 * UN + (int)(threadIdx.x & 31);
+        const int row = token_at<KIND>(idx, t, V, istep);
+        const T* from = table + (long long)(row < 0 ? 0 : row) * F + col;
+        T* to = out + t * F + col;
+        T w[UN];
+#pragma unroll
+        for (int u = 0; u < UN; ++u)
+            if (col + u * 32 < F) w[u] = from[u * 32];
+#pragma unroll
+        for (int u = 0; u < UN; ++u) {
+            if (col + u * 32 >= F) break;
+            float v = row < 0 ? 0.0f : (float)w[u];
+            v = flex ? (v * step) * scale : v * scale;
+            if (row < 0) v = 0.0f;
+            sink.put(to + u * 32, &v);
         }
     }
     sink.done(f);
@@ -621,18 +658,23 @@ template <typename T> constexpr int wide() { return 16 / (int)sizeof(T); }
 template <typename T, int KIND>
 int launch_embed(const void* table, const void* idx, void* out, int V, int F, long long n, float scale, const FlexArgs& f, cudaStream_t st) {
     constexpr int W = wide<T>();
-    const bool vec = F % W == 0 && b2::aligned16(table) && b2::aligned16(out);
-    const long long total = n * (long long)(vec ? F / W : F);
+    if (F % W != 0 || !b2::aligned16(table) || !b2::aligned16(out)) {
+        constexpr int UN = 8;
+        const unsigned col_blocks = (unsigned)((F + 32 * UN - 1) / (32 * UN));
+        long long blocks = (n * (long long)col_blocks + 7) / 8;
+        if (blocks > (1ll << 30)) blocks = 1ll << 30;
+        B2_CUDA((b2::launch_after(embed_apart_kernel<T, KIND, UN>, dim3((unsigned)blocks), 256, 0, st, (const T*)table, idx, (T*)out, V, F, n, col_blocks, scale, f)));
+        return B2_OK;
+    }
+    const long long total = n * (long long)(F / W);
     // four vectors a thread hide the two loads behind one another; where that leaves SMs without a block, one
     const bool deep = total >= 4ll * 256 * b2::kSms;
     long long blocks = (total + (deep ? 1023 : 255)) / (deep ? 1024 : 256);
     if (blocks > (1ll << 30)) blocks = 1ll << 30;
-#define B2_EMBED(VEC, UN) \
-    B2_CUDA((b2::launch_after(embed_kernel<T, VEC, KIND, UN>, dim3((unsigned)blocks), 256, 0, st, (const T*)table, idx, (T*)out, V, F, n, scale, f)))
-    if (vec && deep) B2_EMBED(W, 4);
-    else if (vec) B2_EMBED(W, 1);
-    else if (deep) B2_EMBED(1, 4);
-    else B2_EMBED(1, 1);
+#define B2_EMBED(UN) \
+    B2_CUDA((b2::launch_after(embed_kernel<T, W, KIND, UN>, dim3((unsigned)blocks), 256, 0, st, (const T*)table, idx, (T*)out, V, F, n, scale, f)))
+    if (deep) B2_EMBED(4);
+    else B2_EMBED(1);
 #undef B2_EMBED
     return B2_OK;
 }
