@@ -679,6 +679,141 @@ int launch_embed(const void* table, const void* idx, void* out, int V, int F, lo
     return B2_OK;
 }
 
+// ---- gradient of few tokens: one launch ---------------------------------------------------------------------------
+// A CTA takes its own rows through all steps: its tokens, in order, their numbers within each row, the sums, in parts as
+// above, a warp to a row and its columns at a time, and the zeros.  For more tokens the sums want more warps than those of
+// the CTA that owns a frequent one.
+constexpr int kSmall = 256;
+
+__device__ __forceinline__ int token_of_kind(int kind, const void* idx, int i, int V, float step) {
+    switch (kind) {
+        case B2_IDX_F32: return token_at<B2_IDX_F32>(idx, i, V, step);
+        case B2_IDX_I32: return token_at<B2_IDX_I32>(idx, i, V, step);
+        case B2_IDX_I64: return token_at<B2_IDX_I64>(idx, i, V, step);
+        default: return token_at<B2_IDX_FLEX16>(idx, i, V, step);
+    }
+}
+
+template <typename T, int VEC, int UN, bool ONTO>
+__global__ void __launch_bounds__(512)
+small_update_kernel(const T* __restrict__ delta, T* dW, const OrderArgs a, int kind, int F, float scale, const FlexArgs f) {
+    extern __shared__ unsigned whole[];         // [rows] tokens of each row
+    __shared__ uint2 flat[kSmall];              // position and row of the CTA's tokens
+    __shared__ unsigned ranks[kSmall], found_by[kSmall / 32];
+    constexpr int COLS = 32 * VEC, WARPS = 512 / 32;
+    constexpr bool flex = sizeof(T) == 2;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const unsigned G = gridDim.x, b = blockIdx.x;
+    const int rows = a.rows;
+    for (int i = threadIdx.x; i < rows; i += 512) whole[i] = 0;
+    after_earlier_kernels();
+    const float istep = kind == B2_IDX_FLEX16 ? a.table[a.slot_idx].scale : 1.0f, step = flex ? f.table[f.slot_in].scale : 1.0f;
+    Sink<T, VEC> sink(f);
+    int local = 0;
+    unsigned those = 0;
+    if (warp < kSmall / 32) {
+        const int i = threadIdx.x;
+        const int v = i < a.n ? token_of_kind(kind, a.idx, i, a.V, istep) : -1;
+        local = v / (int)G;
+        those = __ballot_sync(0xffffffffu, v >= 0 && v != a.pad && (unsigned)(v - local * (int)G) == b);
+        if (lane == 0) found_by[warp] = __popc(those);
+    }
+    __syncthreads();
+    unsigned all = 0, before = 0;
+#pragma unroll
+    for (int w = 0; w < kSmall / 32; ++w) {
+        before += w < warp ? found_by[w] : 0u;
+        all += found_by[w];
+    }
+    if (those >> lane & 1u) flat[before + __popc(those & ((1u << lane) - 1u))] = make_uint2(threadIdx.x, (unsigned)local);
+    __syncthreads();
+    if (warp == 0)
+        for (unsigned k = lane; k - lane < all; k += 32) {
+            const unsigned mine = k < all ? flat[k].y : 0xffffffffu;
+            const unsigned same = __match_any_sync(0xffffffffu, mine);
+            const unsigned c = k < all ? whole[mine] : 0u, place = __popc(same & ((1u << lane) - 1u));
+            __syncwarp();
+            if (k < all) {
+                ranks[k] = c + place;
+                if (place == 0) whole[mine] = c + __popc(same);
+            }
+            __syncwarp();
+        }
+    __syncthreads();
+    for (unsigned unit = warp; unit < all * (unsigned)a.col_blocks; unit += WARPS) {
+        const unsigned first = unit / (unsigned)a.col_blocks;
+        if (ranks[first] != 0) continue;        // (a row is taken up where its first token stands)
+        const unsigned mine = flat[first].y;
+        const int count = (int)whole[mine], col0 = (int)(unit - first * a.col_blocks) * COLS * UN + lane * VEC;
+        T* to = dW + ((long long)b + (long long)mine * G) * F + col0;
+        Pack<T, VEC> old[UN];
+        if constexpr (ONTO)
+#pragma unroll
+            for (int u = 0; u < UN; ++u)
+                if (col0 + u * COLS < F) old[u].load(to + u * COLS);
+        float acc[UN][VEC] = {}, sum[UN][VEC] = {};
+        int done = 0;
+        for (unsigned j0 = first; done < count; j0 += 32) {
+            const uint2 e = j0 + lane < all ? flat[j0 + lane] : make_uint2(0, 0xffffffffu);
+            unsigned left = __ballot_sync(0xffffffffu, e.y == mine);
+            while (left) {
+                constexpr int AHEAD = UN == 1 ? 8 : 4;
+                Pack<T, VEC> w[AHEAD][UN];
+                const int now = min(AHEAD, __popc(left));
+#pragma unroll
+                for (int k = 0; k < AHEAD; ++k) {
+                    const long long t = __shfl_sync(0xffffffffu, e.x, left ? __ffs(left) - 1 : 0);
+                    left &= left - 1;
+                    if (k < now)
+#pragma unroll
+                        for (int u = 0; u < UN; ++u)
+                            if (col0 + u * COLS < F) w[k][u].load(delta + t * F + col0 + u * COLS);
+                }
+#pragma unroll
+                for (int k = 0; k < AHEAD; ++k) {
+                    if (k >= now) break;
+#pragma unroll
+                    for (int u = 0; u < UN; ++u)
+                        if (col0 + u * COLS < F) {
+                            float v[VEC];
+                            w[k][u].get(v);
+#pragma unroll
+                            for (int c = 0; c < VEC; ++c) acc[u][c] += v[c];
+                        }
+                    if (++done % kPart == 0 || done == count)
+#pragma unroll
+                        for (int u = 0; u < UN; ++u)
+#pragma unroll
+                            for (int c = 0; c < VEC; ++c) {
+                                sum[u][c] = done <= kPart ? acc[u][c] : sum[u][c] + acc[u][c];
+                                acc[u][c] = 0.0f;
+                            }
+                }
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < UN; ++u) {
+            if (col0 + u * COLS >= F) continue;
+            float v[VEC];
+#pragma unroll
+            for (int c = 0; c < VEC; ++c) v[c] = flex ? (sum[u][c] * step) * scale : sum[u][c] * scale;
+            if constexpr (ONTO) {
+                float o[VEC];
+                old[u].get(o);
+#pragma unroll
+                for (int c = 0; c < VEC; ++c) v[c] = o[c] + v[c];
+            }
+            sink.put(to + u * COLS, v);
+        }
+    }
+    if (!ONTO && !f.probe)
+        for (int r = warp; r < rows; r += WARPS) {
+            const long long row = (long long)b + (long long)r * G;
+            if (row < a.V && whole[r] == 0) zero_row(dW + row * F, F, lane);
+        }
+    sink.done(f);
+}
+
 // Columns of a warp: 16 bytes to a lane, or four values apart where rows are not aligned.
 constexpr int kApart = 4;
 int col_blocks_of(int F, int vec) {
@@ -716,6 +851,19 @@ int launch_update(const void* delta, const void* idx, void* dW, int kind, int V,
     a.s = scratch_of(scratch, V, F, n, a.col_blocks);
     a.table = f.table;
     a.slot_idx = f.slot_idx;
+    if (n <= kSmall) {
+#define B2_SMALL(VEC, UN, ONTO)                                                                                                              \
+    B2_CUDA((b2::launch_after(small_update_kernel<T, VEC, UN, ONTO>, dim3((unsigned)owners), 512, (size_t)a.rows * 4, st, (const T*)delta, (T*)dW, a, kind, \
+                              F, scale, f)))
+        if constexpr (sizeof(T) == 4) {
+            if (onto && vec) B2_SMALL(W, 1, true);
+            else if (onto) B2_SMALL(1, kApart, true);
+        }
+        if (!onto && vec) B2_SMALL(W, 1, false);
+        else if (!onto) B2_SMALL(1, kApart, false);
+#undef B2_SMALL
+        return B2_OK;
+    }
     switch (kind) {
         case B2_IDX_F32: B2_CHECK(launch_order<B2_IDX_F32>(a, owners, st)); break;
         case B2_IDX_I32: B2_CHECK(launch_order<B2_IDX_I32>(a, owners, st)); break;

@@ -144,6 +144,29 @@ def test_sums_are_added_in_the_order_of_the_tokens():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("n", [33, 64, 200, 256, 257, 300, 5000])
+def test_parts_of_long_rows(n):
+    """The bits of parts of 32 tokens added up one after another, whichever kernels a size takes."""
+    rng = np.random.RandomState(n)
+    delta = (rng.standard_normal((n, 12)) * 10.0 ** rng.randint(-3, 4, (n, 1))).astype(np.float32)
+    idx = rng.choice([2, 4], n, p=[0.8, 0.2])
+    want = np.zeros((6, 12), np.float32)
+    for v in (2, 4):
+        rows = delta[idx == v]
+        parts = []
+        for at in range(0, len(rows), 32):
+            part = np.zeros(12, np.float32)
+            for r in rows[at:at + 32]:
+                part = part + r
+            parts.append(part)
+        for part in parts:
+            want[v] = want[v] + part
+    assert np.array_equal(_update(delta, idx, "i32", 6, 1.0), want)
+    old = rng.standard_normal((6, 12)).astype(np.float32)
+    assert np.array_equal(_update(delta, idx, "i64", 6, 1.0, onto=old), old + want)
+
+
+@pytest.mark.gpu
 def test_no_tokens():
     empty = np.zeros((0, 6), np.float32)
     assert not _update(empty, [], "f32", 5, 1.0).any()
