@@ -37,7 +37,12 @@ struct Chunk {
     unsigned vec;                       // all addresses allow vectors
 };
 static_assert(sizeof(Chunk) == 64, "records are read as four vectors");
-constexpr size_t kHeader = 256;         // of a plan: the count of CTAs that have finished, then the records
+constexpr size_t kHeader = 256;         // of a plan: Header, then the records
+struct Header {
+    unsigned finished;                  // CTAs of the running step that have come to their end
+    int state_bits;
+    long long chunks;
+};
 
 struct Rates {
     float b1, c1, b2, c2, eps;
@@ -88,12 +93,17 @@ __device__ __forceinline__ float update(const Rates& r, const Now& now, float ke
 }
 
 // The step is counted by the CTA that finishes last: every other one has read the count by then.
-__device__ __forceinline__ void end_step(unsigned* finished, float* step, float before) {
-    if (threadIdx.x == 0 && atomicInc(finished, gridDim.x - 1) == gridDim.x - 1) *step = before + 1.0f;
+__device__ __forceinline__ void end_step(Header* plan, int state_bits, float* step, float before) {
+    if (threadIdx.x == 0 && atomicInc(&plan->finished, gridDim.x - 1) == gridDim.x - 1 && plan->state_bits == state_bits) *step = before + 1.0f;
+}
+
+// Records that a kernel may go through: those of the plan, however many the caller names; none of a plan for other moments.
+__device__ __forceinline__ long long records(const Header* plan, long long named, int state_bits) {
+    return plan->state_bits == state_bits ? min(named, plan->chunks) : 0;
 }
 
 __global__ void __launch_bounds__(kThreads)
-adamw32_kernel(unsigned* finished, const Chunk* __restrict__ chunks, long long n_chunks, Rates r, const float* lr_at, const float* scale_at, float* step,
+adamw32_kernel(Header* plan, const Chunk* __restrict__ chunks, long long named, Rates r, const float* lr_at, const float* scale_at, float* step,
                unsigned seed) {
     __shared__ Now shared_now;
     after_earlier_kernels();
@@ -101,6 +111,7 @@ adamw32_kernel(unsigned* finished, const Chunk* __restrict__ chunks, long long n
     if (threadIdx.x == 0) before = begin_step(r, lr_at, scale_at, step, seed, &shared_now);
     __syncthreads();
     const Now now = shared_now;
+    const long long n_chunks = records(plan, named, 32);
     for (long long k = blockIdx.x; k < n_chunks; k += gridDim.x) {
         const Chunk c = chunks[k];
         float* m = static_cast<float*>(c.m);
@@ -141,7 +152,7 @@ adamw32_kernel(unsigned* finished, const Chunk* __restrict__ chunks, long long n
             v[i] = vi;
         }
     }
-    end_step(finished, step, before);
+    end_step(plan, 32, step, before);
 }
 
 // The byte (without its sign) of one of the two neighbours in e4m3 of q, |q| <= 448 but for a rounding: of the upper one
@@ -215,7 +226,7 @@ __device__ __forceinline__ void scales_of(float top_m, float top_r, float& to_m,
 }
 
 __global__ void __launch_bounds__(kThreads, 4)
-adamw8_kernel(unsigned* finished, const Chunk* __restrict__ chunks, long long n_chunks, Rates r, const float* lr_at, const float* scale_at, float* step,
+adamw8_kernel(Header* plan, const Chunk* __restrict__ chunks, long long named, Rates r, const float* lr_at, const float* scale_at, float* step,
               unsigned seed) {
     __shared__ Now shared_now;
     after_earlier_kernels();
@@ -223,6 +234,7 @@ adamw8_kernel(unsigned* finished, const Chunk* __restrict__ chunks, long long n_
     if (threadIdx.x == 0) before = begin_step(r, lr_at, scale_at, step, seed, &shared_now);
     __syncthreads();
     const Now now = shared_now;
+    const long long n_chunks = records(plan, named, 8);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     for (long long k = blockIdx.x; k < n_chunks; k += gridDim.x) {
         const Chunk c = chunks[k];
@@ -332,7 +344,7 @@ adamw8_kernel(unsigned* finished, const Chunk* __restrict__ chunks, long long n_
             }
         }
     }
-    end_step(finished, step, before);
+    end_step(plan, 8, step, before);
 }
 
 int count_chunks(const b2_adamw_tensor* list, int count, int state_bits, long long* chunks) {
@@ -380,6 +392,7 @@ extern "C" int b2_adamw_plan(const b2_adamw_tensor* tensors, int32_t count, int3
     B2_REQUIRE(capturing == cudaStreamCaptureStatusNone, "a plan is made before its stream is captured");
     try {
         std::vector<char> host(kHeader + (size_t)chunks * sizeof(Chunk), 0);
+        *reinterpret_cast<Header*>(host.data()) = {0, state_bits, (long long)chunks};
         Chunk* c = reinterpret_cast<Chunk*>(host.data() + kHeader);
         for (int i = 0; i < count; ++i) {
             const b2_adamw_tensor& t = tensors[i];
@@ -431,6 +444,6 @@ extern "C" int b2_adamw_step(void* plan, int64_t chunks, int32_t state_bits, con
     long long blocks = chunks < 1 ? 1 : chunks;
     if (blocks > b2::kSms * 8) blocks = b2::kSms * 8;
     B2_CUDA(b2::launch_after(state_bits == 32 ? adamw32_kernel : adamw8_kernel, dim3((unsigned)blocks), kThreads, 0, (cudaStream_t)stream,
-                             reinterpret_cast<unsigned*>(base), reinterpret_cast<const Chunk*>(base + kHeader), (long long)chunks, r, lr, grad_scale, step, seed));
+                             reinterpret_cast<Header*>(base), reinterpret_cast<const Chunk*>(base + kHeader), (long long)chunks, r, lr, grad_scale, step, seed));
     return B2_OK;
 }

@@ -176,8 +176,8 @@ __device__ __forceinline__ void put_row(float* row, int i0, int F, const float (
         }
 }
 
-__device__ __forceinline__ void fetch_ahead(const float* p, int n) {
-    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p), "r"(n * 4) : "memory");
+__device__ __forceinline__ void fetch_ahead(const float* p, int bytes) {
+    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p), "r"(bytes) : "memory");
 }
 
 // A row to a CTA, held in registers: each tensor is read once.  Both operands are on their way before the first sum.
@@ -213,8 +213,9 @@ norm_row_kernel(const b2_norm a) {
         if (RAGGED && threadIdx.x == 0 && row + gridDim.x < a.rows) {
             // the next row on its way to the second cache
             const long long next = row + gridDim.x;
-            fetch_ahead(a.residual + next * a.residual_stride - shift, width);
-            if (U) fetch_ahead(a.block + next * a.block_stride - shift, width);
+            const int bytes = (shift + F + 3) / 4 * 16;         // (whole vectors, the last with the row's last value)
+            fetch_ahead(a.residual + next * a.residual_stride - shift, bytes);
+            if (U) fetch_ahead(a.block + next * a.block_stride - shift, bytes);
         }
         if constexpr (U) {
             float rho = 1.0f;

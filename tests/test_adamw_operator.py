@@ -110,6 +110,43 @@ def test_steps(bits, sizes, offset):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("offset", [0, 1])
+def test_nothing_beside_the_tensors_is_touched(bits, offset):
+    """Tensors in the midst of marked memory, whose lengths end blocks, words and chunks early."""
+    import torch
+    m = _Model([5, 255, 2051, 1], bits, offset=offset, before=4)
+    around = []
+    for p, state in m.dev:
+        for t in [p] + list(state):
+            whole = torch.as_strided(t, (offset + t.numel() + 8,), (1,), t.storage_offset() - offset)
+            whole[:offset], whole[offset + t.numel():] = 77, 77
+            around.append((whole, t.numel()))
+    m.launch()
+    m.expect()
+    m.check()
+    for whole, n in around:
+        assert bool((whole[:offset] == 77).all()) and bool((whole[offset + n:] == 77).all())
+
+
+@pytest.mark.gpu
+def test_a_plan_for_other_moments_or_fewer_records():
+    """What a plan does not hold is not gone through."""
+    import ctypes
+    import torch
+    from ngraph_python_b200 import lib
+    m = _Model([3000], 32, before=1)
+    before = m.dev[0][0].clone()
+    h = lib.AdamwHyper(*HYPER)
+    lib.check(lib.raw().b2_adamw_step(m.plan.data_ptr(), m.chunks, 8, ctypes.byref(h), None, None, m.step_dev.data_ptr(), 0, 0))
+    torch.cuda.synchronize()
+    assert torch.equal(m.dev[0][0], before) and float(m.step_dev) == 1
+    lib.check(lib.raw().b2_adamw_step(m.plan.data_ptr(), m.chunks + 1000, 32, ctypes.byref(h), None, None, m.step_dev.data_ptr(), m.seed, 0))
+    m.expect()
+    m.check()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [32, 8])
 def test_from_the_first_step_on(bits):
     """All zeros is the state before the first step; a gradient of zeros leaves it so."""
     m = _Model([300, 5000], bits, zero=True)
