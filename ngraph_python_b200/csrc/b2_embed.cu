@@ -3,7 +3,8 @@
 //   forward   out[t, :] = scale * table[token[t], :]
 //   gradient  dW[v, :] = scale * sum of delta[t, :] over the t with token[t] = v, t ascending
 //
-// Both are bound by memory: one multiplication or addition a value.  The gradient is two launches.  The first
+// Both are bound by memory: one multiplication or addition a value (16384 x 1024 looked up: 17.8 us, 0.77 of the rate of a
+// copy; 8192 x 1024 added into 32000 rows: 36 us, of which the sort takes 7 and 18 are zeros).  The gradient is two launches.  The first
 // sorts: a CTA owns the rows v = b (mod CTAs), so that the frequent tokens of a vocabulary, which lie next to one
 // another, go to different CTAs; it reads every token, counts its own per warp, and writes their positions row by
 // row in ascending order.  No counter is shared between CTAs -- where a CTA's positions begin is the number of tokens

@@ -5,6 +5,9 @@
 //   d_stream' = d_stream + through(d_out, stream, w_pre),  d_residual = a d_stream',  d_gate = d_stream' * rms(block) w_post
 //   d_block   = through(gate * d_stream', block, w_post)
 //   through(d, x, w) = rstd (w d - x^ mean(w d x^)),  x^ = x rstd;   d_w = sum over rows of d x^
+//
+// Bound by memory: four tensors of rows forward, six for the gradients, each read or written once.  8192 x 4096: 86 us
+// forward, 0.96 of the rate of a copy, 134 us for the gradients, 0.92.  One row of 2048: 2.3 us in a graph.
 #include <cstdint>
 
 #include "b2_operators.h"
