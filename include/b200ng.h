@@ -567,7 +567,8 @@ int b2_lut_update(const void* delta, const void* idx, void* dW, int32_t flex, in
  * (above), batch normalisation and optimizers they stand beside.  Results must lie on the current
  * device; a launch goes to `stream` of that device.
  * ------------------------------------------------------------------------------------------ */
-/* how tokens are held: fp32, int32, int64, or flex16 mantissas with the exponent of slot_idx */
+/* how tokens are held: fp32 (which names every row up to 2^24), int32, int64, or flex16 mantissas with the exponent
+ * of slot_idx */
 #define B2_IDX_F32 0
 #define B2_IDX_I32 1
 #define B2_IDX_I64 2

@@ -36,7 +36,7 @@ __device__ __forceinline__ void put(float* p, const float* v) {
 // values that a pointer is behind a 16-byte boundary
 __device__ __host__ __forceinline__ int shift_of(const float* p) { return (int)((reinterpret_cast<uintptr_t>(p) >> 2) & 3); }
 
-// Sums of two values over the CTA, the same bits in every thread.  One barrier: calls write to two sets of words by
+// Sums of up to two values over the CTA, the same bits in every thread.  One barrier: calls write to two sets of words by
 // turns, and who comes to write to a set again has passed the barrier behind which everybody had read it.
 struct TwoSums {
     float words[2][2][32];
@@ -186,13 +186,13 @@ __device__ __forceinline__ void fetch_ahead(const float* p, int bytes) {
 // A row to a CTA, held in registers: each tensor is read once.  Both operands are on their way before the first sum.
 // Ragged rows: a CTA's are a multiple of four apart and so lie alike, and it keeps the weights in shared memory as they
 // lie beside them.
-template <int VEC, int IT, bool RAGGED, bool U, bool POST, int GATE>
+template <int IT, bool RAGGED, bool U, bool POST, int GATE>
 __global__ void __launch_bounds__(1024)
 norm_row_kernel(const b2_norm a) {
     extern __shared__ __align__(16) float staged[];         // ragged: post_weight, a gate per feature, pre_weight
     __shared__ TwoSums sums;
     after_earlier_kernels();
-    constexpr int di = 32 * VEC;
+    constexpr int VEC = 4, di = 32 * VEC;
     const int F = a.features, width = (F + 6) / 4 * 4;
     const int shift = RAGGED ? shift_of(a.residual + blockIdx.x * a.residual_stride) : 0, i0 = first_of<VEC, IT>() - shift;
     if (RAGGED) {
@@ -279,7 +279,7 @@ norm_row_kernel(const b2_norm a) {
 // place is free again behind the first of them, the others behind the second.  Ragged rows: a CTA's are a multiple of four
 // apart and so lie alike; a copy starts at the 16-byte boundary below the row, and a thread's columns, whose sums it keeps,
 // are the vectors of memory.  (Value by value 3000 x 5001 took 83 us.)  A wait that runs out turns the results into NaN.
-constexpr int kStages = 4;
+constexpr int kStages = 3;
 
 struct Ring {
     int stages, slot;                   // bytes of one tensor's row, with room for its alignment
@@ -653,7 +653,7 @@ GradPlan grad_plan(const b2_norm& a, int tensors, bool ragged) {
     p.ring.slot = (a.features + 3 + 3) / 4 * 16;
     const int room = (int)((220 << 10) / per_sm) - 1024;
     p.ring.stages = room / (p.ring.slot * tensors);
-    if (p.ring.stages > 3) p.ring.stages = 3;
+    if (p.ring.stages > kStages) p.ring.stages = kStages;
     if (p.ring.stages < 1) p.threads = 0;
     return p;
 }
@@ -674,7 +674,7 @@ int check_stride(const b2_norm* a, const void* p, int64_t stride, const char* wh
 
 bool rows_aligned(const void* p, int64_t stride) { return b2::aligned16(p) && stride % 4 == 0; }
 
-template <int VEC, int IT, bool RAGGED>
+template <int IT, bool RAGGED>
 int launch_rows(const b2_norm& a, int threads, cudaStream_t st) {
     // (148 and so every multiple of it is a multiple of four)
     const long long most = RAGGED ? (long long)b2::kSms * (threads > 512 ? 1 : 1024 / threads > 16 ? 16 : 1024 / threads) : 1ll << 30;
@@ -683,8 +683,8 @@ int launch_rows(const b2_norm& a, int threads, cudaStream_t st) {
 #define B2_LAUNCH(U, POST, GATE)                                                                                                       \
     do {                                                                                                                              \
         static std::atomic<unsigned long long> done{0};                                                                               \
-        if (room > 48 << 10) B2_CHECK(b2::allow_shared((const void*)norm_row_kernel<VEC, IT, RAGGED, U, POST, GATE>, 220 << 10, &done)); \
-        B2_CUDA((b2::launch_after(norm_row_kernel<VEC, IT, RAGGED, U, POST, GATE>, dim3(blocks), threads, room, st, a)));              \
+        if (room > 48 << 10) B2_CHECK(b2::allow_shared((const void*)norm_row_kernel<IT, RAGGED, U, POST, GATE>, 220 << 10, &done)); \
+        B2_CUDA((b2::launch_after(norm_row_kernel<IT, RAGGED, U, POST, GATE>, dim3(blocks), threads, room, st, a)));              \
     } while (0)
 #define B2_GATED(POST)                                                        \
     switch (a.gate_kind) {                                                    \
@@ -757,16 +757,16 @@ extern "C" int b2_norm_fprop(const b2_norm* a, void* stream) {
     // 2048 features on, so that several rows share an SM and the sums over the CTA weigh less (8192 x 4096: 100 us
     // with eight, 85 with sixteen; 16384 x 512: 25 and 27).
     const bool few = a->rows <= b2::kSms * 2, wide = F >= 2048;
-#define B2_ROWS(VEC, IT, RAGGED) \
-    if (const int t = threads_of(F + (RAGGED ? 3 : 0), VEC * IT, 1024)) return launch_rows<VEC, IT, RAGGED>(*a, t, st);
+#define B2_ROWS(IT, RAGGED) \
+    if (const int t = threads_of(F + (RAGGED ? 3 : 0), 4 * IT, 1024)) return launch_rows<IT, RAGGED>(*a, t, st);
     if (vec) {
-        if (few) B2_ROWS(4, 1, false)
-        if (!wide) B2_ROWS(4, 2, false)
-        B2_ROWS(4, 4, false)
+        if (few) B2_ROWS(1, false)
+        if (!wide) B2_ROWS(2, false)
+        B2_ROWS(4, false)
     } else if (ragged) {
-        if (few) B2_ROWS(4, 1, true)
-        if (!wide) B2_ROWS(4, 2, true)
-        B2_ROWS(4, 4, true)
+        if (few) B2_ROWS(1, true)
+        if (!wide) B2_ROWS(2, true)
+        B2_ROWS(4, true)
     }
 #undef B2_ROWS
     B2_CUDA(b2::launch_after(vec ? norm_any_kernel<4> : norm_any_kernel<1>, dim3(blocks), kThreads, 0, st, *a));

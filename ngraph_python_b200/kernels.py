@@ -977,6 +977,13 @@ def rows_of(view, axes, apart):
     return rows[0], features[0], rows[1] if rows[0] > 1 else features[0]
 
 
+def _check_index(op, t, rows):
+    """An index names whole numbers that its tensor can hold."""
+    most = 1 << (15 if t.flex else 24)
+    if rows > most:
+        raise ValueError("Unhandled op: {}: a {} index names at most {} rows".format(op, "flex16" if t.flex else "fp32", most))
+
+
 class EmbedStep(_Step):
     """A table lookup with a scale."""
     kind = "embed"
@@ -990,6 +997,7 @@ class EmbedStep(_Step):
         self.V, self.F = op.args[0].axes.lengths
         self.n = op.args[1].axes.size
         self.flex = t.flex
+        _check_index(op, t, self.V)
 
     def launch(self, t):
         wv, xv = self.in_views
@@ -1025,6 +1033,7 @@ class EmbedGradStep(_Step):
         self.pad_idx = -1 if pad is None else pad
         self.scratch_bytes = lib.embed_update_scratch_bytes(self.V, self.F, self.n)
         self.flex = t.flex
+        _check_index(op, t, self.V)
 
     def launch(self, t):
         dv, xv = self.in_views

@@ -61,6 +61,16 @@ def test_flex_transformers_refuse_norms_and_adamw():
             t.initialize()
 
 
+@pytest.mark.parametrize("flex,rows", [(True, 32769), (False, (1 << 24) + 1)])
+def test_an_index_that_cannot_name_every_row_is_refused(flex, rows):
+    V, F, T = _axes(V=rows, F=1, T=2)
+    idx = ng.placeholder([T])
+    t = _transformer(flex=flex, plan_only=True)
+    t.computation(ng.embedding(ng.placeholder([V, F]), idx), idx)
+    with pytest.raises(ValueError, match="at most"):
+        t.initialize()
+
+
 def test_steps_of_a_plan():
     """One step each, and no copy of operands that lie as they should -- rows of a wider tensor among them."""
     V, F, T = _axes(V=50, F=8, T=16)
