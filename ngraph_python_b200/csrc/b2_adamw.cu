@@ -6,8 +6,9 @@
 // Bound by memory: 28 bytes a value with fp32 moments, 16.06 with moments in 8 bits.  The tensors are cut into chunks
 // of 2048 values, one 64-byte record each, made once (the addresses of a program's tensors stay): a CTA reads a
 // record and its values, whatever tensor they belong to, so that many small tensors cost no launches.  79.5 million values:
-// 345 us with fp32 moments, 0.99 of the rate of a copy; 284 us with 8-bit ones, 0.69 of it and 88 instructions a value, of
-// which division and square root, correctly rounded, are a fifth.  162 000 values: 3.7 us in a graph.
+// 345 us with fp32 moments, 0.99 of the rate of a copy; 252 us with 8-bit ones, 0.78 of it, by issue (some 84 instructions a
+// value, of which division and square root, correctly rounded, are a fifth), and 284 where the power cap has lowered the
+// clock to 1.7 GHz.  162 000 values: 3.7 us in a graph.
 //
 // Moments in 8 bits: a warp holds 256 values and their two scales.  m and sqrt(v) are e4m3 values times the block's
 // largest / 448.  v itself spans the square of what its root does, and e4m3 covers 2.3e5 : 1.  An average with
@@ -79,7 +80,8 @@ __device__ __forceinline__ float begin_step(const Rates& r, const float* lr_at, 
     now->root = (float)(1.0 / sqrt(1.0 - power(r.beta2, t)));
     now->lr_wd = (float)(lr * r.wd);
     now->grad_scale = scale_at ? *scale_at : 1.0f;
-    now->key = mix(seed + 0x9E3779B9u * t);
+    const unsigned key = mix(seed + 0x9E3779B9u * t);
+    now->key = key ^ (key >> 16);               // (as the first step of mix() leaves it)
     return before;
 }
 
@@ -157,12 +159,17 @@ adamw32_kernel(Header* plan, const Chunk* __restrict__ chunks, long long named, 
     end_step(plan, 32, step, before);
 }
 
-// The byte (without its sign) of one of the two neighbours in e4m3 of q, |q| <= 448 but for a rounding: of the upper one
-// with the chance that sixteen random bits give it.  Times 2^-120, exponent and mantissa of an fp32 value have in their
-// upper bits the byte of e4m3, fp32's denormals that of e4m3's, which are 2^-9 apart; what is below these bits is added
-// to and cut off.  (No carry beyond 448: the random bits end above the roundings of q.)
+// The byte (without its sign) of one of the two neighbours in e4m3 of q, |q| <= 448 but for a rounding, in the uppermost byte:
+// of the upper neighbour with the chance that sixteen random bits give it, here in the middle two bytes.  Times 2^-120,
+// exponent and mantissa of an fp32 value have in bits 20 to 27 the byte of e4m3, fp32's denormals that of e4m3's, which
+// are 2^-9 apart; what is below is added to and cut off.  (No carry beyond 448: the random bits end above the roundings
+// of q.)
 __device__ __forceinline__ unsigned to_e4m3(float q, unsigned bits) {
-    return (__float_as_uint(__fmul_rn(fabsf(q), 7.52316384526264e-37f)) + (bits << 4)) >> 20;
+    return (__float_as_uint(__fmul_rn(fabsf(q), 7.52316384526264e-37f)) << 4) + bits;
+}
+// the uppermost bytes of four words
+__device__ __forceinline__ unsigned tops(unsigned a, unsigned b, unsigned c, unsigned d) {
+    return __byte_perm(__byte_perm(a, b, 0x0073), __byte_perm(c, d, 0x0073), 0x5410);
 }
 
 // Two products to an instruction.  Sums are taken one by one: the assembler joins a product and a sum of this form into one
@@ -313,7 +320,7 @@ adamw8_kernel(Header* plan, const Chunk* __restrict__ chunks, long long named, R
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const int i = h * 128 + lane * 4;
-            unsigned mb[4], vb[4];
+            unsigned mb[4], vb[4], qm_bits[4];
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
                 float qm[2], qr[2];
@@ -321,13 +328,19 @@ adamw8_kernel(Header* plan, const Chunk* __restrict__ chunks, long long named, R
                 apart(two(root[4 * h + 2 * k], root[4 * h + 2 * k + 1]) * two(to_r, to_r), qr[0], qr[1]);
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
-                    const unsigned bits = mix((c.counter + (unsigned)(at + i + 2 * k + j)) ^ now.key);
-                    mb[2 * k + j] = to_e4m3(qm[j], bits & 0xffffu) | (__float_as_uint(qm[j]) >> 24 & 0x80u);
-                    vb[2 * k + j] = max(to_e4m3(qr[j], bits >> 16), min(__float_as_uint(qr[j]), 1u));
+                    // mix() of position and key, the first and the last of its steps put together with what is next to them:
+                    // its upper half rounds the root, its lower half the average
+                    const unsigned at_e = c.counter + (unsigned)(at + i + 2 * k + j);
+                    unsigned y = (at_e ^ (at_e >> 16) ^ now.key) * 0x9E3779B9u;
+                    y = (y ^ (y >> 15)) * 0xBB67AE85u;
+                    qm_bits[2 * k + j] = __float_as_uint(qm[j]);
+                    mb[2 * k + j] = to_e4m3(qm[j], __byte_perm(y ^ (y >> 16), 0u, 0x4104));
+                    vb[2 * k + j] = max(to_e4m3(qr[j], __byte_perm(y, 0u, 0x4324)), min(__float_as_uint(qr[j]), 1u) << 24);
                 }
             }
-            const unsigned mo = __byte_perm(__byte_perm(mb[0], mb[1], 0x0040), __byte_perm(mb[2], mb[3], 0x0040), 0x5410);
-            const unsigned vo = __byte_perm(__byte_perm(vb[0], vb[1], 0x0040), __byte_perm(vb[2], vb[3], 0x0040), 0x5410);
+            const unsigned mo = (tops(mb[0], mb[1], mb[2], mb[3]) & 0x7f7f7f7fu) |
+                                (tops(qm_bits[0], qm_bits[1], qm_bits[2], qm_bits[3]) & 0x80808080u);
+            const unsigned vo = tops(vb[0], vb[1], vb[2], vb[3]);
             float x[4];
             apart(p[2 * h], x[0], x[1]);
             apart(p[2 * h + 1], x[2], x[3]);
