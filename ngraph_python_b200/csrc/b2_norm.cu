@@ -683,7 +683,7 @@ int launch_rows(const b2_norm& a, int threads, cudaStream_t st) {
 #define B2_LAUNCH(U, POST, GATE)                                                                                                       \
     do {                                                                                                                              \
         static std::atomic<unsigned long long> done{0};                                                                               \
-        if (room > 48 << 10) B2_CHECK(b2::allow_shared((const void*)norm_row_kernel<IT, RAGGED, U, POST, GATE>, 220 << 10, &done)); \
+        if (room > 40 << 10) B2_CHECK(b2::allow_shared((const void*)norm_row_kernel<IT, RAGGED, U, POST, GATE>, 220 << 10, &done)); \
         B2_CUDA((b2::launch_after(norm_row_kernel<IT, RAGGED, U, POST, GATE>, dim3(blocks), threads, room, st, a)));              \
     } while (0)
 #define B2_GATED(POST)                                                        \

@@ -199,6 +199,20 @@ def test_many_ragged_rows(rows, F, pad, gate):
     _check_backward(_backward(c, gate, x, rstd, rho, *d), c, x, rstd, rho, *d)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("F", [3407, 4053, 4091, 4093, 4095, 4097, 8189, 8190, 8191, 8193, 16381, 16382, 16383])
+def test_ragged_rows_around_the_limits_of_shared_memory(F):
+    for rows in (2, 400):
+        c = _case(rows, F, "feature")
+        got, _ = _forward(c, "feature")
+        _check_forward(got, c, F)
+    if F < 9000:
+        rng = np.random.RandomState(9)
+        x, rstd, rho = _stored(c)
+        d = [rng.standard_normal((rows, F)).astype(np.float32) for _ in range(2)]
+        _check_backward(_backward(c, "feature", x, rstd, rho, *d), c, x, rstd, rho, *d)
+
+
 def _forward_alike(c, gate, pad):
     """All rows `pad` apart."""
     import torch
