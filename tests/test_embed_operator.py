@@ -295,6 +295,29 @@ def test_recorded_and_replayed_on_another_stream():
 
 
 @pytest.mark.gpu
+def test_two_streams_at_once():
+    """Calls on two streams with a scratch each, beside one another, many times over."""
+    import torch
+    from ngraph_python_b200 import lib
+    g = torch.Generator(device="cuda")
+    g.manual_seed(2)
+    jobs = []
+    for V, F, n in ((700, 64, 5000), (3000, 33, 9000)):
+        idx = torch.randint(0, V, (n,), device="cuda", generator=g)
+        delta = torch.randint(-8, 9, (n, F), device="cuda", generator=g).float()
+        nbytes = lib.embed_update_scratch_bytes(V, F, n)
+        jobs.append((V, F, n, idx, delta, torch.empty((V, F), device="cuda"), torch.empty((nbytes,), dtype=torch.uint8, device="cuda"), torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    for _ in range(50):
+        for V, F, n, idx, delta, out, scratch, stream in jobs:
+            lib.check(lib.raw().b2_embed_update(delta.data_ptr(), idx.data_ptr(), out.data_ptr(), 0, 2, V, F, n, 1.0, -1, 0, *PLAIN, scratch.data_ptr(),
+                                                scratch.numel(), stream.cuda_stream))
+    torch.cuda.synchronize()
+    for V, F, n, idx, delta, out, _, _ in jobs:
+        assert torch.equal(out, torch.zeros_like(out).index_add_(0, idx, delta))
+
+
+@pytest.mark.gpu
 def test_large_offsets():
     """A table of more than 2^31 values, its last rows."""
     import torch
