@@ -911,6 +911,8 @@ extern "C" int b2_embed_fprop(const void* table, const void* idx, void* out, int
     if (n_idx == 0) return B2_OK;
     B2_REQUIRE(table && idx && out, "bad lookup: missing tensor");
     B2_CHECK(b2::require_here(out, "the lookup's result"));
+    B2_CHECK(b2::require_read(table, "the table"));
+    B2_CHECK(b2::require_read(idx, "the index"));
     cudaStream_t st = (cudaStream_t)stream;
 #define B2_KIND(T)                                                                                                          \
     switch (idx_kind) {                                                                                                     \
@@ -941,6 +943,9 @@ extern "C" int b2_embed_update(const void* delta, const void* idx, void* dW, int
     B2_REQUIRE(dW && (n_idx == 0 || (delta && idx)), "bad lookup gradient: missing tensor");
     B2_REQUIRE(scratch && scratch_bytes >= need, "the lookup's gradient needs %zu bytes of scratch, got %zu", need, scratch_bytes);
     B2_CHECK(b2::require_here(dW, "the table's gradient"));
+    B2_CHECK(b2::require_here(scratch, "the scratch"));
+    B2_CHECK(b2::require_read(n_idx ? delta : nullptr, "delta"));
+    B2_CHECK(b2::require_read(n_idx ? idx : nullptr, "the index"));
     const int pad = pad_idx >= 0 && pad_idx < V ? (int)pad_idx : -1;
     void* at = (void*)(((uintptr_t)scratch + 255) / 256 * 256);
     if (flex) return launch_update<short>(delta, idx, dW, idx_kind, V, F, n_idx, scale, pad, onto, f, at, (cudaStream_t)stream);

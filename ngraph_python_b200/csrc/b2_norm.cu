@@ -739,7 +739,11 @@ extern "C" int b2_norm_fprop(const b2_norm* a, void* stream) {
     B2_CHECK(check_stride(a, a->stream, a->stream_stride, "stream"));
     B2_CHECK(check_stride(a, a->out, a->out_stride, "result"));
     if (a->gate_kind == B2_GATE_FULL) B2_CHECK(check_stride(a, a->gate, a->gate_stride, "gate"));
-    B2_CHECK(b2::require_here(a->out ? a->out : a->stream, "the norm's result"));
+    if (a->out) B2_CHECK(b2::require_here(a->out, "the norm's result"));
+    if (a->stream) B2_CHECK(b2::require_here(a->stream, "the stream"));
+    B2_CHECK(b2::require_read(a->residual, "the residual"));
+    B2_CHECK(b2::require_read(a->block, "the block"));
+    B2_CHECK(b2::require_read(a->gate, "the gate"));
     const unsigned blocks = (unsigned)(a->rows < (1ll << 30) ? a->rows : (1ll << 30));
     const int F = a->features;
     cudaStream_t st = (cudaStream_t)stream;
@@ -805,6 +809,13 @@ extern "C" int b2_norm_bprop(const b2_norm* a, const b2_norm_grads* d, void* scr
         if (a->gate_kind == B2_GATE_FULL) B2_CHECK(check_stride(a, d->d_gate, d->d_gate_stride, "gate's gradient"));
     }
     B2_CHECK(b2::require_here(scratch, "the norm's scratch"));
+    if (a->rows > 0) {
+        const void* written[] = {d->d_residual, d->d_block, d->d_gate, d->d_pre_weight, d->d_post_weight};
+        for (const void* p : written)
+            if (p) B2_CHECK(b2::require_here(p, "a gradient of the norm"));
+        const void* read[] = {a->block ? a->stream : a->residual, a->block, a->gate, d->d_out, d->d_stream};
+        for (const void* p : read) B2_CHECK(b2::require_read(p, "an operand of the norm's gradient"));
+    }
     cudaStream_t st = (cudaStream_t)stream;
     float* sums = (float*)(((uintptr_t)scratch + 255) / 256 * 256);
     float* gate = a->gate_kind == B2_GATE_FEATURE ? d->d_gate : nullptr;

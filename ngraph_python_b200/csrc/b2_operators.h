@@ -22,6 +22,19 @@ inline int require_here(const void* out, const char* what) {
     return B2_OK;
 }
 
+// The same of an operand, which may also lie in page-locked host memory.  (50 ns.)
+inline int require_read(const void* in, const char* what) {
+    if (!in) return B2_OK;
+    cudaPointerAttributes a;
+    B2_CUDA(cudaPointerGetAttributes(&a, in));
+    B2_REQUIRE(a.type != cudaMemoryTypeUnregistered, "%s is not memory that the device reads", what);
+    if (a.type != cudaMemoryTypeDevice) return B2_OK;
+    int now = 0;
+    B2_CUDA(cudaGetDevice(&now));
+    B2_REQUIRE(a.device == now, "%s lies on device %d, the current device is %d", what, a.device, now);
+    return B2_OK;
+}
+
 // More than 48 KB of dynamic shared memory is asked for once per kernel and device.
 inline int allow_shared(const void* kernel, int bytes, std::atomic<unsigned long long>* done) {
     int now = 0;

@@ -369,3 +369,17 @@ def test_host_memory_is_refused():
     out = torch.zeros((2, 4))
     with pytest.raises(lib.B200Error, match="device memory"):
         lib.check(lib.raw().b2_embed_fprop(table.data_ptr(), idx.data_ptr(), out.data_ptr(), 0, 0, 4, 4, 2, 1.0, *PLAIN, 0))
+    there = torch.zeros((2, 4), device="cuda")
+    for t, x in ((table.cpu(), idx), (table, idx.cpu())):
+        with pytest.raises(lib.B200Error, match="not memory that the device reads"):
+            lib.check(lib.raw().b2_embed_fprop(t.data_ptr(), x.data_ptr(), there.data_ptr(), 0, 0, 4, 4, 2, 1.0, *PLAIN, 0))
+    nbytes = lib.embed_update_scratch_bytes(4, 4, 2)
+    scratch = torch.zeros((nbytes,), dtype=torch.uint8, device="cuda")
+    for d, x, s in ((there.cpu(), idx, scratch), (there, idx.cpu(), scratch), (there, idx, scratch.cpu())):
+        with pytest.raises(lib.B200Error, match="memory"):
+            lib.check(lib.raw().b2_embed_update(d.data_ptr(), x.data_ptr(), table.data_ptr(), 0, 0, 4, 4, 2, 1.0, -1, 0, *PLAIN, s.data_ptr(), nbytes, 0))
+    # page-locked memory is read
+    pinned = torch.arange(16, dtype=torch.float32).view(4, 4).pin_memory()
+    lib.check(lib.raw().b2_embed_fprop(pinned.data_ptr(), idx.data_ptr(), there.data_ptr(), 0, 0, 4, 4, 2, 1.0, *PLAIN, 0))
+    torch.cuda.synchronize()
+    assert torch.equal(there.cpu(), pinned[:1].expand(2, 4))

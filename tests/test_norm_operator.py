@@ -480,3 +480,35 @@ def test_refusals():
     for scratch, nbytes in ((None, 1 << 24), (256, 8)):
         with pytest.raises(lib.B200Error, match="error -1"):
             lib.check(raw.b2_norm_bprop(ctypes.byref(a), ctypes.byref(d), scratch, nbytes, 0))
+
+
+@pytest.mark.gpu
+def test_host_memory_is_refused():
+    import torch
+    from ngraph_python_b200 import lib
+    rows, F = 3, 8
+    host = np.ones((rows, F), np.float32)
+    c = _case(rows, F, "full")
+    _, (a, mem, vecs) = _forward(c, "full")
+    for name in ("residual", "block", "gate", "stream", "out"):
+        held = getattr(a, name)
+        setattr(a, name, host.ctypes.data)
+        with pytest.raises(lib.B200Error, match="memory"):
+            lib.check(lib.raw().b2_norm_fprop(ctypes.byref(a), 0))
+        setattr(a, name, held)
+    t = {k: torch.ones((rows, F), device="cuda") for k in ("d_out", "d_stream", "d_residual", "d_block", "d_gate")}
+    d = lib.NormGrads()
+    for k, v in t.items():
+        setattr(d, k, v.data_ptr())
+        setattr(d, k + "_stride", F)
+    nbytes = lib.norm_bprop_scratch_bytes(a)
+    scratch = torch.zeros((max(nbytes, 256),), dtype=torch.uint8, device="cuda")
+    for name in t:
+        held = getattr(d, name)
+        setattr(d, name, host.ctypes.data)
+        with pytest.raises(lib.B200Error, match="memory"):
+            lib.check(lib.raw().b2_norm_bprop(ctypes.byref(a), ctypes.byref(d), scratch.data_ptr(), scratch.numel(), 0))
+        setattr(d, name, held)
+    lib.check(lib.raw().b2_norm_bprop(ctypes.byref(a), ctypes.byref(d), scratch.data_ptr(), scratch.numel(), 0))
+    torch.cuda.synchronize()
+    assert (host == 1).all()
