@@ -1141,9 +1141,9 @@ class AdamwStep(_Fp32Step):
     kind = "adamw"
     launches = 1
 
-    def __init__(self, index, op, t):
+    def __init__(self, index, op, t, written):
         super(AdamwStep, self).__init__(index, op, t)
-        self.out_views = [t._view_of(x) for x in op.written()]
+        self.out_views = written
         self.gradients = [t._view_of(g) for g in op.gradients]
         self.numbers = [None if x is None or isinstance(x, float) else t._view_of(x) for x in (op.lr, op.grad_scale)]
         self.scale = None              # a tensor of a grad_scale that is a number

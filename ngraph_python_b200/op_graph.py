@@ -974,7 +974,8 @@ class AdamWOp(Op):
         super(AdamWOp, self).__init__(args + [x for x in (self.lr, self.grad_scale) if isinstance(x, Op)], self.count.axes, **kw)
 
     def layouts(self):
-        return [(g, v.axes, 0) for v, g in zip(self.variables, self.gradients)]
+        return [(g, v.axes, 0) for v, g in zip(self.variables, self.gradients)] + \
+            [(x, x.axes, 0) for x in (self.lr, self.grad_scale) if isinstance(x, Op)]
 
     def written(self):
         return list(self.variables) + [s for x in self.states for s in x] + [self.count]

@@ -1260,8 +1260,11 @@ class _Planner(object):
                     if not self.t._view_of(a).is_dense():
                         self._densify(a, list(self.t._view_of(a).axes), saved)
             elif hasattr(op, "layouts"):
+                # (what a step over many tensors reads of one that it writes is taken before it: blocks write at any time)
+                written = set(self.t._buffer_of(x) for x in op.written()) if isinstance(op, AdamWOp) else ()
                 for a, axes, apart in op.layouts():
-                    if kernels.rows_of(self.t._view_of(a), axes, apart) is None:
+                    view = self.t._view_of(a)
+                    if view.buffer in written or kernels.rows_of(view, axes, apart) is None:
                         self._densify(a, list(axes), saved)
             step = self._make_other_step(op, tail)
         finally:
@@ -1327,7 +1330,8 @@ class _Planner(object):
         elif isinstance(op, ResidualNormGradOp):
             step = kernels.NormGradStep(index, op, self.t, self.present)
         elif isinstance(op, AdamWOp):
-            step = kernels.AdamwStep(index, op, self.t)
+            # (views of the tensors themselves: a copy may stand for a variable that is a gradient too)
+            step = kernels.AdamwStep(index, op, self.t, [View.dense(self.t._buffer_of(x)) for x in op.written()])
         else:
             raise ValueError("Unhandled op: {}".format(op))
         if tail:

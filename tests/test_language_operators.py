@@ -92,6 +92,23 @@ def test_steps_of_a_plan():
     assert [s.kind for s in comp.steps] == ["dimshuffle", "norm"]
 
 
+def test_gradients_that_are_variables_of_the_step_are_copied_first():
+    """The loss sum(x * y) has the gradients y and x."""
+    A, B = _axes(A=5, B=4)
+    x, y = ng.variable([A, B], initial_value=1), ng.variable([A, B], initial_value=2)
+    r, g = ng.variable([], initial_value=0.1), ng.placeholder([A, B])
+    for op, copies in ((ng.adamw([x, y], [y, x], lr=0.1), 2), (ng.adamw([x, y], [g, x], lr=0.1), 1), (ng.adamw([x], [y], lr=0.1), 0),
+                       (ng.adamw([x], [x], lr=0.1), 1), (ng.adamw([r, x], [ng.tensor_slice(x, [0, 0]), g], lr=r, grad_scale=r), 2)):
+        t = _transformer(plan_only=True)
+        comp = t.computation(op, g)
+        t.initialize()
+        assert [s.kind for s in comp.steps] == ["dimshuffle"] * copies + ["adamw"]
+        step = comp.steps[-1]
+        written = set(t._buffer_of(v) for v in op.written())
+        assert [v.buffer for v in step.out_views] == [t._buffer_of(v) for v in op.written()]
+        assert not any(v is not None and v.buffer in written for v in step.gradients + step.numbers)
+
+
 # ---- on the device -------------------------------------------------------------------------------------
 @pytest.mark.gpu
 @pytest.mark.parametrize("flex", [False, True])
@@ -239,6 +256,35 @@ def test_adamw_steps(bits):
                 for x, v in zip(s, held):
                     t.device_tensor(x)[...] = np.zeros_like(v)
                     t.device_tensor(x)[...] = v
+    t.close()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adamw_of_gradients_that_are_variables(bits):
+    A, B = _axes(A=3000, B=70)
+    rng = np.random.RandomState(4)
+    values = [rng.standard_normal(210000).astype(np.float32) for _ in range(2)]
+    x, y = [ng.variable([A, B], initial_value=v.reshape(3000, 70)) for v in values]
+    r = ng.variable([], initial_value=0.125)
+    step = ng.adamw([x, y, r], [y, x, ng.tensor_slice(x, [1, 2])], lr=r, weight_decay=0.0, state_bits=bits)
+    t = _transformer()
+    comp = t.computation(step)
+    values.append(np.array([0.125], np.float32))
+    state = [(np.zeros(v.size, np.float32),) * 2 if bits == 32 else
+             (np.zeros(v.size, np.uint8),) * 2 + (np.zeros(-(-v.size // 256), np.float32),) * 2 for v in values]
+    for k in range(4):
+        comp()
+        h = (float(values[2][0]), 0.9, 0.999, 1e-8, 0.0)
+        found, at = [], 0
+        for v, g, s in zip(values, (values[1], values[0], values[0][72:73]), state):
+            found.append(ao.step(v, g, s, k + 1, h, 1.0, 1.0, 0, at))
+            at += -(-v.size // 256) * 256
+        values, state = [f[0] for f in found], [f[1] for f in found]
+        for op, v in zip((x, y, r), values):
+            assert np.array_equal(np.asarray(t.device_tensor(op).get(None)).reshape(-1), v)
+        if k == 1:
+            comp.capture()
     t.close()
 
 
