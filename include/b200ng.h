@@ -641,7 +641,8 @@ int b2_norm_bprop(const b2_norm* norm, const b2_norm_grads* grads, void* scratch
  * held without bias.  The random bits are a hash of (seed, t, counter + position).  All zeros is the state before
  * the first step.  A block whose largest moment is not above 2^-100 is held as zeros.
  *   plan:  a table of the work on the device, made once for given addresses (not while a stream is captured);
- *          the tensors must not overlap; n = 0 is allowed.  A step with other state_bits does nothing.
+ *          tensors that overlap are refused, gradients may be shared; n = 0 is allowed.  A step with other state_bits
+ *          does nothing.
  *   step:  lr and grad_scale, where not NULL, point to a device float that replaces hyper->lr, and one that
  *          multiplies every gradient; *step is a device float that holds t - 1 before and t after
  * A plan is for one stream at a time. */

@@ -15,6 +15,7 @@
 // beta2 = 0.999 moves by at most 0.05 % of its root in a step downwards where e4m3's neighbours are 6 to 12 % apart: rounded to
 // nearest it would never come down.  Rounded at random to either neighbour, with the chance that makes the mean
 // right, it does, on the average.  A root that is not zero is not rounded to zero, which would leave m / eps.
+#include <algorithm>
 #include <cmath>
 #include <cstdint>
 #include <new>
@@ -378,6 +379,38 @@ int count_chunks(const b2_adamw_tensor* list, int count, int state_bits, long lo
 
 }  // namespace
 
+// Blocks write in any order: what one writes no other may read or write.
+static int check_apart(const b2_adamw_tensor* tensors, int32_t count, int32_t state_bits) {
+    struct Range {
+        uintptr_t from, to;
+        bool operator<(const Range& o) const { return from < o.from; }
+    };
+    std::vector<Range> written;
+    const auto range = [](const void* p, size_t bytes) { return Range{(uintptr_t)p, (uintptr_t)p + bytes}; };
+    for (int i = 0; i < count; ++i) {
+        const b2_adamw_tensor& t = tensors[i];
+        if (t.n == 0) continue;
+        const size_t values = (size_t)t.n, scales = (values + kBlock - 1) / kBlock * 4, moments = state_bits == 32 ? 4 * values : values;
+        written.push_back(range(t.param, 4 * values));
+        written.push_back(range(t.m, moments));
+        written.push_back(range(t.v, moments));
+        if (state_bits == 8) {
+            written.push_back(range(t.m_scales, scales));
+            written.push_back(range(t.v_scales, scales));
+        }
+    }
+    std::sort(written.begin(), written.end());
+    for (size_t k = 1; k < written.size(); ++k)
+        B2_REQUIRE(written[k - 1].to <= written[k].from, "tensors of the plan overlap");
+    for (int i = 0; i < count; ++i) {
+        if (tensors[i].n == 0) continue;
+        const Range g = range(tensors[i].grad, 4 * (size_t)tensors[i].n);
+        const auto next = std::lower_bound(written.begin(), written.end(), Range{g.to, 0});     // the first that begins behind it
+        B2_REQUIRE(next == written.begin() || (next - 1)->to <= g.from, "gradient %d overlaps a tensor that the step writes", i);
+    }
+    return B2_OK;
+}
+
 extern "C" int b2_adamw_plan_bytes(const b2_adamw_tensor* tensors, int32_t count, int32_t state_bits, size_t* bytes, int64_t* chunks) {
     B2_REQUIRE(bytes && chunks, "bad argument");
     long long n = 0;
@@ -394,6 +427,11 @@ extern "C" int b2_adamw_plan(const b2_adamw_tensor* tensors, int32_t count, int3
     int64_t chunks = 0;
     B2_CHECK(b2_adamw_plan_bytes(tensors, count, state_bits, &need, &chunks));
     B2_REQUIRE(plan && plan_bytes >= need, "the plan needs %zu bytes, got %zu", need, plan_bytes);
+    try {
+        B2_CHECK(check_apart(tensors, count, state_bits));
+    } catch (const std::bad_alloc&) {
+        return b2::fail(B2_ERR_INVALID, "no memory for a plan of %d tensors", count);
+    }
     B2_CHECK(b2::require_here(plan, "the plan"));
     for (int i = 0; i < count; ++i) {
         if (tensors[i].n == 0) continue;
@@ -401,6 +439,10 @@ extern "C" int b2_adamw_plan(const b2_adamw_tensor* tensors, int32_t count, int3
         for (const float* p : ends) B2_CHECK(b2::require_here(p, "a tensor of the plan"));
         B2_CHECK(b2::require_here(tensors[i].m, "a moment of the plan"));
         B2_CHECK(b2::require_here(tensors[i].v, "a moment of the plan"));
+        if (state_bits == 8) {
+            B2_CHECK(b2::require_here(tensors[i].m_scales, "the scales of a moment"));
+            B2_CHECK(b2::require_here(tensors[i].v_scales, "the scales of a moment"));
+        }
     }
     cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
     B2_CUDA(cudaStreamIsCapturing((cudaStream_t)stream, &capturing));

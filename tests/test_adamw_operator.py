@@ -311,6 +311,38 @@ def test_refusals():
             lib.check(raw.b2_adamw_step(a["plan"], a["chunks"], a["bits"], h, None, None, a["step"], 0, 0))
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+def test_tensors_that_overlap_are_refused(bits):
+    """Of two tensors of 600 values one address at a time moves into another range by a byte, or out of it."""
+    from ngraph_python_b200 import lib
+    names = ("param", "grad", "m", "v") + (("m_scales", "v_scales") if bits == 8 else ())
+    size = dict.fromkeys(names, 2400)
+    if bits == 8:
+        size.update(m=600, v=600, m_scales=12, v_scales=12)
+    at, place = 1 << 20, {}
+    for k in range(2):
+        for name in names:
+            place[k, name] = at
+            at += 8192
+    def message(moved, to):
+        t = (lib.AdamwTensor * 3)()
+        for k in range(2):
+            t[k].n = 600
+            for name in names:
+                setattr(t[k], name, to if (k, name) == moved else place[k, name])
+        with pytest.raises(lib.B200Error) as e:      # (addresses of nothing: refused in any case)
+            lib.adamw_plan(t, bits, 256, 1 << 20)
+        return "overlap" in str(e.value)
+    for moved in place:
+        for other in place:
+            if moved == other:
+                continue
+            both_read = moved[1] == other[1] == "grad"
+            for to, overlap in ((place[other], True), (place[other] + size[other[1]] - 1, True), (place[other] + size[other[1]], False),
+                                (place[other] - size[moved[1]] + 1, True), (place[other] - size[moved[1]], False)):
+                assert message(moved, to) == (overlap and not both_read), (moved, other, to - place[other])
+
+
 @pytest.mark.gpu
 def test_a_plan_is_not_made_in_a_recording():
     import torch
