@@ -566,6 +566,7 @@ int b2_lut_update(const void* delta, const void* idx, void* dW, int32_t flex, in
  * Operators of a language model's training step.  No counterpart in the reference, whose lookup table
  * (above), batch normalisation and optimizers they stand beside.  Results and large operands must lie on the
  * current device (operands also in page-locked host memory), which is checked; a launch goes to `stream` of that device.
+ * Results have memory of their own except where an operator says otherwise.
  * ------------------------------------------------------------------------------------------ */
 /* how tokens are held: fp32 (which names every row up to 2^24), int32, int64, or flex16 mantissas with the exponent
  * of slot_idx */
@@ -603,12 +604,12 @@ int b2_embed_update(const void* delta, const void* idx, void* dW, int32_t flex, 
  * block NULL: the stream is `residual` itself (residual_scale 1, no gate, no post_weight, stream NULL);
  * post_weight NULL: the block's result is not normalised; pre_weight and out NULL: the stream alone.
  * Tensors of rows have a stride in elements, at least `features` where there is more than one row.  `stream` may be
- * the memory of `residual`.  block_rstd and stream_rstd [rows], where not NULL, receive 1 / sqrt(mean + eps), which
- * the gradients read.
+ * the memory of `residual`, with its stride.  block_rstd and stream_rstd [rows], where not NULL, receive
+ * 1 / sqrt(mean + eps), which the gradients read.
  *   bprop: from d_out (NULL without pre_weight) and d_stream (NULL: zero), the gradients of all five operands; those
  *          that are NULL are not stored.  Reads stream (residual where there is no block) and the rstd's as fprop
- *          has left them.  d_residual may be the memory of d_stream.  Sums over rows (of the weights, of a gate per
- *          feature) are added in an order that depends on the sizes alone; rows = 0 leaves them zero.
+ *          has left them.  d_residual may be the memory of d_stream, with its stride.  Sums over rows (of the weights,
+ *          of a gate per feature) are added in an order that depends on the sizes alone; rows = 0 leaves them zero.
  * The scratch needs no initial value; calls on two streams at once need one each. */
 #define B2_GATE_NONE 0
 #define B2_GATE_FEATURE 1 /* [features] */

@@ -902,6 +902,17 @@ int check_flex(int flex, int kind, const FlexArgs& f) {
 
 }  // namespace
 
+static int check_memory(const void* whole, int32_t V, const void* rows, int64_t n, int32_t F, const void* idx, int32_t idx_kind, int32_t flex,
+                        bool whole_written) {
+    const size_t value = flex ? 2 : 4, token = idx_kind == B2_IDX_I64 ? 8 : idx_kind == B2_IDX_FLEX16 ? 2 : 4;
+    B2_REQUIRE((uintptr_t)whole % value == 0 && (uintptr_t)rows % value == 0 && (uintptr_t)idx % token == 0, "a tensor of the lookup lies between two addresses");
+    const size_t table = (size_t)V * F * value, list = (size_t)n * F * value, tokens = (size_t)n * token;
+    B2_REQUIRE(!b2::overlap(whole, table, rows, list) &&
+                   !(whole_written ? b2::overlap(whole, table, idx, tokens) : b2::overlap(rows, list, idx, tokens)),
+               "the result of the lookup, or of its gradient, overlaps an operand");
+    return B2_OK;
+}
+
 extern "C" int b2_embed_fprop(const void* table, const void* idx, void* out, int32_t flex, int32_t idx_kind, int32_t V, int32_t F, int64_t n_idx,
                               float scale, const b2_flex_scale* scales, int32_t slot_table, int32_t slot_idx, int32_t slot_out, int32_t* stats,
                               uint64_t* probe_out, int32_t probe, void* stream) {
@@ -910,6 +921,7 @@ extern "C" int b2_embed_fprop(const void* table, const void* idx, void* out, int
     B2_CHECK(check_flex(flex, idx_kind, f));
     if (n_idx == 0) return B2_OK;
     B2_REQUIRE(table && idx && out, "bad lookup: missing tensor");
+    B2_CHECK(check_memory(table, V, out, n_idx, F, idx, idx_kind, flex, false));
     B2_CHECK(b2::require_here(out, "the lookup's result"));
     B2_CHECK(b2::require_read(table, "the table"));
     B2_CHECK(b2::require_read(idx, "the index"));
@@ -942,6 +954,7 @@ extern "C" int b2_embed_update(const void* delta, const void* idx, void* dW, int
     B2_REQUIRE(!(flex && onto), "flex16 sums have an exponent of their own: they are not added onto a table");
     B2_REQUIRE(dW && (n_idx == 0 || (delta && idx)), "bad lookup gradient: missing tensor");
     B2_REQUIRE(scratch && scratch_bytes >= need, "the lookup's gradient needs %zu bytes of scratch, got %zu", need, scratch_bytes);
+    B2_CHECK(check_memory(dW, V, delta, n_idx, F, idx, idx_kind, flex, true));
     B2_CHECK(b2::require_here(dW, "the table's gradient"));
     B2_CHECK(b2::require_here(scratch, "the scratch"));
     B2_CHECK(b2::require_read(n_idx ? delta : nullptr, "delta"));

@@ -672,6 +672,22 @@ int check_stride(const b2_norm* a, const void* p, int64_t stride, const char* wh
     return B2_OK;
 }
 
+// (Rows of several tensors may lie side by side: tensors are told apart by where they begin.)
+int check_apart(const void* const* written, int count, const void* const* read, int reads) {
+    for (int i = 0; i < count; ++i) {
+        if (!written[i]) continue;
+        for (int k = 0; k < i; ++k) B2_REQUIRE(written[i] != written[k], "two results of the norm lie in one place");
+        for (int k = 0; k < reads; ++k) B2_REQUIRE(written[i] != read[k], "a result of the norm lies in the place of an operand");
+    }
+    return B2_OK;
+}
+
+int check_in_place(const b2_norm* a, const void* result, int64_t result_stride, const void* operand, int64_t stride, const char* what) {
+    B2_REQUIRE(!result || result != operand || a->rows <= 1 || result_stride == stride, "%s in place of its operand has other strides: %lld, %lld", what,
+               (long long)result_stride, (long long)stride);
+    return B2_OK;
+}
+
 bool rows_aligned(const void* p, int64_t stride) { return b2::aligned16(p) && stride % 4 == 0; }
 
 template <int IT, bool RAGGED>
@@ -739,6 +755,10 @@ extern "C" int b2_norm_fprop(const b2_norm* a, void* stream) {
     B2_CHECK(check_stride(a, a->stream, a->stream_stride, "stream"));
     B2_CHECK(check_stride(a, a->out, a->out_stride, "result"));
     if (a->gate_kind == B2_GATE_FULL) B2_CHECK(check_stride(a, a->gate, a->gate_stride, "gate"));
+    const void* results[] = {a->out, a->stream, a->block_rstd, a->stream_rstd};
+    const void* operands[] = {a->block, a->gate, a->post_weight, a->pre_weight, a->stream == a->residual ? nullptr : a->residual};
+    B2_CHECK(check_apart(results, 4, operands, 5));
+    B2_CHECK(check_in_place(a, a->stream, a->stream_stride, a->residual, a->residual_stride, "the stream"));
     if (a->out) B2_CHECK(b2::require_here(a->out, "the norm's result"));
     if (a->stream) B2_CHECK(b2::require_here(a->stream, "the stream"));
     B2_CHECK(b2::require_read(a->residual, "the residual"));
@@ -807,6 +827,11 @@ extern "C" int b2_norm_bprop(const b2_norm* a, const b2_norm_grads* d, void* scr
         B2_CHECK(check_stride(a, d->d_residual, d->d_residual_stride, "residual's gradient"));
         B2_CHECK(check_stride(a, d->d_block, d->d_block_stride, "block's gradient"));
         if (a->gate_kind == B2_GATE_FULL) B2_CHECK(check_stride(a, d->d_gate, d->d_gate_stride, "gate's gradient"));
+        const void* results[] = {d->d_residual, d->d_block, d->d_gate, d->d_post_weight, d->d_pre_weight};
+        const void* operands[] = {a->block ? a->stream : a->residual, a->block, a->gate, a->post_weight, a->pre_weight, d->d_out,
+                                  a->stream_rstd, a->block_rstd, d->d_stream == d->d_residual ? nullptr : d->d_stream};
+        B2_CHECK(check_apart(results, 5, operands, 9));
+        B2_CHECK(check_in_place(a, d->d_residual, d->d_residual_stride, d->d_stream, d->d_stream_stride, "the residual's gradient"));
     }
     B2_CHECK(b2::require_here(scratch, "the norm's scratch"));
     if (a->rows > 0) {

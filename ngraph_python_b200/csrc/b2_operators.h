@@ -35,6 +35,12 @@ inline int require_read(const void* in, const char* what) {
     return B2_OK;
 }
 
+// Blocks write in any order: a dense result has no memory in common with an operand.
+inline bool overlap(const void* a, size_t a_bytes, const void* b, size_t b_bytes) {
+    return a && b && a_bytes && b_bytes && (uintptr_t)a < (uintptr_t)b + b_bytes &&
+           (uintptr_t)b < (uintptr_t)a + a_bytes;
+}
+
 // More than 48 KB of dynamic shared memory is asked for once per kernel and device.
 inline int allow_shared(const void* kernel, int bytes, std::atomic<unsigned long long>* done) {
     int now = 0;

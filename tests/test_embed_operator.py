@@ -361,6 +361,33 @@ def test_refusals():
             update(**kw)
 
 
+@pytest.mark.parametrize("kind,flex", [(0, 0), (1, 0), (2, 0), (3, 1)])
+def test_results_in_the_place_of_operands_are_refused(kind, flex):
+    """8 rows of 4 values, 6 tokens; an operand begins or ends a value inside the result, or beside it."""
+    from ngraph_python_b200 import lib
+    value, token = (2, 2) if flex else (4, {0: 4, 1: 4, 2: 8}[kind])
+    form = (256, 0, 1, 2, 256, 256, 0) if flex else PLAIN
+    base, table, rows, idx = 1 << 20, 32 * value, 24 * value, 6 * token
+    calls = (("overlaps", lambda t, r, x: lib.raw().b2_embed_fprop(t, x, r, flex, kind, 8, 4, 6, 1.0, *form, 0), False),
+             ("overlaps", lambda t, r, x: lib.raw().b2_embed_update(r, x, t, flex, kind, 8, 4, 6, 1.0, -1, 0, *form, 256, 1 << 20, 0), True))
+    for word, call, of_table in calls:
+        def refused(*at):
+            with pytest.raises(lib.B200Error) as e:              # (addresses of nothing: refused in any case)
+                lib.check(call(*at))
+            return word in str(e.value)
+        far = base + (1 << 16)
+        for r, there in ((base, True), (base + table - value, True), (base + table, False), (base - rows + value, True), (base - rows, False)):
+            assert refused(base, r, far) == there
+        size, held = (table, lambda x: (base, far, x)) if of_table else (rows, lambda x: (far, base, x))
+        for x, there in ((base, True), (base + (size - value) // token * token, True), (base + size, False), (base - idx + token, True), (base - idx, False)):
+            assert refused(*held(x)) == there
+        # the index is read, and so is the other: they may lie anywhere
+        word = "between"
+        for at in ((base + 1, far, 2 * far), (base, far + 1, 2 * far), (base, far, 2 * far + 1)):
+            assert refused(*at)
+        word = "overlaps"
+
+
 @pytest.mark.gpu
 def test_host_memory_is_refused():
     import torch

@@ -482,6 +482,46 @@ def test_refusals():
             lib.check(raw.b2_norm_bprop(ctypes.byref(a), ctypes.byref(d), scratch, nbytes, 0))
 
 
+def _apart(**places):
+    """The same with every tensor in a place of its own, but for those named."""
+    a, d = _whole()
+    names = [(a, k) for k in ("block", "residual", "gate", "post_weight", "pre_weight", "stream", "out", "block_rstd", "stream_rstd")] + \
+        [(d, k) for k in ("d_out", "d_stream", "d_residual", "d_block", "d_gate", "d_post_weight", "d_pre_weight")]
+    at = {k: (1 << 20) + 4096 * n for n, (_, k) in enumerate(names)}
+    for x, k in names:
+        setattr(x, k, at[places[k]] if k in places else at[k])
+    return a, d
+
+
+def test_results_in_the_place_of_operands_are_refused():
+    from ngraph_python_b200 import lib
+
+    def message(forward, a, d):
+        with pytest.raises(lib.B200Error) as e:                  # (addresses of nothing: refused in any case)
+            lib.check(lib.raw().b2_norm_fprop(ctypes.byref(a), 0) if forward else
+                      lib.raw().b2_norm_bprop(ctypes.byref(a), ctypes.byref(d), 256, 1 << 24, 0))
+        return str(e.value)
+    results, operands = ("out", "stream", "block_rstd", "stream_rstd"), ("block", "residual", "gate", "post_weight", "pre_weight")
+    for r in results:
+        for o in operands:
+            assert ("place" in message(True, *_apart(**{r: o}))) == ((r, o) != ("stream", "residual"))
+        for o in set(results) - {r}:
+            assert "one place" in message(True, *_apart(**{r: o}))
+    results = ("d_residual", "d_block", "d_gate", "d_post_weight", "d_pre_weight")
+    for r in results:
+        for o in ("d_out", "d_stream", "stream", "block", "gate", "post_weight", "pre_weight", "block_rstd", "stream_rstd"):
+            assert ("place" in message(False, *_apart(**{r: o}))) == ((r, o) != ("d_residual", "d_stream"))
+        for o in set(results) - {r}:
+            assert "one place" in message(False, *_apart(**{r: o}))
+    for forward, place in ((True, dict(stream="residual")), (False, dict(d_residual="d_stream"))):
+        a, d = _apart(**place)
+        assert "strides" not in message(forward, a, d)
+        a.stream_stride, d.d_residual_stride = 12, 12
+        assert "other strides" in message(forward, a, d)
+        a.rows = 1
+        assert "strides" not in message(forward, a, d)
+
+
 @pytest.mark.gpu
 def test_host_memory_is_refused():
     import torch
