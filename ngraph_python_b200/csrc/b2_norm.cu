@@ -280,24 +280,26 @@ norm_row_kernel(const b2_norm a) {
 // apart and so lie alike; a copy starts at the 16-byte boundary below the row, and a thread's columns, whose sums it keeps,
 // are the vectors of memory.  (Value by value 3000 x 5001 took 83 us.)  A wait that runs out turns the results into NaN.
 constexpr int kStages = 3;
+constexpr int kGradShared = 226 << 10;      // (of 227 KB, with the static words)
 
 struct Ring {
     int stages, slot;                   // bytes of one tensor's row, with room for its alignment
 };
 
-template <bool RAGGED, int MOST, bool U, bool POST, int GATE>
+template <bool RAGGED, int MOST, int IT, bool U, bool POST, int GATE>
 __global__ void __launch_bounds__(MOST)
 norm_grad_row_kernel(const b2_norm a, const b2_norm_grads d, float* __restrict__ out_sums, const Ring ring) {
-    extern __shared__ __align__(128) unsigned char room[];
+    extern __shared__ __align__(128) unsigned char shared[];
     __shared__ unsigned long long first_full[kStages], then_full[kStages];
     __shared__ TwoSums sums;
-    constexpr int VEC = 4, IT = 2;
-    constexpr bool HOLD = MOST <= 640;          // weights stay in registers
+    constexpr int VEC = 4;
+    constexpr bool HOLD = IT == 2;              // weights stay in registers, in shared memory otherwise
     constexpr bool FULL = GATE == B2_GATE_FULL, FEATURE = GATE == B2_GATE_FEATURE;
     const bool has_ds = d.d_stream != nullptr;
     // places of the tensors within a stage
     const int at_dy = ring.slot, at_ds = 2 * ring.slot, at_u = at_ds + (has_ds ? ring.slot : 0), at_g = at_u + (U ? ring.slot : 0);
     const int stage_bytes = at_g + (FULL ? ring.slot : 0);
+    unsigned char* const room = shared + (HOLD ? 0 : (1 + POST + FEATURE) * ring.slot);
     const float* xs = U ? a.stream : a.residual;
     const long long xs_stride = U ? a.stream_stride : a.residual_stride;
     const int F = a.features, tid = threadIdx.x, shift = RAGGED ? shift_of(xs + blockIdx.x * xs_stride) : 0, i0 = first_of<VEC, IT>() - shift;
@@ -365,17 +367,21 @@ norm_grad_row_kernel(const b2_norm a, const b2_norm_grads d, float* __restrict__
             get<VEC>(w + i, v);
         }
     };
-    auto weights_first = [&](int k, int i) { weight(a.pre_weight, i, w_pre[k]); };
-    auto weights_then = [&](int k, int i) {
+    // (each thread keeps and reads its own columns)
+    float* const kept = reinterpret_cast<float*>(shared) + shift;
+    const int apart = ring.slot / (int)sizeof(float);
+#pragma unroll
+    for (int k = 0; k < IT; ++k) {
+        const int i = i0 + k * 32 * VEC;
+        weight(a.pre_weight, i, w_pre[k]);
         if (POST) weight(a.post_weight, i, w_post[k]);
         if (FEATURE) weight(a.gate, i, w_gate[k]);
-    };
-    if constexpr (HOLD)
-#pragma unroll
-        for (int k = 0; k < IT; ++k) {
-            weights_first(k, i0 + k * 32 * VEC);
-            weights_then(k, i0 + k * 32 * VEC);
+        if (!HOLD && i < F) {
+            put<VEC>(kept + i, w_pre[k]);
+            if (POST) put<VEC>(kept + apart + i, w_post[k]);
+            if (FEATURE) put<VEC>(kept + (POST ? 2 : 1) * apart + i, w_gate[k]);
         }
+    }
     const float over = 1.0f / (float)F;
     int turn = 0, s = 0;
     unsigned phase = 0;
@@ -394,9 +400,9 @@ norm_grad_row_kernel(const b2_norm a, const b2_norm_grads d, float* __restrict__
 #pragma unroll
             for (int k = 0; k < IT; ++k) {
                 const int i = i0 + k * 32 * VEC;
-                if constexpr (!HOLD) weights_first(k, i);
                 float v[VEC] = {}, y[VEC] = {};
                 if (i < F) {
+                    if constexpr (!HOLD) get<VEC>(kept + i, w_pre[k]);
                     load(x, i, v);
                     load(dy, i, y);
                 }
@@ -440,7 +446,10 @@ norm_grad_row_kernel(const b2_norm a, const b2_norm_grads d, float* __restrict__
                 store(d.d_residual + row * d.d_residual_stride, i, v);
             }
             if constexpr (!U) continue;
-            if constexpr (!HOLD) weights_then(k, i);
+            if constexpr (!HOLD) {
+                if (POST) get<VEC>(kept + apart + i, w_post[k]);
+                if (FEATURE) get<VEC>(kept + (POST ? 2 : 1) * apart + i, w_gate[k]);
+            }
             load(u, i, uh[k]);
             float gv[VEC], dg[VEC];
             if constexpr (FULL) load(g, i, gv);
@@ -637,24 +646,35 @@ int threads_of(int F, int each, int most) {
 }
 
 // How the gradient is launched: eight values of a row to a thread, CTAs for about 512 threads an SM (for 768 or 1024 no
-// registers are left: 16384 x 2048 125, 151 and 141 us) or one of more, three rows ahead where they fit.  Sixteen values
-// to a thread of rows beyond 4096 features: 4096 x 8192 161 us, 154 with eight; 3000 x 5001 180 and 83.
+// registers are left: 16384 x 2048 125, 151 and 141 us) or one of up to 640, three rows ahead where they fit.  Of rows
+// beyond 5120 features sixteen values to a thread, whose weights lie in shared memory, read from there in every row:
+// 4096 x 8192 131 us, 154 with eight values to 1024 threads and weights from L2, 144 with those in shared memory (64
+// registers a thread); a gate for every value 185 and 176, which leaves shared memory for one row at a time.  Of
+// 5000 features 71 us for 3000 rows, 67 with eight.
 struct GradPlan {
-    int threads, ctas;
+    int threads, ctas, each, room;
     Ring ring;
 };
 GradPlan grad_plan(const b2_norm& a, int tensors, bool ragged) {
     GradPlan p = {};
-    p.threads = threads_of(a.features + (ragged ? 3 : 0), 8, 1024);
-    long long per_sm = p.threads > 512 ? 1 : p.threads ? 512 / p.threads : 4;
+    const int values = a.features + (ragged ? 3 : 0);
+    p.each = 8;
+    p.threads = threads_of(values, 8, 640);
+    if (!p.threads) {
+        p.each = 16;
+        p.threads = threads_of(values, 16, 512);
+    }
+    long long per_sm = p.threads * p.each > 512 * 8 ? 1 : p.threads ? 512 / p.threads : 4;
     if (per_sm > 16) per_sm = 16;
     p.ctas = (int)(a.rows < b2::kSms * per_sm ? a.rows : b2::kSms * per_sm);
-    if (!p.threads) return p;
-    p.ring.slot = (a.features + 3 + 3) / 4 * 16;
-    const int room = (int)((220 << 10) / per_sm) - 1024;
+    if (!p.threads || !tensors) return p;
+    p.ring.slot = (values + 3) / 4 * 16;
+    const int weights = p.each == 16 ? 1 + (a.post_weight != nullptr) + (a.gate_kind == B2_GATE_FEATURE) : 0;
+    const int room = p.each == 16 ? kGradShared - weights * p.ring.slot : (int)((220 << 10) / per_sm) - 1024;
     p.ring.stages = room / (p.ring.slot * tensors);
     if (p.ring.stages > kStages) p.ring.stages = kStages;
     if (p.ring.stages < 1) p.threads = 0;
+    p.room = p.ring.slot * (weights + p.ring.stages * tensors);
     return p;
 }
 
@@ -717,24 +737,24 @@ int launch_rows(const b2_norm& a, int threads, cudaStream_t st) {
     return B2_OK;
 }
 
-template <bool RAGGED, int MOST, bool U, bool POST, int GATE>
+template <bool RAGGED, int MOST, int IT, bool U, bool POST, int GATE>
 int launch_grad(const b2_norm& a, const b2_norm_grads& d, const GradPlan& p, int tensors, float* sums, cudaStream_t st) {
     static std::atomic<unsigned long long> done{0};
-    B2_CHECK(b2::allow_shared((const void*)norm_grad_row_kernel<RAGGED, MOST, U, POST, GATE>, 220 << 10, &done));
-    B2_CUDA((b2::launch_after(norm_grad_row_kernel<RAGGED, MOST, U, POST, GATE>, dim3(p.ctas), p.threads, (size_t)p.ring.stages * p.ring.slot * tensors, st, a, d,
+    B2_CHECK(b2::allow_shared((const void*)norm_grad_row_kernel<RAGGED, MOST, IT, U, POST, GATE>, kGradShared, &done));
+    B2_CUDA((b2::launch_after(norm_grad_row_kernel<RAGGED, MOST, IT, U, POST, GATE>, dim3(p.ctas), p.threads, (size_t)p.room, st, a, d,
                               sums, p.ring)));
     return B2_OK;
 }
 
-template <bool RAGGED, int MOST>
+template <bool RAGGED, int MOST, int IT>
 int launch_grad_of(const b2_norm& a, const b2_norm_grads& d, const GradPlan& p, int tensors, float* sums, cudaStream_t st) {
-    if (!a.block) return launch_grad<RAGGED, MOST, false, false, B2_GATE_NONE>(a, d, p, tensors, sums, st);
+    if (!a.block) return launch_grad<RAGGED, MOST, IT, false, false, B2_GATE_NONE>(a, d, p, tensors, sums, st);
 #define B2_GATED(POST)                                                                                               \
     switch (a.gate_kind) {                                                                                           \
-        case B2_GATE_FEATURE: return launch_grad<RAGGED, MOST, true, POST, B2_GATE_FEATURE>(a, d, p, tensors, sums, st);  \
-        case B2_GATE_ROW: return launch_grad<RAGGED, MOST, true, POST, B2_GATE_ROW>(a, d, p, tensors, sums, st);          \
-        case B2_GATE_FULL: return launch_grad<RAGGED, MOST, true, POST, B2_GATE_FULL>(a, d, p, tensors, sums, st);        \
-        default: return launch_grad<RAGGED, MOST, true, POST, B2_GATE_NONE>(a, d, p, tensors, sums, st);                  \
+        case B2_GATE_FEATURE: return launch_grad<RAGGED, MOST, IT, true, POST, B2_GATE_FEATURE>(a, d, p, tensors, sums, st);  \
+        case B2_GATE_ROW: return launch_grad<RAGGED, MOST, IT, true, POST, B2_GATE_ROW>(a, d, p, tensors, sums, st);          \
+        case B2_GATE_FULL: return launch_grad<RAGGED, MOST, IT, true, POST, B2_GATE_FULL>(a, d, p, tensors, sums, st);        \
+        default: return launch_grad<RAGGED, MOST, IT, true, POST, B2_GATE_NONE>(a, d, p, tensors, sums, st);                  \
     }
     if (a.post_weight) B2_GATED(true)
     B2_GATED(false)
@@ -862,14 +882,14 @@ extern "C" int b2_norm_bprop(const b2_norm* a, const b2_norm_grads* d, void* scr
     const GradPlan p = grad_plan(*a, tensors, ragged);
     if (p.ctas > 0) {
         if (!p.threads || !d->d_out || !(vec || ragged)) B2_CUDA(b2::launch_after(vec ? norm_grad_any_kernel<4> : norm_grad_any_kernel<1>, dim3(p.ctas), kThreads, 0, st, *a, *d, sums));
-#define B2_GRAD(MOST)                                                                                       \
-    else if (p.threads <= MOST) {                                                                            \
-        if (vec) B2_CHECK((launch_grad_of<false, MOST>(*a, *d, p, tensors, sums, st)));                      \
-        else B2_CHECK((launch_grad_of<true, MOST>(*a, *d, p, tensors, sums, st)));                           \
+#define B2_GRAD(MOST, EACH)                                                                                  \
+    else if (p.threads <= MOST && p.each == EACH) {                                                          \
+        if (vec) B2_CHECK((launch_grad_of<false, MOST, EACH / 4>(*a, *d, p, tensors, sums, st)));            \
+        else B2_CHECK((launch_grad_of<true, MOST, EACH / 4>(*a, *d, p, tensors, sums, st)));                 \
     }
-        B2_GRAD(512)
-        B2_GRAD(640)
-        B2_GRAD(1024)
+        B2_GRAD(512, 8)
+        B2_GRAD(640, 8)
+        B2_GRAD(512, 16)
 #undef B2_GRAD
     }
     if (d->d_pre_weight || d->d_post_weight || gate)

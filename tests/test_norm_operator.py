@@ -280,6 +280,19 @@ def test_backward_strides(rows, F, pad, offset):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("gate,post", [("feature", True), ("row", True), ("full", True), ("full", False), ("none", False)])
+@pytest.mark.parametrize("rows,F,pad,offset", [(470, 5116, 0, 0), (470, 5120, 4, 4), (310, 5124, 0, 0), (310, 5119, 2, 1), (310, 6141, 1, 3), (450, 6144, 0, 0),
+                                               (200, 8189, 0, 0), (200, 8189, 3, 2), (200, 8190, 2, 0), (200, 8192, 0, 0)])
+def test_backward_of_long_rows(rows, F, pad, offset, gate, post):
+    """Where a thread's share of a row, and the place of its weights, changes: two and more rows to a CTA, one behind another."""
+    c = _case(rows, F, gate, True, post)
+    rng = np.random.RandomState(8)
+    x, rstd, rho = _stored(c)
+    d_out, d_stream = [rng.standard_normal((rows, F)).astype(np.float32) for _ in range(2)]
+    _check_backward(_backward(c, gate, x, rstd, rho, d_out, d_stream, pad, offset), c, x, rstd, rho, d_out, d_stream)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("gate", ["feature", "row", "full"])
 def test_backward_of_some(gate):
     """Gradients that nobody asks for are left out, the others keep their bits."""
@@ -304,6 +317,8 @@ def test_no_rows():
     e = np.zeros((0, 12), np.float32)
     got = _backward(c, "feature", e, np.zeros(0), np.zeros(0), e, e)
     assert not got["pre"].any() and not got["post"].any() and not got["gate"].any()
+    got = _backward(_case(0, 12, block=False, post=False), "none", e, np.zeros(0), None, None, None)
+    assert set(got) == {"residual", "pre"} and not got["pre"].any()
 
 
 @pytest.mark.gpu
