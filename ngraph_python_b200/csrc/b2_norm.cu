@@ -645,14 +645,18 @@ int threads_of(int F, int each, int most) {
     return t <= most ? t : 0;
 }
 
-// How the gradient is launched: eight values of a row to a thread, CTAs for about 512 threads an SM (for 768 or 1024 no
-// registers are left: 16384 x 2048 125, 151 and 141 us) or one of up to 640, three rows ahead where they fit.  Of rows
-// beyond 5120 features sixteen values to a thread, whose weights lie in shared memory, read from there in every row:
-// 4096 x 8192 131 us, 154 with eight values to 1024 threads and weights from L2, 144 with those in shared memory (64
+// How the gradient is launched: eight values of a row to a thread, and CTAs for as many threads an SM as have registers
+// enough, 640 (16384 rows of 1536 features: 119 us with 512, 99; of 2047: 241 and 160; of 2048, 512 in both: 127; for 768
+// or 1024 none are left: 125, 151 and 141).  Two CTAs of more than 320 threads there are only without a block, whose
+// gradient holds less: 1024 threads (6000 x 3501 80 and 59 us; 16384 x 2048 99 and 83).  With a block short rows take 512:
+// more CTAs leave more sums (8000 x 1001 44 us, 48 with 640; without a block 16384 x 1001 61 and 48), and a gate for every
+// value takes room for rows ahead (16384 x 1536 124 and 146).  Three rows ahead where they fit.
+// Of rows beyond 5120 features sixteen values to a thread, whose weights lie in shared memory, read from there in every
+// row: 4096 x 8192 131 us, 154 with eight values to 1024 threads and weights from L2, 144 with those in shared memory (64
 // registers a thread); a gate for every value 185 and 176, which leaves shared memory for one row at a time.  Of
 // 5000 features 71 us for 3000 rows, 67 with eight.
 struct GradPlan {
-    int threads, ctas, each, room;
+    int threads, ctas, each, most, room;             // `most`: threads an SM that registers are shared out for
     Ring ring;
 };
 GradPlan grad_plan(const b2_norm& a, int tensors, bool ragged) {
@@ -664,8 +668,14 @@ GradPlan grad_plan(const b2_norm& a, int tensors, bool ragged) {
         p.each = 16;
         p.threads = threads_of(values, 16, 512);
     }
-    long long per_sm = p.threads * p.each > 512 * 8 ? 1 : p.threads ? 512 / p.threads : 4;
-    if (per_sm > 16) per_sm = 16;
+    long long per_sm = p.threads ? 1 : 4;
+    p.most = 512;
+    if (p.threads && p.each == 8) {
+        const int short_row = !a.block ? 0 : a.gate_kind == B2_GATE_FULL ? 256 : 128;
+        const int total = !a.block && p.threads > 640 / 3 && p.threads <= 512 ? 1024 : p.threads <= short_row ? 512 : 640;
+        per_sm = total / p.threads > 16 ? 16 : total / p.threads;
+        p.most = per_sm * p.threads <= 512 ? 512 : per_sm * p.threads <= 640 ? 640 : 1024;
+    }
     p.ctas = (int)(a.rows < b2::kSms * per_sm ? a.rows : b2::kSms * per_sm);
     if (!p.threads || !tensors) return p;
     p.ring.slot = (values + 3) / 4 * 16;
@@ -712,8 +722,10 @@ bool rows_aligned(const void* p, int64_t stride) { return b2::aligned16(p) && st
 
 template <int IT, bool RAGGED>
 int launch_rows(const b2_norm& a, int threads, cudaStream_t st) {
-    // (148 and so every multiple of it is a multiple of four)
-    const long long most = RAGGED ? (long long)b2::kSms * (threads > 512 ? 1 : 1024 / threads > 16 ? 16 : 1024 / threads) : 1ll << 30;
+    // CTAs that go through several rows: ragged ones (148 and so every multiple of it is a multiple of four), and of up to
+    // 64 threads, since a CTA to a row is bound by their start, 1.1 ns each (16384 x 64: 18 us and 10; x 256: 20 and 15)
+    const int per_sm = !RAGGED || threads <= 32 ? 32 : threads > 512 ? 1 : 1024 / threads;
+    const long long most = RAGGED || threads <= 64 ? (long long)b2::kSms * per_sm : 1ll << 30;
     const unsigned blocks = (unsigned)(a.rows < most ? a.rows : most);
     const size_t room = RAGGED ? (size_t)3 * ((a.features + 6) / 4 * 4) * sizeof(float) : 0;
 #define B2_LAUNCH(U, POST, GATE)                                                                                                       \
@@ -883,13 +895,15 @@ extern "C" int b2_norm_bprop(const b2_norm* a, const b2_norm_grads* d, void* scr
     if (p.ctas > 0) {
         if (!p.threads || !d->d_out || !(vec || ragged)) B2_CUDA(b2::launch_after(vec ? norm_grad_any_kernel<4> : norm_grad_any_kernel<1>, dim3(p.ctas), kThreads, 0, st, *a, *d, sums));
 #define B2_GRAD(MOST, EACH)                                                                                  \
-    else if (p.threads <= MOST && p.each == EACH) {                                                          \
+    else if (p.most == MOST && p.each == EACH) {                                                             \
         if (vec) B2_CHECK((launch_grad_of<false, MOST, EACH / 4>(*a, *d, p, tensors, sums, st)));            \
         else B2_CHECK((launch_grad_of<true, MOST, EACH / 4>(*a, *d, p, tensors, sums, st)));                 \
     }
         B2_GRAD(512, 8)
         B2_GRAD(640, 8)
         B2_GRAD(512, 16)
+        else if (vec) B2_CHECK((launch_grad<false, 1024, 2, false, false, B2_GATE_NONE>(*a, *d, p, tensors, sums, st)));
+        else B2_CHECK((launch_grad<true, 1024, 2, false, false, B2_GATE_NONE>(*a, *d, p, tensors, sums, st)));
 #undef B2_GRAD
     }
     if (d->d_pre_weight || d->d_post_weight || gate)

@@ -293,6 +293,30 @@ def test_backward_of_long_rows(rows, F, pad, offset, gate, post):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("gate,block", [("feature", True), ("full", True), ("none", True), ("none", False)])
+@pytest.mark.parametrize("rows,F", [(3000, 64), (1600, 707), (1000, 1536), (1000, 1792), (700, 2047), (700, 2048), (500, 2560), (500, 3501), (400, 4096)])
+def test_backward_of_many_rows(rows, F, gate, block):
+    """More rows than CTAs, of all numbers of CTAs to an SM."""
+    c = _case(rows, F, gate, block, block)
+    rng = np.random.RandomState(9)
+    x, rstd, rho = _stored(c)
+    d_out, d_stream = [rng.standard_normal((rows, F)).astype(np.float32) for _ in range(2)]
+    got = _backward(c, gate, x, rstd, rho, d_out, d_stream)
+    _check_backward(got, c, x, rstd, rho, d_out, d_stream)
+    again = _backward(c, gate, x, rstd, rho, d_out, d_stream)
+    assert all(np.array_equal(got[k], again[k]) for k in got)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("gate,block", [("feature", True), ("row", True), ("full", True), ("none", False)])
+@pytest.mark.parametrize("rows,F", [(12000, 4), (12000, 64), (12000, 101), (11000, 256), (10000, 260), (10000, 509), (10000, 512), (10000, 516)])
+def test_forward_of_many_short_rows(rows, F, gate, block):
+    c = _case(rows, F, gate, block, block)
+    got, _ = _forward(c, gate)
+    _check_forward(got, c, F)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("gate", ["feature", "row", "full"])
 def test_backward_of_some(gate):
     """Gradients that nobody asks for are left out, the others keep their bits."""
