@@ -70,6 +70,16 @@ template <> struct Pack<short, 8> {
         }
     }
 };
+template <> struct Pack<short, 4> {
+    int2 w;
+    __device__ __forceinline__ void load(const short* p) { w = *reinterpret_cast<const int2*>(p); }
+    __device__ __forceinline__ void get(float* v) const {
+        v[0] = (float)(short)(w.x & 0xffff);
+        v[1] = (float)(w.x >> 16);
+        v[2] = (float)(short)(w.y & 0xffff);
+        v[3] = (float)(w.y >> 16);
+    }
+};
 template <typename T> struct Pack<T, 1> {
     T w;
     __device__ __forceinline__ void load(const T* p) { w = *p; }
@@ -117,6 +127,8 @@ template <int VEC> struct Sink<short, VEC> {
             w.z = (m[4] & 0xffff) | (m[5] << 16);
             w.w = (m[6] & 0xffff) | (m[7] << 16);
             *reinterpret_cast<int4*>(p) = w;
+        } else if constexpr (VEC == 4) {
+            *reinterpret_cast<int2*>(p) = make_int2((m[0] & 0xffff) | (m[1] << 16), (m[2] & 0xffff) | (m[3] << 16));
         } else {
             *p = (short)m[0];
         }
@@ -835,8 +847,10 @@ template <typename T>
 int launch_update(const void* delta, const void* idx, void* dW, int kind, int V, int F, long long n, float scale, int pad, int onto, const FlexArgs& f,
                   void* scratch, cudaStream_t st) {
     if (n == 0 && (onto || f.probe)) return B2_OK;
-    constexpr int W = wide<T>();
-    const bool vec = F % W == 0 && b2::aligned16(delta) && b2::aligned16(dW);
+    // (four values to a lane of either type: with eight mantissas 16384 x 1024 into 30000 rows took 52 us, 49 so; 16384 x 64
+    // into 200 rows 26 and 21)
+    constexpr int W = 4;
+    const bool vec = F % W == 0 && ((uintptr_t)delta | (uintptr_t)dW) % (W * sizeof(T)) == 0;
     const int owners = owners_of(V);
     OrderArgs a;
     a.idx = idx;

@@ -185,7 +185,8 @@ def test_infinities_reach_their_rows_alone():
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("n,F,V,offset", [(1, 1, 1, 0), (300, 24, 37, 0), (3001, 301, 1009, 0), (900, 512, 30, 0), (500, 64, 9, 1)])
+@pytest.mark.parametrize("n,F,V,offset", [(1, 1, 1, 0), (300, 24, 37, 0), (3001, 301, 1009, 0), (900, 512, 30, 0), (500, 64, 9, 1),
+                                          (200, 20, 9, 0), (500, 36, 9, 4), (3001, 132, 1009, 4), (700, 260, 40, 2)])
 def test_flex16(n, F, V, offset):
     """Mantissas in and out, the largest of them, and what a measuring launch leaves."""
     import torch
