@@ -4,7 +4,7 @@
 //   gradient  dW[v, :] = scale * sum of delta[t, :] over the t with token[t] = v, t ascending
 //
 // Both are bound by memory: one multiplication or addition a value (16384 x 1024 looked up: 17.8 us, 0.77 of the rate of a
-// copy; 8192 x 1024 added into 32000 rows: 36 us, of which the sort takes 7 and 18 are zeros).  The gradient is two launches.  The first
+// copy; 8192 x 1024 added into 32000 rows: 32.5 us, of which the sort takes 7 and 18 are zeros).  The gradient is two launches.  The first
 // sorts: a CTA owns the rows v = b (mod CTAs), so that the frequent tokens of a vocabulary, which lie next to one
 // another, go to different CTAs; it reads every token, counts its own per warp, and writes their positions row by
 // row in ascending order.  No counter is shared between CTAs -- where a CTA's positions begin is the number of tokens
@@ -503,22 +503,23 @@ struct SumArgs {
     Scratch s;
 };
 
-// A warp takes the parts that begin among kWindow places of the sorted list, and 32 * VEC * UN columns: first the
+// A warp takes the parts that begin among WINDOW places of the sorted list, and 32 * VEC * UN columns: first the
 // tokens of these places, loaded together whatever rows they belong to, then what the last part has beyond them, eight
 // at a time.  So a thousand tokens that occur once cost little more than one that occurs a thousand times.  The blocks
-// behind the first sum_blocks write the zeros of rows that no token names.  Windows of 4 against 8 and 16: 8192 x 1024 into 32000 rows 42, 43
-// and 46 us a call, 3001 x 301 flex16 18, 20 and 23.
-constexpr int kWindow = 4;
+// behind the first sum_blocks write the zeros of rows that no token names.  Blocks of four warps: where a row has many
+// tokens one warp of eight has a part to add and the others' places wait for it (16384 x 1024 into 300 rows 36 us a call
+// with eight, 30 with four, 32 with two; 16384 x 768 onto 50000 32, 27 and 28).
+constexpr int kSumWarps = 4;
 
-template <typename T, int VEC, int UN, bool ONTO>
-__global__ void __launch_bounds__(256)
+template <typename T, int VEC, int UN, int WINDOW, bool ONTO>
+__global__ void __launch_bounds__(32 * kSumWarps)
 sum_kernel(const T* __restrict__ delta, T* dW, const SumArgs a, const FlexArgs f) {
     after_earlier_kernels();
     constexpr int COLS = 32 * VEC;
     constexpr bool flex = sizeof(T) == 2;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     if (blockIdx.x >= a.sum_blocks) {
-        const long long from = ((long long)(blockIdx.x - a.sum_blocks) * 8 + warp) * a.zero_rows, mine = from + lane;
+        const long long from = ((long long)(blockIdx.x - a.sum_blocks) * kSumWarps + warp) * a.zero_rows, mine = from + lane;
         const bool empty = lane < a.zero_rows && mine < (long long)a.owners * a.rows && !a.s.used[mine];
         for (unsigned left = __ballot_sync(0xffffffffu, empty); left; left &= left - 1) {
             const unsigned k = (unsigned)(from + __ffs(left) - 1);
@@ -530,14 +531,14 @@ sum_kernel(const T* __restrict__ delta, T* dW, const SumArgs a, const FlexArgs f
     const int F = a.F, block = blockIdx.x % a.col_blocks;
     const float step = flex ? f.table[f.slot_in].scale : 1.0f;
     Sink<T, VEC> sink(f);
-    const int base = (int)(blockIdx.x / a.col_blocks * 8 + warp) * kWindow;
+    const int base = (int)(blockIdx.x / a.col_blocks * kSumWarps + warp) * WINDOW;
     // entries of this window and of what a part that begins in it can reach
     const int4 none = make_int4(0, -1, 0, 0);
     const int4* list = reinterpret_cast<const int4*>(a.s.sorted);
     const int4 near = base + lane < a.n ? list[base + lane] : none;
-    const int far = lane < kWindow && base + 32 + lane < a.n ? list[base + 32 + lane].x : 0;
+    const int far = lane < WINDOW && base + 32 + lane < a.n ? list[base + 32 + lane].x : 0;
     // parts begin where the rank is a multiple of kPart; the last of this window ends where its row or its 32 do
-    const unsigned those = __ballot_sync(0xffffffffu, lane < kWindow && near.y >= 0 && near.z % kPart == 0);
+    const unsigned those = __ballot_sync(0xffffffffu, lane < WINDOW && near.y >= 0 && near.z % kPart == 0);
     if (those) {
         const int from = __ffs(those) - 1, last = 31 - __clz(those);
         const int upto = last + __shfl_sync(0xffffffffu, min(kPart, near.w - near.z), last);
@@ -585,9 +586,9 @@ sum_kernel(const T* __restrict__ delta, T* dW, const SumArgs a, const FlexArgs f
             for (int u = 0; u < UN; ++u)
                 if (col0 + u * COLS < F) put_sums<VEC>(a.s.partial + (long long)(join_slot[which] + rank / kPart) * F + col0 + u * COLS, acc[u]);
         };
-        Pack<T, VEC> w[kWindow][UN], old[ONTO ? kWindow : 1][UN];
+        Pack<T, VEC> w[WINDOW][UN], old[ONTO ? WINDOW : 1][UN];
 #pragma unroll
-        for (int k = 0; k < kWindow; ++k) {
+        for (int k = 0; k < WINDOW; ++k) {
             const long long t = __shfl_sync(0xffffffffu, near.x, k);
             const int row = __shfl_sync(0xffffffffu, near.y, k), rank = __shfl_sync(0xffffffffu, near.z, k), count = __shfl_sync(0xffffffffu, near.w, k);
             if (k < from || k >= upto) continue;
@@ -596,7 +597,7 @@ sum_kernel(const T* __restrict__ delta, T* dW, const SumArgs a, const FlexArgs f
                 if (count <= kPart && rank + 1 == count) load(dW + (long long)row * F, old[k]);
         }
 #pragma unroll
-        for (int k = 0; k < kWindow; ++k) {
+        for (int k = 0; k < WINDOW; ++k) {
             const int row = __shfl_sync(0xffffffffu, near.y, k), rank = __shfl_sync(0xffffffffu, near.z, k), count = __shfl_sync(0xffffffffu, near.w, k);
             if (k < from || k >= upto) continue;
             add(w[k]);
@@ -608,13 +609,13 @@ sum_kernel(const T* __restrict__ delta, T* dW, const SumArgs a, const FlexArgs f
 #pragma unroll
                 for (int c = 0; c < VEC; ++c) acc[u][c] = 0.0f;
         }
-        if (upto > kWindow) {
+        if (upto > WINDOW) {
             const int row = __shfl_sync(0xffffffffu, near.y, last), rank = __shfl_sync(0xffffffffu, near.z, last) + upto - 1 - last,
                       count = __shfl_sync(0xffffffffu, near.w, last);
             if constexpr (ONTO)
                 if (count <= kPart) load(dW + (long long)row * F, old[0]);
             constexpr int AHEAD = UN == 1 ? 8 : 4;
-            for (int j = kWindow; j < upto; j += AHEAD) {
+            for (int j = WINDOW; j < upto; j += AHEAD) {
                 Pack<T, VEC> x[AHEAD][UN];
 #pragma unroll
                 for (int k = 0; k < AHEAD; ++k) {
@@ -885,22 +886,28 @@ int launch_update(const void* delta, const void* idx, void* dW, int kind, int V,
         case B2_IDX_I64: B2_CHECK(launch_order<B2_IDX_I64>(a, owners, st)); break;
         default: B2_CHECK(launch_order<B2_IDX_FLEX16>(a, owners, st));
     }
-    const long long sum_blocks = (n + 8 * kWindow - 1) / (8 * kWindow) * a.col_blocks;
+    // Windows of 8 places where these occupy the machine and nothing else is loaded, of 4 elsewhere (8192 x 1024 into
+    // 32000 rows 32.6 us a call, 34.0 with 4; onto them 20.3 and 19.2; 3001 x 301 flex16 17.1 and 15.5; 2000 x 1024 into
+    // 200 rows 12.6 and 11.5).  Of 2: 38, 22, 15.0 and 11.5.
+    auto blocks_of = [&](int window) { return (n + kSumWarps * window - 1) / (kSumWarps * window) * a.col_blocks; };
+    const bool longer = vec && !onto && blocks_of(8) >= 8 * b2::kSms;
+    const long long sum_blocks = blocks_of(longer ? 8 : 4);
     // about 4 KB of zeros to a warp (16: 3001 x 301 flex16 into 10007 rows 22 us, 15 with 4)
     const long long fit = 4096 / ((long long)F * (long long)sizeof(T));
     const int zero_rows = fit < 1 ? 1 : fit > 32 ? 32 : (int)fit;
-    const long long zero_blocks = onto || f.probe ? 0 : ((long long)owners * a.rows + 8 * zero_rows - 1) / (8 * zero_rows);
+    const long long zero_blocks = onto || f.probe ? 0 : ((long long)owners * a.rows + kSumWarps * zero_rows - 1) / (kSumWarps * zero_rows);
     B2_REQUIRE(sum_blocks + zero_blocks < (1ll << 31), "%lld tokens of %d features are too many for one launch", n, F);
     const SumArgs sa = {V, F, (int)n, a.rows, owners, zero_rows, (unsigned)a.col_blocks, (unsigned)sum_blocks, scale, a.s};
     const dim3 grid((unsigned)(sum_blocks + zero_blocks));
-#define B2_SUM(VEC, UN, ONTO) \
-    B2_CUDA((b2::launch_after(sum_kernel<T, VEC, UN, ONTO>, grid, 256, 0, st, (const T*)delta, (T*)dW, sa, f)))
+#define B2_SUM(VEC, UN, WINDOW, ONTO) \
+    B2_CUDA((b2::launch_after(sum_kernel<T, VEC, UN, WINDOW, ONTO>, grid, 32 * kSumWarps, 0, st, (const T*)delta, (T*)dW, sa, f)))
     if constexpr (sizeof(T) == 4) {
-        if (onto && vec) B2_SUM(W, 1, true);
-        else if (onto) B2_SUM(1, kApart, true);
+        if (onto && vec) B2_SUM(W, 1, 4, true);
+        else if (onto) B2_SUM(1, kApart, 4, true);
     }
-    if (!onto && vec) B2_SUM(W, 1, false);
-    else if (!onto) B2_SUM(1, kApart, false);
+    if (longer) B2_SUM(W, 1, 8, false);
+    else if (!onto && vec) B2_SUM(W, 1, 4, false);
+    else if (!onto) B2_SUM(1, kApart, 4, false);
 #undef B2_SUM
     return B2_OK;
 }
