@@ -581,8 +581,8 @@ int b2_lut_update(const void* delta, const void* idx, void* dW, int32_t flex, in
  *           the parts' sums in order: the same bits in every run); rows without tokens, and row pad_idx (-1: none),
  *           become zero; tokens outside [0, V) are left out.  onto != 0 (fp32): added to what dW holds, and only the
  *           rows of tokens are touched.
- * flex != 0: table, out, delta, dW hold int16 mantissas with the exponents of their slots in `scales`; the result is
- * rounded to the nearest even mantissa, its largest goes to stats[slot]; probe != 0 stores nothing and leaves the bit
+ * flex != 0: table, out, delta, dW hold int16 mantissas with the exponents of their slots in `scales`; sums of mantissas
+ * are exact, and rounded to fp32 once; the result is rounded to the nearest even mantissa, its largest goes to stats[slot]; probe != 0 stores nothing and leaves the bit
  * pattern of the largest |value| in *probe_out (maximum with what it holds).
  * `scratch` needs no initial value and may be used again by the next call on the stream, not by calls on two
  * streams at once. */

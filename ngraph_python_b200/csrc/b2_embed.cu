@@ -12,6 +12,7 @@
 // when, and nothing has to be cleared in advance.  The second adds, in parts of at most kPart positions of a row; rows
 // of more leave fp32 partial sums, which the warp that comes last adds in their order.
 #include <cstdint>
+#include <type_traits>
 
 #include "b2_operators.h"
 
@@ -517,6 +518,9 @@ sum_kernel(const T* __restrict__ delta, T* dW, const SumArgs a, const FlexArgs f
     after_earlier_kernels();
     constexpr int COLS = 32 * VEC;
     constexpr bool flex = sizeof(T) == 2;
+    // Of mantissas a part's sum is a whole number of at most 2^20, which fp32 holds.  That of 2^30 tokens is not: the parts
+    // are added as integers, and rounded once.
+    using Sum = typename std::conditional<flex, long long, float>::type;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     if (blockIdx.x >= a.sum_blocks) {
         const long long from = ((long long)(blockIdx.x - a.sum_blocks) * kSumWarps + warp) * a.zero_rows, mine = from + lane;
@@ -644,20 +648,32 @@ sum_kernel(const T* __restrict__ delta, T* dW, const SumArgs a, const FlexArgs f
                 const float* p = a.s.partial + (long long)join_slot[which] * F + col0;
 #pragma unroll
                 for (int u = 0; u < UN; ++u) {
-#pragma unroll
-                    for (int c = 0; c < VEC; ++c) acc[u][c] = 0.0f;
+                    Sum total[VEC] = {};
                     if (col0 + u * COLS >= F) continue;
                     for (int q = 0; q < parts; q += 8) {
                         float v[8][VEC];
 #pragma unroll
                         for (int x = 0; x < 8; ++x)
                             if (q + x < parts) get_sums<VEC>(p + (long long)(q + x) * F + u * COLS, v[x]);
+                        if constexpr (flex) {           // (eight parts are at most 2^23)
 #pragma unroll
-                        for (int x = 0; x < 8; ++x)
-                            if (q + x < parts)
+                            for (int c = 0; c < VEC; ++c) {
+                                float eight = 0.0f;
 #pragma unroll
-                                for (int c = 0; c < VEC; ++c) acc[u][c] += v[x][c];
+                                for (int x = 0; x < 8; ++x)
+                                    if (q + x < parts) eight += v[x][c];
+                                total[c] += (int)eight;
+                            }
+                        } else {
+#pragma unroll
+                            for (int x = 0; x < 8; ++x)
+                                if (q + x < parts)
+#pragma unroll
+                                    for (int c = 0; c < VEC; ++c) total[c] += v[x][c];
+                        }
                     }
+#pragma unroll
+                    for (int c = 0; c < VEC; ++c) acc[u][c] = (float)total[c];
                 }
                 if constexpr (ONTO) load(dW + (long long)join_row[which] * F, old[0]);
                 store(join_row[which], old[0]);
@@ -696,7 +712,7 @@ int launch_embed(const void* table, const void* idx, void* out, int V, int F, lo
 // ---- gradient of few tokens: one launch ---------------------------------------------------------------------------
 // A CTA takes its own rows through all steps: its tokens, in order, their numbers within each row, the sums, in parts as
 // above, a warp to a row and its columns at a time, and the zeros.  For more tokens the sums want more warps than those of
-// the CTA that owns a frequent one.
+// the CTA that owns a frequent one.  (256 mantissas add up to 2^23 at most: fp32 holds every sum of them.)
 constexpr int kSmall = 256;
 
 __device__ __forceinline__ int token_of_kind(int kind, const void* idx, int i, int V, float step) {

@@ -238,6 +238,55 @@ def test_flex16(n, F, V, offset):
         (sums.astype(np.float32) * step) * np.float32(scale), (V, F))
 
 
+def _long_sums(n, F):
+    """n tokens of which nine in ten are one.  The mantissas of the first half are large and positive, and the second half takes
+    them away again but for a few: the sums on the way pass 2^24, beyond which fp32 does not hold every whole number, and
+    end where a mantissa holds them."""
+    rng = np.random.RandomState(n + F)
+    half = n // 2
+    idx = np.where(rng.rand(half) < 0.9, 3, rng.randint(0, 11, half))
+    first = rng.randint(20000, 32760, (half, F))
+    order = rng.permutation(half)
+    idx = np.concatenate([idx, idx[order], [5] * (n % 2)]).astype(np.int16)
+    delta = np.concatenate([first, rng.randint(-3, 4, (half, F)) - first[order], np.ones((n % 2, F), np.int64)]).astype(np.int16)
+    sums = np.zeros((11, F), np.int64)
+    np.add.at(sums, idx, delta.astype(np.int64))
+    assert np.abs(sums).max() < 32767
+    return idx, delta, sums
+
+
+def test_sums_of_mantissas_that_fp32_does_not_hold():
+    """The cases of the next test are such: in parts of 32 that are added in fp32, sums come out wrong."""
+    for n, F in ((1600, 64), (4000, 8)):
+        idx, delta, sums = _long_sums(n, F)
+        rows = delta[idx == 3].astype(np.float32)
+        parts = np.array([np.cumsum(rows[k:k + 32], axis=0, dtype=np.float32)[-1] for k in range(0, len(rows), 32)], np.float32)
+        way = np.cumsum(parts, axis=0, dtype=np.float32)
+        assert np.abs(way).max() > 2 ** 24 - 2 ** 22 and np.any(way[-1] != sums[3])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,F,offset", [(256, 8, 0), (257, 8, 0), (1600, 64, 0), (4000, 8, 0), (4000, 36, 0), (4000, 301, 0), (20011, 12, 4), (20011, 12, 1),
+                                        (60000, 132, 0)])
+def test_flex16_sums_are_exact(n, F, offset):
+    import torch
+    from ngraph_python_b200 import lib
+    idx, delta, sums = _long_sums(n, F)
+    scales = torch.ones((3, 2), dtype=torch.float32, device="cuda")
+    x, d, out = torch.from_numpy(idx).cuda(), _off((n, F), torch.int16, offset), _off((11, F), torch.int16, offset)
+    d.copy_(torch.from_numpy(delta))
+    stats, probe = torch.zeros((3,), dtype=torch.int32, device="cuda"), torch.zeros((1,), dtype=torch.int64, device="cuda")
+    nbytes = lib.embed_update_scratch_bytes(11, F, n)
+    scratch = torch.full((nbytes,), 0x5A, dtype=torch.uint8, device="cuda")
+    for measure in (0, 1):
+        lib.check(lib.raw().b2_embed_update(d.data_ptr(), x.data_ptr(), out.data_ptr(), 1, 3, 11, F, n, 1.0, -1, 0, scales.data_ptr(), 0, 1, 2,
+                                            stats.data_ptr(), probe.data_ptr(), measure, scratch.data_ptr(), nbytes, 0))
+    torch.cuda.synchronize()
+    assert np.array_equal(out.cpu().numpy(), sums)
+    most = np.abs(sums).max()
+    assert stats.tolist() == [0, 0, most] and np.array([int(probe.item())], np.uint32).view(np.float32)[0] == most
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("dec", [2, 9])
 @pytest.mark.parametrize("n", [1, 31, 60, 257, 300])
