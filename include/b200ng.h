@@ -564,8 +564,8 @@ int b2_lut_update(const void* delta, const void* idx, void* dW, int32_t flex, in
 
 /* ------------------------------------------------------------------------------------------
  * Operators of a language model's training step.  No counterpart in the reference, whose lookup table
- * (above), batch normalisation and optimizers they stand beside.  Results and large operands must lie on the
- * current device (operands also in page-locked host memory), which is checked; a launch goes to `stream` of that device.
+ * (above), batch normalisation and optimizers they stand beside.  Results and operands must lie on the current
+ * device (operands also in page-locked host memory), which is checked; a launch goes to `stream` of that device.
  * Results have memory of their own except where an operator says otherwise.
  * ------------------------------------------------------------------------------------------ */
 /* how tokens are held: fp32 (which names every row up to 2^24), int32, int64, or flex16 mantissas with the exponent

@@ -796,6 +796,9 @@ extern "C" int b2_norm_fprop(const b2_norm* a, void* stream) {
     B2_CHECK(b2::require_read(a->residual, "the residual"));
     B2_CHECK(b2::require_read(a->block, "the block"));
     B2_CHECK(b2::require_read(a->gate, "the gate"));
+    for (const float* p : {a->block_rstd, a->stream_rstd})
+        if (p) B2_CHECK(b2::require_here(p, "a reciprocal deviation of the norm"));
+    for (const float* p : {a->post_weight, a->pre_weight}) B2_CHECK(b2::require_read(p, "a weight of the norm"));
     const unsigned blocks = (unsigned)(a->rows < (1ll << 30) ? a->rows : (1ll << 30));
     const int F = a->features;
     cudaStream_t st = (cudaStream_t)stream;
@@ -865,17 +868,24 @@ extern "C" int b2_norm_bprop(const b2_norm* a, const b2_norm_grads* d, void* scr
         B2_CHECK(check_apart(results, 5, operands, 9));
         B2_CHECK(check_in_place(a, d->d_residual, d->d_residual_stride, d->d_stream, d->d_stream_stride, "the residual's gradient"));
     }
+    // (sums over rows are written whatever the number of rows)
+    float* gate = a->gate_kind == B2_GATE_FEATURE ? d->d_gate : nullptr;
+    if (a->rows == 0) {
+        const void* results[] = {d->d_post_weight, d->d_pre_weight, gate};
+        B2_CHECK(check_apart(results, 3, nullptr, 0));
+    }
     B2_CHECK(b2::require_here(scratch, "the norm's scratch"));
+    for (const float* p : {d->d_pre_weight, d->d_post_weight, gate})
+        if (p) B2_CHECK(b2::require_here(p, "a gradient of the norm"));
     if (a->rows > 0) {
-        const void* written[] = {d->d_residual, d->d_block, d->d_gate, d->d_pre_weight, d->d_post_weight};
-        for (const void* p : written)
+        for (const float* p : {d->d_residual, d->d_block, gate ? nullptr : d->d_gate})
             if (p) B2_CHECK(b2::require_here(p, "a gradient of the norm"));
-        const void* read[] = {a->block ? a->stream : a->residual, a->block, a->gate, d->d_out, d->d_stream};
-        for (const void* p : read) B2_CHECK(b2::require_read(p, "an operand of the norm's gradient"));
+        const float* read[] = {a->block ? a->stream : a->residual, a->block, a->gate, a->post_weight, a->pre_weight,
+                               a->post_weight ? a->block_rstd : nullptr, a->pre_weight ? a->stream_rstd : nullptr, d->d_out, d->d_stream};
+        for (const float* p : read) B2_CHECK(b2::require_read(p, "an operand of the norm's gradient"));
     }
     cudaStream_t st = (cudaStream_t)stream;
     float* sums = (float*)(((uintptr_t)scratch + 255) / 256 * 256);
-    float* gate = a->gate_kind == B2_GATE_FEATURE ? d->d_gate : nullptr;
     const bool full = a->gate_kind == B2_GATE_FULL;
     const int tensors = (d->d_out ? 2 : 0) + (d->d_stream ? 1 : 0) + (a->block ? 1 : 0) + (full ? 1 : 0);
     const float* x = a->block ? a->stream : a->residual;

@@ -591,3 +591,50 @@ def test_host_memory_is_refused():
     lib.check(lib.raw().b2_norm_bprop(ctypes.byref(a), ctypes.byref(d), scratch.data_ptr(), scratch.numel(), 0))
     torch.cuda.synchronize()
     assert (host == 1).all()
+
+
+def test_sums_over_no_rows_in_one_place_are_refused():
+    from ngraph_python_b200 import lib
+    for pair in (("d_pre_weight", "d_post_weight"), ("d_gate", "d_pre_weight"), ("d_gate", "d_post_weight")):
+        a, d = _apart(**{pair[0]: pair[1]})
+        a.rows = 0
+        with pytest.raises(lib.B200Error, match="one place"):
+            lib.check(lib.raw().b2_norm_bprop(ctypes.byref(a), ctypes.byref(d), 256, 1 << 24, 0))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [0, 3])
+def test_vectors_in_host_memory_are_refused(rows):
+    """The reciprocal deviations, the weights, and sums over rows, which are written for no rows too."""
+    import torch
+    from ngraph_python_b200 import lib
+    F = 8
+    host = np.ones((64,), np.float32)
+    t = {k: torch.ones((4, F), device="cuda") for k in ("block", "residual", "gate", "post_weight", "pre_weight", "stream", "out", "block_rstd", "stream_rstd",
+                                                        "d_out", "d_stream", "d_residual", "d_block", "d_gate", "d_post_weight", "d_pre_weight")}
+    a, d = _whole()
+    a.rows = rows
+    for x in (a, d):
+        for k, v in t.items():
+            if hasattr(x, k):
+                setattr(x, k, v.data_ptr())
+    scratch = torch.zeros((lib.norm_bprop_scratch_bytes(a) + 256,), dtype=torch.uint8, device="cuda")
+    forward = lambda: lib.check(lib.raw().b2_norm_fprop(ctypes.byref(a), 0))  # noqa: E731
+    backward = lambda: lib.check(lib.raw().b2_norm_bprop(ctypes.byref(a), ctypes.byref(d), scratch.data_ptr(), scratch.numel(), 0))  # noqa: E731
+
+    def refused(call, x, name):
+        held = getattr(x, name)
+        setattr(x, name, host.ctypes.data)
+        with pytest.raises(lib.B200Error, match="memory"):
+            call()
+        setattr(x, name, held)
+    for name in ("d_post_weight", "d_pre_weight", "d_gate"):
+        refused(backward, d, name)
+    if rows:
+        for name in ("block_rstd", "stream_rstd", "post_weight", "pre_weight"):
+            refused(forward, a, name)
+            refused(backward, a, name)
+    forward()
+    backward()
+    torch.cuda.synchronize()
+    assert (host == 1).all()
