@@ -931,10 +931,20 @@ int launch_update(const void* delta, const void* idx, void* dW, int kind, int V,
 int check_flex(int flex, int kind, const FlexArgs& f) {
     B2_REQUIRE(kind >= B2_IDX_F32 && kind <= B2_IDX_FLEX16, "unknown kind of index: %d", kind);
     B2_REQUIRE(kind != B2_IDX_FLEX16 || (f.table && f.slot_idx >= 0), "a flex16 index needs the scale table");
+    B2_REQUIRE((!flex && kind != B2_IDX_FLEX16) || (uintptr_t)f.table % alignof(b2_flex_scale) == 0, "the scale table lies between two addresses");
     if (!flex) return B2_OK;
     B2_REQUIRE(f.table && f.slot_in >= 0 && f.slot_out >= 0, "a flex16 lookup needs the scale table");
     B2_REQUIRE(f.probe ? f.probe_out != nullptr : f.stats != nullptr, "missing statistics destination");
+    B2_REQUIRE((f.probe ? (uintptr_t)f.probe_out % 8 : (uintptr_t)f.stats % 4) == 0, "the statistics lie between two addresses");
     return B2_OK;
+}
+
+// Exponents that the kernels read, and the words that they keep the largest value in.
+int check_flex_memory(int flex, int kind, const FlexArgs& f) {
+    if (flex || kind == B2_IDX_FLEX16) B2_CHECK(b2::require_read(f.table, "the scale table"));
+    if (!flex) return B2_OK;
+    if (f.probe) return b2::require_here(f.probe_out, "the word of a measuring launch");
+    return b2::require_here(f.stats, "the statistics");
 }
 
 }  // namespace
@@ -962,6 +972,7 @@ extern "C" int b2_embed_fprop(const void* table, const void* idx, void* out, int
     B2_CHECK(b2::require_here(out, "the lookup's result"));
     B2_CHECK(b2::require_read(table, "the table"));
     B2_CHECK(b2::require_read(idx, "the index"));
+    B2_CHECK(check_flex_memory(flex, idx_kind, f));
     cudaStream_t st = (cudaStream_t)stream;
 #define B2_KIND(T)                                                                                                          \
     switch (idx_kind) {                                                                                                     \
@@ -996,6 +1007,7 @@ extern "C" int b2_embed_update(const void* delta, const void* idx, void* dW, int
     B2_CHECK(b2::require_here(scratch, "the scratch"));
     B2_CHECK(b2::require_read(n_idx ? delta : nullptr, "delta"));
     B2_CHECK(b2::require_read(n_idx ? idx : nullptr, "the index"));
+    B2_CHECK(check_flex_memory(flex, idx_kind, f));
     const int pad = pad_idx >= 0 && pad_idx < V ? (int)pad_idx : -1;
     void* at = (void*)(((uintptr_t)scratch + 255) / 256 * 256);
     if (flex) return launch_update<short>(delta, idx, dW, idx_kind, V, F, n_idx, scale, pad, onto, f, at, (cudaStream_t)stream);

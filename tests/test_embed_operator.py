@@ -460,3 +460,44 @@ def test_host_memory_is_refused():
     lib.check(lib.raw().b2_embed_fprop(pinned.data_ptr(), idx.data_ptr(), there.data_ptr(), 0, 0, 4, 4, 2, 1.0, *PLAIN, 0))
     torch.cuda.synchronize()
     assert torch.equal(there.cpu(), pinned[:1].expand(2, 4))
+
+
+def test_exponents_and_statistics_between_addresses_are_refused():
+    from ngraph_python_b200 import lib
+    raw = lib.raw()
+    for flex, kind, form in ((1, 3, (258, 0, 1, 2, 256, 256, 0)), (1, 0, (257, 0, 1, 2, 256, 256, 0)), (0, 3, (258, -1, 1, -1, None, None, 0)),
+                             (1, 3, (256, 0, 1, 2, 258, 256, 0)), (1, 3, (256, 0, 1, 2, 256, 260, 1))):
+        for call in (lambda: raw.b2_embed_fprop(1 << 20, 2 << 20, 3 << 20, flex, kind, 8, 4, 6, 1.0, *form, 0),
+                     lambda: raw.b2_embed_update(1 << 20, 2 << 20, 3 << 20, flex, kind, 8, 4, 6, 1.0, -1, 0, *form, 256, 1 << 20, 0)):
+            with pytest.raises(lib.B200Error, match="between two addresses"):
+                lib.check(call())
+
+
+@pytest.mark.gpu
+def test_exponents_and_statistics_in_host_memory_are_refused():
+    import torch
+    from ngraph_python_b200 import lib
+    raw = lib.raw()
+    table, idx, out = [torch.ones(s, dtype=torch.int16, device="cuda") for s in ((4, 4), (2,), (2, 4))]
+    host = np.zeros((64,), np.float32)
+    nbytes = lib.embed_update_scratch_bytes(4, 4, 2)
+    scratch = torch.zeros((nbytes,), dtype=torch.uint8, device="cuda")
+    good = dict(scales=torch.ones((3, 2), device="cuda"), stats=torch.zeros((3,), dtype=torch.int32, device="cuda"),
+                probe_out=torch.zeros((1,), dtype=torch.int64, device="cuda"))
+
+    def calls(probe, **moved):
+        at = {k: v.data_ptr() for k, v in good.items()}
+        at.update(moved)
+        form = (at["scales"], 0, 1, 2, at["stats"], at["probe_out"], probe)
+        return (lambda: raw.b2_embed_fprop(table.data_ptr(), idx.data_ptr(), out.data_ptr(), 1, 3, 4, 4, 2, 1.0, *form, 0),
+                lambda: raw.b2_embed_update(out.data_ptr(), idx.data_ptr(), table.data_ptr(), 1, 3, 4, 4, 2, 1.0, -1, 0, *form, scratch.data_ptr(), nbytes, 0))
+    for probe, name in ((0, "scales"), (1, "scales"), (0, "stats"), (1, "probe_out")):
+        for call in calls(probe, **{name: host.ctypes.data}):
+            with pytest.raises(lib.B200Error, match="memory"):
+                lib.check(call())
+    # (what is not read or written may be anything)
+    for probe, name in ((1, "stats"), (0, "probe_out")):
+        for call in calls(probe, **{name: None}):
+            lib.check(call())
+    torch.cuda.synchronize()
+    assert not host.any()
