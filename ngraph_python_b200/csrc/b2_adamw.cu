@@ -487,6 +487,9 @@ extern "C" int b2_adamw_step(void* plan, int64_t chunks, int32_t state_bits, con
                    std::isfinite(h->weight_decay) && std::isfinite(h->eps),
                "bad rates: lr %g, beta1 %g, beta2 %g, eps %g, weight decay %g", h->lr, h->beta1, h->beta2, h->eps, h->weight_decay);
     B2_CHECK(b2::require_here(step, "the number of the step"));
+    B2_CHECK(b2::require_here(plan, "the plan"));
+    B2_CHECK(b2::require_read(lr, "the rate"));
+    B2_CHECK(b2::require_read(grad_scale, "the scale of the gradients"));
     Rates r;
     r.b1 = (float)h->beta1;
     r.c1 = (float)(1.0 - h->beta1);

@@ -358,3 +358,28 @@ def test_a_plan_is_not_made_in_a_recording():
     graph.replay()
     torch.cuda.synchronize()
     assert float(x[0]) == 1
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_numbers_and_plans_in_host_memory_are_refused(bits):
+    import torch
+    from ngraph_python_b200 import lib
+    m = _Model([300, 5], bits)
+    host = np.full((4096,), 7.0, np.float32)
+    good = dict(plan=m.plan.data_ptr(), lr=None, scale=None, step=m.step_dev.data_ptr())
+
+    def step(**kw):
+        a = dict(good, **kw)
+        h = lib.AdamwHyper(*HYPER)
+        lib.check(lib.raw().b2_adamw_step(a["plan"], m.chunks, bits, ctypes.byref(h), a["lr"], a["scale"], a["step"], m.seed,
+                                          torch.cuda.current_stream().cuda_stream))
+    for name in good:
+        with pytest.raises(lib.B200Error, match="memory"):
+            step(**{name: host.ctypes.data})
+    # numbers in page-locked memory are read
+    numbers = torch.tensor([HYPER[0], 1.0]).pin_memory()
+    step(lr=numbers.data_ptr(), scale=numbers.data_ptr() + 4)
+    m.expect((float(np.float32(HYPER[0])),) + HYPER[1:])
+    m.check()
+    assert (host == 7).all()
