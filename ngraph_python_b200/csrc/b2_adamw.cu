@@ -411,6 +411,9 @@ static int check_apart(const b2_adamw_tensor* tensors, int32_t count, int32_t st
     return B2_OK;
 }
 
+// Addresses between two values would fault on the device.
+static bool whole(const void* p, size_t bytes) { return (uintptr_t)p % bytes == 0; }
+
 extern "C" int b2_adamw_plan_bytes(const b2_adamw_tensor* tensors, int32_t count, int32_t state_bits, size_t* bytes, int64_t* chunks) {
     B2_REQUIRE(bytes && chunks, "bad argument");
     long long n = 0;
@@ -431,6 +434,12 @@ extern "C" int b2_adamw_plan(const b2_adamw_tensor* tensors, int32_t count, int3
         B2_CHECK(check_apart(tensors, count, state_bits));
     } catch (const std::bad_alloc&) {
         return b2::fail(B2_ERR_INVALID, "no memory for a plan of %d tensors", count);
+    }
+    for (int i = 0; i < count; ++i) {
+        const b2_adamw_tensor& t = tensors[i];
+        if (t.n == 0) continue;
+        const bool states = state_bits == 32 ? whole(t.m, 4) && whole(t.v, 4) : whole(t.m_scales, 4) && whole(t.v_scales, 4);
+        B2_REQUIRE(whole(t.param, 4) && whole(t.grad, 4) && states, "tensor %d lies between two addresses", i);
     }
     B2_CHECK(b2::require_here(plan, "the plan"));
     for (int i = 0; i < count; ++i) {
@@ -486,6 +495,7 @@ extern "C" int b2_adamw_step(void* plan, int64_t chunks, int32_t state_bits, con
     B2_REQUIRE(h->beta1 >= 0.0 && h->beta1 < 1.0 && h->beta2 >= 0.0 && h->beta2 < 1.0 && h->eps >= 0.0 && std::isfinite(h->lr) &&
                    std::isfinite(h->weight_decay) && std::isfinite(h->eps),
                "bad rates: lr %g, beta1 %g, beta2 %g, eps %g, weight decay %g", h->lr, h->beta1, h->beta2, h->eps, h->weight_decay);
+    B2_REQUIRE(whole(step, 4) && whole(lr, 4) && whole(grad_scale, 4), "a number of the step lies between two addresses");
     B2_CHECK(b2::require_here(step, "the number of the step"));
     B2_CHECK(b2::require_here(plan, "the plan"));
     B2_CHECK(b2::require_read(lr, "the rate"));

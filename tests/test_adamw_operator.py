@@ -343,6 +343,32 @@ def test_tensors_that_overlap_are_refused(bits):
                 assert message(moved, to) == (overlap and not both_read), (moved, other, to - place[other])
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+def test_addresses_between_two_values_are_refused(bits):
+    from ngraph_python_b200 import lib
+    names = ("param", "grad", "m", "v") + (("m_scales", "v_scales") if bits == 8 else ())
+
+    def message(moved, by):
+        t = (lib.AdamwTensor * 2)()
+        for k in range(2):
+            t[k].n = 100
+            for j, name in enumerate(names):
+                setattr(t[k], name, (1 << 20) + 4096 * (8 * k + j) + (by if (k, name) == moved else 0))
+        with pytest.raises(lib.B200Error) as e:      # (addresses of nothing: refused in any case)
+            lib.adamw_plan(t, bits, 256, 1 << 20)
+        return str(e.value)
+    for moved in [(k, name) for k in range(2) for name in names]:
+        for by in (0, 1, 2, 3, 4, 8):
+            # (moments in 8 bits are bytes)
+            assert ("tensor %d lies between" % moved[0] in message(moved, by)) == (by % 4 != 0 and not (bits == 8 and moved[1] in "mv"))
+    h = lib.AdamwHyper(*HYPER)
+    for k in range(3):
+        at = [256, 512, 768]
+        at[k] += 2
+        with pytest.raises(lib.B200Error, match="between two addresses"):
+            lib.check(lib.raw().b2_adamw_step(4096, 1, bits, ctypes.byref(h), at[0], at[1], at[2], 0, 0))
+
+
 @pytest.mark.gpu
 def test_a_plan_is_not_made_in_a_recording():
     import torch
