@@ -379,14 +379,14 @@ int count_chunks(const b2_adamw_tensor* list, int count, int state_bits, long lo
 
 }  // namespace
 
-// Blocks write in any order: what one writes no other may read or write.
-static int check_apart(const b2_adamw_tensor* tensors, int32_t count, int32_t state_bits) {
+// Blocks write in any order: what one writes no other may read or write.  The plan holds addresses that are written to.
+static int check_apart(const b2_adamw_tensor* tensors, int32_t count, int32_t state_bits, const void* plan, size_t plan_bytes) {
     struct Range {
         uintptr_t from, to;
         bool operator<(const Range& o) const { return from < o.from; }
     };
-    std::vector<Range> written;
     const auto range = [](const void* p, size_t bytes) { return Range{(uintptr_t)p, (uintptr_t)p + bytes}; };
+    std::vector<Range> written = {range(plan, plan_bytes)};
     for (int i = 0; i < count; ++i) {
         const b2_adamw_tensor& t = tensors[i];
         if (t.n == 0) continue;
@@ -401,7 +401,7 @@ static int check_apart(const b2_adamw_tensor* tensors, int32_t count, int32_t st
     }
     std::sort(written.begin(), written.end());
     for (size_t k = 1; k < written.size(); ++k)
-        B2_REQUIRE(written[k - 1].to <= written[k].from, "tensors of the plan overlap");
+        B2_REQUIRE(written[k - 1].to <= written[k].from, "tensors of the plan overlap, or lie in its memory");
     for (int i = 0; i < count; ++i) {
         if (tensors[i].n == 0) continue;
         const Range g = range(tensors[i].grad, 4 * (size_t)tensors[i].n);
@@ -431,7 +431,7 @@ extern "C" int b2_adamw_plan(const b2_adamw_tensor* tensors, int32_t count, int3
     B2_CHECK(b2_adamw_plan_bytes(tensors, count, state_bits, &need, &chunks));
     B2_REQUIRE(plan && plan_bytes >= need, "the plan needs %zu bytes, got %zu", need, plan_bytes);
     try {
-        B2_CHECK(check_apart(tensors, count, state_bits));
+        B2_CHECK(check_apart(tensors, count, state_bits, plan, need));
     } catch (const std::bad_alloc&) {
         return b2::fail(B2_ERR_INVALID, "no memory for a plan of %d tensors", count);
     }

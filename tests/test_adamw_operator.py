@@ -344,6 +344,27 @@ def test_tensors_that_overlap_are_refused(bits):
 
 
 @pytest.mark.parametrize("bits", [32, 8])
+def test_a_plan_in_the_memory_of_a_tensor_is_refused(bits):
+    """A step would write over the addresses that it goes by."""
+    from ngraph_python_b200 import lib
+    names = ("param", "grad", "m", "v") + (("m_scales", "v_scales") if bits == 8 else ())
+    t = (lib.AdamwTensor * 1)()
+    t[0].n = 40000
+    size = dict.fromkeys(names, 160000)
+    if bits == 8:
+        size.update(m=40000, v=40000, m_scales=628, v_scales=628)
+    for k, name in enumerate(names):
+        setattr(t[0], name, (k + 1) << 20)
+    need, _ = lib.adamw_plan_bytes(t, bits)
+    for name in names:
+        at = getattr(t[0], name)
+        for plan, overlap in ((at, True), (at + size[name] - 4, True), (at + size[name], False), (at - need + 4, True), (at - need, False)):
+            with pytest.raises(lib.B200Error) as e:      # (addresses of nothing: refused in any case)
+                lib.adamw_plan(t, bits, plan, need)
+            assert ("overlap" in str(e.value)) == overlap
+
+
+@pytest.mark.parametrize("bits", [32, 8])
 def test_addresses_between_two_values_are_refused(bits):
     from ngraph_python_b200 import lib
     names = ("param", "grad", "m", "v") + (("m_scales", "v_scales") if bits == 8 else ())
