@@ -444,8 +444,8 @@ extern "C" int b2_adamw_plan(const b2_adamw_tensor* tensors, int32_t count, int3
     B2_CHECK(b2::require_here(plan, "the plan"));
     for (int i = 0; i < count; ++i) {
         if (tensors[i].n == 0) continue;
-        const float* ends[2] = {tensors[i].param, tensors[i].grad};
-        for (const float* p : ends) B2_CHECK(b2::require_here(p, "a tensor of the plan"));
+        B2_CHECK(b2::require_here(tensors[i].param, "a tensor of the plan"));
+        B2_CHECK(b2::require_read(tensors[i].grad, "a gradient of the plan"));
         B2_CHECK(b2::require_here(tensors[i].m, "a moment of the plan"));
         B2_CHECK(b2::require_here(tensors[i].v, "a moment of the plan"));
         if (state_bits == 8) {

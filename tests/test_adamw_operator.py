@@ -430,3 +430,29 @@ def test_numbers_and_plans_in_host_memory_are_refused(bits):
     m.expect((float(np.float32(HYPER[0])),) + HYPER[1:])
     m.check()
     assert (host == 7).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("offset", [0, 1])
+def test_gradients_in_page_locked_memory_are_read(bits, offset):
+    import torch
+    from ngraph_python_b200 import lib
+    m = _Model([5000, 7, 2048], bits, offset=offset, before=2)
+    held = []
+    for x, g in zip(m.tensors, m.grads):
+        t = torch.zeros((g[0].size + offset,)).pin_memory()
+        t[offset:] = torch.from_numpy(g[0])
+        held.append(t)
+        x.grad = t.data_ptr() + 4 * offset
+    lib.adamw_plan(m.tensors, bits, m.plan.data_ptr(), m.plan.numel(), torch.cuda.current_stream().cuda_stream)
+    m.launch()
+    m.expect()
+    m.check()
+    pageable, locked = np.zeros(5000, np.float32), torch.zeros((5000,)).pin_memory()
+    for name, data in (("grad", pageable.ctypes.data), ("param", locked.data_ptr())):
+        kept = getattr(m.tensors[0], name)
+        setattr(m.tensors[0], name, data)
+        with pytest.raises(lib.B200Error, match="memory"):
+            lib.adamw_plan(m.tensors, bits, m.plan.data_ptr(), m.plan.numel(), torch.cuda.current_stream().cuda_stream)
+        setattr(m.tensors[0], name, kept)
