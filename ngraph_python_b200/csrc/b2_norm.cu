@@ -693,6 +693,9 @@ int check_norm(const b2_norm* a) {
     B2_REQUIRE(a->rows >= 0 && a->features > 0 && a->features <= (1 << 24), "bad norm: %lld rows of %d features", (long long)a->rows, a->features);
     B2_REQUIRE(a->gate_kind >= B2_GATE_NONE && a->gate_kind <= B2_GATE_FULL, "unknown kind of gate: %d", a->gate_kind);
     B2_REQUIRE((a->gate_kind == B2_GATE_NONE) == (a->gate == nullptr), "a gate and its kind go together");
+    for (const float* p : {a->block, a->residual, a->gate, a->post_weight, a->pre_weight, (const float*)a->stream, (const float*)a->out,
+                           (const float*)a->block_rstd, (const float*)a->stream_rstd})
+        B2_REQUIRE(((uintptr_t)p & 3) == 0, "a tensor of the norm lies between two addresses");
     if (!a->block) B2_REQUIRE(!a->gate && !a->post_weight && a->residual_scale == 1.0f, "a gate, a weight or a scale without a block");
     return B2_OK;
 }
@@ -844,6 +847,9 @@ extern "C" int b2_norm_bprop(const b2_norm* a, const b2_norm_grads* d, void* scr
     size_t need = 0;
     B2_CHECK(b2_norm_bprop_scratch_bytes(a, &need));
     B2_REQUIRE(d, "missing argument");
+    for (const float* p : {d->d_out, d->d_stream, (const float*)d->d_residual, (const float*)d->d_block, (const float*)d->d_gate,
+                           (const float*)d->d_post_weight, (const float*)d->d_pre_weight})
+        B2_REQUIRE(((uintptr_t)p & 3) == 0, "a gradient of the norm lies between two addresses");
     B2_REQUIRE(scratch && scratch_bytes >= need, "the norm's gradient needs %zu bytes of scratch, got %zu", need, scratch_bytes);
     B2_REQUIRE(a->pre_weight ? d->d_out != nullptr || a->rows == 0 : d->d_out == nullptr && d->d_pre_weight == nullptr, "d_out and pre_weight go together");
     B2_REQUIRE(a->pre_weight || d->d_stream || a->rows == 0, "no gradient to start from");

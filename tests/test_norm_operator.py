@@ -638,3 +638,26 @@ def test_vectors_in_host_memory_are_refused(rows):
     backward()
     torch.cuda.synchronize()
     assert (host == 1).all()
+
+
+def test_addresses_between_two_values_are_refused():
+    from ngraph_python_b200 import lib
+    for rows in (0, 4):
+        for forward in (True, False):
+            a, d = _apart()
+            for x in (a, d) if not forward else (a,):
+                for k in [k for k, t in x._fields_ if t is ctypes.c_void_p]:
+                    for by in (1, 2, 3, 4):
+                        a, d = _apart()
+                        a.rows = rows
+                        y = a if type(x) is type(a) else d
+                        setattr(y, k, getattr(y, k) + by)
+                        call = lambda: lib.check(lib.raw().b2_norm_fprop(ctypes.byref(a), 0) if forward else  # noqa: E731
+                                                 lib.raw().b2_norm_bprop(ctypes.byref(a), ctypes.byref(d), 256, 1 << 24, 0))
+                        if by % 4:
+                            with pytest.raises(lib.B200Error, match="between two addresses"):
+                                call()
+                        elif rows or not forward:
+                            with pytest.raises(lib.B200Error) as e:      # (addresses of nothing: refused in any case)
+                                call()
+                            assert "between" not in str(e.value)
