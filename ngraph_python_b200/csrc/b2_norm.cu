@@ -796,8 +796,9 @@ extern "C" int b2_norm_fprop(const b2_norm* a, void* stream) {
     B2_CHECK(check_in_place(a, a->stream, a->stream_stride, a->residual, a->residual_stride, "the stream"));
     if (a->out) B2_CHECK(b2::require_here(a->out, "the norm's result"));
     if (a->stream) B2_CHECK(b2::require_here(a->stream, "the stream"));
-    B2_CHECK(b2::require_read(a->residual, "the residual"));
-    B2_CHECK(b2::require_read(a->block, "the block"));
+    bool elsewhere = false;
+    B2_CHECK(b2::require_read(a->residual, "the residual", &elsewhere));
+    B2_CHECK(b2::require_read(a->block, "the block", &elsewhere));
     B2_CHECK(b2::require_read(a->gate, "the gate"));
     for (const float* p : {a->block_rstd, a->stream_rstd})
         if (p) B2_CHECK(b2::require_here(p, "a reciprocal deviation of the norm"));
@@ -813,7 +814,8 @@ extern "C" int b2_norm_fprop(const b2_norm* a, void* stream) {
     auto alike = [&](const float* p, int64_t stride) {
         return !p || (shift_of(p) == shift_of(a->residual) && (a->rows <= 1 || (stride - a->residual_stride) % 4 == 0));
     };
-    const bool ragged = alike(a->block, a->block_stride) && alike(a->stream, a->stream_stride) && alike(a->out, a->out_stride) &&
+    // (rows fetched ahead are device memory)
+    const bool ragged = !elsewhere && alike(a->block, a->block_stride) && alike(a->stream, a->stream_stride) && alike(a->out, a->out_stride) &&
                         (a->gate_kind != B2_GATE_FULL || alike(a->gate, a->gate_stride));
     // Few rows: as many threads as a row has vectors, for the least latency.  Many: eight values to a thread, sixteen from
     // 2048 features on, so that several rows share an SM and the sums over the CTA weigh less (8192 x 4096: 100 us
@@ -874,6 +876,7 @@ extern "C" int b2_norm_bprop(const b2_norm* a, const b2_norm_grads* d, void* scr
         B2_CHECK(check_apart(results, 5, operands, 9));
         B2_CHECK(check_in_place(a, d->d_residual, d->d_residual_stride, d->d_stream, d->d_stream_stride, "the residual's gradient"));
     }
+    bool elsewhere = false;
     // (sums over rows are written whatever the number of rows)
     float* gate = a->gate_kind == B2_GATE_FEATURE ? d->d_gate : nullptr;
     if (a->rows == 0) {
@@ -888,7 +891,7 @@ extern "C" int b2_norm_bprop(const b2_norm* a, const b2_norm_grads* d, void* scr
             if (p) B2_CHECK(b2::require_here(p, "a gradient of the norm"));
         const float* read[] = {a->block ? a->stream : a->residual, a->block, a->gate, a->post_weight, a->pre_weight,
                                a->post_weight ? a->block_rstd : nullptr, a->pre_weight ? a->stream_rstd : nullptr, d->d_out, d->d_stream};
-        for (const float* p : read) B2_CHECK(b2::require_read(p, "an operand of the norm's gradient"));
+        for (const float* p : read) B2_CHECK(b2::require_read(p, "an operand of the norm's gradient", &elsewhere));
     }
     cudaStream_t st = (cudaStream_t)stream;
     float* sums = (float*)(((uintptr_t)scratch + 255) / 256 * 256);
@@ -909,7 +912,8 @@ extern "C" int b2_norm_bprop(const b2_norm* a, const b2_norm_grads* d, void* scr
                         (!full || (alike(a->gate, a->gate_stride) && alike(d->d_gate, d->d_gate_stride)));
     const GradPlan p = grad_plan(*a, tensors, ragged);
     if (p.ctas > 0) {
-        if (!p.threads || !d->d_out || !(vec || ragged)) B2_CUDA(b2::launch_after(vec ? norm_grad_any_kernel<4> : norm_grad_any_kernel<1>, dim3(p.ctas), kThreads, 0, st, *a, *d, sums));
+        // (bulk copies are from device memory alone)
+        if (!p.threads || !d->d_out || elsewhere || !(vec || ragged)) B2_CUDA(b2::launch_after(vec ? norm_grad_any_kernel<4> : norm_grad_any_kernel<1>, dim3(p.ctas), kThreads, 0, st, *a, *d, sums));
 #define B2_GRAD(MOST, EACH)                                                                                  \
     else if (p.most == MOST && p.each == EACH) {                                                             \
         if (vec) B2_CHECK((launch_grad_of<false, MOST, EACH / 4>(*a, *d, p, tensors, sums, st)));            \

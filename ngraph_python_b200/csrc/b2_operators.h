@@ -22,13 +22,17 @@ inline int require_here(const void* out, const char* what) {
     return B2_OK;
 }
 
-// The same of an operand, which may also lie in page-locked host memory.  (50 ns.)
-inline int require_read(const void* in, const char* what) {
+// The same of an operand, which may also lie in page-locked host memory; `elsewhere` is set where it is not device memory.
+// (50 ns.)
+inline int require_read(const void* in, const char* what, bool* elsewhere = nullptr) {
     if (!in) return B2_OK;
     cudaPointerAttributes a;
     B2_CUDA(cudaPointerGetAttributes(&a, in));
     B2_REQUIRE(a.type != cudaMemoryTypeUnregistered, "%s is not memory that the device reads", what);
-    if (a.type != cudaMemoryTypeDevice) return B2_OK;
+    if (a.type != cudaMemoryTypeDevice) {
+        if (elsewhere) *elsewhere = true;
+        return B2_OK;
+    }
     int now = 0;
     B2_CUDA(cudaGetDevice(&now));
     B2_REQUIRE(a.device == now, "%s lies on device %d, the current device is %d", what, a.device, now);

@@ -661,3 +661,48 @@ def test_addresses_between_two_values_are_refused():
                             with pytest.raises(lib.B200Error) as e:      # (addresses of nothing: refused in any case)
                                 call()
                             assert "between" not in str(e.value)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("gate", ["feature", "row", "full"])
+@pytest.mark.parametrize("rows,F", [(5, 64), (700, 37), (40, 2048), (6, 1001)])
+def test_operands_in_page_locked_memory(rows, F, gate):
+    """All of them at once, and the rows of one at a time."""
+    import torch
+    from ngraph_python_b200 import lib
+    rng = np.random.RandomState(4)
+    c = _case(rows, F, gate)
+    x, rstd, rho = _stored(c)
+    d_out, d_stream = [rng.standard_normal((rows, F)).astype(np.float32) for _ in range(2)]
+    host = dict(residual=c["residual"], block=c["block"], gate=c["gate"], post_weight=c["post"], pre_weight=c["pre"], stream=x, stream_rstd=rstd,
+                block_rstd=rho, d_out=d_out, d_stream=d_stream)
+    host = {k: torch.from_numpy(np.ascontiguousarray(v, dtype=np.float32)).pin_memory() for k, v in host.items()}
+    device = {k: v.cuda() for k, v in host.items()}
+    for locked in (tuple(host), ("residual",), ("block",), ("gate",), ("stream",), ("d_out",), ("d_stream",)):
+        at = {k: (host if k in locked else device)[k].data_ptr() for k in host}
+        a = lib.NormArgs(rows=rows, features=F, gate_kind=GATES[gate], residual_scale=c["a"], eps=1e-6)
+        for k in ("block", "residual", "gate", "stream", "out"):
+            setattr(a, k + "_stride", F)
+        for k in ("block", "residual", "gate", "post_weight", "pre_weight"):
+            setattr(a, k, at[k])
+        got = {k: torch.zeros(s, device="cuda") for k, s in (("stream", (rows, F)), ("out", (rows, F)), ("stream_rstd", (rows,)), ("block_rstd", (rows,)))}
+        for k, v in got.items():
+            setattr(a, k, v.data_ptr())
+        lib.check(lib.raw().b2_norm_fprop(ctypes.byref(a), 0))
+        torch.cuda.synchronize()
+        _check_forward({k: v.cpu().numpy() for k, v in got.items()}, c, F)
+        for k in ("stream", "stream_rstd", "block_rstd"):
+            setattr(a, k, at[k])
+        d = lib.NormGrads(d_out=at["d_out"], d_stream=at["d_stream"])
+        got = {k: torch.zeros(s, device="cuda") for k, s in (("d_residual", (rows, F)), ("d_block", (rows, F)), ("d_gate", c["gate"].shape),
+                                                            ("d_post_weight", (F,)), ("d_pre_weight", (F,)))}
+        for k in ("d_out", "d_stream", "d_residual", "d_block", "d_gate"):
+            setattr(d, k + "_stride", F)
+        for k, v in got.items():
+            setattr(d, k, v.data_ptr())
+        nbytes = lib.norm_bprop_scratch_bytes(a)
+        scratch = torch.full((nbytes,), 0xA5, dtype=torch.uint8, device="cuda")
+        lib.check(lib.raw().b2_norm_bprop(ctypes.byref(a), ctypes.byref(d), scratch.data_ptr(), nbytes, 0))
+        torch.cuda.synchronize()
+        names = dict(d_residual="residual", d_block="block", d_gate="gate", d_post_weight="post", d_pre_weight="pre")
+        _check_backward({names[k]: v.cpu().numpy() for k, v in got.items()}, c, x, rstd, rho, d_out, d_stream)
