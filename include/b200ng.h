@@ -603,8 +603,8 @@ int b2_embed_update(const void* delta, const void* idx, void* dW, int32_t flex, 
  *   out    = rms(stream) * pre_weight
  * block NULL: the stream is `residual` itself (residual_scale 1, no gate, no post_weight, stream NULL);
  * post_weight NULL: the block's result is not normalised; pre_weight and out NULL: the stream alone.
- * Tensors of rows have a stride in elements, at least `features` where there is more than one row.  `stream` may be
- * the memory of `residual`, with its stride.  block_rstd and stream_rstd [rows], where not NULL, receive
+ * Tensors of rows have a stride in elements, at least `features` where there is more than one row; rows of several may lie
+ * side by side, results that overlap are refused.  `stream` may be the memory of `residual`, with its stride.  block_rstd and stream_rstd [rows], where not NULL, receive
  * 1 / sqrt(mean + eps), which the gradients read.
  *   bprop: from d_out (NULL without pre_weight) and d_stream (NULL: zero), the gradients of all five operands; those
  *          that are NULL are not stored.  Reads stream (residual where there is no block) and the rstd's as fprop

@@ -9,6 +9,7 @@
 // Bound by memory: four tensors of rows forward, six for the gradients, each read or written once.  8192 x 4096: 86 us
 // forward, 0.96 of the rate of a copy, 134 us for the gradients, 0.92.  One row of 2048: 2.3 us in a graph.
 #include <cstdint>
+#include <utility>
 
 #include "b2_operators.h"
 #include "b2_ew_device.cuh"
@@ -690,7 +691,7 @@ GradPlan grad_plan(const b2_norm& a, int tensors, bool ragged) {
 
 int check_norm(const b2_norm* a) {
     B2_REQUIRE(a, "missing argument");
-    B2_REQUIRE(a->rows >= 0 && a->features > 0 && a->features <= (1 << 24), "bad norm: %lld rows of %d features", (long long)a->rows, a->features);
+    B2_REQUIRE(a->rows >= 0 && a->rows <= (1ll << 38) && a->features > 0 && a->features <= (1 << 24), "bad norm: %lld rows of %d features", (long long)a->rows, a->features);
     B2_REQUIRE(a->gate_kind >= B2_GATE_NONE && a->gate_kind <= B2_GATE_FULL, "unknown kind of gate: %d", a->gate_kind);
     B2_REQUIRE((a->gate_kind == B2_GATE_NONE) == (a->gate == nullptr), "a gate and its kind go together");
     for (const float* p : {a->block, a->residual, a->gate, a->post_weight, a->pre_weight, (const float*)a->stream, (const float*)a->out,
@@ -702,17 +703,57 @@ int check_norm(const b2_norm* a) {
 
 int check_stride(const b2_norm* a, const void* p, int64_t stride, const char* what) {
     B2_REQUIRE(!p || a->rows <= 1 || stride >= a->features, "rows of the %s overlap: stride %lld, %d features", what, (long long)stride, a->features);
+    B2_REQUIRE(!p || a->rows <= 1 || stride <= (1ll << 46) / a->rows, "%lld rows of the %s have no memory: stride %lld", (long long)a->rows, what,
+               (long long)stride);
     return B2_OK;
 }
 
-// (Rows of several tensors may lie side by side: tensors are told apart by where they begin.)
-int check_apart(const void* const* written, int count, const void* const* read, int reads) {
+// Rows of a tensor, in values.  Dense ones are one long row.
+struct Rows {
+    const float* p;
+    long long rows, width, stride;
+};
+Rows rows_at(const float* p, long long rows, long long width, long long stride) {
+    if (!p || rows <= 0) return {nullptr, 0, 0, 0};
+    if (rows == 1 || stride == width) return {p, 1, rows * width, rows * width};
+    return {p, rows, width, stride};
+}
+
+// Whether two tensors have memory in common.  Their rows may lie side by side.
+bool meet(Rows a, Rows b) {
+    if (!a.p || !b.p) return false;
+    if (a.rows > b.rows) std::swap(a, b);
+    const long long ahead = ((long long)(uintptr_t)b.p - (long long)(uintptr_t)a.p) / 4;     // where b begins, seen from a
+    if (ahead >= (a.rows - 1) * a.stride + a.width || -ahead >= (b.rows - 1) * b.stride + b.width) return false;
+    const auto below = [](long long x, long long y) { return x / y - (x % y < 0); };
+    if (a.stride == b.stride) {
+        // row i of a and row j of b meet where (i - j) stride lies between ahead - a.width and ahead + b.width
+        const long long least = below(ahead - a.width, a.stride) + 1, d = least > 1 - b.rows ? least : 1 - b.rows;
+        return d < a.rows && d * a.stride < ahead + b.width;
+    }
+    for (long long i = 0; i < a.rows; ++i) {
+        // the first row of b that does not end before row i of a begins
+        const long long from = i * a.stride - ahead, least = below(from - b.width, b.stride) + 1, j = least > 0 ? least : 0;
+        if (j < b.rows && j * b.stride < from + a.width) return true;
+    }
+    return false;
+}
+
+// Blocks write in any order: results have memory of their own.
+int check_apart(const Rows* written, int count, const Rows* read, int reads) {
     for (int i = 0; i < count; ++i) {
-        if (!written[i]) continue;
-        for (int k = 0; k < i; ++k) B2_REQUIRE(written[i] != written[k], "two results of the norm lie in one place");
-        for (int k = 0; k < reads; ++k) B2_REQUIRE(written[i] != read[k], "a result of the norm lies in the place of an operand");
+        if (!written[i].p) continue;
+        for (int k = 0; k < i; ++k) B2_REQUIRE(written[i].p != written[k].p, "two results of the norm lie in one place");
+        for (int k = 0; k < reads; ++k) B2_REQUIRE(written[i].p != read[k].p, "a result of the norm lies in the place of an operand");
+        for (int k = 0; k < i; ++k) B2_REQUIRE(!meet(written[i], written[k]), "two results of the norm overlap");
+        for (int k = 0; k < reads; ++k) B2_REQUIRE(!meet(written[i], read[k]), "a result of the norm overlaps an operand");
     }
     return B2_OK;
+}
+
+Rows gate_rows(const b2_norm& a, const float* p, long long stride) {
+    const long long R = a.rows, F = a.features;
+    return a.gate_kind == B2_GATE_FULL ? rows_at(p, R, F, stride) : a.gate_kind == B2_GATE_ROW ? rows_at(p, 1, R, R) : rows_at(p, 1, F, F);
 }
 
 int check_in_place(const b2_norm* a, const void* result, int64_t result_stride, const void* operand, int64_t stride, const char* what) {
@@ -790,8 +831,11 @@ extern "C" int b2_norm_fprop(const b2_norm* a, void* stream) {
     B2_CHECK(check_stride(a, a->stream, a->stream_stride, "stream"));
     B2_CHECK(check_stride(a, a->out, a->out_stride, "result"));
     if (a->gate_kind == B2_GATE_FULL) B2_CHECK(check_stride(a, a->gate, a->gate_stride, "gate"));
-    const void* results[] = {a->out, a->stream, a->block_rstd, a->stream_rstd};
-    const void* operands[] = {a->block, a->gate, a->post_weight, a->pre_weight, a->stream == a->residual ? nullptr : a->residual};
+    const long long R = a->rows, F = a->features;
+    const Rows results[] = {rows_at(a->out, R, F, a->out_stride), rows_at(a->stream, R, F, a->stream_stride), rows_at(a->block_rstd, 1, R, R),
+                            rows_at(a->stream_rstd, 1, R, R)};
+    const Rows operands[] = {rows_at(a->block, R, F, a->block_stride), gate_rows(*a, a->gate, a->gate_stride), rows_at(a->post_weight, 1, F, F),
+                             rows_at(a->pre_weight, 1, F, F), rows_at(a->stream == a->residual ? nullptr : a->residual, R, F, a->residual_stride)};
     B2_CHECK(check_apart(results, 4, operands, 5));
     B2_CHECK(check_in_place(a, a->stream, a->stream_stride, a->residual, a->residual_stride, "the stream"));
     if (a->out) B2_CHECK(b2::require_here(a->out, "the norm's result"));
@@ -804,7 +848,6 @@ extern "C" int b2_norm_fprop(const b2_norm* a, void* stream) {
         if (p) B2_CHECK(b2::require_here(p, "a reciprocal deviation of the norm"));
     for (const float* p : {a->post_weight, a->pre_weight}) B2_CHECK(b2::require_read(p, "a weight of the norm"));
     const unsigned blocks = (unsigned)(a->rows < (1ll << 30) ? a->rows : (1ll << 30));
-    const int F = a->features;
     cudaStream_t st = (cudaStream_t)stream;
     const bool vec = F % 4 == 0 && rows_aligned(a->block, a->block_stride) && rows_aligned(a->residual, a->residual_stride) &&
                      rows_aligned(a->stream, a->stream_stride) && rows_aligned(a->out, a->out_stride) &&
@@ -853,6 +896,7 @@ extern "C" int b2_norm_bprop(const b2_norm* a, const b2_norm_grads* d, void* scr
                            (const float*)d->d_post_weight, (const float*)d->d_pre_weight})
         B2_REQUIRE(((uintptr_t)p & 3) == 0, "a gradient of the norm lies between two addresses");
     B2_REQUIRE(scratch && scratch_bytes >= need, "the norm's gradient needs %zu bytes of scratch, got %zu", need, scratch_bytes);
+    const Rows room = {(const float*)(((uintptr_t)scratch + 3) / 4 * 4), 1, (long long)(need / 4), (long long)(need / 4)};      // (the sums of CTAs)
     B2_REQUIRE(a->pre_weight ? d->d_out != nullptr || a->rows == 0 : d->d_out == nullptr && d->d_pre_weight == nullptr, "d_out and pre_weight go together");
     B2_REQUIRE(a->pre_weight || d->d_stream || a->rows == 0, "no gradient to start from");
     B2_REQUIRE(a->block || (!d->d_block && !d->d_gate), "gradients of a block that is not there");
@@ -870,18 +914,23 @@ extern "C" int b2_norm_bprop(const b2_norm* a, const b2_norm_grads* d, void* scr
         B2_CHECK(check_stride(a, d->d_residual, d->d_residual_stride, "residual's gradient"));
         B2_CHECK(check_stride(a, d->d_block, d->d_block_stride, "block's gradient"));
         if (a->gate_kind == B2_GATE_FULL) B2_CHECK(check_stride(a, d->d_gate, d->d_gate_stride, "gate's gradient"));
-        const void* results[] = {d->d_residual, d->d_block, d->d_gate, d->d_post_weight, d->d_pre_weight};
-        const void* operands[] = {a->block ? a->stream : a->residual, a->block, a->gate, a->post_weight, a->pre_weight, d->d_out,
-                                  a->stream_rstd, a->block_rstd, d->d_stream == d->d_residual ? nullptr : d->d_stream};
-        B2_CHECK(check_apart(results, 5, operands, 9));
+        const long long R = a->rows, F = a->features;
+        const Rows results[] = {rows_at(d->d_residual, R, F, d->d_residual_stride), rows_at(d->d_block, R, F, d->d_block_stride),
+                                gate_rows(*a, d->d_gate, d->d_gate_stride), rows_at(d->d_post_weight, 1, F, F), rows_at(d->d_pre_weight, 1, F, F), room};
+        const Rows operands[] = {a->block ? rows_at(a->stream, R, F, a->stream_stride) : rows_at(a->residual, R, F, a->residual_stride),
+                                 rows_at(a->block, R, F, a->block_stride), gate_rows(*a, a->gate, a->gate_stride), rows_at(a->post_weight, 1, F, F),
+                                 rows_at(a->pre_weight, 1, F, F), rows_at(d->d_out, R, F, d->d_out_stride), rows_at(a->stream_rstd, 1, R, R),
+                                 rows_at(a->block_rstd, 1, R, R), rows_at(d->d_stream == d->d_residual ? nullptr : d->d_stream, R, F, d->d_stream_stride)};
+        B2_CHECK(check_apart(results, 6, operands, 9));
         B2_CHECK(check_in_place(a, d->d_residual, d->d_residual_stride, d->d_stream, d->d_stream_stride, "the residual's gradient"));
     }
     bool elsewhere = false;
     // (sums over rows are written whatever the number of rows)
     float* gate = a->gate_kind == B2_GATE_FEATURE ? d->d_gate : nullptr;
     if (a->rows == 0) {
-        const void* results[] = {d->d_post_weight, d->d_pre_weight, gate};
-        B2_CHECK(check_apart(results, 3, nullptr, 0));
+        const long long F = a->features;
+        const Rows results[] = {rows_at(d->d_post_weight, 1, F, F), rows_at(d->d_pre_weight, 1, F, F), rows_at(gate, 1, F, F), room};
+        B2_CHECK(check_apart(results, 4, nullptr, 0));
     }
     B2_CHECK(b2::require_here(scratch, "the norm's scratch"));
     for (const float* p : {d->d_pre_weight, d->d_post_weight, gate})

@@ -706,3 +706,56 @@ def test_operands_in_page_locked_memory(rows, F, gate):
         torch.cuda.synchronize()
         names = dict(d_residual="residual", d_block="block", d_gate="gate", d_post_weight="post", d_pre_weight="pre")
         _check_backward({names[k]: v.cpu().numpy() for k, v in got.items()}, c, x, rstd, rho, d_out, d_stream)
+
+
+def _held(base, rows, width, stride):
+    return set(base // 4 + i * stride + k for i in range(rows) for k in range(width))
+
+
+@pytest.mark.parametrize("forward", [True, False])
+def test_results_that_overlap_are_refused(forward):
+    """Two tensors at a time near one another, with strides of their own: refused where they share a value and one is
+    written, and not where their rows lie side by side."""
+    from ngraph_python_b200 import lib
+    rng = np.random.RandomState(3 + forward)
+    rowed = ("block", "residual", "gate", "stream", "out") if forward else ("block", "gate", "stream", "d_out", "d_stream", "d_residual", "d_block", "d_gate")
+    vectors = ("post_weight", "pre_weight", "block_rstd", "stream_rstd") + (() if forward else ("d_post_weight", "d_pre_weight"))
+    results = ("stream", "out", "block_rstd", "stream_rstd") if forward else ("d_residual", "d_block", "d_gate", "d_post_weight", "d_pre_weight")
+    seen = {True: 0, False: 0}
+    for _ in range(4000):
+        a, d = _apart()
+        a.gate_kind, a.features, a.rows = 3, int(rng.randint(1, 7)), int(rng.randint(1, 6))
+        F, R = a.features, a.rows
+        of = lambda k: a if hasattr(a, k) else d  # noqa: E731
+        strides = {k: int(F + rng.choice([0, 0, F, 2 * F, rng.randint(0, 9)])) for k in rowed}
+        if rng.rand() < 0.5:
+            strides = dict.fromkeys(rowed, strides[rowed[0]])
+        for k in rowed:
+            setattr(of(k), k + "_stride", strides[k])
+        x, y = [str(k) for k in rng.choice(rowed + vectors, 2, replace=False)]
+        if {x, y} in ({"residual", "stream"}, {"d_residual", "d_stream"}):
+            continue                                # (these may share memory; the strides then have to agree)
+        setattr(of(y), y, getattr(of(x), x) + 4 * int(rng.randint(-30, 31)))
+        held = [_held(getattr(of(k), k), R, F, strides[k]) if k in rowed else _held(getattr(of(k), k), 1, R if k.endswith("rstd") else F, 0) for k in (x, y)]
+        wrong = bool(held[0] & held[1]) and (x in results or y in results)
+        with pytest.raises(lib.B200Error) as e:      # (addresses of nothing: refused in any case)
+            lib.check(lib.raw().b2_norm_fprop(ctypes.byref(a), 0) if forward else
+                      lib.raw().b2_norm_bprop(ctypes.byref(a), ctypes.byref(d), 256, 1 << 24, 0))
+        text = str(e.value)
+        assert any(t in text for t in ("overlaps an operand", "norm overlap", "place")) == wrong, (x, y, text)
+        seen[wrong] += 1
+    assert min(seen.values()) > 500
+
+
+def test_a_scratch_that_overlaps_is_refused():
+    from ngraph_python_b200 import lib
+    for rows in (0, 4):
+        a, d = _apart()
+        a.rows = rows
+        need = lib.norm_bprop_scratch_bytes(a)
+        for k in ("d_post_weight", "d_pre_weight") + (("stream", "d_out", "d_residual", "block_rstd") if rows else ()):
+            at = getattr(a if hasattr(a, k) else d, k)
+            for scratch, overlaps in ((at - need + 8, True), (at, True), (at + 4, True), (at - need, False)):
+                with pytest.raises(lib.B200Error) as e:      # (addresses of nothing: refused in any case)
+                    lib.check(lib.raw().b2_norm_bprop(ctypes.byref(a), ctypes.byref(d), scratch, need, 0))
+                assert any(t in str(e.value) for t in ("overlap", "place")) == overlaps
