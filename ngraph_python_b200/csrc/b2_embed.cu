@@ -1003,6 +1003,10 @@ extern "C" int b2_embed_update(const void* delta, const void* idx, void* dW, int
     B2_REQUIRE(dW && (n_idx == 0 || (delta && idx)), "bad lookup gradient: missing tensor");
     B2_REQUIRE(scratch && scratch_bytes >= need, "the lookup's gradient needs %zu bytes of scratch, got %zu", need, scratch_bytes);
     B2_CHECK(check_memory(dW, V, delta, n_idx, F, idx, idx_kind, flex, true));
+    const size_t value = flex ? 2 : 4, token = idx_kind == B2_IDX_I64 ? 8 : idx_kind == B2_IDX_FLEX16 ? 2 : 4;
+    B2_REQUIRE(!b2::overlap(scratch, need, dW, (size_t)V * F * value) && !b2::overlap(scratch, need, delta, (size_t)n_idx * F * value) &&
+                   !b2::overlap(scratch, need, idx, (size_t)n_idx * token),
+               "the scratch overlaps a tensor of the lookup's gradient");
     B2_CHECK(b2::require_here(dW, "the table's gradient"));
     B2_CHECK(b2::require_here(scratch, "the scratch"));
     B2_CHECK(b2::require_read(n_idx ? delta : nullptr, "delta"));

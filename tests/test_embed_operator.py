@@ -462,6 +462,21 @@ def test_host_memory_is_refused():
     assert torch.equal(there.cpu(), pinned[:1].expand(2, 4))
 
 
+@pytest.mark.parametrize("n", [6, 600])
+@pytest.mark.parametrize("kind,flex", [(0, 0), (1, 0), (2, 0), (3, 1)])
+def test_a_scratch_that_overlaps_is_refused(kind, flex, n):
+    from ngraph_python_b200 import lib
+    value, token = (2, 2) if flex else (4, {0: 4, 1: 4, 2: 8}[kind])
+    form = (64, 0, 1, 2, 64, 64, 0) if flex else PLAIN
+    need = lib.embed_update_scratch_bytes(8, 4, n)
+    delta, idx, dW = 1 << 20, 2 << 20, 3 << 20
+    for at, size in ((delta, n * 4 * value), (idx, n * token), (dW, 32 * value)):
+        for scratch, there in ((at, True), (at + size - 1, True), (at + size, False), (at - need + 1, True), (at - need, False)):
+            with pytest.raises(lib.B200Error) as e:              # (addresses of nothing: refused in any case)
+                lib.check(lib.raw().b2_embed_update(delta, idx, dW, flex, kind, 8, 4, n, 1.0, -1, 0, *form, scratch, need, 0))
+            assert ("overlaps" in str(e.value)) == there
+
+
 def test_exponents_and_statistics_between_addresses_are_refused():
     from ngraph_python_b200 import lib
     raw = lib.raw()
