@@ -627,6 +627,7 @@ typedef struct {
     const float *d_out, *d_stream;
     float *d_residual, *d_block, *d_gate, *d_post_weight, *d_pre_weight;
     int64_t d_out_stride, d_stream_stride, d_residual_stride, d_block_stride, d_gate_stride;
+    int32_t* status; /* device word or NULL: set to 1 if a bounded wait of the kernel ran out, whose results are NaN then */
 } b2_norm_grads;
 int b2_norm_fprop(const b2_norm* norm, void* stream);
 int b2_norm_bprop_scratch_bytes(const b2_norm* norm, size_t* bytes);

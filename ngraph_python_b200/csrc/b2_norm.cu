@@ -279,7 +279,7 @@ norm_row_kernel(const b2_norm a) {
 // since between the loads of a row and its stores there are two sums over the CTA: the first pair (stream, d_out) of a
 // place is free again behind the first of them, the others behind the second.  Ragged rows: a CTA's are a multiple of four
 // apart and so lie alike; a copy starts at the 16-byte boundary below the row, and a thread's columns, whose sums it keeps,
-// are the vectors of memory.  (Value by value 3000 x 5001 took 83 us.)  A wait that runs out turns the results into NaN.
+// are the vectors of memory.  (Value by value 3000 x 5001 took 83 us.)
 constexpr int kStages = 3;
 constexpr int kGradShared = 226 << 10;      // (of 227 KB, with the static words)
 
@@ -287,11 +287,47 @@ struct Ring {
     int stages, slot;                   // bytes of one tensor's row, with room for its alignment
 };
 
+// Waits are bounded.  When one has run out, no thread of the CTA waits any more and thread 0 asks for no more rows; at the end
+// the CTA's results are spoiled.
+struct Waits {
+    unsigned long long first_full[kStages], then_full[kStages];
+    int ran_out;                        // 1: a wait has run out; 2, 3: of thread 0, for the first or the other tensors of row `stopped`
+    long long stopped;
+};
+
+// Sets *status and turns all results of the CTA's rows, and its sums, into NaN.  Copies that are still on their way are waited
+// for once more: the shared memory is another CTA's then.  (A call, which leaves the registers of the rows' loop alone: inlined,
+// 16384 x 2047 with a gate for a row took 180 us, 152 so.)
+__device__ __noinline__ void spoil_rows(const b2_norm& a, const b2_norm_grads& d, float* mine, Waits& waits, int stages, bool two) {
+    if (threadIdx.x == 0) {
+        // thread 0 asks for the tensors of the row `stages` ahead behind each of its two waits
+        const int rows = (int)((a.rows - 1 - blockIdx.x) / gridDim.x) + 1, at = (int)((waits.stopped - blockIdx.x) / gridDim.x) + stages;
+        for (int which = 0; waits.ran_out >= 2 && which < (two ? 2 : 1); ++which) {
+            const int asked = min(rows, at + (which == 0 && waits.ran_out == 3));
+            for (int n = max(0, asked - stages); n < asked; ++n) b2_mbar_wait((which ? waits.then_full : waits.first_full) + n % stages, n / stages & 1);
+        }
+        if (d.status) atomicExch(d.status, 1);
+    }
+    const float nan = __int_as_float(0x7fffffff);
+    const bool full = a.gate_kind == B2_GATE_FULL;
+    for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        for (int i = threadIdx.x; i < a.features; i += blockDim.x) {
+            if (d.d_residual) d.d_residual[row * d.d_residual_stride + i] = nan;
+            if (d.d_block) d.d_block[row * d.d_block_stride + i] = nan;
+            if (full && d.d_gate) d.d_gate[row * d.d_gate_stride + i] = nan;
+        }
+        if (a.gate_kind == B2_GATE_ROW && d.d_gate && threadIdx.x == 0) d.d_gate[row] = nan;
+    }
+    for (int i = threadIdx.x; i < 3 * a.features; i += blockDim.x) mine[i] = nan;
+    __syncthreads();
+}
+
+// (One CTA as the least: left to itself the assembler gives some of these so few registers that they spill.)
 template <bool RAGGED, int MOST, int IT, bool U, bool POST, int GATE>
-__global__ void __launch_bounds__(MOST)
-norm_grad_row_kernel(const b2_norm a, const b2_norm_grads d, float* __restrict__ out_sums, const Ring ring) {
+__global__ void __launch_bounds__(MOST, 1)
+norm_grad_row_kernel(const __grid_constant__ b2_norm a, const __grid_constant__ b2_norm_grads d, float* __restrict__ out_sums, const Ring ring) {
     extern __shared__ __align__(128) unsigned char shared[];
-    __shared__ unsigned long long first_full[kStages], then_full[kStages];
+    __shared__ Waits waits;
     __shared__ TwoSums sums;
     constexpr int VEC = 4;
     constexpr bool HOLD = IT == 2;              // weights stay in registers, in shared memory otherwise
@@ -306,10 +342,11 @@ norm_grad_row_kernel(const b2_norm a, const b2_norm_grads d, float* __restrict__
     const int F = a.features, tid = threadIdx.x, shift = RAGGED ? shift_of(xs + blockIdx.x * xs_stride) : 0, i0 = first_of<VEC, IT>() - shift;
     if (tid == 0) {
         for (int s = 0; s < ring.stages; ++s) {
-            b2_mbar_init(first_full + s, 1);
-            b2_mbar_init(then_full + s, 1);
+            b2_mbar_init(waits.first_full + s, 1);
+            b2_mbar_init(waits.then_full + s, 1);
         }
         b2_mbar_init_fence();
+        waits.ran_out = 0;
     }
     __syncthreads();
     after_earlier_kernels();
@@ -318,18 +355,18 @@ norm_grad_row_kernel(const b2_norm a, const b2_norm_grads d, float* __restrict__
     auto copy = [&](const float* p, int to, unsigned long long* bar) { b2_bulk_g2s(room + to, p - shift_of(p), bytes_of(p), bar); };
     auto fetch_first = [&](long long row, int s) {
         const float *x = xs + row * xs_stride, *dy = d.d_out + row * d.d_out_stride;
-        b2_mbar_expect_tx(first_full + s, bytes_of(x) + bytes_of(dy));
-        copy(x, s * stage_bytes, first_full + s);
-        copy(dy, s * stage_bytes + at_dy, first_full + s);
+        b2_mbar_expect_tx(waits.first_full + s, bytes_of(x) + bytes_of(dy));
+        copy(x, s * stage_bytes, waits.first_full + s);
+        copy(dy, s * stage_bytes + at_dy, waits.first_full + s);
     };
     auto fetch_then = [&](long long row, int s) {
         const float *ds = has_ds ? d.d_stream + row * d.d_stream_stride : nullptr, *u = U ? a.block + row * a.block_stride : nullptr,
                     *g = FULL ? a.gate + row * a.gate_stride : nullptr;
         if (!ds && !u && !g) return;
-        b2_mbar_expect_tx(then_full + s, (ds ? bytes_of(ds) : 0u) + (u ? bytes_of(u) : 0u) + (g ? bytes_of(g) : 0u));
-        if (ds) copy(ds, s * stage_bytes + at_ds, then_full + s);
-        if (u) copy(u, s * stage_bytes + at_u, then_full + s);
-        if (g) copy(g, s * stage_bytes + at_g, then_full + s);
+        b2_mbar_expect_tx(waits.then_full + s, (ds ? bytes_of(ds) : 0u) + (u ? bytes_of(u) : 0u) + (g ? bytes_of(g) : 0u));
+        if (ds) copy(ds, s * stage_bytes + at_ds, waits.then_full + s);
+        if (u) copy(u, s * stage_bytes + at_u, waits.then_full + s);
+        if (g) copy(g, s * stage_bytes + at_g, waits.then_full + s);
     };
     if (tid == 0)
         for (int s = 0; s < ring.stages; ++s) {
@@ -386,7 +423,13 @@ norm_grad_row_kernel(const b2_norm a, const b2_norm_grads d, float* __restrict__
     const float over = 1.0f / (float)F;
     int turn = 0, s = 0;
     unsigned phase = 0;
-    bool late = false;
+    auto wait = [&](unsigned long long* bar, long long row, bool first) {
+        if (b2_mbar_try_wait(bar, phase)) return;
+        for (int i = 0; i < (1 << 22) && *(volatile int*)&waits.ran_out == 0; ++i)
+            if (b2_mbar_try_wait(bar, phase)) return;
+        if (tid == 0 && waits.ran_out < 2) waits.stopped = row;
+        if (tid != 0 || waits.ran_out < 2) atomicMax(&waits.ran_out, tid != 0 ? 1 : first ? 2 : 3);
+    };
     for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
         const long long next = row + (long long)ring.stages * gridDim.x;
         const unsigned char* here = room + s * stage_bytes;
@@ -394,7 +437,7 @@ norm_grad_row_kernel(const b2_norm a, const b2_norm_grads d, float* __restrict__
         const float rho = a.stream_rstd[row], rho_u = POST ? a.block_rstd[row] : 1.0f;
         const float row_gate = GATE == B2_GATE_ROW ? a.gate[row] : 1.0f;
         {
-            late |= !b2_mbar_wait(first_full + s, phase);
+            wait(waits.first_full + s, row, true);
             const float *x = reinterpret_cast<const float*>(here) + shift, *dy = reinterpret_cast<const float*>(here + at_dy) + shift;
             float xh[IT][VEC];
             float q[1] = {0.0f};
@@ -416,14 +459,14 @@ norm_grad_row_kernel(const b2_norm a, const b2_norm_grads d, float* __restrict__
                 }
             }
             cta_sums(q, sums, turn);
-            if (tid == 0 && next < a.rows) fetch_first(next, s);
+            if (tid == 0 && next < a.rows && waits.ran_out < 2) fetch_first(next, s);
             const float mean = q[0] * over;
 #pragma unroll
             for (int k = 0; k < IT; ++k)
 #pragma unroll
                 for (int j = 0; j < VEC; ++j) t[k][j] = rho * fmaf(xh[k][j], -mean, t[k][j]);
         }
-        if (has_ds || U) late |= !b2_mbar_wait(then_full + s, phase);
+        if (has_ds || U) wait(waits.then_full + s, row, false);
         const float *ds = reinterpret_cast<const float*>(here + at_ds) + shift, *u = reinterpret_cast<const float*>(here + at_u) + shift,
                     *g = reinterpret_cast<const float*>(here + at_g) + shift;
         float uh[IT][VEC] = {};
@@ -438,9 +481,6 @@ norm_grad_row_kernel(const b2_norm a, const b2_norm_grads d, float* __restrict__
 #pragma unroll
                 for (int j = 0; j < VEC; ++j) t[k][j] += v[j];
             }
-            if (late)
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) t[k][j] = __int_as_float(0x7fffffff);
             if (d.d_residual) {
 #pragma unroll
                 for (int j = 0; j < VEC; ++j) v[j] = a.residual_scale * t[k][j];
@@ -479,7 +519,7 @@ norm_grad_row_kernel(const b2_norm a, const b2_norm_grads d, float* __restrict__
         } else {
             __syncthreads();
         }
-        if (tid == 0 && next < a.rows) fetch_then(next, s);
+        if (tid == 0 && next < a.rows && waits.ran_out < 2) fetch_then(next, s);
         if (GATE == B2_GATE_ROW && d.d_gate && tid == 0) d.d_gate[row] = dots[1];
         if (U && d.d_block) {
             const float mean = POST ? dots[0] * over : 0.0f;
@@ -517,6 +557,8 @@ norm_grad_row_kernel(const b2_norm a, const b2_norm_grads d, float* __restrict__
             if (FEATURE && d.d_gate) put<VEC>(mine + 2 * F + i, sum_gate[k]);
         }
     }
+    __syncthreads();
+    if (waits.ran_out) spoil_rows(a, d, mine, waits, ring.stages, has_ds || U);
 }
 
 // Rows of any length and alignment: a CTA adds its rows into sums of its own, [CTAs][3][F] of scratch.
@@ -895,6 +937,7 @@ extern "C" int b2_norm_bprop(const b2_norm* a, const b2_norm_grads* d, void* scr
     for (const float* p : {d->d_out, d->d_stream, (const float*)d->d_residual, (const float*)d->d_block, (const float*)d->d_gate,
                            (const float*)d->d_post_weight, (const float*)d->d_pre_weight})
         B2_REQUIRE(((uintptr_t)p & 3) == 0, "a gradient of the norm lies between two addresses");
+    B2_REQUIRE(((uintptr_t)d->status & 3) == 0, "the status lies between two addresses");
     B2_REQUIRE(scratch && scratch_bytes >= need, "the norm's gradient needs %zu bytes of scratch, got %zu", need, scratch_bytes);
     const Rows room = {(const float*)(((uintptr_t)scratch + 3) / 4 * 4), 1, (long long)(need / 4), (long long)(need / 4)};      // (the sums of CTAs)
     B2_REQUIRE(a->pre_weight ? d->d_out != nullptr || a->rows == 0 : d->d_out == nullptr && d->d_pre_weight == nullptr, "d_out and pre_weight go together");
@@ -933,6 +976,7 @@ extern "C" int b2_norm_bprop(const b2_norm* a, const b2_norm_grads* d, void* scr
         B2_CHECK(check_apart(results, 4, nullptr, 0));
     }
     B2_CHECK(b2::require_here(scratch, "the norm's scratch"));
+    if (d->status) B2_CHECK(b2::require_here(d->status, "the status"));
     for (const float* p : {d->d_pre_weight, d->d_post_weight, gate})
         if (p) B2_CHECK(b2::require_here(p, "a gradient of the norm"));
     if (a->rows > 0) {

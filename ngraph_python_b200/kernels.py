@@ -1131,6 +1131,7 @@ class NormGradStep(_Fp32Step):
         for k, v in self.found.items():
             setattr(d, "d_pre_weight" if k == "weight" else "d_" + k, self._ptr(v))
         d.d_residual_stride = d.d_block_stride = d.d_gate_stride = a.features
+        d.status = t._status.data_ptr()
         scratch = t._scratch_aligned()
         lib.check(lib.raw().b2_norm_bprop(C.byref(a), C.byref(d), scratch[0], scratch[1], t.stream.cuda_stream))
         t.kernel_launches += self.launches

@@ -119,7 +119,8 @@ class NormArgs(C.Structure):
 class NormGrads(C.Structure):
     _fields_ = [(f, C.c_void_p) for f in ("d_out", "d_stream", "d_residual", "d_block", "d_gate", "d_post_weight",
                                           "d_pre_weight")] + \
-        [(f, C.c_int64) for f in ("d_out_stride", "d_stream_stride", "d_residual_stride", "d_block_stride", "d_gate_stride")]
+        [(f, C.c_int64) for f in ("d_out_stride", "d_stream_stride", "d_residual_stride", "d_block_stride", "d_gate_stride")] + \
+        [("status", C.c_void_p)]
 
 
 class AdamwTensor(C.Structure):

@@ -388,3 +388,32 @@ def test_a_training_step_of_them_all(bits):
         if k == 1:
             comp.capture()
     t.close()
+
+
+@pytest.mark.gpu
+def test_the_norms_gradients_are_given_the_status_of_their_transformer(monkeypatch):
+    """A wait that runs out in them is an error of the call, as in the other kernels with bounded waits."""
+    from ngraph_python_b200 import lib
+    F, T = _axes(F=12, T=7)
+    x, d, w = ng.placeholder([T, F]), ng.placeholder([T, F]), ng.variable([F], initial_value=1)
+    t = _transformer()
+    comp = t.computation(ng.residual_norm_grad(ng.rms_norm(x, w, axes=[F]), d_out=d)["residual"], x, d)
+    raw, seen = lib.raw(), []
+
+    class Watched(object):
+        def __getattr__(self, name):
+            return getattr(raw, name)
+
+        def b2_norm_bprop(self, a, grads, *rest):
+            seen.append(grads._obj.status)
+            return raw.b2_norm_bprop(a, grads, *rest)
+    monkeypatch.setattr(lib, "raw", lambda: Watched())
+    v = np.ones((7, 12), np.float32)
+    comp(v, v)
+    assert seen == [t._status.data_ptr()]
+    # the word that such a wait sets
+    t._status.fill_(1)
+    with pytest.raises(lib.B200Error, match="wait ran out"):
+        comp(v, v)
+    comp(v, v)
+    t.close()

@@ -646,7 +646,7 @@ def test_addresses_between_two_values_are_refused():
         for forward in (True, False):
             a, d = _apart()
             for x in (a, d) if not forward else (a,):
-                for k in [k for k, t in x._fields_ if t is ctypes.c_void_p]:
+                for k in [k for k, t in x._fields_ if t is ctypes.c_void_p and k != "status"]:
                     for by in (1, 2, 3, 4):
                         a, d = _apart()
                         a.rows = rows
@@ -759,3 +759,44 @@ def test_a_scratch_that_overlaps_is_refused():
                 with pytest.raises(lib.B200Error) as e:      # (addresses of nothing: refused in any case)
                     lib.check(lib.raw().b2_norm_bprop(ctypes.byref(a), ctypes.byref(d), scratch, need, 0))
                 assert any(t in str(e.value) for t in ("overlap", "place")) == overlaps
+
+
+def test_a_status_between_addresses_is_refused():
+    from ngraph_python_b200 import lib
+    a, d = _apart()
+    d.status = 258
+    with pytest.raises(lib.B200Error, match="status lies between"):
+        lib.check(lib.raw().b2_norm_bprop(ctypes.byref(a), ctypes.byref(d), 256, 1 << 24, 0))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,F", [(3, 8), (700, 37), (900, 1001), (200, 8192)])
+def test_the_status_stays_as_it_is_where_no_wait_runs_out(rows, F):
+    import torch
+    from ngraph_python_b200 import lib
+    c = _case(rows, F, "row")
+    rng = np.random.RandomState(5)
+    x, rstd, rho = _stored(c)
+    rows_of = dict(block=c["block"], stream=x, d_out=rng.standard_normal((rows, F)), d_stream=rng.standard_normal((rows, F)))
+    t = {k: _vec(v) for k, v in dict(rows_of, gate=c["gate"], post_weight=c["post"], pre_weight=c["pre"], stream_rstd=rstd, block_rstd=rho).items()}
+    grads = {k: torch.zeros(s, device="cuda") for k, s in (("d_residual", (rows, F)), ("d_block", (rows, F)), ("d_gate", (rows,)), ("d_post_weight", (F,)),
+                                                          ("d_pre_weight", (F,)))}
+    status = torch.tensor([0, 0], dtype=torch.int32, device="cuda")
+    a, d = lib.NormArgs(rows=rows, features=F, gate_kind=2, residual_scale=c["a"], eps=1e-6), lib.NormGrads(status=status.data_ptr())
+    for y, held in ((a, t), (d, dict(t, **grads))):
+        for k, v in held.items():
+            if hasattr(y, k):
+                setattr(y, k, v.data_ptr())
+            if hasattr(y, k + "_stride"):
+                setattr(y, k + "_stride", F)
+    scratch = torch.zeros((lib.norm_bprop_scratch_bytes(a),), dtype=torch.uint8, device="cuda")
+    call = lambda: lib.check(lib.raw().b2_norm_bprop(ctypes.byref(a), ctypes.byref(d), scratch.data_ptr(), scratch.numel(), 0))  # noqa: E731
+    call()
+    torch.cuda.synchronize()
+    assert status.tolist() == [0, 0]
+    names = dict(d_residual="residual", d_block="block", d_gate="gate", d_post_weight="post", d_pre_weight="pre")
+    _check_backward({names[k]: v.cpu().numpy() for k, v in grads.items()}, c, x, rstd, rho, rows_of["d_out"].astype(np.float32),
+                    rows_of["d_stream"].astype(np.float32))
+    d.status = status.cpu().data_ptr()
+    with pytest.raises(lib.B200Error, match="memory"):
+        call()
