@@ -591,6 +591,7 @@ int b2_embed_fprop(const void* table, const void* idx, void* out, int32_t flex, 
                    int32_t slot_table, int32_t slot_idx, int32_t slot_out, int32_t* stats,
                    uint64_t* probe_out, int32_t probe, void* stream);
 int b2_embed_update_scratch_bytes(int32_t V, int32_t F, int64_t n_idx, size_t* bytes);
+int b2_embed_update_launches(int64_t n_idx, int32_t* launches);     /* kernels that an update of so many tokens launches */
 int b2_embed_update(const void* delta, const void* idx, void* dW, int32_t flex, int32_t idx_kind,
                     int32_t V, int32_t F, int64_t n_idx, float scale, int64_t pad_idx, int32_t onto,
                     const b2_flex_scale* scales, int32_t slot_delta, int32_t slot_idx, int32_t slot_dW,

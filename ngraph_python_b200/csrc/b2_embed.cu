@@ -992,6 +992,12 @@ extern "C" int b2_embed_update_scratch_bytes(int32_t V, int32_t F, int64_t n_idx
     return B2_OK;
 }
 
+extern "C" int b2_embed_update_launches(int64_t n_idx, int32_t* launches) {
+    B2_REQUIRE(launches && n_idx >= 0, "bad argument");
+    *launches = n_idx <= kSmall ? 1 : 2;
+    return B2_OK;
+}
+
 extern "C" int b2_embed_update(const void* delta, const void* idx, void* dW, int32_t flex, int32_t idx_kind, int32_t V, int32_t F, int64_t n_idx,
                                float scale, int64_t pad_idx, int32_t onto, const b2_flex_scale* scales, int32_t slot_delta, int32_t slot_idx,
                                int32_t slot_dW, int32_t* stats, uint64_t* probe_out, int32_t probe, void* scratch, size_t scratch_bytes, void* stream) {

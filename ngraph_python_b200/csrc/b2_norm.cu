@@ -836,7 +836,7 @@ int launch_rows(const b2_norm& a, int threads, cudaStream_t st) {
 }
 
 template <bool RAGGED, int MOST, int IT, bool U, bool POST, int GATE>
-int launch_grad(const b2_norm& a, const b2_norm_grads& d, const GradPlan& p, int tensors, float* sums, cudaStream_t st) {
+int launch_grad(const b2_norm& a, const b2_norm_grads& d, const GradPlan& p, float* sums, cudaStream_t st) {
     static std::atomic<unsigned long long> done{0};
     B2_CHECK(b2::allow_shared((const void*)norm_grad_row_kernel<RAGGED, MOST, IT, U, POST, GATE>, kGradShared, &done));
     B2_CUDA((b2::launch_after(norm_grad_row_kernel<RAGGED, MOST, IT, U, POST, GATE>, dim3(p.ctas), p.threads, (size_t)p.room, st, a, d,
@@ -845,14 +845,14 @@ int launch_grad(const b2_norm& a, const b2_norm_grads& d, const GradPlan& p, int
 }
 
 template <bool RAGGED, int MOST, int IT>
-int launch_grad_of(const b2_norm& a, const b2_norm_grads& d, const GradPlan& p, int tensors, float* sums, cudaStream_t st) {
-    if (!a.block) return launch_grad<RAGGED, MOST, IT, false, false, B2_GATE_NONE>(a, d, p, tensors, sums, st);
+int launch_grad_of(const b2_norm& a, const b2_norm_grads& d, const GradPlan& p, float* sums, cudaStream_t st) {
+    if (!a.block) return launch_grad<RAGGED, MOST, IT, false, false, B2_GATE_NONE>(a, d, p, sums, st);
 #define B2_GATED(POST)                                                                                               \
     switch (a.gate_kind) {                                                                                           \
-        case B2_GATE_FEATURE: return launch_grad<RAGGED, MOST, IT, true, POST, B2_GATE_FEATURE>(a, d, p, tensors, sums, st);  \
-        case B2_GATE_ROW: return launch_grad<RAGGED, MOST, IT, true, POST, B2_GATE_ROW>(a, d, p, tensors, sums, st);          \
-        case B2_GATE_FULL: return launch_grad<RAGGED, MOST, IT, true, POST, B2_GATE_FULL>(a, d, p, tensors, sums, st);        \
-        default: return launch_grad<RAGGED, MOST, IT, true, POST, B2_GATE_NONE>(a, d, p, tensors, sums, st);                  \
+        case B2_GATE_FEATURE: return launch_grad<RAGGED, MOST, IT, true, POST, B2_GATE_FEATURE>(a, d, p, sums, st);  \
+        case B2_GATE_ROW: return launch_grad<RAGGED, MOST, IT, true, POST, B2_GATE_ROW>(a, d, p, sums, st);          \
+        case B2_GATE_FULL: return launch_grad<RAGGED, MOST, IT, true, POST, B2_GATE_FULL>(a, d, p, sums, st);        \
+        default: return launch_grad<RAGGED, MOST, IT, true, POST, B2_GATE_NONE>(a, d, p, sums, st);                  \
     }
     if (a.post_weight) B2_GATED(true)
     B2_GATED(false)
@@ -1009,14 +1009,14 @@ extern "C" int b2_norm_bprop(const b2_norm* a, const b2_norm_grads* d, void* scr
         if (!p.threads || !d->d_out || elsewhere || !(vec || ragged)) B2_CUDA(b2::launch_after(vec ? norm_grad_any_kernel<4> : norm_grad_any_kernel<1>, dim3(p.ctas), kThreads, 0, st, *a, *d, sums));
 #define B2_GRAD(MOST, EACH)                                                                                  \
     else if (p.most == MOST && p.each == EACH) {                                                             \
-        if (vec) B2_CHECK((launch_grad_of<false, MOST, EACH / 4>(*a, *d, p, tensors, sums, st)));            \
-        else B2_CHECK((launch_grad_of<true, MOST, EACH / 4>(*a, *d, p, tensors, sums, st)));                 \
+        if (vec) B2_CHECK((launch_grad_of<false, MOST, EACH / 4>(*a, *d, p, sums, st)));            \
+        else B2_CHECK((launch_grad_of<true, MOST, EACH / 4>(*a, *d, p, sums, st)));                 \
     }
         B2_GRAD(512, 8)
         B2_GRAD(640, 8)
         B2_GRAD(512, 16)
-        else if (vec) B2_CHECK((launch_grad<false, 1024, 2, false, false, B2_GATE_NONE>(*a, *d, p, tensors, sums, st)));
-        else B2_CHECK((launch_grad<true, 1024, 2, false, false, B2_GATE_NONE>(*a, *d, p, tensors, sums, st)));
+        else if (vec) B2_CHECK((launch_grad<false, 1024, 2, false, false, B2_GATE_NONE>(*a, *d, p, sums, st)));
+        else B2_CHECK((launch_grad<true, 1024, 2, false, false, B2_GATE_NONE>(*a, *d, p, sums, st)));
 #undef B2_GRAD
     }
     if (d->d_pre_weight || d->d_post_weight || gate)

@@ -1020,7 +1020,6 @@ class EmbedStep(_Step):
 class EmbedGradStep(_Step):
     """Gradient of the table of a lookup with a scale, by sorted tokens."""
     kind = "embed_grad"
-    launches = 2
     probe_is_float = True
 
     def __init__(self, index, op, t):
@@ -1032,6 +1031,7 @@ class EmbedGradStep(_Step):
         pad = op.fprop.pad_idx
         self.pad_idx = -1 if pad is None else pad
         self.scratch_bytes = lib.embed_update_scratch_bytes(self.V, self.F, self.n)
+        self.launches = lib.embed_update_launches(self.n)
         self.flex = t.flex
         _check_index(op, t, self.V)
 
@@ -1107,13 +1107,14 @@ class NormStep(_Fp32Step):
 class NormGradStep(_Fp32Step):
     """All gradients of a NormStep."""
     kind = "norm_grad"
-    launches = 2
 
     def __init__(self, index, op, t, present):
         super(NormGradStep, self).__init__(index, op, t)
         self.views = {k: t._view_of(x) for k, x in op.reads.items()}
         self.in_views = list(self.views.values())
         self.found = self._results(op, t, present)
+        # (sums over rows are added by a second launch)
+        self.launches = 2 if set(self.found) & {"weight", "post_weight"} or ("gate" in self.found and op.fprop.gate_kind == 1) else 1
         a = _norm_args(op.fprop)
         for k in ("block", "gate", "post_weight", "weight"):          # (what the arguments are checked for)
             setattr(a, "pre_weight" if k == "weight" else k, 256 if k in op.reads else None)

@@ -242,6 +242,7 @@ def _load():
                                   vp, vp, i32, vp, vp, i32, vp]),
         "b2_embed_fprop": (C.c_int, [vp, vp, vp, i32, i32, i32, i32, i64, C.c_float, vp, i32, i32, i32, vp, vp, i32, vp]),
         "b2_embed_update_scratch_bytes": (C.c_int, [i32, i32, i64, C.POINTER(sz)]),
+        "b2_embed_update_launches": (C.c_int, [i64, C.POINTER(i32)]),
         "b2_embed_update": (C.c_int, [vp, vp, vp, i32, i32, i32, i32, i64, C.c_float, i64, i32, vp, i32, i32, i32, vp, vp,
                                       i32, vp, sz, vp]),
         "b2_norm_fprop": (C.c_int, [C.POINTER(NormArgs), vp]),
@@ -565,6 +566,12 @@ def embed_update_scratch_bytes(V, F, n):
     out = C.c_size_t()
     check(_lib.b2_embed_update_scratch_bytes(V, F, n, C.byref(out)))
     return int(out.value)
+
+
+def embed_update_launches(n):
+    out = C.c_int32()
+    check(_lib.b2_embed_update_launches(n, C.byref(out)))
+    return out.value
 
 
 def norm_bprop_scratch_bytes(norm):

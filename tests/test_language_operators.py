@@ -109,6 +109,34 @@ def test_gradients_that_are_variables_of_the_step_are_copied_first():
         assert not any(v is not None and v.buffer in written for v in step.gradients + step.numbers)
 
 
+def _gradient_steps(n, gate, which):
+    """A computation of the gradients named, over n tokens or rows, and what it has to be called with."""
+    V, F, T = _axes(V=40, F=8, T=n)
+    rng = np.random.RandomState(n)
+    table, idx, d, block = ng.variable([V, F], initial_value=1), ng.placeholder([T]), ng.placeholder([T, F]), ng.placeholder([T, F])
+    w = ng.variable([F], initial_value=1)
+    e = ng.embedding(table, idx)
+    if which is None:
+        return ng.embedding_grad(d, e), [idx, d], [rng.randint(0, 40, n), rng.standard_normal((n, 8))]
+    g = None if gate is None else ng.variable([dict(F=F, T=T)[k] for k in gate], initial_value=1)
+    stream, out = ng.residual_norm(e, block, w, axes=[F], gate=g, post_weight=w)
+    found = ng.residual_norm_grad(out, d_out=d)
+    return [found[k] for k in which], [idx, d, block], [rng.randint(0, 40, n)] + [rng.standard_normal((n, 8)) for _ in range(2)]
+
+
+LAUNCHES = [(1, None, None, 1), (256, None, None, 1), (257, None, None, 2), (9, None, ("residual", "block"), 1), (9, None, ("weight",), 2),
+            (9, None, ("post_weight",), 2), (9, "F", ("gate",), 2), (9, "T", ("gate", "residual"), 1), (9, "TF", ("gate",), 1)]
+
+
+@pytest.mark.parametrize("n,gate,which,launches", LAUNCHES)
+def test_launches_of_gradients(n, gate, which, launches):
+    op, args, _ = _gradient_steps(n, gate, which)
+    t = _transformer(plan_only=True)
+    comp = t.computation(op, *args)
+    t.initialize()
+    assert [s.launches for s in comp.steps if s.kind in ("embed_grad", "norm_grad")] == [launches]
+
+
 # ---- on the device -------------------------------------------------------------------------------------
 @pytest.mark.gpu
 @pytest.mark.parametrize("flex", [False, True])
@@ -416,4 +444,24 @@ def test_the_norms_gradients_are_given_the_status_of_their_transformer(monkeypat
     with pytest.raises(lib.B200Error, match="wait ran out"):
         comp(v, v)
     comp(v, v)
+    t.close()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,gate,which,launches", LAUNCHES)
+def test_launches_are_counted_as_they_are(n, gate, which, launches):
+    """Nodes of a recording of the step alone."""
+    import ctypes
+    import torch
+    op, args, values = _gradient_steps(n, gate, which)
+    t = _transformer()
+    comp = t.computation(op, *args)
+    comp(*values)
+    step, = [s for s in comp.steps if s.kind in ("embed_grad", "norm_grad")]
+    graph, nodes, before = torch.cuda.CUDAGraph(keep_graph=True), ctypes.c_size_t(), t.kernel_launches
+    with torch.cuda.graph(graph):
+        t._launch_step(step)
+    assert ctypes.CDLL("libcuda.so.1").cuGraphGetNodes(ctypes.c_void_p(graph.raw_cuda_graph()), None, ctypes.byref(nodes)) == 0
+    assert nodes.value == launches == step.launches == t.kernel_launches - before
+    del graph
     t.close()
