@@ -14,7 +14,11 @@
 // largest / 448.  v itself spans the square of what its root does, and e4m3 covers 2.3e5 : 1.  An average with
 // beta2 = 0.999 moves by at most 0.05 % of its root in a step downwards where e4m3's neighbours are 6 to 12 % apart: rounded to
 // nearest it would never come down.  Rounded at random to either neighbour, with the chance that makes the mean
-// right, it does, on the average.  A root that is not zero is not rounded to zero, which would leave m / eps.
+// right, it does, on the average.  That is the mean of m and of the root.  v is the root squared, and each rounding leaves
+// its variance there: a value that moves by d against a grid of distance D is rounded with a variance of about d D, d some
+// (1 - beta2) / 2 of the root and as much for the scale that the grid moves with, D 1/16 to 1/8 of it; over the 1 / (1 - beta2) steps that
+// the average remembers, 4 to 6 % of v, 1 % of a step's size.  A root that is not zero is not rounded to zero, which would
+// leave m / eps.
 #include <algorithm>
 #include <cmath>
 #include <cstdint>
