@@ -109,6 +109,28 @@ def test_gradients_that_are_variables_of_the_step_are_copied_first():
         assert not any(v is not None and v.buffer in written for v in step.gradients + step.numbers)
 
 
+def test_adamw_of_gradients_that_replicas_exchange():
+    """The step comes behind the exchanges of all its gradients, results of norms among them, and reads what they leave."""
+    class Two(object):
+        size, rank = 2, 0
+    V, F, T = _axes(V=50, F=8, T=16)
+    table, idx, w, d = ng.variable([V, F], initial_value=0), ng.placeholder([T]), ng.variable([F], initial_value=1), ng.placeholder([T, F])
+    e = ng.embedding(table, idx)
+    grads = ng.residual_norm_grad(ng.rms_norm(e, w, axes=[F]), d_out=d)
+    shared = [ng.allreduce(ng.embedding_grad(grads["residual"], e)), ng.allreduce(grads["weight"], "mean")]
+    t = _transformer(plan_only=True, comm=Two())
+    comp = t.computation(ng.adamw([table, w], shared, lr=0.1), idx, d)
+    t.initialize()
+    kinds = [s.kind for s in comp.steps]
+    assert sorted(kinds) == sorted(["embed", "norm", "norm_grad", "embed_grad", "comm", "comm", "adamw"]) and kinds[-1] == "adamw"
+    exchanges = [s for s in comp.steps if s.kind == "comm"]
+    assert set(v.buffer for v in comp.steps[-1].gradients) == set(s.arena_buffer for s in exchanges)
+    for s in exchanges:
+        made = [k for k, x in enumerate(comp.steps) if x.kind != "comm" and s.arena_buffer in [v.buffer for v in x.out_views]]
+        assert len(made) == 1 and made[0] < comp.steps.index(s)
+    assert sorted(s.reduce_func for s in exchanges) == ["mean", "sum"]
+
+
 def _gradient_steps(n, gate, which):
     """A computation of the gradients named, over n tokens or rows, and what it has to be called with."""
     V, F, T = _axes(V=40, F=8, T=n)
