@@ -445,16 +445,18 @@ extern "C" int b2_adamw_plan(const b2_adamw_tensor* tensors, int32_t count, int3
         const bool states = state_bits == 32 ? whole(t.m, 4) && whole(t.v, 4) : whole(t.m_scales, 4) && whole(t.v_scales, 4);
         B2_REQUIRE(whole(t.param, 4) && whole(t.grad, 4) && states, "tensor %d lies between two addresses", i);
     }
-    B2_CHECK(b2::require_here(plan, "the plan"));
+    b2::Memory memory;
+    B2_CHECK(memory.find_device());
+    B2_CHECK(memory.written(plan, "the plan"));
     for (int i = 0; i < count; ++i) {
         if (tensors[i].n == 0) continue;
-        B2_CHECK(b2::require_here(tensors[i].param, "a tensor of the plan"));
-        B2_CHECK(b2::require_read(tensors[i].grad, "a gradient of the plan"));
-        B2_CHECK(b2::require_here(tensors[i].m, "a moment of the plan"));
-        B2_CHECK(b2::require_here(tensors[i].v, "a moment of the plan"));
+        B2_CHECK(memory.written(tensors[i].param, "a tensor of the plan"));
+        B2_CHECK(memory.read(tensors[i].grad, "a gradient of the plan"));
+        B2_CHECK(memory.written(tensors[i].m, "a moment of the plan"));
+        B2_CHECK(memory.written(tensors[i].v, "a moment of the plan"));
         if (state_bits == 8) {
-            B2_CHECK(b2::require_here(tensors[i].m_scales, "the scales of a moment"));
-            B2_CHECK(b2::require_here(tensors[i].v_scales, "the scales of a moment"));
+            B2_CHECK(memory.written(tensors[i].m_scales, "the scales of a moment"));
+            B2_CHECK(memory.written(tensors[i].v_scales, "the scales of a moment"));
         }
     }
     cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
@@ -500,10 +502,12 @@ extern "C" int b2_adamw_step(void* plan, int64_t chunks, int32_t state_bits, con
                    std::isfinite(h->weight_decay) && std::isfinite(h->eps),
                "bad rates: lr %g, beta1 %g, beta2 %g, eps %g, weight decay %g", h->lr, h->beta1, h->beta2, h->eps, h->weight_decay);
     B2_REQUIRE(whole(step, 4) && whole(lr, 4) && whole(grad_scale, 4), "a number of the step lies between two addresses");
-    B2_CHECK(b2::require_here(step, "the number of the step"));
-    B2_CHECK(b2::require_here(plan, "the plan"));
-    B2_CHECK(b2::require_read(lr, "the rate"));
-    B2_CHECK(b2::require_read(grad_scale, "the scale of the gradients"));
+    b2::Memory memory;
+    B2_CHECK(memory.find_device());
+    B2_CHECK(memory.written(step, "the number of the step"));
+    B2_CHECK(memory.written(plan, "the plan"));
+    B2_CHECK(memory.read(lr, "the rate"));
+    B2_CHECK(memory.read(grad_scale, "the scale of the gradients"));
     Rates r;
     r.b1 = (float)h->beta1;
     r.c1 = (float)(1.0 - h->beta1);

@@ -940,11 +940,11 @@ int check_flex(int flex, int kind, const FlexArgs& f) {
 }
 
 // Exponents that the kernels read, and the words that they keep the largest value in.
-int check_flex_memory(int flex, int kind, const FlexArgs& f) {
-    if (flex || kind == B2_IDX_FLEX16) B2_CHECK(b2::require_read(f.table, "the scale table"));
+int check_flex_memory(b2::Memory& memory, int flex, int kind, const FlexArgs& f) {
+    if (flex || kind == B2_IDX_FLEX16) B2_CHECK(memory.read(f.table, "the scale table"));
     if (!flex) return B2_OK;
-    if (f.probe) return b2::require_here(f.probe_out, "the word of a measuring launch");
-    return b2::require_here(f.stats, "the statistics");
+    if (f.probe) return memory.written(f.probe_out, "the word of a measuring launch");
+    return memory.written(f.stats, "the statistics");
 }
 
 }  // namespace
@@ -969,10 +969,12 @@ extern "C" int b2_embed_fprop(const void* table, const void* idx, void* out, int
     if (n_idx == 0) return B2_OK;
     B2_REQUIRE(table && idx && out, "bad lookup: missing tensor");
     B2_CHECK(check_memory(table, V, out, n_idx, F, idx, idx_kind, flex, false));
-    B2_CHECK(b2::require_here(out, "the lookup's result"));
-    B2_CHECK(b2::require_read(table, "the table"));
-    B2_CHECK(b2::require_read(idx, "the index"));
-    B2_CHECK(check_flex_memory(flex, idx_kind, f));
+    b2::Memory memory;
+    B2_CHECK(memory.find_device());
+    B2_CHECK(memory.written(out, "the lookup's result"));
+    B2_CHECK(memory.read(table, "the table"));
+    B2_CHECK(memory.read(idx, "the index"));
+    B2_CHECK(check_flex_memory(memory, flex, idx_kind, f));
     cudaStream_t st = (cudaStream_t)stream;
 #define B2_KIND(T)                                                                                                          \
     switch (idx_kind) {                                                                                                     \
@@ -1013,11 +1015,13 @@ extern "C" int b2_embed_update(const void* delta, const void* idx, void* dW, int
     B2_REQUIRE(!b2::overlap(scratch, need, dW, (size_t)V * F * value) && !b2::overlap(scratch, need, delta, (size_t)n_idx * F * value) &&
                    !b2::overlap(scratch, need, idx, (size_t)n_idx * token),
                "the scratch overlaps a tensor of the lookup's gradient");
-    B2_CHECK(b2::require_here(dW, "the table's gradient"));
-    B2_CHECK(b2::require_here(scratch, "the scratch"));
-    B2_CHECK(b2::require_read(n_idx ? delta : nullptr, "delta"));
-    B2_CHECK(b2::require_read(n_idx ? idx : nullptr, "the index"));
-    B2_CHECK(check_flex_memory(flex, idx_kind, f));
+    b2::Memory memory;
+    B2_CHECK(memory.find_device());
+    B2_CHECK(memory.written(dW, "the table's gradient"));
+    B2_CHECK(memory.written(scratch, "the scratch"));
+    B2_CHECK(memory.read(n_idx ? delta : nullptr, "delta"));
+    B2_CHECK(memory.read(n_idx ? idx : nullptr, "the index"));
+    B2_CHECK(check_flex_memory(memory, flex, idx_kind, f));
     const int pad = pad_idx >= 0 && pad_idx < V ? (int)pad_idx : -1;
     void* at = (void*)(((uintptr_t)scratch + 255) / 256 * 256);
     if (flex) return launch_update<short>(delta, idx, dW, idx_kind, V, F, n_idx, scale, pad, onto, f, at, (cudaStream_t)stream);

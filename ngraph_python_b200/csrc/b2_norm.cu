@@ -752,21 +752,19 @@ int check_stride(const b2_norm* a, const void* p, int64_t stride, const char* wh
 
 // Rows of a tensor, in values.  Dense ones are one long row.
 struct Rows {
-    const float* p;
+    const float *p, *end;
     long long rows, width, stride;
 };
-Rows rows_at(const float* p, long long rows, long long width, long long stride) {
-    if (!p || rows <= 0) return {nullptr, 0, 0, 0};
-    if (rows == 1 || stride == width) return {p, 1, rows * width, rows * width};
-    return {p, rows, width, stride};
+inline Rows rows_at(const float* p, long long rows, long long width, long long stride) {
+    if (!p || rows <= 0) return {nullptr, nullptr, 0, 0, 0};
+    if (rows == 1 || stride == width) return {p, p + rows * width, 1, rows * width, rows * width};
+    return {p, p + ((rows - 1) * stride + width), rows, width, stride};
 }
 
-// Whether two tensors have memory in common.  Their rows may lie side by side.
+// Whether two tensors that lie among one another have memory in common.  Their rows may lie side by side.
 bool meet(Rows a, Rows b) {
-    if (!a.p || !b.p) return false;
     if (a.rows > b.rows) std::swap(a, b);
     const long long ahead = ((long long)(uintptr_t)b.p - (long long)(uintptr_t)a.p) / 4;     // where b begins, seen from a
-    if (ahead >= (a.rows - 1) * a.stride + a.width || -ahead >= (b.rows - 1) * b.stride + b.width) return false;
     const auto below = [](long long x, long long y) { return x / y - (x % y < 0); };
     if (a.stride == b.stride) {
         // row i of a and row j of b meet where (i - j) stride lies between ahead - a.width and ahead + b.width
@@ -783,17 +781,25 @@ bool meet(Rows a, Rows b) {
 
 // Blocks write in any order: results have memory of their own.
 int check_apart(const Rows* written, int count, const Rows* read, int reads) {
+    const auto apart = [](const Rows& a, const Rows& b) { return (uintptr_t)a.end <= (uintptr_t)b.p || (uintptr_t)b.end <= (uintptr_t)a.p; };
     for (int i = 0; i < count; ++i) {
-        if (!written[i].p) continue;
-        for (int k = 0; k < i; ++k) B2_REQUIRE(written[i].p != written[k].p, "two results of the norm lie in one place");
-        for (int k = 0; k < reads; ++k) B2_REQUIRE(written[i].p != read[k].p, "a result of the norm lies in the place of an operand");
-        for (int k = 0; k < i; ++k) B2_REQUIRE(!meet(written[i], written[k]), "two results of the norm overlap");
-        for (int k = 0; k < reads; ++k) B2_REQUIRE(!meet(written[i], read[k]), "a result of the norm overlaps an operand");
+        const Rows& w = written[i];
+        if (!w.p) continue;
+        for (int k = 0; k < i; ++k)
+            if (!apart(w, written[k])) {
+                B2_REQUIRE(w.p != written[k].p, "two results of the norm lie in one place");
+                B2_REQUIRE(!meet(w, written[k]), "two results of the norm overlap");
+            }
+        for (int k = 0; k < reads; ++k)
+            if (!apart(w, read[k])) {
+                B2_REQUIRE(w.p != read[k].p, "a result of the norm lies in the place of an operand");
+                B2_REQUIRE(!meet(w, read[k]), "a result of the norm overlaps an operand");
+            }
     }
     return B2_OK;
 }
 
-Rows gate_rows(const b2_norm& a, const float* p, long long stride) {
+inline Rows gate_rows(const b2_norm& a, const float* p, long long stride) {
     const long long R = a.rows, F = a.features;
     return a.gate_kind == B2_GATE_FULL ? rows_at(p, R, F, stride) : a.gate_kind == B2_GATE_ROW ? rows_at(p, 1, R, R) : rows_at(p, 1, F, F);
 }
@@ -880,15 +886,16 @@ extern "C" int b2_norm_fprop(const b2_norm* a, void* stream) {
                              rows_at(a->pre_weight, 1, F, F), rows_at(a->stream == a->residual ? nullptr : a->residual, R, F, a->residual_stride)};
     B2_CHECK(check_apart(results, 4, operands, 5));
     B2_CHECK(check_in_place(a, a->stream, a->stream_stride, a->residual, a->residual_stride, "the stream"));
-    if (a->out) B2_CHECK(b2::require_here(a->out, "the norm's result"));
-    if (a->stream) B2_CHECK(b2::require_here(a->stream, "the stream"));
-    bool elsewhere = false;
-    B2_CHECK(b2::require_read(a->residual, "the residual", &elsewhere));
-    B2_CHECK(b2::require_read(a->block, "the block", &elsewhere));
-    B2_CHECK(b2::require_read(a->gate, "the gate"));
+    b2::Memory memory;
+    B2_CHECK(memory.find_device());
+    if (a->out) B2_CHECK(memory.written(a->out, "the norm's result"));
+    if (a->stream) B2_CHECK(memory.written(a->stream, "the stream"));
     for (const float* p : {a->block_rstd, a->stream_rstd})
-        if (p) B2_CHECK(b2::require_here(p, "a reciprocal deviation of the norm"));
-    for (const float* p : {a->post_weight, a->pre_weight}) B2_CHECK(b2::require_read(p, "a weight of the norm"));
+        if (p) B2_CHECK(memory.written(p, "a reciprocal deviation of the norm"));
+    for (const float* p : {a->post_weight, a->pre_weight}) B2_CHECK(memory.read(p, "a weight of the norm"));
+    B2_CHECK(memory.read(a->gate, "the gate"));
+    B2_CHECK(memory.read(a->residual, "the residual"));
+    B2_CHECK(memory.read(a->block, "the block"));
     const unsigned blocks = (unsigned)(a->rows < (1ll << 30) ? a->rows : (1ll << 30));
     cudaStream_t st = (cudaStream_t)stream;
     const bool vec = F % 4 == 0 && rows_aligned(a->block, a->block_stride) && rows_aligned(a->residual, a->residual_stride) &&
@@ -900,7 +907,7 @@ extern "C" int b2_norm_fprop(const b2_norm* a, void* stream) {
         return !p || (shift_of(p) == shift_of(a->residual) && (a->rows <= 1 || (stride - a->residual_stride) % 4 == 0));
     };
     // (rows fetched ahead are device memory)
-    const bool ragged = !elsewhere && alike(a->block, a->block_stride) && alike(a->stream, a->stream_stride) && alike(a->out, a->out_stride) &&
+    const bool ragged = !memory.elsewhere && alike(a->block, a->block_stride) && alike(a->stream, a->stream_stride) && alike(a->out, a->out_stride) &&
                         (a->gate_kind != B2_GATE_FULL || alike(a->gate, a->gate_stride));
     // Few rows: as many threads as a row has vectors, for the least latency.  Many: eight values to a thread, sixteen from
     // 2048 features on, so that several rows share an SM and the sums over the CTA weigh less (8192 x 4096: 100 us
@@ -939,7 +946,7 @@ extern "C" int b2_norm_bprop(const b2_norm* a, const b2_norm_grads* d, void* scr
         B2_REQUIRE(((uintptr_t)p & 3) == 0, "a gradient of the norm lies between two addresses");
     B2_REQUIRE(((uintptr_t)d->status & 3) == 0, "the status lies between two addresses");
     B2_REQUIRE(scratch && scratch_bytes >= need, "the norm's gradient needs %zu bytes of scratch, got %zu", need, scratch_bytes);
-    const Rows room = {(const float*)(((uintptr_t)scratch + 3) / 4 * 4), 1, (long long)(need / 4), (long long)(need / 4)};      // (the sums of CTAs)
+    const Rows room = rows_at((const float*)(((uintptr_t)scratch + 3) / 4 * 4), 1, (long long)(need / 4), (long long)(need / 4));     // (the sums of CTAs)
     B2_REQUIRE(a->pre_weight ? d->d_out != nullptr || a->rows == 0 : d->d_out == nullptr && d->d_pre_weight == nullptr, "d_out and pre_weight go together");
     B2_REQUIRE(a->pre_weight || d->d_stream || a->rows == 0, "no gradient to start from");
     B2_REQUIRE(a->block || (!d->d_block && !d->d_gate), "gradients of a block that is not there");
@@ -967,7 +974,6 @@ extern "C" int b2_norm_bprop(const b2_norm* a, const b2_norm_grads* d, void* scr
         B2_CHECK(check_apart(results, 6, operands, 9));
         B2_CHECK(check_in_place(a, d->d_residual, d->d_residual_stride, d->d_stream, d->d_stream_stride, "the residual's gradient"));
     }
-    bool elsewhere = false;
     // (sums over rows are written whatever the number of rows)
     float* gate = a->gate_kind == B2_GATE_FEATURE ? d->d_gate : nullptr;
     if (a->rows == 0) {
@@ -975,16 +981,18 @@ extern "C" int b2_norm_bprop(const b2_norm* a, const b2_norm_grads* d, void* scr
         const Rows results[] = {rows_at(d->d_post_weight, 1, F, F), rows_at(d->d_pre_weight, 1, F, F), rows_at(gate, 1, F, F), room};
         B2_CHECK(check_apart(results, 4, nullptr, 0));
     }
-    B2_CHECK(b2::require_here(scratch, "the norm's scratch"));
-    if (d->status) B2_CHECK(b2::require_here(d->status, "the status"));
+    b2::Memory memory;
+    B2_CHECK(memory.find_device());
+    B2_CHECK(memory.written(scratch, "the norm's scratch"));
+    if (d->status) B2_CHECK(memory.written(d->status, "the status"));
     for (const float* p : {d->d_pre_weight, d->d_post_weight, gate})
-        if (p) B2_CHECK(b2::require_here(p, "a gradient of the norm"));
+        if (p) B2_CHECK(memory.written(p, "a gradient of the norm"));
     if (a->rows > 0) {
         for (const float* p : {d->d_residual, d->d_block, gate ? nullptr : d->d_gate})
-            if (p) B2_CHECK(b2::require_here(p, "a gradient of the norm"));
+            if (p) B2_CHECK(memory.written(p, "a gradient of the norm"));
         const float* read[] = {a->block ? a->stream : a->residual, a->block, a->gate, a->post_weight, a->pre_weight,
                                a->post_weight ? a->block_rstd : nullptr, a->pre_weight ? a->stream_rstd : nullptr, d->d_out, d->d_stream};
-        for (const float* p : read) B2_CHECK(b2::require_read(p, "an operand of the norm's gradient", &elsewhere));
+        for (const float* p : read) B2_CHECK(memory.read(p, "an operand of the norm's gradient"));
     }
     cudaStream_t st = (cudaStream_t)stream;
     float* sums = (float*)(((uintptr_t)scratch + 255) / 256 * 256);
@@ -1006,7 +1014,7 @@ extern "C" int b2_norm_bprop(const b2_norm* a, const b2_norm_grads* d, void* scr
     const GradPlan p = grad_plan(*a, tensors, ragged);
     if (p.ctas > 0) {
         // (bulk copies are from device memory alone)
-        if (!p.threads || !d->d_out || elsewhere || !(vec || ragged)) B2_CUDA(b2::launch_after(vec ? norm_grad_any_kernel<4> : norm_grad_any_kernel<1>, dim3(p.ctas), kThreads, 0, st, *a, *d, sums));
+        if (!p.threads || !d->d_out || memory.elsewhere || !(vec || ragged)) B2_CUDA(b2::launch_after(vec ? norm_grad_any_kernel<4> : norm_grad_any_kernel<1>, dim3(p.ctas), kThreads, 0, st, *a, *d, sums));
 #define B2_GRAD(MOST, EACH)                                                                                  \
     else if (p.most == MOST && p.each == EACH) {                                                             \
         if (vec) B2_CHECK((launch_grad_of<false, MOST, EACH / 4>(*a, *d, p, sums, st)));            \

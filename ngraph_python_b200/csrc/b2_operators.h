@@ -10,34 +10,36 @@ namespace b2 {
 
 constexpr int kSms = 148;
 
-// Launches go to the current device.  A result that lies on another one, or on the host, is refused:
-// the kernel would fault, or write across the link.
-inline int require_here(const void* out, const char* what) {
-    int now = 0;
-    B2_CUDA(cudaGetDevice(&now));
-    cudaPointerAttributes a;
-    B2_CUDA(cudaPointerGetAttributes(&a, out));
-    B2_REQUIRE(a.type == cudaMemoryTypeDevice || a.type == cudaMemoryTypeManaged, "%s is not device memory", what);
-    B2_REQUIRE(a.type != cudaMemoryTypeDevice || a.device == now, "%s lies on device %d, the current device is %d", what, a.device, now);
-    return B2_OK;
-}
-
-// The same of an operand, which may also lie in page-locked host memory; `elsewhere` is set where it is not device memory.
-// (50 ns.)
-inline int require_read(const void* in, const char* what, bool* elsewhere = nullptr) {
-    if (!in) return B2_OK;
-    cudaPointerAttributes a;
-    B2_CUDA(cudaPointerGetAttributes(&a, in));
-    B2_REQUIRE(a.type != cudaMemoryTypeUnregistered, "%s is not memory that the device reads", what);
-    if (a.type != cudaMemoryTypeDevice) {
-        if (elsewhere) *elsewhere = true;
+// Launches go to the current device.  A result that lies on another one, or on the host, is refused: the kernel would
+// fault, or write across the link.  Operands may also lie in page-locked host memory.  (50 ns an address, and 25 for the
+// device, which is looked up once in a call.)
+class Memory {
+  public:
+    int find_device() {
+        B2_CUDA(cudaGetDevice(&now_));
         return B2_OK;
     }
-    int now = 0;
-    B2_CUDA(cudaGetDevice(&now));
-    B2_REQUIRE(a.device == now, "%s lies on device %d, the current device is %d", what, a.device, now);
-    return B2_OK;
-}
+    int written(const void* out, const char* what) const {
+        cudaPointerAttributes a;
+        B2_CUDA(cudaPointerGetAttributes(&a, out));
+        B2_REQUIRE(a.type == cudaMemoryTypeDevice || a.type == cudaMemoryTypeManaged, "%s is not device memory", what);
+        B2_REQUIRE(a.type != cudaMemoryTypeDevice || a.device == now_, "%s lies on device %d, the current device is %d", what, a.device, now_);
+        return B2_OK;
+    }
+    int read(const void* in, const char* what) {
+        if (!in) return B2_OK;
+        cudaPointerAttributes a;
+        B2_CUDA(cudaPointerGetAttributes(&a, in));
+        B2_REQUIRE(a.type != cudaMemoryTypeUnregistered, "%s is not memory that the device reads", what);
+        B2_REQUIRE(a.type != cudaMemoryTypeDevice || a.device == now_, "%s lies on device %d, the current device is %d", what, a.device, now_);
+        elsewhere = elsewhere || a.type != cudaMemoryTypeDevice;
+        return B2_OK;
+    }
+    bool elsewhere = false;             // an operand is not device memory
+
+  private:
+    int now_ = 0;
+};
 
 // Blocks write in any order: a dense result has no memory in common with an operand.
 inline bool overlap(const void* a, size_t a_bytes, const void* b, size_t b_bytes) {
