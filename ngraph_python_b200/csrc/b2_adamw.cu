@@ -6,9 +6,9 @@
 // Bound by memory: 28 bytes a value with fp32 moments, 16.06 with moments in 8 bits.  The tensors are cut into chunks
 // of 2048 values, one 64-byte record each, made once (the addresses of a program's tensors stay): a CTA reads a
 // record and its values, whatever tensor they belong to, so that many small tensors cost no launches.  79.5 million values:
-// 345 us with fp32 moments, 0.99 of the rate of a copy; 252 us with 8-bit ones, 0.78 of it, by issue (some 84 instructions a
-// value, of which division and square root, correctly rounded, are a fifth), and 284 where the power cap has lowered the
-// clock to 1.7 GHz.  162 000 values: 3.7 us in a graph.
+// 345 us with fp32 moments, 0.99 of the rate of a copy; 252 us with 8-bit ones, 0.78 of it (some 84 instructions a value, of
+// which division and square root, correctly rounded, are a fifth, issued in 73 % of the cycles; in the others the warps wait
+// for loads), and 284 where the power cap has lowered the clock to 1.7 GHz.  162 000 values: 3.7 us in a graph.
 //
 // Moments in 8 bits: a warp holds 256 values and their two scales.  m and sqrt(v) are e4m3 values times the block's
 // largest / 448.  v itself spans the square of what its root does, and e4m3 covers 2.3e5 : 1.  An average with
