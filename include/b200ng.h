@@ -635,6 +635,65 @@ int b2_norm_bprop_scratch_bytes(const b2_norm* norm, size_t* bytes);
 int b2_norm_bprop(const b2_norm* norm, const b2_norm_grads* grads, void* scratch,
                   size_t scratch_bytes, void* stream);
 
+/* Rotation of heads by their position, and the norm of every head with the rotation in the same pass.  A tensor of heads is
+ * x [rows][heads][head_dim] with strides in elements (features next to one another); a call takes one or two such tensors,
+ * as a rule the queries and the keys of the same rows.  Feature pairs of the first rotary_dim features -- i and
+ * i + rotary_dim / 2, or 2 i and 2 i + 1 where `interleaved` -- turn as one complex number:
+ *   z_i -> amplitude * z_i * exp(2 pi sqrt(-1) * position * turns[i] / 2^64)
+ * `inverse` turns back, which is the gradient.  The other features pass through.  turns[i] is a frequency in 2^-64 of a
+ * turn, so that position * turns[i], modulo 2^64, is the angle of any position up to 2^-65 of a turn times the position.
+ * Row r has the position positions[(r / position_group) % position_count] (position_kind: B2_IDX_*; fp32 and flex16 to the
+ * nearest whole number; NaN and what 64 bits do not hold make the row's rotated features NaN, in flex16 zero), or that index
+ * itself where `positions` is NULL.
+ *   b2_rotary_turns  the frequencies, on the host: base^(-2 i / rotary_dim) radians a position, and for contexts that are
+ *            `factor` times as long as the `original` one: LINEAR all divided by factor; BASE base * factor^(d / (d - 2))
+ *            as base; PARTS pairs that turn at least `high` times over the original context as they are, those that turn at
+ *            most `low` times divided by factor, a mixture between
+ *   b2_rotary  x -> out.  flex != 0: int16 mantissas with the exponents of slot_x, slot_out (slot_positions: of flex16
+ *            positions) in `scales`; one tensor a call; results to the nearest even mantissa, the largest to
+ *            stats[slot_out]; probe != 0 stores nothing and leaves the bit pattern of the largest |value| in *probe_out
+ *   b2_heads_fprop  out = rotated(x * rstd * weight), rstd = 1 / sqrt(mean(x^2) + eps) over the features of a head; weight
+ *            [head_dim] is shared by the heads of a tensor, NULL for none; rstd [rows][heads] is stored where not NULL.
+ *            rotary_dim 0: the norm alone
+ *   b2_heads_bprop  from d_out the gradients d_x and d_weight (NULL: not wanted); reads x, rstd, weight and the
+ *            rotation as fprop had them (`inverse` 0).  d_weight is added in an order that depends on the sizes alone; rows
+ *            = 0 leaves it zero.  The scratch needs no initial value; calls on two streams at once need one each.
+ * fp32 except b2_rotary's flex16.  `out` may be the memory of `x`, d_x that of d_out, with the same strides; results that
+ * overlap one another or an operand are refused.  head_dim is at most 1024. */
+enum b2_rotary_scaling { B2_ROTARY_PLAIN = 0, B2_ROTARY_LINEAR = 1, B2_ROTARY_BASE = 2, B2_ROTARY_PARTS = 3 };
+typedef struct {
+    const void* x;
+    void* out;
+    int64_t x_row, x_head, out_row, out_head;
+    const float* weight;
+    float* rstd;
+    int32_t heads, slot_x, slot_out, reserved;
+} b2_heads_part;
+typedef struct {
+    int64_t rows;
+    int32_t head_dim, rotary_dim, interleaved, inverse;
+    const uint64_t* turns;
+    const void* positions;
+    int64_t position_count, position_group;
+    int32_t position_kind, slot_positions;
+    float amplitude, eps;
+    int32_t parts, reserved;
+    b2_heads_part part[2];
+} b2_heads;
+typedef struct {
+    const float* d_out;
+    float *d_x, *d_weight;
+    int64_t d_out_row, d_out_head, d_x_row, d_x_head;
+} b2_heads_part_grads;
+typedef struct { b2_heads_part_grads part[2]; } b2_heads_grads;
+int b2_rotary_turns(int32_t rotary_dim, double base, int32_t scaling, double factor, double original, double low, double high,
+                    uint64_t* turns);
+int b2_rotary(const b2_heads* heads, int32_t flex, const b2_flex_scale* scales, int32_t* stats, uint64_t* probe_out,
+              int32_t probe, void* stream);
+int b2_heads_fprop(const b2_heads* heads, void* stream);
+int b2_heads_bprop_scratch_bytes(const b2_heads* heads, size_t* bytes);
+int b2_heads_bprop(const b2_heads* heads, const b2_heads_grads* grads, void* scratch, size_t scratch_bytes, void* stream);
+
 /* One AdamW step over many fp32 tensors in one launch.  With t the number of the step, from 1 on:
  *   m = beta1 m + (1 - beta1) g,  v = beta2 v + (1 - beta2) g^2
  *   param = param (1 - lr weight_decay decay) - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps)

@@ -1,0 +1,467 @@
+// Rotation of heads by position, and the norm of every head with the rotation in the same pass:
+//
+//   rotary     z_i -> amplitude z_i exp(i angle),  angle = position * frequency_i,  z_i a pair of features
+//   forward    y = rotated(x^ w),  x^ = x rstd,  rstd = 1 / sqrt(mean(x^2) + eps)
+//   gradients  d = rotated back(dy),  dw = sum over rows and heads of d x^,  dx = rstd (w d - x^ mean(w d x^))
+//
+// Angles: a frequency is a 64-bit fraction of a turn, so that the product with a position, modulo 2^64, is the fraction of a
+// turn that is left, exact but for the rounding of the frequency (2^-45 of a turn at position a million).  In fp32
+// position * frequency would be 0.03 radians off there.  The nearest quarter turn is taken off as an integer and the rest,
+// at most an eighth of a turn, goes to sincospif.
+#include <cmath>
+#include <cstdint>
+
+#include "b2_operators.h"
+#include "b2_ew_device.cuh"
+
+namespace {
+
+using b2::Rows;
+using b2::rows_at;
+using b2::check_apart;
+
+constexpr int kMostDim = 1024;
+constexpr int kWarps = 4;           // of a CTA of the kernel for heads of any length
+
+struct FlexArgs {
+    const b2_flex_scale* table;
+    int* stats;
+    unsigned long long* probe_out;
+    int probe;
+};
+
+// Which position a row has; false: none that 64 bits hold.
+__device__ __forceinline__ bool position_of(const b2_heads& a, long long row, const b2_flex_scale* scales, long long& at) {
+    unsigned long long i = (unsigned long long)row;
+    if (a.position_group != 1) i /= (unsigned long long)a.position_group;
+    if (i >= (unsigned long long)a.position_count) i %= (unsigned long long)a.position_count;
+    at = (long long)i;
+    if (!a.positions) return true;
+    switch (a.position_kind) {
+        case B2_IDX_I32: at = static_cast<const int*>(a.positions)[i]; return true;
+        case B2_IDX_I64: at = static_cast<const long long*>(a.positions)[i]; return true;
+        default: {
+            const float x = a.position_kind == B2_IDX_F32 ? static_cast<const float*>(a.positions)[i]
+                                                          : scales[a.slot_positions].scale * (float)static_cast<const short*>(a.positions)[i];
+            at = __float2ll_rn(x);
+            return fabsf(x) < 9.2e18f;          // (false for NaN)
+        }
+    }
+}
+
+// amplitude * (cos, sin) of the fraction of a turn whose 64 bits are `phase`
+__device__ __forceinline__ float2 turn_of(unsigned long long phase, float amplitude) {
+    const unsigned t = (unsigned)(phase >> 32);
+    const unsigned quarter = (t + 0x20000000u) >> 30;                                     // 0 ... 4
+    float s, c;
+    sincospif((float)(int)(t - (quarter << 30)) * 0x1p-31f, &s, &c);
+    const bool swap = quarter & 1;
+    const float x = swap ? s : c, y = swap ? c : s;
+    return make_float2(amplitude * ((quarter + 1) & 2 ? -x : x), amplitude * (quarter & 2 ? -y : y));
+}
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+
+// fp32 to a mantissa, to the nearest even one; `stat` follows the largest
+template <typename T> __device__ __forceinline__ T held(float v, float& stat);
+template <> __device__ __forceinline__ float held<float>(float v, float&) { return v; }
+template <> __device__ __forceinline__ short held<short>(float v, float& stat) { return (short)b2_f32_to_i16(v, stat); }
+
+enum { ROTATE = 0, FORWARD = 1, BACKWARD = 2 };
+
+// Heads of any length and alignment: a warp to a head, a lane to the pairs (lane, lane + 32, ...), and to what is not
+// rotated; the sums of a norm read the head a second time.  The angles of a row are worked out once, by its CTA.
+template <int MODE, typename T>
+__global__ void __launch_bounds__(kWarps * 32)
+heads_any_kernel(const b2_heads a, const b2_heads_grads g, const FlexArgs flex, float* __restrict__ sums) {
+    extern __shared__ float2 table[];           // (cos, sin) of the row's pairs; BACKWARD: sums of a warp behind them
+    after_earlier_kernels();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int D = a.head_dim, pairs = a.rotary_dim / 2, heads = a.part[0].heads + (a.parts > 1 ? a.part[1].heads : 0);
+    float* mine = reinterpret_cast<float*>(table + pairs) + warp * 2 * D;
+    if constexpr (MODE == BACKWARD) {
+        for (int i = lane; i < 2 * D; i += 32) mine[i] = 0.0f;
+        __syncwarp();
+    }
+    float factor = 1.0f, stat = 0.0f;
+    if constexpr (sizeof(T) == 2) factor = flex.table[a.part[0].slot_x].scale * (flex.probe ? 1.0f : flex.table[a.part[0].slot_out].inv_scale);
+    for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        if (pairs) {
+            __syncthreads();                    // (the row before has been read)
+            long long at;
+            const bool good = position_of(a, row, flex.table, at);
+            for (int i = threadIdx.x; i < pairs; i += kWarps * 32) {
+                float2 w = turn_of((unsigned long long)at * a.turns[i], a.amplitude);
+                if (MODE == BACKWARD || a.inverse) w.y = -w.y;
+                table[i] = good ? w : make_float2(NAN, NAN);
+            }
+            __syncthreads();
+        }
+        for (int head = blockIdx.y * kWarps + warp; head < heads; head += gridDim.y * kWarps) {
+            const int n = head >= a.part[0].heads;
+            const b2_heads_part& p = a.part[n];
+            const int h = head - (n ? a.part[0].heads : 0);
+            const T* x = static_cast<const T*>(p.x) + row * p.x_row + h * p.x_head;
+            const T* in = x;
+            T* out = static_cast<T*>(p.out) + row * p.out_row + h * p.out_head;
+            float rstd = 1.0f, mean = 0.0f;
+            if constexpr (MODE == FORWARD) {
+                float q = 0.0f;
+                for (int i = lane; i < D; i += 32) q = fmaf((float)x[i], (float)x[i], q);
+                rstd = __frsqrt_rn(__fdividef(warp_sum(q), (float)D) + a.eps);
+                if (p.rstd && lane == 0) p.rstd[row * p.heads + h] = rstd;
+            }
+            if constexpr (MODE == BACKWARD) {
+                rstd = p.rstd[row * p.heads + h];
+                in = reinterpret_cast<const T*>(g.part[n].d_out) + row * g.part[n].d_out_row + h * g.part[n].d_out_head;
+                out = g.part[n].d_x ? reinterpret_cast<T*>(g.part[n].d_x) + row * g.part[n].d_x_row + h * g.part[n].d_x_head : nullptr;
+            }
+            // (the rotation mixes two features of one lane)
+            auto places = [&](auto&& visit) {
+                for (int i = lane; i < pairs; i += 32) {
+                    const int e = a.interleaved ? 2 * i : i;
+                    visit(e, a.interleaved ? e + 1 : e + pairs, table[i]);
+                }
+                for (int i = 2 * pairs + lane; i < D; i += 32) visit(i, -1, make_float2(1.0f, 0.0f));
+            };
+            if constexpr (MODE == BACKWARD) {
+                float q = 0.0f;
+                places([&](int e, int f, float2 w) {
+                    const float u = (float)in[e], v = f >= 0 ? (float)in[f] : 0.0f;
+                    const float d = fmaf(u, w.x, -v * w.y), xe = (float)x[e] * rstd;
+                    q = fmaf(p.weight ? p.weight[e] * d : d, xe, q);
+                    mine[n * D + e] = fmaf(d, xe, mine[n * D + e]);
+                    if (f >= 0) {
+                        const float d2 = fmaf(v, w.x, u * w.y), xf = (float)x[f] * rstd;
+                        q = fmaf(p.weight ? p.weight[f] * d2 : d2, xf, q);
+                        mine[n * D + f] = fmaf(d2, xf, mine[n * D + f]);
+                    }
+                });
+                mean = __fdividef(warp_sum(q), (float)D);
+                if (!out) continue;
+            }
+            places([&](int e, int f, float2 w) {
+                float u = (float)in[e], v = f >= 0 ? (float)in[f] : 0.0f;
+                if constexpr (MODE == FORWARD) {
+                    u *= p.weight ? rstd * p.weight[e] : rstd;
+                    if (f >= 0) v *= p.weight ? rstd * p.weight[f] : rstd;
+                }
+                float y = f >= 0 ? fmaf(u, w.x, -v * w.y) : u, z = fmaf(v, w.x, u * w.y);
+                if constexpr (MODE == BACKWARD) {
+                    y = rstd * ((p.weight ? p.weight[e] * y : y) - (float)x[e] * rstd * mean);
+                    if (f >= 0) z = rstd * ((p.weight ? p.weight[f] * z : z) - (float)x[f] * rstd * mean);
+                }
+                if constexpr (sizeof(T) == 2) {
+                    y *= factor;
+                    z = f >= 0 ? z * factor : 0.0f;
+                    if (flex.probe) {
+                        stat = fmaxf(stat, fmaxf(fabsf(y), fabsf(z)));
+                        return;
+                    }
+                }
+                out[e] = held<T>(y, stat);
+                if (f >= 0) out[f] = held<T>(z, stat);
+            });
+        }
+    }
+    if constexpr (MODE == BACKWARD) {
+        __syncthreads();
+        const float* first = reinterpret_cast<const float*>(table + pairs);
+        float* to = sums + (long long)(blockIdx.y * gridDim.x + blockIdx.x) * 2 * D;
+        for (int i = threadIdx.x; i < 2 * D; i += kWarps * 32) {
+            float v = 0.0f;
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) v += first[w * 2 * D + i];
+            to[i] = v;
+        }
+    }
+    if constexpr (sizeof(T) == 2) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) stat = fmaxf(stat, __shfl_xor_sync(0xffffffffu, stat, o));
+        if (lane == 0 && stat > 0.0f) {
+            if (flex.probe) atomicMax(flex.probe_out, (unsigned long long)__float_as_uint(stat));
+            else atomicMax(flex.stats + a.part[0].slot_out, (int)rintf(stat));
+        }
+    }
+}
+
+// Adds the CTAs' sums in their order: a warp to 32 columns and every 32nd CTA, then the warps' sums in their order.
+__global__ void __launch_bounds__(1024)
+heads_sums_kernel(const float* __restrict__ sums, int ctas, int D, float* d_weight0, float* d_weight1) {
+    __shared__ float part[32][33];
+    after_earlier_kernels();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, i = blockIdx.x * 32 + lane;
+    float v = 0.0f;
+    if (i < 2 * D)
+        for (int k = warp; k < ctas; k += 32) v += sums[(long long)k * 2 * D + i];
+    part[warp][lane] = v;
+    __syncthreads();
+    if (warp == 0 && i < 2 * D) {
+        v = 0.0f;
+        for (int w = 0; w < 32; ++w) v += part[w][lane];
+        float* to = i < D ? d_weight0 : d_weight1;
+        if (to) to[i < D ? i : i - D] = v;
+    }
+}
+
+int check_heads(const b2_heads* a, int value_bytes) {
+    B2_REQUIRE(a, "missing argument");
+    B2_REQUIRE(a->rows >= 0 && a->rows <= (1ll << 38), "bad number of rows: %lld", (long long)a->rows);
+    B2_REQUIRE(a->head_dim >= 1 && a->head_dim <= kMostDim, "a head has 1 to %d features, not %d", kMostDim, a->head_dim);
+    B2_REQUIRE(a->rotary_dim >= 0 && a->rotary_dim <= a->head_dim && a->rotary_dim % 2 == 0, "%d of %d features cannot be rotated", a->rotary_dim,
+               a->head_dim);
+    B2_REQUIRE(a->parts == 1 || a->parts == 2, "one or two tensors of heads, not %d", a->parts);
+    B2_REQUIRE(std::isfinite(a->amplitude) && std::isfinite(a->eps) && a->eps >= 0.0f, "bad amplitude %g or eps %g", a->amplitude, a->eps);
+    if (a->rotary_dim > 0) {
+        B2_REQUIRE(a->turns && ((uintptr_t)a->turns & 7) == 0, "the frequencies are missing or lie between two addresses");
+        B2_REQUIRE(a->position_count >= 1 && a->position_group >= 1, "bad positions: %lld of %lld rows each", (long long)a->position_count,
+                   (long long)a->position_group);
+        if (a->positions) {
+            B2_REQUIRE(a->position_kind >= B2_IDX_F32 && a->position_kind <= B2_IDX_FLEX16, "unknown kind of positions: %d", a->position_kind);
+            const uintptr_t size = a->position_kind == B2_IDX_I64 ? 8 : a->position_kind == B2_IDX_FLEX16 ? 2 : 4;
+            B2_REQUIRE((uintptr_t)a->positions % size == 0, "a position lies between two addresses");
+        }
+    }
+    for (int i = 0; i < a->parts; ++i) {
+        const b2_heads_part& p = a->part[i];
+        B2_REQUIRE(p.heads >= 0 && p.heads <= (1 << 20), "bad number of heads: %d", p.heads);
+        B2_REQUIRE(((uintptr_t)p.x | (uintptr_t)p.out) % value_bytes == 0 && (((uintptr_t)p.weight | (uintptr_t)p.rstd) & 3) == 0,
+                   "a tensor of heads lies between two addresses");
+    }
+    return B2_OK;
+}
+
+// Strides that reach only so far, and for a result no two places for one value.
+int check_strides(const b2_heads* a, int heads, int64_t row, int64_t head, bool result, const char* what) {
+    if (a->rows == 0 || heads == 0) return B2_OK;
+    B2_REQUIRE(row >= 0 && head >= 0 && (a->rows == 1 || row <= (1ll << 46) / a->rows) && (heads == 1 || head <= (1ll << 46) / heads),
+               "strides of %s: %lld between rows, %lld between heads", what, (long long)row, (long long)head);
+    if (!result) return B2_OK;
+    const int64_t D = a->head_dim, across_heads = (heads - 1) * head + D, across_rows = (a->rows - 1) * row + D;
+    const bool by_rows = (heads == 1 || head >= D) && (a->rows == 1 || row >= across_heads);
+    const bool by_heads = (a->rows == 1 || row >= D) && (heads == 1 || head >= across_rows);
+    B2_REQUIRE(by_rows || by_heads, "%s overlaps itself: strides %lld between rows, %lld between heads, %lld features", what, (long long)row, (long long)head,
+               (long long)D);
+    return B2_OK;
+}
+
+// The memory of a tensor of heads.
+template <typename T>
+Rows heads_at(const T* p, const b2_heads& a, int heads, int64_t row, int64_t head) {
+    const long long R = a.rows, D = a.head_dim;
+    if (!p || R == 0 || heads == 0) return rows_at(p, 0, 1, 1);
+    if (heads == 1) return row >= D || R == 1 ? rows_at(p, R, D, row) : rows_at(p, 1, (R - 1) * row + D, D);
+    if (R == 1) return head >= D ? rows_at(p, heads, D, head) : rows_at(p, 1, (heads - 1) * head + D, D);
+    if (head >= D && row == heads * head) return rows_at(p, R * heads, D, head);
+    if (row >= (heads - 1) * head + D) return rows_at(p, R, (heads - 1) * head + D, row);
+    if (head >= (R - 1) * row + D) return rows_at(p, heads, (R - 1) * row + D, head);
+    return rows_at(p, 1, (R - 1) * row + (heads - 1) * head + D, D);
+}
+Rows heads_at(const void* p, const b2_heads& a, int heads, int64_t row, int64_t head, int value_bytes) {
+    return value_bytes == 2 ? heads_at(static_cast<const short*>(p), a, heads, row, head) : heads_at(static_cast<const float*>(p), a, heads, row, head);
+}
+Rows positions_at(const b2_heads& a) {
+    if (a.rotary_dim == 0 || !a.positions) return rows_at((const char*)nullptr, 0, 0, 0);
+    const long long groups = (a.rows + a.position_group - 1) / a.position_group, count = a.position_count < groups ? a.position_count : groups;
+    const long long bytes = count * (a.position_kind == B2_IDX_I64 ? 8 : a.position_kind == B2_IDX_FLEX16 ? 2 : 4);
+    return rows_at(static_cast<const char*>(a.positions), 1, bytes, bytes);
+}
+Rows turns_at(const b2_heads& a) { return rows_at(a.rotary_dim ? a.turns : nullptr, 1, a.rotary_dim / 2, a.rotary_dim / 2); }
+Rows dense(const float* p, long long n) { return n > 0 ? rows_at(p, 1, n, n) : rows_at(p, 0, 1, 1); }
+
+int check_reads(const b2_heads* a, b2::Memory& memory) {
+    if (a->rotary_dim > 0) {
+        B2_CHECK(memory.read(a->turns, "the frequencies"));
+        B2_CHECK(memory.read(a->positions, "the positions"));
+    }
+    return B2_OK;
+}
+
+int total_heads(const b2_heads& a) { return a.part[0].heads + (a.parts > 1 ? a.part[1].heads : 0); }
+
+// CTAs for heads of any length: rows, and where they are few parts of a row's heads
+dim3 grid_any(const b2_heads& a) {
+    const long long most = b2::kSms * 16, x = a.rows < most ? a.rows : most;
+    long long y = (total_heads(a) + kWarps - 1) / kWarps, room = most / (x > 0 ? x : 1);
+    if (y > room) y = room;
+    return dim3((unsigned)x, (unsigned)(y < 1 ? 1 : y));
+}
+
+// Checks that forward passes share; `sizes` of the values.
+int check_forward(const b2_heads* a, int value_bytes, b2::Memory& memory) {
+    Rows results[4], operands[6];
+    int n = 0, m = 0;
+    for (int i = 0; i < a->parts; ++i) {
+        const b2_heads_part& p = a->part[i];
+        if (p.heads == 0) continue;
+        B2_REQUIRE(p.x && p.out, "a tensor of heads is missing");
+        B2_CHECK(check_strides(a, p.heads, p.x_row, p.x_head, false, "the heads"));
+        B2_CHECK(check_strides(a, p.heads, p.out_row, p.out_head, true, "the result"));
+        results[n++] = heads_at(p.out, *a, p.heads, p.out_row, p.out_head, value_bytes);
+        if (p.rstd) results[n++] = dense(p.rstd, a->rows * p.heads);
+        if (p.x != p.out) operands[m++] = heads_at(p.x, *a, p.heads, p.x_row, p.x_head, value_bytes);
+        else B2_REQUIRE((a->rows == 1 || p.x_row == p.out_row) && (p.heads == 1 || p.x_head == p.out_head), "a result in place of its operand has other strides");
+        if (p.weight) operands[m++] = dense(p.weight, a->head_dim);
+    }
+    operands[m++] = positions_at(*a);
+    operands[m++] = turns_at(*a);
+    B2_CHECK(check_apart(results, n, operands, m, "heads"));
+    B2_CHECK(memory.find_device());
+    for (int i = 0; i < a->parts; ++i) {
+        const b2_heads_part& p = a->part[i];
+        if (p.heads == 0) continue;
+        B2_CHECK(memory.written(p.out, "the result of heads"));
+        if (p.rstd) B2_CHECK(memory.written(p.rstd, "the reciprocal deviations of heads"));
+        B2_CHECK(memory.read(p.x, "a tensor of heads"));
+        B2_CHECK(memory.read(p.weight, "the weight of heads"));
+    }
+    return check_reads(a, memory);
+}
+
+template <int MODE, typename T>
+int launch_any(const b2_heads& a, const b2_heads_grads& g, const FlexArgs& flex, float* sums, dim3 grid, cudaStream_t st) {
+    const size_t room = a.rotary_dim / 2 * sizeof(float2) + (MODE == BACKWARD ? kWarps * 2 * a.head_dim * sizeof(float) : 0);
+    B2_CUDA((b2::launch_after(heads_any_kernel<MODE, T>, grid, kWarps * 32, room, st, a, g, flex, sums)));
+    return B2_OK;
+}
+
+}  // namespace
+
+extern "C" int b2_rotary_turns(int32_t rotary_dim, double base, int32_t scaling, double factor, double original, double low, double high, uint64_t* turns) {
+    B2_REQUIRE(rotary_dim >= 0 && rotary_dim <= kMostDim && rotary_dim % 2 == 0, "%d features cannot be rotated", rotary_dim);
+    B2_REQUIRE(turns || rotary_dim == 0, "missing argument");
+    B2_REQUIRE(std::isfinite(base) && base > 0.0, "bad base: %g", base);
+    B2_REQUIRE(scaling >= B2_ROTARY_PLAIN && scaling <= B2_ROTARY_PARTS, "unknown scaling: %d", scaling);
+    B2_REQUIRE(scaling == B2_ROTARY_PLAIN || (std::isfinite(factor) && factor > 0.0), "bad factor: %g", factor);
+    B2_REQUIRE(scaling != B2_ROTARY_PARTS || (std::isfinite(original) && original > 0.0 && std::isfinite(low) && std::isfinite(high) && low < high),
+               "bad parts: context %g, from %g to %g turns", original, low, high);
+    const double d = rotary_dim, circle = 6.283185307179586476925;
+    if (scaling == B2_ROTARY_BASE && rotary_dim > 2) base *= std::pow(factor, d / (d - 2));
+    for (int i = 0; i < rotary_dim / 2; ++i) {
+        double f = std::pow(base, -2.0 * i / d) / circle;           // turns a position
+        if (scaling == B2_ROTARY_LINEAR) f /= factor;
+        if (scaling == B2_ROTARY_PARTS) {
+            double keep = (original * f - low) / (high - low);
+            keep = keep < 0.0 ? 0.0 : keep > 1.0 ? 1.0 : keep;
+            f = keep * f + (1.0 - keep) * f / factor;
+        }
+        B2_REQUIRE(std::isfinite(f), "frequency %d is not finite", i);
+        f -= std::floor(f);
+        // (a double just below one may round to a whole turn)
+        const double whole = std::nearbyint(f * 18446744073709551616.0);
+        turns[i] = whole >= 18446744073709551616.0 ? 0 : (uint64_t)whole;
+    }
+    return B2_OK;
+}
+
+extern "C" int b2_rotary(const b2_heads* a, int32_t flex, const b2_flex_scale* scales, int32_t* stats, uint64_t* probe_out, int32_t probe, void* stream) {
+    const int size = flex ? 2 : 4;
+    B2_CHECK(check_heads(a, size));
+    for (int i = 0; i < a->parts; ++i) B2_REQUIRE(!a->part[i].weight && !a->part[i].rstd, "a weight or deviations without a norm");
+    B2_REQUIRE(flex || a->rotary_dim == 0 || !a->positions || a->position_kind != B2_IDX_FLEX16 || scales, "flex16 positions have an exponent");
+    if (flex) {
+        B2_REQUIRE(a->parts == 1, "one tensor in flex16, not %d", a->parts);
+        B2_REQUIRE(scales && a->part[0].slot_x >= 0 && a->part[0].slot_out >= 0 && (probe ? probe_out != nullptr : stats != nullptr), "missing exponents or statistics");
+    }
+    B2_REQUIRE(a->rotary_dim == 0 || !a->positions || a->position_kind != B2_IDX_FLEX16 || a->slot_positions >= 0, "flex16 positions have an exponent");
+    B2_REQUIRE((((uintptr_t)scales | (uintptr_t)stats) & 3) == 0 && ((uintptr_t)probe_out & 7) == 0, "exponents or statistics lie between two addresses");
+    if (a->rows == 0 || total_heads(*a) == 0) return B2_OK;
+    b2::Memory memory;
+    B2_CHECK(check_forward(a, size, memory));
+    const FlexArgs f = {scales, stats, (unsigned long long*)probe_out, probe};
+    const bool scaled = flex || (a->positions && a->position_kind == B2_IDX_FLEX16);
+    if (scaled) B2_CHECK(memory.read(scales, "the exponents"));
+    if (flex) B2_CHECK(probe ? memory.written(probe_out, "the largest value") : memory.written(stats, "the statistics"));
+    cudaStream_t st = (cudaStream_t)stream;
+    if (flex) return launch_any<ROTATE, short>(*a, b2_heads_grads{}, f, nullptr, grid_any(*a), st);
+    return launch_any<ROTATE, float>(*a, b2_heads_grads{}, f, nullptr, grid_any(*a), st);
+}
+
+static int check_norm_of_heads(const b2_heads* a) {
+    B2_CHECK(check_heads(a, 4));
+    B2_REQUIRE(!a->inverse, "a norm's rotation is not turned back: its gradient does that itself");
+    B2_REQUIRE(a->rotary_dim == 0 || !a->positions || a->position_kind != B2_IDX_FLEX16, "flex16 positions of fp32 heads");
+    return B2_OK;
+}
+
+extern "C" int b2_heads_fprop(const b2_heads* a, void* stream) {
+    B2_CHECK(check_norm_of_heads(a));
+    if (a->rows == 0 || total_heads(*a) == 0) return B2_OK;
+    b2::Memory memory;
+    B2_CHECK(check_forward(a, 4, memory));
+    return launch_any<FORWARD, float>(*a, b2_heads_grads{}, FlexArgs{}, nullptr, grid_any(*a), (cudaStream_t)stream);
+}
+
+extern "C" int b2_heads_bprop_scratch_bytes(const b2_heads* a, size_t* bytes) {
+    B2_REQUIRE(bytes, "missing argument");
+    B2_CHECK(check_norm_of_heads(a));
+    const dim3 grid = grid_any(*a);
+    *bytes = (size_t)grid.x * grid.y * 2 * a->head_dim * sizeof(float) + 256;
+    return B2_OK;
+}
+
+extern "C" int b2_heads_bprop(const b2_heads* a, const b2_heads_grads* g, void* scratch, size_t scratch_bytes, void* stream) {
+    size_t need = 0;
+    B2_CHECK(b2_heads_bprop_scratch_bytes(a, &need));
+    B2_REQUIRE(g, "missing argument");
+    B2_REQUIRE(scratch && scratch_bytes >= need, "the gradient of heads needs %zu bytes of scratch, got %zu", need, scratch_bytes);
+    Rows results[5], operands[10];
+    int n = 0, m = 0;
+    float* weights[2] = {nullptr, nullptr};
+    results[n++] = rows_at((const char*)scratch, 1, (long long)need, (long long)need);
+    for (int i = 0; i < a->parts; ++i) {
+        const b2_heads_part& p = a->part[i];
+        const b2_heads_part_grads& d = g->part[i];
+        B2_REQUIRE((((uintptr_t)d.d_out | (uintptr_t)d.d_x | (uintptr_t)d.d_weight) & 3) == 0, "a gradient of heads lies between two addresses");
+        B2_REQUIRE(p.weight || !d.d_weight, "the gradient of a weight that is not there");
+        weights[i] = d.d_weight;
+        if (d.d_weight) results[n++] = dense(d.d_weight, a->head_dim);
+        if (p.weight) operands[m++] = dense(p.weight, a->head_dim);
+        if (a->rows == 0 || p.heads == 0) continue;
+        B2_REQUIRE(p.x && p.rstd && d.d_out, "the gradient of heads reads x, rstd and d_out");
+        B2_CHECK(check_strides(a, p.heads, p.x_row, p.x_head, false, "the heads"));
+        B2_CHECK(check_strides(a, p.heads, d.d_out_row, d.d_out_head, false, "the result's gradient"));
+        operands[m++] = heads_at((const float*)p.x, *a, p.heads, p.x_row, p.x_head);
+        operands[m++] = dense(p.rstd, a->rows * p.heads);
+        if (d.d_x) {
+            B2_CHECK(check_strides(a, p.heads, d.d_x_row, d.d_x_head, true, "the heads' gradient"));
+            results[n++] = heads_at((const float*)d.d_x, *a, p.heads, d.d_x_row, d.d_x_head);
+            B2_REQUIRE(d.d_x != d.d_out || ((a->rows == 1 || d.d_x_row == d.d_out_row) && (p.heads == 1 || d.d_x_head == d.d_out_head)),
+                       "a gradient in place of its operand has other strides");
+        }
+        if (d.d_x != d.d_out) operands[m++] = heads_at(d.d_out, *a, p.heads, d.d_out_row, d.d_out_head);
+    }
+    operands[m++] = positions_at(*a);
+    operands[m++] = turns_at(*a);
+    B2_CHECK(check_apart(results, n, operands, m, "heads' gradient"));
+    b2::Memory memory;
+    B2_CHECK(memory.find_device());
+    B2_CHECK(memory.written(scratch, "the scratch of heads"));
+    const bool work = a->rows > 0 && total_heads(*a) > 0;
+    for (int i = 0; i < a->parts; ++i) {
+        const b2_heads_part& p = a->part[i];
+        const b2_heads_part_grads& d = g->part[i];
+        if (d.d_weight) B2_CHECK(memory.written(d.d_weight, "the gradient of a weight"));
+        B2_CHECK(memory.read(p.weight, "the weight of heads"));
+        if (!work || p.heads == 0) continue;
+        if (d.d_x) B2_CHECK(memory.written(d.d_x, "the gradient of heads"));
+        B2_CHECK(memory.read(p.x, "a tensor of heads"));
+        B2_CHECK(memory.read(p.rstd, "the reciprocal deviations of heads"));
+        B2_CHECK(memory.read(d.d_out, "the gradient of a result"));
+    }
+    if (work) B2_CHECK(check_reads(a, memory));
+    cudaStream_t st = (cudaStream_t)stream;
+    float* sums = (float*)(((uintptr_t)scratch + 255) / 256 * 256);
+    const dim3 grid = grid_any(*a);
+    if (work) B2_CHECK((launch_any<BACKWARD, float>(*a, *g, FlexArgs{}, sums, grid, st)));
+    if (weights[0] || weights[1]) {
+        const int D = a->head_dim;
+        B2_CUDA((b2::launch_after(heads_sums_kernel, dim3((2 * D + 31) / 32), 1024, 0, st, (const float*)sums, work ? (int)(grid.x * grid.y) : 0, D,
+                                  weights[0], weights[1])));
+    }
+    return B2_OK;
+}

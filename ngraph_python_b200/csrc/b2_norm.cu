@@ -16,6 +16,10 @@
 
 namespace {
 
+using b2::Rows;
+using b2::rows_at;
+using b2::check_apart;
+
 constexpr int kThreads = 512;        // of a CTA for rows of any length
 
 // VEC values next to one another
@@ -750,55 +754,6 @@ int check_stride(const b2_norm* a, const void* p, int64_t stride, const char* wh
     return B2_OK;
 }
 
-// Rows of a tensor, in values.  Dense ones are one long row.
-struct Rows {
-    const float *p, *end;
-    long long rows, width, stride;
-};
-inline Rows rows_at(const float* p, long long rows, long long width, long long stride) {
-    if (!p || rows <= 0) return {nullptr, nullptr, 0, 0, 0};
-    if (rows == 1 || stride == width) return {p, p + rows * width, 1, rows * width, rows * width};
-    return {p, p + ((rows - 1) * stride + width), rows, width, stride};
-}
-
-// Whether two tensors that lie among one another have memory in common.  Their rows may lie side by side.
-bool meet(Rows a, Rows b) {
-    if (a.rows > b.rows) std::swap(a, b);
-    const long long ahead = ((long long)(uintptr_t)b.p - (long long)(uintptr_t)a.p) / 4;     // where b begins, seen from a
-    const auto below = [](long long x, long long y) { return x / y - (x % y < 0); };
-    if (a.stride == b.stride) {
-        // row i of a and row j of b meet where (i - j) stride lies between ahead - a.width and ahead + b.width
-        const long long least = below(ahead - a.width, a.stride) + 1, d = least > 1 - b.rows ? least : 1 - b.rows;
-        return d < a.rows && d * a.stride < ahead + b.width;
-    }
-    for (long long i = 0; i < a.rows; ++i) {
-        // the first row of b that does not end before row i of a begins
-        const long long from = i * a.stride - ahead, least = below(from - b.width, b.stride) + 1, j = least > 0 ? least : 0;
-        if (j < b.rows && j * b.stride < from + a.width) return true;
-    }
-    return false;
-}
-
-// Blocks write in any order: results have memory of their own.
-int check_apart(const Rows* written, int count, const Rows* read, int reads) {
-    const auto apart = [](const Rows& a, const Rows& b) { return (uintptr_t)a.end <= (uintptr_t)b.p || (uintptr_t)b.end <= (uintptr_t)a.p; };
-    for (int i = 0; i < count; ++i) {
-        const Rows& w = written[i];
-        if (!w.p) continue;
-        for (int k = 0; k < i; ++k)
-            if (!apart(w, written[k])) {
-                B2_REQUIRE(w.p != written[k].p, "two results of the norm lie in one place");
-                B2_REQUIRE(!meet(w, written[k]), "two results of the norm overlap");
-            }
-        for (int k = 0; k < reads; ++k)
-            if (!apart(w, read[k])) {
-                B2_REQUIRE(w.p != read[k].p, "a result of the norm lies in the place of an operand");
-                B2_REQUIRE(!meet(w, read[k]), "a result of the norm overlaps an operand");
-            }
-    }
-    return B2_OK;
-}
-
 inline Rows gate_rows(const b2_norm& a, const float* p, long long stride) {
     const long long R = a.rows, F = a.features;
     return a.gate_kind == B2_GATE_FULL ? rows_at(p, R, F, stride) : a.gate_kind == B2_GATE_ROW ? rows_at(p, 1, R, R) : rows_at(p, 1, F, F);
@@ -884,7 +839,7 @@ extern "C" int b2_norm_fprop(const b2_norm* a, void* stream) {
                             rows_at(a->stream_rstd, 1, R, R)};
     const Rows operands[] = {rows_at(a->block, R, F, a->block_stride), gate_rows(*a, a->gate, a->gate_stride), rows_at(a->post_weight, 1, F, F),
                              rows_at(a->pre_weight, 1, F, F), rows_at(a->stream == a->residual ? nullptr : a->residual, R, F, a->residual_stride)};
-    B2_CHECK(check_apart(results, 4, operands, 5));
+    B2_CHECK(check_apart(results, 4, operands, 5, "norm"));
     B2_CHECK(check_in_place(a, a->stream, a->stream_stride, a->residual, a->residual_stride, "the stream"));
     b2::Memory memory;
     B2_CHECK(memory.find_device());
@@ -971,7 +926,7 @@ extern "C" int b2_norm_bprop(const b2_norm* a, const b2_norm_grads* d, void* scr
                                  rows_at(a->block, R, F, a->block_stride), gate_rows(*a, a->gate, a->gate_stride), rows_at(a->post_weight, 1, F, F),
                                  rows_at(a->pre_weight, 1, F, F), rows_at(d->d_out, R, F, d->d_out_stride), rows_at(a->stream_rstd, 1, R, R),
                                  rows_at(a->block_rstd, 1, R, R), rows_at(d->d_stream == d->d_residual ? nullptr : d->d_stream, R, F, d->d_stream_stride)};
-        B2_CHECK(check_apart(results, 6, operands, 9));
+        B2_CHECK(check_apart(results, 6, operands, 9, "norm"));
         B2_CHECK(check_in_place(a, d->d_residual, d->d_residual_stride, d->d_stream, d->d_stream_stride, "the residual's gradient"));
     }
     // (sums over rows are written whatever the number of rows)
@@ -979,7 +934,7 @@ extern "C" int b2_norm_bprop(const b2_norm* a, const b2_norm_grads* d, void* scr
     if (a->rows == 0) {
         const long long F = a->features;
         const Rows results[] = {rows_at(d->d_post_weight, 1, F, F), rows_at(d->d_pre_weight, 1, F, F), rows_at(gate, 1, F, F), room};
-        B2_CHECK(check_apart(results, 4, nullptr, 0));
+        B2_CHECK(check_apart(results, 4, nullptr, 0, "norm"));
     }
     b2::Memory memory;
     B2_CHECK(memory.find_device());

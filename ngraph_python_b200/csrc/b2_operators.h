@@ -1,8 +1,9 @@
-// Helpers shared by the language-model operators (b2_embed.cu, b2_norm.cu, b2_adamw.cu).
+// Helpers shared by the language-model operators (b2_embed.cu, b2_norm.cu, b2_adamw.cu, b2_heads.cu, b2_muon.cu).
 #ifndef B2_OPERATORS_H
 #define B2_OPERATORS_H
 
 #include <atomic>
+#include <utility>
 
 #include "b2_common.h"
 
@@ -55,6 +56,58 @@ inline int allow_shared(const void* kernel, int bytes, std::atomic<unsigned long
     if (done->load(std::memory_order_relaxed) & bit) return B2_OK;
     B2_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
     done->fetch_or(bit, std::memory_order_relaxed);
+    return B2_OK;
+}
+
+// Rows of a tensor, in bytes.  Dense ones are one long row.
+struct Rows {
+    uintptr_t p, end;
+    long long rows, width, stride;
+};
+template <typename T>
+inline Rows rows_at(const T* p, long long rows, long long width, long long stride) {
+    const long long size = sizeof(T);
+    const uintptr_t at = (uintptr_t)p;
+    if (!p || rows <= 0) return {0, 0, 0, 0, 0};
+    if (rows == 1 || stride == width) return {at, at + size * rows * width, 1, size * rows * width, size * rows * width};
+    return {at, at + size * ((rows - 1) * stride + width), rows, size * width, size * stride};
+}
+
+// Whether two tensors that lie among one another have memory in common.  Their rows may lie side by side.
+inline bool meet(Rows a, Rows b) {
+    if (a.rows > b.rows) std::swap(a, b);
+    const long long ahead = (long long)b.p - (long long)a.p;     // where b begins, seen from a
+    const auto below = [](long long x, long long y) { return x / y - (x % y < 0); };
+    if (a.stride == b.stride) {
+        // row i of a and row j of b meet where (i - j) stride lies between ahead - a.width and ahead + b.width
+        const long long least = below(ahead - a.width, a.stride) + 1, d = least > 1 - b.rows ? least : 1 - b.rows;
+        return d < a.rows && d * a.stride < ahead + b.width;
+    }
+    for (long long i = 0; i < a.rows; ++i) {
+        // the first row of b that does not end before row i of a begins
+        const long long from = i * a.stride - ahead, least = below(from - b.width, b.stride) + 1, j = least > 0 ? least : 0;
+        if (j < b.rows && j * b.stride < from + a.width) return true;
+    }
+    return false;
+}
+
+// Blocks write in any order: results have memory of their own.
+inline int check_apart(const Rows* written, int count, const Rows* read, int reads, const char* what) {
+    const auto apart = [](const Rows& a, const Rows& b) { return a.end <= b.p || b.end <= a.p; };
+    for (int i = 0; i < count; ++i) {
+        const Rows& w = written[i];
+        if (!w.p) continue;
+        for (int k = 0; k < i; ++k)
+            if (!apart(w, written[k])) {
+                B2_REQUIRE(w.p != written[k].p, "two results of the %s lie in one place", what);
+                B2_REQUIRE(!meet(w, written[k]), "two results of the %s overlap", what);
+            }
+        for (int k = 0; k < reads; ++k)
+            if (!apart(w, read[k])) {
+                B2_REQUIRE(w.p != read[k].p, "a result of the %s lies in the place of an operand", what);
+                B2_REQUIRE(!meet(w, read[k]), "a result of the %s overlaps an operand", what);
+            }
+    }
     return B2_OK;
 }
 

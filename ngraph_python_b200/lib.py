@@ -123,6 +123,32 @@ class NormGrads(C.Structure):
         [("status", C.c_void_p)]
 
 
+ROTARY_SCALINGS = {"none": 0, "linear": 1, "base": 2, "parts": 3}
+
+
+class HeadsPart(C.Structure):
+    """b2_heads_part: one tensor of heads."""
+    _fields_ = [("x", C.c_void_p), ("out", C.c_void_p)] + [(f, C.c_int64) for f in ("x_row", "x_head", "out_row", "out_head")] + \
+        [("weight", C.c_void_p), ("rstd", C.c_void_p)] + [(f, C.c_int32) for f in ("heads", "slot_x", "slot_out", "reserved")]
+
+
+class HeadsArgs(C.Structure):
+    """b2_heads: heads that are normalised or rotated by their position."""
+    _fields_ = [("rows", C.c_int64)] + [(f, C.c_int32) for f in ("head_dim", "rotary_dim", "interleaved", "inverse")] + \
+        [("turns", C.c_void_p), ("positions", C.c_void_p), ("position_count", C.c_int64), ("position_group", C.c_int64),
+         ("position_kind", C.c_int32), ("slot_positions", C.c_int32), ("amplitude", C.c_float), ("eps", C.c_float),
+         ("parts", C.c_int32), ("reserved", C.c_int32), ("part", HeadsPart * 2)]
+
+
+class HeadsPartGrads(C.Structure):
+    _fields_ = [(f, C.c_void_p) for f in ("d_out", "d_x", "d_weight")] + \
+        [(f, C.c_int64) for f in ("d_out_row", "d_out_head", "d_x_row", "d_x_head")]
+
+
+class HeadsGrads(C.Structure):
+    _fields_ = [("part", HeadsPartGrads * 2)]
+
+
 class AdamwTensor(C.Structure):
     _fields_ = [("param", C.c_void_p), ("grad", C.c_void_p), ("m", C.c_void_p), ("v", C.c_void_p), ("m_scales", C.c_void_p),
                 ("v_scales", C.c_void_p), ("n", C.c_int64), ("decay", C.c_float), ("counter", C.c_uint32)]
@@ -248,6 +274,11 @@ def _load():
         "b2_norm_fprop": (C.c_int, [C.POINTER(NormArgs), vp]),
         "b2_norm_bprop_scratch_bytes": (C.c_int, [C.POINTER(NormArgs), C.POINTER(sz)]),
         "b2_norm_bprop": (C.c_int, [C.POINTER(NormArgs), C.POINTER(NormGrads), vp, sz, vp]),
+        "b2_rotary_turns": (C.c_int, [i32, C.c_double, i32, C.c_double, C.c_double, C.c_double, C.c_double, vp]),
+        "b2_rotary": (C.c_int, [C.POINTER(HeadsArgs), i32, vp, vp, vp, i32, vp]),
+        "b2_heads_fprop": (C.c_int, [C.POINTER(HeadsArgs), vp]),
+        "b2_heads_bprop_scratch_bytes": (C.c_int, [C.POINTER(HeadsArgs), C.POINTER(sz)]),
+        "b2_heads_bprop": (C.c_int, [C.POINTER(HeadsArgs), C.POINTER(HeadsGrads), vp, sz, vp]),
         "b2_adamw_plan_bytes": (C.c_int, [C.POINTER(AdamwTensor), i32, i32, C.POINTER(sz), C.POINTER(i64)]),
         "b2_adamw_plan": (C.c_int, [C.POINTER(AdamwTensor), i32, i32, vp, sz, vp]),
         "b2_adamw_step": (C.c_int, [vp, i64, i32, C.POINTER(AdamwHyper), vp, vp, vp, C.c_uint32, vp]),
@@ -577,6 +608,22 @@ def embed_update_launches(n):
 def norm_bprop_scratch_bytes(norm):
     out = C.c_size_t()
     check(_lib.b2_norm_bprop_scratch_bytes(C.byref(norm), C.byref(out)))
+    return int(out.value)
+
+
+def rotary_turns(rotary_dim, base=10000.0, scaling="none", factor=1.0, original=1.0, low=1.0, high=32.0):
+    """Frequencies of rotary_dim / 2 pairs in 2^-64 of a turn a position, an int64 tensor of their bits on the host."""
+    import torch
+    if scaling not in ROTARY_SCALINGS:
+        raise ValueError("unknown scaling %r, not one of %s" % (scaling, ", ".join(sorted(ROTARY_SCALINGS))))
+    out = torch.empty((max(int(rotary_dim), 0) // 2,), dtype=torch.int64)
+    check(_lib.b2_rotary_turns(rotary_dim, base, ROTARY_SCALINGS[scaling], factor, original, low, high, out.data_ptr() or None))
+    return out
+
+
+def heads_bprop_scratch_bytes(heads):
+    out = C.c_size_t()
+    check(_lib.b2_heads_bprop_scratch_bytes(C.byref(heads), C.byref(out)))
     return int(out.value)
 
 
