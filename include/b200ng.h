@@ -728,6 +728,42 @@ int b2_adamw_plan(const b2_adamw_tensor* tensors, int32_t count, int32_t state_b
 int b2_adamw_step(void* plan, int64_t chunks, int32_t state_bits, const b2_adamw_hyper* hyper,
                   const float* lr, const float* grad_scale, float* step, uint32_t seed, void* stream);
 
+/* One optimizer step over many fp32 matrices whose updates are orthogonalised.  With g the gradient (times grad_scale) of a
+ * matrix param [rows][cols], dense:
+ *   mean = momentum mean + (1 - momentum) g
+ *   u    = nesterov ? (1 - momentum) g + momentum mean : mean,   x = u / (|u| + eps),  |u| the root of the sum of squares
+ *   x    = a x + (b A + c A A) x,  A = x x^T, `steps` times      (x^T x from the other side where rows > cols: the same)
+ *   param = param (1 - lr weight_decay decay) - lr scale x
+ * which takes the singular values of x towards one.  Products are accurate to fp32: operands are held as two 16-bit parts, sums
+ * are fp32 of at most 256 products one behind another.  A matrix with a gradient that is not finite becomes NaN, the others are
+ * not touched by it; one whose u is zero only decays.
+ *   sizes: bytes of the plan and of the scratch, and what a step is told of the plan
+ *   plan:  a table of the work on the device, made once for given addresses (not while a stream is captured); tensors that
+ *          overlap are refused, gradients may be shared; matrices without values are allowed
+ *   step:  lr and grad_scale, where not NULL, point to device floats, the first instead of hyper->lr; *step, where not NULL, is a
+ *          device float that is counted up by one; status: a device word that is set to 1 if a bounded wait ran out (the step's
+ *          params are not to be used then), or NULL.  A step with the sizes of another plan does nothing.
+ * The scratch needs no initial value.  A plan and a scratch are for one stream at a time. */
+typedef struct {
+    float* param;
+    const float* grad;
+    float* mean;
+    int64_t rows, cols;
+    float decay, scale;
+} b2_muon_matrix;
+typedef struct {
+    double lr, momentum, eps, weight_decay, a, b, c;
+    int32_t steps, nesterov;
+} b2_muon_hyper;
+typedef struct {
+    size_t plan_bytes, scratch_bytes;
+    int64_t matrices, chunks, items;
+} b2_muon_sizes;
+int b2_muon_plan_sizes(const b2_muon_matrix* matrices, int32_t count, b2_muon_sizes* sizes);
+int b2_muon_plan(const b2_muon_matrix* matrices, int32_t count, void* plan, size_t plan_bytes, void* stream);
+int b2_muon_step(void* plan, const b2_muon_sizes* sizes, const b2_muon_hyper* hyper, const float* lr, const float* grad_scale,
+                 float* step, void* scratch, size_t scratch_bytes, int32_t* status, void* stream);
+
 /* ------------------------------------------------------------------------------------------
  * Gradient allreduce over NCCL (NVLink / NVSwitch), one process per GPU.
  * Replaces: CudaAllReduceKernel and its reduction kernel (ngraph/transformers/gpu/tensor_ops.py:

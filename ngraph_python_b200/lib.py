@@ -159,6 +159,22 @@ class AdamwHyper(C.Structure):
                 ("weight_decay", C.c_double)]
 
 
+class MuonMatrix(C.Structure):
+    """b2_muon_matrix: one matrix of an orthogonalised step."""
+    _fields_ = [("param", C.c_void_p), ("grad", C.c_void_p), ("mean", C.c_void_p), ("rows", C.c_int64), ("cols", C.c_int64),
+                ("decay", C.c_float), ("scale", C.c_float)]
+
+
+class MuonHyper(C.Structure):
+    _fields_ = [(f, C.c_double) for f in ("lr", "momentum", "eps", "weight_decay", "a", "b", "c")] + \
+        [("steps", C.c_int32), ("nesterov", C.c_int32)]
+
+
+class MuonSizes(C.Structure):
+    _fields_ = [("plan_bytes", C.c_size_t), ("scratch_bytes", C.c_size_t), ("matrices", C.c_int64), ("chunks", C.c_int64),
+                ("items", C.c_int64)]
+
+
 class CallArg(C.Structure):
     _fields_ = [("src", C.c_void_p), ("inv_scale", C.c_float), ("in_place", C.c_int32)]
 
@@ -282,6 +298,9 @@ def _load():
         "b2_adamw_plan_bytes": (C.c_int, [C.POINTER(AdamwTensor), i32, i32, C.POINTER(sz), C.POINTER(i64)]),
         "b2_adamw_plan": (C.c_int, [C.POINTER(AdamwTensor), i32, i32, vp, sz, vp]),
         "b2_adamw_step": (C.c_int, [vp, i64, i32, C.POINTER(AdamwHyper), vp, vp, vp, C.c_uint32, vp]),
+        "b2_muon_plan_sizes": (C.c_int, [C.POINTER(MuonMatrix), i32, C.POINTER(MuonSizes)]),
+        "b2_muon_plan": (C.c_int, [C.POINTER(MuonMatrix), i32, vp, sz, vp]),
+        "b2_muon_step": (C.c_int, [vp, C.POINTER(MuonSizes), C.POINTER(MuonHyper), vp, vp, vp, vp, sz, vp, vp]),
         "b2_selftest_bounded_wait": (C.c_int, [i32, vp, vp, vp]),
         "b2_set_nccl_path": (C.c_int, [C.c_char_p]),
         "b2_comm_version": (C.c_int, [C.POINTER(i32)]),
@@ -636,6 +655,17 @@ def adamw_plan_bytes(tensors, state_bits):
 
 def adamw_plan(tensors, state_bits, plan_ptr, plan_bytes, stream=0):
     check(_lib.b2_adamw_plan(tensors, len(tensors), state_bits, plan_ptr, plan_bytes, stream))
+
+
+def muon_plan_sizes(matrices):
+    """Bytes of the plan and the scratch of a step over `matrices`, an array of MuonMatrix."""
+    out = MuonSizes()
+    check(_lib.b2_muon_plan_sizes(matrices, len(matrices), C.byref(out)))
+    return out
+
+
+def muon_plan(matrices, plan_ptr, plan_bytes, stream=0):
+    check(_lib.b2_muon_plan(matrices, len(matrices), plan_ptr, plan_bytes, stream))
 
 
 def dimshuffle(src_ptr, dst_ptr, elem_bytes, shape, src_strides, dst_strides, stream=0):
