@@ -734,8 +734,8 @@ int b2_adamw_step(void* plan, int64_t chunks, int32_t state_bits, const b2_adamw
  *   u    = nesterov ? (1 - momentum) g + momentum mean : mean,   x = u / (|u| + eps),  |u| the root of the sum of squares
  *   x    = a x + (b A + c A A) x,  A = x x^T, `steps` times      (x^T x from the other side where rows > cols: the same)
  *   param = param (1 - lr weight_decay decay) - lr scale x
- * which takes the singular values of x towards one.  Products are accurate to fp32: operands are held as two 16-bit parts, sums
- * are fp32 of at most 256 products one behind another.  A matrix with a gradient that is not finite becomes NaN, the others are
+ * which takes the singular values of x towards one.  Products are accurate to fp32: operands are held as two fp16 parts, which
+ * together round as fp32 does, and three of the four products of parts are added, in fp32.  A matrix with a gradient that is not finite becomes NaN, the others are
  * not touched by it; one whose u is zero only decays.
  *   sizes: bytes of the plan and of the scratch, and what a step is told of the plan
  *   plan:  a table of the work on the device, made once for given addresses (not while a stream is captured); tensors that
@@ -757,7 +757,7 @@ typedef struct {
 } b2_muon_hyper;
 typedef struct {
     size_t plan_bytes, scratch_bytes;
-    int64_t matrices, chunks, items;
+    int64_t matrices, chunks, items, blocks;
 } b2_muon_sizes;
 int b2_muon_plan_sizes(const b2_muon_matrix* matrices, int32_t count, b2_muon_sizes* sizes);
 int b2_muon_plan(const b2_muon_matrix* matrices, int32_t count, void* plan, size_t plan_bytes, void* stream);

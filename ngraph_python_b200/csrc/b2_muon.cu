@@ -1,204 +1,606 @@
 // One optimizer step over many matrices whose updates are orthogonalised:
 //
 //   mean = mu mean + (1 - mu) g,  u = (1 - mu) g + mu mean,  x = u / (|u| + eps)
-//   `steps` times:  A = x x^T,  B = b A + c A A,  x = a x + B x
+//   `steps` times:  A = x x^T,  B = a I + b A + c A A,  x = B x          (x^T x and x B where there are more rows than columns)
 //   param = param (1 - lr wd decay) - lr scale x
+//
+// Bound by the tensor cores: 6 n^2 m + 2 n^3 operations a step for n x m (both squares are symmetric: half of each), three times
+// over, since fp32 accuracy takes three 16-bit products.  x, A and B are held as two fp16 parts, hi = the value rounded to
+// fp16, lo = the rest rounded to fp16, which together round to 2^-24 of the value as fp32 does; of (hi + lo)(hi' + lo') the
+// product lo lo' is left out, 2^-24 again.  fp16 has the range for it because the largest singular value of every operand is
+// known beforehand: x is normalised, and what the polynomial makes of [0, s] is worked out on the host, which gives each operand
+// a power of two that puts its largest possible value next to the largest of fp16.  Values down to 2^-38 of it keep a lo part.
+// (Three tf32 products give the same accuracy at half the rate; bf16 parts have 8 bits each, 2^-17 together.)
+//
+// Storage: blocks of 64 x 64 values, hi and lo behind one another, each 8 KB as the tensor core reads it from shared memory
+// (rows of 128 bytes whose 16-byte pieces are swizzled by the row), so that an operand tile is a few bulk copies without a
+// descriptor, whatever the matrix's own rows are like.  A block serves as rows of an operand (its k along the columns) and
+// as columns of one (k along the rows) alike: the instruction reads both, so that x is neither transposed nor kept twice.
+// What lies outside the matrix is zero and stays zero.
+//
+// Four launches for all matrices and steps: the mean and the sums of squares; x in parts; the products.  The products are
+// one launch for all steps: work items -- a tile of A, B or x of one matrix -- are numbered so that what an item reads has lower
+// numbers, CTAs take the next number when they are done with one, and an item waits until its matrix has counted the items
+// that it reads.  Only items that a running CTA has taken are waited for, so that it does not matter how many CTAs run.
+// With a launch for each product the last wave of tiles of every one of 15 would leave SMs idle.
 #include <algorithm>
 #include <cmath>
 #include <cstdint>
 #include <new>
 #include <vector>
 
+#include <cuda_fp16.h>
+
+#include "b2_gemm_impl.cuh"
 #include "b2_operators.h"
 
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kTile = 64, kDepth = 16;
-constexpr int kMostSteps = 100;
+constexpr int kMeanThreads = 256;
+constexpr int kMostSteps = 32;
 constexpr long long kMostSide = 1 << 20, kMostShort = 1 << 15;
+constexpr int kBlock = 64;                                  // rows and columns of a block
+constexpr int kBlockBytes = kBlock * kBlock * 2;            // of one part
+constexpr int kBlockPair = 2 * kBlockBytes;
 
-// One matrix.  Offsets are values of the scratch, from its aligned start on.
+enum { GRAM = 0, POLY = 1, MULTIPLY = 2 };
+
+// One matrix.  Offsets are bytes of the scratch, from the first plane on.
 struct Matrix {
     float* param;
     const float* grad;
     float* mean;
-    long long x[2], square, poly;            // two turns of x [rows][cols], A and B [n][n]
-    int rows, cols, n, m;                    // n, m: the shorter and the longer side
+    long long x[2], square, poly;            // two turns of x [row blocks][column blocks], A and B [n blocks][n blocks]
+    int rows, cols, row_blocks, col_blocks, n_blocks, tall;
+    int items[3];                            // of a step, by phase
     int first_chunk, chunks;
     float decay, scale;
+    int unused;
 };
-struct Chunk {
+struct Chunk {                               // values of a matrix whose squares one CTA adds
     int matrix, n;
     long long at;
 };
-struct Item {
+struct Block {                               // one block of x
+    int matrix, at;
+};
+struct Item {                                // a tile: 128 rows from block 2 i on, `width` blocks of columns from block j on
     int matrix;
+    short phase, width;
     int i, j;
 };
+struct Group {                               // matrices whose steps run next to one another; items of one step
+    long long first, count;
+};
 struct Header {
-    long long matrices, chunks, items;
-    long long squares, products;             // items of a product n x n, and of one with x
+    long long matrices, chunks, items, blocks, groups;
 };
 constexpr size_t kHeader = 64;
 
 struct Layout {
     std::vector<Matrix> matrices;
     std::vector<Chunk> chunks;
-    std::vector<Item> squares, products;
-    long long values;                        // of the scratch
+    std::vector<Block> blocks;
+    std::vector<Item> items;
+    std::vector<Group> groups;
+    long long bytes;                         // of planes
     size_t plan_bytes() const {
-        return kHeader + matrices.size() * sizeof(Matrix) + chunks.size() * sizeof(Chunk) + (squares.size() + products.size()) * sizeof(Item);
+        return kHeader + matrices.size() * sizeof(Matrix) + chunks.size() * sizeof(Chunk) + blocks.size() * sizeof(Block) + items.size() * sizeof(Item) +
+               groups.size() * sizeof(Group);
     }
 };
 
 struct Rates {
-    float mu, rest, eps, a, b, c;
+    float mu, rest, eps;
     double lr, wd;
     int nesterov;
 };
+// Powers of two that operands are stored with, by step, and the polynomial.
+struct Poly {
+    float a, b, c;
+    int steps;
+    signed char x[kMostSteps + 1], square[kMostSteps], poly[kMostSteps];
+};
+__device__ __forceinline__ float power(int e) { return __int_as_float((e + 127) << 23); }
 
 __device__ __forceinline__ const Header* header_of(const void* plan) { return static_cast<const Header*>(plan); }
 __device__ __forceinline__ const Matrix* matrices_of(const void* plan) { return reinterpret_cast<const Matrix*>(static_cast<const char*>(plan) + kHeader); }
 __device__ __forceinline__ const Chunk* chunks_of(const void* plan) { return reinterpret_cast<const Chunk*>(matrices_of(plan) + header_of(plan)->matrices); }
-__device__ __forceinline__ const Item* items_of(const void* plan) { return reinterpret_cast<const Item*>(chunks_of(plan) + header_of(plan)->chunks); }
-__device__ __forceinline__ bool fits(const void* plan, long long matrices, long long chunks, long long items) {
+__device__ __forceinline__ const Block* blocks_of(const void* plan) { return reinterpret_cast<const Block*>(chunks_of(plan) + header_of(plan)->chunks); }
+__device__ __forceinline__ const Item* items_of(const void* plan) { return reinterpret_cast<const Item*>(blocks_of(plan) + header_of(plan)->blocks); }
+__device__ __forceinline__ const Group* groups_of(const void* plan) { return reinterpret_cast<const Group*>(items_of(plan) + header_of(plan)->items); }
+
+struct Told {                                // what the caller says of the plan; a step with other sizes does nothing
+    long long matrices, chunks, items, blocks;
+};
+__device__ __forceinline__ bool fits(const void* plan, const Told& t) {
     const Header* h = header_of(plan);
-    return h->matrices == matrices && h->chunks == chunks && h->items == items;
+    return h->matrices == t.matrices && h->chunks == t.chunks && h->items == t.items && h->blocks == t.blocks;
 }
 
-// u of a chunk, to the first turn of x, the mean, and the sum of squares in 64 bits
-__global__ void __launch_bounds__(kThreads)
-muon_mean_kernel(const void* plan, long long matrices, long long chunks, long long items, const Rates r, const float* grad_scale, float* step,
-                 double* sums, float* scratch) {
-    __shared__ double words[kThreads / 32];
+// The scratch: sums of squares by chunk; counters; planes.
+struct Room {
+    double* sums;
+    unsigned* next;                          // the number of the next item, whether a wait ran out, and by matrix the items done
+    unsigned* failed;
+    unsigned* done;
+    char* planes;
+};
+
+__device__ __forceinline__ double cta_sum(double q, double* words) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) q += __shfl_xor_sync(0xffffffffu, q, o);
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) words[threadIdx.x >> 5] = q;
+    __syncthreads();
+    q = 0.0;
+    for (int w = 0; w < kMeanThreads / 32; ++w) q += words[w];
+    return q;
+}
+
+// The mean of a chunk and the sum of squares of its u, in 64 bits: squares of any gradient fit
+__global__ void __launch_bounds__(kMeanThreads)
+muon_mean_kernel(const void* plan, const Told told, const Rates r, const float* grad_scale, float* step, const Room room) {
+    __shared__ double words[kMeanThreads / 32];
     after_earlier_kernels();
-    if (!fits(plan, matrices, chunks, items)) return;
-    if (blockIdx.x == 0 && threadIdx.x == 0 && step) *step += 1.0f;
+    if (!fits(plan, told)) return;
+    if (blockIdx.x == 0) {
+        if (threadIdx.x == 0 && step) *step += 1.0f;
+        if (threadIdx.x == 0) *room.next = *room.failed = 0;
+        for (long long i = threadIdx.x; i < told.matrices; i += kMeanThreads) room.done[i] = 0;
+    }
     const float s = grad_scale ? *grad_scale : 1.0f;
-    for (long long k = blockIdx.x; k < chunks; k += gridDim.x) {
+    for (long long k = blockIdx.x; k < told.chunks; k += gridDim.x) {
         const Chunk c = chunks_of(plan)[k];
         const Matrix& t = matrices_of(plan)[c.matrix];
         double q = 0.0;
-        for (int i = threadIdx.x; i < c.n; i += kThreads) {
+        for (int i = threadIdx.x; i < c.n; i += kMeanThreads) {
             const float g = t.grad[c.at + i] * s, m = r.mu * t.mean[c.at + i] + r.rest * g;
             const float u = r.nesterov ? r.rest * g + r.mu * m : m;
             t.mean[c.at + i] = m;
-            scratch[t.x[0] + c.at + i] = u;
             q = fma((double)u, (double)u, q);
         }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) q += __shfl_xor_sync(0xffffffffu, q, o);
-        __syncthreads();
-        if ((threadIdx.x & 31) == 0) words[threadIdx.x >> 5] = q;
-        __syncthreads();
-        if (threadIdx.x == 0) {
-            for (int w = 1; w < kThreads / 32; ++w) q += words[w];
-            sums[k] = q;
-        }
+        q = cta_sum(q, words);
+        if (threadIdx.x == 0) room.sums[k] = q;
     }
 }
 
-__global__ void __launch_bounds__(kThreads)
-muon_scale_kernel(const void* plan, long long matrices, long long chunks, long long items, float eps, const double* sums, float* scratch) {
-    __shared__ double words[kThreads / 32];
+// Two values as two fp16 parts each
+__device__ __forceinline__ void parts(float u, float v, unsigned& hi, unsigned& lo) {
+    const __half2 h = __floats2half2_rn(u, v);
+    const float2 f = __half22float2(h);
+    const __half2 l = __floats2half2_rn(u - f.x, v - f.y);
+    hi = *reinterpret_cast<const unsigned*>(&h);
+    lo = *reinterpret_cast<const unsigned*>(&l);
+}
+// Eight values next to one another of row `row` of a block, 8 `piece` columns in
+__device__ __forceinline__ void put_piece(char* block, int row, int piece, const float* v) {
+    uint4 hi, lo;
+    parts(v[0], v[1], hi.x, lo.x);
+    parts(v[2], v[3], hi.y, lo.y);
+    parts(v[4], v[5], hi.z, lo.z);
+    parts(v[6], v[7], hi.w, lo.w);
+    char* at = block + row * 128 + ((piece ^ (row & 7)) << 4);
+    *reinterpret_cast<uint4*>(at) = hi;
+    *reinterpret_cast<uint4*>(at + kBlockBytes) = lo;
+}
+__device__ __forceinline__ float2 halves(unsigned w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
+__device__ __forceinline__ void get_piece(const char* block, int row, int piece, float* v) {
+    const char* at = block + row * 128 + ((piece ^ (row & 7)) << 4);
+    const uint4 hi = __ldcg(reinterpret_cast<const uint4*>(at)), lo = __ldcg(reinterpret_cast<const uint4*>(at + kBlockBytes));
+    const unsigned h[4] = {hi.x, hi.y, hi.z, hi.w}, l[4] = {lo.x, lo.y, lo.z, lo.w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const float2 a = halves(h[k]), b = halves(l[k]);
+        v[2 * k] = a.x + b.x;
+        v[2 * k + 1] = a.y + b.y;
+    }
+}
+
+// x of the first step, a block at a time
+__global__ void __launch_bounds__(kMeanThreads)
+muon_parts_kernel(const void* plan, const Told told, const Rates r, const float* grad_scale, int exponent, const Room room) {
+    __shared__ double words[kMeanThreads / 32];
     after_earlier_kernels();
-    if (!fits(plan, matrices, chunks, items)) return;
-    for (long long k = blockIdx.x; k < chunks; k += gridDim.x) {
-        const Chunk c = chunks_of(plan)[k];
+    if (!fits(plan, told)) return;
+    const float s = grad_scale ? *grad_scale : 1.0f;
+    for (long long k = blockIdx.x; k < told.blocks; k += gridDim.x) {
+        const Block c = blocks_of(plan)[k];
         const Matrix& t = matrices_of(plan)[c.matrix];
         double q = 0.0;
-        for (int i = threadIdx.x; i < t.chunks; i += kThreads) q += sums[t.first_chunk + i];
+        for (int i = threadIdx.x; i < t.chunks; i += kMeanThreads) q += room.sums[t.first_chunk + i];
+        q = cta_sum(q, words);
+        const float inverse = (float)(1.0 / (sqrt(q) + (double)r.eps)), up = power(exponent);
+        const int rb = c.at / t.col_blocks, cb = c.at - rb * t.col_blocks;
+        char* block = room.planes + t.x[0] + (long long)c.at * kBlockPair;
+        for (int e = threadIdx.x; e < kBlock * 8; e += kMeanThreads) {
+            const int row = e >> 3, piece = e & 7;
+            const int at_row = rb * kBlock + row, at_col = cb * kBlock + piece * 8;
+            float v[8];
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) q += __shfl_xor_sync(0xffffffffu, q, o);
-        __syncthreads();
-        if ((threadIdx.x & 31) == 0) words[threadIdx.x >> 5] = q;
-        __syncthreads();
-        q = 0.0;
-        for (int w = 0; w < kThreads / 32; ++w) q += words[w];
-        const float inverse = (float)(1.0 / (sqrt(q) + (double)eps));
-        for (int i = threadIdx.x; i < c.n; i += kThreads) scratch[t.x[0] + c.at + i] *= inverse;
+            for (int j = 0; j < 8; ++j) {
+                float u = 0.0f;
+                if (at_row < t.rows && at_col + j < t.cols) {
+                    const long long at = (long long)at_row * t.cols + at_col + j;
+                    const float m = t.mean[at];
+                    u = r.nesterov ? r.rest * (t.grad[at] * s) + r.mu * m : m;
+                    u = u * inverse * up;
+                }
+                v[j] = u;
+            }
+            put_piece(block, row, piece, v);
+        }
     }
 }
 
-// A tile of one product.  phase 0: A = x x^T (x^T x), 1: B = b A + c A A, 2: x = a x + B x (x B), the last of which moves the
-// param instead.  P [rows of the tile][k], Q [k][columns], by strides.
-__global__ void __launch_bounds__(kThreads)
-muon_product_kernel(const void* plan, long long matrices, long long chunks, long long items, int phase, int turn, int last, const Rates r, const float* lr,
-                    float* scratch) {
-    __shared__ float p_tile[kDepth][kTile + 4], q_tile[kDepth][kTile + 4];
-    after_earlier_kernels();
-    if (!fits(plan, matrices, chunks, items)) return;
-    if (blockIdx.x >= (phase == 2 ? header_of(plan)->products : header_of(plan)->squares)) return;
-    const Item item = items_of(plan)[(phase == 2 ? header_of(plan)->squares : 0) + blockIdx.x];
-    const Matrix& t = matrices_of(plan)[item.matrix];
-    const bool tall = t.rows > t.cols;
-    const float *x = scratch + t.x[turn], *square = scratch + t.square, *poly = scratch + t.poly;
-    const float *P, *Q;
-    long long p_row, p_k, q_k, q_col;
-    int M = t.n, N = t.n, K = t.n;
-    if (phase == 0) {
-        P = Q = x;
-        K = t.m;
-        p_row = q_col = tall ? 1 : t.cols;
-        p_k = q_k = tall ? t.cols : 1;
-    } else if (phase == 1) {
-        P = Q = square;
-        p_row = q_k = t.n;
-        p_k = q_col = 1;
+// ---- the products ------------------------------------------------------------------------------------------
+constexpr int kUnit = 32 << 10, kUnits = 6;                 // the ring: both parts of 128 rows of P, of Q up to 128, or one part of more
+constexpr int kQueue = 4;
+constexpr int kEpilogueWarps = 8;
+constexpr int kProductThreads = 64 + 32 * kEpilogueWarps;
+constexpr int kStagePitch = 33;
+constexpr int kStage = 32 * kStagePitch * 4;                // of a warp of the epilogue: 32 x 32 values
+constexpr int kProductShared = 1024 + kUnits * kUnit + kEpilogueWarps * kStage + 512;
+static_assert(kProductShared <= 227 << 10, "shared memory of a CTA");
+// Blocks of k that are added in tensor memory, whose sums lose what they add: 640 x 1920 is 2.8e-6 off in the 2-norm with one
+// (numpy's fp32 2.2e-6), 6.4e-6 with two, 1.2e-5 with four, for 3.92, 3.77 and 3.60 ms of 48 matrices.  The small products
+// go first.  The rest is added in registers.
+constexpr int kChain = 1;
+constexpr int kDependencyPolls = 1 << 22;
+
+struct Work {
+    int matrix, phase, step, i, j, width, k_blocks, unused;
+};
+// Where the blocks of an operand lie: 128 rows (or columns) of tiles by `mn`, k by `k`, in blocks
+struct Operand {
+    const char* base;
+    int mn, k, last;
+    unsigned major;                          // 1: k along the rows of the storage
+};
+__device__ __forceinline__ Operand operand_of(const Matrix& t, const char* planes, int phase, int turn, bool second) {
+    const bool x = phase == GRAM || (phase == MULTIPLY && (second != (t.tall != 0)));
+    if (!x) return {planes + (phase == POLY ? t.square : t.poly), t.n_blocks, 1, t.n_blocks - 1, 0};
+    const char* base = planes + t.x[turn];
+    const bool columns = phase == GRAM ? t.tall != 0 : second;
+    if (columns) return {base, 1, t.col_blocks, t.col_blocks - 1, 1};
+    return {base, t.col_blocks, 1, t.row_blocks - 1, 0};
+}
+// a shared-memory descriptor: 128-byte swizzle, groups of eight rows 1024 bytes apart; k along the rows: groups of 64 columns a block apart
+__device__ __forceinline__ unsigned long long describe(unsigned address, unsigned major) {
+    unsigned long long d = (address >> 4) & 0x3FFF;
+    d |= (unsigned long long)(major ? kBlockBytes >> 4 : 1) << 16;
+    d |= (unsigned long long)(1024 >> 4) << 32;
+    d |= (unsigned long long)1 << 46;
+    d |= (unsigned long long)2 << 61;
+    return d;
+}
+__device__ __forceinline__ void multiply_f16(unsigned d, unsigned long long a, unsigned long long b, unsigned instruction, unsigned accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(d), "l"(a), "l"(b), "r"(instruction), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void copy_block(unsigned to, const char* from, unsigned bytes, unsigned long long* bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 ::"r"(to), "l"(from), "r"(bytes), "r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ unsigned load_acquire(const unsigned* p) {
+    unsigned v;
+    asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
+    return v;
+}
+
+__global__ void __launch_bounds__(kProductThreads, 1)
+muon_product_kernel(const void* plan, const Told told, const Rates r, const Poly poly, const float* lr, const Room room, int* status) {
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char* smem = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    float* stages = reinterpret_cast<float*>(smem + kUnits * kUnit);
+    unsigned long long* full_bar = reinterpret_cast<unsigned long long*>(smem + kUnits * kUnit + kEpilogueWarps * kStage);
+    unsigned long long* empty_bar = full_bar + kUnits;
+    unsigned long long* sum_full = empty_bar + kUnits;          // [2]
+    unsigned long long* sum_empty = sum_full + 2;               // [2]
+    unsigned long long* queue_full = sum_empty + 2;
+    unsigned long long* queue_empty = queue_full + kQueue;
+    Work* queue = reinterpret_cast<Work*>(queue_empty + kQueue);
+    unsigned* tmem_holder = reinterpret_cast<unsigned*>(queue + kQueue);
+    int* fail_flag = reinterpret_cast<int*>(tmem_holder + 1);
+
+    const int warp = warp_uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kUnits; ++s) { mbar_init(&full_bar[s], 1); mbar_init(&empty_bar[s], 1); }
+        for (int b = 0; b < 2; ++b) { mbar_init(&sum_full[b], 1); mbar_init(&sum_empty[b], kEpilogueWarps); }
+        for (int q = 0; q < kQueue; ++q) { mbar_init(&queue_full[q], 1); mbar_init(&queue_empty[q], 1 + kEpilogueWarps); }
+        *fail_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        tmem_alloc(tmem_holder, 512);
+        asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    }
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const unsigned tmem_base = (unsigned)warp_uniform((int)*tmem_holder);
+    const bool mine = fits(plan, told);                         // (else no item is taken)
+    const Matrix* matrices = matrices_of(plan);
+
+    if (warp == 0) {
+        if (elect_one()) {
+            int s = 0, q = 0;
+            unsigned parity = 1, queue_parity = 1;
+            bool ok = true;
+            long long group = 0;
+            const long long total = mine ? told.items * poly.steps : 0;
+            for (;;) {
+                // the next item
+                Work w = {};
+                w.phase = -1;
+                const long long number = ok && total ? (long long)atomicAdd(room.next, 1u) : total;
+                if (number < total && !*reinterpret_cast<volatile unsigned*>(room.failed)) {
+                    const Group* g = groups_of(plan) + group;
+                    while (number >= poly.steps * (g->first + g->count)) { ++g; ++group; }
+                    const long long in = number - poly.steps * g->first;
+                    w.step = (int)(in / g->count);
+                    const Item item = items_of(plan)[g->first + (in - w.step * g->count)];
+                    const Matrix& t = matrices[item.matrix];
+                    w.matrix = item.matrix;
+                    w.phase = item.phase;
+                    w.i = item.i;
+                    w.j = item.j;
+                    w.width = item.width;
+                    w.k_blocks = item.phase == GRAM ? (t.tall ? t.row_blocks : t.col_blocks) : t.n_blocks;
+                    // what it reads has been stored
+                    const int before = w.step * (t.items[0] + t.items[1] + t.items[2]) + (item.phase > GRAM ? t.items[0] : 0) + (item.phase > POLY ? t.items[1] : 0);
+                    const unsigned need = (unsigned)before * kEpilogueWarps;
+                    bool there = false;
+                    for (int i = 0; i < kDependencyPolls && !there; ++i) {
+                        there = (int)(load_acquire(room.done + item.matrix) - need) >= 0;
+                        if (!there) {
+                            if (*reinterpret_cast<volatile unsigned*>(room.failed)) break;
+                            __nanosleep(40);
+                        }
+                    }
+                    asm volatile("fence.proxy.async;" ::: "memory");
+                    if (!there) {
+                        atomicExch(fail_flag, 1);
+                        ok = false;
+                        w.phase = -1;
+                    }
+                }
+                if (!mbar_wait(&queue_empty[q], queue_parity)) { atomicExch(fail_flag, 1); break; }
+                queue[q] = w;
+                mbar_arrive(&queue_full[q]);
+                if (++q == kQueue) { q = 0; queue_parity ^= 1u; }
+                if (w.phase < 0) break;
+                const Matrix& t = matrices[w.matrix];
+                const Operand P = operand_of(t, room.planes, w.phase, w.step & 1, false), Q = operand_of(t, room.planes, w.phase, w.step & 1, true);
+                const long long p0 = (long long)(2 * w.i) * P.mn, p1 = (long long)min(2 * w.i + 1, P.last) * P.mn;
+                auto unit = [&](unsigned bytes) {
+                    if (!mbar_wait(&empty_bar[s], parity)) { atomicExch(fail_flag, 1); ok = false; return false; }
+                    mbar_expect_tx(&full_bar[s], bytes);
+                    return true;
+                };
+                auto next = [&] { if (++s == kUnits) { s = 0; parity ^= 1u; } };
+                for (int kb = 0; kb < w.k_blocks && ok; ++kb) {
+                    const long long k = (long long)kb * P.k, l = (long long)kb * Q.k;
+                    if (!unit(4 * kBlockBytes)) break;
+                    unsigned to = smem_u32(smem + s * kUnit);
+                    for (int part = 0; part < 2; ++part) {
+                        copy_block(to + part * 2 * kBlockBytes, P.base + (p0 + k) * kBlockPair + part * kBlockBytes, kBlockBytes, &full_bar[s]);
+                        copy_block(to + part * 2 * kBlockBytes + kBlockBytes, P.base + (p1 + k) * kBlockPair + part * kBlockBytes, kBlockBytes, &full_bar[s]);
+                    }
+                    next();
+                    const bool both = w.width <= 2;             // parts of Q in one unit
+                    for (int part = 0; part < 2; ++part) {
+                        if (part == 0 || !both)
+                            if (!unit((both ? 2 : 1) * w.width * kBlockBytes)) break;
+                        to = smem_u32(smem + s * kUnit) + (both ? part * w.width * kBlockBytes : 0);
+                        for (int n = 0; n < w.width; ++n)
+                            copy_block(to + n * kBlockBytes, Q.base + ((long long)(w.j + n) * Q.mn + l) * kBlockPair + (part ^ 1) * kBlockBytes, kBlockBytes, &full_bar[s]);
+                        if (part == 1 || !both) next();
+                    }
+                }
+            }
+            // copies in flight have landed, and have been read, before the CTA may end
+            for (int i = 0; i < kUnits && ok; ++i) {
+                if (!mbar_wait(&empty_bar[s], parity)) { atomicExch(fail_flag, 1); ok = false; }
+                if (++s == kUnits) { s = 0; parity ^= 1u; }
+            }
+        }
+    } else if (warp == 1) {
+        if (elect_one()) {
+            int s = 0, q = 0, chain = 0;
+            unsigned parity = 0, queue_parity = 0;
+            bool ok = true;
+            auto wait_unit = [&] {
+                if (!mbar_wait(&full_bar[s], parity)) { atomicExch(fail_flag, 1); ok = false; }
+                tc_fence_after();
+                return smem_u32(smem + s * kUnit);
+            };
+            auto next = [&] { if (++s == kUnits) { s = 0; parity ^= 1u; } };
+            while (ok) {
+                if (!mbar_wait_relaxed(&queue_full[q], queue_parity)) { atomicExch(fail_flag, 1); break; }
+                const Work w = queue[q];
+                mbar_arrive(&queue_empty[q]);
+                if (++q == kQueue) { q = 0; queue_parity ^= 1u; }
+                if (w.phase < 0) break;
+                const Matrix& t = matrices[w.matrix];
+                const unsigned p_major = operand_of(t, room.planes, w.phase, 0, false).major, q_major = operand_of(t, room.planes, w.phase, 0, true).major;
+                // fp16 operands, fp32 sums, 128 rows
+                const unsigned instruction = (1u << 4) | (p_major << 15) | (q_major << 16) | ((unsigned)(w.width * kBlock >> 3) << 17) | ((128u >> 4) << 24);
+                const unsigned p_step = p_major ? 2048 >> 4 : 32 >> 4, q_step = q_major ? 2048 >> 4 : 32 >> 4;       // 16 of k
+                const bool both = w.width <= 2;
+                for (int kb = 0; kb < w.k_blocks && ok; ++kb) {
+                    const int in = kb % kChain, b = chain & 1;
+                    if (in == 0) {
+                        // the sums before in these columns have been read
+                        if (chain > 1 && !mbar_wait(&sum_empty[b], ((chain >> 1) - 1) & 1)) { atomicExch(fail_flag, 1); ok = false; break; }
+                        tc_fence_after();
+                    }
+                    const unsigned sum = tmem_base + b * 256;
+                    const int p_unit = s;
+                    const unsigned p_at = wait_unit();
+                    next();
+                    unsigned q_at = wait_unit();
+                    if (!ok) break;
+                    const unsigned long long p_hi = describe(p_at, p_major), p_lo = describe(p_at + 2 * kBlockBytes, p_major);
+                    unsigned long long q_part = describe(q_at, q_major);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) multiply_f16(sum, p_hi + k * p_step, q_part + k * q_step, instruction, in > 0 || k > 0);
+                    if (both) {
+                        q_part = describe(q_at + w.width * kBlockBytes, q_major);
+                    } else {
+                        tc_commit(&empty_bar[s]);
+                        next();
+                        q_at = wait_unit();
+                        if (!ok) break;
+                        q_part = describe(q_at, q_major);
+                    }
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) multiply_f16(sum, p_lo + k * p_step, q_part + k * q_step, instruction, 1);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) multiply_f16(sum, p_hi + k * p_step, q_part + k * q_step, instruction, 1);
+                    tc_commit(&empty_bar[p_unit]);
+                    tc_commit(&empty_bar[s]);
+                    next();
+                    if (in == kChain - 1 || kb == w.k_blocks - 1) {
+                        tc_commit(&sum_full[b]);
+                        ++chain;
+                    }
+                }
+            }
+        }
     } else {
-        M = t.rows;
-        N = t.cols;
-        P = tall ? x : poly;
-        Q = tall ? poly : x;
-        p_row = tall ? t.cols : t.n;
-        q_k = tall ? t.n : t.cols;
-        p_k = q_col = 1;
-    }
-    const int m0 = item.i * kTile, n0 = item.j * kTile;
-    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    float sum[4][4] = {};
-    for (int k0 = 0; k0 < K; k0 += kDepth) {
-        for (int e = threadIdx.x; e < kTile * kDepth; e += kThreads) {
-            // neighbours in memory to neighbouring threads
-            const int a = p_k == 1 ? e / kDepth : e % kTile, ka = p_k == 1 ? e % kDepth : e / kTile;
-            p_tile[ka][a] = m0 + a < M && k0 + ka < K ? P[(m0 + a) * p_row + (k0 + ka) * p_k] : 0.0f;
-            const int b = q_k == 1 ? e / kDepth : e % kTile, kb = q_k == 1 ? e % kDepth : e / kTile;
-            q_tile[kb][b] = n0 + b < N && k0 + kb < K ? Q[(k0 + kb) * q_k + (n0 + b) * q_col] : 0.0f;
-        }
-        __syncthreads();
+        // the epilogue: a quarter of the lanes (32 rows) and half of the columns to a warp
+        const int quarter = warp & 3, half = (warp - 2) >> 2;
+        float* stage = stages + (warp - 2) * (kStage / 4);
+        const unsigned lanes = tmem_base + ((unsigned)(quarter * 32) << 16);
+        int q = 0, chain = 0;
+        unsigned queue_parity = 0;
+        bool ok = true;
+        for (;;) {
+            if (!mbar_wait_relaxed(&queue_full[q], queue_parity)) { atomicExch(fail_flag, 1); break; }
+            const Work w = queue[q];
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&queue_empty[q]);
+            if (++q == kQueue) { q = 0; queue_parity ^= 1u; }
+            if (w.phase < 0) break;
+            const int cols = w.width * 32, from = half * cols;
+            float sum[128];
 #pragma unroll
-        for (int k = 0; k < kDepth; ++k) {
-            float u[4], v[4];
+            for (int j = 0; j < 128; ++j) sum[j] = 0.0f;
+            for (int kb = 0; kb < w.k_blocks; kb += kChain, ++chain) {
+                const int b = chain & 1;
+                if (ok && !mbar_wait(&sum_full[b], (chain >> 1) & 1)) { atomicExch(fail_flag, 1); ok = false; }
+                tc_fence_after();
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                u[j] = p_tile[k][ty * 4 + j];
-                v[j] = q_tile[k][tx * 4 + j];
+                for (int c0 = 0; c0 < 128; c0 += 32) {
+                    if (c0 < cols) {
+                        unsigned v[32];
+                        tmem_ld16(lanes + b * 256 + from + c0, v);
+                        tmem_ld16(lanes + b * 256 + from + c0 + 16, v + 16);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) sum[c0 + j] += __uint_as_float(v[j]);
+                    }
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sum_empty[b]);
             }
+            const Matrix& t = matrices[w.matrix];
+            const int rb = 2 * w.i + (quarter >> 1), in_row = (quarter & 1) * 32 + lane, k = w.step;
+            const bool last = w.phase == MULTIPLY && k == poly.steps - 1;
+            const int row_blocks = w.phase == MULTIPLY ? t.row_blocks : t.n_blocks, col_blocks = w.phase == MULTIPLY ? t.col_blocks : t.n_blocks;
+            char* planes = room.planes + (w.phase == GRAM ? t.square : w.phase == POLY ? t.poly : t.x[(k + 1) & 1]);
+            const int into = w.phase == GRAM ? poly.square[k] - 2 * poly.x[k] : w.phase == POLY ? poly.poly[k] - 2 * poly.square[k] : poly.x[k + 1] - poly.x[k] - poly.poly[k];
+            const float factor = w.phase == POLY ? poly.c * power(into) : last ? power(-poly.x[k] - poly.poly[k]) : power(into);
+            const float linear = poly.b * power(poly.poly[k] - poly.square[k]), diagonal = poly.a * power(poly.poly[k]);
+            float keep = 1.0f, move = 0.0f;
+            if (last) {
+                const double rate = lr ? (double)*lr : r.lr;
+                keep = (float)(1.0 - rate * r.wd * (double)t.decay);
+                move = (float)(rate * (double)t.scale);
+            }
+            if (rb < row_blocks && ok) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+                for (int c0 = 0; c0 < 128; c0 += 32) {
+                    const int cb = w.j + ((from + c0) >> 6), in_col = (from + c0) & 63;
+                    // of what is symmetric the upper half, stored twice
+                    if (c0 >= cols || (w.phase != MULTIPLY && rb > cb)) continue;
+                    float* v = sum + c0;
+                    const long long at = ((long long)rb * col_blocks + cb) * kBlockPair;
+                    if (w.phase == POLY) {
+                        const char* square = room.planes + t.square + at;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) sum[i][j] = fmaf(u[i], v[j], sum[i][j]);
-        }
-        __syncthreads();
-    }
-    const double rate = lr ? (double)*lr : r.lr;
-    const float keep = (float)(1.0 - rate * r.wd * (double)t.decay), move = (float)(rate * (double)t.scale);
+                        for (int e = 0; e < 4; ++e) {
+                            float old[8];
+                            get_piece(square, in_row, (in_col >> 3) + e, old);
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+                            for (int j = 0; j < 8; ++j) {
+                                const int col = cb * kBlock + in_col + 8 * e + j;
+                                v[8 * e + j] = fmaf(linear, old[j], factor * v[8 * e + j]);
+                                if (rb * kBlock + in_row == col && col < min(t.rows, t.cols)) v[8 * e + j] += diagonal;
+                            }
+                        }
+                    } else {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const long long row = m0 + ty * 4 + i, col = n0 + tx * 4 + j;
-            if (row >= M || col >= N) continue;
-            const long long at = row * N + col;
-            if (phase == 0) scratch[t.square + at] = sum[i][j];
-            else if (phase == 1) scratch[t.poly + at] = fmaf(r.b, square[at], r.c * sum[i][j]);
-            else {
-                const float y = fmaf(r.a, x[at], sum[i][j]);
-                if (!last) scratch[t.x[turn ^ 1] + at] = y;
-                else t.param[at] = t.param[at] * keep - move * y;
+                        for (int j = 0; j < 32; ++j) v[j] *= factor;
+                    }
+                    if (!last) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) put_piece(planes + at, in_row, (in_col >> 3) + e, v + 8 * e);
+                    }
+                    const bool mirror = w.phase != MULTIPLY && rb < cb;
+                    if (!mirror && !last) continue;
+                    __syncwarp();
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) stage[lane * kStagePitch + j] = v[j];
+                    __syncwarp();
+                    if (mirror) {
+                        // a lane to eight rows of a column: four lanes to a column of the 32 rows
+                        char* there = planes + ((long long)cb * col_blocks + rb) * kBlockPair;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int col = 8 * e + (lane >> 2), row = 8 * (lane & 3);
+                            float y[8];
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) y[j] = stage[(row + j) * kStagePitch + col];
+                            put_piece(there, in_col + col, ((quarter & 1) * 32 + row) >> 3, y);
+                        }
+                    } else {
+                        const int col = cb * kBlock + in_col + lane, row0 = rb * kBlock + (quarter & 1) * 32;
+                        if (col < t.cols)
+#pragma unroll 8
+                            for (int j = 0; j < 32; ++j)
+                                if (row0 + j < t.rows) {
+                                    float* p = t.param + (long long)(row0 + j) * t.cols + col;
+                                    *p = *p * keep - move * stage[j * kStagePitch + lane];
+                                }
+                    }
+                }
+            }
+            if (!last) {
+                // stored for the copies of other CTAs
+                asm volatile("fence.proxy.async;" ::: "memory");
+                __threadfence();
+                __syncwarp();
+                if (lane == 0) asm volatile("red.release.gpu.global.add.u32 [%0], %1;" ::"l"(room.done + w.matrix), "r"(ok ? 1u : 0u) : "memory");
             }
         }
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc(tmem_base, 512);
+    }
+    if (threadIdx.x == 0 && *fail_flag) {
+        atomicExch(room.failed, 1u);
+        if (status) atomicExch(status, 1);
+    }
 }
 
 int check_matrices(const b2_muon_matrix* list, int count) {
@@ -215,12 +617,28 @@ int check_matrices(const b2_muon_matrix* list, int count) {
     return B2_OK;
 }
 
+constexpr int blocks_in(long long n) { return (int)((n + kBlock - 1) / kBlock); }
+
+// The tiles of a product of rb x cb blocks, upper triangle alone where `half`: [i, j, width]
+template <typename F>
+void tiles_of(int rb, int cb, bool half, int width, F&& tile) {
+    for (int i = 0; 2 * i < rb; ++i)
+        for (int j = half ? 2 * i : 0; j < cb; j += width) tile(i, j, std::min(width, cb - j));
+}
+
+// Cycles of an item: blocks of k, each bound by the tensor core from 192 columns on and by its copies below, and what starts and
+// ends it.
+double cycles_of(int width, int k_blocks) {
+    static const double block[5] = {0, 700, 950, 1300, 1600};
+    return block[width] * k_blocks + 3000;
+}
+
 Layout layout_of(const b2_muon_matrix* list, int count) {
     Layout found;
     long long at = 0;
-    const auto take = [&](long long n) {
+    const auto take = [&](long long blocks) {
         const long long from = at;
-        at += (n + 63) / 64 * 64;
+        at += blocks * kBlockPair;
         return from;
     };
     for (int i = 0; i < count; ++i) {
@@ -232,40 +650,100 @@ Layout layout_of(const b2_muon_matrix* list, int count) {
         t.mean = s.mean;
         t.rows = (int)s.rows;
         t.cols = (int)s.cols;
-        t.n = std::min(t.rows, t.cols);
-        t.m = std::max(t.rows, t.cols);
+        t.tall = t.rows > t.cols;
         t.decay = s.decay;
         t.scale = s.scale;
-        const long long size = s.rows * s.cols;
-        t.x[0] = take(size);
-        t.x[1] = take(size);
-        t.square = take((long long)t.n * t.n);
-        t.poly = take((long long)t.n * t.n);
-        t.first_chunk = (int)found.chunks.size();
-        const long long each = std::max(2048ll, (size / 512 + 2047) / 2048 * 2048);
-        const int index = (int)found.matrices.size();
-        for (long long k = 0; k < size; k += each) found.chunks.push_back({index, (int)std::min(each, size - k), k});
-        t.chunks = (int)found.chunks.size() - t.first_chunk;
-        for (int a = 0; a < (t.n + kTile - 1) / kTile; ++a)
-            for (int b = 0; b < (t.n + kTile - 1) / kTile; ++b) found.squares.push_back({index, a, b});
-        for (int a = 0; a < (t.rows + kTile - 1) / kTile; ++a)
-            for (int b = 0; b < (t.cols + kTile - 1) / kTile; ++b) found.products.push_back({index, a, b});
+        t.row_blocks = blocks_in(t.rows);
+        t.col_blocks = blocks_in(t.cols);
+        t.n_blocks = std::min(t.row_blocks, t.col_blocks);
         found.matrices.push_back(t);
     }
-    found.values = at;
+    // long sums first: the last items of a phase are short ones
+    std::stable_sort(found.matrices.begin(), found.matrices.end(),
+                     [](const Matrix& a, const Matrix& b) { return std::max(a.row_blocks, a.col_blocks) > std::max(b.row_blocks, b.col_blocks); });
+    for (int index = 0; index < (int)found.matrices.size(); ++index) {
+        Matrix& t = found.matrices[index];
+        const long long size = (long long)t.rows * t.cols, blocks = (long long)t.row_blocks * t.col_blocks;
+        t.x[0] = take(blocks);
+        t.x[1] = take(blocks);
+        t.square = take((long long)t.n_blocks * t.n_blocks);
+        t.poly = take((long long)t.n_blocks * t.n_blocks);
+        t.first_chunk = (int)found.chunks.size();
+        const long long each = std::max(2048ll, (size / 512 + 2047) / 2048 * 2048);
+        for (long long k = 0; k < size; k += each) found.chunks.push_back({index, (int)std::min(each, size - k), k});
+        t.chunks = (int)found.chunks.size() - t.first_chunk;
+        for (int k = 0; k < blocks; ++k) found.blocks.push_back({index, k});
+    }
+    // Groups of matrices whose phases keep the machine busy while another's end: some three tiles to an SM
+    for (size_t from = 0; from < found.matrices.size();) {
+        size_t to = from;
+        for (long long tiles = 0; to < found.matrices.size() && tiles < 3 * b2::kSms; ++to) {
+            const Matrix& t = found.matrices[to];
+            tiles_of(t.n_blocks, t.n_blocks, true, 4, [&](int, int, int) { ++tiles; });
+        }
+        const long long first = (long long)found.items.size();
+        for (int phase = GRAM; phase <= MULTIPLY; ++phase) {
+            // the width of tiles that ends the phase first, by its longest item and by all of them
+            int best = 4;
+            double least = 1e300;
+            for (int width : {4, 2, 1}) {
+                double all = 0, longest = 0;
+                for (size_t m = from; m < to; ++m) {
+                    const Matrix& t = found.matrices[m];
+                    const int k_blocks = phase == GRAM ? std::max(t.row_blocks, t.col_blocks) : t.n_blocks;
+                    tiles_of(phase == MULTIPLY ? t.row_blocks : t.n_blocks, phase == MULTIPLY ? t.col_blocks : t.n_blocks, phase != MULTIPLY, width, [&](int, int, int w) {
+                        all += cycles_of(w, k_blocks);
+                        longest = std::max(longest, cycles_of(w, k_blocks));
+                    });
+                }
+                const double end = std::max(all / b2::kSms, longest);
+                if (end < least * 0.97) {
+                    least = end;
+                    best = width;
+                }
+            }
+            for (size_t m = from; m < to; ++m) {
+                Matrix& t = found.matrices[m];
+                const size_t before = found.items.size();
+                tiles_of(phase == MULTIPLY ? t.row_blocks : t.n_blocks, phase == MULTIPLY ? t.col_blocks : t.n_blocks, phase != MULTIPLY, best,
+                         [&](int i, int j, int w) { found.items.push_back({(int)m, (short)phase, (short)w, i, j}); });
+                t.items[phase] = (int)(found.items.size() - before);
+            }
+        }
+        found.groups.push_back({first, (long long)found.items.size() - first});
+        from = to;
+    }
+    found.bytes = at;
     return found;
 }
 
-// The scratch: sums of squares, and behind them the values
-size_t sums_bytes(long long chunks) { return ((size_t)chunks * 8 + 255) / 256 * 256; }
+size_t counter_bytes(const b2_muon_sizes& s) { return ((size_t)s.chunks * 8 + 16 + (size_t)s.matrices * 4 + 1023) / 1024 * 1024; }
 
 int sizes_of(const Layout& l, b2_muon_sizes* s) {
     s->plan_bytes = l.plan_bytes() + 64;
-    s->scratch_bytes = sums_bytes((long long)l.chunks.size()) + (size_t)l.values * 4 + 256;
     s->matrices = (int64_t)l.matrices.size();
     s->chunks = (int64_t)l.chunks.size();
-    s->items = (int64_t)(l.squares.size() + l.products.size());
+    s->items = (int64_t)l.items.size();
+    s->blocks = (int64_t)l.blocks.size();
+    s->scratch_bytes = counter_bytes(*s) + (size_t)l.bytes + 1024;
     return B2_OK;
+}
+
+// The largest values that |p| and |p(s) / s| have over [0, top]
+void reach(double a, double b, double c, double top, double* of_p, double* of_factor) {
+    *of_p = *of_factor = 0.0;
+    for (int i = 0; i <= 4096; ++i) {
+        const double s = top * i / 4096, t = s * s, f = std::fabs(a + (b + c * t) * t);
+        *of_factor = std::max(*of_factor, f);
+        *of_p = std::max(*of_p, s * f);
+    }
+}
+// The power of two that takes values up to `most` next to fp16's largest, 65504; a value that is no larger than its operand's largest
+// singular value, 1 % of rounding included, stays below 60000
+int exponent_of(double most) {
+    int e;
+    std::frexp(60000.0 / (1.01 * most + 1e-30), &e);
+    return std::max(-30, std::min(20, e - 1));
 }
 
 char* aligned(void* p, size_t to) { return (char*)(((uintptr_t)p + to - 1) / to * to); }
@@ -330,7 +808,7 @@ extern "C" int b2_muon_plan(const b2_muon_matrix* list, int32_t count, void* pla
         B2_CUDA(cudaStreamIsCapturing((cudaStream_t)stream, &capturing));
         B2_REQUIRE(capturing == cudaStreamCaptureStatusNone, "a plan is made before its stream is captured");
         std::vector<char> host(l.plan_bytes(), 0);
-        *reinterpret_cast<Header*>(host.data()) = {s.matrices, s.chunks, s.items, (long long)l.squares.size(), (long long)l.products.size()};
+        *reinterpret_cast<Header*>(host.data()) = {s.matrices, s.chunks, s.items, s.blocks, (long long)l.groups.size()};
         char* to = host.data() + kHeader;
         const auto put = [&](const void* from, size_t bytes) {
             std::copy((const char*)from, (const char*)from + bytes, to);
@@ -338,8 +816,9 @@ extern "C" int b2_muon_plan(const b2_muon_matrix* list, int32_t count, void* pla
         };
         put(l.matrices.data(), l.matrices.size() * sizeof(Matrix));
         put(l.chunks.data(), l.chunks.size() * sizeof(Chunk));
-        put(l.squares.data(), l.squares.size() * sizeof(Item));
-        put(l.products.data(), l.products.size() * sizeof(Item));
+        put(l.blocks.data(), l.blocks.size() * sizeof(Block));
+        put(l.items.data(), l.items.size() * sizeof(Item));
+        put(l.groups.data(), l.groups.size() * sizeof(Group));
         // (pageable memory: the copy has been staged when the call returns)
         B2_CUDA(cudaMemcpyAsync(aligned(plan, 64), host.data(), host.size(), cudaMemcpyHostToDevice, (cudaStream_t)stream));
         B2_CUDA(cudaStreamSynchronize((cudaStream_t)stream));
@@ -351,7 +830,7 @@ extern "C" int b2_muon_plan(const b2_muon_matrix* list, int32_t count, void* pla
 
 extern "C" int b2_muon_step(void* plan, const b2_muon_sizes* s, const b2_muon_hyper* h, const float* lr, const float* grad_scale, float* step, void* scratch,
                             size_t scratch_bytes, int32_t* status, void* stream) {
-    B2_REQUIRE(plan && s && h && s->matrices >= 0 && s->chunks >= 0 && s->items >= 0, "bad argument");
+    B2_REQUIRE(plan && s && h && s->matrices >= 0 && s->chunks >= 0 && s->items >= 0 && s->blocks >= 0, "bad argument");
     B2_REQUIRE(scratch && scratch_bytes >= s->scratch_bytes, "the step needs %zu bytes of scratch, got %zu", s->scratch_bytes, scratch_bytes);
     B2_REQUIRE(std::isfinite(h->lr) && h->momentum >= 0.0 && h->momentum < 1.0 && std::isfinite(h->eps) && h->eps >= 0.0 && std::isfinite(h->weight_decay),
                "bad rates: lr %g, momentum %g, eps %g, weight decay %g", h->lr, h->momentum, h->eps, h->weight_decay);
@@ -371,25 +850,38 @@ extern "C" int b2_muon_step(void* plan, const b2_muon_sizes* s, const b2_muon_hy
     r.mu = (float)h->momentum;
     r.rest = (float)(1.0 - h->momentum);
     r.eps = (float)h->eps;
-    r.a = (float)h->a;
-    r.b = (float)h->b;
-    r.c = (float)h->c;
     r.lr = h->lr;
     r.wd = h->weight_decay;
     r.nesterov = h->nesterov != 0;
+    Poly p = {(float)h->a, (float)h->b, (float)h->c, h->steps, {}, {}, {}};
+    double top = 1.0;
+    for (int k = 0; k < h->steps; ++k) {
+        double next, factor;
+        reach(h->a, h->b, h->c, top, &next, &factor);
+        B2_REQUIRE(next <= 1e6 && factor <= 1e6, "the polynomial of %g, %g, %g takes singular values to %g in step %d", h->a, h->b, h->c, std::max(next, factor), k + 1);
+        p.x[k] = (signed char)exponent_of(top);
+        p.square[k] = (signed char)exponent_of(top * top);
+        p.poly[k] = (signed char)exponent_of(factor);
+        top = 1.001 * next;
+    }
+    p.x[h->steps] = (signed char)exponent_of(top);
+    B2_REQUIRE(s->items <= (1ll << 30) / h->steps, "%lld items of %d steps", (long long)s->items, h->steps);
     cudaStream_t st = (cudaStream_t)stream;
     const void* base = aligned(plan, 64);
-    double* sums = (double*)aligned(scratch, 256);
-    float* values = (float*)((char*)sums + sums_bytes(s->chunks));
-    const long long most = b2::kSms * 8, blocks = s->chunks < 1 ? 1 : s->chunks < most ? s->chunks : most;
-    B2_CUDA((b2::launch_after(muon_mean_kernel, dim3((unsigned)blocks), kThreads, 0, st, base, (long long)s->matrices, (long long)s->chunks, (long long)s->items, r,
-                              grad_scale, step, sums, values)));
+    Room room;
+    char* at = aligned(scratch, 1024);
+    room.sums = (double*)at;
+    room.next = (unsigned*)(at + (size_t)s->chunks * 8);
+    room.failed = room.next + 1;
+    room.done = room.next + 4;
+    room.planes = at + counter_bytes(*s);
+    const Told told = {s->matrices, s->chunks, s->items, s->blocks};
+    const auto grid = [](long long work, long long most) { return dim3((unsigned)(work < 1 ? 1 : work < most ? work : most)); };
+    B2_CUDA((b2::launch_after(muon_mean_kernel, grid(s->chunks, b2::kSms * 8), kMeanThreads, 0, st, base, told, r, grad_scale, step, room)));
     if (s->items == 0) return B2_OK;
-    B2_CUDA((b2::launch_after(muon_scale_kernel, dim3((unsigned)blocks), kThreads, 0, st, base, (long long)s->matrices, (long long)s->chunks, (long long)s->items,
-                              r.eps, (const double*)sums, values)));
-    for (int k = 0; k < h->steps; ++k)
-        for (int phase = 0; phase < 3; ++phase)
-            B2_CUDA((b2::launch_after(muon_product_kernel, dim3((unsigned)s->items), kThreads, 0, st, base, (long long)s->matrices, (long long)s->chunks,
-                                      (long long)s->items, phase, k & 1, (int)(k == h->steps - 1), r, lr, values)));
+    B2_CUDA((b2::launch_after(muon_parts_kernel, grid(s->blocks, b2::kSms * 8), kMeanThreads, 0, st, base, told, r, grad_scale, (int)p.x[0], room)));
+    static std::atomic<unsigned long long> done{0};
+    B2_CHECK(b2::allow_shared((const void*)muon_product_kernel, kProductShared, &done));
+    B2_CUDA((b2::launch_after(muon_product_kernel, grid(s->items, b2::kSms), kProductThreads, (size_t)kProductShared, st, base, told, r, p, lr, room, status)));
     return B2_OK;
 }
