@@ -760,6 +760,7 @@ typedef struct {
     int64_t matrices, chunks, items, blocks;
 } b2_muon_sizes;
 int b2_muon_plan_sizes(const b2_muon_matrix* matrices, int32_t count, b2_muon_sizes* sizes);
+int b2_muon_launches(const b2_muon_sizes* sizes, int32_t* launches);     /* kernels that a step launches */
 int b2_muon_plan(const b2_muon_matrix* matrices, int32_t count, void* plan, size_t plan_bytes, void* stream);
 int b2_muon_step(void* plan, const b2_muon_sizes* sizes, const b2_muon_hyper* hyper, const float* lr, const float* grad_scale,
                  float* step, void* scratch, size_t scratch_bytes, int32_t* status, void* stream);

@@ -787,6 +787,12 @@ extern "C" int b2_muon_plan_sizes(const b2_muon_matrix* list, int32_t count, b2_
     }
 }
 
+extern "C" int b2_muon_launches(const b2_muon_sizes* s, int32_t* launches) {
+    B2_REQUIRE(s && launches, "missing argument");
+    *launches = s->items == 0 ? 1 : 3;
+    return B2_OK;
+}
+
 extern "C" int b2_muon_plan(const b2_muon_matrix* list, int32_t count, void* plan, size_t plan_bytes, void* stream) {
     B2_CHECK(check_matrices(list, count));
     try {

@@ -977,6 +977,22 @@ def rows_of(view, axes, apart):
     return rows[0], features[0], rows[1] if rows[0] > 1 else features[0]
 
 
+def heads_of(view, axes, apart):
+    """(distance of the rows, of the heads) of a view whose memory has `axes` in the order rows, heads, features, with apart[0] axes
+    of rows and apart[1] of heads, each of which may lie apart; None where it has not."""
+    axes = list(axes)
+    rows, heads = _merge(view, axes[:apart[0]]), _merge(view, axes[apart[0]:sum(apart)])
+    features = _merge(view, axes[sum(apart):])
+    if rows is None or heads is None or features is None or (features[0] > 1 and features[1] != 1):
+        return None
+    return rows[1], heads[1]
+
+
+def lies(view, axes, apart):
+    """Whether an operand lies as its step reads it: see rows_of, and heads_of where `apart` is a pair."""
+    return (heads_of if isinstance(apart, tuple) else rows_of)(view, axes, apart) is not None
+
+
 def _check_index(op, t, rows):
     """An index names whole numbers that its tensor can hold."""
     most = 1 << (15 if t.flex else 24)
@@ -1135,6 +1151,186 @@ class NormGradStep(_Fp32Step):
         d.status = t._status.data_ptr()
         scratch = t._scratch_aligned()
         lib.check(lib.raw().b2_norm_bprop(C.byref(a), C.byref(d), scratch[0], scratch[1], t.stream.cuda_stream))
+        t.kernel_launches += self.launches
+
+
+class _Turns(object):
+    """The frequencies of a rotation on the device, made before the first launch (outside recordings)."""
+
+    def __init__(self, rotation, rotary_dim):
+        self.rotation, self.rotary_dim, self.table = rotation, rotary_dim, None
+
+    def fill(self, a, t, place):
+        r = self.rotation
+        if self.table is None:
+            self.table = lib.rotary_turns(self.rotary_dim, scaling=r.scaling, **r.numbers).to(t.device)
+        a.rotary_dim, a.interleaved, a.turns, a.amplitude = self.rotary_dim, int(r.interleaved), self.table.data_ptr(), r.amplitude
+        a.position_count, a.position_group = place
+
+
+class RotaryStep(_Step):
+    """Heads rotated by their position."""
+    kind = "rotary"
+    launches = 1
+    probe_is_float = True
+
+    def __init__(self, index, op, t):
+        super(RotaryStep, self).__init__(index, op)
+        self.in_views = [t._view_of(a) for a in op.args]
+        self.out_views = [t._view_of(op)]
+        self.turns = _Turns(op.rotation, op.rotary_dim)
+        self.flex = t.flex
+
+    def launch(self, t):
+        op, a = self.op, lib.HeadsArgs()
+        xv, ov, p = self.in_views[0], self.out_views[0], a.part[0]
+        apart = (len(op.row_axes), len(op.head_axes))
+        a.rows, a.head_dim, a.parts, a.inverse = op.row_axes.size, op.feature_axes.size, 1, int(op.inverse)
+        self.turns.fill(a, t, op.place)
+        p.heads, p.x, p.out = op.head_axes.size, self._ptr(xv), self._ptr(ov)
+        (p.x_row, p.x_head), (p.out_row, p.out_head) = heads_of(xv, op.axes, apart), heads_of(ov, op.axes, apart)
+        if len(self.in_views) > 1:
+            a.positions, a.position_kind = self._ptr(self.in_views[1]), lib.IDX_FLEX16 if self.flex else lib.IDX_F32
+        raw, st = lib.raw(), t.stream.cuda_stream
+        if not self.flex:
+            lib.check(raw.b2_rotary(C.byref(a), 0, None, None, None, 0, st))
+            t.kernel_launches += 1
+            return
+        p.slot_x, p.slot_out = t._slot_for_read(xv.buffer, self), ov.buffer.slot_write
+        if len(self.in_views) > 1:
+            a.slot_positions = t._slot_for_read(self.in_views[1].buffer, self)
+
+        def call(probe):
+            lib.check(raw.b2_rotary(C.byref(a), 1, t._table.data_ptr(), t._stats.data_ptr(), t._probe64.data_ptr(), probe, st))
+        self._flex_probe_then(t, ov.buffer, [v.buffer for v in self.in_views], call)
+
+
+def _head_norm_args(op, turns, t, ptr):
+    """What the forward pass and the gradients of a HeadNormOp have alike, but for the tensors."""
+    a = lib.HeadsArgs()
+    a.rows, a.head_dim, a.parts, a.eps = op.row_axes.size, op.feature_axes.size, len(op.xs), op.eps
+    if op.rotation is not None:
+        turns.fill(a, t, op.place)
+    for i, h in enumerate(op.head_axes):
+        a.part[i].heads = h.size
+    return a
+
+
+class HeadNormStep(_Fp32Step):
+    """Norms of heads with the rotation in the same pass."""
+    kind = "head_norm"
+    launches = 1
+
+    def __init__(self, index, op, t, present):
+        super(HeadNormStep, self).__init__(index, op, t)
+        view = lambda x: None if x is None else t._view_of(x)  # noqa: E731
+        self.xs, self.weights, self.positions = [[view(x) for x in some] for some in (op.xs, op.weights, op.positions)]
+        self.in_views = self.xs + [w for w in self.weights if w is not None] + self.positions
+        # (the kernel stores both results, whoever reads them)
+        present = set(present) | set(r for k, r in op.results.items() if k.startswith("out"))
+        self.found = self._results(op, t, present)
+        self.turns = _Turns(op.rotation, op.rotary_dim)
+
+    def launch(self, t):
+        op = self.op
+        a = _head_norm_args(op, self.turns, t, self._ptr)
+        if self.positions:
+            a.positions, a.position_kind = self._ptr(self.positions[0]), lib.IDX_F32
+        for i, (x, w, h, ax) in enumerate(zip(self.xs, self.weights, op.head_axes, op.tensor_axes)):
+            p, out, apart = a.part[i], self.found["out%d" % i], (len(op.row_axes), len(h))
+            p.x, p.out, p.weight = self._ptr(x), self._ptr(out), None if w is None else self._ptr(w)
+            (p.x_row, p.x_head), (p.out_row, p.out_head) = heads_of(x, ax, apart), heads_of(out, ax, apart)
+            if "rstd%d" % i in self.found:
+                p.rstd = self._ptr(self.found["rstd%d" % i])
+        lib.check(lib.raw().b2_heads_fprop(C.byref(a), t.stream.cuda_stream))
+        t.kernel_launches += 1
+
+
+class HeadNormGradStep(_Fp32Step):
+    """All gradients of a HeadNormStep."""
+    kind = "head_norm_grad"
+
+    def __init__(self, index, op, t, present):
+        super(HeadNormGradStep, self).__init__(index, op, t)
+        f, view = op.fprop, lambda x: None if x is None else t._view_of(x)  # noqa: E731
+        self.deltas, self.xs, self.weights, self.positions, self.rstds = [[view(x) for x in some] for some in (op.deltas, f.xs, f.weights, f.positions, op.rstds)]
+        self.in_views = self.deltas + self.xs + [w for w in self.weights if w is not None] + self.positions + self.rstds
+        self.found = self._results(op, t, present)
+        self.turns = _Turns(f.rotation, f.rotary_dim)
+        # (sums over rows are added by a second launch)
+        self.launches = 2 if any(k.startswith("weight") for k in self.found) else 1
+        a = lib.HeadsArgs()
+        a.rows, a.head_dim, a.parts, a.eps = f.row_axes.size, f.feature_axes.size, len(f.xs), f.eps
+        for i, h in enumerate(f.head_axes):
+            a.part[i].heads = h.size
+        self.scratch_bytes = lib.heads_bprop_scratch_bytes(a)
+
+    def launch(self, t):
+        f, d = self.op.fprop, lib.HeadsGrads()
+        a = _head_norm_args(f, self.turns, t, self._ptr)
+        if self.positions:
+            a.positions, a.position_kind = self._ptr(self.positions[0]), lib.IDX_F32
+        for i, (x, w, h, ax) in enumerate(zip(self.xs, self.weights, f.head_axes, f.tensor_axes)):
+            p, g, apart = a.part[i], d.part[i], (len(f.row_axes), len(h))
+            p.x, p.weight, p.rstd = self._ptr(x), None if w is None else self._ptr(w), self._ptr(self.rstds[i])
+            p.x_row, p.x_head = heads_of(x, ax, apart)
+            g.d_out = self._ptr(self.deltas[i])
+            g.d_out_row, g.d_out_head = heads_of(self.deltas[i], ax, apart)
+            if "x%d" % i in self.found:
+                g.d_x = self._ptr(self.found["x%d" % i])
+                g.d_x_row, g.d_x_head = heads_of(self.found["x%d" % i], ax, apart)
+            if "weight%d" % i in self.found:
+                g.d_weight = self._ptr(self.found["weight%d" % i])
+        scratch = t._scratch_aligned()
+        lib.check(lib.raw().b2_heads_bprop(C.byref(a), C.byref(d), scratch[0], scratch[1], t.stream.cuda_stream))
+        t.kernel_launches += self.launches
+
+
+class MuonStep(_Fp32Step):
+    """One step of orthogonalised updates over many matrices."""
+    kind = "muon"
+
+    def __init__(self, index, op, t, written):
+        super(MuonStep, self).__init__(index, op, t)
+        self.out_views = written
+        self.gradients = [t._view_of(g) for g in op.gradients]
+        self.numbers = [None if x is None or isinstance(x, float) else t._view_of(x) for x in (op.lr, op.grad_scale)]
+        self.scale = None              # a tensor of a grad_scale that is a number
+        self.in_views = self.gradients + self.out_views + [v for v in self.numbers if v is not None]
+        self.plan = None
+        # (what the sizes are checked for: addresses are not known yet)
+        self.sizes = lib.muon_plan_sizes(self._matrices(lambda v: 256))
+        self.scratch_bytes = self.sizes.scratch_bytes + 1024
+        self.launches = lib.muon_launches(self.sizes)
+
+    def _matrices(self, at):
+        """The list of matrices, a stack one behind another; `at` gives a tensor's address."""
+        op, states = self.op, self.out_views[len(self.op.variables):]
+        found = (lib.MuonMatrix * sum(n for n, _, _ in op.shapes))()
+        k = 0
+        for i, (n, r, c) in enumerate(op.shapes):
+            bases = [at(v) for v in (self.out_views[i], self.gradients[i], states[i])]
+            for j in range(n):
+                x = found[k]
+                x.param, x.grad, x.mean = [b + 4 * j * r * c for b in bases]
+                x.rows, x.cols, x.decay, x.scale = r, c, float(op.decayed[i]), op.scales[i]
+                k += 1
+        return found
+
+    def launch(self, t):
+        op = self.op
+        if self.plan is None:          # (outside recordings: before the first call's launch)
+            self.plan = t.torch.empty((self.sizes.plan_bytes,), dtype=t.torch.uint8, device=t.device)
+            if isinstance(op.grad_scale, float) and op.grad_scale != 1.0:
+                self.scale = t.torch.full((1,), op.grad_scale, device=t.device)
+            lib.muon_plan(self._matrices(self._ptr), self.plan.data_ptr(), self.sizes.plan_bytes, t.stream.cuda_stream)
+        lr, scale = [None if v is None else self._ptr(v) for v in self.numbers]
+        if self.scale is not None:
+            scale = self.scale.data_ptr()
+        h = lib.MuonHyper(lr=op.lr if lr is None else 0.0, **op.rates)
+        scratch = t._scratch_aligned()
+        lib.check(lib.raw().b2_muon_step(self.plan.data_ptr(), C.byref(self.sizes), C.byref(h), lr, scale, self._ptr(t._view_of(op.count)), scratch[0],
+                                         scratch[1], t._status.data_ptr(), t.stream.cuda_stream))
         t.kernel_launches += self.launches
 
 

@@ -299,6 +299,7 @@ def _load():
         "b2_adamw_plan": (C.c_int, [C.POINTER(AdamwTensor), i32, i32, vp, sz, vp]),
         "b2_adamw_step": (C.c_int, [vp, i64, i32, C.POINTER(AdamwHyper), vp, vp, vp, C.c_uint32, vp]),
         "b2_muon_plan_sizes": (C.c_int, [C.POINTER(MuonMatrix), i32, C.POINTER(MuonSizes)]),
+        "b2_muon_launches": (C.c_int, [C.POINTER(MuonSizes), C.POINTER(i32)]),
         "b2_muon_plan": (C.c_int, [C.POINTER(MuonMatrix), i32, vp, sz, vp]),
         "b2_muon_step": (C.c_int, [vp, C.POINTER(MuonSizes), C.POINTER(MuonHyper), vp, vp, vp, vp, sz, vp, vp]),
         "b2_selftest_bounded_wait": (C.c_int, [i32, vp, vp, vp]),
@@ -662,6 +663,13 @@ def muon_plan_sizes(matrices):
     out = MuonSizes()
     check(_lib.b2_muon_plan_sizes(matrices, len(matrices), C.byref(out)))
     return out
+
+
+def muon_launches(sizes):
+    """Kernels that a step launches."""
+    out = C.c_int32()
+    check(_lib.b2_muon_launches(C.byref(sizes), C.byref(out)))
+    return out.value
 
 
 def muon_plan(matrices, plan_ptr, plan_bytes, stream=0):

@@ -7,6 +7,7 @@ reductions, dot, convolution, pooling, assign and sequential.  Names, argument m
 behaviour follow the reference so that tests read like the reference's own; autodiff, serde and
 the frontends are not part of this package.
 """
+import builtins
 import itertools
 import numbers
 
@@ -927,6 +928,181 @@ def residual_norm_grad(fprop, d_out=None, d_stream=None):
     return dict(ResidualNormGradOp(fprop, d_out, d_stream).results)
 
 
+class Rotation(object):
+    """How heads are rotated by position.  positions: an op over axes of the heads' rows that lie next to one another, or one of
+    these axes, whose indices are the positions then.  Pairs of the first rotary_dim features (None: all) -- pairs "halves" or
+    "neighbours" -- turn by position * frequency, and are multiplied by amplitude.  Frequencies are base^(-2 i / rotary_dim), for
+    contexts `factor` times as long as the `original` one: scaling "linear" divides all, "base" takes a larger base, "parts" divides
+    those that turn less than `low` times over the original context and keeps those that turn more than `high` times."""
+
+    def __init__(self, positions, rotary_dim=None, pairs="halves", base=10000.0, scaling="none", factor=1.0, original=1.0, low=1.0, high=32.0,
+                 amplitude=1.0):
+        self.positions = positions if isinstance(positions, Axis) else as_op(positions)
+        self.rotary_dim = None if rotary_dim is None else int(rotary_dim)
+        if pairs not in ("halves", "neighbours"):
+            raise ValueError("pairs are halves or neighbours, not %r" % (pairs,))
+        if scaling not in ("none", "linear", "base", "parts"):
+            raise ValueError("unknown scaling: %r" % (scaling,))
+        self.interleaved, self.scaling, self.amplitude = pairs == "neighbours", scaling, float(amplitude)
+        self.numbers = dict(base=float(base), factor=float(factor), original=float(original), low=float(low), high=float(high))
+        if not (self.numbers["base"] > 0 and self.numbers["factor"] > 0 and self.numbers["original"] > 0 and self.numbers["low"] < self.numbers["high"]
+                and np.isfinite(list(self.numbers.values()) + [self.amplitude]).all()):
+            raise ValueError("bad frequencies: %s, amplitude %s" % (self.numbers, amplitude))
+
+    def over(self, features):
+        """How many of so many features are rotated."""
+        d = features // 2 * 2 if self.rotary_dim is None else self.rotary_dim
+        if d < 2 or d > features or d % 2:
+            raise ValueError("%d of %d features cannot be rotated" % (d, features))
+        return d
+
+    def place(self, rows):
+        """(how many positions, how many rows behind one another have each) for rows with these axes."""
+        axes = make_axes([self.positions]) if isinstance(self.positions, Axis) else self.positions.axes
+        if not len(axes):
+            return 1, builtins.max(rows.size, 1)
+        if not axes.is_sub_set(rows):
+            raise ValueError("positions have the axes %s, the heads' rows %s" % (axes, rows))
+        first = builtins.min(rows.index(a) for a in axes)
+        if not rows[first:first + len(axes)].is_equal_set(axes):
+            raise ValueError("the axes of the positions, %s, lie apart in those of the rows, %s" % (axes, rows))
+        return axes.size, builtins.max(rows[first + len(axes):].size, 1)
+
+
+def _heads_axes(x, heads, features):
+    """(axes of the rows, axes of the heads, the features) of a tensor of heads."""
+    features = make_axes([features]) if isinstance(features, Axis) else make_axes(features)
+    heads = make_axes([]) if heads is None else make_axes([heads]) if isinstance(heads, Axis) else make_axes(heads)
+    if len(features) != 1 or not features.is_sub_set(x.axes) or features[0].length > 1024:
+        raise ValueError("the features %s are not one axis of %s, of at most 1024" % (features, x.axes))
+    if not heads.is_sub_set(x.axes) or features[0] in heads:
+        raise ValueError("the heads %s are not axes of %s" % (heads, x.axes))
+    return x.axes - heads - features, heads, features
+
+
+class RotaryOp(Op):
+    """Heads rotated by their position: args (x[, positions]), result on the axes rows, heads, features."""
+
+    def __init__(self, x, rotation, heads, features, inverse=False, **kw):
+        x = as_op(x)
+        if not isinstance(rotation, Rotation):
+            raise ValueError("a rotation is a Rotation, not %r" % (rotation,))
+        self.row_axes, self.head_axes, self.feature_axes = _heads_axes(x, heads, features)
+        self.rotary_dim = rotation.over(self.feature_axes.size)
+        self.place = rotation.place(self.row_axes)
+        self.rotation, self.inverse = rotation, bool(inverse)
+        positions = [] if isinstance(rotation.positions, Axis) else [rotation.positions]
+        super(RotaryOp, self).__init__([x] + positions, self.row_axes + self.head_axes + self.feature_axes, **kw)
+
+    def layouts(self):
+        return [(self.args[0], self.axes, (len(self.row_axes), len(self.head_axes)))] + _positions_layout(self.row_axes, self.args[1:])
+
+
+def _positions_layout(rows, positions):
+    """Positions lie as their axes do among the rows."""
+    return [(p, [a for a in rows if a in p.axes], 0) for p in positions]
+
+
+def rotary(x, rotation, heads, features):
+    """`x` with the feature pairs of every head rotated by the row's position (see Rotation).  heads: the axes of the heads
+    (None: one head); the axes that are neither heads nor features are the rows."""
+    return RotaryOp(x, rotation, heads, features)
+
+
+def rotary_grad(delta, fprop):
+    """Gradient of the operand of the rotary op `fprop` from that of its result: rotated back."""
+    if not isinstance(fprop, RotaryOp):
+        raise ValueError("rotary_grad needs the forward RotaryOp, got {}".format(fprop))
+    delta = as_op(delta)
+    _check_operand("delta", delta, fprop.axes)
+    return RotaryOp(axes_with_order(delta, fprop.axes), fprop.rotation, fprop.head_axes, fprop.feature_axes, inverse=not fprop.inverse)
+
+
+class HeadNormOp(Op):
+    """Norms of the heads of one or two tensors of the same rows, with a rotation in the same pass."""
+
+    def __init__(self, xs, weights, heads, features, rotation=None, eps=1e-6, **kw):
+        xs = list(as_ops(xs))
+        if len(xs) not in (1, 2) or len(weights) != len(xs) or len(heads) != len(xs):
+            raise ValueError("one or two tensors of heads, with a weight (or None) and the axes of the heads each")
+        if rotation is not None and not isinstance(rotation, Rotation):
+            raise ValueError("a rotation is a Rotation, not %r" % (rotation,))
+        self.xs, self.rotation, self.eps = xs, rotation, float(eps)
+        if not (self.eps >= 0 and np.isfinite(self.eps)):
+            raise ValueError("eps is not negative: %r" % (eps,))
+        found = [_heads_axes(x, h, features) for x, h in zip(xs, heads)]
+        self.row_axes, _, self.feature_axes = found[0]
+        self.head_axes = [f[1] for f in found]
+        for x, (rows, _, _) in zip(xs, found):
+            if not rows.is_equal_set(self.row_axes):
+                raise ValueError("the rows of two tensors of heads differ: %s, %s" % (self.row_axes, rows))
+        self.weights = [None if w is None else as_op(w) for w in weights]
+        for w in self.weights:
+            if w is not None:
+                _check_operand("weight", w, self.feature_axes)
+        self.rotary_dim = 0 if rotation is None else rotation.over(self.feature_axes.size)
+        self.place = (1, 1) if rotation is None else rotation.place(self.row_axes)
+        self.positions = [] if rotation is None or isinstance(rotation.positions, Axis) else [rotation.positions]
+        self.tensor_axes = [self.row_axes + h + self.feature_axes for h in self.head_axes]
+        operands = xs + [w for w in self.weights if w is not None] + self.positions
+        super(HeadNormOp, self).__init__(operands, self.tensor_axes[0], **kw)
+        self.results = {}
+        for i, h in enumerate(self.head_axes):
+            self.results["out%d" % i] = ResultOp(self, "out%d" % i, self.tensor_axes[i])
+            self.results["rstd%d" % i] = ResultOp(self, "rstd%d" % i, self.row_axes + h)
+
+    def heads_layouts(self, tensors):
+        return [(x, ax, (len(self.row_axes), len(h))) for x, ax, h in zip(tensors, self.tensor_axes, self.head_axes) if x is not None]
+
+    def layouts(self):
+        return self.heads_layouts(self.xs) + [(w, self.feature_axes, 0) for w in self.weights if w is not None] + \
+            _positions_layout(self.row_axes, self.positions)
+
+
+def head_norm(xs, weights, heads, features, rotation=None, eps=1e-6):
+    """x / sqrt(mean(x^2) + eps) * weight over the features of every head of the tensors `xs` -- as a rule the queries and the
+    keys of the same rows -- each then rotated by the row's position (rotation None: not).  weights: one for every tensor, shared
+    by its heads, or None; heads: the axes of the heads of every tensor.  A list of results on the axes rows, heads, features."""
+    op = HeadNormOp(xs, weights, heads, features, rotation, eps)
+    return [op.results["out%d" % i] for i in range(len(op.xs))]
+
+
+class HeadNormGradOp(Op):
+    """All gradients of a HeadNormOp in one step."""
+
+    def __init__(self, deltas, fprop, **kw):
+        if isinstance(fprop, (list, tuple)) and fprop:
+            fprop = fprop[0]
+        if isinstance(fprop, ResultOp):
+            fprop = fprop.args[0]
+        if not isinstance(fprop, HeadNormOp):
+            raise ValueError("head_norm_grad needs a result of the forward op, got {}".format(fprop))
+        deltas = list(as_ops(deltas))
+        if len(deltas) != len(fprop.xs):
+            raise ValueError("%d gradients of %d results" % (len(deltas), len(fprop.xs)))
+        for d, ax in zip(deltas, fprop.tensor_axes):
+            _check_operand("delta", d, ax)
+        self.fprop, self.deltas = fprop, deltas
+        self.rstds = [fprop.results["rstd%d" % i] for i in range(len(deltas))]
+        reads = deltas + list(fprop.args) + self.rstds
+        super(HeadNormGradOp, self).__init__(reads, fprop.tensor_axes[0], **kw)
+        self.results = {}
+        for i, ax in enumerate(fprop.tensor_axes):
+            self.results["x%d" % i] = ResultOp(self, "x%d" % i, ax)
+            if fprop.weights[i] is not None:
+                self.results["weight%d" % i] = ResultOp(self, "weight%d" % i, fprop.feature_axes)
+
+    def layouts(self):
+        return self.fprop.heads_layouts(self.deltas) + self.fprop.layouts() + [(r, r.axes, 0) for r in self.rstds]
+
+
+def head_norm_grad(deltas, fprop):
+    """Gradients of head_norm (`fprop` is its list of results, or one of them) from those of its results: a dict of x and weight,
+    a list each with one for every tensor; None where there is no weight."""
+    op = HeadNormGradOp(deltas, fprop)
+    return {k: [op.results.get("%s%d" % (k, i)) for i in range(len(op.deltas))] for k in ("x", "weight")}
+
+
 class AdamWOp(Op):
     """One AdamW step over all of `variables` (see adamw).  Its value is the number of steps made."""
     is_tensor_op = False
@@ -988,6 +1164,69 @@ def adamw(variables, gradients, lr, beta1=0.9, beta2=0.999, eps=1e-8, weight_dec
     e4m3 bytes with a scale for every 256, rounded at random (from `seed`, the position and the step).  The
     moments (op.states) and the number of steps (op.count) are persistent tensors, zero before the first."""
     return AdamWOp(variables, gradients, lr, beta1, beta2, eps, weight_decay, no_decay, state_bits, grad_scale, seed)
+
+
+class MuonOp(Op):
+    """One step of orthogonalised updates over all of `variables` (see muon).  Its value is the number of steps made."""
+    is_tensor_op = False
+
+    def __init__(self, variables, gradients, lr, momentum=0.95, nesterov=True, weight_decay=0.0, no_decay=(), scale="sides", iterations=5,
+                 coefficients=(3.4445, -4.7750, 2.0315), eps=1e-7, grad_scale=None, **kw):
+        variables, gradients = as_ops(variables), as_ops(gradients)
+        if len(variables) != len(gradients):
+            raise ValueError("%d variables and %d gradients" % (len(variables), len(gradients)))
+        if len(set(variables)) != len(variables):
+            raise ValueError("a variable occurs twice")
+        for v, g in zip(variables, gradients):
+            if not isinstance(v, AssignableTensorOp) or v.is_constant:
+                raise ValueError("{} is not assignable.".format(v))
+            if len(v.axes) not in (2, 3):
+                raise ValueError("{} is no matrix, nor a stack of matrices: {}".format(v, v.axes))
+            _check_operand("the gradient of %s" % v, g, v.axes)
+        for x in no_decay:
+            if x not in variables:
+                raise ValueError("{} is not among the variables".format(x))
+        self.variables, self.gradients = variables, gradients
+        a, b, c = [float(x) for x in coefficients]
+        self.rates = dict(momentum=float(momentum), eps=float(eps), weight_decay=float(weight_decay), a=a, b=b, c=c, steps=int(iterations), nesterov=int(bool(nesterov)))
+        if not (0 <= self.rates["momentum"] < 1 and self.rates["eps"] >= 0 and 1 <= self.rates["steps"] <= 32 and np.isfinite(list(self.rates.values())).all()):
+            raise ValueError("bad rates: %s" % self.rates)
+        self.decayed = [v not in no_decay for v in variables]
+        # (stacks: how many matrices, rows and columns of one)
+        self.shapes = [((1,) + tuple(v.axes.lengths))[-3:] for v in variables]
+        sides = {"sides": lambda r, c: builtins.max(1.0, r / c) ** 0.5, "rms": lambda r, c: 0.2 * builtins.max(r, c) ** 0.5}
+        if not isinstance(scale, numbers.Number) and scale not in sides:
+            raise ValueError("the scale of an update is a number, sides or rms, not %r" % (scale,))
+        self.scales = [float(scale) if isinstance(scale, numbers.Number) else sides[scale](builtins.max(r, 1), builtins.max(c, 1)) for _, r, c in self.shapes]
+        # (numbers stay as they are: an op of one would be rounded to fp32)
+        self.lr = float(lr) if isinstance(lr, numbers.Number) else as_op(lr)
+        self.grad_scale = float(grad_scale) if isinstance(grad_scale, numbers.Number) else None if grad_scale is None else as_op(grad_scale)
+        for what, x in (("lr", self.lr), ("grad_scale", self.grad_scale)):
+            if isinstance(x, Op) and x.axes.size != 1:
+                raise ValueError("%s is a number, not a tensor with axes %s" % (what, x.axes))
+        self.count = persistent_tensor([make_axis(1, name="steps")], initial_value=0.0)
+        self.states = [persistent_tensor(v.axes, initial_value=0.0, name="%s_mean" % v.name) for v in variables]
+        args = list(variables) + list(gradients) + self.states + [self.count]
+        super(MuonOp, self).__init__(args + [x for x in (self.lr, self.grad_scale) if isinstance(x, Op)], self.count.axes, **kw)
+
+    def layouts(self):
+        return [(g, v.axes, 0) for v, g in zip(self.variables, self.gradients)] + \
+            [(x, x.axes, 0) for x in (self.lr, self.grad_scale) if isinstance(x, Op)]
+
+    def written(self):
+        return list(self.variables) + self.states + [self.count]
+
+
+def muon(variables, gradients, lr, momentum=0.95, nesterov=True, weight_decay=0.0, no_decay=(), scale="sides", iterations=5,
+         coefficients=(3.4445, -4.7750, 2.0315), eps=1e-7, grad_scale=None):
+    """One step over many matrices at once whose updates are orthogonalised: the running mean of the gradients, with momentum and,
+    where nesterov, the newest gradient once more, is divided by its norm and taken `iterations` times through the odd polynomial with
+    these coefficients, which leads its singular values towards one, and moves the variable by lr * scale.  Variables have two
+    axes, rows and columns, or three: a stack of matrices along the first.  scale: "sides" sqrt(max(1, rows / columns)), "rms"
+    0.2 sqrt(max(rows, columns)), or a number.  lr, and grad_scale, which multiplies every gradient, are numbers or ops whose value
+    is one.  The means (op.states) and the number of steps (op.count) are persistent tensors, zero before the first.  Tables, vectors
+    and output layers are better left to adamw."""
+    return MuonOp(variables, gradients, lr, momentum, nesterov, weight_decay, no_decay, scale, iterations, coefficients, eps, grad_scale)
 
 
 # ---- communication ----------------------------------------------------------------------------

@@ -28,9 +28,9 @@ from . import comm as commmod
 from . import tracing
 from .op_graph import (AdamWOp, AllReduceOp, AssignableTensorOp, AssignOp, Axes, AxesCastOp, BroadcastOp,
                        ConvolutionOp, DotOp, bprop_conv, update_conv,
-                       BpropPoolOp, ElementWiseOp, EmbeddingGradOp, EmbeddingOp, LookupTableOp, Op,
+                       BpropPoolOp, ElementWiseOp, EmbeddingGradOp, EmbeddingOp, HeadNormGradOp, HeadNormOp, LookupTableOp, MuonOp, Op,
                        PoolingOp, ReductionOp, ResidualNormGradOp, ResidualNormOp, ResultOp, RngOp,
-                       ReorderAxes, ReshapeOp, SequentialOp, TensorSliceOp, update_lut,
+                       ReorderAxes, ReshapeOp, RotaryOp, SequentialOp, TensorSliceOp, update_lut,
                        ViewOp, as_op, make_axes)
 
 
@@ -1261,10 +1261,10 @@ class _Planner(object):
                         self._densify(a, list(self.t._view_of(a).axes), saved)
             elif hasattr(op, "layouts"):
                 # (what a step over many tensors reads of one that it writes is taken before it: blocks write at any time)
-                written = set(self.t._buffer_of(x) for x in op.written()) if isinstance(op, AdamWOp) else ()
+                written = set(self.t._buffer_of(x) for x in op.written()) if isinstance(op, (AdamWOp, MuonOp)) else ()
                 for a, axes, apart in op.layouts():
                     view = self.t._view_of(a)
-                    if view.buffer in written or kernels.rows_of(view, axes, apart) is None:
+                    if view.buffer in written or not kernels.lies(view, axes, apart):
                         self._densify(a, list(axes), saved)
             step = self._make_other_step(op, tail)
         finally:
@@ -1329,6 +1329,14 @@ class _Planner(object):
             step = kernels.NormStep(index, op, self.t, self.present)
         elif isinstance(op, ResidualNormGradOp):
             step = kernels.NormGradStep(index, op, self.t, self.present)
+        elif isinstance(op, RotaryOp):
+            step = kernels.RotaryStep(index, op, self.t)
+        elif isinstance(op, HeadNormOp):
+            step = kernels.HeadNormStep(index, op, self.t, self.present)
+        elif isinstance(op, HeadNormGradOp):
+            step = kernels.HeadNormGradStep(index, op, self.t, self.present)
+        elif isinstance(op, MuonOp):
+            step = kernels.MuonStep(index, op, self.t, [View.dense(self.t._buffer_of(x)) for x in op.written()])
         elif isinstance(op, AdamWOp):
             # (views of the tensors themselves: a copy may stand for a variable that is a gradient too)
             step = kernels.AdamwStep(index, op, self.t, [View.dense(self.t._buffer_of(x)) for x in op.written()])
@@ -1367,7 +1375,7 @@ class _Planner(object):
         self.producer[op] = index
         for r in getattr(op, "results", {}).values():
             self.producer[r] = index
-        if isinstance(op, AdamWOp):
+        if isinstance(op, (AdamWOp, MuonOp)):
             for x in op.written():         # in place: later readers come behind this step
                 self.t._buffer_of(x).last_write_step = index
                 self.last_assign[x] = None
@@ -2008,7 +2016,7 @@ class B200Transformer(object):
             v = View(src.buffer, op.axes, strides, offset)
         elif isinstance(op, AssignOp):
             v = self._view_of(op.args[0])
-        elif isinstance(op, AdamWOp):
+        elif isinstance(op, (AdamWOp, MuonOp)):
             v = self._view_of(op.count)
         else:
             v = View.dense(self._buffer_of(op))
