@@ -189,6 +189,242 @@ heads_any_kernel(const b2_heads a, const b2_heads_grads g, const FlexArgs flex, 
     }
 }
 
+// How a launch deals out heads: `lanes` (as a power of two) to a head, so that a warp takes 32 >> lanes heads at a time, `turns` times;
+// that is a task, of the queries or of the keys of one row.
+struct Deal {
+    int lanes, turns, first_tasks, row_tasks;       // tasks of a row: of the first tensor, of both
+    long long tasks;
+};
+constexpr int kThreads = 256;
+
+template <int VEC, typename T>
+__device__ __forceinline__ void get(const T* p, float* v) {
+    if constexpr (VEC == 1) {
+        v[0] = (float)*p;
+    } else if constexpr (sizeof(T) == 4) {
+        const float4 w = *reinterpret_cast<const float4*>(p);
+        v[0] = w.x; v[1] = w.y; v[2] = w.z; v[3] = w.w;
+    } else {
+        const int2 w = *reinterpret_cast<const int2*>(p);
+        v[0] = (float)(short)(w.x & 0xffff);
+        v[1] = (float)(w.x >> 16);
+        v[2] = (float)(short)(w.y & 0xffff);
+        v[3] = (float)(w.y >> 16);
+    }
+}
+template <int VEC, typename T>
+__device__ __forceinline__ void put(T* p, const float* v, float& stat) {
+    if constexpr (VEC == 1) {
+        *p = held<T>(v[0], stat);
+    } else if constexpr (sizeof(T) == 4) {
+        *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+    } else {
+        short q[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) q[k] = held<T>(v[k], stat);
+        *reinterpret_cast<short4*>(p) = make_short4(q[0], q[1], q[2], q[3]);
+    }
+}
+
+// Heads of up to 256 features: a lane holds the same features of every head that it comes to, EACH times two runs of VEC features
+// that hold both features of their pairs, so that it works out its angles once a task, while the loads are on their way, and neither
+// shares them nor waits for anybody.  All loads of a task are issued before the first is needed.
+//   HALVES: a run lies as far from the other as the features of a pair; the features behind the rotated ones likewise
+//   else:   VEC 4: two runs half a head apart, each of two pairs; VEC 1: a pair
+// BACKWARD: sums for the weights stay in registers and are added over the CTA at the end.
+template <int MODE, typename T, int VEC, int EACH, bool HALVES>
+__global__ void __launch_bounds__(kThreads, MODE == BACKWARD ? 2 : 3)
+heads_kernel(const b2_heads a, const b2_heads_grads g, const FlexArgs flex, const Deal deal, float* __restrict__ sums) {
+    constexpr int N = 2 * VEC * EACH, P = N / 2, U = MODE == BACKWARD ? (N > 4 ? 2 : 4) : 4;
+    static_assert(VEC == 1 || EACH == 1, "one pair of vectors");
+    constexpr bool APART = VEC == 4 && HALVES;                  // the features of pair k: k and VEC + k, else 2 k and 2 k + 1
+    after_earlier_kernels();
+    const int lane = threadIdx.x & 31, sub = lane & ((1 << deal.lanes) - 1), beside = 32 >> deal.lanes, mine = lane >> deal.lanes;
+    const int D = a.head_dim, r = a.rotary_dim;
+    // where this lane's runs of features begin (-1: none), and its pairs' frequencies
+    int at[2 * EACH];
+    unsigned long long frequency[P];
+    unsigned turning = 0;
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) {
+        const int i = VEC * (sub + 32 * e);                     // of the first run
+        int first, second;
+        if (HALVES) {
+            const int rest = (D - r + 1) / 2, j = i - r / 2;
+            first = i < r / 2 ? i : j < rest ? r + j : -1;
+            second = i < r / 2 ? i + r / 2 : j < rest && r + rest + j < D ? r + rest + j : -1;
+        } else if (VEC == 4) {
+            first = i < D / 2 ? i : -1;
+            second = i < D / 2 ? D / 2 + i : -1;
+        } else {
+            first = 2 * i < D ? 2 * i : -1;
+            second = 2 * i + 1 < D ? 2 * i + 1 : -1;
+        }
+        at[2 * e] = first;
+        at[2 * e + 1] = second;
+#pragma unroll
+        for (int k = 0; k < P / EACH; ++k) {
+            const int feature = HALVES ? first + k : VEC == 4 ? (k < 2 ? first + 2 * k : second + 2 * k - 4) : first;
+            const bool turns = first >= 0 && feature < (HALVES ? r / 2 : r);
+            frequency[e * (P / EACH) + k] = turns ? a.turns[HALVES ? feature : feature / 2] : 0;
+            turning |= (unsigned)turns << (e * (P / EACH) + k);
+        }
+    }
+    float acc[2][MODE == BACKWARD ? N : 1];
+#pragma unroll
+    for (int j = 0; j < (MODE == BACKWARD ? N : 1); ++j) acc[0][j] = acc[1][j] = 0.0f;
+    float factor = 1.0f, stat = 0.0f;
+    if constexpr (sizeof(T) == 2) factor = flex.table[a.part[0].slot_x].scale * (flex.probe ? 1.0f : flex.table[a.part[0].slot_out].inv_scale);
+
+    const auto load = [&](const T* from, float* v) {
+#pragma unroll
+        for (int e = 0; e < 2 * EACH; ++e)
+            if (at[e] >= 0) get<VEC>(from + at[e], v + VEC * e);
+            else
+#pragma unroll
+                for (int k = 0; k < VEC; ++k) v[VEC * e + k] = 0.0f;
+    };
+    const long long step = (long long)gridDim.x * (kThreads / 32);
+    for (long long task = (long long)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5); task < deal.tasks; task += step) {
+        const long long row = deal.tasks <= 0xffffffffll ? (long long)((unsigned)task / (unsigned)deal.row_tasks) : task / deal.row_tasks;
+        const int in_row = (int)(task - row * deal.row_tasks), n = in_row >= deal.first_tasks;
+        const b2_heads_part& p = a.part[n];
+        const b2_heads_part_grads& d = g.part[n];
+        const int head = (in_row - (n ? deal.first_tasks : 0)) * deal.turns * beside + mine;
+        float x[U][N], y[MODE == BACKWARD ? U : 1][N], rstd[U];
+        long long position = 0;
+        const bool good = r == 0 || position_of(a, row, flex.table, position);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int h = head + u * beside;
+            const bool live = u < deal.turns && h < p.heads;
+            rstd[u] = 1.0f;
+            if (live) {
+                load(static_cast<const T*>(p.x) + row * p.x_row + h * p.x_head, x[u]);
+                if constexpr (MODE == BACKWARD) {
+                    load(reinterpret_cast<const T*>(d.d_out) + row * d.d_out_row + h * d.d_out_head, y[u]);
+                    rstd[u] = p.rstd[row * p.heads + h];
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < N; ++j) {
+                    x[u][j] = 0.0f;
+                    if constexpr (MODE == BACKWARD) y[u][j] = 0.0f;
+                }
+            }
+        }
+        float w[N];
+        if constexpr (MODE != ROTATE) {
+#pragma unroll
+            for (int e = 0; e < 2 * EACH; ++e)
+                if (p.weight && at[e] >= 0) get<VEC>(p.weight + at[e], w + VEC * e);
+                else
+#pragma unroll
+                    for (int k = 0; k < VEC; ++k) w[VEC * e + k] = 1.0f;
+        }
+        float2 turn[P];
+#pragma unroll
+        for (int k = 0; k < P; ++k) {
+            turn[k] = make_float2(1.0f, 0.0f);
+            if (turning >> k & 1) turn[k] = good ? turn_of((unsigned long long)position * frequency[k], a.amplitude) : make_float2(NAN, NAN);
+            if (MODE == BACKWARD || (MODE == ROTATE && a.inverse)) turn[k].y = -turn[k].y;
+        }
+        const auto rotate = [&](float* v) {
+#pragma unroll
+            for (int k = 0; k < P; ++k) {
+                const int i = APART ? k : 2 * k, j = APART ? VEC + k : 2 * k + 1;
+                if (turning >> k & 1) {
+                    const float s = v[i], t = v[j];
+                    v[i] = fmaf(s, turn[k].x, -t * turn[k].y);
+                    v[j] = fmaf(t, turn[k].x, s * turn[k].y);
+                }
+            }
+        };
+        const auto over_head = [&](float q) {
+            for (int o = 1 << deal.lanes >> 1; o > 0; o >>= 1) q += __shfl_xor_sync(0xffffffffu, q, o);
+            return q;
+        };
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (u >= deal.turns) break;
+            const int h = head + u * beside;
+            const bool live = h < p.heads;
+            float* v = x[u];
+            T* out = nullptr;
+            if constexpr (MODE == FORWARD) {
+                float q = 0.0f;
+#pragma unroll
+                for (int j = 0; j < N; ++j) q = fmaf(v[j], v[j], q);
+                const float root = __frsqrt_rn(__fdividef(over_head(q), (float)D) + a.eps);
+                if (p.rstd && live && sub == 0) p.rstd[row * p.heads + h] = root;
+#pragma unroll
+                for (int j = 0; j < N; ++j) v[j] *= root * w[j];
+            }
+            if constexpr (MODE == BACKWARD) {
+                rotate(y[u]);
+                float q = 0.0f;
+#pragma unroll
+                for (int j = 0; j < N; ++j) {
+                    v[j] *= rstd[u];                            // x^
+                    const float dw = y[u][j] * v[j];
+                    q = fmaf(w[j], dw, q);
+                    if (n) acc[1][j] += dw;
+                    else acc[0][j] += dw;
+                }
+                const float mean = __fdividef(over_head(q), (float)D);
+#pragma unroll
+                for (int j = 0; j < N; ++j) v[j] = rstd[u] * (w[j] * y[u][j] - v[j] * mean);
+                if (d.d_x && live) out = reinterpret_cast<T*>(d.d_x) + row * d.d_x_row + h * d.d_x_head;
+            } else {
+                rotate(v);
+                if (live) out = static_cast<T*>(p.out) + row * p.out_row + h * p.out_head;
+            }
+            if (!out) continue;
+            if constexpr (sizeof(T) == 2) {
+#pragma unroll
+                for (int j = 0; j < N; ++j) v[j] *= factor;
+                if (flex.probe) {
+#pragma unroll
+                    for (int j = 0; j < N; ++j) stat = fmaxf(stat, fabsf(v[j]));
+                    continue;
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 2 * EACH; ++e)
+                if (at[e] >= 0) put<VEC>(out + at[e], v + VEC * e, stat);
+        }
+    }
+    if constexpr (MODE == BACKWARD) {
+        extern __shared__ float2 table[];
+        float* words = reinterpret_cast<float*>(table) + (threadIdx.x >> 5) * 2 * D;
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int e = 0; e < 2 * EACH; ++e)
+#pragma unroll
+                for (int k = 0; k < VEC; ++k) {
+                    float q = acc[n][VEC * e + k];
+                    for (int o = 1 << deal.lanes; o < 32; o <<= 1) q += __shfl_xor_sync(0xffffffffu, q, o);
+                    if (mine == 0 && at[e] >= 0) words[n * D + at[e] + k] = q;
+                }
+        __syncthreads();
+        for (int i = threadIdx.x; i < 2 * D; i += kThreads) {
+            float v = 0.0f;
+#pragma unroll
+            for (int k = 0; k < kThreads / 32; ++k) v += reinterpret_cast<const float*>(table)[k * 2 * D + i];
+            sums[(long long)blockIdx.x * 2 * D + i] = v;
+        }
+    }
+    if constexpr (sizeof(T) == 2) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) stat = fmaxf(stat, __shfl_xor_sync(0xffffffffu, stat, o));
+        if (lane == 0 && stat > 0.0f) {
+            if (flex.probe) atomicMax(flex.probe_out, (unsigned long long)__float_as_uint(stat));
+            else atomicMax(flex.stats + a.part[0].slot_out, (int)rintf(stat));
+        }
+    }
+}
+
 // Adds the CTAs' sums in their order: a warp to 32 columns and every 32nd CTA, then the warps' sums in their order.
 __global__ void __launch_bounds__(1024)
 heads_sums_kernel(const float* __restrict__ sums, int ctas, int D, float* d_weight0, float* d_weight1) {
@@ -329,6 +565,76 @@ int launch_any(const b2_heads& a, const b2_heads_grads& g, const FlexArgs& flex,
     return B2_OK;
 }
 
+// What a launch of heads_kernel deals out, with `pairs` of features to a lane ...
+Deal deal_of(const b2_heads& a, int runs, int turns) {
+    Deal d = {};
+    while (d.lanes < 5 && 1 << d.lanes < runs) ++d.lanes;
+    const int beside = 32 >> d.lanes;
+    // turns that the tensors' heads fill, so that both have tasks of one size
+    const int most = a.part[0].heads > (a.parts > 1 ? a.part[1].heads : 0) ? a.part[0].heads : a.part[1].heads;
+    const int rounds = (most + beside - 1) / beside, tasks = (rounds + turns - 1) / turns;
+    d.turns = tasks > 0 ? (rounds + tasks - 1) / tasks : 1;
+    // few rows: a turn to a task, for the least latency
+    if (a.rows * rounds < b2::kSms * 8) d.turns = 1;
+    const int each = d.turns * beside;
+    d.first_tasks = (a.part[0].heads + each - 1) / each;
+    d.row_tasks = d.first_tasks + (a.parts > 1 ? (a.part[1].heads + each - 1) / each : 0);
+    d.tasks = a.rows * d.row_tasks;
+    return d;
+}
+constexpr int kBackwardCtas = b2::kSms * 2;
+int ctas_of(const Deal& d, bool backward) {
+    const long long all = (d.tasks + kThreads / 32 - 1) / (kThreads / 32), most = backward ? kBackwardCtas : 1ll << 30;
+    return (int)(all < most ? all : most);
+}
+
+// Vectors: whole ones of every head lie on 16 bytes, and a run of four features is rotated as a whole or not at all.
+bool vectors(const b2_heads& a) { return a.head_dim % 8 == 0 && a.rotary_dim % (a.interleaved ? 4 : 8) == 0; }
+bool aligned_heads(const b2_heads& a, const void* p, int64_t row, int64_t head, int heads, int value_bytes) {
+    return (uintptr_t)p % (4 * value_bytes) == 0 && (a.rows <= 1 || row % 4 == 0) && (heads <= 1 || head % 4 == 0);
+}
+
+template <int MODE, typename T, int VEC, int EACH, bool HALVES>
+int launch_dealt(const b2_heads& a, const b2_heads_grads& g, const FlexArgs& flex, const Deal& deal, float* sums, cudaStream_t st) {
+    const size_t room = MODE == BACKWARD ? (size_t)kThreads / 32 * 2 * a.head_dim * sizeof(float) : 0;
+    B2_CUDA((b2::launch_after(heads_kernel<MODE, T, VEC, EACH, HALVES>, dim3(ctas_of(deal, MODE == BACKWARD)), kThreads, room, st, a, g, flex, deal, sums)));
+    return B2_OK;
+}
+
+// Heads of up to 256 features by heads_kernel, longer ones by heads_any_kernel; `vec`: as vectors.  `ctas` receives how many sums there are.
+template <int MODE, typename T>
+int launch_heads(const b2_heads& a, const b2_heads_grads& g, const FlexArgs& flex, bool vec, float* sums, int* ctas, cudaStream_t st) {
+    const int pairs = a.rotary_dim / 2 + (a.head_dim - a.rotary_dim + 1) / 2;
+    if (pairs > 128) {
+        const dim3 grid = grid_any(a);
+        *ctas = (int)(grid.x * grid.y);
+        return launch_any<MODE, T>(a, g, flex, sums, grid, st);
+    }
+    const int runs = vec ? a.head_dim / 8 : pairs, each = vec || runs <= 32 ? 1 : runs <= 64 ? 2 : 4;
+    const Deal deal = deal_of(a, runs, MODE == BACKWARD && (vec || each > 2) ? 2 : 4);
+    *ctas = ctas_of(deal, MODE == BACKWARD);
+#define B2_DEALT(VEC, EACH)                                                                                          \
+    if (vec == (VEC == 4) && each == EACH)                                                                           \
+        return a.interleaved ? launch_dealt<MODE, T, VEC, EACH, false>(a, g, flex, deal, sums, st)                   \
+                             : launch_dealt<MODE, T, VEC, EACH, true>(a, g, flex, deal, sums, st);
+    B2_DEALT(4, 1)
+    B2_DEALT(1, 1)
+    B2_DEALT(1, 2)
+    B2_DEALT(1, 4)
+#undef B2_DEALT
+    return b2::fail(B2_ERR_INVALID, "no kernel for heads of %d features", a.head_dim);
+}
+
+bool forward_vectors(const b2_heads& a, int value_bytes) {
+    bool vec = vectors(a);
+    for (int i = 0; i < a.parts; ++i) {
+        const b2_heads_part& p = a.part[i];
+        vec = vec && (p.heads == 0 || (aligned_heads(a, p.x, p.x_row, p.x_head, p.heads, value_bytes) && aligned_heads(a, p.out, p.out_row, p.out_head, p.heads, value_bytes) &&
+                                       b2::aligned16(p.weight)));
+    }
+    return vec;
+}
+
 }  // namespace
 
 extern "C" int b2_rotary_turns(int32_t rotary_dim, double base, int32_t scaling, double factor, double original, double low, double high, uint64_t* turns) {
@@ -377,8 +683,9 @@ extern "C" int b2_rotary(const b2_heads* a, int32_t flex, const b2_flex_scale* s
     if (scaled) B2_CHECK(memory.read(scales, "the exponents"));
     if (flex) B2_CHECK(probe ? memory.written(probe_out, "the largest value") : memory.written(stats, "the statistics"));
     cudaStream_t st = (cudaStream_t)stream;
-    if (flex) return launch_any<ROTATE, short>(*a, b2_heads_grads{}, f, nullptr, grid_any(*a), st);
-    return launch_any<ROTATE, float>(*a, b2_heads_grads{}, f, nullptr, grid_any(*a), st);
+    int ctas;
+    if (flex) return launch_heads<ROTATE, short>(*a, b2_heads_grads{}, f, forward_vectors(*a, 2), nullptr, &ctas, st);
+    return launch_heads<ROTATE, float>(*a, b2_heads_grads{}, f, forward_vectors(*a, 4), nullptr, &ctas, st);
 }
 
 static int check_norm_of_heads(const b2_heads* a) {
@@ -393,14 +700,16 @@ extern "C" int b2_heads_fprop(const b2_heads* a, void* stream) {
     if (a->rows == 0 || total_heads(*a) == 0) return B2_OK;
     b2::Memory memory;
     B2_CHECK(check_forward(a, 4, memory));
-    return launch_any<FORWARD, float>(*a, b2_heads_grads{}, FlexArgs{}, nullptr, grid_any(*a), (cudaStream_t)stream);
+    int ctas;
+    return launch_heads<FORWARD, float>(*a, b2_heads_grads{}, FlexArgs{}, forward_vectors(*a, 4), nullptr, &ctas, (cudaStream_t)stream);
 }
 
 extern "C" int b2_heads_bprop_scratch_bytes(const b2_heads* a, size_t* bytes) {
     B2_REQUIRE(bytes, "missing argument");
     B2_CHECK(check_norm_of_heads(a));
     const dim3 grid = grid_any(*a);
-    *bytes = (size_t)grid.x * grid.y * 2 * a->head_dim * sizeof(float) + 256;
+    const size_t ctas = (size_t)grid.x * grid.y;
+    *bytes = (ctas > kBackwardCtas ? ctas : kBackwardCtas) * 2 * a->head_dim * sizeof(float) + 256;
     return B2_OK;
 }
 
@@ -456,11 +765,18 @@ extern "C" int b2_heads_bprop(const b2_heads* a, const b2_heads_grads* g, void* 
     if (work) B2_CHECK(check_reads(a, memory));
     cudaStream_t st = (cudaStream_t)stream;
     float* sums = (float*)(((uintptr_t)scratch + 255) / 256 * 256);
-    const dim3 grid = grid_any(*a);
-    if (work) B2_CHECK((launch_any<BACKWARD, float>(*a, *g, FlexArgs{}, sums, grid, st)));
+    bool vec = vectors(*a);
+    for (int i = 0; i < a->parts; ++i) {
+        const b2_heads_part& p = a->part[i];
+        const b2_heads_part_grads& d = g->part[i];
+        vec = vec && (p.heads == 0 || (aligned_heads(*a, p.x, p.x_row, p.x_head, p.heads, 4) && aligned_heads(*a, d.d_out, d.d_out_row, d.d_out_head, p.heads, 4) &&
+                                       (!d.d_x || aligned_heads(*a, d.d_x, d.d_x_row, d.d_x_head, p.heads, 4)) && b2::aligned16(p.weight)));
+    }
+    int ctas = 0;
+    if (work) B2_CHECK((launch_heads<BACKWARD, float>(*a, *g, FlexArgs{}, vec, sums, &ctas, st)));
     if (weights[0] || weights[1]) {
         const int D = a->head_dim;
-        B2_CUDA((b2::launch_after(heads_sums_kernel, dim3((2 * D + 31) / 32), 1024, 0, st, (const float*)sums, work ? (int)(grid.x * grid.y) : 0, D,
+        B2_CUDA((b2::launch_after(heads_sums_kernel, dim3((2 * D + 31) / 32), 1024, 0, st, (const float*)sums, ctas, D,
                                   weights[0], weights[1])));
     }
     return B2_OK;
