@@ -7,7 +7,7 @@
 // Angles: a frequency is a 64-bit fraction of a turn, so that the product with a position, modulo 2^64, is the fraction of a
 // turn that is left, exact but for the rounding of the frequency (2^-45 of a turn at position a million).  In fp32
 // position * frequency would be 0.03 radians off there.  The nearest quarter turn is taken off as an integer and the rest,
-// at most an eighth of a turn, goes to sincospif.
+// at most an eighth of a turn, goes into the series of sine and cosine.
 #include <cmath>
 #include <cstdint>
 
@@ -49,15 +49,25 @@ __device__ __forceinline__ bool position_of(const b2_heads& a, long long row, co
     }
 }
 
-// amplitude * (cos, sin) of the fraction of a turn whose 64 bits are `phase`
+// amplitude * (cos, sin) of the fraction of a turn whose 64 bits are `phase`: of what is left of the nearest quarter turn by
+// their series, up to x^9 / 9! and x^10 / 10!, whose next terms are 2e-9 and 5e-10 at an eighth of a turn.  (A third of the
+// instructions of sincospif, which would look for the quarter turn again: the forward pass of 8192 x 40 heads took 70 us with it, 66 so.)
 __device__ __forceinline__ float2 turn_of(unsigned long long phase, float amplitude) {
     const unsigned t = (unsigned)(phase >> 32);
     const unsigned quarter = (t + 0x20000000u) >> 30;                                     // 0 ... 4
-    float s, c;
-    sincospif((float)(int)(t - (quarter << 30)) * 0x1p-31f, &s, &c);
+    const float x = (float)(int)(t - (quarter << 30)) * 1.4629180792671596e-9f;           // 2 pi / 2^32
+    const float z = x * x;
+    float s = fmaf(z, 2.7557319e-6f, -1.9841270e-4f), c = fmaf(z, -2.7557319e-7f, 2.4801587e-5f);
+    s = fmaf(z, s, 8.3333333e-3f);
+    c = fmaf(z, c, -1.3888889e-3f);
+    s = fmaf(z, s, -1.6666667e-1f);
+    c = fmaf(z, c, 4.1666667e-2f);
+    s = fmaf(x * z, s, x);
+    c = fmaf(z, c, -0.5f);
+    c = fmaf(z, c, 1.0f);
     const bool swap = quarter & 1;
-    const float x = swap ? s : c, y = swap ? c : s;
-    return make_float2(amplitude * ((quarter + 1) & 2 ? -x : x), amplitude * (quarter & 2 ? -y : y));
+    const float u = swap ? s : c, v = swap ? c : s;
+    return make_float2(amplitude * ((quarter + 1) & 2 ? -u : u), amplitude * (quarter & 2 ? -v : v));
 }
 
 __device__ __forceinline__ float warp_sum(float v) {
@@ -193,9 +203,18 @@ heads_any_kernel(const b2_heads a, const b2_heads_grads g, const FlexArgs flex, 
 // that is a task, of the queries or of the keys of one row.
 struct Deal {
     int lanes, turns, first_tasks, row_tasks;       // tasks of a row: of the first tensor, of both
+    int ahead;                                      // whether the next task's heads are fetched into L2
     long long tasks;
 };
 constexpr int kThreads = 256;
+// Heads that a lane loads at once, by how many features of each it holds, and CTAs to an SM.  Eight features, 8192 rows of 40 heads of
+// 128 forward, four heads: 59 us with two CTAs, 63 with three; two heads and four CTAs 72; one and five 85.  Gradients, two heads: 127
+// with two, 120 with three; one and three 146.  Rotation alone, 8192 x 20, four heads: 28.5 with three, 33 with two.
+__host__ __device__ constexpr int unrolled(int mode, int values) { return mode == BACKWARD && values >= 8 ? 2 : 4; }
+__host__ __device__ constexpr int blocks_to(int mode, int values) { return values < 8 ? (mode == BACKWARD ? 2 : 3) : mode == FORWARD ? 2 : 3; }
+// CTAs that stay, and fetch the heads of their next task into L2 meanwhile: gradients 142 us without, 127 with; forward 62 and 59; a
+// rotation, which waits for nothing but its loads, 28.5 without and 31 with.
+__host__ __device__ constexpr bool stays(int mode) { return mode != ROTATE; }
 
 template <int VEC, typename T>
 __device__ __forceinline__ void get(const T* p, float* v) {
@@ -233,9 +252,9 @@ __device__ __forceinline__ void put(T* p, const float* v, float& stat) {
 //   else:   VEC 4: two runs half a head apart, each of two pairs; VEC 1: a pair
 // BACKWARD: sums for the weights stay in registers and are added over the CTA at the end.
 template <int MODE, typename T, int VEC, int EACH, bool HALVES>
-__global__ void __launch_bounds__(kThreads, MODE == BACKWARD ? 2 : 3)
+__global__ void __launch_bounds__(kThreads, blocks_to(MODE, 2 * VEC * EACH))
 heads_kernel(const b2_heads a, const b2_heads_grads g, const FlexArgs flex, const Deal deal, float* __restrict__ sums) {
-    constexpr int N = 2 * VEC * EACH, P = N / 2, U = MODE == BACKWARD ? (N > 4 ? 2 : 4) : 4;
+    constexpr int N = 2 * VEC * EACH, P = N / 2, U = unrolled(MODE, N);
     static_assert(VEC == 1 || EACH == 1, "one pair of vectors");
     constexpr bool APART = VEC == 4 && HALVES;                  // the features of pair k: k and VEC + k, else 2 k and 2 k + 1
     after_earlier_kernels();
@@ -284,26 +303,45 @@ heads_kernel(const b2_heads a, const b2_heads_grads g, const FlexArgs flex, cons
 #pragma unroll
                 for (int k = 0; k < VEC; ++k) v[VEC * e + k] = 0.0f;
     };
+    const float share = 1.0f / (float)D;
     const long long step = (long long)gridDim.x * (kThreads / 32);
     for (long long task = (long long)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5); task < deal.tasks; task += step) {
         const long long row = deal.tasks <= 0xffffffffll ? (long long)((unsigned)task / (unsigned)deal.row_tasks) : task / deal.row_tasks;
         const int in_row = (int)(task - row * deal.row_tasks), n = in_row >= deal.first_tasks;
         const b2_heads_part& p = a.part[n];
         const b2_heads_part_grads& d = g.part[n];
-        const int head = (in_row - (n ? deal.first_tasks : 0)) * deal.turns * beside + mine;
+        const int head = (in_row - (n ? deal.first_tasks : 0)) * deal.turns * beside + mine, left = p.heads - head;
+        const T* from = static_cast<const T*>(p.x) + row * p.x_row + head * p.x_head;
+        const T* from_grad = MODE == BACKWARD ? reinterpret_cast<const T*>(d.d_out) + row * d.d_out_row + head * d.d_out_head : nullptr;
+        // (heads of the next task are on their way into L2 meanwhile)
+        if (deal.ahead && task + step < deal.tasks) {
+            const long long then = task + step, row2 = deal.tasks <= 0xffffffffll ? (long long)((unsigned)then / (unsigned)deal.row_tasks) : then / deal.row_tasks;
+            const int in_row2 = (int)(then - row2 * deal.row_tasks), n2 = in_row2 >= deal.first_tasks;
+            const b2_heads_part& p2 = a.part[n2];
+            const int head2 = (in_row2 - (n2 ? deal.first_tasks : 0)) * deal.turns * beside, count = min(deal.turns * beside, p2.heads - head2);
+            const auto fetch = [&](const T* at, long long head_stride) {
+                if (head_stride != D) return;
+                const char* first = reinterpret_cast<const char*>(at);
+                for (int i = lane * 128; i < count * D * (int)sizeof(T); i += 32 * 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(first + i));
+            };
+            fetch(static_cast<const T*>(p2.x) + row2 * p2.x_row + head2 * p2.x_head, p2.x_head);
+            if constexpr (MODE == BACKWARD) {
+                const b2_heads_part_grads& d2 = g.part[n2];
+                fetch(reinterpret_cast<const T*>(d2.d_out) + row2 * d2.d_out_row + head2 * d2.d_out_head, d2.d_out_head);
+            }
+        }
         float x[U][N], y[MODE == BACKWARD ? U : 1][N], rstd[U];
         long long position = 0;
         const bool good = r == 0 || position_of(a, row, flex.table, position);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int h = head + u * beside;
-            const bool live = u < deal.turns && h < p.heads;
+            const bool live = u < deal.turns && u * beside < left;
             rstd[u] = 1.0f;
             if (live) {
-                load(static_cast<const T*>(p.x) + row * p.x_row + h * p.x_head, x[u]);
+                load(from + u * beside * p.x_head, x[u]);
                 if constexpr (MODE == BACKWARD) {
-                    load(reinterpret_cast<const T*>(d.d_out) + row * d.d_out_row + h * d.d_out_head, y[u]);
-                    rstd[u] = p.rstd[row * p.heads + h];
+                    load(from_grad + u * beside * d.d_out_head, y[u]);
+                    rstd[u] = p.rstd[row * p.heads + head + u * beside];
                 }
             } else {
 #pragma unroll
@@ -326,9 +364,12 @@ heads_kernel(const b2_heads a, const b2_heads_grads g, const FlexArgs flex, cons
 #pragma unroll
         for (int k = 0; k < P; ++k) {
             turn[k] = make_float2(1.0f, 0.0f);
-            if (turning >> k & 1) turn[k] = good ? turn_of((unsigned long long)position * frequency[k], a.amplitude) : make_float2(NAN, NAN);
+            if (r > 0) turn[k] = turn_of((unsigned long long)position * frequency[k], a.amplitude);
+            if (!good) turn[k] = make_float2(NAN, NAN);
             if (MODE == BACKWARD || (MODE == ROTATE && a.inverse)) turn[k].y = -turn[k].y;
         }
+        const long long out_head = MODE == BACKWARD ? d.d_x_head : p.out_head;
+        T* to = MODE == BACKWARD ? reinterpret_cast<T*>(d.d_x) + row * d.d_x_row + head * out_head : static_cast<T*>(p.out) + row * p.out_row + head * out_head;
         const auto rotate = [&](float* v) {
 #pragma unroll
             for (int k = 0; k < P; ++k) {
@@ -340,44 +381,60 @@ heads_kernel(const b2_heads a, const b2_heads_grads g, const FlexArgs flex, cons
                 }
             }
         };
-        const auto over_head = [&](float q) {
-            for (int o = 1 << deal.lanes >> 1; o > 0; o >>= 1) q += __shfl_xor_sync(0xffffffffu, q, o);
-            return q;
+        float sum[MODE == BACKWARD ? N : 1];                    // of the task, for its weight
+        // sums over the lanes of each head, of all heads next to one another
+        const auto over_heads = [&](float (&q)[U]) {
+#pragma unroll
+            for (int o = 0; o < 5; ++o)
+                if (o < deal.lanes)
+#pragma unroll
+                    for (int u = 0; u < U; ++u) q[u] += __shfl_xor_sync(0xffffffffu, q[u], 1 << o);
         };
+        float q[U];
+        if constexpr (MODE == FORWARD) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                q[u] = 0.0f;
+#pragma unroll
+                for (int j = 0; j < N; ++j) q[u] = fmaf(x[u][j], x[u][j], q[u]);
+            }
+            over_heads(q);
+        }
+        if constexpr (MODE == BACKWARD) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                rotate(y[u]);
+                q[u] = 0.0f;
+#pragma unroll
+                for (int j = 0; j < N; ++j) {
+                    x[u][j] *= rstd[u];                         // x^
+                    sum[j] = u == 0 ? y[u][j] * x[u][j] : fmaf(y[u][j], x[u][j], sum[j]);
+                    y[u][j] *= w[j];
+                    q[u] = fmaf(y[u][j], x[u][j], q[u]);
+                }
+            }
+            over_heads(q);
+        }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             if (u >= deal.turns) break;
-            const int h = head + u * beside;
-            const bool live = h < p.heads;
+            const bool live = u * beside < left;
             float* v = x[u];
             T* out = nullptr;
             if constexpr (MODE == FORWARD) {
-                float q = 0.0f;
-#pragma unroll
-                for (int j = 0; j < N; ++j) q = fmaf(v[j], v[j], q);
-                const float root = __frsqrt_rn(__fdividef(over_head(q), (float)D) + a.eps);
-                if (p.rstd && live && sub == 0) p.rstd[row * p.heads + h] = root;
+                const float root = rsqrtf(fmaf(q[u], share, a.eps));
+                if (p.rstd && live && sub == 0) p.rstd[row * p.heads + head + u * beside] = root;
 #pragma unroll
                 for (int j = 0; j < N; ++j) v[j] *= root * w[j];
             }
             if constexpr (MODE == BACKWARD) {
-                rotate(y[u]);
-                float q = 0.0f;
+                const float mean = q[u] * share * rstd[u];
 #pragma unroll
-                for (int j = 0; j < N; ++j) {
-                    v[j] *= rstd[u];                            // x^
-                    const float dw = y[u][j] * v[j];
-                    q = fmaf(w[j], dw, q);
-                    if (n) acc[1][j] += dw;
-                    else acc[0][j] += dw;
-                }
-                const float mean = __fdividef(over_head(q), (float)D);
-#pragma unroll
-                for (int j = 0; j < N; ++j) v[j] = rstd[u] * (w[j] * y[u][j] - v[j] * mean);
-                if (d.d_x && live) out = reinterpret_cast<T*>(d.d_x) + row * d.d_x_row + h * d.d_x_head;
+                for (int j = 0; j < N; ++j) v[j] = fmaf(-v[j], mean, rstd[u] * y[u][j]);
+                if (d.d_x && live) out = to + u * beside * out_head;
             } else {
                 rotate(v);
-                if (live) out = static_cast<T*>(p.out) + row * p.out_row + h * p.out_head;
+                if (live) out = to + u * beside * out_head;
             }
             if (!out) continue;
             if constexpr (sizeof(T) == 2) {
@@ -392,6 +449,15 @@ heads_kernel(const b2_heads a, const b2_heads_grads g, const FlexArgs flex, cons
 #pragma unroll
             for (int e = 0; e < 2 * EACH; ++e)
                 if (at[e] >= 0) put<VEC>(out + at[e], v + VEC * e, stat);
+        }
+        if constexpr (MODE == BACKWARD) {
+            if (n) {
+#pragma unroll
+                for (int j = 0; j < N; ++j) acc[1][j] += sum[j];
+            } else {
+#pragma unroll
+                for (int j = 0; j < N; ++j) acc[0][j] += sum[j];
+            }
         }
     }
     if constexpr (MODE == BACKWARD) {
@@ -582,9 +648,9 @@ Deal deal_of(const b2_heads& a, int runs, int turns) {
     d.tasks = a.rows * d.row_tasks;
     return d;
 }
-constexpr int kBackwardCtas = b2::kSms * 2;
-int ctas_of(const Deal& d, bool backward) {
-    const long long all = (d.tasks + kThreads / 32 - 1) / (kThreads / 32), most = backward ? kBackwardCtas : 1ll << 30;
+constexpr int kBackwardCtas = b2::kSms * 3;
+int ctas_of(const Deal& d, int mode, int values) {
+    const long long all = (d.tasks + kThreads / 32 - 1) / (kThreads / 32), most = stays(mode) ? b2::kSms * blocks_to(mode, values) : 1 << 30;
     return (int)(all < most ? all : most);
 }
 
@@ -597,13 +663,14 @@ bool aligned_heads(const b2_heads& a, const void* p, int64_t row, int64_t head, 
 template <int MODE, typename T, int VEC, int EACH, bool HALVES>
 int launch_dealt(const b2_heads& a, const b2_heads_grads& g, const FlexArgs& flex, const Deal& deal, float* sums, cudaStream_t st) {
     const size_t room = MODE == BACKWARD ? (size_t)kThreads / 32 * 2 * a.head_dim * sizeof(float) : 0;
-    B2_CUDA((b2::launch_after(heads_kernel<MODE, T, VEC, EACH, HALVES>, dim3(ctas_of(deal, MODE == BACKWARD)), kThreads, room, st, a, g, flex, deal, sums)));
+    B2_CUDA((b2::launch_after(heads_kernel<MODE, T, VEC, EACH, HALVES>, dim3(ctas_of(deal, MODE, 2 * VEC * EACH)), kThreads, room, st, a, g, flex, deal, sums)));
     return B2_OK;
 }
 
-// Heads of up to 256 features by heads_kernel, longer ones by heads_any_kernel; `vec`: as vectors.  `ctas` receives how many sums there are.
+// Heads of up to 256 features by heads_kernel, longer ones by heads_any_kernel; `vec`: as vectors; `elsewhere`: operands
+// in page-locked memory, which are not fetched ahead.  `ctas` receives how many sums there are.
 template <int MODE, typename T>
-int launch_heads(const b2_heads& a, const b2_heads_grads& g, const FlexArgs& flex, bool vec, float* sums, int* ctas, cudaStream_t st) {
+int launch_heads(const b2_heads& a, const b2_heads_grads& g, const FlexArgs& flex, bool vec, bool elsewhere, float* sums, int* ctas, cudaStream_t st) {
     const int pairs = a.rotary_dim / 2 + (a.head_dim - a.rotary_dim + 1) / 2;
     if (pairs > 128) {
         const dim3 grid = grid_any(a);
@@ -611,8 +678,9 @@ int launch_heads(const b2_heads& a, const b2_heads_grads& g, const FlexArgs& fle
         return launch_any<MODE, T>(a, g, flex, sums, grid, st);
     }
     const int runs = vec ? a.head_dim / 8 : pairs, each = vec || runs <= 32 ? 1 : runs <= 64 ? 2 : 4;
-    const Deal deal = deal_of(a, runs, MODE == BACKWARD && (vec || each > 2) ? 2 : 4);
-    *ctas = ctas_of(deal, MODE == BACKWARD);
+    Deal deal = deal_of(a, runs, unrolled(MODE, vec ? 8 : 2 * each));
+    deal.ahead = stays(MODE) && !elsewhere;
+    *ctas = ctas_of(deal, MODE, vec ? 8 : 2 * each);
 #define B2_DEALT(VEC, EACH)                                                                                          \
     if (vec == (VEC == 4) && each == EACH)                                                                           \
         return a.interleaved ? launch_dealt<MODE, T, VEC, EACH, false>(a, g, flex, deal, sums, st)                   \
@@ -684,8 +752,8 @@ extern "C" int b2_rotary(const b2_heads* a, int32_t flex, const b2_flex_scale* s
     if (flex) B2_CHECK(probe ? memory.written(probe_out, "the largest value") : memory.written(stats, "the statistics"));
     cudaStream_t st = (cudaStream_t)stream;
     int ctas;
-    if (flex) return launch_heads<ROTATE, short>(*a, b2_heads_grads{}, f, forward_vectors(*a, 2), nullptr, &ctas, st);
-    return launch_heads<ROTATE, float>(*a, b2_heads_grads{}, f, forward_vectors(*a, 4), nullptr, &ctas, st);
+    if (flex) return launch_heads<ROTATE, short>(*a, b2_heads_grads{}, f, forward_vectors(*a, 2), memory.elsewhere, nullptr, &ctas, st);
+    return launch_heads<ROTATE, float>(*a, b2_heads_grads{}, f, forward_vectors(*a, 4), memory.elsewhere, nullptr, &ctas, st);
 }
 
 static int check_norm_of_heads(const b2_heads* a) {
@@ -701,7 +769,7 @@ extern "C" int b2_heads_fprop(const b2_heads* a, void* stream) {
     b2::Memory memory;
     B2_CHECK(check_forward(a, 4, memory));
     int ctas;
-    return launch_heads<FORWARD, float>(*a, b2_heads_grads{}, FlexArgs{}, forward_vectors(*a, 4), nullptr, &ctas, (cudaStream_t)stream);
+    return launch_heads<FORWARD, float>(*a, b2_heads_grads{}, FlexArgs{}, forward_vectors(*a, 4), memory.elsewhere, nullptr, &ctas, (cudaStream_t)stream);
 }
 
 extern "C" int b2_heads_bprop_scratch_bytes(const b2_heads* a, size_t* bytes) {
@@ -773,7 +841,7 @@ extern "C" int b2_heads_bprop(const b2_heads* a, const b2_heads_grads* g, void* 
                                        (!d.d_x || aligned_heads(*a, d.d_x, d.d_x_row, d.d_x_head, p.heads, 4)) && b2::aligned16(p.weight)));
     }
     int ctas = 0;
-    if (work) B2_CHECK((launch_heads<BACKWARD, float>(*a, *g, FlexArgs{}, vec, sums, &ctas, st)));
+    if (work) B2_CHECK((launch_heads<BACKWARD, float>(*a, *g, FlexArgs{}, vec, memory.elsewhere, sums, &ctas, st)));
     if (weights[0] || weights[1]) {
         const int D = a->head_dim;
         B2_CUDA((b2::launch_after(heads_sums_kernel, dim3((2 * D + 31) / 32), 1024, 0, st, (const float*)sums, ctas, D,
