@@ -757,7 +757,7 @@ typedef struct {
 } b2_muon_hyper;
 typedef struct {
     size_t plan_bytes, scratch_bytes;
-    int64_t matrices, chunks, items, blocks;
+    int64_t matrices, chunks, items, blocks, solos;
 } b2_muon_sizes;
 int b2_muon_plan_sizes(const b2_muon_matrix* matrices, int32_t count, b2_muon_sizes* sizes);
 int b2_muon_launches(const b2_muon_sizes* sizes, int32_t* launches);     /* kernels that a step launches */

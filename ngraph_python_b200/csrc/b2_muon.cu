@@ -73,7 +73,7 @@ struct Group {                               // matrices whose steps run next to
     long long first, count;
 };
 struct Header {
-    long long matrices, chunks, items, blocks, groups;
+    long long matrices, chunks, items, blocks, solos, groups;
 };
 constexpr size_t kHeader = 64;
 
@@ -83,6 +83,7 @@ struct Layout {
     std::vector<Block> blocks;
     std::vector<Item> items;
     std::vector<Group> groups;
+    long long solos;                         // the last of the matrices, which have a CTA to themselves
     long long bytes;                         // of planes
     size_t plan_bytes() const {
         return kHeader + matrices.size() * sizeof(Matrix) + chunks.size() * sizeof(Chunk) + blocks.size() * sizeof(Block) + items.size() * sizeof(Item) +
@@ -111,11 +112,11 @@ __device__ __forceinline__ const Item* items_of(const void* plan) { return reint
 __device__ __forceinline__ const Group* groups_of(const void* plan) { return reinterpret_cast<const Group*>(items_of(plan) + header_of(plan)->items); }
 
 struct Told {                                // what the caller says of the plan; a step with other sizes does nothing
-    long long matrices, chunks, items, blocks;
+    long long matrices, chunks, items, blocks, solos;
 };
 __device__ __forceinline__ bool fits(const void* plan, const Told& t) {
     const Header* h = header_of(plan);
-    return h->matrices == t.matrices && h->chunks == t.chunks && h->items == t.items && h->blocks == t.blocks;
+    return h->matrices == t.matrices && h->chunks == t.chunks && h->items == t.items && h->blocks == t.blocks && h->solos == t.solos;
 }
 
 // The scratch: sums of squares by chunk; counters; planes.
@@ -154,11 +155,22 @@ muon_mean_kernel(const void* plan, const Told told, const Rates r, const float* 
         const Chunk c = chunks_of(plan)[k];
         const Matrix& t = matrices_of(plan)[c.matrix];
         double q = 0.0;
-        for (int i = threadIdx.x; i < c.n; i += kMeanThreads) {
-            const float g = t.grad[c.at + i] * s, m = r.mu * t.mean[c.at + i] + r.rest * g;
-            const float u = r.nesterov ? r.rest * g + r.mu * m : m;
-            t.mean[c.at + i] = m;
-            q = fma((double)u, (double)u, q);
+        for (int i0 = threadIdx.x; i0 < c.n; i0 += 8 * kMeanThreads) {
+            float g[8], m[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int i = i0 + j * kMeanThreads;
+                g[j] = i < c.n ? t.grad[c.at + i] : 0.0f;
+                m[j] = i < c.n ? t.mean[c.at + i] : 0.0f;
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int i = i0 + j * kMeanThreads;
+                m[j] = r.mu * m[j] + r.rest * (g[j] * s);
+                const float u = r.nesterov ? r.rest * (g[j] * s) + r.mu * m[j] : m[j];
+                if (i < c.n) t.mean[c.at + i] = m[j];
+                q = fma((double)u, (double)u, q);
+            }
         }
         q = cta_sum(q, words);
         if (threadIdx.x == 0) room.sums[k] = q;
@@ -174,7 +186,7 @@ __device__ __forceinline__ void parts(float u, float v, unsigned& hi, unsigned& 
     lo = *reinterpret_cast<const unsigned*>(&l);
 }
 // Eight values next to one another of row `row` of a block, 8 `piece` columns in
-__device__ __forceinline__ void put_piece(char* block, int row, int piece, const float* v) {
+__device__ __forceinline__ void put_piece(char* block, int row, int piece, const float* v, int to_lo = kBlockBytes) {
     uint4 hi, lo;
     parts(v[0], v[1], hi.x, lo.x);
     parts(v[2], v[3], hi.y, lo.y);
@@ -182,7 +194,7 @@ __device__ __forceinline__ void put_piece(char* block, int row, int piece, const
     parts(v[6], v[7], hi.w, lo.w);
     char* at = block + row * 128 + ((piece ^ (row & 7)) << 4);
     *reinterpret_cast<uint4*>(at) = hi;
-    *reinterpret_cast<uint4*>(at + kBlockBytes) = lo;
+    *reinterpret_cast<uint4*>(at + to_lo) = lo;
 }
 __device__ __forceinline__ float2 halves(unsigned w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
 __device__ __forceinline__ void get_piece(const char* block, int row, int piece, float* v) {
@@ -313,11 +325,10 @@ muon_product_kernel(const void* plan, const Told told, const Rates r, const Poly
         *fail_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 1) {
-        tmem_alloc(tmem_holder, 512);
-        asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    }
+    if (warp == 1) tmem_alloc(tmem_holder, 512);
+    // (the launch for small matrices goes by this: where it starts, all that came before this kernel has ended)
     asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -603,6 +614,251 @@ muon_product_kernel(const void* plan, const Told told, const Rates r, const Poly
     }
 }
 
+// ---- small matrices: all of a step in one CTA ----------------------------------------------------------------
+// x and A (then B in its place) stay in shared memory in the form above, sums in tensor memory, in columns of their own for every block
+// of k; a product is a few instructions between two barriers, 1.2 us where the launch for all matrices takes 8.  A matrix that has more rows
+// than columns is taken as its transpose.  x: [part][block along][block across], across the shorter side.
+constexpr int kSoloThreads = 256;
+constexpr int kSoloBlocks = 13;                             // of x and A in both parts
+constexpr int kSoloColumns = 512;                           // of tensor memory
+constexpr int kSoloShared = 1024 + (2 * kSoloBlocks + 1) * kBlockBytes + 512;       // (the tensor core reads 128 rows, of 64 the next block as well)
+static_assert(kSoloShared <= 227 << 10, "shared memory of a CTA");
+
+__device__ __forceinline__ unsigned long long describe_apart(unsigned address, unsigned apart) {
+    return (describe(address, 0) & ~(0x3FFFull << 16)) | (unsigned long long)(apart >> 4) << 16;
+}
+
+__global__ void __launch_bounds__(kSoloThreads, 1)
+muon_solo_kernel(const void* plan, const Told told, const Rates r, const Poly poly, const float* lr, const float* grad_scale, float* step, int alone, int* status) {
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char* smem = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    __shared__ double words[kMeanThreads / 32];
+    __shared__ unsigned long long bar;
+    __shared__ unsigned tmem_holder;
+    __shared__ int fail_flag;
+    const int warp = warp_uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        mbar_init(&bar, 1);
+        fail_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 0) tmem_alloc(&tmem_holder, kSoloColumns);
+    // Behind the launch for the other matrices, which lets this one start when all earlier kernels have ended: nothing of it is
+    // waited for until the end.
+    if (alone) asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (alone) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const unsigned tmem = (unsigned)warp_uniform((int)tmem_holder);
+    if (fits(plan, told)) {
+        if (alone && blockIdx.x == 0 && threadIdx.x == 0 && step) *step += 1.0f;
+        const Matrix& t = matrices_of(plan)[told.matrices - told.solos + blockIdx.x];
+        const bool tall = t.tall != 0;
+        const int across = t.n_blocks, along = max(t.row_blocks, t.col_blocks), n = min(t.rows, t.cols), m = max(t.rows, t.cols);
+        const int x_part = across * along * kBlockBytes, s_part = across * across * kBlockBytes;
+        char *x = reinterpret_cast<char*>(smem), *square = x + 2 * x_part;
+        const unsigned x_at = smem_u32(x), s_at = smem_u32(square);
+        // the mean, and the sum of squares of u
+        const float s = grad_scale ? *grad_scale : 1.0f;
+        const auto u_of = [&](float mean, float grad) { return r.nesterov ? r.rest * (grad * s) + r.mu * mean : mean; };
+        const int size = t.rows * t.cols;
+        double q = 0.0;
+        constexpr int kBatch = 8;                           // values of a thread whose loads are issued together
+        for (int i0 = threadIdx.x; i0 < size; i0 += kBatch * kSoloThreads) {
+            float g[kBatch], mean[kBatch];
+#pragma unroll
+            for (int j = 0; j < kBatch; ++j) {
+                const int i = i0 + j * kSoloThreads;
+                g[j] = i < size ? t.grad[i] : 0.0f;
+                mean[j] = i < size ? t.mean[i] : 0.0f;
+            }
+#pragma unroll
+            for (int j = 0; j < kBatch; ++j) {
+                const int i = i0 + j * kSoloThreads;
+                mean[j] = r.mu * mean[j] + r.rest * (g[j] * s);
+                const float u = u_of(mean[j], g[j]);
+                if (i < size) t.mean[i] = mean[j];
+                q = fma((double)u, (double)u, q);
+            }
+        }
+        q = cta_sum(q, words);
+        __syncthreads();                                    // (means of other threads are read)
+        const float inverse = (float)(1.0 / (sqrt(q) + (double)r.eps)), up = power(poly.x[0]);
+        for (int e = threadIdx.x; e < across * kBlock * along * 8; e += kSoloThreads) {
+            // neighbours in memory to neighbouring threads
+            const int i = tall ? e % (across * kBlock) : e / (along * 8), piece = tall ? e / (across * kBlock) : e % (along * 8);
+            float v[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int at = piece * 8 + j;
+                v[j] = 0.0f;
+                if (i < n && at < m) {
+                    const int place = tall ? at * t.cols + i : i * t.cols + at;
+                    v[j] = u_of(t.mean[place], t.grad[place]) * inverse * up;
+                }
+            }
+            put_piece(x + ((piece >> 3) * across + (i >> 6)) * kBlockBytes, i & 63, piece & 7, v, x_part);
+        }
+
+        const int quarter = warp & 3, half = warp >> 2, row = quarter * 32 + lane;
+        const bool used = row < across * kBlock;            // (of a warp all or none)
+        const unsigned lanes = tmem + ((unsigned)(quarter * 32) << 16);
+        unsigned parity = 0;
+        // what has been stored is there for the tensor core; `issue` by one thread; its results are there for everybody
+        const auto products = [&](auto&& issue) {
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            tc_fence_before();
+            __syncthreads();
+            if (warp == 0 && elect_one()) {
+                tc_fence_after();
+                issue();
+                tc_commit(&bar);
+            }
+            __syncwarp();
+            if (!mbar_wait(&bar, parity)) atomicExch(&fail_flag, 1);
+            parity ^= 1u;
+            tc_fence_after();
+        };
+        // three products of parts, the small ones first, of 64 of k
+        const auto three = [&](unsigned sum, unsigned p, unsigned p_part, unsigned long long q_hi, unsigned q_part, unsigned q_step, unsigned instruction, bool more) {
+            const unsigned long long p_hi = describe(p, 0), p_lo = describe(p + p_part, 0), q_lo = q_hi + (q_part >> 4);
+            for (int k = 0; k < 4; ++k) multiply_f16(sum, p_hi + 2 * k, q_lo + k * q_step, instruction, more || k > 0);
+            for (int k = 0; k < 4; ++k) multiply_f16(sum, p_lo + 2 * k, q_hi + k * q_step, instruction, 1);
+            for (int k = 0; k < 4; ++k) multiply_f16(sum, p_hi + 2 * k, q_hi + k * q_step, instruction, 1);
+        };
+        const auto instruction_of = [](int width, unsigned q_major) { return (1u << 4) | (q_major << 16) | ((unsigned)(width >> 3) << 17) | ((128u >> 4) << 24); };
+        const auto add_columns = [&](unsigned from, float* v) {             // 32 columns of sums
+            unsigned w[32];
+            tmem_ld16(lanes + from, w);
+            tmem_ld16(lanes + from + 16, w + 16);
+            tmem_ld_wait();
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] += __uint_as_float(w[j]);
+        };
+        const int side = across * kBlock, per_sum = (along * side + kSoloColumns - 1) / kSoloColumns, sums = (along + per_sum - 1) / per_sum;
+        const int chunk = kSoloColumns / across;            // columns of x that are multiplied at a time
+        // the last x in fp32, a block in the place of its two parts: 32 rows in either
+        const auto value_at = [&](int block, int row_of) {
+            return reinterpret_cast<float*>(x + (block * across + (row_of >> 6)) * kBlockBytes + (row_of & 32 ? x_part : 0)) + (row_of & 31) * kBlock;
+        };
+        const double rate = lr ? (double)*lr : r.lr;
+        const float keep = (float)(1.0 - rate * r.wd * (double)t.decay), move = (float)(rate * (double)t.scale);
+        for (int k = 0; k < poly.steps; ++k) {
+            const bool last = k == poly.steps - 1;
+            float held[64];                                 // this thread's part of A
+            products([&] {
+                for (int b = 0; b < along; ++b) {
+                    const unsigned at = x_at + b * across * kBlockBytes;
+                    three(tmem + b / per_sum * side, at, x_part, describe(at, 0), x_part, 2, instruction_of(side, 0), b % per_sum > 0);
+                }
+            });
+            if (used) {
+                const float factor = power(poly.square[k] - 2 * poly.x[k]);
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    if (c >= across) continue;
+                    const int col = (half * across + c) * 32;
+                    float* v = held + 32 * c;
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) v[j] = 0.0f;
+                    for (int b = 0; b < sums; ++b) add_columns(b * side + col, v);
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) v[j] *= factor;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) put_piece(square + ((col >> 6) * across + (row >> 6)) * kBlockBytes, row & 63, ((col & 63) >> 3) + e, v + 8 * e, s_part);
+                }
+            }
+            products([&] {
+                for (int b = 0; b < across; ++b) {
+                    const unsigned at = s_at + b * across * kBlockBytes;
+                    three(tmem + b * side, at, s_part, describe(at, 0), s_part, 2, instruction_of(side, 0), false);
+                }
+            });
+            if (used) {
+                const float factor = poly.c * power(poly.poly[k] - 2 * poly.square[k]), linear = poly.b * power(poly.poly[k] - poly.square[k]);
+                const float diagonal = poly.a * power(poly.poly[k]);
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    if (c >= across) continue;
+                    const int col = (half * across + c) * 32;
+                    float v[32];
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) v[j] = 0.0f;
+                    for (int b = 0; b < across; ++b) add_columns(b * side + col, v);
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) {
+                        v[j] = fmaf(linear, held[32 * c + j], factor * v[j]);
+                        if (row == col + j && row < n) v[j] += diagonal;
+                    }
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) put_piece(square + ((col >> 6) * across + (row >> 6)) * kBlockBytes, row & 63, ((col & 63) >> 3) + e, v + 8 * e, s_part);
+                }
+            }
+            for (int c0 = 0; c0 < along * kBlock; c0 += chunk) {
+                const int width = min(chunk, along * kBlock - c0);
+                products([&] {
+                    for (int b = 0; b < across; ++b)
+                        for (int w0 = 0; w0 < width; w0 += 256) {
+                            const unsigned at = x_at + (((c0 + w0) >> 6) * across + b) * kBlockBytes;
+                            three(tmem + b * chunk + w0, s_at + b * across * kBlockBytes, s_part, describe_apart(at, across * kBlockBytes), x_part, 2048 >> 4,
+                                  instruction_of(min(256, width - w0), 1), false);
+                        }
+                });
+                // (the products have been made: their operand's place is free)
+                if (used) {
+                    const float factor = last ? power(-poly.x[k] - poly.poly[k]) : power(poly.x[k + 1] - poly.x[k] - poly.poly[k]);
+                    for (int w0 = half * (width / 2); w0 < (half + 1) * (width / 2); w0 += 32) {
+                        float v[32];
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) v[j] = 0.0f;
+                        for (int b = 0; b < across; ++b) add_columns(b * chunk + w0, v);
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) v[j] *= factor;
+                        const int col = c0 + w0;
+                        if (!last) {
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) put_piece(x + ((col >> 6) * across + (row >> 6)) * kBlockBytes, row & 63, ((col & 63) >> 3) + e, v + 8 * e, x_part);
+                        } else if (row < n) {
+                            float* to = value_at(col >> 6, row);
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) to[((col & 63) + j) ^ (row & 31)] = v[j];
+                        }
+                    }
+                }
+            }
+            if (last) {
+                __syncthreads();
+                for (int i0 = threadIdx.x; i0 < size; i0 += kBatch * kSoloThreads) {
+                    float v[kBatch];
+#pragma unroll
+                    for (int j = 0; j < kBatch; ++j) v[j] = i0 + j * kSoloThreads < size ? t.param[i0 + j * kSoloThreads] : 0.0f;
+#pragma unroll
+                    for (int j = 0; j < kBatch; ++j) {
+                        const int i = i0 + j * kSoloThreads;
+                        if (i >= size) break;
+                        const int at_row = i / t.cols, at_col = i - at_row * t.cols;
+                        const int a = tall ? at_col : at_row, b = tall ? at_row : at_col;
+                        const float y = value_at(b >> 6, a)[(b & 63) ^ (a & 31)];
+                        t.param[i] = v[j] * keep - move * y;
+                    }
+                }
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 0) {
+        tc_fence_after();
+        tmem_dealloc(tmem, kSoloColumns);
+    }
+    if (threadIdx.x == 0 && fail_flag && status) atomicExch(status, 1);
+    if (!alone) {
+        asm volatile("griddepcontrol.wait;" ::: "memory");
+        asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    }
+}
+
 int check_matrices(const b2_muon_matrix* list, int count) {
     B2_REQUIRE(count >= 0 && (count == 0 || list), "bad list of matrices");
     for (int i = 0; i < count; ++i) {
@@ -661,7 +917,12 @@ Layout layout_of(const b2_muon_matrix* list, int count) {
     // long sums first: the last items of a phase are short ones
     std::stable_sort(found.matrices.begin(), found.matrices.end(),
                      [](const Matrix& a, const Matrix& b) { return std::max(a.row_blocks, a.col_blocks) > std::max(b.row_blocks, b.col_blocks); });
-    for (int index = 0; index < (int)found.matrices.size(); ++index) {
+    const auto rest = std::stable_partition(found.matrices.begin(), found.matrices.end(), [](const Matrix& t) {
+        return (long long)t.row_blocks * t.col_blocks + (long long)t.n_blocks * t.n_blocks > kSoloBlocks;
+    });
+    found.solos = found.matrices.end() - rest;
+    const size_t shared = rest - found.matrices.begin();     // matrices that share the launch for all
+    for (int index = 0; index < (int)shared; ++index) {
         Matrix& t = found.matrices[index];
         const long long size = (long long)t.rows * t.cols, blocks = (long long)t.row_blocks * t.col_blocks;
         t.x[0] = take(blocks);
@@ -675,9 +936,9 @@ Layout layout_of(const b2_muon_matrix* list, int count) {
         for (int k = 0; k < blocks; ++k) found.blocks.push_back({index, k});
     }
     // Groups of matrices whose phases keep the machine busy while another's end: some three tiles to an SM
-    for (size_t from = 0; from < found.matrices.size();) {
+    for (size_t from = 0; from < shared;) {
         size_t to = from;
-        for (long long tiles = 0; to < found.matrices.size() && tiles < 3 * b2::kSms; ++to) {
+        for (long long tiles = 0; to < shared && tiles < 3 * b2::kSms; ++to) {
             const Matrix& t = found.matrices[to];
             tiles_of(t.n_blocks, t.n_blocks, true, 4, [&](int, int, int) { ++tiles; });
         }
@@ -725,17 +986,29 @@ int sizes_of(const Layout& l, b2_muon_sizes* s) {
     s->chunks = (int64_t)l.chunks.size();
     s->items = (int64_t)l.items.size();
     s->blocks = (int64_t)l.blocks.size();
+    s->solos = (int64_t)l.solos;
     s->scratch_bytes = counter_bytes(*s) + (size_t)l.bytes + 1024;
     return B2_OK;
 }
 
-// The largest values that |p| and |p(s) / s| have over [0, top]
+// The largest values that |p| and |p(s) / s| have over [0, top]: at the ends, where p' = a + 3 b t + 5 c t^2 is zero, t = s^2, and where
+// a + b t + c t^2 turns
 void reach(double a, double b, double c, double top, double* of_p, double* of_factor) {
+    double at[5] = {0.0, top * top, 0.0, 0.0, 0.0};
+    if (c != 0.0) {
+        const double inside = 9.0 * b * b - 20.0 * a * c, root = inside > 0.0 ? std::sqrt(inside) : 0.0;
+        at[2] = (-3.0 * b + root) / (10.0 * c);
+        at[3] = (-3.0 * b - root) / (10.0 * c);
+        at[4] = -b / (2.0 * c);
+    } else if (b != 0.0) {
+        at[2] = -a / (3.0 * b);
+    }
     *of_p = *of_factor = 0.0;
-    for (int i = 0; i <= 4096; ++i) {
-        const double s = top * i / 4096, t = s * s, f = std::fabs(a + (b + c * t) * t);
+    for (double t : at) {
+        if (!(t >= 0.0 && t <= top * top)) continue;
+        const double f = std::fabs(a + (b + c * t) * t);
         *of_factor = std::max(*of_factor, f);
-        *of_p = std::max(*of_p, s * f);
+        *of_p = std::max(*of_p, std::sqrt(t) * f);
     }
 }
 // The power of two that takes values up to `most` next to fp16's largest, 65504; a value that is no larger than its operand's largest
@@ -789,7 +1062,8 @@ extern "C" int b2_muon_plan_sizes(const b2_muon_matrix* list, int32_t count, b2_
 
 extern "C" int b2_muon_launches(const b2_muon_sizes* s, int32_t* launches) {
     B2_REQUIRE(s && launches, "missing argument");
-    *launches = s->items == 0 ? 1 : 3;
+    *launches = (s->items > 0 ? 3 : 0) + (s->solos > 0 ? 1 : 0);
+    if (*launches == 0) *launches = 1;               // (the number of the step)
     return B2_OK;
 }
 
@@ -814,7 +1088,7 @@ extern "C" int b2_muon_plan(const b2_muon_matrix* list, int32_t count, void* pla
         B2_CUDA(cudaStreamIsCapturing((cudaStream_t)stream, &capturing));
         B2_REQUIRE(capturing == cudaStreamCaptureStatusNone, "a plan is made before its stream is captured");
         std::vector<char> host(l.plan_bytes(), 0);
-        *reinterpret_cast<Header*>(host.data()) = {s.matrices, s.chunks, s.items, s.blocks, (long long)l.groups.size()};
+        *reinterpret_cast<Header*>(host.data()) = {s.matrices, s.chunks, s.items, s.blocks, s.solos, (long long)l.groups.size()};
         char* to = host.data() + kHeader;
         const auto put = [&](const void* from, size_t bytes) {
             std::copy((const char*)from, (const char*)from + bytes, to);
@@ -836,7 +1110,7 @@ extern "C" int b2_muon_plan(const b2_muon_matrix* list, int32_t count, void* pla
 
 extern "C" int b2_muon_step(void* plan, const b2_muon_sizes* s, const b2_muon_hyper* h, const float* lr, const float* grad_scale, float* step, void* scratch,
                             size_t scratch_bytes, int32_t* status, void* stream) {
-    B2_REQUIRE(plan && s && h && s->matrices >= 0 && s->chunks >= 0 && s->items >= 0 && s->blocks >= 0, "bad argument");
+    B2_REQUIRE(plan && s && h && s->matrices >= 0 && s->chunks >= 0 && s->items >= 0 && s->blocks >= 0 && s->solos >= 0 && s->solos <= s->matrices, "bad argument");
     B2_REQUIRE(scratch && scratch_bytes >= s->scratch_bytes, "the step needs %zu bytes of scratch, got %zu", s->scratch_bytes, scratch_bytes);
     B2_REQUIRE(std::isfinite(h->lr) && h->momentum >= 0.0 && h->momentum < 1.0 && std::isfinite(h->eps) && h->eps >= 0.0 && std::isfinite(h->weight_decay),
                "bad rates: lr %g, momentum %g, eps %g, weight decay %g", h->lr, h->momentum, h->eps, h->weight_decay);
@@ -881,13 +1155,20 @@ extern "C" int b2_muon_step(void* plan, const b2_muon_sizes* s, const b2_muon_hy
     room.failed = room.next + 1;
     room.done = room.next + 4;
     room.planes = at + counter_bytes(*s);
-    const Told told = {s->matrices, s->chunks, s->items, s->blocks};
+    const Told told = {s->matrices, s->chunks, s->items, s->blocks, s->solos};
     const auto grid = [](long long work, long long most) { return dim3((unsigned)(work < 1 ? 1 : work < most ? work : most)); };
-    B2_CUDA((b2::launch_after(muon_mean_kernel, grid(s->chunks, b2::kSms * 8), kMeanThreads, 0, st, base, told, r, grad_scale, step, room)));
-    if (s->items == 0) return B2_OK;
-    B2_CUDA((b2::launch_after(muon_parts_kernel, grid(s->blocks, b2::kSms * 8), kMeanThreads, 0, st, base, told, r, grad_scale, (int)p.x[0], room)));
-    static std::atomic<unsigned long long> done{0};
-    B2_CHECK(b2::allow_shared((const void*)muon_product_kernel, kProductShared, &done));
-    B2_CUDA((b2::launch_after(muon_product_kernel, grid(s->items, b2::kSms), kProductThreads, (size_t)kProductShared, st, base, told, r, p, lr, room, status)));
+    static std::atomic<unsigned long long> done{0}, done_solo{0};
+    if (s->items > 0 || s->solos == 0)
+        B2_CUDA((b2::launch_after(muon_mean_kernel, grid(s->chunks, b2::kSms * 8), kMeanThreads, 0, st, base, told, r, grad_scale, step, room)));
+    if (s->items > 0) {
+        B2_CUDA((b2::launch_after(muon_parts_kernel, grid(s->blocks, b2::kSms * 8), kMeanThreads, 0, st, base, told, r, grad_scale, (int)p.x[0], room)));
+        B2_CHECK(b2::allow_shared((const void*)muon_product_kernel, kProductShared, &done));
+        B2_CUDA((b2::launch_after(muon_product_kernel, grid(s->items, b2::kSms), kProductThreads, (size_t)kProductShared, st, base, told, r, p, lr, room, status)));
+    }
+    if (s->solos > 0) {
+        B2_CHECK(b2::allow_shared((const void*)muon_solo_kernel, kSoloShared, &done_solo));
+        B2_CUDA((b2::launch_after(muon_solo_kernel, grid(s->solos, 1 << 30), kSoloThreads, (size_t)kSoloShared, st, base, told, r, p, lr, grad_scale, step,
+                                  (int)(s->items == 0), status)));
+    }
     return B2_OK;
 }

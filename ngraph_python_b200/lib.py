@@ -172,7 +172,7 @@ class MuonHyper(C.Structure):
 
 class MuonSizes(C.Structure):
     _fields_ = [("plan_bytes", C.c_size_t), ("scratch_bytes", C.c_size_t), ("matrices", C.c_int64), ("chunks", C.c_int64),
-                ("items", C.c_int64), ("blocks", C.c_int64)]
+                ("items", C.c_int64), ("blocks", C.c_int64), ("solos", C.c_int64)]
 
 
 class CallArg(C.Structure):

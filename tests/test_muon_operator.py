@@ -84,7 +84,7 @@ def _check(got, d, scale=1.0, decay=1.0, grad_scale=1.0, mu=0.95, nesterov=True,
 
 
 SHAPES = [(1, 1), (1, 640), (129, 1), (2, 3), (64, 64), (63, 65), (128, 128), (77, 77), (65, 300), (300, 65), (301, 1001), (1001, 301), (130, 127), (16, 4096),
-          (640, 192), (257, 513), (513, 257), (192, 640)]
+          (640, 192), (257, 513), (513, 257), (192, 640), (64, 512), (64, 768), (64, 769), (768, 33), (520, 64), (65, 256), (128, 256), (128, 257), (256, 100), (2, 700)]
 
 
 @pytest.mark.gpu
