@@ -128,6 +128,7 @@ struct Room {
     char* planes;
 };
 
+template <int THREADS>
 __device__ __forceinline__ double cta_sum(double q, double* words) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) q += __shfl_xor_sync(0xffffffffu, q, o);
@@ -135,7 +136,7 @@ __device__ __forceinline__ double cta_sum(double q, double* words) {
     if ((threadIdx.x & 31) == 0) words[threadIdx.x >> 5] = q;
     __syncthreads();
     q = 0.0;
-    for (int w = 0; w < kMeanThreads / 32; ++w) q += words[w];
+    for (int w = 0; w < THREADS / 32; ++w) q += words[w];
     return q;
 }
 
@@ -172,7 +173,7 @@ muon_mean_kernel(const void* plan, const Told told, const Rates r, const float* 
                 q = fma((double)u, (double)u, q);
             }
         }
-        q = cta_sum(q, words);
+        q = cta_sum<kMeanThreads>(q, words);
         if (threadIdx.x == 0) room.sums[k] = q;
     }
 }
@@ -221,7 +222,7 @@ muon_parts_kernel(const void* plan, const Told told, const Rates r, const float*
         const Matrix& t = matrices_of(plan)[c.matrix];
         double q = 0.0;
         for (int i = threadIdx.x; i < t.chunks; i += kMeanThreads) q += room.sums[t.first_chunk + i];
-        q = cta_sum(q, words);
+        q = cta_sum<kMeanThreads>(q, words);
         const float inverse = (float)(1.0 / (sqrt(q) + (double)r.eps)), up = power(exponent);
         const int rb = c.at / t.col_blocks, cb = c.at - rb * t.col_blocks;
         char* block = room.planes + t.x[0] + (long long)c.at * kBlockPair;
@@ -618,7 +619,7 @@ muon_product_kernel(const void* plan, const Told told, const Rates r, const Poly
 // x and A (then B in its place) stay in shared memory in the form above, sums in tensor memory, in columns of their own for every block
 // of k; a product is a few instructions between two barriers, 1.2 us where the launch for all matrices takes 8.  A matrix that has more rows
 // than columns is taken as its transpose.  x: [part][block along][block across], across the shorter side.
-constexpr int kSoloThreads = 256;
+constexpr int kSoloThreads = 512;
 constexpr int kSoloBlocks = 13;                             // of x and A in both parts
 constexpr int kSoloColumns = 512;                           // of tensor memory
 constexpr int kSoloShared = 1024 + (2 * kSoloBlocks + 1) * kBlockBytes + 512;       // (the tensor core reads 128 rows, of 64 the next block as well)
@@ -632,7 +633,7 @@ __global__ void __launch_bounds__(kSoloThreads, 1)
 muon_solo_kernel(const void* plan, const Told told, const Rates r, const Poly poly, const float* lr, const float* grad_scale, float* step, int alone, int* status) {
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-    __shared__ double words[kMeanThreads / 32];
+    __shared__ double words[kSoloThreads / 32];
     __shared__ unsigned long long bar;
     __shared__ unsigned tmem_holder;
     __shared__ int fail_flag;
@@ -659,49 +660,87 @@ muon_solo_kernel(const void* plan, const Told told, const Rates r, const Poly po
         const int x_part = across * along * kBlockBytes, s_part = across * across * kBlockBytes;
         char *x = reinterpret_cast<char*>(smem), *square = x + 2 * x_part;
         const unsigned x_at = smem_u32(x), s_at = smem_u32(square);
-        // the mean, and the sum of squares of u
-        const float s = grad_scale ? *grad_scale : 1.0f;
-        const auto u_of = [&](float mean, float grad) { return r.nesterov ? r.rest * (grad * s) + r.mu * mean : mean; };
-        const int size = t.rows * t.cols;
-        double q = 0.0;
-        constexpr int kBatch = 8;                           // values of a thread whose loads are issued together
-        for (int i0 = threadIdx.x; i0 < size; i0 += kBatch * kSoloThreads) {
-            float g[kBatch], mean[kBatch];
-#pragma unroll
-            for (int j = 0; j < kBatch; ++j) {
-                const int i = i0 + j * kSoloThreads;
-                g[j] = i < size ? t.grad[i] : 0.0f;
-                mean[j] = i < size ? t.mean[i] : 0.0f;
-            }
-#pragma unroll
-            for (int j = 0; j < kBatch; ++j) {
-                const int i = i0 + j * kSoloThreads;
-                mean[j] = r.mu * mean[j] + r.rest * (g[j] * s);
-                const float u = u_of(mean[j], g[j]);
-                if (i < size) t.mean[i] = mean[j];
-                q = fma((double)u, (double)u, q);
-            }
+        // The place of x(i, j) in fp32: a block's 64 x 64 values in the place of its two parts, 32 rows in either
+        const auto value_at = [&](int i, int j) {
+            return reinterpret_cast<float*>(x + ((j >> 6) * across + (i >> 6)) * kBlockBytes + (i & 32 ? x_part : 0)) + (i & 31) * kBlock + ((j & 63) ^ (i & 31));
+        };
+        if (n < across * kBlock || m < along * kBlock) {
+            for (int e = threadIdx.x; e < 2 * x_part / 16; e += kSoloThreads) reinterpret_cast<uint4*>(x)[e] = make_uint4(0, 0, 0, 0);
+            __syncthreads();
         }
-        q = cta_sum(q, words);
-        __syncthreads();                                    // (means of other threads are read)
+        // the mean, u, and the sum of its squares; values by fours where the tensors lie so
+        const float s = grad_scale ? *grad_scale : 1.0f;
+        const int size = t.rows * t.cols;
+        const bool vec = (((uintptr_t)t.grad | (uintptr_t)t.mean | (uintptr_t)t.param) & 15) == 0;
+        // all of a tensor's values, a run of them next to one another by a thread and BATCH runs at a time
+        const auto walk = [&](auto&& load, auto&& use) {
+            constexpr int BATCH = 4;
+            const int whole = vec ? size / 4 : 0;
+            for (int i0 = threadIdx.x; i0 < whole; i0 += BATCH * kSoloThreads) {
+                float4 v[BATCH][2];
+#pragma unroll
+                for (int k = 0; k < BATCH; ++k)
+                    if (i0 + k * kSoloThreads < whole) load(4 * (i0 + k * kSoloThreads), v[k], std::integral_constant<int, 4>());
+#pragma unroll
+                for (int k = 0; k < BATCH; ++k)
+                    if (i0 + k * kSoloThreads < whole) use(4 * (i0 + k * kSoloThreads), v[k], std::integral_constant<int, 4>());
+            }
+            for (int i0 = 4 * whole + threadIdx.x; i0 < size; i0 += 2 * BATCH * kSoloThreads) {
+                float4 v[2 * BATCH][2];
+#pragma unroll
+                for (int k = 0; k < 2 * BATCH; ++k)
+                    if (i0 + k * kSoloThreads < size) load(i0 + k * kSoloThreads, v[k], std::integral_constant<int, 1>());
+#pragma unroll
+                for (int k = 0; k < 2 * BATCH; ++k)
+                    if (i0 + k * kSoloThreads < size) use(i0 + k * kSoloThreads, v[k], std::integral_constant<int, 1>());
+            }
+        };
+        const auto get = [](const float* from, float4& v, auto count) {
+            if constexpr (decltype(count)::value == 4) v = *reinterpret_cast<const float4*>(from);
+            else v.x = *from;
+        };
+        const auto put = [](float* to, const float4& v, auto count) {
+            if constexpr (decltype(count)::value == 4) *reinterpret_cast<float4*>(to) = v;
+            else *to = v.x;
+        };
+        // visits the places of `count` values from number i on
+        const auto places = [&](int i, auto count, auto&& visit) {
+            int at_row = i / t.cols, at_col = i - at_row * t.cols;
+#pragma unroll
+            for (int j = 0; j < decltype(count)::value; ++j) {
+                visit(j, tall ? value_at(at_col, at_row) : value_at(at_row, at_col));
+                if (++at_col == t.cols) { at_col = 0; ++at_row; }
+            }
+        };
+        double q = 0.0;
+        walk([&](int i, float4* v, auto count) {
+                 get(t.grad + i, v[0], count);
+                 get(t.mean + i, v[1], count);
+             },
+             [&](int i, float4* v, auto count) {
+                 float* g = reinterpret_cast<float*>(&v[0]);
+                 float* mean = reinterpret_cast<float*>(&v[1]);
+                 places(i, count, [&](int j, float* place) {
+                     mean[j] = r.mu * mean[j] + r.rest * (g[j] * s);
+                     const float u = r.nesterov ? r.rest * (g[j] * s) + r.mu * mean[j] : mean[j];
+                     *place = u;
+                     q = fma((double)u, (double)u, q);
+                 });
+                 put(t.mean + i, v[1], count);
+             });
+        q = cta_sum<kSoloThreads>(q, words);
         const float inverse = (float)(1.0 / (sqrt(q) + (double)r.eps)), up = power(poly.x[0]);
-        for (int e = threadIdx.x; e < across * kBlock * along * 8; e += kSoloThreads) {
-            // neighbours in memory to neighbouring threads
-            const int i = tall ? e % (across * kBlock) : e / (along * 8), piece = tall ? e / (across * kBlock) : e % (along * 8);
+        // x in parts, block by block: a thread to eight values next to one another
+        for (int b = 0; b < across * along; ++b) {
+            const int in_row = threadIdx.x >> 3, piece = threadIdx.x & 7, i = (b % across) * kBlock + in_row, j0 = (b / across) * kBlock + piece * 8;
             float v[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const int at = piece * 8 + j;
-                v[j] = 0.0f;
-                if (i < n && at < m) {
-                    const int place = tall ? at * t.cols + i : i * t.cols + at;
-                    v[j] = u_of(t.mean[place], t.grad[place]) * inverse * up;
-                }
-            }
-            put_piece(x + ((piece >> 3) * across + (i >> 6)) * kBlockBytes, i & 63, piece & 7, v, x_part);
+            for (int j = 0; j < 8; ++j) v[j] = *value_at(i, j0 + j) * inverse * up;
+            __syncthreads();
+            put_piece(x + b * kBlockBytes, in_row, piece, v, x_part);
         }
 
-        const int quarter = warp & 3, half = warp >> 2, row = quarter * 32 + lane;
+        const int quarter = warp & 3, turn = warp >> 2, row = quarter * 32 + lane;     // (sixteen columns by turns of four warps)
         const bool used = row < across * kBlock;            // (of a warp all or none)
         const unsigned lanes = tmem + ((unsigned)(quarter * 32) << 16);
         unsigned parity = 0;
@@ -728,25 +767,34 @@ muon_solo_kernel(const void* plan, const Told told, const Rates r, const Poly po
             for (int k = 0; k < 4; ++k) multiply_f16(sum, p_hi + 2 * k, q_hi + k * q_step, instruction, 1);
         };
         const auto instruction_of = [](int width, unsigned q_major) { return (1u << 4) | (q_major << 16) | ((unsigned)(width >> 3) << 17) | ((128u >> 4) << 24); };
-        const auto add_columns = [&](unsigned from, float* v) {             // 32 columns of sums
-            unsigned w[32];
-            tmem_ld16(lanes + from, w);
-            tmem_ld16(lanes + from + 16, w + 16);
-            tmem_ld_wait();
+        // sixteen columns of `count` sums that lie `apart`, two sums at a time
+        const auto columns = [&](unsigned from, int count, int apart, float* v) {
+            unsigned w[2][16];
 #pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] += __uint_as_float(w[j]);
+            for (int j = 0; j < 16; ++j) v[j] = 0.0f;
+            for (int b = 0; b < count; b += 2) {
+                tmem_ld16(lanes + from + b * apart, w[0]);
+                if (b + 1 < count) tmem_ld16(lanes + from + (b + 1) * apart, w[1]);
+                tmem_ld_wait();
+#pragma unroll
+                for (int j = 0; j < 16; ++j) v[j] += __uint_as_float(w[0][j]);
+                if (b + 1 < count)
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) v[j] += __uint_as_float(w[1][j]);
+            }
+        };
+        const auto put_columns = [&](char* first, int col, const float* v, int part) {
+            char* block = first + ((col >> 6) * across + (row >> 6)) * kBlockBytes;
+            put_piece(block, row & 63, (col & 63) >> 3, v, part);
+            put_piece(block, row & 63, ((col & 63) >> 3) + 1, v + 8, part);
         };
         const int side = across * kBlock, per_sum = (along * side + kSoloColumns - 1) / kSoloColumns, sums = (along + per_sum - 1) / per_sum;
         const int chunk = kSoloColumns / across;            // columns of x that are multiplied at a time
-        // the last x in fp32, a block in the place of its two parts: 32 rows in either
-        const auto value_at = [&](int block, int row_of) {
-            return reinterpret_cast<float*>(x + (block * across + (row_of >> 6)) * kBlockBytes + (row_of & 32 ? x_part : 0)) + (row_of & 31) * kBlock;
-        };
         const double rate = lr ? (double)*lr : r.lr;
         const float keep = (float)(1.0 - rate * r.wd * (double)t.decay), move = (float)(rate * (double)t.scale);
         for (int k = 0; k < poly.steps; ++k) {
             const bool last = k == poly.steps - 1;
-            float held[64];                                 // this thread's part of A
+            float held[32];                                 // this thread's part of A
             products([&] {
                 for (int b = 0; b < along; ++b) {
                     const unsigned at = x_at + b * across * kBlockBytes;
@@ -758,15 +806,12 @@ muon_solo_kernel(const void* plan, const Told told, const Rates r, const Poly po
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
                     if (c >= across) continue;
-                    const int col = (half * across + c) * 32;
-                    float* v = held + 32 * c;
+                    const int col = (4 * c + turn) * 16;
+                    float* v = held + 16 * c;
+                    columns(col, sums, side, v);
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) v[j] = 0.0f;
-                    for (int b = 0; b < sums; ++b) add_columns(b * side + col, v);
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) v[j] *= factor;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) put_piece(square + ((col >> 6) * across + (row >> 6)) * kBlockBytes, row & 63, ((col & 63) >> 3) + e, v + 8 * e, s_part);
+                    for (int j = 0; j < 16; ++j) v[j] *= factor;
+                    put_columns(square, col, v, s_part);
                 }
             }
             products([&] {
@@ -781,18 +826,15 @@ muon_solo_kernel(const void* plan, const Told told, const Rates r, const Poly po
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
                     if (c >= across) continue;
-                    const int col = (half * across + c) * 32;
-                    float v[32];
+                    const int col = (4 * c + turn) * 16;
+                    float v[16];
+                    columns(col, across, side, v);
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) v[j] = 0.0f;
-                    for (int b = 0; b < across; ++b) add_columns(b * side + col, v);
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) {
-                        v[j] = fmaf(linear, held[32 * c + j], factor * v[j]);
+                    for (int j = 0; j < 16; ++j) {
+                        v[j] = fmaf(linear, held[16 * c + j], factor * v[j]);
                         if (row == col + j && row < n) v[j] += diagonal;
                     }
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) put_piece(square + ((col >> 6) * across + (row >> 6)) * kBlockBytes, row & 63, ((col & 63) >> 3) + e, v + 8 * e, s_part);
+                    put_columns(square, col, v, s_part);
                 }
             }
             for (int c0 = 0; c0 < along * kBlock; c0 += chunk) {
@@ -808,41 +850,30 @@ muon_solo_kernel(const void* plan, const Told told, const Rates r, const Poly po
                 // (the products have been made: their operand's place is free)
                 if (used) {
                     const float factor = last ? power(-poly.x[k] - poly.poly[k]) : power(poly.x[k + 1] - poly.x[k] - poly.poly[k]);
-                    for (int w0 = half * (width / 2); w0 < (half + 1) * (width / 2); w0 += 32) {
-                        float v[32];
+#pragma unroll 2
+                    for (int w0 = turn * 16; w0 < width; w0 += 64) {
+                        float v[16];
+                        columns(w0, across, chunk, v);
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) v[j] = 0.0f;
-                        for (int b = 0; b < across; ++b) add_columns(b * chunk + w0, v);
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) v[j] *= factor;
+                        for (int j = 0; j < 16; ++j) v[j] *= factor;
                         const int col = c0 + w0;
                         if (!last) {
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) put_piece(x + ((col >> 6) * across + (row >> 6)) * kBlockBytes, row & 63, ((col & 63) >> 3) + e, v + 8 * e, x_part);
+                            put_columns(x, col, v, x_part);
                         } else if (row < n) {
-                            float* to = value_at(col >> 6, row);
 #pragma unroll
-                            for (int j = 0; j < 32; ++j) to[((col & 63) + j) ^ (row & 31)] = v[j];
+                            for (int j = 0; j < 16; ++j) *value_at(row, col + j) = v[j];
                         }
                     }
                 }
             }
             if (last) {
                 __syncthreads();
-                for (int i0 = threadIdx.x; i0 < size; i0 += kBatch * kSoloThreads) {
-                    float v[kBatch];
-#pragma unroll
-                    for (int j = 0; j < kBatch; ++j) v[j] = i0 + j * kSoloThreads < size ? t.param[i0 + j * kSoloThreads] : 0.0f;
-#pragma unroll
-                    for (int j = 0; j < kBatch; ++j) {
-                        const int i = i0 + j * kSoloThreads;
-                        if (i >= size) break;
-                        const int at_row = i / t.cols, at_col = i - at_row * t.cols;
-                        const int a = tall ? at_col : at_row, b = tall ? at_row : at_col;
-                        const float y = value_at(b >> 6, a)[(b & 63) ^ (a & 31)];
-                        t.param[i] = v[j] * keep - move * y;
-                    }
-                }
+                walk([&](int i, float4* v, auto count) { get(t.param + i, v[0], count); },
+                     [&](int i, float4* v, auto count) {
+                         float* p = reinterpret_cast<float*>(&v[0]);
+                         places(i, count, [&](int j, float* place) { p[j] = p[j] * keep - move * *place; });
+                         put(t.param + i, v[0], count);
+                     });
             }
         }
     }
