@@ -50,7 +50,7 @@ struct Matrix {
     float* param;
     const float* grad;
     float* mean;
-    long long x[2], square, poly;            // two turns of x [row blocks][column blocks], A and B [n blocks][n blocks]
+    long long x[2], square, poly, held;      // two turns of x [row blocks][column blocks], A and B [n blocks][n blocks], A in fp32
     int rows, cols, row_blocks, col_blocks, n_blocks, tall;
     int items[3];                            // of a step, by phase
     int first_chunk, chunks;
@@ -197,19 +197,6 @@ __device__ __forceinline__ void put_piece(char* block, int row, int piece, const
     *reinterpret_cast<uint4*>(at) = hi;
     *reinterpret_cast<uint4*>(at + to_lo) = lo;
 }
-__device__ __forceinline__ float2 halves(unsigned w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
-__device__ __forceinline__ void get_piece(const char* block, int row, int piece, float* v) {
-    const char* at = block + row * 128 + ((piece ^ (row & 7)) << 4);
-    const uint4 hi = __ldcg(reinterpret_cast<const uint4*>(at)), lo = __ldcg(reinterpret_cast<const uint4*>(at + kBlockBytes));
-    const unsigned h[4] = {hi.x, hi.y, hi.z, hi.w}, l[4] = {lo.x, lo.y, lo.z, lo.w};
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        const float2 a = halves(h[k]), b = halves(l[k]);
-        v[2 * k] = a.x + b.x;
-        v[2 * k + 1] = a.y + b.y;
-    }
-}
-
 // x of the first step, a block at a time
 __global__ void __launch_bounds__(kMeanThreads)
 muon_parts_kernel(const void* plan, const Told told, const Rates r, const float* grad_scale, int exponent, const Room room) {
@@ -250,10 +237,12 @@ muon_parts_kernel(const void* plan, const Told told, const Rates r, const float*
 constexpr int kUnit = 32 << 10, kUnits = 6;                 // the ring: both parts of 128 rows of P, of Q up to 128, or one part of more
 constexpr int kQueue = 4;
 constexpr int kEpilogueWarps = 8;
-constexpr int kProductThreads = 64 + 32 * kEpilogueWarps;
-constexpr int kStagePitch = 33;
-constexpr int kStage = 32 * kStagePitch * 4;                // of a warp of the epilogue: 32 x 32 values
-constexpr int kProductShared = 1024 + kUnits * kUnit + kEpilogueWarps * kStage + 512;
+constexpr int kProductThreads = 128 + 32 * kEpilogueWarps;  // (a warp group for the two that copy and multiply)
+// Registers of a thread: 168 at the start, of which the first group gives so many to the epilogue's two, 56 + 2 x 224 = 3 x 168
+constexpr int kFewRegisters = 56, kManyRegisters = 224;
+static_assert(kFewRegisters + 2 * kManyRegisters <= 3 * 168, "what the block was launched with");
+constexpr int kPairs = kEpilogueWarps / 2;                  // two warps of the epilogue have the rows of a block, and room for one part of it
+constexpr int kProductShared = 1024 + kUnits * kUnit + kPairs * kBlockBytes + 512;
 static_assert(kProductShared <= 227 << 10, "shared memory of a CTA");
 // Blocks of k that are added in tensor memory, whose sums lose what they add: 640 x 1920 is 2.8e-6 off in the 2-norm with one
 // (numpy's fp32 2.2e-6), 6.4e-6 with two, 1.2e-5 with four, for 3.92, 3.77 and 3.60 ms of 48 matrices.  The small products
@@ -307,8 +296,8 @@ __global__ void __launch_bounds__(kProductThreads, 1)
 muon_product_kernel(const void* plan, const Told told, const Rates r, const Poly poly, const float* lr, const Room room, int* status) {
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-    float* stages = reinterpret_cast<float*>(smem + kUnits * kUnit);
-    unsigned long long* full_bar = reinterpret_cast<unsigned long long*>(smem + kUnits * kUnit + kEpilogueWarps * kStage);
+    char* rooms = reinterpret_cast<char*>(smem + kUnits * kUnit);
+    unsigned long long* full_bar = reinterpret_cast<unsigned long long*>(smem + kUnits * kUnit + kPairs * kBlockBytes);
     unsigned long long* empty_bar = full_bar + kUnits;
     unsigned long long* sum_full = empty_bar + kUnits;          // [2]
     unsigned long long* sum_empty = sum_full + 2;               // [2]
@@ -337,35 +326,41 @@ muon_product_kernel(const void* plan, const Told told, const Rates r, const Poly
     const bool mine = fits(plan, told);                         // (else no item is taken)
     const Matrix* matrices = matrices_of(plan);
 
+    if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFewRegisters));
     if (warp == 0) {
-        if (elect_one()) {
-            int s = 0, q = 0;
-            unsigned parity = 1, queue_parity = 1;
-            bool ok = true;
-            long long group = 0;
-            const long long total = mine ? told.items * poly.steps : 0;
-            for (;;) {
-                // the next item
-                Work w = {};
-                w.phase = -1;
-                const long long number = ok && total ? (long long)atomicAdd(room.next, 1u) : total;
-                if (number < total && !*reinterpret_cast<volatile unsigned*>(room.failed)) {
-                    const Group* g = groups_of(plan) + group;
-                    while (number >= poly.steps * (g->first + g->count)) { ++g; ++group; }
-                    const long long in = number - poly.steps * g->first;
-                    w.step = (int)(in / g->count);
-                    const Item item = items_of(plan)[g->first + (in - w.step * g->count)];
-                    const Matrix& t = matrices[item.matrix];
-                    w.matrix = item.matrix;
-                    w.phase = item.phase;
-                    w.i = item.i;
-                    w.j = item.j;
-                    w.width = item.width;
-                    w.k_blocks = item.phase == GRAM ? (t.tall ? t.row_blocks : t.col_blocks) : t.n_blocks;
-                    // what it reads has been stored
-                    const int before = w.step * (t.items[0] + t.items[1] + t.items[2]) + (item.phase > GRAM ? t.items[0] : 0) + (item.phase > POLY ? t.items[1] : 0);
-                    const unsigned need = (unsigned)before * kEpilogueWarps;
-                    bool there = false;
+        // A lane to each copy of a block of k, with its addresses worked out once an item: one thread for all of them took 150 cycles a
+        // copy, 1900 a block of k of 256 columns, of which the products take 1536.
+        int s = 0, q = 0;
+        unsigned parity = 1, queue_parity = 1;
+        bool ok = true;
+        long long group = 0;
+        const long long total = mine ? told.items * poly.steps : 0;
+        for (;;) {
+            // the next item
+            Work w = {};
+            w.phase = -1;
+            long long number = total;
+            if (lane == 0 && ok && total && !*reinterpret_cast<volatile unsigned*>(room.failed)) number = (long long)atomicAdd(room.next, 1u);
+            number = __shfl_sync(0xffffffffu, number, 0);
+            if (number < total) {
+                const Group* g = groups_of(plan) + group;
+                while (number >= poly.steps * (g->first + g->count)) { ++g; ++group; }
+                const long long in = number - poly.steps * g->first;
+                w.step = (int)(in / g->count);
+                const Item item = items_of(plan)[g->first + (in - w.step * g->count)];
+                const Matrix& t = matrices[item.matrix];
+                w.matrix = item.matrix;
+                w.phase = item.phase;
+                w.i = item.i;
+                w.j = item.j;
+                w.width = item.width;
+                w.k_blocks = item.phase == GRAM ? (t.tall ? t.row_blocks : t.col_blocks) : t.n_blocks;
+                // what it reads has been stored
+                const int before = w.step * (t.items[0] + t.items[1] + t.items[2]) + (item.phase > GRAM ? t.items[0] : 0) + (item.phase > POLY ? t.items[1] : 0);
+                const unsigned need = (unsigned)before * kEpilogueWarps;
+                bool there = false;
+                if (lane == 0)
                     for (int i = 0; i < kDependencyPolls && !there; ++i) {
                         there = (int)(load_acquire(room.done + item.matrix) - need) >= 0;
                         if (!there) {
@@ -373,52 +368,57 @@ muon_product_kernel(const void* plan, const Told told, const Rates r, const Poly
                             __nanosleep(40);
                         }
                     }
-                    asm volatile("fence.proxy.async;" ::: "memory");
-                    if (!there) {
-                        atomicExch(fail_flag, 1);
-                        ok = false;
-                        w.phase = -1;
-                    }
+                there = __shfl_sync(0xffffffffu, (int)there, 0) != 0;
+                asm volatile("fence.proxy.async;" ::: "memory");
+                if (!there) {
+                    if (lane == 0) atomicExch(fail_flag, 1);
+                    ok = false;
+                    w.phase = -1;
                 }
-                if (!mbar_wait(&queue_empty[q], queue_parity)) { atomicExch(fail_flag, 1); break; }
+            }
+            if (!__all_sync(0xffffffffu, mbar_wait(&queue_empty[q], queue_parity))) {
+                if (lane == 0) atomicExch(fail_flag, 1);
+                ok = false;
+                break;
+            }
+            if (lane == 0) {
                 queue[q] = w;
                 mbar_arrive(&queue_full[q]);
-                if (++q == kQueue) { q = 0; queue_parity ^= 1u; }
-                if (w.phase < 0) break;
-                const Matrix& t = matrices[w.matrix];
-                const Operand P = operand_of(t, room.planes, w.phase, w.step & 1, false), Q = operand_of(t, room.planes, w.phase, w.step & 1, true);
-                const long long p0 = (long long)(2 * w.i) * P.mn, p1 = (long long)min(2 * w.i + 1, P.last) * P.mn;
-                auto unit = [&](unsigned bytes) {
-                    if (!mbar_wait(&empty_bar[s], parity)) { atomicExch(fail_flag, 1); ok = false; return false; }
-                    mbar_expect_tx(&full_bar[s], bytes);
-                    return true;
-                };
-                auto next = [&] { if (++s == kUnits) { s = 0; parity ^= 1u; } };
-                for (int kb = 0; kb < w.k_blocks && ok; ++kb) {
-                    const long long k = (long long)kb * P.k, l = (long long)kb * Q.k;
-                    if (!unit(4 * kBlockBytes)) break;
-                    unsigned to = smem_u32(smem + s * kUnit);
-                    for (int part = 0; part < 2; ++part) {
-                        copy_block(to + part * 2 * kBlockBytes, P.base + (p0 + k) * kBlockPair + part * kBlockBytes, kBlockBytes, &full_bar[s]);
-                        copy_block(to + part * 2 * kBlockBytes + kBlockBytes, P.base + (p1 + k) * kBlockPair + part * kBlockBytes, kBlockBytes, &full_bar[s]);
+            }
+            if (++q == kQueue) { q = 0; queue_parity ^= 1u; }
+            if (w.phase < 0) break;
+            const Matrix& t = matrices[w.matrix];
+            const Operand P = operand_of(t, room.planes, w.phase, w.step & 1, false), Q = operand_of(t, room.planes, w.phase, w.step & 1, true);
+            // lanes 0 to 3: P, (part, block of rows); then Q, (part, block of columns), the lo part first.  Parts of Q in one unit up to 128
+            // columns, in two beyond
+            const bool both = w.width <= 2, of_p = lane < 4;
+            const int turn = of_p ? lane >> 1 : (lane - 4) / w.width, place = of_p ? lane & 1 : (lane - 4) % w.width;
+            const int my_unit = of_p ? 0 : lane >= 4 + 2 * w.width ? -1 : both ? 1 : 1 + turn;
+            const unsigned offset = (of_p ? turn * 2 + place : both ? turn * w.width + place : place) * kBlockBytes;
+            const long long row = of_p ? (long long)min(2 * w.i + place, P.last) * P.mn : (long long)(w.j + place) * Q.mn;
+            const char* from = (of_p ? P.base : Q.base) + row * kBlockPair + (of_p ? turn : turn ^ 1) * kBlockBytes;
+            const long long along = (of_p ? P.k : Q.k) * (long long)kBlockPair;
+            const int units = both ? 2 : 3;
+            for (int kb = 0; kb < w.k_blocks && ok; ++kb) {
+                for (int u = 0; u < units; ++u) {
+                    ok = __all_sync(0xffffffffu, mbar_wait(&empty_bar[s], parity));
+                    if (!ok) {
+                        if (lane == 0) atomicExch(fail_flag, 1);
+                        break;
                     }
-                    next();
-                    const bool both = w.width <= 2;             // parts of Q in one unit
-                    for (int part = 0; part < 2; ++part) {
-                        if (part == 0 || !both)
-                            if (!unit((both ? 2 : 1) * w.width * kBlockBytes)) break;
-                        to = smem_u32(smem + s * kUnit) + (both ? part * w.width * kBlockBytes : 0);
-                        for (int n = 0; n < w.width; ++n)
-                            copy_block(to + n * kBlockBytes, Q.base + ((long long)(w.j + n) * Q.mn + l) * kBlockPair + (part ^ 1) * kBlockBytes, kBlockBytes, &full_bar[s]);
-                        if (part == 1 || !both) next();
-                    }
+                    if (lane == 0) mbar_expect_tx(&full_bar[s], (u == 0 ? 4 : both ? 2 * w.width : w.width) * kBlockBytes);
+                    __syncwarp();
+                    if (my_unit == u) copy_block(smem_u32(smem + s * kUnit) + offset, from, kBlockBytes, &full_bar[s]);
+                    if (++s == kUnits) { s = 0; parity ^= 1u; }
                 }
+                from += along;
             }
-            // copies in flight have landed, and have been read, before the CTA may end
-            for (int i = 0; i < kUnits && ok; ++i) {
-                if (!mbar_wait(&empty_bar[s], parity)) { atomicExch(fail_flag, 1); ok = false; }
-                if (++s == kUnits) { s = 0; parity ^= 1u; }
-            }
+        }
+        // copies in flight have landed, and have been read, before the CTA may end
+        for (int i = 0; i < kUnits && ok; ++i) {
+            ok = __all_sync(0xffffffffu, mbar_wait(&empty_bar[s], parity));
+            if (!ok && lane == 0) atomicExch(fail_flag, 1);
+            if (++s == kUnits) { s = 0; parity ^= 1u; }
         }
     } else if (warp == 1) {
         if (elect_one()) {
@@ -483,14 +483,33 @@ muon_product_kernel(const void* plan, const Told told, const Rates r, const Poly
                 }
             }
         }
+    }
     } else {
-        // the epilogue: a quarter of the lanes (32 rows) and half of the columns to a warp
-        const int quarter = warp & 3, half = (warp - 2) >> 2;
-        float* stage = stages + (warp - 2) * (kStage / 4);
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kManyRegisters));
+        // The epilogue: a quarter of the lanes (32 rows) to a warp, and every other block of columns.  Two warps have the rows of a block;
+        // its parts go to memory as whole blocks, by way of a room of theirs in shared memory: stored from registers, sixteen bytes
+        // a row, a tile of 256 columns took 13000 cycles, and 5000 more until the stores were done.
+        const int quarter = warp & 3, half = (warp - 4) >> 2, in_row = (quarter & 1) * 32 + lane, pair = half * 2 + (quarter >> 1);
         const unsigned lanes = tmem_base + ((unsigned)(quarter * 32) << 16);
+        char* space = rooms + pair * kBlockBytes;
+        const bool sender = (quarter & 1) == 0 && lane == 0;
+        const auto together = [&] { asm volatile("bar.sync %0, 64;" ::"r"(1 + pair) : "memory"); };
         int q = 0, chain = 0;
         unsigned queue_parity = 0;
         bool ok = true;
+        // what the pair has written in its room to a block in memory; the room is free again when the next one is to be written
+        const auto free_room = [&] {
+            if (sender) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+            together();
+        };
+        const auto send = [&](char* to) {
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            together();
+            if (sender) {
+                asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(to), "r"(smem_u32(space)), "r"(kBlockBytes) : "memory");
+                asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+            }
+        };
         for (;;) {
             if (!mbar_wait_relaxed(&queue_full[q], queue_parity)) { atomicExch(fail_flag, 1); break; }
             const Work w = queue[q];
@@ -498,7 +517,6 @@ muon_product_kernel(const void* plan, const Told told, const Rates r, const Poly
             if (lane == 0) mbar_arrive(&queue_empty[q]);
             if (++q == kQueue) { q = 0; queue_parity ^= 1u; }
             if (w.phase < 0) break;
-            const int cols = w.width * 32, from = half * cols;
             float sum[128];
 #pragma unroll
             for (int j = 0; j < 128; ++j) sum[j] = 0.0f;
@@ -508,10 +526,11 @@ muon_product_kernel(const void* plan, const Told told, const Rates r, const Poly
                 tc_fence_after();
 #pragma unroll
                 for (int c0 = 0; c0 < 128; c0 += 32) {
-                    if (c0 < cols) {
+                    const int n = half + 2 * (c0 >> 6);
+                    if (n < w.width) {
                         unsigned v[32];
-                        tmem_ld16(lanes + b * 256 + from + c0, v);
-                        tmem_ld16(lanes + b * 256 + from + c0 + 16, v + 16);
+                        tmem_ld16(lanes + b * 256 + n * 64 + (c0 & 63), v);
+                        tmem_ld16(lanes + b * 256 + n * 64 + (c0 & 63) + 16, v + 16);
                         tmem_ld_wait();
 #pragma unroll
                         for (int j = 0; j < 32; ++j) sum[c0 + j] += __uint_as_float(v[j]);
@@ -522,85 +541,112 @@ muon_product_kernel(const void* plan, const Told told, const Rates r, const Poly
                 if (lane == 0) mbar_arrive(&sum_empty[b]);
             }
             const Matrix& t = matrices[w.matrix];
-            const int rb = 2 * w.i + (quarter >> 1), in_row = (quarter & 1) * 32 + lane, k = w.step;
+            const int rb = 2 * w.i + (quarter >> 1), k = w.step;
             const bool last = w.phase == MULTIPLY && k == poly.steps - 1;
             const int row_blocks = w.phase == MULTIPLY ? t.row_blocks : t.n_blocks, col_blocks = w.phase == MULTIPLY ? t.col_blocks : t.n_blocks;
             char* planes = room.planes + (w.phase == GRAM ? t.square : w.phase == POLY ? t.poly : t.x[(k + 1) & 1]);
             const int into = w.phase == GRAM ? poly.square[k] - 2 * poly.x[k] : w.phase == POLY ? poly.poly[k] - 2 * poly.square[k] : poly.x[k + 1] - poly.x[k] - poly.poly[k];
             const float factor = w.phase == POLY ? poly.c * power(into) : last ? power(-poly.x[k] - poly.poly[k]) : power(into);
-            const float linear = poly.b * power(poly.poly[k] - poly.square[k]), diagonal = poly.a * power(poly.poly[k]);
-            float keep = 1.0f, move = 0.0f;
-            if (last) {
-                const double rate = lr ? (double)*lr : r.lr;
-                keep = (float)(1.0 - rate * r.wd * (double)t.decay);
-                move = (float)(rate * (double)t.scale);
-            }
-            if (rb < row_blocks && ok) {
 #pragma unroll
-                for (int c0 = 0; c0 < 128; c0 += 32) {
-                    const int cb = w.j + ((from + c0) >> 6), in_col = (from + c0) & 63;
-                    // of what is symmetric the upper half, stored twice
-                    if (c0 >= cols || (w.phase != MULTIPLY && rb > cb)) continue;
-                    float* v = sum + c0;
-                    const long long at = ((long long)rb * col_blocks + cb) * kBlockPair;
-                    if (w.phase == POLY) {
-                        const char* square = room.planes + t.square + at;
+            for (int i = 0; i < 2; ++i) {
+                const int n = half + 2 * i, cb = w.j + n;
+                // of what is symmetric the upper half, stored twice
+                if (n >= w.width || rb >= row_blocks || (w.phase != MULTIPLY && rb > cb)) continue;
+                float* v = sum + 64 * i;
+                if (w.phase == MULTIPLY) {
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            float old[8];
-                            get_piece(square, in_row, (in_col >> 3) + e, old);
+                    for (int j = 0; j < 64; ++j) v[j] *= factor;
+                } else {
+                    // A in fp32 for the step's second product, four values of a row and the next row's behind them
+                    float4* held = reinterpret_cast<float4*>(room.planes + t.held + ((long long)rb * col_blocks + cb) * kBlockPair) + in_row;
+                    const float linear = poly.b * power(poly.poly[k] - poly.square[k]), diagonal = poly.a * power(poly.poly[k]);
 #pragma unroll
-                            for (int j = 0; j < 8; ++j) {
-                                const int col = cb * kBlock + in_col + 8 * e + j;
-                                v[8 * e + j] = fmaf(linear, old[j], factor * v[8 * e + j]);
-                                if (rb * kBlock + in_row == col && col < min(t.rows, t.cols)) v[8 * e + j] += diagonal;
-                            }
+                    for (int j = 0; j < 64; j += 4) {
+                        if (w.phase == GRAM) {
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) v[j + e] *= factor;
+                            __stcg(held + (j >> 2) * kBlock, make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]));
+                        } else {
+                            const float4 old = __ldcg(held + (j >> 2) * kBlock);
+                            const float a[4] = {old.x, old.y, old.z, old.w};
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) v[j + e] = fmaf(linear, a[e], factor * v[j + e]);
                         }
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) v[j] *= factor;
                     }
-                    if (!last) {
+                    if (w.phase == POLY && rb == cb && rb * kBlock + in_row < min(t.rows, t.cols)) {
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) put_piece(planes + at, in_row, (in_col >> 3) + e, v + 8 * e);
+                        for (int j = 0; j < 64; ++j)
+                            if (j == in_row) v[j] += diagonal;
                     }
-                    const bool mirror = w.phase != MULTIPLY && rb < cb;
-                    if (!mirror && !last) continue;
-                    __syncwarp();
+                }
+                if (!ok) continue;
+                if (!last) {
+                    const int copies = w.phase != MULTIPLY && rb < cb ? 2 : 1;
+                    for (int copy = 0; copy < copies; ++copy) {
+                        char* to = planes + (copy ? (long long)cb * col_blocks + rb : (long long)rb * col_blocks + cb) * kBlockPair;
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) stage[lane * kStagePitch + j] = v[j];
-                    __syncwarp();
-                    if (mirror) {
-                        // a lane to eight rows of a column: four lanes to a column of the 32 rows
-                        char* there = planes + ((long long)cb * col_blocks + rb) * kBlockPair;
+                        for (int part = 0; part < 2; ++part) {
+                            // (one part of two values, worked out each time: all of them would not fit the registers)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const int col = 8 * e + (lane >> 2), row = 8 * (lane & 3);
-                            float y[8];
+                            for (int j = 0; j < 64; ++j) asm volatile("" : "+f"(v[j]));
+                            const auto word = [&](int j) {
+                                unsigned hi, lo;
+                                parts(v[2 * j], v[2 * j + 1], hi, lo);
+                                return part ? lo : hi;
+                            };
+                            free_room();
+                            if (copy == 0) {
 #pragma unroll
-                            for (int j = 0; j < 8; ++j) y[j] = stage[(row + j) * kStagePitch + col];
-                            put_piece(there, in_col + col, ((quarter & 1) * 32 + row) >> 3, y);
-                        }
-                    } else {
-                        const int col = cb * kBlock + in_col + lane, row0 = rb * kBlock + (quarter & 1) * 32;
-                        if (col < t.cols)
-#pragma unroll 8
-                            for (int j = 0; j < 32; ++j)
-                                if (row0 + j < t.rows) {
-                                    float* p = t.param + (long long)(row0 + j) * t.cols + col;
-                                    *p = *p * keep - move * stage[j * kStagePitch + lane];
+                                for (int e = 0; e < 8; ++e)
+                                    *reinterpret_cast<uint4*>(space + in_row * 128 + ((e ^ (in_row & 7)) << 4)) = make_uint4(word(4 * e), word(4 * e + 1), word(4 * e + 2), word(4 * e + 3));
+                            } else {
+#pragma unroll
+                                for (int j = 0; j < 64; j += 2) {
+                                    const unsigned two = word(j >> 1);
+                                    char* there = space + j * 128 + (in_row & 7) * 2;
+                                    *reinterpret_cast<unsigned short*>(there + (((in_row >> 3) ^ (j & 7)) << 4)) = (unsigned short)two;
+                                    *reinterpret_cast<unsigned short*>(there + 128 + (((in_row >> 3) ^ ((j + 1) & 7)) << 4)) = (unsigned short)(two >> 16);
                                 }
+                            }
+                            send(to + part * kBlockBytes);
+                        }
+                    }
+                } else {
+                    // the param: 32 x 32 values at a time, a lane to a column; this warp's half of the room
+                    const double rate = lr ? (double)*lr : r.lr;
+                    const float keep = (float)(1.0 - rate * r.wd * (double)t.decay), move = (float)(rate * (double)t.scale);
+                    float* square = reinterpret_cast<float*>(space) + (quarter & 1) * 1024;
+                    free_room();
+#pragma unroll
+                    for (int c0 = 0; c0 < 64; c0 += 32) {
+                        __syncwarp();
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) square[lane * 32 + (j ^ lane)] = v[c0 + j];
+                        __syncwarp();
+                        const int col = cb * kBlock + c0 + lane, row0 = rb * kBlock + (quarter & 1) * 32, rows = col < t.cols ? min(32, t.rows - row0) : 0;
+                        float* param = t.param + (long long)row0 * t.cols + col;
+#pragma unroll
+                        for (int j0 = 0; j0 < 32; j0 += 16) {
+                            float old[16];
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) old[j] = j0 + j < rows ? param[(long long)(j0 + j) * t.cols] : 0.0f;
+#pragma unroll
+                            for (int j = 0; j < 16; ++j)
+                                if (j0 + j < rows) param[(long long)(j0 + j) * t.cols] = old[j] * keep - move * square[(j0 + j) * 32 + (lane ^ (j0 + j))];
+                        }
                     }
                 }
             }
             if (!last) {
                 // stored for the copies of other CTAs
+                if (sender) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
                 asm volatile("fence.proxy.async;" ::: "memory");
                 __threadfence();
                 __syncwarp();
                 if (lane == 0) asm volatile("red.release.gpu.global.add.u32 [%0], %1;" ::"l"(room.done + w.matrix), "r"(ok ? 1u : 0u) : "memory");
             }
         }
+        if (sender) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     }
     __syncwarp();
     tc_fence_before();
@@ -960,6 +1006,7 @@ Layout layout_of(const b2_muon_matrix* list, int count) {
         t.x[1] = take(blocks);
         t.square = take((long long)t.n_blocks * t.n_blocks);
         t.poly = take((long long)t.n_blocks * t.n_blocks);
+        t.held = take((long long)t.n_blocks * t.n_blocks);
         t.first_chunk = (int)found.chunks.size();
         const long long each = std::max(2048ll, (size / 512 + 2047) / 2048 * 2048);
         for (long long k = 0; k < size; k += each) found.chunks.push_back({index, (int)std::min(each, size - k), k});
