@@ -234,15 +234,16 @@ muon_parts_kernel(const void* plan, const Told told, const Rates r, const float*
 }
 
 // ---- the products ------------------------------------------------------------------------------------------
-constexpr int kUnit = 32 << 10, kUnits = 6;                 // the ring: both parts of 128 rows of P, of Q up to 128, or one part of more
+constexpr int kUnit = 32 << 10, kUnits = 5;                 // the ring: both parts of 128 rows of P, of Q up to 128, or one part of more
 constexpr int kQueue = 4;
 constexpr int kEpilogueWarps = 8;
 constexpr int kProductThreads = 128 + 32 * kEpilogueWarps;  // (a warp group for the two that copy and multiply)
 // Registers of a thread: 168 at the start, of which the first group gives so many to the epilogue's two, 56 + 2 x 224 = 3 x 168
 constexpr int kFewRegisters = 56, kManyRegisters = 224;
 static_assert(kFewRegisters + 2 * kManyRegisters <= 3 * 168, "what the block was launched with");
-constexpr int kPairs = kEpilogueWarps / 2;                  // two warps of the epilogue have the rows of a block, and room for one part of it
-constexpr int kProductShared = 1024 + kUnits * kUnit + kPairs * kBlockBytes + 512;
+constexpr int kPairs = kEpilogueWarps / 2;                  // two warps of the epilogue have the rows of a block
+constexpr int kRooms = 2 * kPairs;                          // for a part of a block each
+constexpr int kProductShared = 1024 + kUnits * kUnit + kRooms * kBlockBytes + 512;
 static_assert(kProductShared <= 227 << 10, "shared memory of a CTA");
 // Blocks of k that are added in tensor memory, whose sums lose what they add: 640 x 1920 is 2.8e-6 off in the 2-norm with one
 // (numpy's fp32 2.2e-6), 6.4e-6 with two, 1.2e-5 with four, for 3.92, 3.77 and 3.60 ms of 48 matrices.  The small products
@@ -292,12 +293,22 @@ __device__ __forceinline__ unsigned load_acquire(const unsigned* p) {
     return v;
 }
 
+__device__ __forceinline__ bool test_wait(unsigned long long* bar, unsigned parity) {       // without waiting
+    unsigned ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+    return ok != 0;
+}
+
 __global__ void __launch_bounds__(kProductThreads, 1)
 muon_product_kernel(const void* plan, const Told told, const Rates r, const Poly poly, const float* lr, const Room room, int* status) {
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     char* rooms = reinterpret_cast<char*>(smem + kUnits * kUnit);
-    unsigned long long* full_bar = reinterpret_cast<unsigned long long*>(smem + kUnits * kUnit + kPairs * kBlockBytes);
+    unsigned long long* full_bar = reinterpret_cast<unsigned long long*>(smem + kUnits * kUnit + kRooms * kBlockBytes);
     unsigned long long* empty_bar = full_bar + kUnits;
     unsigned long long* sum_full = empty_bar + kUnits;          // [2]
     unsigned long long* sum_empty = sum_full + 2;               // [2]
@@ -390,10 +401,10 @@ muon_product_kernel(const void* plan, const Told told, const Rates r, const Poly
             const Matrix& t = matrices[w.matrix];
             const Operand P = operand_of(t, room.planes, w.phase, w.step & 1, false), Q = operand_of(t, room.planes, w.phase, w.step & 1, true);
             // lanes 0 to 3: P, (part, block of rows); then Q, (part, block of columns), the lo part first.  Parts of Q in one unit up to 128
-            // columns, in two beyond
+            // columns, behind it P; beyond, the lo part, P, the hi part: what is done with first makes room for what is wanted last
             const bool both = w.width <= 2, of_p = lane < 4;
             const int turn = of_p ? lane >> 1 : (lane - 4) / w.width, place = of_p ? lane & 1 : (lane - 4) % w.width;
-            const int my_unit = of_p ? 0 : lane >= 4 + 2 * w.width ? -1 : both ? 1 : 1 + turn;
+            const int my_unit = of_p ? 1 : lane >= 4 + 2 * w.width ? -1 : both ? 0 : 2 * turn;
             const unsigned offset = (of_p ? turn * 2 + place : both ? turn * w.width + place : place) * kBlockBytes;
             const long long row = of_p ? (long long)min(2 * w.i + place, P.last) * P.mn : (long long)(w.j + place) * Q.mn;
             const char* from = (of_p ? P.base : Q.base) + row * kBlockPair + (of_p ? turn : turn ^ 1) * kBlockBytes;
@@ -406,7 +417,7 @@ muon_product_kernel(const void* plan, const Told told, const Rates r, const Poly
                         if (lane == 0) atomicExch(fail_flag, 1);
                         break;
                     }
-                    if (lane == 0) mbar_expect_tx(&full_bar[s], (u == 0 ? 4 : both ? 2 * w.width : w.width) * kBlockBytes);
+                    if (lane == 0) mbar_expect_tx(&full_bar[s], (u == 1 ? 4 : both ? 2 * w.width : w.width) * kBlockBytes);
                     __syncwarp();
                     if (my_unit == u) copy_block(smem_u32(smem + s * kUnit) + offset, from, kBlockBytes, &full_bar[s]);
                     if (++s == kUnits) { s = 0; parity ^= 1u; }
@@ -451,21 +462,25 @@ muon_product_kernel(const void* plan, const Told told, const Rates r, const Poly
                         tc_fence_after();
                     }
                     const unsigned sum = tmem_base + b * 256;
+                    const int q_unit = s;
+                    unsigned q_at = wait_unit();
+                    next();
                     const int p_unit = s;
                     const unsigned p_at = wait_unit();
                     next();
-                    unsigned q_at = wait_unit();
                     if (!ok) break;
                     const unsigned long long p_hi = describe(p_at, p_major), p_lo = describe(p_at + 2 * kBlockBytes, p_major);
                     unsigned long long q_part = describe(q_at, q_major);
 #pragma unroll
                     for (int k = 0; k < 4; ++k) multiply_f16(sum, p_hi + k * p_step, q_part + k * q_step, instruction, in > 0 || k > 0);
+                    int last_unit = q_unit;
                     if (both) {
                         q_part = describe(q_at + w.width * kBlockBytes, q_major);
                     } else {
-                        tc_commit(&empty_bar[s]);
-                        next();
+                        tc_commit(&empty_bar[q_unit]);
+                        last_unit = s;
                         q_at = wait_unit();
+                        next();
                         if (!ok) break;
                         q_part = describe(q_at, q_major);
                     }
@@ -474,8 +489,7 @@ muon_product_kernel(const void* plan, const Told told, const Rates r, const Poly
 #pragma unroll
                     for (int k = 0; k < 4; ++k) multiply_f16(sum, p_hi + k * p_step, q_part + k * q_step, instruction, 1);
                     tc_commit(&empty_bar[p_unit]);
-                    tc_commit(&empty_bar[s]);
-                    next();
+                    tc_commit(&empty_bar[last_unit]);
                     if (in == kChain - 1 || kb == w.k_blocks - 1) {
                         tc_commit(&sum_full[b]);
                         ++chain;
@@ -486,41 +500,51 @@ muon_product_kernel(const void* plan, const Told told, const Rates r, const Poly
     }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kManyRegisters));
-        // The epilogue: a quarter of the lanes (32 rows) to a warp, and every other block of columns.  Two warps have the rows of a block;
-        // its parts go to memory as whole blocks, by way of a room of theirs in shared memory: stored from registers, sixteen bytes
-        // a row, a tile of 256 columns took 13000 cycles, and 5000 more until the stores were done.
+        // The epilogue: a quarter of the lanes (32 rows) to a warp, and every other block of columns.  Two warps have the rows of a block,
+        // whose parts go to memory as whole blocks, by way of rooms in shared memory: stored from registers, sixteen bytes a row, a
+        // tile of 256 columns took 13000 cycles, and 5000 more until the stores were done.
         const int quarter = warp & 3, half = (warp - 4) >> 2, in_row = (quarter & 1) * 32 + lane, pair = half * 2 + (quarter >> 1);
         const unsigned lanes = tmem_base + ((unsigned)(quarter * 32) << 16);
-        char* space = rooms + pair * kBlockBytes;
+        char* space = rooms + pair * 2 * kBlockBytes;           // for both parts of a block
         const bool sender = (quarter & 1) == 0 && lane == 0;
         const auto together = [&] { asm volatile("bar.sync %0, 64;" ::"r"(1 + pair) : "memory"); };
-        int q = 0, chain = 0;
+        int q = 0, chain = 0, stored = -1;                      // whose item has been sent, but is not said to be stored
         unsigned queue_parity = 0;
         bool ok = true;
-        // what the pair has written in its room to a block in memory; the room is free again when the next one is to be written
-        const auto free_room = [&] {
-            if (sender) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-            together();
-        };
-        const auto send = [&](char* to) {
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            together();
-            if (sender) {
-                asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(to), "r"(smem_u32(space)), "r"(kBlockBytes) : "memory");
-                asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-            }
+        // An item is said to be stored when its copies have been made, which nobody waits for while there are other items: some blocks of k
+        // into the next one.  (Waited for at once, 4000 cycles a tile.)
+        const auto say = [&] {
+            if (stored < 0) return;
+            if (sender) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+            asm volatile("fence.proxy.async;" ::: "memory");
+            __threadfence();
+            __syncwarp();
+            if (lane == 0) asm volatile("red.release.gpu.global.add.u32 [%0], %1;" ::"l"(room.done + stored), "r"(ok ? 1u : 0u) : "memory");
+            stored = -1;
         };
         for (;;) {
+            if (!__all_sync(0xffffffffu, test_wait(&queue_full[q], queue_parity))) say();
             if (!mbar_wait_relaxed(&queue_full[q], queue_parity)) { atomicExch(fail_flag, 1); break; }
             const Work w = queue[q];
             __syncwarp();
             if (lane == 0) mbar_arrive(&queue_empty[q]);
             if (++q == kQueue) { q = 0; queue_parity ^= 1u; }
             if (w.phase < 0) break;
+            if (w.phase == MULTIPLY && w.step == poly.steps - 1) {
+                // the param's values are on their way into L2 meanwhile: a row to a lane, by 32 columns
+                const Matrix& t = matrices[w.matrix];
+                const int row = w.i * 128 + quarter * 32 + lane;
+                for (int n = half; n < w.width; n += 2)
+                    for (int c0 = 0; c0 < kBlock; c0 += 32) {
+                        const int col = (w.j + n) * kBlock + c0;
+                        if (row < t.rows && col < t.cols) asm volatile("prefetch.global.L2 [%0];" ::"l"(t.param + (long long)row * t.cols + col));
+                    }
+            }
             float sum[128];
 #pragma unroll
             for (int j = 0; j < 128; ++j) sum[j] = 0.0f;
             for (int kb = 0; kb < w.k_blocks; kb += kChain, ++chain) {
+                if (kb == 2 * kChain) say();
                 const int b = chain & 1;
                 if (ok && !mbar_wait(&sum_full[b], (chain >> 1) & 1)) { atomicExch(fail_flag, 1); ok = false; }
                 tc_fence_after();
@@ -540,6 +564,7 @@ muon_product_kernel(const void* plan, const Told told, const Rates r, const Poly
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&sum_empty[b]);
             }
+            say();
             const Matrix& t = matrices[w.matrix];
             const int rb = 2 * w.i + (quarter >> 1), k = w.step;
             const bool last = w.phase == MULTIPLY && k == poly.steps - 1;
@@ -581,34 +606,36 @@ muon_product_kernel(const void* plan, const Told told, const Rates r, const Poly
                 }
                 if (!ok) continue;
                 if (!last) {
+                    // both parts, two values to a word, in the place of the values
+                    unsigned hi[32], lo[32];
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) parts(v[2 * j], v[2 * j + 1], hi[j], lo[j]);
                     const int copies = w.phase != MULTIPLY && rb < cb ? 2 : 1;
                     for (int copy = 0; copy < copies; ++copy) {
                         char* to = planes + (copy ? (long long)cb * col_blocks + rb : (long long)rb * col_blocks + cb) * kBlockPair;
+                        if (sender) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+                        together();
+                        if (copy == 0) {
 #pragma unroll
-                        for (int part = 0; part < 2; ++part) {
-                            // (one part of two values, worked out each time: all of them would not fit the registers)
-#pragma unroll
-                            for (int j = 0; j < 64; ++j) asm volatile("" : "+f"(v[j]));
-                            const auto word = [&](int j) {
-                                unsigned hi, lo;
-                                parts(v[2 * j], v[2 * j + 1], hi, lo);
-                                return part ? lo : hi;
-                            };
-                            free_room();
-                            if (copy == 0) {
-#pragma unroll
-                                for (int e = 0; e < 8; ++e)
-                                    *reinterpret_cast<uint4*>(space + in_row * 128 + ((e ^ (in_row & 7)) << 4)) = make_uint4(word(4 * e), word(4 * e + 1), word(4 * e + 2), word(4 * e + 3));
-                            } else {
-#pragma unroll
-                                for (int j = 0; j < 64; j += 2) {
-                                    const unsigned two = word(j >> 1);
-                                    char* there = space + j * 128 + (in_row & 7) * 2;
-                                    *reinterpret_cast<unsigned short*>(there + (((in_row >> 3) ^ (j & 7)) << 4)) = (unsigned short)two;
-                                    *reinterpret_cast<unsigned short*>(there + 128 + (((in_row >> 3) ^ ((j + 1) & 7)) << 4)) = (unsigned short)(two >> 16);
-                                }
+                            for (int e = 0; e < 8; ++e) {
+                                const int at = in_row * 128 + ((e ^ (in_row & 7)) << 4);
+                                *reinterpret_cast<uint4*>(space + at) = make_uint4(hi[4 * e], hi[4 * e + 1], hi[4 * e + 2], hi[4 * e + 3]);
+                                *reinterpret_cast<uint4*>(space + kBlockBytes + at) = make_uint4(lo[4 * e], lo[4 * e + 1], lo[4 * e + 2], lo[4 * e + 3]);
                             }
-                            send(to + part * kBlockBytes);
+                        } else {
+#pragma unroll
+                            for (int j = 0; j < 64; ++j) {
+                                const int at = j * 128 + (((in_row >> 3) ^ (j & 7)) << 4) + (in_row & 7) * 2;
+                                *reinterpret_cast<unsigned short*>(space + at) = (unsigned short)(hi[j >> 1] >> (16 * (j & 1)));
+                                *reinterpret_cast<unsigned short*>(space + kBlockBytes + at) = (unsigned short)(lo[j >> 1] >> (16 * (j & 1)));
+                            }
+                        }
+                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                        together();
+                        if (sender) {
+                            // (both parts lie behind one another, here and there)
+                            asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(to), "r"(smem_u32(space)), "r"(kBlockPair) : "memory");
+                            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
                         }
                     }
                 } else {
@@ -616,7 +643,8 @@ muon_product_kernel(const void* plan, const Told told, const Rates r, const Poly
                     const double rate = lr ? (double)*lr : r.lr;
                     const float keep = (float)(1.0 - rate * r.wd * (double)t.decay), move = (float)(rate * (double)t.scale);
                     float* square = reinterpret_cast<float*>(space) + (quarter & 1) * 1024;
-                    free_room();
+                    if (sender) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+                    together();
 #pragma unroll
                     for (int c0 = 0; c0 < 64; c0 += 32) {
                         __syncwarp();
@@ -637,15 +665,9 @@ muon_product_kernel(const void* plan, const Told told, const Rates r, const Poly
                     }
                 }
             }
-            if (!last) {
-                // stored for the copies of other CTAs
-                if (sender) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
-                asm volatile("fence.proxy.async;" ::: "memory");
-                __threadfence();
-                __syncwarp();
-                if (lane == 0) asm volatile("red.release.gpu.global.add.u32 [%0], %1;" ::"l"(room.done + w.matrix), "r"(ok ? 1u : 0u) : "memory");
-            }
+            if (!last) stored = w.matrix;
         }
+        say();
         if (sender) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     }
     __syncwarp();
