@@ -10,6 +10,7 @@
 // at most an eighth of a turn, goes into the series of sine and cosine.
 #include <cmath>
 #include <cstdint>
+#include <type_traits>
 
 #include "b2_operators.h"
 #include "b2_ew_device.cuh"
@@ -199,11 +200,14 @@ heads_any_kernel(const b2_heads a, const b2_heads_grads g, const FlexArgs flex, 
     }
 }
 
-// How a launch deals out heads: `lanes` (as a power of two) to a head, so that a warp takes 32 >> lanes heads at a time, `turns` times;
-// that is a task, of the queries or of the keys of one row.
+// How a launch deals out heads: `lanes` (as a power of two) to a head, so that a warp takes 32 >> lanes heads of one tensor at a
+// time, `turns` times: that is a task.  Tasks are of one row, or, where a row's heads would leave many lanes without one, of heads next
+// to one another whatever their rows (FLAT).
 struct Deal {
-    int lanes, turns, first_tasks, row_tasks;       // tasks of a row: of the first tensor, of both
+    int lanes, turns;
     int ahead;                                      // whether the next task's heads are fetched into L2
+    int narrow;                                     // 32 bits number what is divided
+    long long first_tasks, row_tasks;               // of the first tensor (in a row, or FLAT in all), of a row
     long long tasks;
 };
 constexpr int kThreads = 256;
@@ -211,7 +215,11 @@ constexpr int kThreads = 256;
 // 128 forward, four heads: 59 us with two CTAs, 63 with three; two heads and four CTAs 72; one and five 85.  Gradients, two heads: 127
 // with two, 120 with three; one and three 146.  Rotation alone, 8192 x 20, four heads: 28.5 with three, 33 with two.
 __host__ __device__ constexpr int unrolled(int mode, int values) { return mode == BACKWARD && values >= 8 ? 2 : 4; }
-__host__ __device__ constexpr int blocks_to(int mode, int values) { return values < 8 ? (mode == BACKWARD ? 2 : 3) : mode == FORWARD ? 2 : 3; }
+__host__ __device__ constexpr int blocks_to(int mode, int values) { return values < 8 ? (mode == BACKWARD ? 2 : 3) : mode == ROTATE ? 3 : 2; }
+// How many tasks' heads a warp of whole vectors of a row has in shared memory or on their way there
+constexpr int kAhead = 3;
+__host__ __device__ constexpr bool runs_ahead(int mode, int vec, bool flat) { return mode == BACKWARD && vec == 4 && !flat; }
+__host__ __device__ constexpr int slot_bytes(int mode) { return 32 * 16 * 2 * unrolled(mode, 8) * (mode == BACKWARD ? 2 : 1) + (mode == BACKWARD ? 32 * 4 * unrolled(mode, 8) : 0); }
 // CTAs that stay, and fetch the heads of their next task into L2 meanwhile: gradients 142 us without, 127 with; forward 62 and 59; a
 // rotation, which waits for nothing but its loads, 28.5 without and 31 with.
 __host__ __device__ constexpr bool stays(int mode) { return mode != ROTATE; }
@@ -245,13 +253,17 @@ __device__ __forceinline__ void put(T* p, const float* v, float& stat) {
     }
 }
 
+// Two values next to one another, for instructions that take two at a time
+__device__ __forceinline__ float2 two(const float* v) { return make_float2(v[0], v[1]); }
+__device__ __forceinline__ void apart(float2 w, float* v) { v[0] = w.x; v[1] = w.y; }
+
 // Heads of up to 256 features: a lane holds the same features of every head that it comes to, EACH times two runs of VEC features
 // that hold both features of their pairs, so that it works out its angles once a task, while the loads are on their way, and neither
 // shares them nor waits for anybody.  All loads of a task are issued before the first is needed.
 //   HALVES: a run lies as far from the other as the features of a pair; the features behind the rotated ones likewise
 //   else:   VEC 4: two runs half a head apart, each of two pairs; VEC 1: a pair
 // BACKWARD: sums for the weights stay in registers and are added over the CTA at the end.
-template <int MODE, typename T, int VEC, int EACH, bool HALVES>
+template <int MODE, typename T, int VEC, int EACH, bool HALVES, bool FLAT>
 __global__ void __launch_bounds__(kThreads, blocks_to(MODE, 2 * VEC * EACH))
 heads_kernel(const b2_heads a, const b2_heads_grads g, const FlexArgs flex, const Deal deal, float* __restrict__ sums) {
     constexpr int N = 2 * VEC * EACH, P = N / 2, U = unrolled(MODE, N);
@@ -305,43 +317,155 @@ heads_kernel(const b2_heads a, const b2_heads_grads g, const FlexArgs flex, cons
     };
     const float share = 1.0f / (float)D;
     const long long step = (long long)gridDim.x * (kThreads / 32);
-    for (long long task = (long long)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5); task < deal.tasks; task += step) {
-        const long long row = deal.tasks <= 0xffffffffll ? (long long)((unsigned)task / (unsigned)deal.row_tasks) : task / deal.row_tasks;
-        const int in_row = (int)(task - row * deal.row_tasks), n = in_row >= deal.first_tasks;
+    const int each = deal.turns * beside;                   // heads of a task
+    const auto quotient = [&](long long i, long long by) { return deal.narrow ? (long long)((unsigned)i / (unsigned)by) : i / by; };
+    // The tensor of a task, its row, and of its first head the place in the row or, FLAT, in the tensor
+    struct Begin {
+        int n;
+        long long row;
+        typename std::conditional<FLAT, long long, int>::type head;
+    };
+    const auto begin_of = [&](long long task) {
+        Begin t;
+        t.row = FLAT ? 0 : quotient(task, deal.row_tasks);
+        if constexpr (FLAT) {
+            t.n = task >= deal.first_tasks;
+            t.head = (task - (t.n ? deal.first_tasks : 0)) * each;
+        } else {
+            const int in = (int)(task - t.row * deal.row_tasks), first_tasks = (int)deal.first_tasks;
+            t.n = in >= first_tasks;
+            t.head = (in - (t.n ? first_tasks : 0)) * each;
+        }
+        return t;
+    };
+    // Whole vectors of a row's heads come by way of shared memory, kAhead - 1 tasks ahead: a lane copies what it will read itself, so that
+    // it waits for nobody else.
+    constexpr bool RING = runs_ahead(MODE, VEC, FLAT);
+    extern __shared__ float2 table[];
+    char* slots = reinterpret_cast<char*>(table) + (threadIdx.x >> 5) * (RING ? kAhead * slot_bytes(MODE) : 0) + lane * 16;
+    const auto slot_of = [&](int stage, int tensor, int u, int e) { return slots + stage * slot_bytes(MODE) + ((tensor * U + u) * 2 + e) * 512; };
+    const auto rstd_slot = [&](int stage, int u) { return slots + stage * slot_bytes(MODE) + 2 * U * 2 * 512 + u * 128 - lane * 12; };
+    const auto copy_ahead = [&](long long task, int stage) {
+        if (task < deal.tasks) {
+            const Begin t = begin_of(task);
+            const b2_heads_part& p = a.part[t.n];
+            const b2_heads_part_grads& d = g.part[t.n];
+            const int first = (int)t.head + mine, left = p.heads - first;
+            const auto copy = [&](const T* from, int tensor, long long head_stride) {
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const bool live = u < deal.turns && u * beside < left;
+#pragma unroll
+                    for (int e = 0; e < 2; ++e)
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((unsigned)__cvta_generic_to_shared(slot_of(stage, tensor, u, e))),
+                                     "l"(live && at[e] >= 0 ? from + u * beside * head_stride + at[e] : static_cast<const T*>(p.x)), "r"(live && at[e] >= 0 ? 16 : 0)
+                                     : "memory");
+                }
+            };
+            copy(static_cast<const T*>(p.x) + t.row * p.x_row + first * p.x_head, 0, p.x_head);
+            if constexpr (MODE == BACKWARD) {
+                copy(reinterpret_cast<const T*>(d.d_out) + t.row * d.d_out_row + first * d.d_out_head, 1, d.d_out_head);
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const bool live = u < deal.turns && u * beside < left;
+                    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"((unsigned)__cvta_generic_to_shared(rstd_slot(stage, u))),
+                                 "l"(live ? p.rstd + t.row * p.heads + first + u * beside : p.rstd), "r"(live ? 4 : 0)
+                                 : "memory");
+                }
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    const long long task0 = (long long)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
+    long long next_position = 0;
+    bool next_good = true;
+    int stage = 0;
+    if constexpr (RING) {
+#pragma unroll
+        for (int k = 0; k < kAhead - 1; ++k) copy_ahead(task0 + k * step, k);
+        if (r > 0 && task0 < deal.tasks) next_good = position_of(a, begin_of(task0).row, flex.table, next_position);
+    }
+    for (long long task = task0; task < deal.tasks; task += step) {
+        const Begin t = begin_of(task);
+        const int n = t.n;
         const b2_heads_part& p = a.part[n];
         const b2_heads_part_grads& d = g.part[n];
-        const int head = (in_row - (n ? deal.first_tasks : 0)) * deal.turns * beside + mine, left = p.heads - head;
-        const T* from = static_cast<const T*>(p.x) + row * p.x_row + head * p.x_head;
-        const T* from_grad = MODE == BACKWARD ? reinterpret_cast<const T*>(d.d_out) + row * d.d_out_row + head * d.d_out_head : nullptr;
         // (heads of the next task are on their way into L2 meanwhile)
-        if (deal.ahead && task + step < deal.tasks) {
-            const long long then = task + step, row2 = deal.tasks <= 0xffffffffll ? (long long)((unsigned)then / (unsigned)deal.row_tasks) : then / deal.row_tasks;
-            const int in_row2 = (int)(then - row2 * deal.row_tasks), n2 = in_row2 >= deal.first_tasks;
-            const b2_heads_part& p2 = a.part[n2];
-            const int head2 = (in_row2 - (n2 ? deal.first_tasks : 0)) * deal.turns * beside, count = min(deal.turns * beside, p2.heads - head2);
-            const auto fetch = [&](const T* at, long long head_stride) {
-                if (head_stride != D) return;
-                const char* first = reinterpret_cast<const char*>(at);
-                for (int i = lane * 128; i < count * D * (int)sizeof(T); i += 32 * 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(first + i));
+        if (!RING && deal.ahead && task + step < deal.tasks) {
+            const Begin t2 = begin_of(task + step);
+            const b2_heads_part& p2 = a.part[t2.n];
+            const b2_heads_part_grads& d2 = g.part[t2.n];
+            const auto fetch = [&](const void* of, long long row_stride, long long head_stride) {
+                const T* tensor = static_cast<const T*>(of);
+                if constexpr (FLAT) {                       // a lane to a head
+                    for (int i = lane; i < each && t2.head + i < a.rows * p2.heads; i += 32) {
+                        const long long row = quotient(t2.head + i, p2.heads);
+                        const char* at = reinterpret_cast<const char*>(tensor + row * row_stride + (t2.head + i - row * p2.heads) * head_stride);
+                        for (int byte = 0; byte < D * (int)sizeof(T); byte += 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(at + byte));
+                    }
+                } else {                                    // heads next to one another, a lane to 128 bytes
+                    if (head_stride != D) return;
+                    const char* at = reinterpret_cast<const char*>(tensor + t2.row * row_stride + t2.head * head_stride);
+                    const int bytes = min(each, p2.heads - t2.head) * D * (int)sizeof(T);
+                    for (int i = lane * 128; i < bytes; i += 32 * 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(at + i));
+                }
             };
-            fetch(static_cast<const T*>(p2.x) + row2 * p2.x_row + head2 * p2.x_head, p2.x_head);
-            if constexpr (MODE == BACKWARD) {
-                const b2_heads_part_grads& d2 = g.part[n2];
-                fetch(reinterpret_cast<const T*>(d2.d_out) + row2 * d2.d_out_row + head2 * d2.d_out_head, d2.d_out_head);
-            }
+            fetch(p2.x, p2.x_row, p2.x_head);
+            if constexpr (MODE == BACKWARD) fetch(d2.d_out, d2.d_out_row, d2.d_out_head);
         }
         float x[U][N], y[MODE == BACKWARD ? U : 1][N], rstd[U];
         long long position = 0;
-        const bool good = r == 0 || position_of(a, row, flex.table, position);
+        bool good = true;
+        // rows and heads of each turn, FLAT; else of the task's first turn
+        int row[FLAT ? U : 1] = {}, head[FLAT ? U : 1] = {};
+        const auto first = t.head + mine;
+        const auto left = (FLAT ? a.rows * p.heads : p.heads) - first;      // heads from this lane's first one on
+        if constexpr (FLAT) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (u == 0 || head[u - 1] + beside >= p.heads) {
+                    const long long i = first + (u * beside < left ? u * beside : left - 1);       // (of lanes without a head the last one's)
+                    row[u] = (int)quotient(i, p.heads);
+                    head[u] = (int)(first + u * beside - (long long)row[u] * p.heads);
+                } else {
+                    row[u] = row[u - 1];
+                    head[u] = head[u - 1] + beside;
+                }
+            }
+        }
+        // a tensor's head of turn u
+        const auto start = [&](auto* tensor, long long row_stride, long long head_stride) { return FLAT ? tensor : tensor + t.row * row_stride + first * head_stride; };
+        const auto at_turn = [&](auto* begin, int u, long long row_stride, long long head_stride) {
+            if constexpr (FLAT) return begin + (long long)row[u] * row_stride + head[u] * head_stride;
+            else return begin + u * beside * head_stride;
+        };
+        const T* from = start(static_cast<const T*>(p.x), p.x_row, p.x_head);
+        const T* from_grad = MODE == BACKWARD ? start(reinterpret_cast<const T*>(d.d_out), d.d_out_row, d.d_out_head) : nullptr;
+        if constexpr (RING) {
+            copy_ahead(task + (kAhead - 1) * step, stage == 0 ? kAhead - 1 : stage - 1);
+            position = next_position;
+            good = next_good;
+            if (r > 0 && task + step < deal.tasks) next_good = position_of(a, begin_of(task + step).row, flex.table, next_position);
+            asm volatile("cp.async.wait_group %0;" ::"n"(kAhead - 1) : "memory");
+        } else if (r > 0) {
+            good = position_of(a, FLAT ? row[0] : t.row, flex.table, position);
+        }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const bool live = u < deal.turns && u * beside < left;
             rstd[u] = 1.0f;
-            if (live) {
-                load(from + u * beside * p.x_head, x[u]);
+            if constexpr (RING) {
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    get<4>(reinterpret_cast<const float*>(slot_of(stage, 0, u, e)), x[u] + 4 * e);
+                    if constexpr (MODE == BACKWARD) get<4>(reinterpret_cast<const float*>(slot_of(stage, 1, u, e)), y[u] + 4 * e);
+                }
+                if constexpr (MODE == BACKWARD) rstd[u] = *reinterpret_cast<const float*>(rstd_slot(stage, u));
+            } else if (live) {
+                load(at_turn(from, u, p.x_row, p.x_head), x[u]);
                 if constexpr (MODE == BACKWARD) {
-                    load(from_grad + u * beside * d.d_out_head, y[u]);
-                    rstd[u] = p.rstd[row * p.heads + head + u * beside];
+                    load(at_turn(from_grad, u, d.d_out_row, d.d_out_head), y[u]);
+                    rstd[u] = p.rstd[t.row * p.heads + first + u * beside];
                 }
             } else {
 #pragma unroll
@@ -351,6 +475,7 @@ heads_kernel(const b2_heads a, const b2_heads_grads g, const FlexArgs flex, cons
                 }
             }
         }
+        if constexpr (RING) stage = stage == kAhead - 1 ? 0 : stage + 1;
         float w[N];
         if constexpr (MODE != ROTATE) {
 #pragma unroll
@@ -360,17 +485,36 @@ heads_kernel(const b2_heads a, const b2_heads_grads g, const FlexArgs flex, cons
 #pragma unroll
                     for (int k = 0; k < VEC; ++k) w[VEC * e + k] = 1.0f;
         }
+        // the angles of turn u, where its rows are not those of the turn before
         float2 turn[P];
+        const auto face = [&](int u) {
+            if (!FLAT && u > 0) return;
+            if constexpr (FLAT) {
+                if (u > 0) {
+                    if (!__any_sync(0xffffffffu, row[u] != row[u - 1])) return;
+                    if (r > 0) good = position_of(a, row[u], flex.table, position);
+                }
+            }
 #pragma unroll
-        for (int k = 0; k < P; ++k) {
-            turn[k] = make_float2(1.0f, 0.0f);
-            if (r > 0) turn[k] = turn_of((unsigned long long)position * frequency[k], a.amplitude);
-            if (!good) turn[k] = make_float2(NAN, NAN);
-            if (MODE == BACKWARD || (MODE == ROTATE && a.inverse)) turn[k].y = -turn[k].y;
-        }
-        const long long out_head = MODE == BACKWARD ? d.d_x_head : p.out_head;
-        T* to = MODE == BACKWARD ? reinterpret_cast<T*>(d.d_x) + row * d.d_x_row + head * out_head : static_cast<T*>(p.out) + row * p.out_row + head * out_head;
+            for (int k = 0; k < P; ++k) {
+                turn[k] = make_float2(1.0f, 0.0f);
+                if (r > 0) turn[k] = turn_of((unsigned long long)position * frequency[k], a.amplitude);
+                if (!good) turn[k] = make_float2(NAN, NAN);
+                if (MODE == BACKWARD || (MODE == ROTATE && a.inverse)) turn[k].y = -turn[k].y;
+            }
+        };
+        T* to = MODE == BACKWARD ? start(reinterpret_cast<T*>(d.d_x), d.d_x_row, d.d_x_head) : start(static_cast<T*>(p.out), p.out_row, p.out_head);
         const auto rotate = [&](float* v) {
+            if constexpr (APART) {                              // (a lane's pairs turn all or none)
+                if (!turning) return;
+#pragma unroll
+                for (int k = 0; k < P; k += 2) {
+                    const float2 s = two(v + k), t = two(v + VEC + k), c = make_float2(turn[k].x, turn[k + 1].x);
+                    apart(__ffma2_rn(t, make_float2(-turn[k].y, -turn[k + 1].y), __fmul2_rn(s, c)), v + k);
+                    apart(__ffma2_rn(s, make_float2(turn[k].y, turn[k + 1].y), __fmul2_rn(t, c)), v + VEC + k);
+                }
+                return;
+            }
 #pragma unroll
             for (int k = 0; k < P; ++k) {
                 const int i = APART ? k : 2 * k, j = APART ? VEC + k : 2 * k + 1;
@@ -394,24 +538,28 @@ heads_kernel(const b2_heads a, const b2_heads_grads g, const FlexArgs flex, cons
         if constexpr (MODE == FORWARD) {
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                q[u] = 0.0f;
+                float2 square = make_float2(0.0f, 0.0f);
 #pragma unroll
-                for (int j = 0; j < N; ++j) q[u] = fmaf(x[u][j], x[u][j], q[u]);
+                for (int j = 0; j < N; j += 2) square = __ffma2_rn(two(x[u] + j), two(x[u] + j), square);
+                q[u] = square.x + square.y;
             }
             over_heads(q);
         }
         if constexpr (MODE == BACKWARD) {
 #pragma unroll
             for (int u = 0; u < U; ++u) {
+                face(u);
                 rotate(y[u]);
-                q[u] = 0.0f;
+                float2 dot = make_float2(0.0f, 0.0f);
 #pragma unroll
-                for (int j = 0; j < N; ++j) {
-                    x[u][j] *= rstd[u];                         // x^
-                    sum[j] = u == 0 ? y[u][j] * x[u][j] : fmaf(y[u][j], x[u][j], sum[j]);
-                    y[u][j] *= w[j];
-                    q[u] = fmaf(y[u][j], x[u][j], q[u]);
+                for (int j = 0; j < N; j += 2) {
+                    const float2 hat = __fmul2_rn(two(x[u] + j), make_float2(rstd[u], rstd[u])), dy = two(y[u] + j), weighted = __fmul2_rn(dy, two(w + j));
+                    apart(u == 0 ? __fmul2_rn(dy, hat) : __ffma2_rn(dy, hat, two(sum + j)), sum + j);
+                    dot = __ffma2_rn(weighted, hat, dot);
+                    apart(hat, x[u] + j);
+                    apart(weighted, y[u] + j);
                 }
+                q[u] = dot.x + dot.y;
             }
             over_heads(q);
         }
@@ -423,18 +571,20 @@ heads_kernel(const b2_heads a, const b2_heads_grads g, const FlexArgs flex, cons
             T* out = nullptr;
             if constexpr (MODE == FORWARD) {
                 const float root = rsqrtf(fmaf(q[u], share, a.eps));
-                if (p.rstd && live && sub == 0) p.rstd[row * p.heads + head + u * beside] = root;
+                if (p.rstd && live && sub == 0) p.rstd[t.row * p.heads + first + u * beside] = root;
 #pragma unroll
-                for (int j = 0; j < N; ++j) v[j] *= root * w[j];
+                for (int j = 0; j < N; j += 2) apart(__fmul2_rn(two(v + j), __fmul2_rn(two(w + j), make_float2(root, root))), v + j);
             }
             if constexpr (MODE == BACKWARD) {
-                const float mean = q[u] * share * rstd[u];
+                const float mean = -q[u] * share * rstd[u];
 #pragma unroll
-                for (int j = 0; j < N; ++j) v[j] = fmaf(-v[j], mean, rstd[u] * y[u][j]);
-                if (d.d_x && live) out = to + u * beside * out_head;
+                for (int j = 0; j < N; j += 2)
+                    apart(__ffma2_rn(two(v + j), make_float2(mean, mean), __fmul2_rn(two(y[u] + j), make_float2(rstd[u], rstd[u]))), v + j);
+                if (d.d_x && live) out = at_turn(to, u, d.d_x_row, d.d_x_head);
             } else {
+                face(u);
                 rotate(v);
-                if (live) out = to + u * beside * out_head;
+                if (live) out = at_turn(to, u, p.out_row, p.out_head);
             }
             if (!out) continue;
             if constexpr (sizeof(T) == 2) {
@@ -461,7 +611,10 @@ heads_kernel(const b2_heads a, const b2_heads_grads g, const FlexArgs flex, cons
         }
     }
     if constexpr (MODE == BACKWARD) {
-        extern __shared__ float2 table[];
+        if constexpr (RING) {
+            asm volatile("cp.async.wait_group 0;" ::: "memory");
+            __syncthreads();
+        }
         float* words = reinterpret_cast<float*>(table) + (threadIdx.x >> 5) * 2 * D;
 #pragma unroll
         for (int n = 0; n < 2; ++n)
@@ -512,7 +665,7 @@ heads_sums_kernel(const float* __restrict__ sums, int ctas, int D, float* d_weig
 
 int check_heads(const b2_heads* a, int value_bytes) {
     B2_REQUIRE(a, "missing argument");
-    B2_REQUIRE(a->rows >= 0 && a->rows <= (1ll << 38), "bad number of rows: %lld", (long long)a->rows);
+    B2_REQUIRE(a->rows >= 0 && a->rows < (1ll << 31), "bad number of rows: %lld", (long long)a->rows);
     B2_REQUIRE(a->head_dim >= 1 && a->head_dim <= kMostDim, "a head has 1 to %d features, not %d", kMostDim, a->head_dim);
     B2_REQUIRE(a->rotary_dim >= 0 && a->rotary_dim <= a->head_dim && a->rotary_dim % 2 == 0, "%d of %d features cannot be rotated", a->rotary_dim,
                a->head_dim);
@@ -631,21 +784,22 @@ int launch_any(const b2_heads& a, const b2_heads_grads& g, const FlexArgs& flex,
     return B2_OK;
 }
 
-// What a launch of heads_kernel deals out, with `pairs` of features to a lane ...
-Deal deal_of(const b2_heads& a, int runs, int turns) {
+// What a launch of heads_kernel deals out, with `runs` lanes wanted by a head and `turns` heads to a lane at once; `flat` receives
+// whether by heads: where rows would leave a quarter of the lanes without one, or where loads are value by value.
+Deal deal_of(const b2_heads& a, int runs, int turns, bool vec, bool* flat) {
     Deal d = {};
     while (d.lanes < 5 && 1 << d.lanes < runs) ++d.lanes;
     const int beside = 32 >> d.lanes;
-    // turns that the tensors' heads fill, so that both have tasks of one size
-    const int most = a.part[0].heads > (a.parts > 1 ? a.part[1].heads : 0) ? a.part[0].heads : a.part[1].heads;
-    const int rounds = (most + beside - 1) / beside, tasks = (rounds + turns - 1) / turns;
-    d.turns = tasks > 0 ? (rounds + tasks - 1) / tasks : 1;
-    // few rows: a turn to a task, for the least latency
-    if (a.rows * rounds < b2::kSms * 8) d.turns = 1;
-    const int each = d.turns * beside;
-    d.first_tasks = (a.part[0].heads + each - 1) / each;
-    d.row_tasks = d.first_tasks + (a.parts > 1 ? (a.part[1].heads + each - 1) / each : 0);
-    d.tasks = a.rows * d.row_tasks;
+    const long long heads[2] = {a.part[0].heads, a.parts > 1 ? a.part[1].heads : 0};
+    // few heads: one turn to a task, for the least latency
+    d.turns = a.rows * (heads[0] + heads[1]) / beside < b2::kSms * 8 ? 1 : turns;
+    const long long each = d.turns * beside;
+    const long long tasks[2] = {(heads[0] + each - 1) / each, (heads[1] + each - 1) / each};
+    *flat = !vec || (heads[0] + heads[1]) * 4 < (tasks[0] + tasks[1]) * each * 3;
+    d.row_tasks = tasks[0] + tasks[1];
+    d.first_tasks = *flat ? (a.rows * heads[0] + each - 1) / each : tasks[0];
+    d.tasks = *flat ? d.first_tasks + (a.rows * heads[1] + each - 1) / each : a.rows * d.row_tasks;
+    d.narrow = a.rows * (heads[0] + heads[1]) < 1ll << 32;
     return d;
 }
 constexpr int kBackwardCtas = b2::kSms * 3;
@@ -660,10 +814,13 @@ bool aligned_heads(const b2_heads& a, const void* p, int64_t row, int64_t head, 
     return (uintptr_t)p % (4 * value_bytes) == 0 && (a.rows <= 1 || row % 4 == 0) && (heads <= 1 || head % 4 == 0);
 }
 
-template <int MODE, typename T, int VEC, int EACH, bool HALVES>
+template <int MODE, typename T, int VEC, int EACH, bool HALVES, bool FLAT>
 int launch_dealt(const b2_heads& a, const b2_heads_grads& g, const FlexArgs& flex, const Deal& deal, float* sums, cudaStream_t st) {
-    const size_t room = MODE == BACKWARD ? (size_t)kThreads / 32 * 2 * a.head_dim * sizeof(float) : 0;
-    B2_CUDA((b2::launch_after(heads_kernel<MODE, T, VEC, EACH, HALVES>, dim3(ctas_of(deal, MODE, 2 * VEC * EACH)), kThreads, room, st, a, g, flex, deal, sums)));
+    constexpr bool ring = runs_ahead(MODE, VEC, FLAT);
+    const size_t room = ring ? (size_t)kThreads / 32 * kAhead * slot_bytes(MODE) : MODE == BACKWARD ? (size_t)kThreads / 32 * 2 * a.head_dim * sizeof(float) : 0;
+    static std::atomic<unsigned long long> done{0};
+    if (ring) B2_CHECK(b2::allow_shared((const void*)heads_kernel<MODE, T, VEC, EACH, HALVES, FLAT>, (int)room, &done));
+    B2_CUDA((b2::launch_after(heads_kernel<MODE, T, VEC, EACH, HALVES, FLAT>, dim3(ctas_of(deal, MODE, 2 * VEC * EACH)), kThreads, room, st, a, g, flex, deal, sums)));
     return B2_OK;
 }
 
@@ -678,17 +835,19 @@ int launch_heads(const b2_heads& a, const b2_heads_grads& g, const FlexArgs& fle
         return launch_any<MODE, T>(a, g, flex, sums, grid, st);
     }
     const int runs = vec ? a.head_dim / 8 : pairs, each = vec || runs <= 32 ? 1 : runs <= 64 ? 2 : 4;
-    Deal deal = deal_of(a, runs, unrolled(MODE, vec ? 8 : 2 * each));
+    bool flat;
+    Deal deal = deal_of(a, runs, unrolled(MODE, vec ? 8 : 2 * each), vec, &flat);
     deal.ahead = stays(MODE) && !elsewhere;
     *ctas = ctas_of(deal, MODE, vec ? 8 : 2 * each);
-#define B2_DEALT(VEC, EACH)                                                                                          \
-    if (vec == (VEC == 4) && each == EACH)                                                                           \
-        return a.interleaved ? launch_dealt<MODE, T, VEC, EACH, false>(a, g, flex, deal, sums, st)                   \
-                             : launch_dealt<MODE, T, VEC, EACH, true>(a, g, flex, deal, sums, st);
-    B2_DEALT(4, 1)
-    B2_DEALT(1, 1)
-    B2_DEALT(1, 2)
-    B2_DEALT(1, 4)
+#define B2_DEALT(VEC, EACH, FLAT)                                                                                    \
+    if (vec == (VEC == 4) && each == EACH && flat == FLAT)                                                           \
+        return a.interleaved ? launch_dealt<MODE, T, VEC, EACH, false, FLAT>(a, g, flex, deal, sums, st)             \
+                             : launch_dealt<MODE, T, VEC, EACH, true, FLAT>(a, g, flex, deal, sums, st);
+    B2_DEALT(4, 1, false)
+    B2_DEALT(4, 1, true)
+    B2_DEALT(1, 1, true)
+    B2_DEALT(1, 2, true)
+    B2_DEALT(1, 4, true)
 #undef B2_DEALT
     return b2::fail(B2_ERR_INVALID, "no kernel for heads of %d features", a.head_dim);
 }
