@@ -728,9 +728,11 @@ muon_solo_kernel(const void* plan, const Told told, const Rates r, const Poly po
         const int x_part = across * along * kBlockBytes, s_part = across * across * kBlockBytes;
         char *x = reinterpret_cast<char*>(smem), *square = x + 2 * x_part;
         const unsigned x_at = smem_u32(x), s_at = smem_u32(square);
-        // The place of x(i, j) in fp32: a block's 64 x 64 values in the place of its two parts, 32 rows in either
+        // The place of x(i, j) in fp32: a block's 64 x 64 values in the place of its two parts, 32 rows in either, fours of a row
+        // swizzled so that neighbours by rows, and every fourth one, lie in different banks
         const auto value_at = [&](int i, int j) {
-            return reinterpret_cast<float*>(x + ((j >> 6) * across + (i >> 6)) * kBlockBytes + (i & 32 ? x_part : 0)) + (i & 31) * kBlock + ((j & 63) ^ (i & 31));
+            return reinterpret_cast<float*>(x + ((j >> 6) * across + (i >> 6)) * kBlockBytes + (i & 32 ? x_part : 0)) + (i & 31) * kBlock +
+                   ((((j & 63) >> 2) ^ ((i ^ (i >> 2)) & 7)) << 2) + (j & 3);
         };
         if (n < across * kBlock || m < along * kBlock) {
             for (int e = threadIdx.x; e < 2 * x_part / 16; e += kSoloThreads) reinterpret_cast<uint4*>(x)[e] = make_uint4(0, 0, 0, 0);
@@ -771,12 +773,22 @@ muon_solo_kernel(const void* plan, const Told told, const Rates r, const Poly po
             if constexpr (decltype(count)::value == 4) *reinterpret_cast<float4*>(to) = v;
             else *to = v.x;
         };
-        // visits the places of `count` values from number i on
-        const auto places = [&](int i, auto count, auto&& visit) {
+        // visits `count` values from number i on: use(j, value) may change it where it lies in fp32
+        const auto places = [&](int i, auto count, auto&& use) {
             int at_row = i / t.cols, at_col = i - at_row * t.cols;
+            if (decltype(count)::value == 4 && !tall && (t.cols & 3) == 0) {
+                float4* four = reinterpret_cast<float4*>(value_at(at_row, at_col));
+                float4 v = *four;
+                use(0, v.x);
+                use(1, v.y);
+                use(2, v.z);
+                use(3, v.w);
+                *four = v;
+                return;
+            }
 #pragma unroll
             for (int j = 0; j < decltype(count)::value; ++j) {
-                visit(j, tall ? value_at(at_col, at_row) : value_at(at_row, at_col));
+                use(j, *(tall ? value_at(at_col, at_row) : value_at(at_row, at_col)));
                 if (++at_col == t.cols) { at_col = 0; ++at_row; }
             }
         };
@@ -788,24 +800,33 @@ muon_solo_kernel(const void* plan, const Told told, const Rates r, const Poly po
              [&](int i, float4* v, auto count) {
                  float* g = reinterpret_cast<float*>(&v[0]);
                  float* mean = reinterpret_cast<float*>(&v[1]);
-                 places(i, count, [&](int j, float* place) {
+                 places(i, count, [&](int j, float& value) {
                      mean[j] = r.mu * mean[j] + r.rest * (g[j] * s);
                      const float u = r.nesterov ? r.rest * (g[j] * s) + r.mu * mean[j] : mean[j];
-                     *place = u;
+                     value = u;
                      q = fma((double)u, (double)u, q);
                  });
                  put(t.mean + i, v[1], count);
              });
         q = cta_sum<kSoloThreads>(q, words);
         const float inverse = (float)(1.0 / (sqrt(q) + (double)r.eps)), up = power(poly.x[0]);
-        // x in parts, block by block: a thread to eight values next to one another
-        for (int b = 0; b < across * along; ++b) {
-            const int in_row = threadIdx.x >> 3, piece = threadIdx.x & 7, i = (b % across) * kBlock + in_row, j0 = (b / across) * kBlock + piece * 8;
-            float v[8];
+        // x in parts, four blocks at a time: a thread to eight values next to one another of each
+        for (int b0 = 0; b0 < across * along; b0 += 4) {
+            const int in_row = threadIdx.x >> 3, piece = threadIdx.x & 7;
+            float v[4][8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = *value_at(i, j0 + j) * inverse * up;
+            for (int b = 0; b < 4; ++b) {
+                if (b0 + b >= across * along) break;
+                const int i = ((b0 + b) % across) * kBlock + in_row, j = ((b0 + b) / across) * kBlock + piece * 8;
+                const float4 first = *reinterpret_cast<const float4*>(value_at(i, j)), second = *reinterpret_cast<const float4*>(value_at(i, j + 4));
+                const float w[8] = {first.x, first.y, first.z, first.w, second.x, second.y, second.z, second.w};
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[b][e] = w[e] * inverse * up;
+            }
             __syncthreads();
-            put_piece(x + b * kBlockBytes, in_row, piece, v, x_part);
+#pragma unroll
+            for (int b = 0; b < 4; ++b)
+                if (b0 + b < across * along) put_piece(x + (b0 + b) * kBlockBytes, in_row, piece, v[b], x_part);
         }
 
         const int quarter = warp & 3, turn = warp >> 2, row = quarter * 32 + lane;     // (sixteen columns by turns of four warps)
@@ -929,7 +950,7 @@ muon_solo_kernel(const void* plan, const Told told, const Rates r, const Poly po
                             put_columns(x, col, v, x_part);
                         } else if (row < n) {
 #pragma unroll
-                            for (int j = 0; j < 16; ++j) *value_at(row, col + j) = v[j];
+                            for (int j = 0; j < 16; j += 4) *reinterpret_cast<float4*>(value_at(row, col + j)) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
                         }
                     }
                 }
@@ -939,7 +960,7 @@ muon_solo_kernel(const void* plan, const Told told, const Rates r, const Poly po
                 walk([&](int i, float4* v, auto count) { get(t.param + i, v[0], count); },
                      [&](int i, float4* v, auto count) {
                          float* p = reinterpret_cast<float*>(&v[0]);
-                         places(i, count, [&](int j, float* place) { p[j] = p[j] * keep - move * *place; });
+                         places(i, count, [&](int j, const float& value) { p[j] = p[j] * keep - move * value; });
                          put(t.param + i, v[0], count);
                      });
             }
@@ -981,11 +1002,11 @@ void tiles_of(int rb, int cb, bool half, int width, F&& tile) {
         for (int j = half ? 2 * i : 0; j < cb; j += width) tile(i, j, std::min(width, cb - j));
 }
 
-// Cycles of an item: blocks of k, each bound by the tensor core from 192 columns on and by its copies below, and what starts and
-// ends it.
+// Cycles of an item, as measured: blocks of k, which wait for shared memory (64 columns want 72 KB read and 48 KB written a block at 128
+// bytes a cycle, 256 columns 144 and 96), and what starts and ends it.
 double cycles_of(int width, int k_blocks) {
-    static const double block[5] = {0, 700, 950, 1300, 1600};
-    return block[width] * k_blocks + 3000;
+    static const double block[5] = {0, 1150, 1430, 1700, 1960};
+    return block[width] * k_blocks + 8000;
 }
 
 Layout layout_of(const b2_muon_matrix* list, int count) {
@@ -1263,7 +1284,9 @@ extern "C" int b2_muon_step(void* plan, const b2_muon_sizes* s, const b2_muon_hy
     if (s->items > 0) {
         B2_CUDA((b2::launch_after(muon_parts_kernel, grid(s->blocks, b2::kSms * 8), kMeanThreads, 0, st, base, told, r, grad_scale, (int)p.x[0], room)));
         B2_CHECK(b2::allow_shared((const void*)muon_product_kernel, kProductShared, &done));
-        B2_CUDA((b2::launch_after(muon_product_kernel, grid(s->items, b2::kSms), kProductThreads, (size_t)kProductShared, st, base, told, r, p, lr, room, status)));
+        // (SMs for the small matrices where few items would leave some idle anyway: these need 50 us, which would come on top)
+        const long long left = s->items < 8 * b2::kSms ? b2::kSms - std::min<long long>(s->solos, 8) : b2::kSms;
+        B2_CUDA((b2::launch_after(muon_product_kernel, grid(s->items, left), kProductThreads, (size_t)kProductShared, st, base, told, r, p, lr, room, status)));
     }
     if (s->solos > 0) {
         B2_CHECK(b2::allow_shared((const void*)muon_solo_kernel, kSoloShared, &done_solo));
