@@ -736,7 +736,7 @@ int b2_adamw_step(void* plan, int64_t chunks, int32_t state_bits, const b2_adamw
  *   param = param (1 - lr weight_decay decay) - lr scale x
  * which takes the singular values of x towards one.  Products are accurate to fp32: operands are held as two fp16 parts, which
  * together round as fp32 does, and three of the four products of parts are added, in fp32.  A matrix with a gradient that is not finite becomes NaN, the others are
- * not touched by it; one whose u is zero only decays.
+ * not touched by it; one whose u is zero only decays (where eps is not zero).
  *   sizes: bytes of the plan and of the scratch, and what a step is told of the plan
  *   plan:  a table of the work on the device, made once for given addresses (not while a stream is captured); tensors that
  *          overlap are refused, gradients may be shared; matrices without values are allowed

@@ -792,8 +792,9 @@ int launch_any(const b2_heads& a, const b2_heads_grads& g, const FlexArgs& flex,
 }
 
 // What a launch of heads_kernel deals out, with `runs` lanes wanted by a head and `turns` heads to a lane at once; `flat` receives
-// whether by heads: where rows would leave a quarter of the lanes without one, or where loads are value by value.
-Deal deal_of(const b2_heads& a, int runs, int turns, bool vec, bool* flat) {
+// whether by heads: where rows would leave a quarter of the lanes without one, or, `by_heads`, where loads are value by value or from
+// page-locked memory.
+Deal deal_of(const b2_heads& a, int runs, int turns, bool by_heads, bool* flat) {
     Deal d = {};
     while (d.lanes < 5 && 1 << d.lanes < runs) ++d.lanes;
     const int beside = 32 >> d.lanes;
@@ -802,7 +803,7 @@ Deal deal_of(const b2_heads& a, int runs, int turns, bool vec, bool* flat) {
     d.turns = a.rows * (heads[0] + heads[1]) / beside < b2::kSms * 8 ? 1 : turns;
     const long long each = d.turns * beside;
     const long long tasks[2] = {(heads[0] + each - 1) / each, (heads[1] + each - 1) / each};
-    *flat = !vec || (heads[0] + heads[1]) * 4 < (tasks[0] + tasks[1]) * each * 3;
+    *flat = by_heads || (heads[0] + heads[1]) * 4 < (tasks[0] + tasks[1]) * each * 3;
     d.row_tasks = tasks[0] + tasks[1];
     d.first_tasks = *flat ? (a.rows * heads[0] + each - 1) / each : tasks[0];
     d.tasks = *flat ? d.first_tasks + (a.rows * heads[1] + each - 1) / each : a.rows * d.row_tasks;
@@ -843,7 +844,7 @@ int launch_heads(const b2_heads& a, const b2_heads_grads& g, const FlexArgs& fle
     }
     const int runs = vec ? a.head_dim / 8 : pairs, each = vec || runs <= 32 ? 1 : runs <= 64 ? 2 : 4;
     bool flat;
-    Deal deal = deal_of(a, runs, unrolled(MODE, vec ? 8 : 2 * each), vec, &flat);
+    Deal deal = deal_of(a, runs, unrolled(MODE, vec ? 8 : 2 * each), !vec || elsewhere, &flat);
     deal.ahead = stays(MODE) && !elsewhere;
     *ctas = ctas_of(deal, MODE, vec ? 8 : 2 * each);
 #define B2_DEALT(VEC, EACH, FLAT)                                                                                    \

@@ -73,7 +73,7 @@ struct Group {                               // matrices whose steps run next to
     long long first, count;
 };
 struct Header {
-    long long matrices, chunks, items, blocks, solos, groups;
+    long long matrices, chunks, items, blocks, solos, bytes, groups;      // bytes: of the scratch
 };
 constexpr size_t kHeader = 64;
 
@@ -112,11 +112,12 @@ __device__ __forceinline__ const Item* items_of(const void* plan) { return reint
 __device__ __forceinline__ const Group* groups_of(const void* plan) { return reinterpret_cast<const Group*>(items_of(plan) + header_of(plan)->items); }
 
 struct Told {                                // what the caller says of the plan; a step with other sizes does nothing
-    long long matrices, chunks, items, blocks, solos;
+    long long matrices, chunks, items, blocks, solos, bytes;
 };
 __device__ __forceinline__ bool fits(const void* plan, const Told& t) {
     const Header* h = header_of(plan);
-    return h->matrices == t.matrices && h->chunks == t.chunks && h->items == t.items && h->blocks == t.blocks && h->solos == t.solos;
+    return h->matrices == t.matrices && h->chunks == t.chunks && h->items == t.items && h->blocks == t.blocks && h->solos == t.solos &&
+           h->bytes == t.bytes;
 }
 
 // The scratch: sums of squares by chunk; counters; planes.
@@ -314,7 +315,8 @@ muon_product_kernel(const void* plan, const Told told, const Rates r, const Poly
     unsigned long long* sum_empty = sum_full + 2;               // [2]
     unsigned long long* queue_full = sum_empty + 2;
     unsigned long long* queue_empty = queue_full + kQueue;
-    Work* queue = reinterpret_cast<Work*>(queue_empty + kQueue);
+    unsigned long long* idle = queue_empty + kQueue;
+    Work* queue = reinterpret_cast<Work*>(idle + 1);
     unsigned* tmem_holder = reinterpret_cast<unsigned*>(queue + kQueue);
     int* fail_flag = reinterpret_cast<int*>(tmem_holder + 1);
 
@@ -323,6 +325,7 @@ muon_product_kernel(const void* plan, const Told told, const Rates r, const Poly
         for (int s = 0; s < kUnits; ++s) { mbar_init(&full_bar[s], 1); mbar_init(&empty_bar[s], 1); }
         for (int b = 0; b < 2; ++b) { mbar_init(&sum_full[b], 1); mbar_init(&sum_empty[b], kEpilogueWarps); }
         for (int q = 0; q < kQueue; ++q) { mbar_init(&queue_full[q], 1); mbar_init(&queue_empty[q], 1 + kEpilogueWarps); }
+        mbar_init(idle, 1);
         *fail_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -338,166 +341,167 @@ muon_product_kernel(const void* plan, const Told told, const Rates r, const Poly
     const Matrix* matrices = matrices_of(plan);
 
     if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFewRegisters));
-    if (warp == 0) {
-        // A lane to each copy of a block of k, with its addresses worked out once an item: one thread for all of them took 150 cycles a
-        // copy, 1900 a block of k of 256 columns, of which the products take 1536.
-        int s = 0, q = 0;
-        unsigned parity = 1, queue_parity = 1;
-        bool ok = true;
-        long long group = 0;
-        const long long total = mine ? told.items * poly.steps : 0;
-        for (;;) {
-            // the next item
-            Work w = {};
-            w.phase = -1;
-            long long number = total;
-            if (lane == 0 && ok && total && !*reinterpret_cast<volatile unsigned*>(room.failed)) number = (long long)atomicAdd(room.next, 1u);
-            number = __shfl_sync(0xffffffffu, number, 0);
-            if (number < total) {
-                const Group* g = groups_of(plan) + group;
-                while (number >= poly.steps * (g->first + g->count)) { ++g; ++group; }
-                const long long in = number - poly.steps * g->first;
-                w.step = (int)(in / g->count);
-                const Item item = items_of(plan)[g->first + (in - w.step * g->count)];
-                const Matrix& t = matrices[item.matrix];
-                w.matrix = item.matrix;
-                w.phase = item.phase;
-                w.i = item.i;
-                w.j = item.j;
-                w.width = item.width;
-                w.k_blocks = item.phase == GRAM ? (t.tall ? t.row_blocks : t.col_blocks) : t.n_blocks;
-                // what it reads has been stored
-                const int before = w.step * (t.items[0] + t.items[1] + t.items[2]) + (item.phase > GRAM ? t.items[0] : 0) + (item.phase > POLY ? t.items[1] : 0);
-                const unsigned need = (unsigned)before * kEpilogueWarps;
-                bool there = false;
-                if (lane == 0)
-                    for (int i = 0; i < kDependencyPolls && !there; ++i) {
-                        there = (int)(load_acquire(room.done + item.matrix) - need) >= 0;
-                        if (!there) {
-                            if (*reinterpret_cast<volatile unsigned*>(room.failed)) break;
-                            __nanosleep(40);
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFewRegisters));
+        if (warp == 0) {
+            // A lane to each copy of a block of k, with its addresses worked out once an item: one thread for all of them took 150 cycles a
+            // copy, 1900 a block of k of 256 columns, of which the products take 1536.
+            int s = 0, q = 0;
+            unsigned parity = 1, queue_parity = 1;
+            bool ok = true;
+            long long group = 0, issued = 0;                    // units that copies have been started into
+            const long long total = mine ? told.items * poly.steps : 0;
+            for (;;) {
+                // the next item
+                Work w = {};
+                w.phase = -1;
+                long long number = total;
+                if (lane == 0 && ok && total && !*reinterpret_cast<volatile unsigned*>(room.failed)) number = (long long)atomicAdd(room.next, 1u);
+                number = __shfl_sync(0xffffffffu, number, 0);
+                if (number < total) {
+                    const Group* g = groups_of(plan) + group;
+                    while (number >= poly.steps * (g->first + g->count)) { ++g; ++group; }
+                    const long long in = number - poly.steps * g->first;
+                    w.step = (int)(in / g->count);
+                    const Item item = items_of(plan)[g->first + (in - w.step * g->count)];
+                    const Matrix& t = matrices[item.matrix];
+                    w.matrix = item.matrix;
+                    w.phase = item.phase;
+                    w.i = item.i;
+                    w.j = item.j;
+                    w.width = item.width;
+                    w.k_blocks = item.phase == GRAM ? (t.tall ? t.row_blocks : t.col_blocks) : t.n_blocks;
+                    // what it reads has been stored
+                    const int before = w.step * (t.items[0] + t.items[1] + t.items[2]) + (item.phase > GRAM ? t.items[0] : 0) + (item.phase > POLY ? t.items[1] : 0);
+                    const unsigned need = (unsigned)before * kEpilogueWarps;
+                    bool there = false;
+                    if (lane == 0)
+                        for (int i = 0; i < kDependencyPolls && !there; ++i) {
+                            there = (int)(load_acquire(room.done + item.matrix) - need) >= 0;
+                            if (!there) {
+                                if (*reinterpret_cast<volatile unsigned*>(room.failed)) break;
+                                __nanosleep(40);
+                            }
                         }
+                    there = __shfl_sync(0xffffffffu, (int)there, 0) != 0;
+                    asm volatile("fence.proxy.async;" ::: "memory");
+                    if (!there) {
+                        if (lane == 0) atomicExch(fail_flag, 1);
+                        ok = false;
+                        w.phase = -1;
                     }
-                there = __shfl_sync(0xffffffffu, (int)there, 0) != 0;
-                asm volatile("fence.proxy.async;" ::: "memory");
-                if (!there) {
+                }
+                if (!__all_sync(0xffffffffu, mbar_wait(&queue_empty[q], queue_parity))) {
                     if (lane == 0) atomicExch(fail_flag, 1);
                     ok = false;
-                    w.phase = -1;
+                    break;
                 }
-            }
-            if (!__all_sync(0xffffffffu, mbar_wait(&queue_empty[q], queue_parity))) {
-                if (lane == 0) atomicExch(fail_flag, 1);
-                ok = false;
-                break;
-            }
-            if (lane == 0) {
-                queue[q] = w;
-                mbar_arrive(&queue_full[q]);
-            }
-            if (++q == kQueue) { q = 0; queue_parity ^= 1u; }
-            if (w.phase < 0) break;
-            const Matrix& t = matrices[w.matrix];
-            const Operand P = operand_of(t, room.planes, w.phase, w.step & 1, false), Q = operand_of(t, room.planes, w.phase, w.step & 1, true);
-            // lanes 0 to 3: P, (part, block of rows); then Q, (part, block of columns), the lo part first.  Parts of Q in one unit up to 128
-            // columns, behind it P; beyond, the lo part, P, the hi part: what is done with first makes room for what is wanted last
-            const bool both = w.width <= 2, of_p = lane < 4;
-            const int turn = of_p ? lane >> 1 : (lane - 4) / w.width, place = of_p ? lane & 1 : (lane - 4) % w.width;
-            const int my_unit = of_p ? 1 : lane >= 4 + 2 * w.width ? -1 : both ? 0 : 2 * turn;
-            const unsigned offset = (of_p ? turn * 2 + place : both ? turn * w.width + place : place) * kBlockBytes;
-            const long long row = of_p ? (long long)min(2 * w.i + place, P.last) * P.mn : (long long)(w.j + place) * Q.mn;
-            const char* from = (of_p ? P.base : Q.base) + row * kBlockPair + (of_p ? turn : turn ^ 1) * kBlockBytes;
-            const long long along = (of_p ? P.k : Q.k) * (long long)kBlockPair;
-            const int units = both ? 2 : 3;
-            for (int kb = 0; kb < w.k_blocks && ok; ++kb) {
-                for (int u = 0; u < units; ++u) {
-                    ok = __all_sync(0xffffffffu, mbar_wait(&empty_bar[s], parity));
-                    if (!ok) {
-                        if (lane == 0) atomicExch(fail_flag, 1);
-                        break;
-                    }
-                    if (lane == 0) mbar_expect_tx(&full_bar[s], (u == 1 ? 4 : both ? 2 * w.width : w.width) * kBlockBytes);
-                    __syncwarp();
-                    if (my_unit == u) copy_block(smem_u32(smem + s * kUnit) + offset, from, kBlockBytes, &full_bar[s]);
-                    if (++s == kUnits) { s = 0; parity ^= 1u; }
+                if (lane == 0) {
+                    queue[q] = w;
+                    mbar_arrive(&queue_full[q]);
                 }
-                from += along;
-            }
-        }
-        // copies in flight have landed, and have been read, before the CTA may end
-        for (int i = 0; i < kUnits && ok; ++i) {
-            ok = __all_sync(0xffffffffu, mbar_wait(&empty_bar[s], parity));
-            if (!ok && lane == 0) atomicExch(fail_flag, 1);
-            if (++s == kUnits) { s = 0; parity ^= 1u; }
-        }
-    } else if (warp == 1) {
-        if (elect_one()) {
-            int s = 0, q = 0, chain = 0;
-            unsigned parity = 0, queue_parity = 0;
-            bool ok = true;
-            auto wait_unit = [&] {
-                if (!mbar_wait(&full_bar[s], parity)) { atomicExch(fail_flag, 1); ok = false; }
-                tc_fence_after();
-                return smem_u32(smem + s * kUnit);
-            };
-            auto next = [&] { if (++s == kUnits) { s = 0; parity ^= 1u; } };
-            while (ok) {
-                if (!mbar_wait_relaxed(&queue_full[q], queue_parity)) { atomicExch(fail_flag, 1); break; }
-                const Work w = queue[q];
-                mbar_arrive(&queue_empty[q]);
                 if (++q == kQueue) { q = 0; queue_parity ^= 1u; }
                 if (w.phase < 0) break;
                 const Matrix& t = matrices[w.matrix];
-                const unsigned p_major = operand_of(t, room.planes, w.phase, 0, false).major, q_major = operand_of(t, room.planes, w.phase, 0, true).major;
-                // fp16 operands, fp32 sums, 128 rows
-                const unsigned instruction = (1u << 4) | (p_major << 15) | (q_major << 16) | ((unsigned)(w.width * kBlock >> 3) << 17) | ((128u >> 4) << 24);
-                const unsigned p_step = p_major ? 2048 >> 4 : 32 >> 4, q_step = q_major ? 2048 >> 4 : 32 >> 4;       // 16 of k
-                const bool both = w.width <= 2;
+                const Operand P = operand_of(t, room.planes, w.phase, w.step & 1, false), Q = operand_of(t, room.planes, w.phase, w.step & 1, true);
+                // lanes 0 to 3: P, (part, block of rows); then Q, (part, block of columns), the lo part first.  Parts of Q in one unit up to 128
+                // columns, behind it P; beyond, the lo part, P, the hi part: what is done with first makes room for what is wanted last
+                const bool both = w.width <= 2, of_p = lane < 4;
+                const int turn = of_p ? lane >> 1 : (lane - 4) / w.width, place = of_p ? lane & 1 : (lane - 4) % w.width;
+                const int my_unit = of_p ? 1 : lane >= 4 + 2 * w.width ? -1 : both ? 0 : 2 * turn;
+                const unsigned offset = (of_p ? turn * 2 + place : both ? turn * w.width + place : place) * kBlockBytes;
+                const long long row = of_p ? (long long)min(2 * w.i + place, P.last) * P.mn : (long long)(w.j + place) * Q.mn;
+                const char* from = (of_p ? P.base : Q.base) + row * kBlockPair + (of_p ? turn : turn ^ 1) * kBlockBytes;
+                const long long along = (of_p ? P.k : Q.k) * (long long)kBlockPair;
+                const int units = both ? 2 : 3;
                 for (int kb = 0; kb < w.k_blocks && ok; ++kb) {
-                    const int in = kb % kChain, b = chain & 1;
-                    if (in == 0) {
-                        // the sums before in these columns have been read
-                        if (chain > 1 && !mbar_wait(&sum_empty[b], ((chain >> 1) - 1) & 1)) { atomicExch(fail_flag, 1); ok = false; break; }
-                        tc_fence_after();
+                    for (int u = 0; u < units; ++u) {
+                        ok = __all_sync(0xffffffffu, mbar_wait(&empty_bar[s], parity));
+                        if (!ok) {
+                            if (lane == 0) atomicExch(fail_flag, 1);
+                            break;
+                        }
+                        if (lane == 0) mbar_expect_tx(&full_bar[s], (u == 1 ? 4 : both ? 2 * w.width : w.width) * kBlockBytes);
+                        __syncwarp();
+                        if (my_unit == u) copy_block(smem_u32(smem + s * kUnit) + offset, from, kBlockBytes, &full_bar[s]);
+                        ++issued;
+                        if (++s == kUnits) { s = 0; parity ^= 1u; }
                     }
-                    const unsigned sum = tmem_base + b * 256;
-                    const int q_unit = s;
-                    unsigned q_at = wait_unit();
-                    next();
-                    const int p_unit = s;
-                    const unsigned p_at = wait_unit();
-                    next();
-                    if (!ok) break;
-                    const unsigned long long p_hi = describe(p_at, p_major), p_lo = describe(p_at + 2 * kBlockBytes, p_major);
-                    unsigned long long q_part = describe(q_at, q_major);
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) multiply_f16(sum, p_hi + k * p_step, q_part + k * q_step, instruction, in > 0 || k > 0);
-                    int last_unit = q_unit;
-                    if (both) {
-                        q_part = describe(q_at + w.width * kBlockBytes, q_major);
-                    } else {
-                        tc_commit(&empty_bar[q_unit]);
-                        last_unit = s;
-                        q_at = wait_unit();
-                        next();
-                        if (!ok) break;
-                        q_part = describe(q_at, q_major);
-                    }
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) multiply_f16(sum, p_lo + k * p_step, q_part + k * q_step, instruction, 1);
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) multiply_f16(sum, p_hi + k * p_step, q_part + k * q_step, instruction, 1);
-                    tc_commit(&empty_bar[p_unit]);
-                    tc_commit(&empty_bar[last_unit]);
-                    if (in == kChain - 1 || kb == w.k_blocks - 1) {
-                        tc_commit(&sum_full[b]);
-                        ++chain;
-                    }
+                    from += along;
                 }
             }
+            // copies in flight have landed before the CTA may end, whatever came of the others' waiting
+            for (long long i = issued < kUnits ? 0 : issued - kUnits; i < issued; ++i)
+                if (!__all_sync(0xffffffffu, mbar_wait(&full_bar[i % kUnits], (unsigned)(i / kUnits) & 1)) && lane == 0) atomicExch(fail_flag, 1);
+        } else if (warp == 1) {
+            if (elect_one()) {
+                int s = 0, q = 0, chain = 0;
+                unsigned parity = 0, queue_parity = 0;
+                bool ok = true;
+                auto wait_unit = [&] {
+                    if (!mbar_wait(&full_bar[s], parity)) { atomicExch(fail_flag, 1); ok = false; }
+                    tc_fence_after();
+                    return smem_u32(smem + s * kUnit);
+                };
+                auto next = [&] { if (++s == kUnits) { s = 0; parity ^= 1u; } };
+                while (ok) {
+                    if (!mbar_wait_relaxed(&queue_full[q], queue_parity)) { atomicExch(fail_flag, 1); break; }
+                    const Work w = queue[q];
+                    mbar_arrive(&queue_empty[q]);
+                    if (++q == kQueue) { q = 0; queue_parity ^= 1u; }
+                    if (w.phase < 0) break;
+                    const Matrix& t = matrices[w.matrix];
+                    const unsigned p_major = operand_of(t, room.planes, w.phase, 0, false).major, q_major = operand_of(t, room.planes, w.phase, 0, true).major;
+                    // fp16 operands, fp32 sums, 128 rows
+                    const unsigned instruction = (1u << 4) | (p_major << 15) | (q_major << 16) | ((unsigned)(w.width * kBlock >> 3) << 17) | ((128u >> 4) << 24);
+                    const unsigned p_step = p_major ? 2048 >> 4 : 32 >> 4, q_step = q_major ? 2048 >> 4 : 32 >> 4;       // 16 of k
+                    const bool both = w.width <= 2;
+                    for (int kb = 0; kb < w.k_blocks && ok; ++kb) {
+                        const int in = kb % kChain, b = chain & 1;
+                        if (in == 0) {
+                            // the sums before in these columns have been read
+                            if (chain > 1 && !mbar_wait(&sum_empty[b], ((chain >> 1) - 1) & 1)) { atomicExch(fail_flag, 1); ok = false; break; }
+                            tc_fence_after();
+                        }
+                        const unsigned sum = tmem_base + b * 256;
+                        const int q_unit = s;
+                        unsigned q_at = wait_unit();
+                        next();
+                        const int p_unit = s;
+                        const unsigned p_at = wait_unit();
+                        next();
+                        if (!ok) break;
+                        const unsigned long long p_hi = describe(p_at, p_major), p_lo = describe(p_at + 2 * kBlockBytes, p_major);
+                        unsigned long long q_part = describe(q_at, q_major);
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) multiply_f16(sum, p_hi + k * p_step, q_part + k * q_step, instruction, in > 0 || k > 0);
+                        int last_unit = q_unit;
+                        if (both) {
+                            q_part = describe(q_at + w.width * kBlockBytes, q_major);
+                        } else {
+                            tc_commit(&empty_bar[q_unit]);
+                            last_unit = s;
+                            q_at = wait_unit();
+                            next();
+                            if (!ok) break;
+                            q_part = describe(q_at, q_major);
+                        }
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) multiply_f16(sum, p_lo + k * p_step, q_part + k * q_step, instruction, 1);
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) multiply_f16(sum, p_hi + k * p_step, q_part + k * q_step, instruction, 1);
+                        tc_commit(&empty_bar[p_unit]);
+                        tc_commit(&empty_bar[last_unit]);
+                        if (in == kChain - 1 || kb == w.k_blocks - 1) {
+                            tc_commit(&sum_full[b]);
+                            ++chain;
+                        }
+                    }
+                }
+                // products in flight have been made before tensor memory is freed
+                tc_commit(idle);
+                if (!mbar_wait(idle, 0)) atomicExch(fail_flag, 1);
+            }
         }
-    }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kManyRegisters));
         // The epilogue: a quarter of the lanes (32 rows) to a warp, and every other block of columns.  Two warps have the rows of a block,
@@ -1209,7 +1213,7 @@ extern "C" int b2_muon_plan(const b2_muon_matrix* list, int32_t count, void* pla
         B2_CUDA(cudaStreamIsCapturing((cudaStream_t)stream, &capturing));
         B2_REQUIRE(capturing == cudaStreamCaptureStatusNone, "a plan is made before its stream is captured");
         std::vector<char> host(l.plan_bytes(), 0);
-        *reinterpret_cast<Header*>(host.data()) = {s.matrices, s.chunks, s.items, s.blocks, s.solos, (long long)l.groups.size()};
+        *reinterpret_cast<Header*>(host.data()) = {s.matrices, s.chunks, s.items, s.blocks, s.solos, (long long)s.scratch_bytes, (long long)l.groups.size()};
         char* to = host.data() + kHeader;
         const auto put = [&](const void* from, size_t bytes) {
             std::copy((const char*)from, (const char*)from + bytes, to);
@@ -1276,7 +1280,7 @@ extern "C" int b2_muon_step(void* plan, const b2_muon_sizes* s, const b2_muon_hy
     room.failed = room.next + 1;
     room.done = room.next + 4;
     room.planes = at + counter_bytes(*s);
-    const Told told = {s->matrices, s->chunks, s->items, s->blocks, s->solos};
+    const Told told = {s->matrices, s->chunks, s->items, s->blocks, s->solos, (long long)s->scratch_bytes};
     const auto grid = [](long long work, long long most) { return dim3((unsigned)(work < 1 ? 1 : work < most ? work : most)); };
     static std::atomic<unsigned long long> done{0}, done_solo{0};
     if (s->items > 0 || s->solos == 0)
