@@ -449,6 +449,10 @@ class Computation(object):
 builtin_sum = sum
 
 
+def _closed():
+    raise lib.B200Error("the transformer of this computation is closed")
+
+
 # ---------------------------------------------------------------------------------------------
 class _CallIO(object):
     """Arguments and results of a recorded step list: its first node, or a launch in front of it, reads the
@@ -1964,6 +1968,11 @@ class B200Transformer(object):
         self.closed = True
         if getattr(self, "tracer", None) is not None and self.tracer.events:
             self.tracer.serialize_to_file()
+        # (recordings end here: one that only the collector finds is destroyed at any time, in the middle of another's
+        # recording, say, which that ends with an error)
+        for c in self.computations:
+            if getattr(c, "_graphs", None) is not None:
+                c._graphs, c.executor = None, _closed
         self._buffers.clear()
         self._views.clear()
         self._scratch = self._table = self._stats = self._status = self._probe64 = None
