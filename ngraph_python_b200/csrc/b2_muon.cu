@@ -1060,12 +1060,22 @@ Layout layout_of(const b2_muon_matrix* list, int count) {
         t.chunks = (int)found.chunks.size() - t.first_chunk;
         for (int k = 0; k < blocks; ++k) found.blocks.push_back({index, k});
     }
-    // Groups of matrices whose phases keep the machine busy while another's end: some three tiles to an SM
-    for (size_t from = 0; from < shared;) {
+    // Groups of matrices whose phases keep the machine busy while another's end: some three tiles to an SM or more, in groups of one
+    // size (a last group of few matrices would wait for each of its phases)
+    const auto tiles_in = [&](size_t m) {
+        long long tiles = 0;
+        tiles_of(found.matrices[m].n_blocks, found.matrices[m].n_blocks, true, 4, [&](int, int, int) { ++tiles; });
+        return tiles;
+    };
+    long long tiles_left = 0;
+    for (size_t m = 0; m < shared; ++m) tiles_left += tiles_in(m);
+    long long groups_left = std::max(1ll, tiles_left / (3 * b2::kSms));
+    for (size_t from = 0; from < shared; --groups_left) {
         size_t to = from;
-        for (long long tiles = 0; to < shared && tiles < 3 * b2::kSms; ++to) {
-            const Matrix& t = found.matrices[to];
-            tiles_of(t.n_blocks, t.n_blocks, true, 4, [&](int, int, int) { ++tiles; });
+        const long long enough = tiles_left / std::max(1ll, groups_left);
+        for (long long tiles = 0; to < shared && (tiles < enough || groups_left <= 1); ++to) {
+            tiles += tiles_in(to);
+            tiles_left -= tiles_in(to);
         }
         const long long first = (long long)found.items.size();
         for (int phase = GRAM; phase <= MULTIPLY; ++phase) {
