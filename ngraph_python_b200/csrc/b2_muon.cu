@@ -589,17 +589,20 @@ muon_product_kernel(const void* plan, const Told told, const Rates r, const Poly
                     // A in fp32 for the step's second product, four values of a row and the next row's behind them
                     float4* held = reinterpret_cast<float4*>(room.planes + t.held + ((long long)rb * col_blocks + cb) * kBlockPair) + in_row;
                     const float linear = poly.b * power(poly.poly[k] - poly.square[k]), diagonal = poly.a * power(poly.poly[k]);
+                    if (w.phase == GRAM) {
 #pragma unroll
-                    for (int j = 0; j < 64; j += 4) {
-                        if (w.phase == GRAM) {
+                        for (int j = 0; j < 64; ++j) v[j] *= factor;
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) v[j + e] *= factor;
-                            __stcg(held + (j >> 2) * kBlock, make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]));
-                        } else {
-                            const float4 old = __ldcg(held + (j >> 2) * kBlock);
-                            const float a[4] = {old.x, old.y, old.z, old.w};
+                        for (int j = 0; j < 64; j += 4) __stcg(held + (j >> 2) * kBlock, make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]));
+                    } else {
+                        float4 old[16];                         // (all on their way before the first is used)
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) v[j + e] = fmaf(linear, a[e], factor * v[j + e]);
+                        for (int j = 0; j < 16; ++j) old[j] = __ldcg(held + j * kBlock);
+#pragma unroll
+                        for (int j = 0; j < 64; ++j) {
+                            const float4 four = old[j >> 2];
+                            const float a = (j & 3) == 0 ? four.x : (j & 3) == 1 ? four.y : (j & 3) == 2 ? four.z : four.w;
+                            v[j] = fmaf(linear, a, factor * v[j]);
                         }
                     }
                     if (w.phase == POLY && rb == cb && rb * kBlock + in_row < min(t.rows, t.cols)) {
@@ -614,26 +617,7 @@ muon_product_kernel(const void* plan, const Told told, const Rates r, const Poly
                     unsigned hi[32], lo[32];
 #pragma unroll
                     for (int j = 0; j < 32; ++j) parts(v[2 * j], v[2 * j + 1], hi[j], lo[j]);
-                    const int copies = w.phase != MULTIPLY && rb < cb ? 2 : 1;
-                    for (int copy = 0; copy < copies; ++copy) {
-                        char* to = planes + (copy ? (long long)cb * col_blocks + rb : (long long)rb * col_blocks + cb) * kBlockPair;
-                        if (sender) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-                        together();
-                        if (copy == 0) {
-#pragma unroll
-                            for (int e = 0; e < 8; ++e) {
-                                const int at = in_row * 128 + ((e ^ (in_row & 7)) << 4);
-                                *reinterpret_cast<uint4*>(space + at) = make_uint4(hi[4 * e], hi[4 * e + 1], hi[4 * e + 2], hi[4 * e + 3]);
-                                *reinterpret_cast<uint4*>(space + kBlockBytes + at) = make_uint4(lo[4 * e], lo[4 * e + 1], lo[4 * e + 2], lo[4 * e + 3]);
-                            }
-                        } else {
-#pragma unroll
-                            for (int j = 0; j < 64; ++j) {
-                                const int at = j * 128 + (((in_row >> 3) ^ (j & 7)) << 4) + (in_row & 7) * 2;
-                                *reinterpret_cast<unsigned short*>(space + at) = (unsigned short)(hi[j >> 1] >> (16 * (j & 1)));
-                                *reinterpret_cast<unsigned short*>(space + kBlockBytes + at) = (unsigned short)(lo[j >> 1] >> (16 * (j & 1)));
-                            }
-                        }
+                    const auto send = [&](char* to) {
                         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                         together();
                         if (sender) {
@@ -641,6 +625,40 @@ muon_product_kernel(const void* plan, const Told told, const Rates r, const Poly
                             asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(to), "r"(smem_u32(space)), "r"(kBlockPair) : "memory");
                             asm volatile("cp.async.bulk.commit_group;" ::: "memory");
                         }
+                    };
+                    const auto free_space = [&] {
+                        if (sender) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+                        together();
+                    };
+                    free_space();
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const int at = in_row * 128 + ((e ^ (in_row & 7)) << 4);
+                        *reinterpret_cast<uint4*>(space + at) = make_uint4(hi[4 * e], hi[4 * e + 1], hi[4 * e + 2], hi[4 * e + 3]);
+                        *reinterpret_cast<uint4*>(space + kBlockBytes + at) = make_uint4(lo[4 * e], lo[4 * e + 1], lo[4 * e + 2], lo[4 * e + 3]);
+                    }
+                    send(planes + ((long long)rb * col_blocks + cb) * kBlockPair);
+                    if (w.phase != MULTIPLY && rb < cb) {
+                        // the block on the other side of the diagonal: 8 x 8 values at a time turned about on the way through registers, half
+                        // of the rows to a warp
+                        unsigned turned[2][8][4];
+                        const unsigned base = smem_u32(space), mine = 4 * (quarter & 1) + (lane >> 3), in = lane & 7;
+#pragma unroll
+                        for (int part = 0; part < 2; ++part)
+#pragma unroll
+                            for (int e = 0; e < 8; ++e)
+                                asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                                             : "=r"(turned[part][e][0]), "=r"(turned[part][e][1]), "=r"(turned[part][e][2]), "=r"(turned[part][e][3])
+                                             : "r"(base + part * kBlockBytes + (8 * mine + in) * 128 + ((e ^ in) << 4)) : "memory");
+                        free_space();
+#pragma unroll
+                        for (int part = 0; part < 2; ++part)
+#pragma unroll
+                            for (int e = 0; e < 8; ++e)
+                                asm volatile("stmatrix.sync.aligned.m8n8.x4.shared.b16 [%4], {%0, %1, %2, %3};"
+                                             ::"r"(turned[part][e][0]), "r"(turned[part][e][1]), "r"(turned[part][e][2]), "r"(turned[part][e][3]),
+                                               "r"(base + part * kBlockBytes + (8 * e + in) * 128 + ((mine ^ in) << 4)) : "memory");
+                        send(planes + ((long long)cb * col_blocks + rb) * kBlockPair);
                     }
                 } else {
                     // the param: 32 x 32 values at a time, a lane to a column; this warp's half of the room
