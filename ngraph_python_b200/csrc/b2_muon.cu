@@ -511,7 +511,17 @@ muon_product_kernel(const void* plan, const Told told, const Rates r, const Poly
         const unsigned lanes = tmem_base + ((unsigned)(quarter * 32) << 16);
         char* space = rooms + pair * 2 * kBlockBytes;           // for both parts of a block
         const bool sender = (quarter & 1) == 0 && lane == 0;
+        // The two warps meet as often as each other whatever becomes of their waits: of items both take the next one or neither, and where
+        // sums did not come they store what they have, which is never said to be stored (of the param nothing).
         const auto together = [&] { asm volatile("bar.sync %0, 64;" ::"r"(1 + pair) : "memory"); };
+        const auto both_warps = [&](bool mine) {
+            unsigned all;
+            asm volatile(
+                "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %2, 0;\n\t"
+                "barrier.cta.red.and.pred q, %1, 64, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+                : "=r"(all) : "r"(1 + pair), "r"((unsigned)mine) : "memory");
+            return all != 0;
+        };
         int q = 0, chain = 0, stored = -1;                      // whose item has been sent, but is not said to be stored
         unsigned queue_parity = 0;
         bool ok = true;
@@ -528,7 +538,7 @@ muon_product_kernel(const void* plan, const Told told, const Rates r, const Poly
         };
         for (;;) {
             if (!__all_sync(0xffffffffu, test_wait(&queue_full[q], queue_parity))) say();
-            if (!mbar_wait_relaxed(&queue_full[q], queue_parity)) { atomicExch(fail_flag, 1); break; }
+            if (!both_warps(mbar_wait_relaxed(&queue_full[q], queue_parity))) { atomicExch(fail_flag, 1); break; }
             const Work w = queue[q];
             __syncwarp();
             if (lane == 0) mbar_arrive(&queue_empty[q]);
@@ -550,7 +560,7 @@ muon_product_kernel(const void* plan, const Told told, const Rates r, const Poly
             for (int kb = 0; kb < w.k_blocks; kb += kChain, ++chain) {
                 if (kb == 2 * kChain) say();
                 const int b = chain & 1;
-                if (ok && !mbar_wait(&sum_full[b], (chain >> 1) & 1)) { atomicExch(fail_flag, 1); ok = false; }
+                if (ok && !__all_sync(0xffffffffu, mbar_wait(&sum_full[b], (chain >> 1) & 1))) { atomicExch(fail_flag, 1); ok = false; }
                 tc_fence_after();
 #pragma unroll
                 for (int c0 = 0; c0 < 128; c0 += 32) {
@@ -611,7 +621,6 @@ muon_product_kernel(const void* plan, const Told told, const Rates r, const Poly
                             if (j == in_row) v[j] += diagonal;
                     }
                 }
-                if (!ok) continue;
                 if (!last) {
                     // both parts, two values to a word, in the place of the values
                     unsigned hi[32], lo[32];
@@ -673,7 +682,7 @@ muon_product_kernel(const void* plan, const Told told, const Rates r, const Poly
 #pragma unroll
                         for (int j = 0; j < 32; ++j) square[lane * 32 + (j ^ lane)] = v[c0 + j];
                         __syncwarp();
-                        const int col = cb * kBlock + c0 + lane, row0 = rb * kBlock + (quarter & 1) * 32, rows = col < t.cols ? min(32, t.rows - row0) : 0;
+                        const int col = cb * kBlock + c0 + lane, row0 = rb * kBlock + (quarter & 1) * 32, rows = ok && col < t.cols ? min(32, t.rows - row0) : 0;
                         float* param = t.param + (long long)row0 * t.cols + col;
 #pragma unroll
                         for (int j0 = 0; j0 < 32; j0 += 16) {
@@ -1091,7 +1100,7 @@ Layout layout_of(const b2_muon_matrix* list, int count) {
     for (size_t from = 0; from < shared; --groups_left) {
         size_t to = from;
         const long long enough = tiles_left / std::max(1ll, groups_left);
-        for (long long tiles = 0; to < shared && (tiles < enough || groups_left <= 1); ++to) {
+        for (long long tiles = 0; to < shared && (to == from || tiles < enough || groups_left <= 1); ++to) {
             tiles += tiles_in(to);
             tiles_left -= tiles_in(to);
         }
