@@ -8,6 +8,12 @@
 // turn that is left, exact but for the rounding of the frequency (2^-45 of a turn at position a million).  In fp32
 // position * frequency would be 0.03 radians off there.  The nearest quarter turn is taken off as an integer and the rest,
 // at most an eighth of a turn, goes into the series of sine and cosine.
+//
+// Bound by memory: 8 bytes a value forward, 12 backward, each tensor read once and its angles worked out from 8 bytes a row.  8192
+// rows, heads of 128: rotation of 16 + 4 heads 28.1 us (168 MB, 6.0 TB/s), norm and rotation of 32 + 8 57.4 (337 MB, 5.9), their
+// gradients 101.9 (505 MB, 5.0), where a copy has 6.55.  A lane takes the same features of several heads, so that the angles, some
+// twenty instructions a pair, are shared by the heads of a row; what is left between this and a copy is instructions (each of four
+// schedulers issues in about half of its cycles, with 8 to 16 warps) and, of gradients, the sums over CTAs in a second launch.
 #include <cmath>
 #include <cstdint>
 #include <type_traits>
@@ -52,7 +58,7 @@ __device__ __forceinline__ bool position_of(const b2_heads& a, long long row, co
 
 // amplitude * (cos, sin) of the fraction of a turn whose 64 bits are `phase`: of what is left of the nearest quarter turn by
 // their series, up to x^9 / 9! and x^10 / 10!, whose next terms are 2e-9 and 5e-10 at an eighth of a turn.  (A third of the
-// instructions of sincospif, which would look for the quarter turn again: the forward pass of 8192 x 40 heads took 70 us with it, 66 so.)
+// instructions of sincospif, which would look for the quarter turn again: the forward pass of 8192 x 40 heads took 70 us with it, 66 without, as the kernel was then.)
 __device__ __forceinline__ float2 turn_of(unsigned long long phase, float amplitude) {
     const unsigned t = (unsigned)(phase >> 32);
     const unsigned quarter = (t + 0x20000000u) >> 30;                                     // 0 ... 4
@@ -211,8 +217,8 @@ struct Deal {
     long long tasks;
 };
 constexpr int kThreads = 256;
-// Heads that a lane loads at once, by how many features of each it holds, and CTAs to an SM.  Eight features, 8192 rows of 40 heads of
-// 128 forward, four heads: 59 us with two CTAs, 63 with three; two heads and four CTAs 72; one and five 85.  Gradients, two heads: 127
+// Heads that a lane loads at once, by how many features of each it holds, and CTAs to an SM (measured without the ring, which made
+// gradients 105 us).  Eight features, 8192 rows of 40 heads of 128 forward, four heads: 59 us with two CTAs, 63 with three; two heads and four CTAs 72; one and five 85.  Gradients, two heads: 127
 // with two, 120 with three; one and three 146.  Rotation alone, 8192 x 20, four heads: 28.5 with three, 33 with two.
 __host__ __device__ constexpr int unrolled(int mode, int values) { return mode == BACKWARD && values >= 8 ? 2 : 4; }
 __host__ __device__ constexpr int blocks_to(int mode, int values) { return values < 8 ? (mode == BACKWARD ? 2 : 3) : mode == ROTATE ? 3 : 2; }
@@ -220,7 +226,8 @@ __host__ __device__ constexpr int blocks_to(int mode, int values) { return value
 constexpr int kAhead = 3;
 __host__ __device__ constexpr bool runs_ahead(int mode, int vec, bool flat) { return mode == BACKWARD && vec == 4 && !flat; }
 __host__ __device__ constexpr int slot_bytes(int mode) { return 32 * 16 * 2 * unrolled(mode, 8) * (mode == BACKWARD ? 2 : 1) + (mode == BACKWARD ? 32 * 4 * unrolled(mode, 8) : 0); }
-// CTAs that stay, and fetch the heads of their next task into L2 meanwhile: gradients 142 us without, 127 with; forward 62 and 59; a
+// CTAs that stay, and fetch the heads of their next task into L2 meanwhile: forward 62 us without, 59 with (gradients 142 and 127, before
+// whole vectors came by way of shared memory); a
 // rotation, which waits for nothing but its loads, 28.5 without and 31 with.
 __host__ __device__ constexpr bool stays(int mode) { return mode != ROTATE; }
 

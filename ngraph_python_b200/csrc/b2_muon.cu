@@ -24,6 +24,11 @@
 // numbers, CTAs take the next number when they are done with one, and an item waits until its matrix has counted the items
 // that it reads.  Only items that a running CTA has taken are waited for, so that it does not matter how many CTAs run.
 // With a launch for each product the last wave of tiles of every one of 15 would leave SMs idle.
+//
+// 48 matrices of 12 layers of 640 (59 million values): 2.9 ms in a loop, where power caps the clock, 2.5 alone; the 16-bit products
+// by themselves would take 1.14 at the rate of a large product, 1.35 at its sustained one.  A tile of 256 columns keeps shared memory busy for
+// 1875 of the 1960 cycles of a block of k (144 KB read by the tensor core, 96 KB written by the copies, 128 bytes a cycle); what comes
+// on top is the storing of tiles, some 5000 cycles after ten blocks of k, which the next tile's first two blocks hide in part.
 #include <algorithm>
 #include <cmath>
 #include <cstdint>
