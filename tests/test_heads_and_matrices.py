@@ -379,3 +379,59 @@ def test_a_training_step_of_them_all():
         if step == 1:
             comp.capture()
     t.close()
+
+
+@pytest.mark.gpu
+def test_one_operand_twice_and_gradients_that_are_broadcast():
+    """Both tensors of heads are one placeholder with one weight, the results' gradients are the same for all rows or for all heads and
+    features, and one position is everybody's."""
+    T, H, D = _axes(T=333, H=3, D=16)
+    rng = np.random.RandomState(8)
+    x, at, by_feature, by_row = ng.placeholder([T, H, D]), ng.placeholder([]), ng.placeholder([D]), ng.placeholder([T])
+    weight = (1 + 0.3 * rng.standard_normal(16)).astype(np.float32)
+    w = ng.variable([D], initial_value=weight)
+    out = ng.head_norm([x, x], [w, w], heads=[H, H], features=D, rotation=ng.Rotation(at))
+    g = ng.head_norm_grad([ng.broadcast(by_feature, [T, H, D]), ng.broadcast(by_row, [T, H, D])], out)
+    t = _transformer()
+    comp = t.computation(out + g["x"] + g["weight"], x, at, by_feature, by_row)
+    for recorded in (False, True):
+        v, d0, d1, p = [rng.standard_normal(s).astype(np.float32) for s in ((333, 3, 16), (16,), (333,))] + [int(rng.randint(9999))]
+        got = comp(v, p, d0, d1)
+        angle = p * ho.frequencies(16)[None, :] + np.zeros((333, 1))
+        want, rstd, size = ho.forward(v, weight, 1e-6, angle, 16, False, 1.0)
+        for i, delta in enumerate((np.broadcast_to(d0, v.shape), np.broadcast_to(d1[:, None, None], v.shape))):
+            _far(got[i], want, size, 30)
+            dx, dw, dx_size, dw_size = ho.backward(delta, v, weight, rstd, angle, 16, False, 1.0)
+            _far(got[2 + i], dx, dx_size, 70)
+            _far(got[4 + i], dw, dw_size, 200)
+        if not recorded:
+            comp.capture()
+    t.close()
+
+
+@pytest.mark.gpu
+def test_one_gradient_of_two_matrices_and_one_step_of_two_computations():
+    """Two variables follow one gradient; computations that share the step, one of them recorded, go on from one another's state."""
+    A, B = _axes(A=100, B=150)
+    rng = np.random.RandomState(9)
+    start = [(rng.standard_normal((100, 150)) * 0.1).astype(np.float32) for _ in range(2)]
+    g = ng.placeholder([A, B])
+    ws = [ng.variable([A, B], initial_value=s) for s in start]
+    step = ng.muon(ws, [g, g], lr=0.05, nesterov=True)
+    t = _transformer()
+    one, two = t.computation(step, g), t.computation([step, ng.sum(g, out_axes=[])], g)
+    values, mean = [s.copy() for s in start], np.zeros((100, 150))
+    for k in range(4):
+        grad = rng.standard_normal((100, 150)).astype(np.float32)
+        got = two(grad)[0] if k % 2 else one(grad)
+        assert float(np.asarray(got).reshape(-1)[0]) == k + 1
+        for i, w in enumerate(ws):
+            want, m, far = _moved(values[i], mean, grad, 0.05, 1.0)
+            held = np.array(t.device_tensor(w).get(None))
+            assert np.sqrt(np.sum((held - want) ** 2)) <= far
+            values[i] = held
+        mean = np.array(t.device_tensor(step.states[0]).get(None))
+        assert np.array_equal(mean, np.array(t.device_tensor(step.states[1]).get(None)))
+        if k == 1:
+            two.capture()
+    t.close()
