@@ -734,7 +734,7 @@ Rows heads_at(const void* p, const b2_heads& a, int heads, int64_t row, int64_t 
     return value_bytes == 2 ? heads_at(static_cast<const short*>(p), a, heads, row, head) : heads_at(static_cast<const float*>(p), a, heads, row, head);
 }
 Rows positions_at(const b2_heads& a) {
-    if (a.rotary_dim == 0 || !a.positions) return rows_at((const char*)nullptr, 0, 0, 0);
+    if (a.rotary_dim == 0 || !a.positions || a.rows == 0) return rows_at((const char*)nullptr, 0, 0, 0);
     const long long groups = (a.rows + a.position_group - 1) / a.position_group, count = a.position_count < groups ? a.position_count : groups;
     const long long bytes = count * (a.position_kind == B2_IDX_I64 ? 8 : a.position_kind == B2_IDX_FLEX16 ? 2 : 4);
     return rows_at(static_cast<const char*>(a.positions), 1, bytes, bytes);

@@ -68,7 +68,7 @@ template <typename T>
 inline Rows rows_at(const T* p, long long rows, long long width, long long stride) {
     const long long size = sizeof(T);
     const uintptr_t at = (uintptr_t)p;
-    if (!p || rows <= 0) return {0, 0, 0, 0, 0};
+    if (!p || rows <= 0 || width <= 0) return {0, 0, 0, 0, 0};
     if (rows == 1 || stride == width) return {at, at + size * rows * width, 1, size * rows * width, size * rows * width};
     return {at, at + size * ((rows - 1) * stride + width), rows, size * width, size * stride};
 }
