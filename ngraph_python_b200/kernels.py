@@ -1190,14 +1190,14 @@ class RotaryStep(_Step):
         p.heads, p.x, p.out = op.head_axes.size, self._ptr(xv), self._ptr(ov)
         (p.x_row, p.x_head), (p.out_row, p.out_head) = heads_of(xv, op.axes, apart), heads_of(ov, op.axes, apart)
         if len(self.in_views) > 1:
-            a.positions, a.position_kind = self._ptr(self.in_views[1]), lib.IDX_FLEX16 if self.flex else lib.IDX_F32
+            a.positions, a.position_kind = self._ptr(self.in_views[1]), lib.IDX_FLEX16 if self.in_views[1].buffer.flex else lib.IDX_F32
         raw, st = lib.raw(), t.stream.cuda_stream
         if not self.flex:
             lib.check(raw.b2_rotary(C.byref(a), 0, None, None, None, 0, st))
             t.kernel_launches += 1
             return
         p.slot_x, p.slot_out = t._slot_for_read(xv.buffer, self), ov.buffer.slot_write
-        if len(self.in_views) > 1:
+        if a.position_kind == lib.IDX_FLEX16:
             a.slot_positions = t._slot_for_read(self.in_views[1].buffer, self)
 
         def call(probe):

@@ -930,7 +930,9 @@ def residual_norm_grad(fprop, d_out=None, d_stream=None):
 
 class Rotation(object):
     """How heads are rotated by position.  positions: an op over axes of the heads' rows that lie next to one another, or one of
-    these axes, whose indices are the positions then.  Pairs of the first rotary_dim features (None: all) -- pairs "halves" or
+    these axes, whose indices are the positions then.  Positions of an op are what its tensor holds: whole numbers to 2^24 in fp32, which
+    in a flex16 transformer is the type of a placeholder that nothing but rotations reads; other flex16 tensors end at 32767, and at
+    what the exponent of their earlier values lets them hold.  Pairs of the first rotary_dim features (None: all) -- pairs "halves" or
     "neighbours" -- turn by position * frequency, and are multiplied by amplitude.  Frequencies are base^(-2 i / rotary_dim), for
     contexts `factor` times as long as the `original` one: scaling "linear" divides all, "base" takes a larger base, "parts" divides
     those that turn less than `low` times over the original context and keeps those that turn more than `high` times."""

@@ -1870,6 +1870,7 @@ class B200Transformer(object):
         # is taken from the register; flex16: re-quantised as the store quantises it)
         self.forward_inplace = bool(kwargs.pop("forward_inplace", True))
         self.flex = bool(flex)
+        self._fp32_tensors = ()     # (of a flex transformer)
         self.fixed_point = bool(fixed_point)
         self.flex_manager = flexmod.FlexManager(fixed_point=fixed_point, verbose=flex_verbose)
         self.computations = []
@@ -1948,8 +1949,24 @@ class B200Transformer(object):
         if self.finalized:
             return
         self.finalized = True
+        if self.flex:
+            self._fp32_tensors = self._position_arguments()
         for c in self.computations:
             c.build()
+
+    def _position_arguments(self):
+        """Placeholders that nothing but rotations read, as positions: held in fp32, where every whole number to 2^24 is what it
+        is.  A flex16 tensor's exponent follows the values of earlier calls, and a position that outgrows it is another one."""
+        as_position = collections.defaultdict(list)
+        for c in self.computations:
+            for op in c._ordered_ops():
+                if isinstance(op, (ViewOp, SequentialOp)):
+                    continue
+                for i, a in enumerate(op.args):
+                    while isinstance(a, (ViewOp, SequentialOp)):
+                        a = a.value_tensor if isinstance(a, SequentialOp) else a.args[0]
+                    as_position[a].append(isinstance(op, RotaryOp) and i == 1)
+        return set(a for a, found in as_position.items() if isinstance(a, AssignableTensorOp) and a.is_placeholder and all(found))
 
     def _collect_trace(self, comp, pairs):
         """After the call's synchronisation: one 'X' event per step (device time, microseconds
@@ -1988,10 +2005,10 @@ class B200Transformer(object):
         b = self._buffers.get(op)
         if b is None:
             persistent = isinstance(op, AssignableTensorOp)
-            b = Buffer(op.name, op.axes, self.flex, persistent)
+            b = Buffer(op.name, op.axes, self.flex and op not in self._fp32_tensors, persistent)
             if persistent:
                 b.init_array = op.initial_array()
-            if self.flex:
+            if b.flex:
                 b.entry = self.flex_manager.make_flex_entry(op.name)
                 b.slot = self.flex_manager.new_slot()
                 b.slot_write = b.slot
