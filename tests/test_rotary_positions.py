@@ -66,7 +66,7 @@ def test_positions_that_outgrow_the_first_calls_in_flex16(pairs, order):
         p.flat[-1] = max(most - 1, 0)
         given = torch.from_numpy(p).cuda() if call % 2 else p
         out = comp(v, given)
-        rows = dict(T=np.broadcast_to(p, (2, 9)), BT=p, TB=p.T)[order]
+        rows = p.T if order == "TB" else np.broadcast_to(p, (2, 9))
         angle = rows.reshape(18)[:, None].astype(np.float64) * ho.frequencies(16, base=100000.0)
         want, _ = ho.rotate(v.reshape(18, 3, 16), angle, 16, pairs == "neighbours")
         assert np.abs(out.reshape(18, 3, 16) - want).max() <= 2 * 2.0 ** -14 + 2.0 ** -13, (call, most)
