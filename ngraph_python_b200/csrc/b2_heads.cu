@@ -723,12 +723,19 @@ template <typename T>
 Rows heads_at(const T* p, const b2_heads& a, int heads, int64_t row, int64_t head) {
     const long long R = a.rows, D = a.head_dim;
     if (!p || R == 0 || heads == 0) return rows_at(p, 0, 1, 1);
-    if (heads == 1) return row >= D || R == 1 ? rows_at(p, R, D, row) : rows_at(p, 1, (R - 1) * row + D, D);
-    if (R == 1) return head >= D ? rows_at(p, heads, D, head) : rows_at(p, 1, (heads - 1) * head + D, D);
-    if (head >= D && row == heads * head) return rows_at(p, R * heads, D, head);
-    if (row >= (heads - 1) * head + D) return rows_at(p, R, (heads - 1) * head + D, row);
-    if (head >= (R - 1) * row + D) return rows_at(p, heads, (R - 1) * row + D, head);
-    return rows_at(p, 1, (R - 1) * row + (heads - 1) * head + D, D);
+    Rows found = heads == 1                             ? row >= D || R == 1 ? rows_at(p, R, D, row) : rows_at(p, 1, (R - 1) * row + D, D)
+                 : R == 1                               ? head >= D ? rows_at(p, heads, D, head) : rows_at(p, 1, (heads - 1) * head + D, D)
+                 : head >= D && row == heads * head     ? rows_at(p, R * heads, D, head)
+                 : row >= (heads - 1) * head + D        ? rows_at(p, R, (heads - 1) * head + D, row)
+                 : head >= (R - 1) * row + D            ? rows_at(p, heads, (R - 1) * row + D, head)
+                                                        : rows_at(p, 1, (R - 1) * row + (heads - 1) * head + D, D);
+    if (R > 1 && row == 0) return found;                // (one row for all)
+    found.at_rows = R;
+    found.at_heads = heads;
+    found.row_stride = row * (long long)sizeof(T);
+    found.head_stride = head * (long long)sizeof(T);
+    found.head_width = D * (long long)sizeof(T);
+    return found;
 }
 Rows heads_at(const void* p, const b2_heads& a, int heads, int64_t row, int64_t head, int value_bytes) {
     return value_bytes == 2 ? heads_at(static_cast<const short*>(p), a, heads, row, head) : heads_at(static_cast<const float*>(p), a, heads, row, head);

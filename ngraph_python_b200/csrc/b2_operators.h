@@ -63,6 +63,8 @@ inline int allow_shared(const void* kernel, int bytes, std::atomic<unsigned long
 struct Rows {
     uintptr_t p, end;
     long long rows, width, stride;
+    // of tensors of heads the heads themselves: `at_rows` x `at_heads` of `head_width` bytes (0: no such tensor)
+    long long at_rows = 0, at_heads = 0, row_stride = 0, head_stride = 0, head_width = 0;
 };
 template <typename T>
 inline Rows rows_at(const T* p, long long rows, long long width, long long stride) {
@@ -73,11 +75,22 @@ inline Rows rows_at(const T* p, long long rows, long long width, long long strid
     return {at, at + size * ((rows - 1) * stride + width), rows, size * width, size * stride};
 }
 
-// Whether two tensors that lie among one another have memory in common.  Their rows may lie side by side.
+// Whether two tensors that lie among one another have memory in common.  Their rows may lie side by side, and heads of one between
+// those of the other.
 inline bool meet(Rows a, Rows b) {
     if (a.rows > b.rows) std::swap(a, b);
     const long long ahead = (long long)b.p - (long long)a.p;     // where b begins, seen from a
     const auto below = [](long long x, long long y) { return x / y - (x % y < 0); };
+    const auto alike = [](long long x, long long y, long long of_x, long long of_y) { return x == 1 || y == 1 || of_x == of_y; };
+    if (a.at_heads && b.at_heads && alike(a.at_rows, b.at_rows, a.row_stride, b.row_stride) && alike(a.at_heads, b.at_heads, a.head_stride, b.head_stride)) {
+        // as for rows below, at every distance that two heads have
+        const long long by_row = a.at_rows > 1 ? a.row_stride : b.at_rows > 1 ? b.row_stride : 1, by_head = a.at_heads > 1 ? a.head_stride : b.head_stride;
+        for (long long e = 1 - b.at_heads; e < a.at_heads; ++e) {
+            const long long from = ahead - e * by_head, least = below(from - a.head_width, by_row) + 1, d = least > 1 - b.at_rows ? least : 1 - b.at_rows;
+            if (d < a.at_rows && d * by_row < from + b.head_width) return true;
+        }
+        return false;
+    }
     if (a.stride == b.stride) {
         // row i of a and row j of b meet where (i - j) stride lies between ahead - a.width and ahead + b.width
         const long long least = below(ahead - a.width, a.stride) + 1, d = least > 1 - b.rows ? least : 1 - b.rows;
