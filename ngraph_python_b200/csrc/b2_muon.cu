@@ -212,6 +212,14 @@ muon_mean_kernel(const void* plan, const Told told, const Rates r, const float* 
     }
 }
 
+// What u is multiplied by, one factor behind the other, for u * up / norm.  A norm of fp32 values may be more or less than fp32 holds,
+// and so may its reciprocal: the first factor takes u by a power of two to where neither is.
+__device__ __forceinline__ float2 over_norm(double norm, float up) {
+    const int e = ((__double2hiint(norm) >> 20) & 0x7ff) - 1023;
+    const int first = e > 100 ? -100 : e < -100 ? 100 : 0;
+    return make_float2(power(first), (float)((double)up * (double)power(-first) / norm));
+}
+
 // Two values as two fp16 parts each
 __device__ __forceinline__ void parts(float u, float v, unsigned& hi, unsigned& lo) {
     const __half2 h = __floats2half2_rn(u, v);
@@ -238,9 +246,9 @@ muon_parts_kernel(const void* plan, const Told told, const Rates r, const float*
     __shared__ double words[kMeanThreads / 32];
     after_earlier_kernels();
     if (!fits(plan, told)) return;
-    const float s = grad_scale ? *grad_scale : 1.0f, up = power(exponent);
+    const float s = grad_scale ? *grad_scale : 1.0f;
     const long long run = (told.blocks + gridDim.x - 1) / gridDim.x, end = min((blockIdx.x + 1) * run, told.blocks);
-    float inverse = 0.0f;
+    float2 factors = make_float2(0.0f, 0.0f);
     int matrix = -1;
     for (long long k = blockIdx.x * run; k < end; ++k) {
         const Block c = blocks_of(plan)[k];
@@ -248,7 +256,7 @@ muon_parts_kernel(const void* plan, const Told told, const Rates r, const float*
         if (c.matrix != matrix) {
             double q = 0.0;
             for (int i = threadIdx.x; i < t.chunks; i += kMeanThreads) q += room.sums[t.first_chunk + i];
-            inverse = (float)(1.0 / (sqrt(cta_sum<kMeanThreads>(q, words)) + (double)r.eps));
+            factors = over_norm(sqrt(cta_sum<kMeanThreads>(q, words)) + (double)r.eps, power(exponent));
             matrix = c.matrix;
         }
         const int rb = c.at / t.col_blocks, cb = c.at - rb * t.col_blocks;
@@ -287,9 +295,9 @@ muon_parts_kernel(const void* plan, const Told told, const Rates r, const float*
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const float u = r.nesterov ? r.rest * (g[e][j] * s) + r.mu * m[e][j] : m[e][j];
-                m[e][j] = u * inverse * up;
+                m[e][j] = u * factors.x * factors.y;
             }
-            // (what lies outside the matrix is zero, whatever `inverse` is)
+            // (what lies outside the matrix is zero, whatever the factors are)
             const int at_row = rb * kBlock + (threadIdx.x >> 3) + e * (kMeanThreads / 8), there = at_row < t.rows ? t.cols - at_col : 0;
 #pragma unroll
             for (int j = 0; j < 8; ++j) m[e][j] = j < there ? m[e][j] : 0.0f;
@@ -904,7 +912,7 @@ muon_solo_kernel(const void* plan, const Told told, const Rates r, const Poly po
                  put(t.mean + i, v[1], count);
              });
         q = cta_sum<kSoloThreads>(q, words);
-        const float inverse = (float)(1.0 / (sqrt(q) + (double)r.eps)), up = power(poly.x[0]);
+        const float2 factors = over_norm(sqrt(q) + (double)r.eps, power(poly.x[0]));
         // x in parts, four blocks at a time: a thread to eight values next to one another of each
         for (int b0 = 0; b0 < across * along; b0 += 4) {
             const int in_row = threadIdx.x >> 3, piece = threadIdx.x & 7;
@@ -916,7 +924,7 @@ muon_solo_kernel(const void* plan, const Told told, const Rates r, const Poly po
                 const float4 first = *reinterpret_cast<const float4*>(value_at(i, j)), second = *reinterpret_cast<const float4*>(value_at(i, j + 4));
                 const float w[8] = {first.x, first.y, first.z, first.w, second.x, second.y, second.z, second.w};
 #pragma unroll
-                for (int e = 0; e < 8; ++e) v[b][e] = w[e] * inverse * up;
+                for (int e = 0; e < 8; ++e) v[b][e] = w[e] * factors.x * factors.y;
             }
             __syncthreads();
 #pragma unroll
