@@ -759,7 +759,11 @@ typedef struct {
     size_t plan_bytes, scratch_bytes;
     int64_t matrices, chunks, items, blocks, solos;
 } b2_muon_sizes;
+typedef struct { int64_t groups, tiles[3][4]; } b2_muon_tiles;
 int b2_muon_plan_sizes(const b2_muon_matrix* matrices, int32_t count, b2_muon_sizes* sizes);
+/* What a step is cut into: groups of matrices that run next to one another, and the tiles of 128 rows of A, of B and of x by their
+ * width, 64 to 256 columns (of one step's products; those of small matrices, which have a CTA each, are not cut). */
+int b2_muon_plan_tiles(const b2_muon_matrix* matrices, int32_t count, b2_muon_tiles* tiles);
 int b2_muon_launches(const b2_muon_sizes* sizes, int32_t* launches);     /* kernels that a step launches */
 int b2_muon_plan(const b2_muon_matrix* matrices, int32_t count, void* plan, size_t plan_bytes, void* stream);
 int b2_muon_step(void* plan, const b2_muon_sizes* sizes, const b2_muon_hyper* hyper, const float* lr, const float* grad_scale,

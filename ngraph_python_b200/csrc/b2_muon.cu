@@ -1294,6 +1294,20 @@ extern "C" int b2_muon_plan_sizes(const b2_muon_matrix* list, int32_t count, b2_
     }
 }
 
+extern "C" int b2_muon_plan_tiles(const b2_muon_matrix* list, int32_t count, b2_muon_tiles* tiles) {
+    B2_REQUIRE(tiles, "missing argument");
+    B2_CHECK(check_matrices(list, count));
+    try {
+        const Layout l = layout_of(list, count);
+        *tiles = {};
+        tiles->groups = (int64_t)l.groups.size();
+        for (const Item& item : l.items) ++tiles->tiles[item.phase][item.width - 1];
+    } catch (const std::bad_alloc&) {
+        return b2::fail(B2_ERR_INVALID, "no memory for a plan of %d matrices", count);
+    }
+    return B2_OK;
+}
+
 extern "C" int b2_muon_launches(const b2_muon_sizes* s, int32_t* launches) {
     B2_REQUIRE(s && launches, "missing argument");
     *launches = (s->items > 0 ? 3 : 0) + (s->solos > 0 ? 1 : 0);

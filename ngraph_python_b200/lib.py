@@ -175,6 +175,10 @@ class MuonSizes(C.Structure):
                 ("items", C.c_int64), ("blocks", C.c_int64), ("solos", C.c_int64)]
 
 
+class MuonTiles(C.Structure):
+    _fields_ = [("groups", C.c_int64), ("tiles", (C.c_int64 * 4) * 3)]
+
+
 class CallArg(C.Structure):
     _fields_ = [("src", C.c_void_p), ("inv_scale", C.c_float), ("in_place", C.c_int32)]
 
@@ -299,6 +303,7 @@ def _load():
         "b2_adamw_plan": (C.c_int, [C.POINTER(AdamwTensor), i32, i32, vp, sz, vp]),
         "b2_adamw_step": (C.c_int, [vp, i64, i32, C.POINTER(AdamwHyper), vp, vp, vp, C.c_uint32, vp]),
         "b2_muon_plan_sizes": (C.c_int, [C.POINTER(MuonMatrix), i32, C.POINTER(MuonSizes)]),
+        "b2_muon_plan_tiles": (C.c_int, [C.POINTER(MuonMatrix), i32, C.POINTER(MuonTiles)]),
         "b2_muon_launches": (C.c_int, [C.POINTER(MuonSizes), C.POINTER(i32)]),
         "b2_muon_plan": (C.c_int, [C.POINTER(MuonMatrix), i32, vp, sz, vp]),
         "b2_muon_step": (C.c_int, [vp, C.POINTER(MuonSizes), C.POINTER(MuonHyper), vp, vp, vp, vp, sz, vp, vp]),
@@ -663,6 +668,13 @@ def muon_plan_sizes(matrices):
     out = MuonSizes()
     check(_lib.b2_muon_plan_sizes(matrices, len(matrices), C.byref(out)))
     return out
+
+
+def muon_plan_tiles(matrices):
+    """(groups of matrices, [[tiles of 64, 128, 192, 256 columns] of A, of B, of x]) of a step over `matrices`."""
+    out = MuonTiles()
+    check(_lib.b2_muon_plan_tiles(matrices, len(matrices), C.byref(out)))
+    return out.groups, [list(t) for t in out.tiles]
 
 
 def muon_launches(sizes):
