@@ -1366,6 +1366,12 @@ extern "C" int b2_muon_step(void* plan, const b2_muon_sizes* s, const b2_muon_hy
                h->steps, h->a, h->b, h->c);
     B2_REQUIRE((((uintptr_t)lr | (uintptr_t)grad_scale | (uintptr_t)step | (uintptr_t)status) & 3) == 0, "a number of the step lies between two addresses");
     B2_REQUIRE(!b2::overlap(plan, s->plan_bytes, scratch, s->scratch_bytes), "the plan lies in the scratch");
+    for (const void* number : {(const void*)lr, (const void*)grad_scale, (const void*)step, (const void*)status})
+        B2_REQUIRE(!b2::overlap(number, 4, plan, s->plan_bytes) && !b2::overlap(number, 4, scratch, s->scratch_bytes),
+                   "a number of the step lies in the plan or the scratch");
+    for (const void* number : {(const void*)lr, (const void*)grad_scale, (const void*)status})
+        B2_REQUIRE(!b2::overlap(step, 4, number, 4), "the number of the step lies in the place of another");
+    B2_REQUIRE(!b2::overlap(status, 4, lr, 4) && !b2::overlap(status, 4, grad_scale, 4), "the status lies in the place of a number of the step");
     b2::Memory memory;
     B2_CHECK(memory.find_device());
     B2_CHECK(memory.written(plan, "the plan"));

@@ -1,9 +1,12 @@
-"""Orthogonalised updates of gradients whose norm, or its reciprocal, is no fp32 number."""
+"""Orthogonalised updates of gradients whose norm, or its reciprocal, is no fp32 number, and where the numbers of a step may lie."""
+import ctypes
+
 import numpy as np
 import pytest
 
+from ngraph_python_b200 import lib
 from oracle import muon_oracle as mo
-from tests.test_muon_operator import HALF, _Step
+from tests.test_muon_operator import HALF, STEP, _Step
 
 
 @pytest.mark.gpu
@@ -33,3 +36,27 @@ def test_norms_beyond_fp32(r, c):
     limit = 4 * plain + 8 * HALF * np.sqrt(np.sum(want ** 2))
     for s, g in zip(sizes, got):
         assert np.sqrt(np.sum((g + want) ** 2)) <= limit, (s, np.sqrt(np.sum((g + want) ** 2)), limit)
+
+
+def test_numbers_in_the_memory_of_a_step_are_refused():
+    """The rate, the scale, the count and the status: none in the plan or the scratch, which the step writes, and what is written not
+    in the place of another."""
+    m = (lib.MuonMatrix * 1)()
+    m[0].param, m[0].grad, m[0].mean, m[0].rows, m[0].cols, m[0].decay, m[0].scale = 1 << 20, 2 << 20, 3 << 20, 200, 300, 1.0, 1.0
+    sizes, h = lib.muon_plan_sizes(m), lib.MuonHyper(**STEP)
+    plan, scratch, apart = 1 << 33, 1 << 34, [(1 << 35) + 256 * i for i in range(4)]
+
+    def said(*numbers):
+        rc = lib.raw().b2_muon_step(plan, ctypes.byref(sizes), ctypes.byref(h), *numbers[:3], scratch, sizes.scratch_bytes, numbers[3], None)
+        return lib.raw().b2_last_error().decode() if rc == -1 else ""
+    assert "lies in" not in said(*apart)
+    for i in range(4):
+        for place in (plan, plan + sizes.plan_bytes - 4, scratch, scratch + sizes.scratch_bytes - 4):
+            assert "in the plan or the scratch" in said(*(apart[:i] + [place] + apart[i + 1:])), i
+        for place in (plan - 4, plan + (sizes.plan_bytes + 3) // 4 * 4, scratch - 4, scratch + (sizes.scratch_bytes + 3) // 4 * 4):
+            assert "lies in" not in said(*(apart[:i] + [place] + apart[i + 1:])), i
+    for i, j in ((0, 2), (1, 2), (2, 3), (0, 3), (1, 3)):
+        numbers = list(apart)
+        numbers[j] = numbers[i]
+        assert "in the place of" in said(*numbers), (i, j)
+    assert "lies in" not in said(apart[0], apart[0], apart[2], apart[3])        # (one number for both that are only read)
