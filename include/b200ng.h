@@ -641,7 +641,8 @@ int b2_norm_bprop(const b2_norm* norm, const b2_norm_grads* grads, void* scratch
  * i + rotary_dim / 2, or 2 i and 2 i + 1 where `interleaved` -- turn as one complex number:
  *   z_i -> amplitude * z_i * exp(2 pi sqrt(-1) * position * turns[i] / 2^64)
  * `inverse` turns back, which is the gradient.  The other features pass through.  turns[i] is a frequency in 2^-64 of a
- * turn, so that position * turns[i], modulo 2^64, is the angle of any position up to 2^-65 of a turn times the position.
+ * turn, so that position * turns[i], modulo 2^64, is the angle of any position, off by what the frequency is, 2^-61 of a turn at
+ * most (b2_rotary_turns), times the position.
  * Row r has the position positions[(r / position_group) % position_count] (position_kind: B2_IDX_*; fp32 and flex16 to the
  * nearest whole number; NaN and what 64 bits do not hold make the row's rotated features NaN, in flex16 zero), or that index
  * itself where `positions` is NULL.

@@ -5,7 +5,7 @@
 //   gradients  d = rotated back(dy),  dw = sum over rows and heads of d x^,  dx = rstd (w d - x^ mean(w d x^))
 //
 // Angles: a frequency is a 64-bit fraction of a turn, so that the product with a position, modulo 2^64, is the fraction of a
-// turn that is left, exact but for the rounding of the frequency (2^-45 of a turn at position a million).  In fp32
+// turn that is left, exact but for the frequency, which is good to 2^-61 of a turn (2^-41 at position a million).  In fp32
 // position * frequency would be 0.03 radians off there.  The nearest quarter turn is taken off as an integer and the rest,
 // at most an eighth of a turn, goes into the series of sine and cosine.
 //
@@ -16,6 +16,7 @@
 // schedulers issues in about half of its cycles, with 8 to 16 warps) and, of gradients, the sums over CTAs in a second launch.
 #include <cmath>
 #include <cstdint>
+#include <limits>
 #include <type_traits>
 
 #include "b2_operators.h"
@@ -894,21 +895,24 @@ extern "C" int b2_rotary_turns(int32_t rotary_dim, double base, int32_t scaling,
     B2_REQUIRE(scaling == B2_ROTARY_PLAIN || (std::isfinite(factor) && factor > 0.0), "bad factor: %g", factor);
     B2_REQUIRE(scaling != B2_ROTARY_PARTS || (std::isfinite(original) && original > 0.0 && std::isfinite(low) && std::isfinite(high) && low < high),
                "bad parts: context %g, from %g to %g turns", original, low, high);
-    const double d = rotary_dim, circle = 6.283185307179586476925;
-    if (scaling == B2_ROTARY_BASE && rotary_dim > 2) base *= std::pow(factor, d / (d - 2));
+    // (64 bits of a fraction want a significand of 64 bits: angles by frequencies of doubles are off by 2^-36 of a turn at position a million)
+    static_assert(std::numeric_limits<long double>::digits >= 64, "frequencies have 64 bits");
+    const long double d = rotary_dim, circle = 6.28318530717958647692528676655900577L, by = factor;
+    long double from = base;
+    if (scaling == B2_ROTARY_BASE && rotary_dim > 2) from *= std::pow(by, d / (d - 2));
     for (int i = 0; i < rotary_dim / 2; ++i) {
-        double f = std::pow(base, -2.0 * i / d) / circle;           // turns a position
-        if (scaling == B2_ROTARY_LINEAR) f /= factor;
+        long double f = std::pow(from, -2.0L * i / d) / circle;     // turns a position
+        if (scaling == B2_ROTARY_LINEAR) f /= by;
         if (scaling == B2_ROTARY_PARTS) {
-            double keep = (original * f - low) / (high - low);
-            keep = keep < 0.0 ? 0.0 : keep > 1.0 ? 1.0 : keep;
-            f = keep * f + (1.0 - keep) * f / factor;
+            long double keep = (original * f - low) / ((long double)high - low);
+            keep = keep < 0.0L ? 0.0L : keep > 1.0L ? 1.0L : keep;
+            f = keep * f + (1.0L - keep) * f / by;
         }
-        B2_REQUIRE(std::isfinite(f), "frequency %d is not finite", i);
+        B2_REQUIRE(std::isfinite((double)f), "frequency %d is not finite", i);
         f -= std::floor(f);
-        // (a double just below one may round to a whole turn)
-        const double whole = std::nearbyint(f * 18446744073709551616.0);
-        turns[i] = whole >= 18446744073709551616.0 ? 0 : (uint64_t)whole;
+        // (a value just below one may round to a whole turn)
+        const long double whole = std::nearbyint(f * 18446744073709551616.0L);
+        turns[i] = whole >= 18446744073709551616.0L ? 0 : (uint64_t)whole;
     }
     return B2_OK;
 }

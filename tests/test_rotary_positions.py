@@ -1,7 +1,8 @@
-"""Positions of rotations whose values go beyond those of earlier calls, in a flex16 transformer, and beyond what other types name."""
+"""Positions of rotations whose values go beyond those of earlier calls, in a flex16 transformer, and frequencies to the last bit."""
 import numpy as np
 import pytest
 
+from ngraph_python_b200 import lib
 from ngraph_python_b200 import op_graph as ng
 from ngraph_python_b200.transformers import make_transformer_factory
 from oracle import heads_oracle as ho
@@ -73,3 +74,40 @@ def test_positions_that_outgrow_the_first_calls_in_flex16(pairs, order):
         if call == 2:
             comp.capture()
     t.close()
+
+
+PI = "3.14159265358979323846264338327950288419716939937510582097494459230781640628620899862803"
+
+
+def _exact_turns(d, base=10000.0, scaling="none", factor=1.0, original=1.0, low=1.0, high=32.0):
+    """Turns a position of each pair, in 80 digits."""
+    import decimal
+    with decimal.localcontext(decimal.Context(prec=80)):
+        D = decimal.Decimal
+        base, factor, original, low, high, found = D(base), D(factor), D(original), D(low), D(high), []
+        if scaling == "base" and d > 2:
+            base = base * factor ** (D(d) / D(d - 2))
+        for i in range(d // 2):
+            f = base ** (D(-2 * i) / D(d)) / (2 * D(PI))
+            if scaling == "linear":
+                f /= factor
+            if scaling == "parts":
+                keep = min(max((original * f - low) / (high - low), D(0)), D(1))
+                f = keep * f + (1 - keep) * f / factor
+            found.append(f)
+        return [int((f % 1 * 2 ** 64).to_integral_value()) for f in found], [float(f) for f in found]
+
+
+@pytest.mark.parametrize("d", [2, 6, 40, 128, 256, 1024])
+@pytest.mark.parametrize("scaling", ["none", "linear", "base", "parts"])
+@pytest.mark.parametrize("base", [500.0, 10000.0, 1e6, 0.25])
+def test_frequencies_to_64_bits(d, scaling, base):
+    """A fraction of a turn is rounded to 2^-64 of one (half a step), and the operations before it round to 64 bits each: a power by a
+    step (2^-63 of itself), its exponent by half a step times the logarithm of the base, the others by half a step.  With
+    up to eight of them, and a power and a logarithm of 14 within one, that is 2^-59 of a frequency."""
+    kw = dict(base=base, scaling=scaling, factor=8.0, original=300.0, low=1.0, high=20.0)
+    want, size = _exact_turns(d, **kw)
+    got = [int(v) for v in lib.rotary_turns(d, **kw).numpy().view(np.uint64)]
+    for g, w, f in zip(got, want, size):
+        off = (g - w + (1 << 63)) % (1 << 64) - (1 << 63)
+        assert abs(off) <= 1 + f * 2.0 ** 5, (off, f)
