@@ -52,7 +52,7 @@ __device__ __forceinline__ bool position_of(const b2_heads& a, long long row, co
             const float x = a.position_kind == B2_IDX_F32 ? static_cast<const float*>(a.positions)[i]
                                                           : scales[a.slot_positions].scale * (float)static_cast<const short*>(a.positions)[i];
             at = __float2ll_rn(x);
-            return fabsf(x) < 9.2e18f;          // (false for NaN)
+            return x >= -0x1p63f && x < 0x1p63f;        // (false for NaN)
         }
     }
 }

@@ -111,3 +111,25 @@ def test_frequencies_to_64_bits(d, scaling, base):
     for g, w, f in zip(got, want, size):
         off = (g - w + (1 << 63)) % (1 << 64) - (1 << 63)
         assert abs(off) <= 1 + f * 2.0 ** 5, (off, f)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 21, 520])
+def test_the_largest_fp32_positions_that_64_bits_hold(D):
+    """Whole numbers up to the last fp32 value below 2^63, and -2^63 itself; beyond, a rotation is NaN.  (Off as any rotation is.)"""
+    import ctypes
+    import torch
+    p = np.array([np.nextafter(np.float32(2.0 ** 63), np.float32(0)), 9.21e18, -2.0 ** 63, 2.0 ** 63, np.nextafter(np.float32(-2.0 ** 63), np.float32(-np.inf))], np.float32)
+    x = np.random.RandomState(0).standard_normal((5, 2, D)).astype(np.float32)
+    rotary = D // 2 * 2
+    turns = lib.rotary_turns(rotary)
+    at, on, turns_on = torch.from_numpy(p).cuda(), torch.from_numpy(x).cuda(), turns.cuda()
+    out = torch.empty_like(on)
+    a = lib.HeadsArgs(rows=5, head_dim=D, rotary_dim=rotary, parts=1, turns=turns_on.data_ptr(), positions=at.data_ptr(), position_kind=lib.IDX_F32,
+                      position_count=5, position_group=1, amplitude=1.0)
+    a.part[0] = lib.HeadsPart(x=on.data_ptr(), out=out.data_ptr(), x_row=2 * D, x_head=D, out_row=2 * D, out_head=D, heads=2)
+    lib.check(lib.raw().b2_rotary(ctypes.byref(a), 0, None, None, None, 0, None))
+    got = out.cpu().numpy()
+    want, size = ho.rotate(x[:3], ho.angles(np.array([int(v) for v in p[:3]]), turns.numpy()), rotary, False)
+    assert np.all(np.abs(got[:3] - want) <= 6 * 2.0 ** -24 * size)
+    assert np.isnan(got[3:, :, :rotary]).all() and np.array_equal(got[..., rotary:], x[..., rotary:])
