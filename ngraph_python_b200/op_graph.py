@@ -1224,7 +1224,8 @@ def muon(variables, gradients, lr, momentum=0.95, nesterov=True, weight_decay=0.
     """One step over many matrices at once whose updates are orthogonalised: the running mean of the gradients, with momentum and,
     where nesterov, the newest gradient once more, is divided by its norm and taken `iterations` times through the odd polynomial with
     these coefficients, which leads its singular values towards one, and moves the variable by lr * scale.  Variables have two
-    axes, rows and columns, or three: a stack of matrices along the first.  scale: "sides" sqrt(max(1, rows / columns)), "rms"
+    axes, rows and columns, or three: a stack of matrices along the first, each by itself.  (A weight that makes heads is one matrix, of
+    features by heads times features: a variable of two axes, reshaped for the product, and its gradient reshaped back.)  scale: "sides" sqrt(max(1, rows / columns)), "rms"
     0.2 sqrt(max(rows, columns)), or a number.  lr, and grad_scale, which multiplies every gradient, are numbers or ops whose value
     is one.  The means (op.states) and the number of steps (op.count) are persistent tensors, zero before the first.  Tables, vectors
     and output layers are better left to adamw."""
