@@ -223,10 +223,10 @@ constexpr int kThreads = 256;
 // with two, 120 with three; one and three 146.  Rotation alone, 8192 x 20, four heads: 28.5 with three, 33 with two.
 __host__ __device__ constexpr int unrolled(int mode, int values) { return mode == BACKWARD && values >= 8 ? 2 : 4; }
 __host__ __device__ constexpr int blocks_to(int mode, int values) { return values < 8 ? (mode == BACKWARD ? 2 : 3) : mode == ROTATE ? 3 : 2; }
-// How many tasks' heads a warp of whole vectors of a row has in shared memory or on their way there
+// How many tasks' heads a warp of whole vectors of a row has in shared memory or on their way there, of gradients: x, d_out and rstd
 constexpr int kAhead = 3;
 __host__ __device__ constexpr bool runs_ahead(int mode, int vec, bool flat) { return mode == BACKWARD && vec == 4 && !flat; }
-__host__ __device__ constexpr int slot_bytes(int mode) { return 32 * 16 * 2 * unrolled(mode, 8) * (mode == BACKWARD ? 2 : 1) + (mode == BACKWARD ? 32 * 4 * unrolled(mode, 8) : 0); }
+constexpr int kSlotBytes = (2 * 32 * 16 * 2 + 32 * 4) * unrolled(BACKWARD, 8);
 // CTAs that stay, and fetch the heads of their next task into L2 meanwhile: forward 62 us without, 59 with (gradients 142 and 127, before
 // whole vectors came by way of shared memory); a
 // rotation, which waits for nothing but its loads, 28.5 without and 31 with.
@@ -353,9 +353,9 @@ heads_kernel(const b2_heads a, const b2_heads_grads g, const FlexArgs flex, cons
     // Whole vectors of a row's heads come by way of shared memory, kAhead - 1 tasks ahead: a lane copies what it will read itself, so that
     // it waits for nobody else.
     extern __shared__ float2 table[];
-    char* slots = reinterpret_cast<char*>(table) + (threadIdx.x >> 5) * (RING ? kAhead * slot_bytes(MODE) : 0) + lane * 16;
-    const auto slot_of = [&](int stage, int tensor, int u, int e) { return slots + stage * slot_bytes(MODE) + ((tensor * U + u) * 2 + e) * 512; };
-    const auto rstd_slot = [&](int stage, int u) { return slots + stage * slot_bytes(MODE) + 2 * U * 2 * 512 + u * 128 - lane * 12; };
+    char* slots = reinterpret_cast<char*>(table) + (threadIdx.x >> 5) * (RING ? kAhead * kSlotBytes : 0) + lane * 16;
+    const auto slot_of = [&](int stage, int tensor, int u, int e) { return slots + stage * kSlotBytes + ((tensor * U + u) * 2 + e) * 512; };
+    const auto rstd_slot = [&](int stage, int u) { return slots + stage * kSlotBytes + 2 * U * 2 * 512 + u * 128 - lane * 12; };
     const auto copy_ahead = [&](long long task, int stage) {
         if (task < end) {
             const Begin t = begin_of(task);
@@ -374,15 +374,13 @@ heads_kernel(const b2_heads a, const b2_heads_grads g, const FlexArgs flex, cons
                 }
             };
             copy(static_cast<const T*>(p.x) + t.row * p.x_row + first * p.x_head, 0, p.x_head);
-            if constexpr (MODE == BACKWARD) {
-                copy(reinterpret_cast<const T*>(d.d_out) + t.row * d.d_out_row + first * d.d_out_head, 1, d.d_out_head);
+            copy(reinterpret_cast<const T*>(d.d_out) + t.row * d.d_out_row + first * d.d_out_head, 1, d.d_out_head);
 #pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    const bool live = u < deal.turns && u * beside < left;
-                    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"((unsigned)__cvta_generic_to_shared(rstd_slot(stage, u))),
-                                 "l"(live ? p.rstd + t.row * p.heads + first + u * beside : p.rstd), "r"(live ? 4 : 0)
-                                 : "memory");
-                }
+            for (int u = 0; u < U; ++u) {
+                const bool live = u < deal.turns && u * beside < left;
+                asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"((unsigned)__cvta_generic_to_shared(rstd_slot(stage, u))),
+                             "l"(live ? p.rstd + t.row * p.heads + first + u * beside : p.rstd), "r"(live ? 4 : 0)
+                             : "memory");
             }
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
@@ -473,9 +471,9 @@ heads_kernel(const b2_heads a, const b2_heads_grads g, const FlexArgs flex, cons
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                     get<4>(reinterpret_cast<const float*>(slot_of(stage, 0, u, e)), x[u] + 4 * e);
-                    if constexpr (MODE == BACKWARD) get<4>(reinterpret_cast<const float*>(slot_of(stage, 1, u, e)), y[u] + 4 * e);
+                    get<4>(reinterpret_cast<const float*>(slot_of(stage, 1, u, e)), y[u] + 4 * e);
                 }
-                if constexpr (MODE == BACKWARD) rstd[u] = *reinterpret_cast<const float*>(rstd_slot(stage, u));
+                rstd[u] = *reinterpret_cast<const float*>(rstd_slot(stage, u));
             } else if (live) {
                 load(at_turn(from, u, p.x_row, p.x_head), x[u]);
                 if constexpr (MODE == BACKWARD) {
@@ -532,11 +530,10 @@ heads_kernel(const b2_heads a, const b2_heads_grads g, const FlexArgs flex, cons
             }
 #pragma unroll
             for (int k = 0; k < P; ++k) {
-                const int i = APART ? k : 2 * k, j = APART ? VEC + k : 2 * k + 1;
                 if (turning >> k & 1) {
-                    const float s = v[i], t = v[j];
-                    v[i] = fmaf(s, turn[k].x, -t * turn[k].y);
-                    v[j] = fmaf(t, turn[k].x, s * turn[k].y);
+                    const float s = v[2 * k], t = v[2 * k + 1];
+                    v[2 * k] = fmaf(s, turn[k].x, -t * turn[k].y);
+                    v[2 * k + 1] = fmaf(t, turn[k].x, s * turn[k].y);
                 }
             }
         };
@@ -840,7 +837,7 @@ bool aligned_heads(const b2_heads& a, const void* p, int64_t row, int64_t head, 
 template <int MODE, typename T, int VEC, int EACH, bool HALVES, bool FLAT>
 int launch_dealt(const b2_heads& a, const b2_heads_grads& g, const FlexArgs& flex, const Deal& deal, float* sums, cudaStream_t st) {
     constexpr bool ring = runs_ahead(MODE, VEC, FLAT);
-    const size_t room = ring ? (size_t)kThreads / 32 * kAhead * slot_bytes(MODE) : MODE == BACKWARD ? (size_t)kThreads / 32 * 2 * a.head_dim * sizeof(float) : 0;
+    const size_t room = ring ? (size_t)kThreads / 32 * kAhead * kSlotBytes : MODE == BACKWARD ? (size_t)kThreads / 32 * 2 * a.head_dim * sizeof(float) : 0;
     static std::atomic<unsigned long long> done{0};
     if (ring) B2_CHECK(b2::allow_shared((const void*)heads_kernel<MODE, T, VEC, EACH, HALVES, FLAT>, (int)room, &done));
     B2_CUDA((b2::launch_after(heads_kernel<MODE, T, VEC, EACH, HALVES, FLAT>, dim3(ctas_of(deal, MODE, 2 * VEC * EACH)), kThreads, room, st, a, g, flex, deal, sums)));

@@ -61,7 +61,6 @@ struct Matrix {
     int items[3];                            // of a step, by phase
     int first_chunk, chunks;
     float decay, scale;
-    int unused;
 };
 struct Chunk {                               // values of a matrix whose squares one CTA adds
     int matrix, n;
@@ -325,7 +324,7 @@ constexpr int kChain = 1;
 constexpr int kDependencyPolls = 1 << 22;
 
 struct Work {
-    int matrix, phase, step, i, j, width, k_blocks, unused;
+    int matrix, phase, step, i, j, width, k_blocks;
 };
 // Where the blocks of an operand lie: 128 rows (or columns) of tiles by `mn`, k by `k`, in blocks
 struct Operand {

@@ -1205,14 +1205,19 @@ class RotaryStep(_Step):
         self._flex_probe_then(t, ov.buffer, [v.buffer for v in self.in_views], call)
 
 
-def _head_norm_args(op, turns, t, ptr):
-    """What the forward pass and the gradients of a HeadNormOp have alike, but for the tensors."""
+def _head_norm_sizes(op):
+    """What the forward pass and the gradients of a HeadNormOp have alike, but for the tensors and the rotation."""
     a = lib.HeadsArgs()
     a.rows, a.head_dim, a.parts, a.eps = op.row_axes.size, op.feature_axes.size, len(op.xs), op.eps
-    if op.rotation is not None:
-        turns.fill(a, t, op.place)
     for i, h in enumerate(op.head_axes):
         a.part[i].heads = h.size
+    return a
+
+
+def _head_norm_args(op, turns, t):
+    a = _head_norm_sizes(op)
+    if op.rotation is not None:
+        turns.fill(a, t, op.place)
     return a
 
 
@@ -1233,7 +1238,7 @@ class HeadNormStep(_Fp32Step):
 
     def launch(self, t):
         op = self.op
-        a = _head_norm_args(op, self.turns, t, self._ptr)
+        a = _head_norm_args(op, self.turns, t)
         if self.positions:
             a.positions, a.position_kind = self._ptr(self.positions[0]), lib.IDX_F32
         for i, (x, w, h, ax) in enumerate(zip(self.xs, self.weights, op.head_axes, op.tensor_axes)):
@@ -1259,15 +1264,11 @@ class HeadNormGradStep(_Fp32Step):
         self.turns = _Turns(f.rotation, f.rotary_dim)
         # (sums over rows are added by a second launch)
         self.launches = 2 if any(k.startswith("weight") for k in self.found) else 1
-        a = lib.HeadsArgs()
-        a.rows, a.head_dim, a.parts, a.eps = f.row_axes.size, f.feature_axes.size, len(f.xs), f.eps
-        for i, h in enumerate(f.head_axes):
-            a.part[i].heads = h.size
-        self.scratch_bytes = lib.heads_bprop_scratch_bytes(a)
+        self.scratch_bytes = lib.heads_bprop_scratch_bytes(_head_norm_sizes(f))
 
     def launch(self, t):
         f, d = self.op.fprop, lib.HeadsGrads()
-        a = _head_norm_args(f, self.turns, t, self._ptr)
+        a = _head_norm_args(f, self.turns, t)
         if self.positions:
             a.positions, a.position_kind = self._ptr(self.positions[0]), lib.IDX_F32
         for i, (x, w, h, ax) in enumerate(zip(self.xs, self.weights, f.head_axes, f.tensor_axes)):
