@@ -735,16 +735,22 @@ int b2_adamw_step(void* plan, int64_t chunks, int32_t state_bits, const b2_adamw
  *   u    = nesterov ? (1 - momentum) g + momentum mean : mean,   x = u / (|u| + eps),  |u| the root of the sum of squares
  *   x    = a x + (b A + c A A) x,  A = x x^T, `steps` times      (x^T x from the other side where rows > cols: the same)
  *   param = param (1 - lr weight_decay decay) - lr scale x
- * which takes the singular values of x towards one.  Products are accurate to fp32: operands are held as two fp16 parts, which
- * together round as fp32 does, and three of the four products of parts are added, in fp32.  A matrix with a gradient that is not finite becomes NaN, the others are
- * not touched by it; one whose u is zero only decays (where eps is not zero).
+ * which takes the singular values of x towards one.  Operands of the products are held as two fp16 parts, off by up to 2^-23 of a
+ * value (fp32: 2^-24), and three of the four products of parts are added, in fp32.  The update is as exact as one of fp32 products
+ * in the norm of its matrix, some 1e-6 of it; rows that are smaller than others by many orders are not as exact as these in
+ * themselves (a millionth as large: 4e-5, where fp32 has 3e-7).  A matrix with a gradient that is not finite becomes NaN, the
+ * others are not touched by it; one whose u is zero only decays (where eps is not zero).
  *   sizes: bytes of the plan and of the scratch, and what a step is told of the plan
  *   plan:  a table of the work on the device, made once for given addresses (not while a stream is captured); tensors that
  *          overlap are refused, gradients may be shared; matrices without values are allowed
  *   step:  lr and grad_scale, where not NULL, point to device floats, the first instead of hyper->lr; *step, where not NULL, is a
  *          device float that is counted up by one; status: a device word that is set to 1 if a bounded wait ran out (the step's
  *          params are not to be used then), or NULL.  A step with the sizes of another plan does nothing.
- * The scratch needs no initial value.  A plan and a scratch are for one stream at a time. */
+ * The scratch needs no initial value.  A plan and a scratch are for one stream at a time.  Neither they nor the numbers may lie in
+ * one another's memory, nor in the tensors of the plan: a step is not told these again, and does not look.  The scratch holds all
+ * matrices at once but small ones: 8 bytes a value and 12 for each of n x n, n the shorter side, in blocks of 64 x 64 (some 12 bytes a value
+ * for the matrices of a transformer's layers).  Where that is too much, several plans, one step behind another, may share one
+ * scratch as large as the largest of them needs. */
 typedef struct {
     float* param;
     const float* grad;

@@ -10,8 +10,8 @@
 // at most an eighth of a turn, goes into the series of sine and cosine.
 //
 // Bound by memory: 8 bytes a value forward, 12 backward, each tensor read once and its angles worked out from 8 bytes a row.  8192
-// rows, heads of 128: rotation of 16 + 4 heads 28.1 us (168 MB, 6.0 TB/s), norm and rotation of 32 + 8 57.4 (337 MB, 5.9), their
-// gradients 101.9 (505 MB, 5.0), where a copy has 6.55.  A lane takes the same features of several heads, so that the angles, some
+// rows, heads of 128: rotation of 16 + 4 heads 28.9 us (168 MB, 5.8 TB/s), norm and rotation of 32 + 8 59.8 (337 MB, 5.6), their
+// gradients 105 (505 MB, 4.8), where a copy has 6.55.  A lane takes the same features of several heads, so that the angles, some
 // twenty instructions a pair, are shared by the heads of a row; what is left between this and a copy is instructions (each of four
 // schedulers issues in about half of its cycles, with 8 to 16 warps) and, of gradients, the sums over CTAs in a second launch.
 #include <cmath>
@@ -58,11 +58,11 @@ __device__ __forceinline__ bool position_of(const b2_heads& a, long long row, co
 }
 
 // amplitude * (cos, sin) of the fraction of a turn whose 64 bits are `phase`: of what is left of the nearest quarter turn by
-// their series, up to x^9 / 9! and x^10 / 10!, whose next terms are 2e-9 and 5e-10 at an eighth of a turn.  (A third of the
-// instructions of sincospif, which would look for the quarter turn again: the forward pass of 8192 x 40 heads took 70 us with it, 66 without, as the kernel was then.)
+// their series, up to x^9 / 9! and x^10 / 10!, whose next terms are 2e-9 and 5e-10 at an eighth of a turn.  (sincospif would look for
+// the quarter turn again: the forward pass of 8192 x 40 heads of 128 takes 60.6 us with it, 59.9 so.)
 __device__ __forceinline__ float2 turn_of(unsigned long long phase, float amplitude) {
     const unsigned t = (unsigned)(phase >> 32);
-    const unsigned quarter = (t + 0x20000000u) >> 30;                                     // 0 ... 4
+    const unsigned quarter = (t + 0x20000000u) >> 30;                                     // 0 ... 3: the fourth is the first
     const float x = (float)(int)(t - (quarter << 30)) * 1.4629180792671596e-9f;           // 2 pi / 2^32
     const float z = x * x;
     float s = fmaf(z, 2.7557319e-6f, -1.9841270e-4f), c = fmaf(z, -2.7557319e-7f, 2.4801587e-5f);
@@ -218,18 +218,18 @@ struct Deal {
     long long tasks;
 };
 constexpr int kThreads = 256;
-// Heads that a lane loads at once, by how many features of each it holds, and CTAs to an SM (measured without the ring, which made
-// gradients 105 us).  Eight features, 8192 rows of 40 heads of 128 forward, four heads: 59 us with two CTAs, 63 with three; two heads and four CTAs 72; one and five 85.  Gradients, two heads: 127
-// with two, 120 with three; one and three 146.  Rotation alone, 8192 x 20, four heads: 28.5 with three, 33 with two.
+// Heads that a lane loads at once, by how many features of each it holds, and CTAs to an SM.  Eight features, 8192 rows of 40 heads of
+// 128 forward, four heads: 59.9 us with two CTAs, 63.0 with three; two heads and four CTAs 78; one and five 108.  Gradients,
+// two heads and two CTAs, for which shared memory has room: 105; one and three 144.  Rotation alone, 8192 x 20, four heads: 28.9 with
+// three CTAs, 29.1 with two.
 __host__ __device__ constexpr int unrolled(int mode, int values) { return mode == BACKWARD && values >= 8 ? 2 : 4; }
 __host__ __device__ constexpr int blocks_to(int mode, int values) { return values < 8 ? (mode == BACKWARD ? 2 : 3) : mode == ROTATE ? 3 : 2; }
 // How many tasks' heads a warp of whole vectors of a row has in shared memory or on their way there, of gradients: x, d_out and rstd
 constexpr int kAhead = 3;
 __host__ __device__ constexpr bool runs_ahead(int mode, int vec, bool flat) { return mode == BACKWARD && vec == 4 && !flat; }
 constexpr int kSlotBytes = (2 * 32 * 16 * 2 + 32 * 4) * unrolled(BACKWARD, 8);
-// CTAs that stay, and fetch the heads of their next task into L2 meanwhile: forward 62 us without, 59 with (gradients 142 and 127, before
-// whole vectors came by way of shared memory); a
-// rotation, which waits for nothing but its loads, 28.5 without and 31 with.
+// CTAs that stay, and fetch the heads of their next task into L2 meanwhile: forward 65.8 us without, 59.9 with; a rotation, which waits
+// for nothing but its loads, 28.9 without and 32.4 with.  (Of gradients a sum a CTA is stored, so that there are few of them.)
 __host__ __device__ constexpr bool stays(int mode) { return mode != ROTATE; }
 
 template <int VEC, typename T>
@@ -324,8 +324,8 @@ heads_kernel(const b2_heads a, const b2_heads_grads g, const FlexArgs flex, cons
                 for (int k = 0; k < VEC; ++k) v[VEC * e + k] = 0.0f;
     };
     const float share = 1.0f / (float)D;
-    // A warp's tasks: every so manieth; of gradients, which take longer, so many next to one another, whose rows and angles are often the
-    // same (105.8 and 102.7 us; forward 57.4 and 64.7, since the last ones end later)
+    // A warp's tasks: every so manieth; where they come by way of shared memory, so many next to one another, whose rows and angles are
+    // often the same (3 us of 105; the forward pass takes as long either way, 59.9 and 60.1)
     constexpr bool RING = runs_ahead(MODE, VEC, FLAT);
     const long long warps = (long long)gridDim.x * (kThreads / 32), run = (deal.tasks + warps - 1) / warps, me = (long long)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
     const long long task0 = RING ? me * run : me, end = RING && task0 + run < deal.tasks ? task0 + run : deal.tasks, step = RING ? 1 : warps;

@@ -4,12 +4,15 @@
 //   `steps` times:  A = x x^T,  B = a I + b A + c A A,  x = B x          (x^T x and x B where there are more rows than columns)
 //   param = param (1 - lr wd decay) - lr scale x
 //
-// Bound by the tensor cores: 6 n^2 m + 2 n^3 operations a step for n x m (both squares are symmetric: half of each), three times
-// over, since fp32 accuracy takes three 16-bit products.  x, A and B are held as two fp16 parts, hi = the value rounded to
-// fp16, lo = the rest rounded to fp16, which together round to 2^-24 of the value as fp32 does; of (hi + lo)(hi' + lo') the
-// product lo lo' is left out, 2^-24 again.  fp16 has the range for it because the largest singular value of every operand is
+// Bound by the tensor cores: 3 n^2 m + n^3 operations a step for n x m (of both squares, which are symmetric, half), three times
+// over, for what comes near fp32.  x, A and B are held as two fp16 parts, hi = the value rounded to fp16, lo = the rest rounded to
+// fp16: together off by up to 2^-23 of the value, where fp32 rounds to 2^-24; of (hi + lo)(hi' + lo') the product lo lo' is
+// left out, up to 2^-22 of the whole.  fp16 has the range for it because the largest singular value of every operand is
 // known beforehand: x is normalised, and what the polynomial makes of [0, s] is worked out on the host, which gives each operand
-// a power of two that puts its largest possible value next to the largest of fp16.  Values down to 2^-38 of it keep a lo part.
+// a power of two that puts its largest possible value next to the largest of fp16.  Values down to 2^-18 of it keep all of
+// their lo part, those below 2^-29 none: it ends at fp16's last bit, 2^-41 of the largest.  So the update is as exact as one of fp32
+// products in the norm of the matrix (640 x 1920: 2.8e-6 of it, numpy's fp32 2.2e-6), but rows a million times smaller than others are
+// off by 4e-5 of themselves, where fp32 has 3e-7.
 // (Three tf32 products give the same accuracy at half the rate; bf16 parts have 8 bits each, 2^-17 together.)
 //
 // Storage: blocks of 64 x 64 values, hi and lo behind one another, each 8 KB as the tensor core reads it from shared memory
@@ -25,9 +28,9 @@
 // that it reads.  Only items that a running CTA has taken are waited for, so that it does not matter how many CTAs run.
 // With a launch for each product the last wave of tiles of every one of 15 would leave SMs idle.
 //
-// 48 matrices of 12 layers of 640 (59 million values): 2.9 ms in a loop, where power caps the clock, 2.5 alone; the 16-bit products
+// 48 matrices of 12 layers of 640 (59 million values): 2.95 ms in a loop, where power caps the clock, 2.5 alone; the 16-bit products
 // by themselves would take 1.14 at the rate of a large product, 1.35 at its sustained one.  A tile of 256 columns keeps shared memory busy for
-// 1875 of the 1960 cycles of a block of k (144 KB read by the tensor core, 96 KB written by the copies, 128 bytes a cycle); what comes
+// 1920 of the 1960 cycles of a block of k (144 KB read by the tensor core, 96 KB written by the copies, 128 bytes a cycle); what comes
 // on top is the storing of tiles, some 5000 cycles after ten blocks of k, which the next tile's first two blocks hide in part.
 #include <algorithm>
 #include <cmath>
@@ -318,7 +321,7 @@ constexpr int kRooms = 2 * kPairs;                          // for a part of a b
 constexpr int kProductShared = 1024 + kUnits * kUnit + kRooms * kBlockBytes + 512;
 static_assert(kProductShared <= 227 << 10, "shared memory of a CTA");
 // Blocks of k that are added in tensor memory, whose sums lose what they add: 640 x 1920 is 2.8e-6 off in the 2-norm with one
-// (numpy's fp32 2.2e-6), 6.4e-6 with two, 1.2e-5 with four, for 3.92, 3.77 and 3.60 ms of 48 matrices.  The small products
+// (numpy's fp32 2.2e-6), 6.4e-6 with two, 1.2e-5 with four, for 2.97, 2.82 and 2.73 ms of 48 matrices.  The small products
 // go first.  The rest is added in registers.
 constexpr int kChain = 1;
 constexpr int kDependencyPolls = 1 << 22;
@@ -787,8 +790,8 @@ muon_product_kernel(const void* plan, const Told told, const Rates r, const Poly
 
 // ---- small matrices: all of a step in one CTA ----------------------------------------------------------------
 // x and A (then B in its place) stay in shared memory in the form above, sums in tensor memory, in columns of their own for every block
-// of k; a product is a few instructions between two barriers, 1.2 us where the launch for all matrices takes 8.  A matrix that has more rows
-// than columns is taken as its transpose.  x: [part][block along][block across], across the shorter side.
+// of k; a product is a few instructions between two barriers.  Eight matrices of 64 to 256: 58 us, 3.9 for each of 15 products with its
+// epilogue, where the launch for all matrices takes 8.  A matrix that has more rows than columns is taken as its transpose.  x: [part][block along][block across], across the shorter side.
 constexpr int kSoloThreads = 512;
 constexpr int kSoloBlocks = 13;                             // of x and A in both parts
 constexpr int kSoloColumns = 512;                           // of tensor memory
@@ -1105,7 +1108,8 @@ void tiles_of(int rb, int cb, bool half, int width, F&& tile) {
 }
 
 // Cycles of an item, as measured: blocks of k, which wait for shared memory (64 columns want 72 KB read and 48 KB written a block at 128
-// bytes a cycle, 256 columns 144 and 96), and what starts and ends it.
+// bytes a cycle, 256 columns 144 and 96), and what starts and ends it (lists of 8 to 48 matrices of 64 to 8192 took as long with 4000,
+// 12000 and 20000 for that).
 double cycles_of(int width, int k_blocks) {
     static const double block[5] = {0, 1150, 1430, 1700, 1960};
     return block[width] * k_blocks + 8000;
@@ -1159,7 +1163,8 @@ Layout layout_of(const b2_muon_matrix* list, int count) {
         for (int k = 0; k < blocks; ++k) found.blocks.push_back({index, k});
     }
     // Groups of matrices whose phases keep the machine busy while another's end: some three tiles to an SM or more, in groups of one
-    // size (a last group of few matrices would wait for each of its phases)
+    // size (a last group of few matrices would wait for each of its phases).  48 matrices of 640 to 2560 and 8 of 2048 to 8192: 3.23 and 12.5
+    // ms with half a tile to an SM, 2.95 and 11.4 with one, 2.93 and 11.1 with two, 2.94 and 11.1 with three
     const auto tiles_in = [&](size_t m) {
         long long tiles = 0;
         tiles_of(found.matrices[m].n_blocks, found.matrices[m].n_blocks, true, 4, [&](int, int, int) { ++tiles; });
@@ -1416,7 +1421,7 @@ extern "C" int b2_muon_step(void* plan, const b2_muon_sizes* s, const b2_muon_hy
     if (s->items > 0) {
         B2_CUDA((b2::launch_after(muon_parts_kernel, grid(s->blocks, b2::kSms * 8), kMeanThreads, 0, st, base, told, r, grad_scale, (int)p.x[0], room)));
         B2_CHECK(b2::allow_shared((const void*)muon_product_kernel, kProductShared, &done));
-        // (SMs for the small matrices where few items would leave some idle anyway: these need 50 us, which would come on top)
+        // (SMs for the small matrices where few items would leave some idle anyway: these need 58 us, which would come on top)
         const long long left = s->items < 8 * b2::kSms ? b2::kSms - std::min<long long>(s->solos, 8) : b2::kSms;
         B2_CUDA((b2::launch_after(muon_product_kernel, grid(s->items, left), kProductThreads, (size_t)kProductShared, st, base, told, r, p, lr, room, status)));
     }
