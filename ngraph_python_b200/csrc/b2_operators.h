@@ -81,9 +81,15 @@ inline bool meet(Rows a, Rows b) {
     if (a.rows > b.rows) std::swap(a, b);
     const long long ahead = (long long)b.p - (long long)a.p;     // where b begins, seen from a
     const auto below = [](long long x, long long y) { return x / y - (x % y < 0); };
+    if (a.stride == b.stride) {
+        // row i of a and row j of b meet where (i - j) stride lies between ahead - a.width and ahead + b.width
+        const long long least = below(ahead - a.width, a.stride) + 1, d = least > 1 - b.rows ? least : 1 - b.rows;
+        if (d >= a.rows || d * a.stride >= ahead + b.width) return false;
+        if (!a.at_heads || !b.at_heads) return true;
+    }
     const auto alike = [](long long x, long long y, long long of_x, long long of_y) { return x == 1 || y == 1 || of_x == of_y; };
     if (a.at_heads && b.at_heads && alike(a.at_rows, b.at_rows, a.row_stride, b.row_stride) && alike(a.at_heads, b.at_heads, a.head_stride, b.head_stride)) {
-        // as for rows below, at every distance that two heads have
+        // the same at every distance that two heads have
         const long long by_row = a.at_rows > 1 ? a.row_stride : b.at_rows > 1 ? b.row_stride : 1, by_head = a.at_heads > 1 ? a.head_stride : b.head_stride;
         for (long long e = 1 - b.at_heads; e < a.at_heads; ++e) {
             const long long from = ahead - e * by_head, least = below(from - a.head_width, by_row) + 1, d = least > 1 - b.at_rows ? least : 1 - b.at_rows;
@@ -91,11 +97,7 @@ inline bool meet(Rows a, Rows b) {
         }
         return false;
     }
-    if (a.stride == b.stride) {
-        // row i of a and row j of b meet where (i - j) stride lies between ahead - a.width and ahead + b.width
-        const long long least = below(ahead - a.width, a.stride) + 1, d = least > 1 - b.rows ? least : 1 - b.rows;
-        return d < a.rows && d * a.stride < ahead + b.width;
-    }
+    if (a.stride == b.stride) return true;
     for (long long i = 0; i < a.rows; ++i) {
         // the first row of b that does not end before row i of a begins
         const long long from = i * a.stride - ahead, least = below(from - b.width, b.stride) + 1, j = least > 0 ? least : 0;

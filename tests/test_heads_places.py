@@ -1,5 +1,6 @@
 """Which places of tensors of heads are taken and which are refused, and what the arguments of a call may not do to the process."""
 import ctypes
+import os
 import subprocess
 import sys
 
@@ -24,7 +25,8 @@ print(lib.raw().b2_heads_bprop(ctypes.byref(a), ctypes.byref(g), 1 << 30, n, Non
 @pytest.mark.parametrize("positions", ["(1 << 30) + 256", "1 << 30", "(1 << 22) + 8"])
 def test_no_rows_and_positions_in_a_results_memory(positions):
     """Positions of no rows are no memory: nothing to overlap, and nothing to divide by.  (A process of its own, which a signal would end.)"""
-    done = subprocess.run([sys.executable, "-c", NO_ROWS % positions], capture_output=True, text=True, timeout=300)
+    done = subprocess.run([sys.executable, "-c", NO_ROWS % positions], capture_output=True, text=True, timeout=300,
+                          cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
     assert done.returncode == 0, (done.returncode, done.stderr[-500:])
     assert "overlap" not in done.stdout and "one place" not in done.stdout, done.stdout
 
